@@ -341,6 +341,27 @@ int TfStepReplay(void *graph, const unsigned *seeds, int nseeds, float b1t, floa
                  const DLArrayHandle *params, int nparams, void **cudaStream);
 int TfStepGraphFree(void *graph);
 
+/* Layer normalisation over the last axis: y = gamma * (x - mean) / sqrt(var + eps) + beta with each row's own mean and variance
+ * (of the row, not of a sample of it).  gamma and beta have the extent of that axis.
+ * Backward: dinput, dgamma, dbeta, each of which may be null; sums over the rows are in a fixed order (the same bits every run).
+ * These calls, and those below, refuse arrays that are not on the current GPU and outputs that share memory with another array. */
+int TfLayerNormForward(const DLArrayHandle input, const DLArrayHandle gamma, const DLArrayHandle beta, DLArrayHandle output, float eps,
+                       void **cudaStream);
+int TfLayerNormBackward(const DLArrayHandle input, const DLArrayHandle gamma, const DLArrayHandle doutput, DLArrayHandle dinput,
+                        DLArrayHandle dgamma, DLArrayHandle dbeta, float eps, int *memorytoSaving, void **cudaStream);
+/* The residual sum of a dropped-out branch and the layer normalisation behind it: sum = residual + dropout(input), output =
+ * layer_norm(sum).  The mask is DLGpuDropoutForward's for the same seed, drawn again by the backward call; nothing of it is stored.
+ * TfDropoutState makes the state that both calls take (in an empty cell), or gives an existing one another rate and seed; the cell
+ * and the state are the caller's for the life of the operator.  output may be null (the sum alone).
+ * Backward: dsum is the gradient that the sum has from elsewhere (the next residual sum), or null; dresidual = that + the gradient
+ * through the normalisation, dinput = dropout of it.  Each result may be null. */
+int TfDropoutState(float dropout, int seed, void ***state);
+int TfDropoutAddLayerNormForward(const DLArrayHandle input, const DLArrayHandle residual, const DLArrayHandle gamma, const DLArrayHandle beta,
+                                 DLArrayHandle sum, DLArrayHandle output, float eps, void ***state, void **cudaStream);
+int TfDropoutAddLayerNormBackward(const DLArrayHandle sum, const DLArrayHandle gamma, const DLArrayHandle doutput, const DLArrayHandle dsum,
+                                  DLArrayHandle dinput, DLArrayHandle dresidual, DLArrayHandle dgamma, DLArrayHandle dbeta, float eps,
+                                  void ***state, int *memorytoSaving, void **cudaStream);
+
 /* Test / profiling hooks. */
 int TfPoolingArgmax(const DLArrayHandle input, int32_t *indices_dev, void ***cudnnlist,
                     void **cudaStream);   /* first-maximum index (h*W+w in the input plane) per output */

@@ -127,6 +127,20 @@ __device__ __forceinline__ void amax_commit(const AmaxOut& am, uint32_t m) {
 }
 #endif
 
+// ---- dropout: counter-based keep mask ---------------------------------------------------
+// keep(i) is a pure function of (seed, i), so backward regenerates the forward mask and no
+// mask tensor is stored.  The generator is a 64-bit mix (splitmix64 finaliser) of the
+// element index keyed by the seed.
+#ifdef __CUDACC__
+__device__ __forceinline__ float uniform01(unsigned long long seed, unsigned long long i) {
+  unsigned long long z = (i + 1) * 0x9E3779B97F4A7C15ull + seed * 0xD1342543DE82EF95ull;
+  z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+  z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+  z ^= z >> 31;
+  return (float)(z >> 40) * (1.0f / 16777216.0f);
+}
+#endif
+
 // A gradient's call may wait for others (see hold_products in gemm_tcgen05.cu) until launch_held(): true, and the caller keeps it until
 // its own launch_held_...() is called
 bool may_hold(cudaStream_t s);
@@ -199,7 +213,7 @@ void pool_free(void* p);
 // block to the last launch that uses it.  A block is the same at every call until a larger one is asked for; slot ids are per
 // purpose, so that what one operator uses together does not collide.
 struct StreamScratch;
-enum { kScratchSums = 0, kScratchTiles = 1, kScratchSplit = 2, kScratchContract = 3, kScratchPackA = 4, kScratchPackB = 5, kScratchGroup = 6, kScratchSlots = 7 };
+enum { kScratchSums = 0, kScratchTiles = 1, kScratchSplit = 2, kScratchContract = 3, kScratchPackA = 4, kScratchPackB = 5, kScratchGroup = 6, kScratchNorm = 7, kScratchGates = 8, kScratchSlots = 9 };
 class StreamLease {
  public:
   explicit StreamLease(cudaStream_t s);
@@ -286,7 +300,7 @@ cudaError_t clear_now(void* p, size_t bytes);                                   
 cudaError_t copy_on_stream(void* to, const void* from, size_t bytes, cudaStream_t s);     // device to device
 
 // ---- plan structs stored in slot 0 of a descriptor list ----------------------
-enum PlanKind : int { kPlanConv = 0x7f01, kPlanPool, kPlanAct, kPlanReduce, kPlanBN, kPlanTensor, kPlanDropout };
+enum PlanKind : int { kPlanConv = 0x7f01, kPlanPool, kPlanAct, kPlanReduce, kPlanBN, kPlanTensor, kPlanDropout, kPlanResidualDropout };
 
 struct ConvPlan {
   int kind;
@@ -340,6 +354,13 @@ struct DropoutState {
   unsigned long long seed;
   const uint32_t* seed_word;   // a recorded step's seed of this replay, in device memory
   int64_t count;
+};
+struct ResidualDropoutState {  // of a residual sum, kept from call to call
+  int kind;
+  float p;
+  unsigned long long seed;
+  const uint32_t* seed_word;   // inside the recording of that number only
+  uint64_t recording;
 };
 
 template <class T> T* plan_of(void*** cell, int kind) {

@@ -566,16 +566,6 @@ static void launch_slice(float* part, const float* whole, int64_t rows, int64_t 
 }
 
 // ---- dropout: counter-based keep mask ---------------------------------------------------
-// keep(i) is a pure function of (seed, i), so backward regenerates the forward mask and no
-// mask tensor is stored.  The generator is a 64-bit mix (splitmix64 finaliser) of the
-// element index keyed by the seed.
-__device__ __forceinline__ float uniform01(unsigned long long seed, unsigned long long i) {
-  unsigned long long z = (i + 1) * 0x9E3779B97F4A7C15ull + seed * 0xD1342543DE82EF95ull;
-  z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
-  z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
-  z ^= z >> 31;
-  return (float)(z >> 40) * (1.0f / 16777216.0f);
-}
 // Bound by HBM (8 bytes per element) with the hash just below it: about 30 integer instructions per element.  Four
 // elements per thread and trip; the largest magnitude is folded in for the convolution that packs the result.
 __global__ void __launch_bounds__(kBlock) dropout_kernel(const float* __restrict__ in, float* __restrict__ out, int64_t n, float p, float scale, unsigned long long seed_value,

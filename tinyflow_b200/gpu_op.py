@@ -458,6 +458,42 @@ def adam_update_many(params, m, v, grads, b1, b2, b1t, b2t, e, learning_rate, cu
     check_call(_LIB.TfAdamUpdateMany(params, m, v, grads, len(params), _F(b1), _F(b2), _F(b1t), _F(b2t), _F(e), _F(learning_rate), cudaStream))
 
 
+# ---- layer normalisation, alone and behind a residual sum (no counterpart in the reference) ----------------------------
+def _o(arr):
+    """The handle of an array that may be missing."""
+    return None if arr is None else _h(arr)
+
+
+def layer_norm_forward(in_arr, gamma, beta, out_arr, eps, cudaStream):
+    """out = gamma * (in - mean) / sqrt(var + eps) + beta, mean and variance of each row of the last axis."""
+    check_call(_LIB.TfLayerNormForward(_h(in_arr), _h(gamma), _h(beta), _h(out_arr), _F(eps), cudaStream))
+
+
+def layer_norm_backward(in_arr, gamma, dout_arr, din_arr, dgamma, dbeta, eps, cudaStream):
+    """Gradients of :func:`layer_norm_forward`; each of ``din_arr``, ``dgamma``, ``dbeta`` may be None."""
+    return _with_short(_LIB.TfLayerNormBackward, _h(in_arr), _h(gamma), _h(dout_arr), _o(din_arr), _o(dgamma), _o(dbeta), _F(eps), cudaStream)
+
+
+def dropout_state(dropout, seed, state=None):
+    """What the two calls below share: rate and seed.  With ``state`` (from an earlier call) that one gets them, else a new one."""
+    assert seed >= 0
+    state = new_cell(3) if state is None else state
+    check_call(_LIB.TfDropoutState(_F(dropout), ctypes.c_int(seed), state))
+    return state
+
+
+def dropout_add_layer_norm_forward(in_arr, residual, gamma, beta, sum_arr, out_arr, state, eps, cudaStream):
+    """sum = residual + dropout(in), out = layer_norm(sum), in one pass.  ``out_arr`` may be None."""
+    check_call(_LIB.TfDropoutAddLayerNormForward(_h(in_arr), _h(residual), _h(gamma), _h(beta), _h(sum_arr), _o(out_arr), _F(eps), state, cudaStream))
+
+
+def dropout_add_layer_norm_backward(sum_arr, gamma, dout_arr, dsum_arr, din_arr, dresidual, dgamma, dbeta, state, eps, cudaStream):
+    """Gradients of :func:`dropout_add_layer_norm_forward`.  ``dsum_arr``: the gradient that the sum has from elsewhere, or None; each of the
+    results ``din_arr``, ``dresidual``, ``dgamma``, ``dbeta`` may be None."""
+    return _with_short(_LIB.TfDropoutAddLayerNormBackward, _h(sum_arr), _h(gamma), _h(dout_arr), _o(dsum_arr), _o(din_arr), _o(dresidual), _o(dgamma),
+                       _o(dbeta), _F(eps), state, cudaStream)
+
+
 def getInt(intp):
     return _LIB.getInt(intp)
 
