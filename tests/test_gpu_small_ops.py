@@ -279,3 +279,17 @@ def test_column_sums_of_nothing(env, rows, cols):
     ins, outs = gpu.reduce_sum_get_real_shape(x.shape, (cols,), "NHWC")
     gpu.reduce_sum_new(x, out, gpu.reduce_sum_get_cudnnlist(ins, outs, "NHWC", env.cudnn), env.cudnn, env.stream)
     np.testing.assert_array_equal(out.asnumpy(), np.zeros(cols, np.float32))
+
+
+# every place a product may lie at: results, and operands, that begin between two 16-byte boundaries
+@pytest.mark.parametrize("M,K,N", [(777, 2006, 500), (300, 520, 1000), (64, 784, 256), (7, 4608, 4096), (1300, 768, 256)])
+@pytest.mark.parametrize("tA,tB", [(False, False), (True, False), (False, True)])
+@pytest.mark.parametrize("shift", [1, 2, 3])
+def test_products_of_arrays_that_begin_between_16_byte_boundaries(env, M, K, N, tA, tB, shift):
+    from tests.test_gpu_norm import place, read
+    rng = np.random.RandomState(M + K + N)
+    a, b = rng.randn(M, K).astype(np.float32), rng.randn(K, N).astype(np.float32)
+    A, B, C = place(env, np.ascontiguousarray(a.T) if tA else a, shift), place(env, np.ascontiguousarray(b.T) if tB else b, shift), place(env, (M, N), shift)
+    env.gpu_op.matrix_multiply(A, tA, B, tB, C, env.cublas, env.stream)
+    want, mag = a.astype(np.float64) @ b.astype(np.float64), np.abs(a).astype(np.float64) @ np.abs(b).astype(np.float64)
+    assert np.all(np.abs(read(C) - want) <= 1e-4 * np.abs(want) + 8 * 2.0 ** -24 * mag)

@@ -881,7 +881,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm3x_kernel(const __grid_co
       const uint32_t col_bytes = ra.col_stride * 4u;
       char* const row_out = reinterpret_cast<char*>(p.out + ra.base + (long long)n0 * ra.col_stride);
       const int ncols = max(0, min(HC, p.N - n0));
-      const bool vec_ok = p.epi == kEpiRowMajor && ((ra.base + n0) & 3) == 0;
+      const bool vec_ok = p.epi == kEpiRowMajor && (reinterpret_cast<uintptr_t>(row_out) & 15) == 0;
 
       auto wait_group = [&](int acc_buf, int grp) -> bool {   // lane 0 polls, the warp follows (keeps .sync.aligned loads converged)
         int got = lane == 0 ? (int)mbar_wait(&acc_full[acc_buf], (grp >> 1) & 1, abort_flag) : 1;
@@ -1315,7 +1315,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm3x_group_kernel(const __g
       float* const dst = q.out + ra.base + (long long)n0 * ra.col_stride;
 #pragma unroll
       for (int c = 0; c < HC / 2; ++c) total[c] = __fmul2_rn(total[c], scale2);
-      if (q.epi == kEpiRowMajor && ((ra.base + n0) & 3) == 0 && ncols == HC) {
+      if (q.epi == kEpiRowMajor && (reinterpret_cast<uintptr_t>(dst) & 15) == 0 && ncols == HC) {
 #pragma unroll
         for (int c = 0; c < HC / 4; ++c) reinterpret_cast<float4*>(dst)[c] = make_float4(total[2 * c].x, total[2 * c].y, total[2 * c + 1].x, total[2 * c + 1].y);
       } else {
@@ -1494,7 +1494,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm3x_pair_kernel(const __grid_c
       const uint32_t col_stride = ra.col_stride;
       float* const row_out = p.out + ra.base + (long long)n0 * col_stride;
       const int ncols = max(0, min(HC, p.N - n0));
-      const bool vec_ok = p.epi == kEpiRowMajor && ((ra.base + n0) & 3) == 0;
+      const bool vec_ok = p.epi == kEpiRowMajor && (reinterpret_cast<uintptr_t>(row_out) & 15) == 0;
       float accv[HC];
 #pragma unroll
       for (int q = 0; q < HC; ++q) accv[q] = 0.f;
@@ -2304,6 +2304,7 @@ void drop_held_direct();
 static thread_local bool t_waiting = false;           // something is held, on t_waiting_stream
 static thread_local cudaStream_t t_waiting_stream = nullptr;
 void hold_products(bool on) { t_hold = on; }
+bool pause_holding() { const bool was = t_hold; t_hold = false; return was; }
 static void forget_held() { t_held.clear(); t_held_work = 0; t_waiting = false; drop_held_simt(); drop_held_sums(); drop_held_direct(); }
 void drop_held() { forget_held(); t_hold = false; }
 static bool capturing(cudaStream_t s) {
