@@ -362,6 +362,16 @@ int TfDropoutAddLayerNormBackward(const DLArrayHandle sum, const DLArrayHandle g
                                   DLArrayHandle dinput, DLArrayHandle dresidual, DLArrayHandle dgamma, DLArrayHandle dbeta, float eps,
                                   void ***state, int *memorytoSaving, void **cudaStream);
 
+/* Gated dense layer: output = act(input Wg) * (input Wv), weight = [Wg | Wv] (K x 2F, both halves side by side).  activation: 0 sigmoid, 1 relu,
+ * 2 tanh, 4 silu (g * sigmoid(g)), 5 gelu (g times the normal distribution's share below g; by erf, not an approximation of it).
+ * gates (M x 2F), what the activation and the product are applied to, is written for the backward call; null: not kept.
+ * Backward: dinput and dweight, either of which may be null.  Products run on the engine and in the arithmetic that are selected
+ * (TfSetContractionPath, TfSetArithmetic), at once, also between TfHoldProducts(1) and (0). */
+int TfGatedLinearForward(const DLArrayHandle input, const DLArrayHandle weight, DLArrayHandle gates, DLArrayHandle output, int activation,
+                         int *memorytoSaving, void **cudaStream);
+int TfGatedLinearBackward(const DLArrayHandle input, const DLArrayHandle weight, const DLArrayHandle gates, const DLArrayHandle doutput,
+                          DLArrayHandle dinput, DLArrayHandle dweight, int activation, int *memorytoSaving, void **cudaStream);
+
 /* Test / profiling hooks. */
 int TfPoolingArgmax(const DLArrayHandle input, int32_t *indices_dev, void ***cudnnlist,
                     void **cudaStream);   /* first-maximum index (h*W+w in the input plane) per output */

@@ -19,11 +19,15 @@ class OracleExecutor:
         self.topo = list(topo_order)
         self.dtype = dtype
         self.values = {}
+        self.parts = {}             # node of several results -> those besides its own
         self.dropout_seeds = dropout_seeds or {}    # DropoutForward node -> seed used by the GPU run
         self.adam_powers = None     # (b1^t, b2^t) of the step being checked; default: the node's current values
 
     def _conv_geom(self, node, x, w):
         return ops.conv_geometry(x.shape, w.shape, node.padding, node.u, node.v)
+
+    def _residual_dropout(self, forward, x):
+        return x.copy() if forward.dropout == 0 else ops.dropout(x, forward.dropout, self.dropout_seeds.get(forward, forward.seed[0]))
 
     def run(self, feed):
         v = self.values = {n: np.asarray(a, dtype=self.dtype) for n, a in feed.items()}
@@ -152,6 +156,32 @@ class OracleExecutor:
             w, m, vv = ops.adam(ins[0], ins[1], ins[2], ins[3], dt(node.b1), dt(node.b2), dt(b1t), dt(b2t), dt(node.e), dt(node.learning_rate))
             self.values[node.inputs[0]], self.values[node.inputs[1]], self.values[node.inputs[2]] = w, m, vv
             return None
+        if kind in ("PartOp", "NormalisedSumOp"):
+            return self.parts[node.inputs[0]][node.part - 1]
+        if kind == "LayerNormForwardOp":
+            return ops.layer_norm(ins[0], ins[1], ins[2], node.eps)[0]
+        if kind == "LayerNormBackwardOp":
+            dx, dgamma, dbeta = ops.layer_norm_backward(ins[0], ins[1], ins[2], node.eps)
+            self.parts[node] = (dbeta, dx)
+            return dgamma
+        if kind == "DropoutAddLayerNormForwardOp":
+            total = ins[1] + self._residual_dropout(node, ins[0])
+            self.parts[node] = (ops.layer_norm(total, ins[2], ins[3], node.eps)[0],)
+            return total
+        if kind == "DropoutAddLayerNormBackwardOp":
+            dx, dgamma, dbeta = ops.layer_norm_backward(ins[0], ins[1], ins[2], node.eps)
+            if len(ins) > 3:
+                dx = dx + ins[3]
+            self.parts[node] = (dbeta, dx, self._residual_dropout(node.inputs[0], dx))
+            return dgamma
+        if kind == "GatedLinearForwardOp":
+            out, z = ops.gated_linear(ins[0], ins[1], node.activation)
+            self.parts[node] = (z,)
+            return out
+        if kind == "GatedLinearBackwardOp":
+            dx, dweight = ops.gated_linear_backward(ins[0], ins[1], ins[2], ins[3], node.activation)
+            self.parts[node] = (dx,)
+            return dweight
         if kind == "ExpOp":
             return np.exp(ins[0])
         if kind == "LogOp":

@@ -408,3 +408,51 @@ def adam(w, m, v, g, b1, b2, b1t, b2t, e, lr):
     v = v * b2 + g * g * (1 - b2)
     w = w - lr * m / (1 - b1t) / (np.sqrt(v / (1 - b2t)) + e)
     return w, m, v
+
+
+# ---- layer normalisation and the gated dense layer (no counterpart in the reference) ---------------
+def layer_norm(x, gamma, beta, eps):
+    """(y, normalised x, 1 / spread) over the last axis."""
+    mean = x.mean(axis=-1, keepdims=True)
+    inv = 1 / np.sqrt(((x - mean) ** 2).mean(axis=-1, keepdims=True) + eps)
+    xh = (x - mean) * inv
+    return gamma * xh + beta, xh, inv
+
+
+def layer_norm_backward(x, gamma, dy, eps):
+    """(dx, dgamma, dbeta)"""
+    _, xh, inv = layer_norm(x, gamma, 0, eps)
+    g = gamma * dy
+    dx = inv * (g - g.mean(axis=-1, keepdims=True) - xh * (g * xh).mean(axis=-1, keepdims=True))
+    axes = tuple(range(x.ndim - 1))
+    return dx, (dy * xh).sum(axis=axes), dy.sum(axis=axes)
+
+
+def gate(activation, g):
+    """(value, derivative) of the activation of a gated layer."""
+    if activation == "relu":
+        return np.where(g > 0, g, 0), np.where(g > 0, 1.0, 0.0)
+    if activation == "tanh":
+        return np.tanh(g), 1 / np.cosh(np.clip(g, -300, 300)) ** 2
+    if activation == "gelu":
+        from scipy.special import erfc
+        share = 0.5 * erfc(-g / np.sqrt(2))
+        return g * share, share + g * np.exp(-g * g / 2) / np.sqrt(2 * np.pi)
+    from scipy.special import expit
+    s, rest = expit(g), expit(-g)
+    return (s, s * rest) if activation == "sigmoid" else (g * s, s * (1 + g * rest))
+
+
+def gated_linear(x, weight, activation):
+    """(out, both projections)"""
+    z = x @ weight
+    half = weight.shape[1] // 2
+    return gate(activation, z[:, :half])[0] * z[:, half:], z
+
+
+def gated_linear_backward(x, weight, z, dout, activation):
+    """(dx, dweight)"""
+    half = weight.shape[1] // 2
+    value, slope = gate(activation, z[:, :half])
+    dz = np.concatenate([dout * z[:, half:] * slope, dout * value], axis=1)
+    return dz @ weight.T, x.T @ dz

@@ -38,6 +38,19 @@ int tc_fused_relu_bwd_pack(ConvPlan* p, const float* mask, const float* dy, floa
 // which engine served this thread's most recent contraction: 1 = CUDA cores, 2 = tensor cores (0 = none yet)
 static thread_local int t_last_path = 0;
 
+// C[M x N] = op(A) op(B) of contiguous matrices on the engine that is selected
+int matmul_any(const float* A, bool tA, const float* B, bool tB, float* C, int64_t M, int64_t N, int64_t K, cudaStream_t s, const char* what) {
+  if (g_path != 1) {
+    int oom = 0;
+    int r = tc_matmul(A, tA, B, tB, C, M, N, K, s, &oom);
+    if (r < 0) return -1;
+    if (r == 1) { t_last_path = 2; return 0; }
+    TF_REQUIRE(g_path != 2, "%s: shape not taken by the tensor-core path (forced)", what);
+  }
+  t_last_path = 1;
+  return simt_matmul(A, tA, B, tB, C, M, N, K, tA ? M : K, tB ? K : N, N, s, what);
+}
+
 }  // namespace tf
 
 using namespace tf;
@@ -92,18 +105,7 @@ int DLGpuMatrixMultiply(const DLArrayHandle matA, bool transposeA, const DLArray
   TF_REQUIRE(K == Kb, "DLGpuMatrixMultiply: inner extents differ (%lld vs %lld)", (long long)K, (long long)Kb);
   TF_REQUIRE(matC->shape[0] == M && matC->shape[1] == N, "DLGpuMatrixMultiply: output shape mismatch");
   cudaStream_t s = stream_of(cudaStream);
-  const float* A = (const float*)matA->data;
-  const float* B = (const float*)matB->data;
-  float* C = out_f32(matC);
-  if (g_path != 1) {
-    int oom = 0;
-    int r = tc_matmul(A, transposeA, B, transposeB, C, M, N, K, s, &oom);
-    if (r < 0) return -1;
-    if (r == 1) { t_last_path = 2; return 0; }
-    TF_REQUIRE(g_path != 2, "DLGpuMatrixMultiply: shape not taken by the tensor-core path (forced)");
-  }
-  t_last_path = 1;
-  return simt_matmul(A, transposeA, B, transposeB, C, M, N, K, matA->shape[1], matB->shape[1], N, s, "DLGpuMatrixMultiply");
+  return matmul_any((const float*)matA->data, transposeA, (const float*)matB->data, transposeB, out_f32(matC), M, N, K, s, "DLGpuMatrixMultiply");
 }
 
 // Output extent = 1 + (in + 2*pad - window) / stride with pad = window/2 for SAME, 0 for VALID

@@ -26,7 +26,7 @@ import warnings
 import weakref
 
 from . import gpu_op, ndarray, step_graph
-from .graph import (AddOp, AdamOp, BNForwardOp, BroadcastToGradientOp, Convolution2DBackwardOp, Convolution2DForwardOp, MatMulOp, OnesLikeOp, Pooling2DForwardOp, SgdOp, Variable, ZerosLikeOp, adam_op, find_topo_sort, get_Variable_node_list, gradients, sgd_op)
+from .graph import (AddOp, AdamOp, BNForwardOp, BroadcastToGradientOp, Convolution2DBackwardOp, Convolution2DForwardOp, ManyOp, MatMulOp, OnesLikeOp, PartOp, Pooling2DForwardOp, SgdOp, Variable, ZerosLikeOp, adam_op, find_topo_sort, get_Variable_node_list, gradients, sgd_op)
 
 
 def getcomputelist(Variable_node_list, Variable_node_grad_list, b1, b2, b1t, b2t, e, learning_rate):
@@ -190,6 +190,12 @@ class Executor(object):
         # convolutions of a fed filter, and their descriptors as the library takes them (with the objects behind)
         self._convs = [n for n in self.topo_order if type(n.op) is Convolution2DForwardOp and not n.inputs[1].inputs]
         self._conv_cells = ([], None)
+        # further results of operators that have several: node -> {number of the result: its node}
+        self._parts = {}
+        for node in self.topo_order:
+            if isinstance(node.op, PartOp):
+                if self._parts.setdefault(node.inputs[0], {}).setdefault(node.part, node) is not node:
+                    raise ValueError("result %d of %s is in the graph twice" % (node.part, node.inputs[0].name))
         # gradients of parameters that only the optimiser reads: they may wait and share launches
         readers = {}
         for node in self.topo_order:
@@ -341,6 +347,30 @@ class Executor(object):
             self._leases = {i: live for i, live in ((i, [r for r in refs if r() is not None]) for i, refs in self._leases.items()) if live}
         return self._leases
 
+    def _compute_many(self, node, arrays, stream, only=None):
+        """A node of several results: all of them that the graph has, into ``arrays`` (by node) or new ones.  ``only``: that one again."""
+        results = [node] + [self._parts.get(node, {}).get(k) for k in range(1, node.op.parts + 1)]
+        if only is not None:
+            results[1:] = [n if n is only else None for n in results[1:]]
+        inputs = [self._resident(n) for n in node.inputs]
+        outs = []
+        for n in results:
+            out = None
+            if n is not None:
+                out = arrays.get(n)
+                if out is None:
+                    out = ndarray.empty(self.node_to_shape_map[n], self.ctx_gpu)
+                if isinstance(out, int):
+                    raise MemoryError("device out of memory allocating %d bytes for node %d (%s)" % (out, n.index, n.name))
+            outs.append(out)
+        compute = node.op.compute if only is None else node.op.recompute
+        short = compute(node, inputs, outs, self.cudnnHandle, self.cublasHandle, stream)
+        if short:
+            raise MemoryError("device out of memory inside node %d (%s): %d bytes short" % (node.index, node.name, short))
+        for n, out in zip(results, outs):
+            if n is not None and only in (None, n):
+                self._values[n.index] = out
+
     def _compute(self, node, out, stream):
         inputs = [self._resident(n) for n in node.inputs]
         if node.issgd:
@@ -407,17 +437,20 @@ class Executor(object):
         updates, holding = [], False
         if together and self._convs and all(n.inputs[1] in self._feed for n in self._convs):
             self._pack_filters(stream)
+
+        def earlier(node):                               # the array of the step before
+            out = previous.pop(node.index, None)
+            return None if out is not None and (self.have_plan or out.is_freed or out.shape != shapes[node]) else out
+
         for node in self.topo_order:
-            if not node.inputs and node in self._feed:
+            if (not node.inputs and node in self._feed) or isinstance(node.op, PartOp):      # a part was computed with its whole
                 if self.have_plan:
                     self._after_node(node)
                 continue
             if together and node.issgd and type(node.op) in (SgdOp, AdamOp):
                 updates.append(node)
                 continue
-            out = previous.pop(node.index, None)
-            if out is not None and (self.have_plan or out.is_freed or out.shape != shapes[node]):
-                out = None
+            out = earlier(node)
             if together and type(node.op) in (ZerosLikeOp, OnesLikeOp):
                 # nobody else writes its array, so the constant of the first step is still there
                 if out is None or node.index not in self._constants:
@@ -433,16 +466,24 @@ class Executor(object):
                     continue
             if self.have_plan:
                 for idx in node.recompute_list:
-                    self._compute(self.topo_order[idx], None, stream)
+                    again = self.topo_order[idx]
+                    if isinstance(again.op, (ManyOp, PartOp)):
+                        self._compute_many(again.inputs[0] if isinstance(again.op, PartOp) else again, {}, stream, only=again)
+                    else:
+                        self._compute(again, None, stream)
             if together and (node in self._patient) != holding:        # an error drops what is held, and the switch
                 holding = not holding
                 gpu_op.hold_products(holding)
-            if timed:
-                t0 = time.perf_counter()
-                self._compute(node, out, stream)
-                node.runtime = (time.perf_counter() - t0) * 1000.0
+            t0 = time.perf_counter()
+            if isinstance(node.op, ManyOp):
+                arrays = {n: earlier(n) for n in self._parts.get(node, {}).values()}
+                arrays[node] = out
+                self._compute_many(node, arrays, stream)
+                del arrays
             else:
                 self._compute(node, out, stream)
+            if timed:
+                node.runtime = (time.perf_counter() - t0) * 1000.0
             if self.have_plan:
                 self._after_node(node)
         if together:

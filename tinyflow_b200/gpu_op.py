@@ -494,6 +494,20 @@ def dropout_add_layer_norm_backward(sum_arr, gamma, dout_arr, dsum_arr, din_arr,
                        _o(dbeta), _F(eps), state, cudaStream)
 
 
+# ---- gated dense layer (no counterpart in the reference) -----------------------------------------------------------------
+_GATE = {"sigmoid": 0, "relu": 1, "tanh": 2, "silu": 4, "gelu": 5}
+
+
+def gated_linear_forward(in_arr, weight, gates, out_arr, activation, cudaStream):
+    """out = act(in Wg) * (in Wv), ``weight`` = [Wg | Wv].  ``gates`` gets both projections, for the gradient; None: they are not kept."""
+    return _with_short(_LIB.TfGatedLinearForward, _h(in_arr), _h(weight), _o(gates), _h(out_arr), _code(_GATE, activation), cudaStream)
+
+
+def gated_linear_backward(in_arr, weight, gates, dout_arr, din_arr, dweight, activation, cudaStream):
+    """Gradients of :func:`gated_linear_forward`; either of ``din_arr`` and ``dweight`` may be None."""
+    return _with_short(_LIB.TfGatedLinearBackward, _h(in_arr), _h(weight), _h(gates), _h(dout_arr), _o(din_arr), _o(dweight), _code(_GATE, activation), cudaStream)
+
+
 def getInt(intp):
     return _LIB.getInt(intp)
 

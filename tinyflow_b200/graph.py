@@ -870,6 +870,194 @@ class FullyBNBackwardOp(BNBackwardOp):
     name = "FullyBNBackward"
 
 
+# ---- operators of several results (no counterpart in the reference) -------------------------------
+class ManyOp(Op):
+    """An operator of one launch and several results.  Its node stands for the first of them; each of the others is a node of a
+    :class:`PartOp` that has this node as its first input.  ``compute`` gets a list of ``1 + parts`` arrays; the array of a part that
+    is not in the graph is None and is not computed."""
+    parts = 0
+
+    def _node(self, inputs, **attrs):
+        return Op._node(self, inputs, shapes=[], **attrs)
+
+    def infer_shape(self, node, input_shapes, cudnnHandle):
+        node.shapes[:] = input_shapes
+        return self.result_shapes(input_shapes)[0]
+
+    def result_shapes(self, input_shapes):
+        raise NotImplementedError
+
+    def recompute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream):
+        """``compute`` once more in the same step: the same results."""
+        return self.compute(node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream)
+
+
+class PartOp(Op):
+    """Result ``part`` (1 is the first besides the node's own) of a :class:`ManyOp` node."""
+    name = "Part"
+
+    def __call__(self, node_A, part):
+        return self._node([node_A], part=part)
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        raise AssertionError("%s is computed with node %s" % (node.name, node.inputs[0].name))
+
+    def infer_shape(self, node, input_shapes, cudnnHandle):
+        whole = node.inputs[0]
+        return tuple(whole.op.result_shapes(whole.shapes)[node.part])
+
+
+# ---- layer normalisation over the last axis, alone and behind a residual sum (no counterpart in the reference) ----
+class LayerNormForwardOp(Op):
+    name = "LayerNormForward"
+
+    def __call__(self, node_A, gamma, beta, eps=1e-5):
+        return self._node([node_A, gamma, beta], eps=eps)
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        gpu_op.layer_norm_forward(input_vals[0], input_vals[1], input_vals[2], output_val, node.eps, cudaStream)
+        return 0
+
+    def gradient(self, node, output_grad):
+        dgamma = layer_norm_backward_op(node.inputs[0], node.inputs[1], output_grad, node.eps)
+        return [part_op(dgamma, 2), dgamma, part_op(dgamma, 1)]
+
+    def infer_shape(self, node, input_shapes, cudnnHandle):
+        return input_shapes[0]
+
+
+class LayerNormBackwardOp(ManyOp):
+    """Results: dgamma; dbeta, dinput."""
+    name = "LayerNormBackward"
+    parts = 2
+
+    def __call__(self, node_A, gamma, node_C, eps):
+        return self._node([node_A, gamma, node_C], eps=eps)
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        dgamma, dbeta, dinput = output_val
+        return gpu_op.layer_norm_backward(input_vals[0], input_vals[1], input_vals[2], dinput, dgamma, dbeta, node.eps, cudaStream)
+
+    def result_shapes(self, input_shapes):
+        return input_shapes[1], input_shapes[1], input_shapes[0]
+
+
+class DropoutAddLayerNormForwardOp(ManyOp):
+    """sum = residual + dropout(input) and layer_norm(sum): the operator gives both nodes.  Results: the sum; its normalisation."""
+    name = "DropoutAddLayerNormForward"
+    parts = 1
+
+    def __call__(self, node_A, residual, gamma, beta, dropout=0.0, eps=1e-5):
+        total = self._node([node_A, residual, gamma, beta], dropout=dropout, eps=eps, seed=[0], state=[None])
+        return total, normalised_sum_op(total, gamma, beta)
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        node.seed[0] = random.randint(0, 100)     # a fresh mask every step, as dropout draws it
+        return self.recompute(node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream)
+
+    def recompute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream):
+        node.state[0] = gpu_op.dropout_state(node.dropout, node.seed[0], node.state[0])
+        gpu_op.dropout_add_layer_norm_forward(*input_vals, *output_val, node.state[0], node.eps, cudaStream)
+        return 0
+
+    def gradient(self, node, output_grad):
+        # The gradient through the normalisation is one of the summands; the kernel that computes it adds the others.
+        summands, through = [output_grad], None
+        while type(summands[0].op) is AddOp:
+            summands[:1] = summands[0].inputs
+        for g in summands:
+            if type(g.op) is PartOp and type(g.inputs[0].op) is DropoutAddLayerNormBackwardOp and g.part == 2 and g.inputs[0].inputs[0] is node and len(g.inputs[0].inputs) == 3:
+                through = g
+        if through is None:                       # the normalisation has no reader
+            whole = dropout_add_layer_norm_backward_op(node, node.inputs[2], zeroslike_op(node), node)
+            whole.inputs.append(output_grad)
+            return [part_op(whole, 3), part_op(whole, 2), whole, part_op(whole, 1)]
+        whole = through.inputs[0]
+        rest = [g for g in summands if g is not through]
+        if rest:
+            whole.inputs.append(sum_node_list(rest))
+        return [part_op(whole, 3), through]           # gamma and beta have theirs from the normalisation
+
+    def result_shapes(self, input_shapes):
+        return input_shapes[0], input_shapes[0]
+
+
+class NormalisedSumOp(PartOp):
+    name = "NormalisedSum"
+
+    def __call__(self, total, gamma, beta):
+        return self._node([total, gamma, beta], part=1)
+
+    def gradient(self, node, output_grad):
+        total, gamma, _ = node.inputs
+        dgamma = dropout_add_layer_norm_backward_op(total, gamma, output_grad, total)
+        return [part_op(dgamma, 2), dgamma, part_op(dgamma, 1)]
+
+
+class DropoutAddLayerNormBackwardOp(ManyOp):
+    """Inputs: the sum, gamma, the normalisation's gradient, and what else reaches the sum, if anything does.
+    Results: dgamma; dbeta, dresidual, dinput."""
+    name = "DropoutAddLayerNormBackward"
+    parts = 3
+
+    def __call__(self, total, gamma, node_C, forward):
+        return self._node([total, gamma, node_C], eps=forward.eps, state=forward.state)
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        dgamma, dbeta, dresidual, dinput = output_val
+        total, gamma, dout = input_vals[:3]
+        return gpu_op.dropout_add_layer_norm_backward(total, gamma, dout, input_vals[3] if len(input_vals) > 3 else None, dinput, dresidual, dgamma, dbeta,
+                                                      node.state[0], node.eps, cudaStream)
+
+    def result_shapes(self, input_shapes):
+        return input_shapes[1], input_shapes[1], input_shapes[0], input_shapes[0]
+
+
+# ---- gated dense layer (no counterpart in the reference) -------------------------------------------
+class GatedLinearForwardOp(ManyOp):
+    """act(X Wg) * (X Wv), weight = [Wg | Wv].  Results: that; both projections, where a gradient needs them."""
+    name = "GatedLinearForward"
+    parts = 1
+
+    def __call__(self, node_A, weight, activation="silu"):
+        return self._node([node_A, weight], activation=activation, gates=[None])
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        return gpu_op.gated_linear_forward(input_vals[0], input_vals[1], output_val[1], output_val[0], node.activation, cudaStream)
+
+    def gradient(self, node, output_grad):
+        if node.gates[0] is None:
+            node.gates[0] = part_op(node, 1)
+        dweight = gated_linear_backward_op(node.inputs[0], node.inputs[1], node.gates[0], output_grad, node.activation)
+        return [part_op(dweight, 1), dweight]
+
+    def result_shapes(self, input_shapes):
+        x, weight = input_shapes
+        return (x[0], weight[1] // 2), (x[0], weight[1])
+
+
+class GatedLinearBackwardOp(ManyOp):
+    """Results: dweight; dinput."""
+    name = "GatedLinearBackward"
+    parts = 1
+
+    def __call__(self, node_A, weight, gates, node_D, activation):
+        return self._node([node_A, weight, gates, node_D], activation=activation)
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        x, weight, gates, dout = input_vals
+        return gpu_op.gated_linear_backward(x, weight, gates, dout, output_val[1], output_val[0], node.activation, cudaStream)
+
+    def result_shapes(self, input_shapes):
+        return input_shapes[1], input_shapes[0]
+
+
 # ---- concat (ConcatForwardOp / ConcatBackwardOp: autodiff.py:1935-1984) ---------------------------
 class ConcatForwardOp(Op):
     name = "ConcatForward"
@@ -1052,6 +1240,14 @@ concat_forward_op = ConcatForwardOp()
 concat_backward_op = ConcatBackwardOp()
 squeeze_op = SqueezeOp()
 squeeze_gradient_op = SqueezeGradientOp()
+part_op = PartOp()
+layer_norm_op = LayerNormForwardOp()
+layer_norm_backward_op = LayerNormBackwardOp()
+dropout_add_layer_norm_op = DropoutAddLayerNormForwardOp()
+dropout_add_layer_norm_backward_op = DropoutAddLayerNormBackwardOp()
+normalised_sum_op = NormalisedSumOp()
+gated_linear_op = GatedLinearForwardOp()
+gated_linear_backward_op = GatedLinearBackwardOp()
 
 
 # ---- autodiff and graph utilities (autodiff.py:2894-3027) ------------------------------------------------
