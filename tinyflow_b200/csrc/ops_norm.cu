@@ -33,6 +33,7 @@ struct NormArgs {
   int64_t rows;
   int D;
   float eps, p, scale;
+  uint32_t threshold;        // of the upper word of the mixed number: below it an element is dropped
   unsigned long long seed;
   const uint32_t* seed_word;
   AmaxOut am;
@@ -40,13 +41,15 @@ struct NormArgs {
 
 template <int VEC> struct Pieces;
 template <> struct Pieces<4> { typedef float4 T; };
+template <> struct Pieces<2> { typedef float2 T; };
 template <> struct Pieces<1> { typedef float T; };
 template <int VEC> __device__ __forceinline__ void get(float* v, const float* __restrict__ p) { *reinterpret_cast<typename Pieces<VEC>::T*>(v) = __ldg(reinterpret_cast<const typename Pieces<VEC>::T*>(p)); }
+template <int VEC> __device__ __forceinline__ void held_at(float* v, const float* p) { *reinterpret_cast<typename Pieces<VEC>::T*>(v) = *reinterpret_cast<const typename Pieces<VEC>::T*>(p); }
 template <int VEC> __device__ __forceinline__ void put(float* p, const float* v) { *reinterpret_cast<typename Pieces<VEC>::T*>(p) = *reinterpret_cast<const typename Pieces<VEC>::T*>(v); }
 
 // Sums over the G threads that share a row, the same in all of them.  Two buffers in turn: a thread that writes one for the next sum
 // has passed the barrier behind which every thread had read the one before.
-template <int G, int R> struct RowSum {
+template <int G> struct RowSum {
   static constexpr int kWarps = G / 32;
   float (*held)[2][3][kWarps];
   int group, turn = 0;
@@ -61,8 +64,7 @@ template <int G, int R> struct RowSum {
 #pragma unroll
       for (int i = 0; i < N; ++i) held[group][turn][i][w] = v[i];
     }
-    if (R == 1) __syncthreads();
-    else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(G) : "memory");
+    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(G) : "memory");
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       v[i] = held[group][turn][i][0];
@@ -74,183 +76,253 @@ template <int G, int R> struct RowSum {
 };
 
 __device__ __forceinline__ unsigned long long seed_of(const NormArgs& a) { return a.seed_word ? (unsigned long long)__ldg(a.seed_word) : a.seed; }
-__device__ __forceinline__ float dropped(const NormArgs& a, unsigned long long seed, int64_t i, float v) {
-  return a.p == 0.f || uniform01(seed, (unsigned long long)i) >= a.p ? v * a.scale : 0.f;
+// What uniform01(seed, i) >= p says, from z = (i + 1) * step + seed * key: its 24 bits are compared as a whole number, and only the
+// upper word of the mix decides.  z of the elements of a thread differ by constants.
+constexpr unsigned long long kMixStep = 0x9E3779B97F4A7C15ull, kMixKey = 0xD1342543DE82EF95ull;
+__device__ __forceinline__ float dropped(const NormArgs& a, unsigned long long z, float v) {
+  if (a.p == 0.f) return v * a.scale;
+  z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+  z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+  const uint32_t upper = (uint32_t)(z >> 32);
+  return (upper ^ upper >> 31) >= a.threshold ? v * a.scale : 0.f;
+}
+__device__ __forceinline__ unsigned long long mix_start(unsigned long long seed, int64_t i) { return (unsigned long long)(i + 1) * kMixStep + seed * kMixKey; }
+
+// A row of D elements is dealt to G threads, NV pieces of VEC elements each: piece v of thread t begins at element (v * G + t) * VEC.
+// The shape of a launch (with_shape) is the smallest that fits, in steps of four elements a thread, so only the last of them need a look
+// at D; the rest are there at compile time.  (With pieces of 4 to 16 elements and a look at every one, scalar rows of 2050 elements took
+// 234 instructions an element in the backward kernel.)
+template <int VEC, int G, int NV> struct Row {
+  static constexpr int kStep = 4 / VEC;
+  int D, t;
+  __device__ __forceinline__ int at(int v) const { return (v * G + t) * VEC; }
+  __device__ __forceinline__ bool has(int v) const { return v < NV - kStep || at(v) < D; }
+  // pair i of the thread's elements: v where the row has it, else 0 (a pair may lie in two pieces of one element)
+  __device__ __forceinline__ float2 where(int i, float v) const {
+    const int first = 2 * i / VEC, second = (2 * i + 1) / VEC;
+    return make_float2(has(first) ? v : 0.f, has(second) ? v : 0.f);
+  }
+};
+
+// Arithmetic goes two elements at a time (a packed instruction each).
+template <int N> __device__ __forceinline__ float2& pair(float (&x)[N], int i) { return reinterpret_cast<float2*>(x)[i]; }
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+// The sum of a thread's elements, in four chains
+template <int E> __device__ __forceinline__ float row_part(float (&x)[E]) {
+  float2 p[2] = {both(0.f), both(0.f)};
+#pragma unroll
+  for (int i = 0; i < E / 2; ++i) p[i & 1] = __fadd2_rn(p[i & 1], pair(x, i));
+  p[0] = __fadd2_rn(p[0], p[1]);
+  return p[0].x + p[0].y;
 }
 
-// R groups of G threads, a row each, NV * VEC elements of it per thread.
+// R groups, a row each.
 template <int VEC, int G, int R, int NV, bool RES>
 __global__ void __launch_bounds__(G * R) norm_fwd_kernel(const NormArgs a) {
   __shared__ float held[R][2][3][G / 32];
   grid_dep_sync();
-  const int t = threadIdx.x % G, group = threadIdx.x / G, D = a.D;
-  RowSum<G, R> add{held, group};
+  const int group = threadIdx.x / G, D = a.D;
+  constexpr int E = NV * VEC;
+  const Row<VEC, G, NV> r{D, (int)(threadIdx.x % G)};
+  const float over_d = 1.f / (float)D;
+  RowSum<G> add{held, group};
   const unsigned long long seed = RES ? seed_of(a) : 0;
-  uint32_t m = 0;
+  float m = 0.f;              // a NaN does not raise it: it goes through the pack whatever the scale
   for (int64_t row = (int64_t)blockIdx.x * R + group; row < a.rows; row += (int64_t)gridDim.x * R) {
     const int64_t base = row * D;
-    float x[NV][VEC];
+    const unsigned long long z = RES ? mix_start(seed, base + r.t * VEC) : 0;
+    float x[E];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = (v * G + t) * VEC;
-      if (c < D) get<VEC>(x[v], a.x + base + c);
+      if (r.has(v)) get<VEC>(x + v * VEC, a.x + base + r.at(v));
       else
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) x[v][j] = 0.f;
+        for (int j = 0; j < VEC; ++j) x[v * VEC + j] = 0.f;
     }
     if (RES) {
-      float r[NV][VEC];
+      float old[E];
+#pragma unroll
+      for (int v = 0; v < NV; ++v) if (r.has(v)) get<VEC>(old + v * VEC, a.residual + base + r.at(v));
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        const int c = (v * G + t) * VEC;
-        if (c < D) get<VEC>(r[v], a.residual + base + c);
-      }
+        if (r.has(v)) {
 #pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        const int c = (v * G + t) * VEC;
-        if (c < D) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) x[v][j] = r[v][j] + dropped(a, seed, base + c + j, x[v][j]);
-          put<VEC>(a.sum + base + c, x[v]);
+          for (int j = 0; j < VEC; ++j) x[v * VEC + j] = old[v * VEC + j] + dropped(a, z + (v * G * VEC + j) * kMixStep, x[v * VEC + j]);
+          put<VEC>(a.sum + base + r.at(v), x + v * VEC);
         }
       }
       if (!a.y) continue;
     }
-    float sum[1] = {0.f};
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) sum[0] += x[v][j];
+    float sum[1] = {row_part(x)};
     add(sum);
-    const float mean = sum[0] / (float)D;
-    float squares[1] = {0.f};
+    const float mean = sum[0] * over_d;
+    float2 sq = both(0.f);
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const bool there = (v * G + t) * VEC < D;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) { x[v][j] = there ? x[v][j] - mean : 0.f; squares[0] = fmaf(x[v][j], x[v][j], squares[0]); }
+    for (int i = 0; i < E / 2; ++i) {
+      pair(x, i) = __fadd2_rn(pair(x, i), r.where(i, -mean));
+      sq = __ffma2_rn(pair(x, i), pair(x, i), sq);
     }
+    float squares[1] = {sq.x + sq.y};
     add(squares);
-    const float inv = __frsqrt_rn(squares[0] / (float)D + a.eps);
+    const float2 inv = both(rsqrtf(fmaf(squares[0], over_d, a.eps)));
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = (v * G + t) * VEC;
-      if (c < D) {
+      if (r.has(v)) {
         float w[VEC], b[VEC];
-        get<VEC>(w, a.gamma + c);
-        get<VEC>(b, a.beta + c);
+        get<VEC>(w, a.gamma + r.at(v));
+        get<VEC>(b, a.beta + r.at(v));
+        if (VEC > 1) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) { b[j] = fmaf(x[v][j] * inv, w[j], b[j]); m = max(m, amax_bits(b[j])); }
-        put<VEC>(a.y + base + c, b);
+          for (int i = 0; i < VEC / 2; ++i) pair(b, i) = __ffma2_rn(__fmul2_rn(pair(x, v * VEC / 2 + i), inv), pair(w, i), pair(b, i));
+        } else {
+          b[0] = fmaf(x[v] * inv.x, w[0], b[0]);
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) m = fmaxf(m, fabsf(b[j]));
+        put<VEC>(a.y + base + r.at(v), b);
       }
     }
   }
-  amax_commit(a.am, m);
+  amax_commit(a.am, __float_as_uint(m));
 }
 
-// Persistent: a group takes every (grid * R)-th row, so a thread always has the same columns and keeps their parts of dgamma and dbeta
-// in registers; the groups' parts are added in group order and left as one row of `part` per block.
-template <int VEC, int G, int R, int NV, bool RES>
-__global__ void __launch_bounds__(G * R) norm_bwd_kernel(const NormArgs a) {
-  __shared__ float held[R][2][3][G / 32];
-  extern __shared__ float sums[];              // [2 * D], with more than one group
-  grid_dep_sync();
-  const int t = threadIdx.x % G, group = threadIdx.x / G, D = a.D;
-  RowSum<G, R> add{held, group};
-  const unsigned long long seed = RES ? seed_of(a) : 0;
-  uint32_t m = 0;
-  float dgamma[NV][VEC], dbeta[NV][VEC];
+// A copy of this thread's own, or zeros
+template <int BYTES> __device__ __forceinline__ void copy_ahead(uint32_t to, const float* from, bool there) {
+  const int bytes = there ? BYTES : 0;
+  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES), "r"(bytes) : "memory");
+}
+
+// Persistent: blockDim / G groups, each taking every (grid * groups)-th row, so a thread always has the same columns and keeps their
+// parts of dgamma and dbeta in registers; the groups' parts are added in group order and left as one row of `part` per block.
+// A thread copies its elements of the rows ahead of the present one to shared memory itself (`depth` of them in flight), and nobody
+// else reads them: the copies need no barrier.
+constexpr int kBwdThreads = 512;            // most threads of a block
+constexpr int kBwdSmem = 224 * 1024;
+template <int VEC, int G, int NV, bool RES>
+__global__ void __launch_bounds__(kBwdThreads, 1) norm_bwd_kernel(const NormArgs a, int depth) {
+  constexpr int kArrays = RES ? 3 : 2;
+  constexpr uint32_t kPiece = kBwdThreads * VEC * 4, kStage = kArrays * NV * kPiece;
+  __shared__ float held[kBwdThreads / G][2][3][G / 32];
+  extern __shared__ __align__(16) float ring[];            // [depth][array][NV][kBwdThreads][VEC], then gamma; at the end the groups' sums [group][2 * D]
+  float* const gamma = ring + depth * (kStage / 4);
+  const int group = threadIdx.x / G, groups = blockDim.x / G, D = a.D;
+  const Row<VEC, G, NV> r{D, (int)(threadIdx.x % G)};
+  const float over_d = 1.f / (float)D;
+  const bool with_sum = RES && a.dsum;
+  const int64_t first = (int64_t)blockIdx.x * groups + group, stride = (int64_t)gridDim.x * groups;
+  const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * VEC * 4u;
+  auto fetch = [&](int64_t row, uint32_t stage) {          // `stage` in bytes
+    if (row < a.rows) {
+      const int64_t from = row * D + r.t * VEC;
 #pragma unroll
-  for (int v = 0; v < NV; ++v)
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) dgamma[v][j] = dbeta[v][j] = 0.f;
-  for (int64_t row = (int64_t)blockIdx.x * R + group; row < a.rows; row += (int64_t)gridDim.x * R) {
-    const int64_t base = row * D;
-    float x[NV][VEC], dy[NV][VEC];
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int c = (v * G + t) * VEC;
-      if (c < D) { get<VEC>(x[v], a.x + base + c); get<VEC>(dy[v], a.dy + base + c); }
-      else
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) x[v][j] = dy[v][j] = 0.f;
-    }
-    float sum[1] = {0.f};
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) sum[0] += x[v][j];
-    add(sum);
-    const float mean = sum[0] / (float)D;
-    float three[3] = {0.f, 0.f, 0.f};          // (x - mean)^2, g, g * (x - mean)
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int c = (v * G + t) * VEC;
-      if (c < D) {
-        float w[VEC];
-        get<VEC>(w, a.gamma + c);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          x[v][j] -= mean;
-          const float g = w[j] * dy[v][j];
-          three[0] = fmaf(x[v][j], x[v][j], three[0]);
-          three[1] += g;
-          three[2] = fmaf(g, x[v][j], three[2]);
-        }
+      for (int v = 0; v < NV; ++v) {
+        const bool there = r.has(v);
+        const int64_t e = there ? from + v * G * VEC : 0;
+        copy_ahead<VEC * 4>(mine + stage + v * kPiece, a.x + e, there);
+        copy_ahead<VEC * 4>(mine + stage + (NV + v) * kPiece, a.dy + e, there);
+        if (with_sum) copy_ahead<VEC * 4>(mine + stage + (2 * NV + v) * kPiece, a.dsum + e, there);
       }
     }
-    add(three);
-    const float inv = __frsqrt_rn(three[0] / (float)D + a.eps);
-    const float mean_g = three[1] / (float)D, mean_gx = three[2] * inv / (float)D;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const char* const own = reinterpret_cast<const char*>(ring) + threadIdx.x * VEC * 4;
+  auto fetched = [&](float* to, uint32_t stage, int piece) {
+    *reinterpret_cast<typename Pieces<VEC>::T*>(to) = *reinterpret_cast<const typename Pieces<VEC>::T*>(own + stage + piece * kPiece);
+  };
+  // gamma of pair i of the thread's elements (what lies behind the last one meets zeros)
+  auto gammas = [&](int i) -> float2 {
+    if (VEC > 1) return *reinterpret_cast<const float2*>(gamma + r.at(2 * i / VEC) + 2 * i % VEC);
+    return make_float2(gamma[r.at(2 * i)], gamma[r.at(2 * i + 1)]);
+  };
+  grid_dep_sync();
+  RowSum<G> add{held, group};
+  const unsigned long long seed = RES ? seed_of(a) : 0;
+  float m = 0.f;
+  constexpr int E = NV * VEC;
+  float dgamma[E], dbeta[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) dgamma[i] = dbeta[i] = 0.f;
+  for (int i = 0; i < depth; ++i) fetch(first + i * stride, i * kStage);
+  for (int c = threadIdx.x; c < G * E; c += blockDim.x) gamma[c] = c < D ? __ldg(a.gamma + c) : 0.f;
+  __syncthreads();
+  uint32_t stage = 0;
+  for (int64_t row = first; row < a.rows; row += stride) {
+    if (depth == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else if (depth == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else asm volatile("cp.async.wait_group 3;" ::: "memory");
+    float x[E], dy[E], ds[RES ? E : 1];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = (v * G + t) * VEC;
-      if (c < D) {
-        float w[VEC], ds[VEC];
-        get<VEC>(w, a.gamma + c);
-        if (RES && a.dsum) get<VEC>(ds, a.dsum + base + c);
+      if (with_sum) fetched(ds + v * VEC, stage, 2 * NV + v);
+      fetched(dy + v * VEC, stage, NV + v);
+      fetched(x + v * VEC, stage, v);
+    }
+    float sum[1] = {row_part(x)};
+    add(sum);
+    const float mean = sum[0] * over_d;
+    float2 sq = both(0.f), sg = both(0.f), sgx = both(0.f);      // (x - mean)^2, g, g * (x - mean)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float xh = x[v][j] * inv;
-          dgamma[v][j] = fmaf(dy[v][j], xh, dgamma[v][j]);
-          dbeta[v][j] += dy[v][j];
-          const float d = inv * (w[j] * dy[v][j] - mean_g - xh * mean_gx);
-          ds[j] = RES && a.dsum ? ds[j] + d : d;
-        }
+    for (int i = 0; i < E / 2; ++i) {
+      pair(x, i) = __fadd2_rn(pair(x, i), r.where(i, -mean));
+      const float2 g = __fmul2_rn(gammas(i), pair(dy, i));       // where the row has ended dy is zero
+      sq = __ffma2_rn(pair(x, i), pair(x, i), sq);
+      sg = __fadd2_rn(sg, g);
+      sgx = __ffma2_rn(g, pair(x, i), sgx);
+    }
+    float three[3] = {sq.x + sq.y, sg.x + sg.y, sgx.x + sgx.y};
+    add(three);
+    fetch(row + depth * stride, stage);        // what was there has been read: three depends on the last of it
+    stage += kStage;
+    if (stage == depth * kStage) stage = 0;
+    const float inv = rsqrtf(fmaf(three[0], over_d, a.eps));
+    // ds = inv * g - inv * mean(g) - (x - mean) * inv^2 * mean(g * xh)
+    const float2 inv2 = both(inv), shift = both(-inv * (three[1] * over_d)), slope = both(-inv * (inv * (inv * (three[2] * over_d))));
+    const int64_t base = row * D + r.t * VEC;
+    const unsigned long long z = RES ? mix_start(seed, base) : 0;
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      const float2 g = __fmul2_rn(gammas(i), pair(dy, i));
+      pair(dgamma, i) = __ffma2_rn(__fmul2_rn(pair(dy, i), inv2), pair(x, i), pair(dgamma, i));
+      pair(dbeta, i) = __fadd2_rn(pair(dbeta, i), pair(dy, i));
+      pair(x, i) = __ffma2_rn(g, inv2, __ffma2_rn(pair(x, i), slope, shift));
+      if (with_sum) pair(x, i) = __fadd2_rn(pair(x, i), pair(ds, i));
+    }
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      if (r.has(v)) {
+        float* const d = x + v * VEC;
         if (a.dx) {
-          put<VEC>(a.dx + base + c, ds);
+          put<VEC>(a.dx + base + v * G * VEC, d);
           if (!RES || !a.dbranch)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) m = max(m, amax_bits(ds[j]));
+            for (int j = 0; j < VEC; ++j) m = fmaxf(m, fabsf(d[j]));
         }
         if (RES && a.dbranch) {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) { ds[j] = dropped(a, seed, base + c + j, ds[j]); m = max(m, amax_bits(ds[j])); }
-          put<VEC>(a.dbranch + base + c, ds);
+          for (int j = 0; j < VEC; ++j) { d[j] = dropped(a, z + (v * G * VEC + j) * kMixStep, d[j]); m = fmaxf(m, fabsf(d[j])); }
+          put<VEC>(a.dbranch + base + v * G * VEC, d);
         }
       }
     }
   }
-  amax_commit(a.am, m);
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  amax_commit(a.am, __float_as_uint(m));
   if (!a.part) return;
-  float* const out = a.part + (int64_t)blockIdx.x * 2 * D;
-#pragma unroll 1
-  for (int r = 0; r < R; ++r) {
-    if (R > 1) __syncthreads();
-    if (group != r) continue;
+  __syncthreads();
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int c = (v * G + t) * VEC;
-      if (c < D) {
-        if (r) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) { dgamma[v][j] += sums[c + j]; dbeta[v][j] += sums[D + c + j]; }
-        }
-        float* const to = R > 1 && r + 1 < R ? sums : out;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) { to[c + j] = dgamma[v][j]; to[D + c + j] = dbeta[v][j]; }
-      }
+  for (int v = 0; v < NV; ++v) {
+    if (r.has(v)) {
+      put<VEC>(ring + (size_t)group * 2 * D + r.at(v), dgamma + v * VEC);
+      put<VEC>(ring + (size_t)group * 2 * D + D + r.at(v), dbeta + v * VEC);
     }
+  }
+  __syncthreads();
+  float* const out = a.part + (int64_t)blockIdx.x * 2 * D;
+  for (int c = threadIdx.x; c < 2 * D; c += blockDim.x) {
+    float total = ring[c];
+    for (int g = 1; g < groups; ++g) total += ring[(size_t)g * 2 * D + c];
+    out[c] = total;
   }
 }
 
@@ -259,7 +331,7 @@ constexpr int kLongThreads = 512;
 template <bool RES> __global__ void __launch_bounds__(kLongThreads) norm_long_fwd_kernel(const NormArgs a) {
   __shared__ float held[1][2][3][kLongThreads / 32];
   grid_dep_sync();
-  RowSum<kLongThreads, 1> add{held, 0};
+  RowSum<kLongThreads> add{held, 0};
   const unsigned long long seed = RES ? seed_of(a) : 0;
   const int D = a.D;
   uint32_t m = 0;
@@ -269,7 +341,7 @@ template <bool RES> __global__ void __launch_bounds__(kLongThreads) norm_long_fw
     float sum[1] = {0.f};
     for (int c = threadIdx.x; c < D; c += kLongThreads) {
       float v = a.x[base + c];
-      if (RES) { v = a.residual[base + c] + dropped(a, seed, base + c, v); a.sum[base + c] = v; }
+      if (RES) { v = a.residual[base + c] + dropped(a, mix_start(seed, base + c), v); a.sum[base + c] = v; }
       sum[0] += v;
     }
     if (RES && !a.y) continue;
@@ -290,7 +362,7 @@ template <bool RES> __global__ void __launch_bounds__(kLongThreads) norm_long_fw
 template <bool RES> __global__ void __launch_bounds__(kLongThreads) norm_long_bwd_kernel(const NormArgs a) {
   __shared__ float held[1][2][3][kLongThreads / 32];
   grid_dep_sync();
-  RowSum<kLongThreads, 1> add{held, 0};
+  RowSum<kLongThreads> add{held, 0};
   const unsigned long long seed = RES ? seed_of(a) : 0;
   const int D = a.D;
   uint32_t m = 0;
@@ -319,7 +391,7 @@ template <bool RES> __global__ void __launch_bounds__(kLongThreads) norm_long_bw
         a.dx[row * D + c] = d;
         if (!RES || !a.dbranch) m = max(m, amax_bits(d));
       }
-      if (RES && a.dbranch) { d = dropped(a, seed, row * D + c, d); a.dbranch[row * D + c] = d; m = max(m, amax_bits(d)); }
+      if (RES && a.dbranch) { d = dropped(a, mix_start(seed, row * D + c), d); a.dbranch[row * D + c] = d; m = max(m, amax_bits(d)); }
     }
   }
   amax_commit(a.am, m);
@@ -351,8 +423,13 @@ __global__ void __launch_bounds__(1024) norm_params_kernel(const float* __restri
   const int per_run = (blocks + 31) / 32, b0 = run * per_run, b1 = min(blocks, b0 + per_run);
   float sum = 0.f;
   if (c < 2ll * D) {
-#pragma unroll 8
-    for (int b = b0; b < b1; ++b) sum += __ldg(part + (int64_t)b * 2 * D + c);
+    for (int b = b0; b < b1; b += 8) {           // eight loads in flight
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = b + i < b1 ? __ldg(part + (int64_t)(b + i) * 2 * D + c) : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += v[i];
+    }
   }
   held[run][lane] = sum;
   __syncthreads();
@@ -367,43 +444,46 @@ __global__ void __launch_bounds__(1024) norm_params_kernel(const float* __restri
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------
-// Threads of a row and elements of it per thread; calls f(G, R, NV as constants), or returns false where the row is too long.
+// Threads of a row, rows of a block (forward) and pieces of a row per thread: calls f with them as constants, or returns false where the
+// row is too long for MOST threads.
 template <int VEC, int MOST, class F> static bool with_shape(int D, F&& f) {
-#define TF_NORM_SHAPE(G, R, E) if constexpr (E <= MOST) if (D <= G * E) { f(std::integral_constant<int, G>(), std::integral_constant<int, R>(), std::integral_constant<int, E / VEC>()); return true; }
+#define TF_NORM_SHAPE(G, R, E) if constexpr (G <= MOST) if (D <= G * E) { f(std::integral_constant<int, G>(), std::integral_constant<int, R>(), std::integral_constant<int, E / VEC>()); return true; }
   TF_NORM_SHAPE(32, 8, 4)
   TF_NORM_SHAPE(32, 8, 8)
+  TF_NORM_SHAPE(32, 8, 12)
   TF_NORM_SHAPE(32, 8, 16)
+  TF_NORM_SHAPE(64, 4, 12)
   TF_NORM_SHAPE(64, 4, 16)
+  TF_NORM_SHAPE(128, 2, 12)
   TF_NORM_SHAPE(128, 2, 16)
+  TF_NORM_SHAPE(256, 1, 12)
   TF_NORM_SHAPE(256, 1, 16)
+  TF_NORM_SHAPE(512, 1, 12)
   TF_NORM_SHAPE(512, 1, 16)
-  TF_NORM_SHAPE(512, 1, 32)
+  TF_NORM_SHAPE(1024, 1, 12)
+  TF_NORM_SHAPE(1024, 1, 16)
 #undef TF_NORM_SHAPE
   return false;
 }
-static bool vectors(int D, std::initializer_list<const void*> all) {
-  if (D % 4) return false;
-  for (const void* p : all) if (!aligned16(p)) return false;         // a null pointer counts as aligned
-  return true;
+// Elements that one access takes: f(4), f(2) or f(1) as a constant
+template <class F> static bool with_width(int D, std::initializer_list<const void*> all, F&& f) {
+  uintptr_t bits = (uintptr_t)D * 4;
+  for (const void* p : all) bits |= reinterpret_cast<uintptr_t>(p);         // a null pointer counts as aligned
+  return bits % 16 == 0 ? f(std::integral_constant<int, 4>()) : bits % 8 == 0 ? f(std::integral_constant<int, 2>()) : f(std::integral_constant<int, 1>());
 }
 template <bool RES> static cudaError_t launch_norm_fwd(const NormArgs& a, cudaStream_t s) {
   cudaError_t e = cudaSuccess;
   auto run = [&](auto vec) {
     constexpr int VEC = decltype(vec)::value;
-    return with_shape<VEC, 32>(a.D, [&](auto g, auto r, auto nv) {
+    return with_shape<VEC, 1024>(a.D, [&](auto g, auto r, auto nv) {
       constexpr int G = decltype(g)::value, R = decltype(r)::value, NV = decltype(nv)::value;
       const int64_t blocks = (a.rows + R - 1) / R;
       e = launch_dep(norm_fwd_kernel<VEC, G, R, NV, RES>, dim3((unsigned)std::min<int64_t>(blocks, 1 << 20)), dim3(G * R), 0, s, a);
     });
   };
-  const bool vec = vectors(a.D, {a.x, a.residual, a.gamma, a.beta, a.sum, a.y});
-  if (!(vec ? run(std::integral_constant<int, 4>()) : run(std::integral_constant<int, 1>())))
+  if (!with_width(a.D, {a.x, a.residual, a.gamma, a.beta, a.sum, a.y}, run))
     e = launch_dep(norm_long_fwd_kernel<RES>, dim3((unsigned)std::min<int64_t>(a.rows, 4 * device_sm_count())), dim3(kLongThreads), 0, s, a);
   return e;
-}
-constexpr int kBwdRegs = 16;             // elements per thread of the backward kernel
-static int norm_bwd_blocks(int64_t rows, int R, int threads) {
-  return (int)std::min<int64_t>((rows + R - 1) / R, (int64_t)device_sm_count() * std::max(1, 512 / threads));
 }
 template <bool RES> static int run_norm_bwd(NormArgs a, float* dgamma, float* dbeta, int* memorytoSaving, cudaStream_t s, const char* what) {
   const bool sums = dgamma || dbeta;
@@ -413,16 +493,22 @@ template <bool RES> static int run_norm_bwd(NormArgs a, float* dgamma, float* db
   cudaError_t e = cudaSuccess;
   auto run = [&](auto vec) {
     constexpr int VEC = decltype(vec)::value;
-    return with_shape<VEC, kBwdRegs>(a.D, [&](auto g, auto r, auto nv) {
-      constexpr int G = decltype(g)::value, R = decltype(r)::value, NV = decltype(nv)::value;
-      blocks = norm_bwd_blocks(a.rows, R, G * R);
+    return with_shape<VEC, kBwdThreads>(a.D, [&](auto g, auto, auto nv) {
+      constexpr int G = decltype(g)::value, NV = decltype(nv)::value;
+      // one block per SM, with as many groups as there are rows for
+      const int sms = device_sm_count(), groups = (int)std::max<int64_t>(1, std::min<int64_t>(kBwdThreads / G, (a.rows + sms - 1) / sms)), threads = groups * G;
+      blocks = (int)std::min<int64_t>((a.rows + groups - 1) / groups, sms);
       const size_t bytes = sizeof(float) * 2 * (size_t)a.D * blocks;
       if (sums && blocks && !(a.part = (float*)lease.scratch(kScratchNorm, bytes))) { out_of_memory = 1; shortage(bytes); return; }
-      if (blocks) e = launch_dep(norm_bwd_kernel<VEC, G, R, NV, RES>, dim3(blocks), dim3(G * R), R > 1 && sums ? sizeof(float) * 2 * a.D : 0, s, a);
+      const int stage = kBwdThreads * NV * VEC * (int)sizeof(float) * (RES ? 3 : 2), depth = std::min(4, (kBwdSmem - G * NV * VEC * (int)sizeof(float)) / stage);
+      static_assert(kBwdThreads * NV * VEC * 4 * 3 * 2 + G * NV * VEC * 4 <= kBwdSmem, "two rows ahead and gamma always fit");
+      static const cudaError_t attr = cudaFuncSetAttribute(norm_bwd_kernel<VEC, G, NV, RES>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBwdSmem);
+      e = attr;
+      if (blocks && e == cudaSuccess)
+        e = launch_dep(norm_bwd_kernel<VEC, G, NV, RES>, dim3(blocks), dim3(threads), (size_t)stage * depth + sizeof(float) * G * NV * VEC, s, a, depth);
     });
   };
-  const bool vec = vectors(a.D, {a.x, a.gamma, a.dy, a.dsum, a.dx, a.dbranch});
-  if (!(vec ? run(std::integral_constant<int, 4>()) : run(std::integral_constant<int, 1>()))) {
+  if (!with_width(a.D, {a.x, a.gamma, a.dy, a.dsum, a.dx, a.dbranch}, run)) {
     const unsigned across = (unsigned)((a.D + 255) / 256);
     const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(a.rows, 65535), 4 * device_sm_count() / across));
     const int64_t per_block = (a.rows + shares - 1) / shares;
@@ -464,6 +550,10 @@ int check_norm(const char* what, const DLArray* x, float eps, int64_t* rows, int
   for (int i = 0; i + 1 < x->ndim; ++i) r *= x->shape[i];
   *rows = r; *D = (int)last;
   return 0;
+}
+void set_dropout(NormArgs& a, const ResidualDropoutState* st) {
+  a.p = st->p; a.scale = 1.f / (1.f - st->p); a.seed = st->seed;
+  a.threshold = (uint32_t)ceil((double)st->p * 16777216.0) << 8;          // k * 2^-24 >= p is k >= p * 2^24, and a rate below one has 24 bits at most
 }
 float* opt_out(DLArrayHandle a) { return a ? out_f32(a) : nullptr; }
 
@@ -538,7 +628,7 @@ int TfDropoutAddLayerNormForward(const DLArrayHandle input, const DLArrayHandle 
   a.sum = out_f32(sum); a.y = opt_out(output); a.eps = eps;
   st->seed_word = t_recording ? recording_seed((unsigned)st->seed) : nullptr;
   st->recording = recording_id();
-  a.p = st->p; a.scale = 1.f / (1.f - st->p); a.seed = st->seed; a.seed_word = st->seed_word;
+  set_dropout(a, st); a.seed_word = st->seed_word;
   if (n == 0) return 0;
   if (a.y) a.am = amax_track_begin(a.y);
   note_compute_stream(s);
@@ -565,7 +655,7 @@ int TfDropoutAddLayerNormBackward(const DLArrayHandle sum, const DLArrayHandle g
   a.x = (const float*)sum->data; a.gamma = (const float*)gamma->data; a.dy = (const float*)doutput->data; a.dsum = dsum ? (const float*)dsum->data : nullptr; a.eps = eps;
   a.dx = opt_out(dresidual); a.dbranch = opt_out(dinput);
   float *dg = opt_out(dgamma), *db = opt_out(dbeta);
-  a.p = st->p; a.scale = 1.f / (1.f - st->p); a.seed = st->seed;
+  set_dropout(a, st);
   a.seed_word = st->recording && st->recording == recording_id() ? st->seed_word : nullptr;
   if (a.D == 0 || !(a.dx || a.dbranch || dg || db)) return 0;
   if (a.rows && (a.dx || a.dbranch)) a.am = amax_track_begin(a.dbranch ? a.dbranch : a.dx);
