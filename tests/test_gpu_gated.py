@@ -63,7 +63,7 @@ def check(env, M, K, F, activation, misaligned=0, path=0, arithmetic="3xfp16", s
 
 SMALL = [(1, 1, 1), (1, 7, 3), (3, 1, 5), (5, 9, 2), (16, 33, 31), (17, 64, 32), (64, 100, 33), (33, 65, 64), (130, 129, 65), (7, 1000, 130)]
 LARGE = [(1, 1024, 1024), (2, 1500, 1002), (9, 1024, 2048), (16, 2052, 514), (64, 784, 256), (100, 300, 1000), (300, 520, 500), (777, 500, 1003), (129, 1030, 1024), (1000, 784, 132), (2500, 256, 516),
-         (512, 512, 2048), (1300, 768, 1536)]
+         (512, 512, 2048), (1300, 768, 1536), (4000, 512, 1000), (1664, 2048, 2080), (3333, 130, 700), (5000, 4100, 96)]
 
 
 @pytest.mark.parametrize("activation", ACTIVATIONS)

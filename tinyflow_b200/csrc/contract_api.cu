@@ -37,6 +37,7 @@ int tc_pack_filters(ConvPlan* const* plans, const float* const* filters, const i
 int tc_fused_relu_bwd_pack(ConvPlan* p, const float* mask, const float* dy, float* out, cudaStream_t s);
 // which engine served this thread's most recent contraction: 1 = CUDA cores, 2 = tensor cores (0 = none yet)
 static thread_local int t_last_path = 0;
+void note_contraction_path(int path) { t_last_path = path; }
 
 // C[M x N] = op(A) op(B) of contiguous matrices on the engine that is selected
 int matmul_any(const float* A, bool tA, const float* B, bool tB, float* C, int64_t M, int64_t N, int64_t K, cudaStream_t s, const char* what) {

@@ -40,6 +40,7 @@
 #include <type_traits>
 #include <unordered_map>
 #include <vector>
+#include "gated.h"
 
 namespace tf {
 
@@ -401,6 +402,12 @@ struct alignas(128) GemmParams {
   int chunks_per_tap;             // kModeConv: K stages per tap
   int b_tap_pitch;                // kModeConv: columns per tap in the packed filter
   int ntaps;
+  // Order of the tiles: 0, column tiles first; else bands of this many row tiles, within a band row tiles first.  A wave of 148 tiles of
+  // a product whose operands L2 does not hold then reads about 12 + 12 blocks of them and not 1 + 128.
+  int band;
+  // Gated layers (kernels with GATED): the packed columns of B are 32 of the gate and the 32 of the value that they meet in turn, F of each.
+  int gated_f, activation;
+  float* gates;                   // both projections, or null
   float* out;
   uint32_t *amax, *amax_clear;    // where the epilogue leaves max|out| (null: nobody asked), and the word the next write of `out` will use
   const float* a_scale; const float* b_scale;   // device words: the power-of-two scales the packs were made with
@@ -498,6 +505,12 @@ struct WorkIter {
 };
 // tile index -> coordinates; n fastest so consecutive CTAs share the A tile through L2
 __device__ __forceinline__ void decode_tile(const GemmParams& p, int tile, int& mt, int& nt, int& tap) {
+  if (p.band) {
+    const int per_band = p.band * p.n_tiles, b = tile / per_band, in_band = tile - b * per_band, height = min(p.band, p.m_tiles - b * p.band);
+    nt = in_band / height; tap = 0;
+    mt = b * p.band + in_band - nt * height;
+    return;
+  }
   nt = tile % p.n_tiles; tile /= p.n_tiles;
   tap = tile % p.tap_tiles;
   mt = tile / p.tap_tiles;
@@ -565,6 +578,48 @@ template <int NC, int BLOCKS> __device__ __forceinline__ void load_sum(uint32_t 
     for (int q = 0; q < NC / 2; ++q) v[q] = __fadd2_rn(v[q], b[i - 1][q]);
 }
 
+// Gated layers: n gates of row m, in front of the n values that they meet, become n outputs from column f on; both are kept where the
+// caller wants them for the gradient.  Returns the largest magnitude stored.  Activation and product cost the layer no pass of its own
+// and no read of the projections: they run beside the products of the next tile.
+__device__ __forceinline__ void store_run(float* to, const float* v, int n) {
+  if (n == 32 && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) reinterpret_cast<float4*>(to)[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 32; ++q) if (q < n) to[q] = v[q];
+  }
+}
+template <int ACT> __device__ __forceinline__ uint32_t gate_run(const float* g, float* v, int n) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int q = 0; q < 32; ++q) {
+    v[q] *= gate_value<ACT>(g[q]);
+    if (q < n) top = max(top, amax_bits(v[q]));
+  }
+  return top;
+}
+template <int N> __device__ __forceinline__ uint32_t store_gated(const GemmParams& p, int m, int f, float* v) {
+  static_assert(N == 32, "an epilogue warp's columns");
+  const int n = min(32, p.gated_f - f);
+  if (n <= 0) return 0;
+  if (p.gates) {
+    float* const z = p.gates + (long long)m * 2 * p.gated_f + f;
+    store_run(z, v, n);
+    store_run(z + p.gated_f, v + 32, n);
+  }
+  uint32_t top = 0;
+  switch (p.activation) {
+    case kGateSigmoid: top = gate_run<kGateSigmoid>(v, v + 32, n); break;
+    case kGateRelu: top = gate_run<kGateRelu>(v, v + 32, n); break;
+    case kGateTanh: top = gate_run<kGateTanh>(v, v + 32, n); break;
+    case kGateSilu: top = gate_run<kGateSilu>(v, v + 32, n); break;
+    default: top = gate_run<kGateGelu>(v, v + 32, n); break;
+  }
+  store_run(p.out + (long long)m * p.gated_f + f, v + 32, n);
+  return top;
+}
+
 // What bounds it.  A K step of 16 is 192 tensor cycles at BN = 128 (N = 2*BN and N = BN).  Its operands are read from shared
 // memory at 128 bytes per cycle: 12 KB for the wide and 8 KB for the narrow instruction, 160 cycles; TMA writes another 64 KB per
 // stage of four K steps, 512 cycles, so with one block per stage shared memory alone takes 1152 cycles against 768 of the
@@ -572,7 +627,8 @@ template <int NC, int BLOCKS> __device__ __forceinline__ void load_sum(uint32_t 
 // stages (36 KB a stage for a 3x3 window of a 28-wide image) and filters of one tile that fit stay in shared memory: with
 // 512 channels, 28 x 28, 3x3, batch 64 the product went from 625 to 548 us, with 64 channels, 224 x 224, from 1128 to 886.
 // Short reductions are bound by start and epilogue: 4000 cycles to the first MMA, 2500-4000 from the last to the end.
-template <int BN, int AR>
+// GATED: the epilogue applies the activation and the product of a gated layer (see store_gated).
+template <int BN, int AR, bool GATED = false>
 __global__ void __launch_bounds__(kGemmThreads, 1) gemm3x_kernel(const __grid_constant__ GemmParams p) {
   using T = Arith<AR>;
   constexpr int BK = T::kBK;
@@ -911,7 +967,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm3x_kernel(const __grid_co
       };
       const uint32_t t_lane = tmem_base + half * HC + ((uint32_t)(quarter * 32) << 16);
 
-      if (w.slot < 0 && kcount <= p.group_iters && p.cluster <= 1 && !three) {
+      if (!GATED && w.slot < 0 && kcount <= p.group_iters && p.cluster <= 1 && !three) {
         // One accumulator group: stream TMEM straight to memory.
         const int acc = group & 1;
         if (!wait_group(acc, group)) { ok = false; break; }
@@ -987,6 +1043,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm3x_kernel(const __grid_co
         float* ws = (p.cluster > 1 ? reinterpret_cast<float*>(smem) : p.workspace + (size_t)w.slot * BN * BM) + half * HC * BM + row_in_tile;
 #pragma unroll
         for (int q = 0; q < HC / 2; ++q) { ws[(size_t)(2 * q) * BM] = accv[q].x; ws[(size_t)(2 * q + 1) * BM] = accv[q].y; }
+        continue;
+      }
+      if constexpr (GATED) {
+#pragma unroll
+        for (int q = 0; q < HC / 2; ++q) accv[q] = __fmul2_rn(accv[q], scale2);
+        const int m = mt * BM + row_in_tile;
+        if (m < p.M) top = max(top, store_gated<HC / 2>(p, m, (nt * BN + half * HC) / 2, reinterpret_cast<float*>(accv)));
         continue;
       }
 #pragma unroll
@@ -1659,6 +1722,73 @@ __global__ void __launch_bounds__(kReduceThreads<MANY>) reduce_partials_kernel(c
   });
 }
 
+// The same for the split tiles of a gated layer: a thread adds 4 gates and the 4 values that they meet, of one row, and finishes them.
+// grid (tiles, 8), 256 threads.
+__global__ void __launch_bounds__(256) reduce_gated_kernel(const __grid_constant__ GemmParams p) {
+  constexpr int BN = 128, COLS = 4, DEPTH = 2;
+  grid_dep_sync();
+  const int t = blockIdx.x, row = threadIdx.x & (BM - 1), gate = (int)blockIdx.y * 8 + (int)threadIdx.x / BM * COLS;      // of the tile's 64
+  const int col = gate / 32 * 64 + gate % 32;
+  const bool aligned = p.tail_pieces > 0;
+  const int first = aligned ? 0 : (int)(((long long)t * p.k_total) / p.tail_share);
+  const int last = aligned ? p.tail_pieces - 1 : (int)((((long long)t + 1) * p.k_total - 1) / p.tail_share);
+  float sum[2 * COLS], lost[2 * COLS];
+#pragma unroll
+  for (int q = 0; q < 2 * COLS; ++q) sum[q] = lost[q] = 0.f;
+  for (int g0 = first; g0 <= last; g0 += DEPTH) {
+    float v[DEPTH][2 * COLS];
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      const int g = g0 + d;
+      if (g <= last) {
+        const int slot = aligned ? g * p.tail_tiles + t : g * p.slots_per_cta + (t - (int)(((long long)g * p.tail_share) / p.k_total));
+        const float* const ws = p.workspace + (size_t)slot * BN * BM + row;
+#pragma unroll
+        for (int q = 0; q < 2 * COLS; ++q) v[d][q] = __ldcg(ws + (size_t)(col + q % COLS + q / COLS * 32) * BM);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d)
+      if (g0 + d <= last) {
+#pragma unroll
+        for (int q = 0; q < 2 * COLS; ++q) {          // two-sum
+          const float s = __fadd_rn(sum[q], v[d][q]), b = __fsub_rn(s, sum[q]);
+          lost[q] = __fadd_rn(lost[q], __fadd_rn(__fsub_rn(sum[q], __fsub_rn(s, b)), __fsub_rn(v[d][q], b)));
+          sum[q] = s;
+        }
+      }
+  }
+  int mt, nt, tap;
+  decode_tile(p, p.full_tiles + t, mt, nt, tap);
+  const int m = mt * BM + row, f = nt * (BN / 2) + gate, F = p.gated_f;
+  const float inv_scale = (1.f / __ldg(p.a_scale)) * (1.f / __ldg(p.b_scale));
+  uint32_t top = 0;
+#pragma unroll
+  for (int q = 0; q < COLS; ++q) {
+    if (m >= p.M || f + q >= F) continue;
+    // infinities and NaN as a plain sum has them
+    float g = sum[q], v = sum[COLS + q];
+    if (fabsf(g) <= FLT_MAX) g = __fadd_rn(g, lost[q]);
+    if (fabsf(v) <= FLT_MAX) v = __fadd_rn(v, lost[COLS + q]);
+    g *= inv_scale; v *= inv_scale;
+    if (p.gates) { p.gates[(long long)m * 2 * F + f + q] = g; p.gates[(long long)m * 2 * F + F + f + q] = v; }
+    float a;
+    switch (p.activation) {
+      case kGateSigmoid: a = gate_value<kGateSigmoid>(g); break;
+      case kGateRelu: a = gate_value<kGateRelu>(g); break;
+      case kGateTanh: a = gate_value<kGateTanh>(g); break;
+      case kGateSilu: a = gate_value<kGateSilu>(g); break;
+      default: a = gate_value<kGateGelu>(g); break;
+    }
+    v *= a;
+    p.out[(long long)m * F + f + q] = v;
+    top = max(top, amax_bits(v));
+  }
+  if (!p.amax) return;
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0 && top) atomicMax(p.amax, top);
+}
+
 template <int BN, bool MANY>
 __global__ void __launch_bounds__(kReduceThreads<MANY>) reduce_group_kernel(const __grid_constant__ GroupTable t) {
   grid_dep_sync();
@@ -1795,6 +1925,79 @@ __global__ void __launch_bounds__(256) pack_matrix_kernel(const float* __restric
       lo[r * dst_ld + c] = l;
     }
   }
+}
+
+// The weight of a gated layer, [K][gate columns | value columns] of F each -> [K][pitch]: 32 gate columns, the 32 value columns that they
+// meet, and so on, zeros past F, so that one epilogue thread of the product has both.  Eight packed columns a thread.
+template <bool VEC4, class E>
+__global__ void __launch_bounds__(256) pack_gated_weight_kernel(const float* __restrict__ src, E* __restrict__ hi, E* __restrict__ lo, long long pitch, long long rows, int F, ScaleRef sr) {
+  grid_dep_sync();
+  const float sc = pack_scale(sr, blockIdx.x == 0 && threadIdx.x == 0);
+  const long long stride = (long long)gridDim.x * blockDim.x, groups = pitch >> 3, total = rows * groups;
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += stride) {
+    const long long r = i / groups;
+    const int c = (int)(i - r * groups) << 3, f = c / 64 * 32 + c % 32;
+    const float* const from = src + r * 2 * F + (c & 32 ? F : 0) + f;
+    float v[8];
+    if (VEC4 && f + 8 <= F) {
+      const float4 a = __ldg(reinterpret_cast<const float4*>(from)), b = __ldg(reinterpret_cast<const float4*>(from) + 1);
+      v[0] = a.x * sc; v[1] = a.y * sc; v[2] = a.z * sc; v[3] = a.w * sc; v[4] = b.x * sc; v[5] = b.y * sc; v[6] = b.z * sc; v[7] = b.w * sc;
+    } else {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = f + q < F ? __ldg(from + q) * sc : 0.f;
+    }
+    store8(hi, lo, r * pitch + c, v);
+  }
+}
+// The gradient of a gated layer's projections, dz = [dout * value * act'(gate) | dout * act(gate)], packed as it is computed: it is never
+// written as numbers of its own.  STORE = false: only its largest magnitude, which the pack's scale needs.  8 columns of each half a
+// thread (VEC8: F a multiple of 8, 16-byte aligned rows), else one.  12 bytes read per column and pass, 8 written.
+template <int ACT, bool STORE, bool VEC8, class E>
+__global__ void __launch_bounds__(256) pack_gate_gradient_kernel(const float* __restrict__ z, const float* __restrict__ dout, E* __restrict__ hi, E* __restrict__ lo, long long pitch,
+                                                                 long long rows, int F, ScaleRef sr, uint32_t* amax) {
+  grid_dep_sync();
+  const float sc = STORE ? pack_scale(sr, blockIdx.x == 0 && threadIdx.x == 0) : 1.f;
+  constexpr int N = VEC8 ? 8 : 1;
+  const int groups = F / N;
+  const long long stride = (long long)gridDim.x * blockDim.x, total = rows * groups;
+  uint32_t top = 0;
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += stride) {
+    const long long r = i / groups;
+    const int f = (int)(i - r * groups) * N;
+    const float *const zr = z + r * 2 * F + f, *const dr = dout + r * F + f;
+    float g[N], v[N], d[N];
+    if (VEC8) {
+#pragma unroll
+      for (int q = 0; q < N; q += 4) {
+        *reinterpret_cast<float4*>(g + q) = __ldg(reinterpret_cast<const float4*>(zr + q));
+        *reinterpret_cast<float4*>(v + q) = __ldg(reinterpret_cast<const float4*>(zr + F + q));
+        *reinterpret_cast<float4*>(d + q) = __ldg(reinterpret_cast<const float4*>(dr + q));
+      }
+    } else {
+      g[0] = __ldg(zr); v[0] = __ldg(zr + F); d[0] = __ldg(dr);
+    }
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      float value, slope;
+      gate_slope<ACT>(g[q], value, slope);
+      g[q] = d[q] * v[q] * slope;
+      v[q] = d[q] * value;
+      if (!STORE) top = max(top, max(amax_bits(g[q]), amax_bits(v[q])));
+      g[q] *= sc; v[q] *= sc;
+    }
+    if (!STORE) continue;
+    const long long o = r * pitch + f;
+    if constexpr (VEC8) {
+      store8(hi, lo, o, g);
+      store8(hi, lo, o + F, v);
+    } else {
+      split_pair(g[0], hi[o], lo[o]);
+      split_pair(v[0], hi[o + F], lo[o + F]);
+    }
+  }
+  if (STORE) return;
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0 && top) atomicMax(amax, top);
 }
 
 // NCHW activations -> pixel-major frame [N][frame_h][frame_w][pitch]:
@@ -2224,8 +2427,7 @@ template <int BN> static bool could_wait(const GemmParams& p) {
   return BN != 96 && p.group_iters == 1 && p.acc_mode == kAccPair && longest_run(p) < kHeldRun<BN> && (p.tail_share == 0 || p.tail_pieces > 0);
 }
 // Schedule, stages per accumulator group and accumulator blocks of a launch: what decides the bits of its result
-template <int BN, int AR> static size_t plan_launch(GemmParams& p) {
-  const size_t bytes = plan_schedule(p, BN, max_clusters_of<BN, AR>);
+template <int BN, int AR> static void plan_groups(GemmParams& p) {
   static const int group_iters = getenv("TINYFLOW_GROUP_ITERS") ? atoi(getenv("TINYFLOW_GROUP_ITERS")) : 0;
   p.group_iters = group_iters > 0 ? group_iters : (p.data_by_data ? kGroupItersDataByData : (AR == kArithTF32 ? kGroupItersTF32 : kGroupIters));
   if (p.group_limit) p.group_iters = std::min(p.group_iters, p.group_limit);
@@ -2237,7 +2439,18 @@ template <int BN, int AR> static size_t plan_launch(GemmParams& p) {
   // at 55, 9 % at 841 (512 -> 512 channels, 28 x 28, 3x3, batch 64: 750 -> 673 us).
   p.acc_mode = BN != 64 && p.k_total > p.group_iters && longest_run(p) >= (BN == 128 && p.group_iters > 1 ? 8 : 24) ? kAccThree : kAccPair;
   p.sum_run = could_wait<BN>(p) ? kSumChunk : 1;
+}
+template <int BN, int AR> static size_t plan_launch(GemmParams& p) {
+  const size_t bytes = plan_schedule(p, BN, max_clusters_of<BN, AR>);
+  plan_groups<BN, AR>(p);
   return bytes;
+}
+static int plan_grid(const GemmParams& p) {
+  const int sms = device_sm_count(), tiles = p.full_tiles + p.tail_tiles;
+  if (p.cluster > 1) return tiles * p.cluster;
+  if (p.tail_share == 0) return tiles < sms ? tiles : sms;
+  if (p.full_tiles > 0) return sms;
+  return p.tail_pieces > 0 ? p.tail_tiles * (p.tail_pieces / p.tail_run) : (int)(((long long)p.tail_tiles * p.k_total + p.tail_share - 1) / p.tail_share);
 }
 template <int BN, int AR> static bool held_back(const GemmParams& p, size_t workspace_bytes, cudaStream_t s, double flops);
 template <int BN, int AR> static int launch_planned(GemmParams& p, size_t workspace_bytes, bool may_wait, cudaStream_t s, double flops, const char* what, int* oom);
@@ -2255,15 +2468,7 @@ template <int BN, int AR> static int launch_planned(GemmParams& p, size_t bytes,
     return 1;
   }
   if (may_wait && held_back<BN, AR>(p, bytes, s, flops)) return 0;
-  const int sms = device_sm_count();
-  const int tiles = p.full_tiles + p.tail_tiles;
-  int grid = tiles < sms ? tiles : sms;
-  if (p.tail_share > 0) {
-    const int ctas = p.tail_pieces > 0 ? p.tail_tiles * (p.tail_pieces / p.tail_run) : (int)(((long long)p.tail_tiles * p.k_total + p.tail_share - 1) / p.tail_share);
-    grid = p.full_tiles > 0 ? sms : ctas;
-  }
-  if (p.cluster > 1) grid = tiles * p.cluster;
-  grid = plan_smem(p, BN, grid);
+  const int tiles = p.full_tiles + p.tail_tiles, grid = plan_smem(p, BN, plan_grid(p));
   TF_REQUIRE(p.cluster == 1 || BM * BN * 4 <= p.a_slots * p.a_rows * 256 + p.b_slots * BN * 256, "%s: a piece of a tile does not fit where its operands were", what);
   note_compute_stream(s);
   static const bool detail = getenv("TINYFLOW_TIMING_DETAIL") != nullptr;    // one timing row per distinct problem shape
@@ -2687,6 +2892,138 @@ int tc_matmul(const float* A, bool tA, const float* B, bool tB, float* C, int64_
     rc = launch_gemm_bn(bn, ar, p, s, 2.0 * M * N * K, "DLGpuMatrixMultiply", oom);
   }
   return rc < 0 ? -1 : (rc > 0 ? 0 : 1);    // a missing workspace sends the call to the CUDA-core kernel
+}
+
+// ---- gated dense layers (ops_gated.cu) ----------------------------------------------------------------
+// Row tiles of a band: a wave then covers about as many row tiles as column tiles.  8192 x 2048 x 16384: TIMES
+static int band_of(const GemmParams& p) {
+  const int want = 12, bands = std::max(1, (p.m_tiles + want / 2) / want);
+  return p.n_tiles > 4 && p.m_tiles * p.n_tiles > device_sm_count() ? (p.m_tiles + bands - 1) / bands : 0;       // (up to 4 column tiles B may stay in shared memory)
+}
+static bool tc_takes(double M, double N, double K) { return M >= 16 && N >= 16 && K >= 64 && M * N * K >= (contraction_path() == 2 ? 4e6 : 1.5e8); }
+static int gemm_maps(GemmParams& p, int ar, const Pack& pa, const Pack& pb, int bn) {
+  int rc = p.a_mn ? make_map_mn(&p.a_hi, ar, pa.hi, pa.rows, pa.pitch, BM) : make_map(&p.a_hi, ar, pa.hi, pa.rows, pa.cols, pa.pitch, BM);
+  if (!rc) rc = p.a_mn ? make_map_mn(&p.a_lo, ar, pa.lo, pa.rows, pa.pitch, BM) : make_map(&p.a_lo, ar, pa.lo, pa.rows, pa.cols, pa.pitch, BM);
+  if (!rc) rc = p.b_mn ? make_map_mn(&p.b_hi, ar, pb.hi, pb.rows, pb.pitch, bn) : make_map(&p.b_hi, ar, pb.hi, pb.rows, pb.cols, pb.pitch, bn);
+  if (!rc) rc = p.b_mn ? make_map_mn(&p.b_lo, ar, pb.lo, pb.rows, pb.pitch, bn) : make_map(&p.b_lo, ar, pb.lo, pb.rows, pb.cols, pb.pitch, bn);
+  p.a_scale = pa.scale(); p.b_scale = pb.scale();
+  return rc;
+}
+template <int AR> static int launch_gated(GemmParams& p, cudaStream_t s, double flops, const char* what, int* oom) {
+  constexpr int BN = 128;
+  static const cudaError_t attr = cudaFuncSetAttribute(gemm3x_kernel<BN, AR, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit + 1024);
+  TF_CUDA(attr);
+  TF_REQUIRE(tensor_path_error() == 0, "%s: an earlier tensor-core kernel timed out on a barrier; refusing to launch", what);
+  const size_t bytes = plan_schedule(p, BN, [](int) { return 0; });          // no clusters: their sum does not know of gates
+  plan_groups<BN, AR>(p);
+  StreamLease lease(s);
+  if (bytes && !(p.workspace = (float*)lease.scratch(kScratchTiles, bytes))) {
+    if (oom) *oom = bytes > 0x7fffffffu ? 0x7fffffff : (int)bytes;
+    return 1;
+  }
+  const int grid = plan_smem(p, BN, plan_grid(p));
+  note_compute_stream(s);
+  KernelTimer kt(AR == kArithTF32 ? "gemm3xtf32_gated" : "gemm3xf16_gated", s, flops, 0, 1);
+  TF_CUDA(launch_dep(gemm3x_kernel<BN, AR, true>, dim3(grid), dim3(kGemmThreads), (size_t)gemm_smem_bytes(p, BN), s, p));
+  TF_AFTER(s, what);
+  if (p.tail_share > 0) {
+    TF_CUDA(launch_dep(reduce_gated_kernel, dim3(p.tail_tiles, 8), dim3(256), 0, s, p));
+    TF_AFTER(s, what);
+  }
+  return 0;
+}
+// out = act(x Wg) * (x Wv): 1 done, 0 not a shape for the tensor path (or no memory for its packs), -1 error
+int tc_gated_fwd(const float* x, const float* w, float* gates, float* out, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s, const char* what) {
+  if (!tc_takes((double)M, 2.0 * F, (double)K) || !encode_fn()) return 0;
+  const int ar = tensor_arithmetic(), bk = bk_of(ar);
+  Pack pa, pb;
+  StreamLease lease(s);
+  const long long cols = (F + 31) / 32 * 64;
+  int rc = pack_in_scratch(pa, lease, kScratchPackA, ar, M, K, s, nullptr);
+  if (!rc) rc = pack_in_scratch(pb, lease, kScratchPackB, ar, K, cols, s, nullptr);
+  if (rc) return rc < 0 ? -1 : 0;
+  if (run_pack_matrix(x, K, pa, s)) return -1;
+  {
+    const ScaleRef sr = begin_pack(pb, w, K * 2 * F, s);
+    KernelTimer kt("pack_gated_weight", s, 0, 4.0 * K * 2 * F + 2.0 * elem_of(ar) * K * cols);
+    const bool vec = F % 4 == 0 && aligned16(w);
+    cudaError_t e = cudaSuccess;
+    with_elems(pb, [&](auto* hi, auto* lo) {
+      using E = std::remove_pointer_t<decltype(hi)>;
+      const dim3 grid(grid_for(K * cols / 8, 256, 2));
+      e = vec ? launch_dep(pack_gated_weight_kernel<true, E>, grid, dim3(256), 0, s, w, hi, lo, pb.pitch, (long long)K, (int)F, sr)
+              : launch_dep(pack_gated_weight_kernel<false, E>, grid, dim3(256), 0, s, w, hi, lo, pb.pitch, (long long)K, (int)F, sr);
+    });
+    TF_CUDA(e);
+    TF_AFTER(s, what);
+  }
+  GemmParams p;
+  memset(&p, 0, sizeof(p));
+  p.mode = kModeGemm; p.b_mn = 1; p.epi = kEpiRowMajor; p.a_rows = BM;
+  if (gemm_maps(p, ar, pa, pb, 128)) return -1;
+  p.M = (int)M; p.N = (int)cols; p.m_tiles = (int)((M + BM - 1) / BM); p.n_tiles = (int)((cols + 127) / 128); p.tap_tiles = 1;
+  p.k_total = (int)((K + bk - 1) / bk);
+  p.out = out; p.gates = gates; p.gated_f = (int)F; p.activation = activation; p.err = error_word(); p.band = band_of(p);
+  const AmaxOut am = amax_track_begin(out);
+  p.amax = am.word; p.amax_clear = am.clear;
+  rc = ar == kArithTF32 ? launch_gated<kArithTF32>(p, s, 4.0 * M * F * K, what, nullptr) : launch_gated<kArithF16>(p, s, 4.0 * M * F * K, what, nullptr);
+  return rc < 0 ? -1 : (rc > 0 ? 0 : 1);
+}
+// dx = dz W^T and dW = x^T dz (either may be null) with dz packed once for both: 1 done, 0 not both are shapes for the tensor path, -1 error
+int tc_gated_bwd(const float* x, const float* w, const float* z, const float* dout, float* dx, float* dw, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s,
+                 const char* what) {
+  if ((dx && !tc_takes((double)M, (double)K, 2.0 * F)) || (dw && !tc_takes((double)K, 2.0 * F, (double)M)) || !encode_fn()) return 0;
+  const int ar = tensor_arithmetic(), bk = bk_of(ar);
+  Pack pz, pw, px;
+  StreamLease lease(s);
+  int rc = pack_in_scratch(pz, lease, kScratchGates, ar, M, 2 * F, s, nullptr);
+  if (!rc && dx) rc = pack_in_scratch(pw, lease, kScratchPackB, ar, K, 2 * F, s, nullptr);
+  if (!rc && dw) rc = pack_in_scratch(px, lease, kScratchPackA, ar, M, K, s, nullptr);
+  if (rc) return rc < 0 ? -1 : 0;
+  note_compute_stream(s);
+  {
+    ScaleRef sr{nullptr, nullptr, reinterpret_cast<float*>(pz.words + 2), nullptr};
+    KernelTimer kt("pack_gate_gradient", s, 0, (ar == kArithTF32 ? 12.0 : 24.0) * M * F + 4.0 * elem_of(ar) * M * F);
+    const bool vec = F % 8 == 0 && aligned16(z) && aligned16(dout);
+    cudaError_t e = cudaSuccess;
+    with_gate(activation, [&](auto act) {
+      constexpr int ACT = decltype(act)::value;
+      with_elems(pz, [&](auto* hi, auto* lo) {
+        using E = std::remove_pointer_t<decltype(hi)>;
+        const dim3 grid(grid_for(vec ? M * F / 8 : M * F, 256, vec ? 2 : 4));
+        auto run = [&](auto v8) {
+          constexpr bool VEC8 = decltype(v8)::value;
+          if (std::is_same<E, __half>::value) {
+            uint32_t* const word = t_recording ? recording_word() : pz.words;
+            e = launch_dep(pack_gate_gradient_kernel<ACT, false, VEC8, E>, grid, dim3(256), 0, s, z, dout, hi, lo, pz.pitch, (long long)M, (int)F, sr, word);
+            sr.amax_cur = word;
+          }
+          if (e == cudaSuccess) e = launch_dep(pack_gate_gradient_kernel<ACT, true, VEC8, E>, grid, dim3(256), 0, s, z, dout, hi, lo, pz.pitch, (long long)M, (int)F, sr, (uint32_t*)nullptr);
+        };
+        vec ? run(std::true_type()) : run(std::false_type());
+      });
+    });
+    TF_CUDA(e);
+    TF_AFTER(s, what);
+  }
+  for (int k = 0; k < 2; ++k) {
+    if (!(k ? dw : dx)) continue;
+    const Pack &pa = k ? px : pz, &pb = k ? pz : pw;
+    if (k ? run_pack_matrix(x, K, px, s) : run_pack_matrix(w, 2 * F, pw, s)) return -1;
+    const int64_t rows = k ? K : M, cols = k ? 2 * F : K, depth = k ? M : 2 * F;
+    const int bn = pick_bn(cols, !k);
+    GemmParams p;
+    memset(&p, 0, sizeof(p));
+    p.mode = kModeGemm; p.a_mn = k; p.b_mn = k; p.epi = kEpiRowMajor; p.data_by_data = k;
+    if (gemm_maps(p, ar, pa, pb, bn)) return -1;
+    p.M = (int)rows; p.N = (int)cols; p.m_tiles = (int)((rows + BM - 1) / BM); p.n_tiles = (int)((cols + bn - 1) / bn); p.tap_tiles = 1;
+    p.k_total = (int)((depth + bk - 1) / bk);
+    p.out = k ? dw : dx; p.ldc = cols; p.err = error_word(); p.band = band_of(p);
+    int oom = 0;
+    rc = launch_gemm_bn(bn, ar, p, s, 2.0 * rows * cols * depth, what, &oom);
+    if (rc) return rc < 0 ? -1 : 0;
+  }
+  return 1;
 }
 
 // ---- convolution -------------------------------------------------------------------------------------

@@ -13,6 +13,9 @@
 namespace tf {
 
 int matmul_any(const float* A, bool tA, const float* B, bool tB, float* C, int64_t M, int64_t N, int64_t K, cudaStream_t s, const char* what);
+int tc_gated_fwd(const float* x, const float* w, float* gates, float* out, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s, const char* what);
+int tc_gated_bwd(const float* x, const float* w, const float* z, const float* dout, float* dx, float* dw, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s, const char* what);
+void note_contraction_path(int path);
 bool pause_holding();                    // what follows is not to wait; returns whether it could have
 void hold_products(bool on);
 
@@ -138,6 +141,12 @@ int TfGatedLinearForward(const DLArrayHandle input, const DLArrayHandle weight, 
   float* z = gates ? out_f32(gates) : nullptr;
   if (M == 0 || F == 0) return 0;
   const NoHolding launched;
+  if (!contraction_path_is_cuda_cores()) {
+    if (const int r = tc_gated_fwd((const float*)input->data, (const float*)weight->data, z, out, M, F, K, activation, s, what)) {
+      note_contraction_path(2);
+      return r < 0 ? -1 : 0;
+    }
+  }
   StreamLease lease(s);
   const size_t bytes = sizeof(float) * (size_t)M * 2 * F;
   if (!z && !(z = (float*)lease.scratch(kScratchGates, bytes))) return short_of(bytes, memorytoSaving);
@@ -163,6 +172,12 @@ int TfGatedLinearBackward(const DLArrayHandle input, const DLArrayHandle weight,
   float *dx = dinput ? out_f32(dinput) : nullptr, *dw = dweight ? out_f32(dweight) : nullptr;
   if (!dx && !dw) return 0;
   const NoHolding launched;
+  if (!contraction_path_is_cuda_cores()) {
+    if (const int r = tc_gated_bwd((const float*)input->data, (const float*)weight->data, (const float*)gates->data, (const float*)doutput->data, dx, dw, M, F, K, activation, s, what)) {
+      note_contraction_path(2);
+      return r < 0 ? -1 : 0;
+    }
+  }
   StreamLease lease(s);
   const size_t bytes = sizeof(float) * (size_t)std::max<int64_t>(1, M * 2 * F);
   float* const dz = (float*)lease.scratch(kScratchGates, bytes);
