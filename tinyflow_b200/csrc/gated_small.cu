@@ -1,0 +1,304 @@
+// Gated dense layers of the sizes that the tensor path is too long a road for, in exact fp32: one launch forward, one backward.
+//
+// Latency is the bound (launches, and one chain of loads and sums per block), so everything that can be formed on the way is: the forward
+// kernel computes the gate columns and the value columns that they meet in the same block and finishes them; the backward kernel holds the
+// tiles of dx and of dW, and forms dz from the projections while it loads, once per tile that reads it.  Long reductions are cut over the
+// CTAs of a cluster and added in rank order through distributed shared memory, as in the plain products.
+// 64 x 784 x 256, forward and backward: products and elementwise kernels one by one 30 us, so TIMES.
+#include "common.h"
+#include <algorithm>
+#include <type_traits>
+#include <cooperative_groups.h>
+#include "gated.h"
+#include "simt.h"
+
+namespace cg = cooperative_groups;
+
+namespace tf {
+
+namespace {
+
+constexpr int kTile = 32, kDepth = 32, kThreads = 128, kPitch = kTile + 4;
+struct Small {
+  const float *x, *w, *z, *dout;
+  float *gates, *out, *dx, *dw;
+  int M, K, F;
+  int per_cta;              // of the reduction that is cut (forward: K, a multiple of 32; dx: F, a multiple of 16)
+  int x_vec, w_vec, z_vec;  // 16-byte accesses allowed
+  int dx_tiles, dw_tiles, dx_across, dw_across;
+  AmaxOut am;
+};
+
+typedef float Block[kDepth][kPitch];
+// thread (ty, tx) of 8 x 16: 4 rows x 2 columns
+__device__ __forceinline__ void multiply(const Block& a, const Block& b, int ty, int tx, float (&acc)[4][2]) {
+#pragma unroll
+  for (int k = 0; k < kDepth; ++k) {
+    const float4 r = *reinterpret_cast<const float4*>(&a[k][ty * 4]);
+    const float2 c = *reinterpret_cast<const float2*>(&b[k][tx * 2]);
+    acc[0][0] = fmaf(r.x, c.x, acc[0][0]); acc[0][1] = fmaf(r.x, c.y, acc[0][1]);
+    acc[1][0] = fmaf(r.y, c.x, acc[1][0]); acc[1][1] = fmaf(r.y, c.y, acc[1][1]);
+    acc[2][0] = fmaf(r.z, c.x, acc[2][0]); acc[2][1] = fmaf(r.z, c.y, acc[2][1]);
+    acc[3][0] = fmaf(r.w, c.x, acc[3][0]); acc[3][1] = fmaf(r.w, c.y, acc[3][1]);
+  }
+}
+// four elements of a row from column c on, zeros from `cols` on
+__device__ __forceinline__ float4 four(const float* __restrict__ row, int c, int cols, bool vec) {
+  if (vec && c + 4 <= cols) return __ldg(reinterpret_cast<const float4*>(row + c));
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (c < cols) v.x = __ldg(row + c);
+  if (c + 1 < cols) v.y = __ldg(row + c + 1);
+  if (c + 2 < cols) v.z = __ldg(row + c + 2);
+  if (c + 3 < cols) v.w = __ldg(row + c + 3);
+  return v;
+}
+// dz of four columns of one row: loaded, then formed
+template <int ACT> struct GateGradient {
+  float4 g, v, d;
+  __device__ __forceinline__ void fetch(const Small& p, int m, int f) {
+    g = v = d = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (m >= p.M) return;
+    const float* const z = p.z + (long long)m * 2 * p.F;
+    g = four(z, f, p.F, p.z_vec);
+    v = four(z + p.F, f, p.F, p.z_vec);
+    d = four(p.dout + (long long)m * p.F, f, p.F, p.z_vec);            // zeros past the end: so is dz
+  }
+  __device__ __forceinline__ void form(float (&dg)[4], float (&dv)[4]) const {
+    const float gg[4] = {g.x, g.y, g.z, g.w}, vv[4] = {v.x, v.y, v.z, v.w}, dd[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float value, slope;
+      gate_slope<ACT>(gg[i], value, slope);
+      dg[i] = dd[i] * vv[i] * slope;
+      dv[i] = dd[i] * value;
+    }
+  }
+};
+
+// grid (ranks * ceil(F / 32), ceil(M / 32)), clusters of `ranks` along x
+template <int ACT> __global__ void __launch_bounds__(kThreads) gated_small_fwd_kernel(const Small p) {
+  __shared__ __align__(16) Block xs[2], gs[2], vs[2];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
+  grid_dep_sync();
+  const int m0 = blockIdx.y * kTile, f0 = (int)(blockIdx.x / ranks) * kTile, tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  const int kbeg = rank * p.per_cta, kend = min(p.K, kbeg + p.per_cta);
+  float g[4][2] = {}, v[4][2] = {};
+  BlockLoader<kTile, kDepth, kThreads, true> lx;
+  BlockLoader<kTile, kDepth, kThreads, false> lg, lv;
+  auto fetch = [&](int k) {
+    lx.fetch(p.x, p.K, m0, p.M, k, kend, p.x_vec);
+    lg.fetch(p.w, 2ll * p.F, f0, p.F, k, kend, p.w_vec);
+    lv.fetch(p.w + p.F, 2ll * p.F, f0, p.F, k, kend, p.w_vec);
+  };
+  auto put = [&](int to) { lx.put(xs[to]); lg.put(gs[to]); lv.put(vs[to]); };
+  if (kbeg < kend) { fetch(kbeg); put(0); }
+  __syncthreads();
+  int buf = 0;
+  for (int k = kbeg; k < kend; k += kDepth, buf ^= 1) {
+    const bool more = k + kDepth < kend;
+    if (more) fetch(k + kDepth);
+    multiply(xs[buf], gs[buf], ty, tx, g);
+    multiply(xs[buf], vs[buf], ty, tx, v);
+    if (more) put(buf ^ 1);
+    __syncthreads();
+  }
+  uint32_t top = 0;
+  auto finish = [&](int row, int col, float gate, float value) {
+    const int m = m0 + row, f = f0 + col;
+    if (m >= p.M || f >= p.F) return;
+    if (p.gates) { p.gates[(long long)m * 2 * p.F + f] = gate; p.gates[(long long)m * 2 * p.F + p.F + f] = value; }
+    value *= gate_value<ACT>(gate);
+    p.out[(long long)m * p.F + f] = value;
+    top = max(top, amax_bits(value));
+  };
+  if (ranks == 1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) finish(ty * 4 + i, tx * 2 + j, g[i][j], v[i][j]);
+  } else {
+    float* const part = &xs[0][0][0];            // gates, then values, 32 x 32 each (both blocks of x are done with)
+    static_assert(sizeof(xs) >= 2 * kTile * kTile * sizeof(float), "a tile's partial sums fit where x was");
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) { part[(ty * 4 + i) * kTile + tx * 2 + j] = g[i][j]; part[kTile * kTile + (ty * 4 + i) * kTile + tx * 2 + j] = v[i][j]; }
+    cluster.sync();
+    const int slice = (kTile * kTile + ranks - 1) / ranks, end = min(kTile * kTile, (rank + 1) * slice);
+    for (int e = rank * slice + threadIdx.x; e < end; e += kThreads) {
+      float a[8], b[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const float* const from = cluster.map_shared_rank(part, min(r, ranks - 1));
+        a[r] = from[e]; b[r] = from[kTile * kTile + e];
+      }
+      float gate = a[0], value = b[0];
+#pragma unroll
+      for (int r = 1; r < 8; ++r) if (r < ranks) { gate += a[r]; value += b[r]; }
+      finish(e / kTile, e % kTile, gate, value);
+    }
+    cluster.sync();           // nobody leaves while its shared memory is still read
+  }
+  amax_commit(p.am, top);
+}
+
+// Clusters of `ranks`: the first dx_tiles of them a tile of dx each, cut over the cluster, the others `ranks` tiles of dW, one a CTA.
+// A step of 32 of the reduction is 16 columns of each half for dx, 32 rows for dW; a tile of dW is 32 rows x 16 columns of each half.
+template <int ACT> __global__ void __launch_bounds__(kThreads) gated_small_bwd_kernel(const Small p) {
+  __shared__ __align__(16) Block as[2], bs[2];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks(), id = (int)blockIdx.x / ranks;
+  grid_dep_sync();
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16, line = threadIdx.x / 4, quad = threadIdx.x % 4 * 4;
+  float acc[4][2] = {};
+  GateGradient<ACT> dz;
+  int buf = 0;
+  if (id < p.dx_tiles) {
+    const int m0 = id / p.dx_across * kTile, n0 = id % p.dx_across * kTile, fbeg = rank * p.per_cta, fend = min(p.F, fbeg + p.per_cta);
+    float4 wg, wv;
+    auto fetch = [&](int f) {
+      dz.fetch(p, m0 + line, f + quad);
+      wg = wv = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (n0 + line < p.K) {
+        const float* const row = p.w + (long long)(n0 + line) * 2 * p.F;
+        wg = four(row, f + quad, p.F, p.w_vec);
+        wv = four(row + p.F, f + quad, p.F, p.w_vec);
+      }
+    };
+    auto put = [&](int to) {
+      float dg[4], dv[4];
+      dz.form(dg, dv);
+      const float g[4] = {wg.x, wg.y, wg.z, wg.w}, v[4] = {wv.x, wv.y, wv.z, wv.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        as[to][quad + i][line] = dg[i]; as[to][16 + quad + i][line] = dv[i];
+        bs[to][quad + i][line] = g[i]; bs[to][16 + quad + i][line] = v[i];
+      }
+    };
+    if (fbeg < fend) { fetch(fbeg); put(0); }
+    __syncthreads();
+    for (int f = fbeg; f < fend; f += kDepth / 2, buf ^= 1) {
+      const bool more = f + kDepth / 2 < fend;
+      if (more) fetch(f + kDepth / 2);
+      multiply(as[buf], bs[buf], ty, tx, acc);
+      if (more) put(buf ^ 1);
+      __syncthreads();
+    }
+    if (ranks == 1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int m = m0 + ty * 4 + i, n = n0 + tx * 2 + j;
+          if (m < p.M && n < p.K) p.dx[(long long)m * p.K + n] = acc[i][j];
+        }
+      return;
+    }
+    float* const part = &as[0][0][0];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) part[(ty * 4 + i) * kTile + tx * 2 + j] = acc[i][j];
+    cluster.sync();
+    const int slice = (kTile * kTile + ranks - 1) / ranks, end = min(kTile * kTile, (rank + 1) * slice);
+    for (int e = rank * slice + threadIdx.x; e < end; e += kThreads) {
+      float a[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) a[r] = cluster.map_shared_rank(part, min(r, ranks - 1))[e];
+      float total = a[0];
+#pragma unroll
+      for (int r = 1; r < 8; ++r) if (r < ranks) total += a[r];
+      const int m = m0 + e / kTile, n = n0 + e % kTile;
+      if (m < p.M && n < p.K) p.dx[(long long)m * p.K + n] = total;
+    }
+    cluster.sync();
+    return;
+  }
+  const int tile = (id - p.dx_tiles) * ranks + rank;
+  if (tile >= p.dw_tiles) return;
+  const int k0 = tile / p.dw_across * kTile, f0 = tile % p.dw_across * 16;
+  BlockLoader<kTile, kDepth, kThreads, false> lx;
+  auto fetch = [&](int m) {
+    lx.fetch(p.x, p.K, k0, p.K, m, p.M, p.x_vec);
+    dz.fetch(p, m + line, f0 + quad);
+  };
+  auto put = [&](int to) {
+    float dg[4], dv[4];
+    lx.put(as[to]);
+    dz.form(dg, dv);
+    *reinterpret_cast<float4*>(&bs[to][line][quad]) = make_float4(dg[0], dg[1], dg[2], dg[3]);
+    *reinterpret_cast<float4*>(&bs[to][line][16 + quad]) = make_float4(dv[0], dv[1], dv[2], dv[3]);
+  };
+  if (p.M > 0) { fetch(0); put(0); }
+  __syncthreads();
+  for (int m = 0; m < p.M; m += kDepth, buf ^= 1) {
+    const bool more = m + kDepth < p.M;
+    if (more) fetch(m + kDepth);
+    multiply(as[buf], bs[buf], ty, tx, acc);
+    if (more) put(buf ^ 1);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int k = k0 + ty * 4 + i, c = tx * 2 + j, f = f0 + (c & 15);
+      if (k < p.K && f < p.F) p.dw[(long long)k * 2 * p.F + (c < 16 ? 0 : p.F) + f] = acc[i][j];
+    }
+}
+
+// Blocks of 64 x 64 would leave SMs idle: above that the plain products with their larger tiles are faster
+bool small_product(int64_t M, int64_t N) { return ((M + 63) / 64) * ((N + 63) / 64) < device_sm_count(); }
+int cluster_for(long long tiles, long long steps, int want) {
+  int c = 1;
+  while (c < 8 && tiles * c < want && steps >= 4 * c) c *= 2;
+  return c;
+}
+
+}  // namespace
+
+// 1: done, 0: too large, -1: error
+int gated_small_fwd(const float* x, const float* w, float* gates, float* out, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s, const char* what) {
+  if (!small_product(M, 2 * F)) return 0;
+  Small p;
+  memset(&p, 0, sizeof(p));
+  p.x = x; p.w = w; p.gates = gates; p.out = out; p.M = (int)M; p.K = (int)K; p.F = (int)F;
+  p.x_vec = K % 4 == 0 && aligned16(x); p.w_vec = F % 4 == 0 && aligned16(w);
+  const unsigned across = (unsigned)((F + kTile - 1) / kTile), down = (unsigned)((M + kTile - 1) / kTile);
+  const int cluster = cluster_for((long long)across * down, (K + kDepth - 1) / kDepth, 3 * device_sm_count());
+  p.per_cta = (int)(((K + cluster - 1) / cluster + kDepth - 1) / kDepth * kDepth);
+  p.am = amax_track_begin(out);
+  note_compute_stream(s);
+  KernelTimer kt("gated_small_fwd", s, 4.0 * M * F * K, 0, 1);
+  cudaError_t e = cudaSuccess;
+  with_gate(activation, [&](auto act) { e = launch_cluster(gated_small_fwd_kernel<decltype(act)::value>, cluster, dim3(across * cluster, down), dim3(kThreads), 0, s, p); });
+  TF_CUDA(e);
+  TF_AFTER(s, what);
+  return 1;
+}
+int gated_small_bwd(const float* x, const float* w, const float* z, const float* dout, float* dx, float* dw, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s,
+                    const char* what) {
+  if ((dx && !small_product(M, K)) || (dw && !small_product(K, 2 * F))) return 0;
+  Small p;
+  memset(&p, 0, sizeof(p));
+  p.x = x; p.w = w; p.z = z; p.dout = dout; p.dx = dx; p.dw = dw; p.M = (int)M; p.K = (int)K; p.F = (int)F;
+  p.x_vec = K % 4 == 0 && aligned16(x); p.w_vec = F % 4 == 0 && aligned16(w); p.z_vec = F % 4 == 0 && aligned16(z) && aligned16(dout);
+  p.dx_across = (int)((K + kTile - 1) / kTile);
+  p.dw_across = (int)((F + 15) / 16);
+  p.dx_tiles = dx ? p.dx_across * (int)((M + kTile - 1) / kTile) : 0;
+  p.dw_tiles = dw ? p.dw_across * (int)((K + kTile - 1) / kTile) : 0;
+  const int cluster = dx ? cluster_for(p.dx_tiles, (F + 15) / 16, device_sm_count()) : 1;
+  p.per_cta = (int)(((F + cluster - 1) / cluster + 15) / 16 * 16);
+  const int clusters = p.dx_tiles + (p.dw_tiles + cluster - 1) / cluster;
+  if (clusters == 0) return 1;
+  note_compute_stream(s);
+  KernelTimer kt("gated_small_bwd", s, 4.0 * M * F * K * ((dx != nullptr) + (dw != nullptr)), 0, 1);
+  cudaError_t e = cudaSuccess;
+  with_gate(activation, [&](auto act) { e = launch_cluster(gated_small_bwd_kernel<decltype(act)::value>, cluster, dim3((unsigned)(clusters * cluster)), dim3(kThreads), 0, s, p); });
+  TF_CUDA(e);
+  TF_AFTER(s, what);
+  return 1;
+}
+
+}  // namespace tf

@@ -9,6 +9,9 @@
 //
 // Measured against the kernel it replaced and against the tensor path: the table in simt_matmul(), where the tile is chosen.
 #include "common.h"
+#include "gated.h"
+#include "simt.h"
+#include <type_traits>
 #include <algorithm>
 #include <vector>
 #include <cooperative_groups.h>
@@ -16,57 +19,6 @@
 namespace cg = cooperative_groups;
 
 namespace tf {
-
-struct SimtGemm {
-  const float* A; const float* B; float* C;
-  int M, N, K;
-  long long lda, ldb, ldc;
-  int k_per_cta;            // multiple of BK
-  int a_vec, b_vec, c_vec;  // 16-byte accesses allowed
-};
-
-// One BMxBK (or BKxBN) block of an operand: `rows` index M (or N), `k` the reduction.  KFAST: k is contiguous in memory.
-// A thread moves VPT groups of four elements along the contiguous direction.
-template <int ROWS, int BK, int THREADS, bool KFAST> struct BlockLoader {
-  static constexpr int kGroups = ROWS * BK / 4;
-  static constexpr int VPT = (kGroups + THREADS - 1) / THREADS;
-  float4 v[VPT];
-  __device__ __forceinline__ void fetch(const float* __restrict__ p, long long ld, int row0, int rows, int k0, int k1, bool vec) {
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int g = threadIdx.x + i * THREADS;
-      v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (kGroups % THREADS && g >= kGroups) continue;
-      if (KFAST) {
-        const int r = row0 + g / (BK / 4), k = k0 + (g % (BK / 4)) * 4;
-        if (r >= rows || k >= k1) continue;
-        const float* q = p + (long long)r * ld + k;
-        if (vec && k + 4 <= k1) v[i] = __ldg(reinterpret_cast<const float4*>(q));
-        else { v[i].x = __ldg(q); if (k + 1 < k1) v[i].y = __ldg(q + 1); if (k + 2 < k1) v[i].z = __ldg(q + 2); if (k + 3 < k1) v[i].w = __ldg(q + 3); }
-      } else {
-        const int k = k0 + g / (ROWS / 4), r = row0 + (g % (ROWS / 4)) * 4;
-        if (r >= rows || k >= k1) continue;
-        const float* q = p + (long long)k * ld + r;
-        if (vec && r + 4 <= rows) v[i] = __ldg(reinterpret_cast<const float4*>(q));
-        else { v[i].x = __ldg(q); if (r + 1 < rows) v[i].y = __ldg(q + 1); if (r + 2 < rows) v[i].z = __ldg(q + 2); if (r + 3 < rows) v[i].w = __ldg(q + 3); }
-      }
-    }
-  }
-  // into s[k][row], row pitch ROWS + 4: 16-byte aligned rows for the vector reads
-  __device__ __forceinline__ void put(float (*s)[ROWS + 4]) const {
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int g = threadIdx.x + i * THREADS;
-      if (kGroups % THREADS && g >= kGroups) continue;
-      if (KFAST) {
-        const int r = g / (BK / 4), k = (g % (BK / 4)) * 4;
-        s[k][r] = v[i].x; s[k + 1][r] = v[i].y; s[k + 2][r] = v[i].z; s[k + 3][r] = v[i].w;
-      } else {
-        *reinterpret_cast<float4*>(&s[g / (ROWS / 4)][(g % (ROWS / 4)) * 4]) = v[i];
-      }
-    }
-  }
-};
 
 // One tile, or the share of it of CTA `rank` of `ranks` (the first of them is CTA `first` of the cluster)
 template <int BM, int BN, int TM, int TN, int BK, bool A_KFAST, bool B_KFAST>
@@ -269,6 +221,85 @@ __global__ void __launch_bounds__(kRowThreads) rows_nn_kernel(const SimtGemm p) 
   cluster.sync();           // nobody leaves while its shared memory is still read
 }
 
+// A gated layer on a handful of rows: as rows_nn_kernel, with 64 gate columns in the lower half of the lanes and the 64 value columns that they
+// meet in the upper one.  1 x 1024 x 4096: TIMES
+struct RowsGated { SimtGemm g; float* gates; float* out; int F; AmaxOut am; };
+template <int MR, int ACT>
+__global__ void __launch_bounds__(kRowThreads) rows_gated_kernel(const RowsGated q) {
+  extern __shared__ __align__(16) float rows_smem[];
+  const SimtGemm& p = q.g;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kw = p.k_per_cta / kRowWarps, seg = p.k_per_cta;
+  const int f = (int)(blockIdx.x / ranks) * 64 + (lane & 15) * 4;
+  grid_dep_sync();
+  const int kbeg = rank * seg, count = max(0, min(seg, p.K - kbeg)), k1 = min((warp + 1) * kw, count);
+  float4 w[8];
+  const float* const b0 = p.B + (long long)kbeg * p.ldb + (lane < 16 ? 0 : q.F) + f;
+  auto fetch = [&](int k) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = f < q.F && k + j < k1 ? __ldg(reinterpret_cast<const float4*>(b0 + (long long)(k + j) * p.ldb)) : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  fetch(warp * kw);                      // the first rows of the weight come with those of x
+  for (int m = warp; m < MR; m += kRowWarps)
+    for (int k = lane; k < seg; k += 32) rows_smem[m * seg + k] = m < p.M && k < count ? __ldg(p.A + (long long)m * p.lda + kbeg + k) : 0.f;
+  __syncthreads();
+  float2 acc[MR][2];
+#pragma unroll
+  for (int m = 0; m < MR; ++m) acc[m][0] = acc[m][1] = make_float2(0.f, 0.f);
+  for (int k = warp * kw; k < k1; k += 8) {
+    float4 now[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) now[j] = w[j];
+    if (k + 8 < k1) fetch(k + 8);
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+      const float4 x0 = *reinterpret_cast<const float4*>(rows_smem + m * seg + k), x1 = *reinterpret_cast<const float4*>(rows_smem + m * seg + k + 4);
+      const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float2 xx = make_float2(x[j], x[j]);
+        acc[m][0] = __ffma2_rn(xx, make_float2(now[j].x, now[j].y), acc[m][0]);
+        acc[m][1] = __ffma2_rn(xx, make_float2(now[j].z, now[j].w), acc[m][1]);
+      }
+    }
+  }
+  __syncthreads();                       // the rows are done with
+  float4* const part = reinterpret_cast<float4*>(rows_smem);               // [warp][MR][32 lanes]
+#pragma unroll
+  for (int m = 0; m < MR; ++m) part[(warp * MR + m) * 32 + lane] = make_float4(acc[m][0].x, acc[m][0].y, acc[m][1].x, acc[m][1].y);
+  __syncthreads();
+  auto add = [](float4& a, const float4 b) { a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w; };
+  for (int i = threadIdx.x; i < MR * 32; i += kRowThreads) {
+    float4 t = part[i];
+#pragma unroll
+    for (int v = 1; v < kRowWarps; ++v) add(t, part[v * MR * 32 + i]);
+    part[i] = t;
+  }
+  if (ranks > 1) cluster.sync(); else __syncthreads();
+  uint32_t top = 0;
+  for (int i = rank * kRowThreads + threadIdx.x; i < MR * 16; i += ranks * kRowThreads) {
+    const int m = i >> 4, l = i & 15, c = (int)(blockIdx.x / ranks) * 64 + l * 4;
+    if (m >= p.M || c >= q.F) continue;
+    float4 g = make_float4(0.f, 0.f, 0.f, 0.f), v = g;
+    for (int r = 0; r < ranks; ++r) {
+      const float4* const from = ranks > 1 ? cluster.map_shared_rank(part, r) : part;
+      add(g, from[m * 32 + l]);
+      add(v, from[m * 32 + 16 + l]);
+    }
+    const float gate[4] = {g.x, g.y, g.z, g.w}, value[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (q.gates) { q.gates[(long long)m * 2 * q.F + c + j] = gate[j]; q.gates[(long long)m * 2 * q.F + q.F + c + j] = value[j]; }
+      const float o = gate_value<ACT>(gate[j]) * value[j];
+      q.out[(long long)m * q.F + c + j] = o;
+      top = max(top, amax_bits(o));
+    }
+  }
+  if (ranks > 1) cluster.sync();           // nobody leaves while its shared memory is still read
+  amax_commit(q.am, top);
+}
+
 // C = A[M x K] B[N x K]^T: a warp owns two rows of B along a run of K, a lane 4 columns at a time; the rows of A come through L1.
 // (Four rows a warp halve those reads and take registers: the same time.)
 constexpr int kRowSet = 2;
@@ -398,6 +429,36 @@ static int rows_matmul(const SimtGemm& p, bool tA, bool tB, cudaStream_t s) {
     return 1;
   }
   return 0;
+}
+
+// A gated layer on up to 16 rows with a million weights and more: 1 done, 0 not one of those, -1 error
+template <int MR> static int launch_rows_gated(RowsGated q, int activation, cudaStream_t s) {
+  SimtGemm& p = q.g;
+  const int sms = device_sm_count(), groups = (q.F + 63) / 64;
+  int cluster = 1;
+  auto smem = [&] { return std::max((size_t)p.k_per_cta * MR, (size_t)kRowWarps * MR * kRowCols) * sizeof(float); };
+  auto cut = [&] { p.k_per_cta = (int)(((long long)p.K + cluster * kRowWarps * 8 - 1) / (cluster * kRowWarps * 8)) * kRowWarps * 8; };        // a warp's run is a multiple of 8
+  cut();
+  while (cluster < 8 && (groups * cluster < 2 * sms || smem() > kRowSmem / 2) && p.K >= 64 * kRowWarps * cluster) { cluster *= 2; cut(); }
+  if (smem() > kRowSmem || groups * cluster < sms) return 0;
+  KernelTimer kt("rows_gated", s, 4.0 * (double)p.M * q.F * p.K, 0, 1);
+  q.am = amax_track_begin(q.out);
+  cudaError_t e = cudaSuccess;
+  with_gate(activation, [&](auto act) {
+    constexpr int ACT = decltype(act)::value;
+    static const cudaError_t attr = cudaFuncSetAttribute(rows_gated_kernel<MR, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRowSmem);
+    e = attr;
+    if (e == cudaSuccess) e = launch_cluster(rows_gated_kernel<MR, ACT>, cluster, dim3(groups * cluster), dim3(kRowThreads), smem(), s, q);
+  });
+  TF_CUDA(e);
+  TF_AFTER(s, "rows_gated");
+  return 1;
+}
+int rows_gated(const float* x, const float* w, float* gates, float* out, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s) {
+  if (M > kFewRows || (double)K * 2 * F < 1e6 || F % 4 || !aligned16(w)) return 0;
+  RowsGated q{SimtGemm{x, w, nullptr, (int)M, (int)(2 * F), (int)K, K, 2 * F, 0, 0, 0, 1, 0}, gates, out, (int)F, AmaxOut{}};
+  note_compute_stream(s);
+  return M == 1 ? launch_rows_gated<1>(q, activation, s) : M <= 8 ? launch_rows_gated<8>(q, activation, s) : launch_rows_gated<16>(q, activation, s);
 }
 
 static thread_local std::vector<SimtJob> t_held_simt;

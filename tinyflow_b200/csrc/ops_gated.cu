@@ -15,6 +15,9 @@ namespace tf {
 int matmul_any(const float* A, bool tA, const float* B, bool tB, float* C, int64_t M, int64_t N, int64_t K, cudaStream_t s, const char* what);
 int tc_gated_fwd(const float* x, const float* w, float* gates, float* out, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s, const char* what);
 int tc_gated_bwd(const float* x, const float* w, const float* z, const float* dout, float* dx, float* dw, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s, const char* what);
+int rows_gated(const float* x, const float* w, float* gates, float* out, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s);
+int gated_small_fwd(const float* x, const float* w, float* gates, float* out, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s, const char* what);
+int gated_small_bwd(const float* x, const float* w, const float* z, const float* dout, float* dx, float* dw, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s, const char* what);
 void note_contraction_path(int path);
 bool pause_holding();                    // what follows is not to wait; returns whether it could have
 void hold_products(bool on);
@@ -147,6 +150,11 @@ int TfGatedLinearForward(const DLArrayHandle input, const DLArrayHandle weight, 
       return r < 0 ? -1 : 0;
     }
   }
+  if (contraction_path() != 2) {
+    int r = rows_gated((const float*)input->data, (const float*)weight->data, z, out, M, F, K, activation, s);
+    if (!r) r = gated_small_fwd((const float*)input->data, (const float*)weight->data, z, out, M, F, K, activation, s, what);
+    if (r) { note_contraction_path(1); return r < 0 ? -1 : 0; }
+  }
   StreamLease lease(s);
   const size_t bytes = sizeof(float) * (size_t)M * 2 * F;
   if (!z && !(z = (float*)lease.scratch(kScratchGates, bytes))) return short_of(bytes, memorytoSaving);
@@ -175,6 +183,12 @@ int TfGatedLinearBackward(const DLArrayHandle input, const DLArrayHandle weight,
   if (!contraction_path_is_cuda_cores()) {
     if (const int r = tc_gated_bwd((const float*)input->data, (const float*)weight->data, (const float*)gates->data, (const float*)doutput->data, dx, dw, M, F, K, activation, s, what)) {
       note_contraction_path(2);
+      return r < 0 ? -1 : 0;
+    }
+  }
+  if (contraction_path() != 2 && !(M <= 16 && (double)K * 2 * F >= 1e6)) {          // (few rows against large weights: the products have kernels for them)
+    if (const int r = gated_small_bwd((const float*)input->data, (const float*)weight->data, (const float*)gates->data, (const float*)doutput->data, dx, dw, M, F, K, activation, s, what)) {
+      note_contraction_path(1);
       return r < 0 ? -1 : 0;
     }
   }
