@@ -75,34 +75,72 @@ template <int ACT> struct GateGradient {
   }
 };
 
-// grid (ranks * ceil(F / 32), ceil(M / 32)), clusters of `ranks` along x
+// grid (ranks * ceil(F / 32), ceil(M / 32)), clusters of `ranks` along x.  Steps of 32 of K come by asynchronous copies, kAhead of them in
+// flight: a CTA of a cut reduction has them all under way at once.
+constexpr int kAhead = 4;
+struct FwdStep { float x[kTile][kPitch]; float g[kDepth][kTile], v[kDepth][kTile]; };      // x by rows, 16-byte aligned ones
 template <int ACT> __global__ void __launch_bounds__(kThreads) gated_small_fwd_kernel(const Small p) {
-  __shared__ __align__(16) Block xs[2], gs[2], vs[2];
+  extern __shared__ __align__(16) unsigned char small_smem[];
+  FwdStep* const ring = reinterpret_cast<FwdStep*>(small_smem);
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
   grid_dep_sync();
   const int m0 = blockIdx.y * kTile, f0 = (int)(blockIdx.x / ranks) * kTile, tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  const int kbeg = rank * p.per_cta, kend = min(p.K, kbeg + p.per_cta);
+  const int kbeg = rank * p.per_cta, kend = min(p.K, kbeg + p.per_cta), steps = max(0, (kend - kbeg + kDepth - 1) / kDepth);
   float g[4][2] = {}, v[4][2] = {};
-  BlockLoader<kTile, kDepth, kThreads, true> lx;
-  BlockLoader<kTile, kDepth, kThreads, false> lg, lv;
-  auto fetch = [&](int k) {
-    lx.fetch(p.x, p.K, m0, p.M, k, kend, p.x_vec);
-    lg.fetch(p.w, 2ll * p.F, f0, p.F, k, kend, p.w_vec);
-    lv.fetch(p.w + p.F, 2ll * p.F, f0, p.F, k, kend, p.w_vec);
+  // `there` of the four elements at `from`, zeros for the rest
+  auto copy4 = [](float* to, const float* from, int there, bool vec) {
+    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to);
+    if (vec) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(max(0, min(4, there)) * 4) : "memory");
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + 4 * i), "l"(i < there ? from + i : from), "r"(i < there ? 4 : 0) : "memory");
+    }
   };
-  auto put = [&](int to) { lx.put(xs[to]); lg.put(gs[to]); lv.put(vs[to]); };
-  if (kbeg < kend) { fetch(kbeg); put(0); }
-  __syncthreads();
-  int buf = 0;
-  for (int k = kbeg; k < kend; k += kDepth, buf ^= 1) {
-    const bool more = k + kDepth < kend;
-    if (more) fetch(k + kDepth);
-    multiply(xs[buf], gs[buf], ty, tx, g);
-    multiply(xs[buf], vs[buf], ty, tx, v);
-    if (more) put(buf ^ 1);
+  auto fetch = [&](int step) {
+    if (step < steps) {
+      FwdStep& st = ring[step % kAhead];
+      const int k0 = kbeg + step * kDepth;
+#pragma unroll
+      for (int i = 0; i < kTile * kDepth / 4 / kThreads; ++i) {
+        const int e = threadIdx.x + i * kThreads, line = e / 8, quad = e % 8 * 4;
+        const bool row = m0 + line < p.M, deep = k0 + line < kend;
+        const int xs = row ? kend - k0 - quad : 0, ws = deep ? p.F - f0 - quad : 0;
+        copy4(&st.x[line][quad], xs > 0 ? p.x + (long long)(m0 + line) * p.K + k0 + quad : p.x, xs, p.x_vec);
+        const float* const w = ws > 0 ? p.w + (long long)(k0 + line) * 2 * p.F + f0 + quad : p.w;
+        copy4(&st.g[line][quad], w, ws, p.w_vec);
+        copy4(&st.v[line][quad], ws > 0 ? w + p.F : p.w, ws, p.w_vec);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) fetch(i);
+  for (int step = 0; step < steps; ++step) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
     __syncthreads();
+    const FwdStep& st = ring[step % kAhead];
+#pragma unroll
+    for (int k = 0; k < kDepth; k += 4) {
+      float x[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(x[i]) = *reinterpret_cast<const float4*>(&st.x[ty * 4 + i][k]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 a = *reinterpret_cast<const float2*>(&st.g[k + j][tx * 2]), b = *reinterpret_cast<const float2*>(&st.v[k + j][tx * 2]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          g[i][0] = fmaf(x[i][j], a.x, g[i][0]); g[i][1] = fmaf(x[i][j], a.y, g[i][1]);
+          v[i][0] = fmaf(x[i][j], b.x, v[i][0]); v[i][1] = fmaf(x[i][j], b.y, v[i][1]);
+        }
+      }
+    }
+    if (step + kAhead < steps) __syncthreads();                // nobody reads what comes next into its place
+    fetch(step + kAhead);
   }
+  __syncthreads();
   uint32_t top = 0;
   auto finish = [&](int row, int col, float gate, float value) {
     const int m = m0 + row, f = f0 + col;
@@ -118,8 +156,8 @@ template <int ACT> __global__ void __launch_bounds__(kThreads) gated_small_fwd_k
 #pragma unroll
       for (int j = 0; j < 2; ++j) finish(ty * 4 + i, tx * 2 + j, g[i][j], v[i][j]);
   } else {
-    float* const part = &xs[0][0][0];            // gates, then values, 32 x 32 each (both blocks of x are done with)
-    static_assert(sizeof(xs) >= 2 * kTile * kTile * sizeof(float), "a tile's partial sums fit where x was");
+    float* const part = reinterpret_cast<float*>(small_smem);            // gates, then values, 32 x 32 each, where the first step was
+    static_assert(sizeof(FwdStep) >= 2 * kTile * kTile * sizeof(float), "a tile's partial sums fit there");
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -145,6 +183,7 @@ template <int ACT> __global__ void __launch_bounds__(kThreads) gated_small_fwd_k
 
 // Clusters of `ranks`: the first dx_tiles of them a tile of dx each, cut over the cluster, the others `ranks` tiles of dW, one a CTA.
 // A step of 32 of the reduction is 16 columns of each half for dx, 32 rows for dW; a tile of dW is 32 rows x 16 columns of each half.
+constexpr int kLoads = 4;           // steps of dx whose loads are in flight at once
 template <int ACT> __global__ void __launch_bounds__(kThreads) gated_small_bwd_kernel(const Small p) {
   __shared__ __align__(16) Block as[2], bs[2];
   cg::cluster_group cluster = cg::this_cluster();
@@ -152,37 +191,40 @@ template <int ACT> __global__ void __launch_bounds__(kThreads) gated_small_bwd_k
   grid_dep_sync();
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16, line = threadIdx.x / 4, quad = threadIdx.x % 4 * 4;
   float acc[4][2] = {};
-  GateGradient<ACT> dz;
-  int buf = 0;
+  GateGradient<ACT> dz[kLoads];
   if (id < p.dx_tiles) {
     const int m0 = id / p.dx_across * kTile, n0 = id % p.dx_across * kTile, fbeg = rank * p.per_cta, fend = min(p.F, fbeg + p.per_cta);
-    float4 wg, wv;
-    auto fetch = [&](int f) {
-      dz.fetch(p, m0 + line, f + quad);
-      wg = wv = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (n0 + line < p.K) {
+    float4 wg[kLoads], wv[kLoads];
+    auto fetch = [&](int f, int at) {
+      dz[at].fetch(p, f < fend ? m0 + line : p.M, f + quad);
+      wg[at] = wv[at] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (n0 + line < p.K && f < fend) {
         const float* const row = p.w + (long long)(n0 + line) * 2 * p.F;
-        wg = four(row, f + quad, p.F, p.w_vec);
-        wv = four(row + p.F, f + quad, p.F, p.w_vec);
+        wg[at] = four(row, f + quad, p.F, p.w_vec);
+        wv[at] = four(row + p.F, f + quad, p.F, p.w_vec);
       }
     };
-    auto put = [&](int to) {
+    auto put = [&](int at, int to) {
       float dg[4], dv[4];
-      dz.form(dg, dv);
-      const float g[4] = {wg.x, wg.y, wg.z, wg.w}, v[4] = {wv.x, wv.y, wv.z, wv.w};
+      dz[at].form(dg, dv);
+      const float g[4] = {wg[at].x, wg[at].y, wg[at].z, wg[at].w}, v[4] = {wv[at].x, wv[at].y, wv[at].z, wv[at].w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         as[to][quad + i][line] = dg[i]; as[to][16 + quad + i][line] = dv[i];
         bs[to][quad + i][line] = g[i]; bs[to][16 + quad + i][line] = v[i];
       }
     };
-    if (fbeg < fend) { fetch(fbeg); put(0); }
-    __syncthreads();
-    for (int f = fbeg; f < fend; f += kDepth / 2, buf ^= 1) {
-      const bool more = f + kDepth / 2 < fend;
-      if (more) fetch(f + kDepth / 2);
-      multiply(as[buf], bs[buf], ty, tx, acc);
-      if (more) put(buf ^ 1);
+    for (int f = fbeg; f < fend; f += kLoads * 16) {
+#pragma unroll
+      for (int at = 0; at < kLoads; ++at) fetch(f + at * 16, at);
+#pragma unroll
+      for (int at = 0; at < kLoads; ++at) {
+        if (f + at * 16 < fend) {                // the same for the whole block
+          put(at, at & 1);
+          __syncthreads();
+          multiply(as[at & 1], bs[at & 1], ty, tx, acc);
+        }
+      }
       __syncthreads();
     }
     if (ranks == 1) {
@@ -218,26 +260,29 @@ template <int ACT> __global__ void __launch_bounds__(kThreads) gated_small_bwd_k
   const int tile = (id - p.dx_tiles) * ranks + rank;
   if (tile >= p.dw_tiles) return;
   const int k0 = tile / p.dw_across * kTile, f0 = tile % p.dw_across * 16;
-  BlockLoader<kTile, kDepth, kThreads, false> lx;
-  auto fetch = [&](int m) {
-    lx.fetch(p.x, p.K, k0, p.K, m, p.M, p.x_vec);
-    dz.fetch(p, m + line, f0 + quad);
+  BlockLoader<kTile, kDepth, kThreads, false> lx[2];
+  auto fetch = [&](int m, int at) {
+    lx[at].fetch(p.x, p.K, k0, p.K, m, p.M, p.x_vec);
+    dz[at].fetch(p, m + line, f0 + quad);
   };
-  auto put = [&](int to) {
+  auto put = [&](int at) {
     float dg[4], dv[4];
-    lx.put(as[to]);
-    dz.form(dg, dv);
-    *reinterpret_cast<float4*>(&bs[to][line][quad]) = make_float4(dg[0], dg[1], dg[2], dg[3]);
-    *reinterpret_cast<float4*>(&bs[to][line][16 + quad]) = make_float4(dv[0], dv[1], dv[2], dv[3]);
+    lx[at].put(as[at]);
+    dz[at].form(dg, dv);
+    *reinterpret_cast<float4*>(&bs[at][line][quad]) = make_float4(dg[0], dg[1], dg[2], dg[3]);
+    *reinterpret_cast<float4*>(&bs[at][line][16 + quad]) = make_float4(dv[0], dv[1], dv[2], dv[3]);
   };
-  if (p.M > 0) { fetch(0); put(0); }
-  __syncthreads();
-  for (int m = 0; m < p.M; m += kDepth, buf ^= 1) {
-    const bool more = m + kDepth < p.M;
-    if (more) fetch(m + kDepth);
-    multiply(as[buf], bs[buf], ty, tx, acc);
-    if (more) put(buf ^ 1);
-    __syncthreads();
+  if (p.M > 0) { fetch(0, 0); fetch(kDepth, 1); }
+  for (int m = 0; m < p.M; m += 2 * kDepth) {
+#pragma unroll
+    for (int at = 0; at < 2; ++at) {
+      if (m + at * kDepth < p.M) {               // the same for the whole block
+        put(at);
+        __syncthreads();
+        fetch(m + (at + 2) * kDepth, at);
+        multiply(as[at], bs[at], ty, tx, acc);
+      }
+    }
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -272,7 +317,12 @@ int gated_small_fwd(const float* x, const float* w, float* gates, float* out, in
   note_compute_stream(s);
   KernelTimer kt("gated_small_fwd", s, 4.0 * M * F * K, 0, 1);
   cudaError_t e = cudaSuccess;
-  with_gate(activation, [&](auto act) { e = launch_cluster(gated_small_fwd_kernel<decltype(act)::value>, cluster, dim3(across * cluster, down), dim3(kThreads), 0, s, p); });
+  with_gate(activation, [&](auto act) {
+    constexpr int ACT = decltype(act)::value;
+    static const cudaError_t attr = cudaFuncSetAttribute(gated_small_fwd_kernel<ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(FwdStep) * kAhead);
+    e = attr;
+    if (e == cudaSuccess) e = launch_cluster(gated_small_fwd_kernel<ACT>, cluster, dim3(across * cluster, down), dim3(kThreads), sizeof(FwdStep) * kAhead, s, p);
+  });
   TF_CUDA(e);
   TF_AFTER(s, what);
   return 1;
