@@ -1947,77 +1947,139 @@ __global__ void __launch_bounds__(256) pack_matrix_kernel(const float* __restric
   }
 }
 
-// The weight of a gated layer, [K][gate columns | value columns] of F each -> [K][pitch]: 32 gate columns, the 32 value columns that they
-// meet, and so on, zeros past F, so that one epilogue thread of the product has both.  Eight packed columns a thread.
-template <bool VEC4, class E>
-__global__ void __launch_bounds__(256) pack_gated_weight_kernel(const float* __restrict__ src, E* __restrict__ hi, E* __restrict__ lo, long long pitch, long long rows, int F, ScaleRef sr) {
-  grid_dep_sync();
-  const float sc = pack_scale(sr, blockIdx.x == 0 && threadIdx.x == 0);
-  const long long stride = (long long)gridDim.x * blockDim.x, groups = pitch >> 3, total = rows * groups;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += stride) {
-    const long long r = i / groups;
-    const int c = (int)(i - r * groups) << 3, f = c / 64 * 32 + c % 32;
-    const float* const from = src + r * 2 * F + (c & 32 ? F : 0) + f;
-    float v[8];
-    if (VEC4 && f + 8 <= F) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(from)), b = __ldg(reinterpret_cast<const float4*>(from) + 1);
-      v[0] = a.x * sc; v[1] = a.y * sc; v[2] = a.z * sc; v[3] = a.w * sc; v[4] = b.x * sc; v[5] = b.y * sc; v[6] = b.z * sc; v[7] = b.w * sc;
-    } else {
+// ---- operands of gated layers: all of a call in one launch for their maxima and one for their packs ------------------------------
+// (a launch each and the clearing of their words made eleven of the gradients' call; 777 x 500 x 1003 forward 35.2 us, so TIMES)
+// kRows: a matrix as it lies.  kWeight: [K][gate columns | value columns] of F each -> 32 gate columns, the 32 value columns that they meet,
+// and so on, zeros past F, so that one epilogue thread of the product has both.  kGradient: dz = [dout * value * act'(gate) | dout * act(gate)],
+// formed from the projections wherever it is wanted and never written as numbers of its own.
+enum { kRows = 0, kWeight = 1, kGradient = 2 };
+struct Operand {
+  int kind, F, vec;                // vec: kRows, kWeight: rows can be read 16 bytes at a time; kGradient: eight columns at a time
+  int first, blocks;               // of the launch
+  const float *src, *dout;         // kGradient: the projections, and the gradient of the output
+  void *hi, *lo;
+  long long rows, cols, pitch;     // cols: of src
+  uint32_t* max;                   // where its maximum is reduced to (null: its producer left it, or the arithmetic needs none)
+  ScaleRef scale;
+};
+struct Operands3 { int n; Operand op[3]; uint32_t* words; uint32_t blocks; };            // words: three maxima and a counter, zero between calls
+__device__ __forceinline__ const Operand& operand_of(const Operands3& all) {
+  int k = 0;
+  while (k + 1 < all.n && (int)blockIdx.x >= all.op[k + 1].first) ++k;
+  return all.op[k];
+}
+// dz of N columns from f on: 12 bytes read per column
+template <int ACT, int N> __device__ __forceinline__ void gate_gradient(const Operand& o, long long r, int f, float* dg, float* dv) {
+  const float *const z = o.src + r * 2 * o.F + f, *const d = o.dout + r * o.F + f;
+  float g[N], v[N], t[N];
+  if (N == 8) {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] = f + q < F ? __ldg(from + q) * sc : 0.f;
+    for (int q = 0; q < N; q += 4) {
+      *reinterpret_cast<float4*>(g + q) = __ldg(reinterpret_cast<const float4*>(z + q));
+      *reinterpret_cast<float4*>(v + q) = __ldg(reinterpret_cast<const float4*>(z + o.F + q));
+      *reinterpret_cast<float4*>(t + q) = __ldg(reinterpret_cast<const float4*>(d + q));
     }
-    store8(hi, lo, r * pitch + c, v);
+  } else {
+    g[0] = __ldg(z); v[0] = __ldg(z + o.F); t[0] = __ldg(d);
+  }
+#pragma unroll
+  for (int q = 0; q < N; ++q) {
+    float value, slope;
+    gate_slope<ACT>(g[q], value, slope);
+    dg[q] = t[q] * v[q] * slope;
+    dv[q] = t[q] * value;
   }
 }
-// The gradient of a gated layer's projections, dz = [dout * value * act'(gate) | dout * act(gate)], packed as it is computed: it is never
-// written as numbers of its own.  STORE = false: only its largest magnitude, which the pack's scale needs.  8 columns of each half a
-// thread (VEC8: F a multiple of 8, 16-byte aligned rows), else one.  12 bytes read per column and pass, 8 written.
-template <int ACT, bool STORE, bool VEC8, class E>
-__global__ void __launch_bounds__(256) pack_gate_gradient_kernel(const float* __restrict__ z, const float* __restrict__ dout, E* __restrict__ hi, E* __restrict__ lo, long long pitch,
-                                                                 long long rows, int F, ScaleRef sr, uint32_t* amax) {
-  grid_dep_sync();
-  const float sc = STORE ? pack_scale(sr, blockIdx.x == 0 && threadIdx.x == 0) : 1.f;
-  constexpr int N = VEC8 ? 8 : 1;
-  const int groups = F / N;
-  const long long stride = (long long)gridDim.x * blockDim.x, total = rows * groups;
+template <int ACT, int N> __device__ __forceinline__ uint32_t gradient_max(const Operand& o, long long first, long long stride) {
+  const int groups = o.F / N;
   uint32_t top = 0;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += stride) {
+  for (long long i = first; i < o.rows * groups; i += stride) {
     const long long r = i / groups;
-    const int f = (int)(i - r * groups) * N;
-    const float *const zr = z + r * 2 * F + f, *const dr = dout + r * F + f;
-    float g[N], v[N], d[N];
-    if (VEC8) {
+    float dg[N], dv[N];
+    gate_gradient<ACT, N>(o, r, (int)(i - r * groups) * N, dg, dv);
 #pragma unroll
-      for (int q = 0; q < N; q += 4) {
-        *reinterpret_cast<float4*>(g + q) = __ldg(reinterpret_cast<const float4*>(zr + q));
-        *reinterpret_cast<float4*>(v + q) = __ldg(reinterpret_cast<const float4*>(zr + F + q));
-        *reinterpret_cast<float4*>(d + q) = __ldg(reinterpret_cast<const float4*>(dr + q));
+    for (int q = 0; q < N; ++q) top = max(top, max(amax_bits(dg[q]), amax_bits(dv[q])));
+  }
+  return top;
+}
+template <int ACT> __global__ void __launch_bounds__(256) operand_max_kernel(const __grid_constant__ Operands3 all) {
+  grid_dep_sync();
+  const Operand& o = operand_of(all);
+  if (!o.max) return;
+  const long long first = (long long)((int)blockIdx.x - o.first) * blockDim.x + threadIdx.x, stride = (long long)o.blocks * blockDim.x;
+  uint32_t top = 0;
+  if (o.kind == kGradient) {
+    if (ACT >= 0) top = o.vec ? gradient_max<ACT < 0 ? 0 : ACT, 8>(o, first, stride) : gradient_max<ACT < 0 ? 0 : ACT, 1>(o, first, stride);
+  } else {
+    const long long n = o.rows * o.cols;
+    long long done = 0;
+    if ((reinterpret_cast<uintptr_t>(o.src) & 15) == 0) {
+      const float4* const s4 = reinterpret_cast<const float4*>(o.src);
+      auto fold = [&](float4 v) { top = max(max(top, amax_bits(v.x)), max(amax_bits(v.y), max(amax_bits(v.z), amax_bits(v.w)))); };
+      long long i = first;
+      for (; i + 3 * stride < n / 4; i += 4 * stride) {       // four independent 16-byte loads in flight per thread
+        const float4 a = __ldg(s4 + i), b = __ldg(s4 + i + stride), c = __ldg(s4 + i + 2 * stride), d = __ldg(s4 + i + 3 * stride);
+        fold(a); fold(b); fold(c); fold(d);
       }
-    } else {
-      g[0] = __ldg(zr); v[0] = __ldg(zr + F); d[0] = __ldg(dr);
+      for (; i < n / 4; i += stride) fold(__ldg(s4 + i));
+      done = n / 4 * 4;
     }
+    for (long long k = done + first; k < n; k += stride) top = max(top, amax_bits(__ldg(o.src + k)));
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0 && top) atomicMax(o.max, top);
+}
+// Eight packed columns a thread (kGradient: eight of each half, or one).  The block that arrives last clears the maxima for the next call.
+template <int ACT, class E> __global__ void __launch_bounds__(256) pack_operands_kernel(const __grid_constant__ Operands3 all) {
+  grid_dep_sync();
+  const Operand& o = operand_of(all);
+  const long long first = (long long)((int)blockIdx.x - o.first) * blockDim.x + threadIdx.x, stride = (long long)o.blocks * blockDim.x;
+  const float sc = pack_scale(o.scale, first == 0);
+  E *const hi = (E*)o.hi, *const lo = (E*)o.lo;
+  if (o.kind == kGradient) {
+    if constexpr (ACT >= 0) {
+      if (o.vec) {
+        const int groups = o.F / 8;
+        for (long long i = first; i < o.rows * groups; i += stride) {
+          const long long r = i / groups;
+          const int f = (int)(i - r * groups) * 8;
+          float dg[8], dv[8];
+          gate_gradient<ACT, 8>(o, r, f, dg, dv);
 #pragma unroll
-    for (int q = 0; q < N; ++q) {
-      float value, slope;
-      gate_slope<ACT>(g[q], value, slope);
-      g[q] = d[q] * v[q] * slope;
-      v[q] = d[q] * value;
-      if (!STORE) top = max(top, max(amax_bits(g[q]), amax_bits(v[q])));
-      g[q] *= sc; v[q] *= sc;
+          for (int q = 0; q < 8; ++q) { dg[q] *= sc; dv[q] *= sc; }
+          store8(hi, lo, r * o.pitch + f, dg);
+          store8(hi, lo, r * o.pitch + o.F + f, dv);
+        }
+      } else {
+        for (long long i = first; i < o.rows * o.F; i += stride) {
+          const long long r = i / o.F, at = r * o.pitch + (i - r * o.F);
+          float dg, dv;
+          gate_gradient<ACT, 1>(o, r, (int)(i - r * o.F), &dg, &dv);
+          split_pair(dg * sc, hi[at], lo[at]);
+          split_pair(dv * sc, hi[at + o.F], lo[at + o.F]);
+        }
+      }
     }
-    if (!STORE) continue;
-    const long long o = r * pitch + f;
-    if constexpr (VEC8) {
-      store8(hi, lo, o, g);
-      store8(hi, lo, o + F, v);
-    } else {
-      split_pair(g[0], hi[o], lo[o]);
-      split_pair(v[0], hi[o + F], lo[o + F]);
+  } else {
+    const int groups = (int)(o.pitch >> 3);
+    for (long long i = first; i < o.rows * groups; i += stride) {
+      const long long r = i / groups;
+      const int c = (int)(i - r * groups) << 3, f = o.kind == kWeight ? c / 64 * 32 + c % 32 : c, cols = o.kind == kWeight ? o.F : (int)o.cols;
+      const float* const from = o.src + r * o.cols + (o.kind == kWeight && (c & 32) ? o.F : 0) + f;
+      float v[8];
+      if (o.vec && f + 8 <= cols) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(from)), b = __ldg(reinterpret_cast<const float4*>(from) + 1);
+        v[0] = a.x * sc; v[1] = a.y * sc; v[2] = a.z * sc; v[3] = a.w * sc; v[4] = b.x * sc; v[5] = b.y * sc; v[6] = b.z * sc; v[7] = b.w * sc;
+      } else {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = f + q < cols ? __ldg(from + q) * sc : 0.f;
+      }
+      store8(hi, lo, r * o.pitch + c, v);
     }
   }
-  if (STORE) return;
-  top = __reduce_max_sync(0xffffffffu, top);
-  if ((threadIdx.x & 31) == 0 && top) atomicMax(amax, top);
+  if (!all.words) return;
+  __syncthreads();
+  if (threadIdx.x == 0 && atomicInc(all.words + 3, all.blocks - 1) == all.blocks - 1) all.words[0] = all.words[1] = all.words[2] = 0u;
 }
 
 // NCHW activations -> pixel-major frame [N][frame_h][frame_w][pitch]:
@@ -2952,31 +3014,74 @@ template <int AR> static int launch_gated(GemmParams& p, cudaStream_t s, double 
   }
   return 0;
 }
+// The packs of a call
+struct OperandPacks {
+  Operands3 all;
+  Pack pack[3];
+  int ar;
+  explicit OperandPacks(int arith) : ar(arith) { memset(&all, 0, sizeof(all)); }
+  // 0, or 1: no memory
+  int add(StreamLease& lease, int slot, int kind, const float* src, const float* dout, long long rows, long long cols, long long packed, int F) {
+    Operand& o = all.op[all.n];
+    Pack& pk = pack[all.n++];
+    pk.rows = rows; pk.cols = packed; pk.pitch = round_up(packed, 64); pk.arith = ar;
+    char* const base = (char*)lease.scratch(slot, 2 * pk.bytes() + 16);            // bytes() is a multiple of 128; the scale behind them
+    if (!base) return 1;
+    pk.hi = base; pk.lo = base + pk.bytes(); pk.words = (uint32_t*)(base + 2 * pk.bytes());
+    o.kind = kind; o.F = F; o.src = src; o.dout = dout; o.hi = pk.hi; o.lo = pk.lo; o.rows = rows; o.cols = cols; o.pitch = pk.pitch;
+    o.vec = kind == kGradient ? F % 8 == 0 && aligned16(src) && aligned16(dout) : cols % 4 == 0 && (kind != kWeight || F % 4 == 0) && aligned16(src);
+    o.scale.scale = reinterpret_cast<float*>(pk.words + 2);
+    return 0;
+  }
+  template <int ACT> int run(StreamLease& lease, cudaStream_t s, const char* what) {
+    static const bool no_track = getenv("TINYFLOW_NO_AMAX_TRACKING") != nullptr;
+    bool reduce = false;
+    double bytes = 0;
+    if (ar == kArithF16) {
+      for (int i = 0; i < all.n; ++i) {
+        Operand& o = all.op[i];
+        if (o.kind != kGradient && !no_track && (o.scale.amax_cur = amax_tracked(o.src))) continue;         // its producer reduced it
+        if (!all.words && !(all.words = lease.counters(4))) return 1;
+        o.scale.amax_cur = o.max = all.words + i;
+        reduce = true;
+      }
+    }
+    auto deal = [&](bool maxima) {
+      int at = 0;
+      for (int i = 0; i < all.n; ++i) {
+        Operand& o = all.op[i];
+        const long long items = o.kind == kGradient ? (o.vec ? o.rows * (o.F / 8) : o.rows * o.F / 4) : maxima ? o.rows * o.cols / 16 : o.rows * o.pitch / 8;
+        o.first = at;
+        o.blocks = maxima && !o.max ? 0 : grid_for(items, 256, 2);
+        at += o.blocks;
+        bytes += o.blocks == 0 ? 0.0 : o.kind == kGradient ? 12.0 * o.rows * o.F : 4.0 * o.rows * o.cols;
+        if (!maxima) bytes += 2.0 * elem_of(ar) * o.rows * o.pitch;
+      }
+      all.blocks = (uint32_t)at;
+      return dim3((unsigned)at);
+    };
+    note_compute_stream(s);
+    KernelTimer kt("pack_operands", s, 0, 0);
+    if (reduce) TF_CUDA(launch_dep(operand_max_kernel<ACT>, deal(true), dim3(256), 0, s, all));
+    if (reduce) TF_AFTER(s, what);
+    const dim3 grid = deal(false);
+    if (ar == kArithTF32) TF_CUDA((launch_dep(pack_operands_kernel<ACT, float>, grid, dim3(256), 0, s, all)));
+    else TF_CUDA((launch_dep(pack_operands_kernel<ACT, __half>, grid, dim3(256), 0, s, all)));
+    TF_AFTER(s, what);
+    return 0;
+  }
+};
 // out = act(x Wg) * (x Wv): 1 done, 0 not a shape for the tensor path (or no memory for its packs), -1 error
 int tc_gated_fwd(const float* x, const float* w, float* gates, float* out, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s, const char* what) {
   if (!tc_takes((double)M, 2.0 * F, (double)K) || !encode_fn()) return 0;
   const int ar = tensor_arithmetic(), bk = bk_of(ar);
-  Pack pa, pb;
-  StreamLease lease(s);
   const long long cols = (F + 31) / 32 * 64;
-  int rc = pack_in_scratch(pa, lease, kScratchPackA, ar, M, K, s, nullptr);
-  if (!rc) rc = pack_in_scratch(pb, lease, kScratchPackB, ar, K, cols, s, nullptr);
+  StreamLease lease(s);
+  OperandPacks packs(ar);
+  if (packs.add(lease, kScratchPackA, kRows, x, nullptr, M, K, K, 0) || packs.add(lease, kScratchPackB, kWeight, w, nullptr, K, 2 * F, cols, (int)F)) return 0;
+  int rc = packs.run<-1>(lease, s, what);
   if (rc) return rc < 0 ? -1 : 0;
-  if (run_pack_matrix(x, K, pa, s)) return -1;
-  {
-    const ScaleRef sr = begin_pack(pb, w, K * 2 * F, s);
-    KernelTimer kt("pack_gated_weight", s, 0, 4.0 * K * 2 * F + 2.0 * elem_of(ar) * K * cols);
-    const bool vec = F % 4 == 0 && aligned16(w);
-    cudaError_t e = cudaSuccess;
-    with_elems(pb, [&](auto* hi, auto* lo) {
-      using E = std::remove_pointer_t<decltype(hi)>;
-      const dim3 grid(grid_for(K * cols / 8, 256, 2));
-      e = vec ? launch_dep(pack_gated_weight_kernel<true, E>, grid, dim3(256), 0, s, w, hi, lo, pb.pitch, (long long)K, (int)F, sr)
-              : launch_dep(pack_gated_weight_kernel<false, E>, grid, dim3(256), 0, s, w, hi, lo, pb.pitch, (long long)K, (int)F, sr);
-    });
-    TF_CUDA(e);
-    TF_AFTER(s, what);
-  }
+  const Pack &pa = packs.pack[0], &pb = packs.pack[1];
   GemmParams p;
   memset(&p, 0, sizeof(p));
   p.mode = kModeGemm; p.b_mn = 1; p.epi = kEpiRowMajor; p.a_rows = BM;
@@ -2994,42 +3099,17 @@ int tc_gated_bwd(const float* x, const float* w, const float* z, const float* do
                  const char* what) {
   if ((dx && !tc_takes((double)M, (double)K, 2.0 * F)) || (dw && !tc_takes((double)K, 2.0 * F, (double)M)) || !encode_fn()) return 0;
   const int ar = tensor_arithmetic(), bk = bk_of(ar);
-  Pack pz, pw, px;
   StreamLease lease(s);
-  int rc = pack_in_scratch(pz, lease, kScratchGates, ar, M, 2 * F, s, nullptr);
-  if (!rc && dx) rc = pack_in_scratch(pw, lease, kScratchPackB, ar, K, 2 * F, s, nullptr);
-  if (!rc && dw) rc = pack_in_scratch(px, lease, kScratchPackA, ar, M, K, s, nullptr);
+  OperandPacks packs(ar);
+  if (packs.add(lease, kScratchGates, kGradient, z, dout, M, 2 * F, 2 * F, (int)F) || (dx && packs.add(lease, kScratchPackB, kRows, w, nullptr, K, 2 * F, 2 * F, 0)) ||
+      (dw && packs.add(lease, kScratchPackA, kRows, x, nullptr, M, K, K, 0))) return 0;
+  int rc = 0;
+  with_gate(activation, [&](auto act) { rc = packs.run<decltype(act)::value>(lease, s, what); });
   if (rc) return rc < 0 ? -1 : 0;
-  note_compute_stream(s);
-  {
-    ScaleRef sr{nullptr, nullptr, reinterpret_cast<float*>(pz.words + 2), nullptr};
-    KernelTimer kt("pack_gate_gradient", s, 0, (ar == kArithTF32 ? 12.0 : 24.0) * M * F + 4.0 * elem_of(ar) * M * F);
-    const bool vec = F % 8 == 0 && aligned16(z) && aligned16(dout);
-    cudaError_t e = cudaSuccess;
-    with_gate(activation, [&](auto act) {
-      constexpr int ACT = decltype(act)::value;
-      with_elems(pz, [&](auto* hi, auto* lo) {
-        using E = std::remove_pointer_t<decltype(hi)>;
-        const dim3 grid(grid_for(vec ? M * F / 8 : M * F, 256, vec ? 2 : 4));
-        auto run = [&](auto v8) {
-          constexpr bool VEC8 = decltype(v8)::value;
-          if (std::is_same<E, __half>::value) {
-            uint32_t* const word = t_recording ? recording_word() : pz.words;
-            e = launch_dep(pack_gate_gradient_kernel<ACT, false, VEC8, E>, grid, dim3(256), 0, s, z, dout, hi, lo, pz.pitch, (long long)M, (int)F, sr, word);
-            sr.amax_cur = word;
-          }
-          if (e == cudaSuccess) e = launch_dep(pack_gate_gradient_kernel<ACT, true, VEC8, E>, grid, dim3(256), 0, s, z, dout, hi, lo, pz.pitch, (long long)M, (int)F, sr, (uint32_t*)nullptr);
-        };
-        vec ? run(std::true_type()) : run(std::false_type());
-      });
-    });
-    TF_CUDA(e);
-    TF_AFTER(s, what);
-  }
+  const Pack &pz = packs.pack[0], &pw = packs.pack[1], &px = packs.pack[dx ? 2 : 1];
   for (int k = 0; k < 2; ++k) {
     if (!(k ? dw : dx)) continue;
     const Pack &pa = k ? px : pz, &pb = k ? pz : pw;
-    if (k ? run_pack_matrix(x, K, px, s) : run_pack_matrix(w, 2 * F, pw, s)) return -1;
     const int64_t rows = k ? K : M, cols = k ? 2 * F : K, depth = k ? M : 2 * F;
     const int bn = pick_bn(cols, !k);
     GemmParams p;
