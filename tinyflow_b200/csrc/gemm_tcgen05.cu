@@ -402,12 +402,6 @@ struct alignas(128) GemmParams {
   int chunks_per_tap;             // kModeConv: K stages per tap
   int b_tap_pitch;                // kModeConv: columns per tap in the packed filter
   int ntaps;
-  // Order of the tiles: 0, column tiles first; else bands of this many row tiles, within a band row tiles first.  A wave of 148 tiles of
-  // a product whose operands L2 does not hold then reads about 12 + 12 blocks of them and not 1 + 128.
-  int band;
-  // Gated layers (kernels with GATED): the packed columns of B are 32 of the gate and the 32 of the value that they meet in turn, F of each.
-  int gated_f, activation;
-  float* gates;                   // both projections, or null
   float* out;
   uint32_t *amax, *amax_clear;    // where the epilogue leaves max|out| (null: nobody asked), and the word the next write of `out` will use
   const float* a_scale; const float* b_scale;   // device words: the power-of-two scales the packs were made with
@@ -442,6 +436,13 @@ struct alignas(128) GemmParams {
   short tap_col[kMaxTaps];        // first column of the tap's channels in A (space-to-depth packs keep one phase per column block)
   short tap_b[kMaxTaps];          // which tap block of the packed filter the tap multiplies
   short pair_shift[kMaxTaps];     // pair kernel: the tap's own row shift is tap_off + pair_shift
+  int out_shift;                  // elements from the 16-byte boundary in front of `out` to it
+  // Order of the tiles: 0, column tiles first; else bands of this many row tiles, within a band row tiles first.  A wave of 148 tiles of
+  // a product whose operands L2 does not hold then reads about 12 + 12 blocks of them and not 1 + 128.
+  int band;
+  // Gated layers (kernels with GATED): the packed columns of B are 32 of the gate and the 32 of the value that they meet in turn, F of each.
+  int gated_f, activation;
+  float* gates;                   // both projections, or null
 };
 constexpr int kMaxASlots = 4, kMaxBSlots = 16, kMaxCluster = 8;
 constexpr int kSmemBarriers = 512;
@@ -504,8 +505,9 @@ struct WorkIter {
   }
 };
 // tile index -> coordinates; n fastest so consecutive CTAs share the A tile through L2
-__device__ __forceinline__ void decode_tile(const GemmParams& p, int tile, int& mt, int& nt, int& tap) {
-  if (p.band) {
+// (BANDED: the look at p.band cost the products without bands 1-4 %)
+template <bool BANDED = false> __device__ __forceinline__ void decode_tile(const GemmParams& p, int tile, int& mt, int& nt, int& tap) {
+  if (BANDED && p.band) {
     const int per_band = p.band * p.n_tiles, b = tile / per_band, in_band = tile - b * per_band, height = min(p.band, p.m_tiles - b * p.band);
     nt = in_band / height; tap = 0;
     mt = b * p.band + in_band - nt * height;
@@ -646,10 +648,12 @@ __device__ __forceinline__ uint32_t store_gated(const GemmParams& p, float* stag
 // stages (36 KB a stage for a 3x3 window of a 28-wide image) and filters of one tile that fit stay in shared memory: with
 // 512 channels, 28 x 28, 3x3, batch 64 the product went from 625 to 548 us, with 64 channels, 224 x 224, from 1128 to 886.
 // Short reductions are bound by start and epilogue: 4000 cycles to the first MMA, 2500-4000 from the last to the end.
-// GATED: the epilogue applies the activation and the product of a gated layer (see store_gated).
-template <int BN, int AR, bool GATED = false>
+// FORM: kGated, the epilogue applies the activation and the product of a gated layer (see store_gated); that and kBanded, tiles in bands.
+enum { kPlain = 0, kBanded = 1, kGated = 2 };
+template <int BN, int AR, int FORM = kPlain>
 __global__ void __launch_bounds__(kGemmThreads, 1) gemm3x_kernel(const __grid_constant__ GemmParams p) {
   using T = Arith<AR>;
+  constexpr bool GATED = FORM == kGated;
   constexpr int BK = T::kBK;
   constexpr uint32_t kGroupStride = BK * 128;               // M/N-major operands: bytes between 128-byte-wide column groups
   constexpr int kTmemCols = 512;                            // all of it: one CTA per SM
@@ -722,7 +726,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm3x_kernel(const __grid_co
       WorkItem w;
       while (iter.next(p, w)) {
         int mt, nt, tap;
-        decode_tile(p, w.tile, mt, nt, tap);
+        decode_tile<FORM != kPlain>(p, w.tile, mt, nt, tap);
         const int m0 = mt * BM, n0 = nt * BN;
         int ch = w.k0 / period, ti = w.k0 - ch * period;
         int left = p.group_iters;         // stages to the next accumulator group
@@ -948,7 +952,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm3x_kernel(const __grid_co
     WorkItem w;
     while (ok && iter.next(p, w)) {
       int mt, nt, tap;
-      decode_tile(p, w.tile, mt, nt, tap);
+      decode_tile<FORM != kPlain>(p, w.tile, mt, nt, tap);
       const int kcount = w.kcount;
       const int n0 = nt * BN + half * HC;
       const RowAddr ra = row_address(p, mt, tap, row_in_tile);
@@ -956,7 +960,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm3x_kernel(const __grid_co
       const uint32_t col_bytes = ra.col_stride * 4u;
       char* const row_out = reinterpret_cast<char*>(p.out + ra.base + (long long)n0 * ra.col_stride);
       const int ncols = max(0, min(HC, p.N - n0));
-      const bool vec_ok = p.epi == kEpiRowMajor && (reinterpret_cast<uintptr_t>(row_out) & 15) == 0;
+      const bool vec_ok = p.epi == kEpiRowMajor && ((ra.base + n0 + p.out_shift) & 3) == 0;
 
       auto wait_group = [&](int acc_buf, int grp) -> bool {   // lane 0 polls, the warp follows (keeps .sync.aligned loads converged)
         int got = lane == 0 ? (int)mbar_wait(&acc_full[acc_buf], (grp >> 1) & 1, abort_flag) : 1;
@@ -1093,7 +1097,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm3x_kernel(const __grid_co
     constexpr int kUnroll = 4, kLanes = kGemmThreads / BM;
     const int rank = blockIdx.x % p.cluster, tile = blockIdx.x / p.cluster;
     int mt, nt, tap;
-    decode_tile(p, tile, mt, nt, tap);
+    decode_tile<FORM != kPlain>(p, tile, mt, nt, tap);
     const int row = threadIdx.x & (BM - 1);
     const RowAddr ra = row_address(p, mt, tap, row);
     const float inv_scale = (1.f / __ldg(p.a_scale)) * (1.f / __ldg(p.b_scale));
@@ -1398,7 +1402,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm3x_group_kernel(const __g
       float* const dst = q.out + ra.base + (long long)n0 * ra.col_stride;
 #pragma unroll
       for (int c = 0; c < HC / 2; ++c) total[c] = __fmul2_rn(total[c], scale2);
-      if (q.epi == kEpiRowMajor && (reinterpret_cast<uintptr_t>(dst) & 15) == 0 && ncols == HC) {
+      if (q.epi == kEpiRowMajor && ((ra.base + n0 + q.out_shift) & 3) == 0 && ncols == HC) {
 #pragma unroll
         for (int c = 0; c < HC / 4; ++c) reinterpret_cast<float4*>(dst)[c] = make_float4(total[2 * c].x, total[2 * c].y, total[2 * c + 1].x, total[2 * c + 1].y);
       } else {
@@ -1577,7 +1581,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm3x_pair_kernel(const __grid_c
       const uint32_t col_stride = ra.col_stride;
       float* const row_out = p.out + ra.base + (long long)n0 * col_stride;
       const int ncols = max(0, min(HC, p.N - n0));
-      const bool vec_ok = p.epi == kEpiRowMajor && (reinterpret_cast<uintptr_t>(row_out) & 15) == 0;
+      const bool vec_ok = p.epi == kEpiRowMajor && ((ra.base + n0 + p.out_shift) & 3) == 0;
       float accv[HC];
 #pragma unroll
       for (int q = 0; q < HC; ++q) accv[q] = 0.f;
@@ -1639,7 +1643,7 @@ template <bool MANY> constexpr int kReduceThreads = MANY ? 512 : 256;
 template <int BN, bool MANY, class Piece>
 __device__ __forceinline__ void reduce_tile(const GemmParams& p, int tile, int pieces, int chunk, Piece&& piece) {
   int mt, nt, tap;
-  decode_tile(p, tile, mt, nt, tap);
+  decode_tile<true>(p, tile, mt, nt, tap);
   constexpr int COLS = MANY ? 1 : 4;
   const int row = MANY ? blockIdx.z * 32 + (threadIdx.x & 31) : threadIdx.x & (BM - 1);
   const int c0 = blockIdx.y * kReduceCols + (MANY ? threadIdx.x / 32 : threadIdx.x / BM * COLS);
@@ -1779,7 +1783,7 @@ __global__ void __launch_bounds__(256) reduce_gated_kernel(const __grid_constant
       }
   }
   int mt, nt, tap;
-  decode_tile(p, p.full_tiles + t, mt, nt, tap);
+  decode_tile<true>(p, p.full_tiles + t, mt, nt, tap);
   const int m = mt * BM + row, f = nt * (BN / 2) + gate, F = p.gated_f;
   const float inv_scale = (1.f / __ldg(p.a_scale)) * (1.f / __ldg(p.b_scale));
   uint32_t top = 0;
@@ -2472,8 +2476,8 @@ static int plan_smem(GemmParams& g, int bn, int grid, int reserved = 0) {
 }
 
 // The kernel may use all shared memory: asked for ahead of its first launch and of the first question how many clusters of it fit
-template <int BN, int AR> static cudaError_t gemm_kernel_ready() {
-  static const cudaError_t attr = cudaFuncSetAttribute(gemm3x_kernel<BN, AR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit + 1024);
+template <int BN, int AR, int FORM = kPlain> static cudaError_t gemm_kernel_ready() {
+  static const cudaError_t attr = cudaFuncSetAttribute(gemm3x_kernel<BN, AR, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit + 1024);
   return attr;
 }
 template <int BN, int AR> static int max_clusters_of(int c) {
@@ -2538,6 +2542,7 @@ template <int BN, int AR> static bool held_back(const GemmParams& p, size_t work
 template <int BN, int AR> static int launch_planned(GemmParams& p, size_t workspace_bytes, bool may_wait, cudaStream_t s, double flops, const char* what, int* oom);
 template <int BN, int AR> static int launch_gemm(GemmParams& p, cudaStream_t s, double flops, const char* what, int* oom) {
   TF_CUDA((gemm_kernel_ready<BN, AR>()));
+  if constexpr (BN == 128) if (p.band) TF_CUDA((gemm_kernel_ready<BN, AR, kBanded>()));
   TF_REQUIRE(tensor_path_error() == 0, "%s: an earlier tensor-core kernel timed out on a barrier; refusing to launch", what);
   const size_t bytes = plan_launch<BN, AR>(p);
   return launch_planned<BN, AR>(p, bytes, p.hold != 0, s, flops, what, oom);
@@ -2561,7 +2566,9 @@ template <int BN, int AR> static int launch_planned(GemmParams& p, size_t bytes,
   if (p.cluster > 1) {
     TF_CUDA(launch_cluster(gemm3x_kernel<BN, AR>, p.cluster, dim3(grid), dim3(kGemmThreads), (size_t)gemm_smem_bytes(p, BN), s, p));
   } else {
-    TF_CUDA(launch_dep(gemm3x_kernel<BN, AR>, dim3(grid), dim3(kGemmThreads), (size_t)gemm_smem_bytes(p, BN), s, p));
+    auto kernel = gemm3x_kernel<BN, AR>;
+    if constexpr (BN == 128) if (p.band) kernel = gemm3x_kernel<BN, AR, kBanded>;
+    TF_CUDA(launch_dep(kernel, dim3(grid), dim3(kGemmThreads), (size_t)gemm_smem_bytes(p, BN), s, p));
   }
   TF_AFTER(s, what);
   if (p.tail_share > 0) {
@@ -2800,6 +2807,7 @@ template <int AR> static int launch_gemm_pair(const GemmParams& p, cudaStream_t 
   }
   TF_REQUIRE(tensor_path_error() == 0, "%s: an earlier tensor-core kernel timed out on a barrier; refusing to launch", what);
   static const int group_iters = getenv("TINYFLOW_GROUP_ITERS") ? atoi(getenv("TINYFLOW_GROUP_ITERS")) : 0;
+  const_cast<GemmParams&>(p).out_shift = (int)(reinterpret_cast<uintptr_t>(p.out) >> 2 & 3);
   const_cast<GemmParams&>(p).group_iters = group_iters > 0 ? group_iters : (p.data_by_data ? kGroupItersDataByData : (AR == kArithTF32 ? kGroupItersTF32 : kGroupIters));
   const int pair_tiles = ((p.m_tiles + 1) / 2) * p.n_tiles * p.tap_tiles;
   const int pairs = std::min(device_sm_count() / 2, pair_tiles);
@@ -2826,6 +2834,7 @@ template <int AR> static int launch_gemm_ar(int bn, GemmParams& p, cudaStream_t 
 // Plans the schedule (which may need workspace) and launches.  Returns 0 on success, -1 on error, 1 when the workspace
 // could not be allocated (*oom holds the byte count).
 static int launch_gemm_bn(int bn, int ar, GemmParams& p, cudaStream_t s, double flops, const char* what, int* oom) {
+  p.out_shift = (int)(reinterpret_cast<uintptr_t>(p.out) >> 2 & 3);
   if (p.a_rows == 0) p.a_rows = BM;
   return ar == kArithTF32 ? launch_gemm_ar<kArithTF32>(bn, p, s, flops, what, oom) : launch_gemm_ar<kArithF16>(bn, p, s, flops, what, oom);
 }
@@ -2993,8 +3002,7 @@ static int gemm_maps(GemmParams& p, int ar, const Pack& pa, const Pack& pb, int 
 }
 template <int AR> static int launch_gated(GemmParams& p, cudaStream_t s, double flops, const char* what, int* oom) {
   constexpr int BN = 128;
-  static const cudaError_t attr = cudaFuncSetAttribute(gemm3x_kernel<BN, AR, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit + 1024);
-  TF_CUDA(attr);
+  TF_CUDA((gemm_kernel_ready<BN, AR, kGated>()));
   TF_REQUIRE(tensor_path_error() == 0, "%s: an earlier tensor-core kernel timed out on a barrier; refusing to launch", what);
   const size_t bytes = plan_schedule(p, BN, [](int) { return 0; });          // no clusters: their sum does not know of gates
   plan_groups<BN, AR>(p);
@@ -3006,7 +3014,7 @@ template <int AR> static int launch_gated(GemmParams& p, cudaStream_t s, double 
   const int grid = plan_smem(p, BN, plan_grid(p), kGatedStage);
   note_compute_stream(s);
   KernelTimer kt(AR == kArithTF32 ? "gemm3xtf32_gated" : "gemm3xf16_gated", s, flops, 0, 1);
-  TF_CUDA(launch_dep(gemm3x_kernel<BN, AR, true>, dim3(grid), dim3(kGemmThreads), (size_t)gemm_smem_bytes(p, BN) + kGatedStage, s, p));
+  TF_CUDA(launch_dep(gemm3x_kernel<BN, AR, kGated>, dim3(grid), dim3(kGemmThreads), (size_t)gemm_smem_bytes(p, BN) + kGatedStage, s, p));
   TF_AFTER(s, what);
   if (p.tail_share > 0) {
     TF_CUDA(launch_dep(reduce_gated_kernel, dim3(p.tail_tiles, 8), dim3(256), 0, s, p));
@@ -3118,7 +3126,7 @@ int tc_gated_bwd(const float* x, const float* w, const float* z, const float* do
     if (gemm_maps(p, ar, pa, pb, bn)) return -1;
     p.M = (int)rows; p.N = (int)cols; p.m_tiles = (int)((rows + BM - 1) / BM); p.n_tiles = (int)((cols + bn - 1) / bn); p.tap_tiles = 1;
     p.k_total = (int)((depth + bk - 1) / bk);
-    p.out = k ? dw : dx; p.ldc = cols; p.err = error_word(); p.band = band_of(p);
+    p.out = k ? dw : dx; p.ldc = cols; p.err = error_word(); p.band = bn == 128 ? band_of(p) : 0;
     int oom = 0;
     rc = launch_gemm_bn(bn, ar, p, s, 2.0 * rows * cols * depth, what, &oom);
     if (rc) return rc < 0 ? -1 : 0;
