@@ -165,6 +165,109 @@ def test_the_call_does_not_wait_where_products_are_held(env):
     assert all(np.array_equal(a, b) for a, b in zip(*got))
 
 
+@pytest.mark.parametrize("M,K,F", [(40, 96, 64), (9, 1024, 2048), (700, 512, 520), (20, 1024, 4100)])
+def test_a_captured_block_replayed_on_other_data(env, M, K, F):
+    """Norm, gated layer and both backward calls in a graph that the caller captures: its replays have the bits of ordinary calls whatever the
+    sizes of the numbers were at the capture, before it and in the replays in between."""
+    import ctypes
+    import torch
+    nd, op = env.nd, env.gpu_op
+    rng = np.random.RandomState(M)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    cell = ctypes.pointer(ctypes.c_void_p(side.cuda_stream))
+    shapes = {"h": (M, K), "r": (M, K), "g": (K,), "b": (K,), "s": (M, K), "y": (M, K), "w": (K, 2 * F), "z": (M, 2 * F), "o": (M, F), "do": (M, F), "dy": (M, K), "dw": (K, 2 * F),
+              "dh": (M, K), "dr": (M, K), "dg": (K,), "db": (K,)}
+    a = {n: nd.array(rng.randn(*s).astype(np.float32), env.ctx) for n, s in shapes.items()}
+    state = op.dropout_state(0.3, 4)
+
+    def work(stream):
+        op.dropout_add_layer_norm_forward(a["h"], a["r"], a["g"], a["b"], a["s"], a["y"], state, 1e-5, stream)
+        op.gated_linear_forward(a["y"], a["w"], a["z"], a["o"], "silu", stream)
+        op.gated_linear_backward(a["y"], a["w"], a["z"], a["do"], a["dy"], a["dw"], "silu", stream)
+        op.dropout_add_layer_norm_backward(a["s"], a["g"], a["dy"], None, a["dh"], a["dr"], a["dg"], a["db"], state, 1e-5, stream)
+
+    def fill(size):
+        for n in ("h", "r", "g", "w", "do"):
+            a[n][:] = (size * rng.randn(*shapes[n])).astype(np.float32)
+
+    results = ("s", "y", "z", "o", "dy", "dw", "dh", "dr", "dg", "db")
+    fill(30.0)
+    work(cell)                                               # ordinary calls that leave their maxima
+    op.device_synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        work(cell)
+    for size in (1.0, 1e4, 1e-3, 0.5):
+        fill(size)
+        for n in results:
+            a[n][:] = np.full(shapes[n], np.nan, np.float32)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = {n: a[n].asnumpy() for n in results}
+        work(env.stream)
+        op.device_synchronize()
+        for n in results:
+            assert np.isfinite(got[n]).all(), (size, n)
+            np.testing.assert_array_equal(got[n], a[n].asnumpy(), err_msg="%s at %g" % (n, size))
+
+
+@pytest.mark.parametrize("M,K,F", [(40, 96, 64), (9, 1024, 2048), (700, 512, 520)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_a_row_that_is_not_finite_stays_by_itself(env, M, K, F, bad):
+    """The other rows keep their precision: the scale of the tensor path is taken from finite values."""
+    x, w, dout = inputs(M, K, F)
+    x *= np.float32(1e-3)
+    row = M // 2
+    x[row, K // 3] = bad
+    X, W, D = (env.nd.array(v, env.ctx) for v in (x, w, dout))
+    Z, H, DX, DW = (env.nd.empty(s, env.ctx) for s in ((M, 2 * F), (M, F), (M, K), (K, 2 * F)))
+    env.gpu_op.gated_linear_forward(X, W, Z, H, "silu", env.stream)
+    env.gpu_op.gated_linear_backward(X, W, Z, D, DX, DW, "silu", env.stream)
+    z, rest = Z.asnumpy(), np.arange(M) != row
+    assert not np.isfinite(z[row]).any() and not np.isfinite(H.asnumpy()[row]).all()
+    x64, w64 = x[rest].astype(np.float64), w.astype(np.float64)
+    close_dot(z[rest], x64 @ w64, np.abs(x64) @ np.abs(w64), what="gates")
+    assert np.isfinite(H.asnumpy()[rest]).all() and np.isfinite(DX.asnumpy()[rest]).all()
+
+
+def test_two_streams_at_once(env):
+    """Calls on two streams from two threads: scratch, states and counters are each stream's own."""
+    import threading
+    nd, op, runs = env.nd, env.gpu_op, 12
+    cells = [env.stream, op.create_cudaStream()]
+    want, got, errors = [], [], []
+
+    def work(k, seen, stream):
+        x, w, dout = inputs((700, 333)[k], 512, 520, seed=k)
+        X, W, D = (nd.array(v, env.ctx) for v in (x, w, dout))
+        G, B = (nd.array(np.ones(512, np.float32), env.ctx) for _ in range(2))
+        Z, H, DX, DW, Y, DN, DG, DB = (nd.empty(s, env.ctx) for s in ((len(x), 1040), (len(x), 520), x.shape, w.shape, x.shape, x.shape, (512,), (512,)))
+        op.device_synchronize()
+        for _ in range(runs):
+            op.layer_norm_forward(X, G, B, Y, 1e-5, stream)
+            op.gated_linear_forward(Y, W, Z, H, "gelu", stream)
+            op.gated_linear_backward(Y, W, Z, D, DX, DW, "gelu", stream)
+            op.layer_norm_backward(X, G, DX, DN, DG, DB, 1e-5, stream)
+        op.device_synchronize()
+        seen.append((k, [v.asnumpy() for v in (Z, H, DX, DW, DN, DG, DB)]))
+
+    def guarded(k, seen, stream):
+        try:
+            work(k, seen, stream)
+        except Exception as e:       # noqa: BLE001
+            errors.append(e)
+
+    for k in range(2):
+        work(k, want, cells[k])
+    threads = [threading.Thread(target=guarded, args=(k, got, cells[k])) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for k, arrays in got:
+        assert all(np.array_equal(a, b) for a, b in zip(arrays, dict(want)[k]))
+
+
 # ---- graphs ---------------------------------------------------------------------------------------------------------
 def block_step(monkeypatch, recorded=False, steps=1, plan=None, optimizer="sgd", **kind):
     import queue

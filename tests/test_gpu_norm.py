@@ -271,3 +271,31 @@ def test_gradients_against_differences(env, shape):
                 sides.append(loss(*moved))
             want = (sides[0] - sides[1]) / 2e-5
             assert abs(got[at] - want) <= bound[at] + 1e-7 * (1 + abs(want)), (k, at, got[at], want)
+
+
+def test_elements_beyond_32_bits(env):
+    """The last rows of an array of 2^31 + elements.  The numbers are a dropout of ones, made on the GPU."""
+    D = 4096
+    rows = (1 << 31) // D + 130
+    op, nd = env.gpu_op, env.nd
+    X, Y = nd.empty((rows, D), env.ctx), nd.empty((rows, D), env.ctx)
+    if isinstance(X, int) or isinstance(Y, int):
+        pytest.skip("not enough device memory")
+    op.array_set(Y, 1.0, env.stream)
+    op.dropout_forward(Y, X, "NCHW", 0.5, 3, op.get_input_descriptor((rows, D), "NCHW"), env.cudnn, env.stream)
+    rng = np.random.RandomState(0)
+    gamma, beta = (1 + 0.1 * rng.randn(D)).astype(np.float32), rng.randn(D).astype(np.float32)
+    G, B, DG, DB = nd.array(gamma, env.ctx), nd.array(beta, env.ctx), nd.empty((D,), env.ctx), nd.empty((D,), env.ctx)
+    last = slice((rows - 3) * D, rows * D)
+    x = view(env, X, last.start, (3, D)).asnumpy()
+    op.layer_norm_forward(X, G, B, Y, EPS, env.stream)
+    y, bound = forward(x, gamma, beta)[:2]
+    within(view(env, Y, last.start, (3, D)).asnumpy(), y, bound, "y")
+    # backward in place of y: the gradient is x itself
+    assert op.layer_norm_backward(X, G, X, Y, DG, DB, EPS, env.stream) == 0
+    (dx, _, _), (bx, _, _) = backward(x, gamma, x)
+    within(view(env, Y, last.start, (3, D)).asnumpy(), dx, bx, "dx")
+    # dbeta is the sum of x: twice the count of kept elements, exact in fp32 up to 2^24
+    assert np.all(np.abs(DB.asnumpy() - rows) < 8 * np.sqrt(rows))
+    del X, Y
+    op.release_cached_memory()

@@ -100,6 +100,10 @@ void invalidate_all_versions();             // every tensor counts as rewritten 
 // writes (the kernel of write k clears the word write k+1 will use), so no clearing launch is needed.
 struct AmaxOut { uint32_t* word = nullptr; uint32_t* clear = nullptr; };
 AmaxOut amax_track_begin(const void* data);
+// A graph that the caller captures replays the kernels and not what is kept on the host: a word that an earlier call left may be cleared or
+// belong to other data by then, and one that the graph fills is not cleared between replays.  Inside one, nothing is tracked or taken.
+bool stream_captured(cudaStream_t s);
+inline AmaxOut amax_track_begin_on(const void* data, cudaStream_t s) { return stream_captured(s) ? AmaxOut{} : amax_track_begin(data); }
 const uint32_t* amax_tracked(const void* data);
 // The maximum of a tensor that a recorded step reads before it writes it (see step_graph.cu): `carry` keeps the value
 // between replays, valid while the tensor's version is `*version`.
@@ -110,6 +114,9 @@ void amax_set_carry_valid(const void* data);
 void bump_versions(const void* const* ptrs, size_t n);
 #ifdef __CUDACC__
 __device__ __forceinline__ uint32_t amax_bits(float v) { return __float_as_uint(fabsf(v)); }
+// Of finite values only: an infinity or a NaN makes what reads it NaN whatever the scale, and the rows beside it keep their precision.
+__device__ __forceinline__ uint32_t finite_bits(float v) { const uint32_t b = amax_bits(v); return b < 0x7f800000u ? b : 0u; }
+__device__ __forceinline__ float finite_max(float m, float v) { v = fabsf(v); return v < __int_as_float(0x7f800000) ? fmaxf(m, v) : m; }
 // Every thread of the block calls this once, after its last store, with the largest bit pattern it produced.
 __device__ __forceinline__ void amax_commit(const AmaxOut& am, uint32_t m) {
   if (!am.word) return;                                  // uniform over the grid

@@ -148,7 +148,7 @@ template <int ACT> __global__ void __launch_bounds__(kThreads) gated_small_fwd_k
     if (p.gates) { p.gates[(long long)m * 2 * p.F + f] = gate; p.gates[(long long)m * 2 * p.F + p.F + f] = value; }
     value *= gate_value<ACT>(gate);
     p.out[(long long)m * p.F + f] = value;
-    top = max(top, amax_bits(value));
+    top = max(top, finite_bits(value));
   };
   if (ranks == 1) {
 #pragma unroll
@@ -313,7 +313,7 @@ int gated_small_fwd(const float* x, const float* w, float* gates, float* out, in
   const unsigned across = (unsigned)((F + kTile - 1) / kTile), down = (unsigned)((M + kTile - 1) / kTile);
   const int cluster = cluster_for((long long)across * down, (K + kDepth - 1) / kDepth, 3 * device_sm_count());
   p.per_cta = (int)(((K + cluster - 1) / cluster + kDepth - 1) / kDepth * kDepth);
-  p.am = amax_track_begin(out);
+  p.am = amax_track_begin_on(out, s);
   note_compute_stream(s);
   KernelTimer kt("gated_small_fwd", s, 4.0 * M * F * K, 0, 1);
   cudaError_t e = cudaSuccess;

@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kRowThreads) rows_gated_kernel(const RowsGated
       if (q.gates) { q.gates[(long long)m * 2 * q.F + c + j] = gate[j]; q.gates[(long long)m * 2 * q.F + q.F + c + j] = value[j]; }
       const float o = gate_value<ACT>(gate[j]) * value[j];
       q.out[(long long)m * q.F + c + j] = o;
-      top = max(top, amax_bits(o));
+      top = max(top, finite_bits(o));
     }
   }
   if (ranks > 1) cluster.sync();           // nobody leaves while its shared memory is still read
@@ -442,7 +442,7 @@ template <int MR> static int launch_rows_gated(RowsGated q, int activation, cuda
   while (cluster < 8 && (groups * cluster < 2 * sms || smem() > kRowSmem / 2) && p.K >= 64 * kRowWarps * cluster) { cluster *= 2; cut(); }
   if (smem() > kRowSmem || groups * cluster < sms) return 0;
   KernelTimer kt("rows_gated", s, 4.0 * (double)p.M * q.F * p.K, 0, 1);
-  q.am = amax_track_begin(q.out);
+  q.am = amax_track_begin_on(q.out, s);
   cudaError_t e = cudaSuccess;
   with_gate(activation, [&](auto act) {
     constexpr int ACT = decltype(act)::value;

@@ -616,7 +616,7 @@ template <int ACT> __device__ __forceinline__ uint32_t gate_run(const float* g, 
 #pragma unroll
   for (int q = 0; q < 32; ++q) {
     v[q] *= gate_value<ACT>(g[q]);
-    top = max(top, amax_bits(v[q]));
+    top = max(top, finite_bits(v[q]));
   }
   return top;
 }
@@ -1806,7 +1806,7 @@ __global__ void __launch_bounds__(256) reduce_gated_kernel(const __grid_constant
     }
     v *= a;
     p.out[(long long)m * F + f + q] = v;
-    top = max(top, amax_bits(v));
+    top = max(top, finite_bits(v));
   }
   if (!p.amax) return;
   top = __reduce_max_sync(0xffffffffu, top);
@@ -2002,7 +2002,7 @@ template <int ACT, int N> __device__ __forceinline__ uint32_t gradient_max(const
     float dg[N], dv[N];
     gate_gradient<ACT, N>(o, r, (int)(i - r * groups) * N, dg, dv);
 #pragma unroll
-    for (int q = 0; q < N; ++q) top = max(top, max(amax_bits(dg[q]), amax_bits(dv[q])));
+    for (int q = 0; q < N; ++q) top = max(top, max(finite_bits(dg[q]), finite_bits(dv[q])));
   }
   return top;
 }
@@ -2019,7 +2019,7 @@ template <int ACT> __global__ void __launch_bounds__(256) operand_max_kernel(con
     long long done = 0;
     if ((reinterpret_cast<uintptr_t>(o.src) & 15) == 0) {
       const float4* const s4 = reinterpret_cast<const float4*>(o.src);
-      auto fold = [&](float4 v) { top = max(max(top, amax_bits(v.x)), max(amax_bits(v.y), max(amax_bits(v.z), amax_bits(v.w)))); };
+      auto fold = [&](float4 v) { top = max(max(top, finite_bits(v.x)), max(finite_bits(v.y), max(finite_bits(v.z), finite_bits(v.w)))); };
       long long i = first;
       for (; i + 3 * stride < n / 4; i += 4 * stride) {       // four independent 16-byte loads in flight per thread
         const float4 a = __ldg(s4 + i), b = __ldg(s4 + i + stride), c = __ldg(s4 + i + 2 * stride), d = __ldg(s4 + i + 3 * stride);
@@ -2028,7 +2028,7 @@ template <int ACT> __global__ void __launch_bounds__(256) operand_max_kernel(con
       for (; i < n / 4; i += stride) fold(__ldg(s4 + i));
       done = n / 4 * 4;
     }
-    for (long long k = done + first; k < n; k += stride) top = max(top, amax_bits(__ldg(o.src + k)));
+    for (long long k = done + first; k < n; k += stride) top = max(top, finite_bits(__ldg(o.src + k)));
   }
   top = __reduce_max_sync(0xffffffffu, top);
   if ((threadIdx.x & 31) == 0 && top) atomicMax(o.max, top);
@@ -2607,6 +2607,7 @@ static bool capturing(cudaStream_t s) {
   cudaGetLastError();
   return true;
 }
+bool stream_captured(cudaStream_t s) { return !t_recording && capturing(s); }
 // The call may wait: its caller says so, nothing that waits was called on another stream, and no graph of the caller's own is being
 // captured (it would copy from a table that is gone).  True: the caller holds it now.
 bool may_hold(cudaStream_t s) {
@@ -2917,7 +2918,7 @@ static ScaleRef begin_pack(Pack& pk, const float* src, long long n, cudaStream_t
   r.amax_cur = bound ? bound : fresh;
   if (bound) return r;
   static const bool no_track = getenv("TINYFLOW_NO_AMAX_TRACKING") != nullptr;
-  if (const uint32_t* tracked = no_track ? nullptr : amax_tracked(src)) {
+  if (const uint32_t* tracked = no_track || stream_captured(s) ? nullptr : amax_tracked(src)) {
     r.amax_cur = tracked;               // the producer of src already reduced max|src| in its own pass
     return r;
   }
@@ -3043,12 +3044,13 @@ struct OperandPacks {
   }
   template <int ACT> int run(StreamLease& lease, cudaStream_t s, const char* what) {
     static const bool no_track = getenv("TINYFLOW_NO_AMAX_TRACKING") != nullptr;
+    const bool captured = stream_captured(s);
     bool reduce = false;
     double bytes = 0;
     if (ar == kArithF16) {
       for (int i = 0; i < all.n; ++i) {
         Operand& o = all.op[i];
-        if (o.kind != kGradient && !no_track && (o.scale.amax_cur = amax_tracked(o.src))) continue;         // its producer reduced it
+        if (o.kind != kGradient && !no_track && !captured && (o.scale.amax_cur = amax_tracked(o.src))) continue;         // its producer reduced it
         if (!all.words && !(all.words = lease.counters(4))) return 1;
         o.scale.amax_cur = o.max = all.words + i;
         reduce = true;
@@ -3097,7 +3099,7 @@ int tc_gated_fwd(const float* x, const float* w, float* gates, float* out, int64
   p.M = (int)M; p.N = (int)cols; p.m_tiles = (int)((M + BM - 1) / BM); p.n_tiles = (int)((cols + 127) / 128); p.tap_tiles = 1;
   p.k_total = (int)((K + bk - 1) / bk);
   p.out = out; p.gates = gates; p.gated_f = (int)F; p.activation = activation; p.err = error_word(); p.band = band_of(p);
-  const AmaxOut am = amax_track_begin(out);
+  const AmaxOut am = amax_track_begin_on(out, s);
   p.amax = am.word; p.amax_clear = am.clear;
   rc = ar == kArithTF32 ? launch_gated<kArithTF32>(p, s, 4.0 * M * F * K, what, nullptr) : launch_gated<kArithF16>(p, s, 4.0 * M * F * K, what, nullptr);
   return rc < 0 ? -1 : (rc > 0 ? 0 : 1);

@@ -43,7 +43,7 @@ __global__ void __launch_bounds__(kThreads) gate_kernel(const float* __restrict_
       get<VEC>(g, zr + c);
       get<VEC>(v, zr + F + c);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) { v[j] *= gate_value<ACT>(g[j]); m = max(m, amax_bits(v[j])); }
+      for (int j = 0; j < VEC; ++j) { v[j] *= gate_value<ACT>(g[j]); m = max(m, finite_bits(v[j])); }
       put<VEC>(out + row * F + c, v);
     }
   }
@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(kThreads) gate_gradient_kernel(const float* __
         gate_slope<ACT>(g[j], value, slope);
         g[j] = d[j] * v[j] * slope;
         v[j] = d[j] * value;
-        m = max(m, max(amax_bits(g[j]), amax_bits(v[j])));
+        m = max(m, max(finite_bits(g[j]), finite_bits(v[j])));
       }
       put<VEC>(dz + at + c, g);
       put<VEC>(dz + at + F + c, v);
@@ -161,7 +161,7 @@ int TfGatedLinearForward(const DLArrayHandle input, const DLArrayHandle weight, 
   if (matmul_any((const float*)input->data, false, (const float*)weight->data, false, z, M, 2 * F, K, s, what)) return -1;
   note_compute_stream(s);
   KernelTimer kt(what, s, 0, 12.0 * M * F);
-  TF_CUDA(launch_gate(activation, z, out, M, (int)F, amax_track_begin(out), s));
+  TF_CUDA(launch_gate(activation, z, out, M, (int)F, amax_track_begin_on(out, s), s));
   TF_AFTER(s, what);
   return 0;
 }
@@ -200,7 +200,7 @@ int TfGatedLinearBackward(const DLArrayHandle input, const DLArrayHandle weight,
   note_write(dz);                        // scratch: whatever was known of an array at this address does not hold
   if (M && F) {
     KernelTimer kt(what, s, 0, 20.0 * M * F);
-    TF_CUDA(launch_gate_gradient(activation, (const float*)gates->data, (const float*)doutput->data, dz, M, (int)F, amax_track_begin(dz), s));
+    TF_CUDA(launch_gate_gradient(activation, (const float*)gates->data, (const float*)doutput->data, dz, M, (int)F, amax_track_begin_on(dz, s), s));
     TF_AFTER(s, what);
   }
   if (dx && matmul_any(dz, false, (const float*)weight->data, true, dx, M, K, 2 * F, s, what)) return -1;

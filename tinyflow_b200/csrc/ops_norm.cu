@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(G * R) norm_fwd_kernel(const NormArgs a) {
           b[0] = fmaf(x[v] * inv.x, w[0], b[0]);
         }
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) m = fmaxf(m, fabsf(b[j]));
+        for (int j = 0; j < VEC; ++j) m = finite_max(m, b[j]);
         put<VEC>(a.y + base + r.at(v), b);
       }
     }
@@ -296,11 +296,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1) norm_bwd_kernel(const NormArgs
           put<VEC>(a.dx + base + v * G * VEC, d);
           if (!RES || !a.dbranch)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) m = fmaxf(m, fabsf(d[j]));
+            for (int j = 0; j < VEC; ++j) m = finite_max(m, d[j]);
         }
         if (RES && a.dbranch) {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) { d[j] = dropped(a, z + (v * G * VEC + j) * kMixStep, d[j]); m = fmaxf(m, fabsf(d[j])); }
+          for (int j = 0; j < VEC; ++j) { d[j] = dropped(a, z + (v * G * VEC + j) * kMixStep, d[j]); m = finite_max(m, d[j]); }
           put<VEC>(a.dbranch + base + v * G * VEC, d);
         }
       }
@@ -354,7 +354,7 @@ template <bool RES> __global__ void __launch_bounds__(kLongThreads) norm_long_fw
     for (int c = threadIdx.x; c < D; c += kLongThreads) {
       const float y = fmaf((x[c] - mean) * inv, a.gamma[c], a.beta[c]);
       a.y[base + c] = y;
-      m = max(m, amax_bits(y));
+      m = max(m, finite_bits(y));
     }
   }
   amax_commit(a.am, m);
@@ -389,9 +389,9 @@ template <bool RES> __global__ void __launch_bounds__(kLongThreads) norm_long_bw
       if (RES && a.dsum) d += a.dsum[row * D + c];
       if (a.dx) {
         a.dx[row * D + c] = d;
-        if (!RES || !a.dbranch) m = max(m, amax_bits(d));
+        if (!RES || !a.dbranch) m = max(m, finite_bits(d));
       }
-      if (RES && a.dbranch) { d = dropped(a, mix_start(seed, row * D + c), d); a.dbranch[row * D + c] = d; m = max(m, amax_bits(d)); }
+      if (RES && a.dbranch) { d = dropped(a, mix_start(seed, row * D + c), d); a.dbranch[row * D + c] = d; m = max(m, finite_bits(d)); }
     }
   }
   amax_commit(a.am, m);
@@ -572,7 +572,7 @@ int TfLayerNormForward(const DLArrayHandle input, const DLArrayHandle gamma, con
   cudaStream_t s = stream_of(cudaStream);
   a.x = (const float*)input->data; a.gamma = (const float*)gamma->data; a.beta = (const float*)beta->data; a.y = out_f32(output); a.eps = eps;
   if (numel(input) == 0) return 0;
-  a.am = amax_track_begin(a.y);
+  a.am = amax_track_begin_on(a.y, s);
   note_compute_stream(s);
   KernelTimer kt(what, s, 0, 8.0 * numel(input));
   TF_CUDA(launch_norm_fwd<false>(a, s));
@@ -595,7 +595,7 @@ int TfLayerNormBackward(const DLArrayHandle input, const DLArrayHandle gamma, co
   a.dx = opt_out(dinput);
   float *dg = opt_out(dgamma), *db = opt_out(dbeta);
   if (a.D == 0 || !(a.dx || dg || db)) return 0;
-  if (a.dx && a.rows) a.am = amax_track_begin(a.dx);
+  if (a.dx && a.rows) a.am = amax_track_begin_on(a.dx, s);
   note_compute_stream(s);
   KernelTimer kt(what, s, 0, 12.0 * numel(input));
   return run_norm_bwd<false>(a, dg, db, memorytoSaving, s, what);
@@ -630,7 +630,7 @@ int TfDropoutAddLayerNormForward(const DLArrayHandle input, const DLArrayHandle 
   st->recording = recording_id();
   set_dropout(a, st); a.seed_word = st->seed_word;
   if (n == 0) return 0;
-  if (a.y) a.am = amax_track_begin(a.y);
+  if (a.y) a.am = amax_track_begin_on(a.y, s);
   note_compute_stream(s);
   KernelTimer kt(what, s, 0, 16.0 * n);
   TF_CUDA(launch_norm_fwd<true>(a, s));
@@ -658,7 +658,7 @@ int TfDropoutAddLayerNormBackward(const DLArrayHandle sum, const DLArrayHandle g
   set_dropout(a, st);
   a.seed_word = st->recording && st->recording == recording_id() ? st->seed_word : nullptr;
   if (a.D == 0 || !(a.dx || a.dbranch || dg || db)) return 0;
-  if (a.rows && (a.dx || a.dbranch)) a.am = amax_track_begin(a.dbranch ? a.dbranch : a.dx);
+  if (a.rows && (a.dx || a.dbranch)) a.am = amax_track_begin_on(a.dbranch ? a.dbranch : a.dx, s);
   note_compute_stream(s);
   KernelTimer kt(what, s, 0, 20.0 * n);
   return run_norm_bwd<true>(a, dg, db, memorytoSaving, s, what);
