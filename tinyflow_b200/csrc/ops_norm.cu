@@ -97,6 +97,8 @@ template <int VEC, int G, int NV> struct Row {
   int D, t;
   __device__ __forceinline__ int at(int v) const { return (v * G + t) * VEC; }
   __device__ __forceinline__ bool has(int v) const { return v < NV - kStep || at(v) < D; }
+  // whether the row has any of the pair that piece v begins or ends: what has none is skipped, not computed on zeros
+  __device__ __forceinline__ bool begins(int v) const { return has(VEC == 1 ? v & ~1 : v); }
   // pair i of the thread's elements: v where the row has it, else 0 (a pair may lie in two pieces of one element)
   __device__ __forceinline__ float2 where(int i, float v) const {
     const int first = 2 * i / VEC, second = (2 * i + 1) / VEC;
@@ -159,8 +161,10 @@ __global__ void __launch_bounds__(G * R) norm_fwd_kernel(const NormArgs a) {
     float2 sq = both(0.f);
 #pragma unroll
     for (int i = 0; i < E / 2; ++i) {
-      pair(x, i) = __fadd2_rn(pair(x, i), r.where(i, -mean));
-      sq = __ffma2_rn(pair(x, i), pair(x, i), sq);
+      if (r.begins(2 * i / VEC)) {
+        pair(x, i) = __fadd2_rn(pair(x, i), r.where(i, -mean));
+        sq = __ffma2_rn(pair(x, i), pair(x, i), sq);
+      }
     }
     float squares[1] = {sq.x + sq.y};
     add(squares);
@@ -217,11 +221,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1) norm_bwd_kernel(const NormArgs
       const int64_t from = row * D + r.t * VEC;
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        const bool there = r.has(v);
-        const int64_t e = there ? from + v * G * VEC : 0;
-        copy_ahead<VEC * 4>(mine + stage + v * kPiece, a.x + e, there);
-        copy_ahead<VEC * 4>(mine + stage + (NV + v) * kPiece, a.dy + e, there);
-        if (with_sum) copy_ahead<VEC * 4>(mine + stage + (2 * NV + v) * kPiece, a.dsum + e, there);
+        if (r.begins(v)) {
+          const bool there = r.has(v);
+          const int64_t e = there ? from + v * G * VEC : 0;
+          copy_ahead<VEC * 4>(mine + stage + v * kPiece, a.x + e, there);
+          copy_ahead<VEC * 4>(mine + stage + (NV + v) * kPiece, a.dy + e, there);
+          if (with_sum) copy_ahead<VEC * 4>(mine + stage + (2 * NV + v) * kPiece, a.dsum + e, there);
+        }
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -254,9 +260,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1) norm_bwd_kernel(const NormArgs
     float x[E], dy[E], ds[RES ? E : 1];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      if (with_sum) fetched(ds + v * VEC, stage, 2 * NV + v);
-      fetched(dy + v * VEC, stage, NV + v);
-      fetched(x + v * VEC, stage, v);
+      if (r.begins(v)) {
+        if (with_sum) fetched(ds + v * VEC, stage, 2 * NV + v);
+        fetched(dy + v * VEC, stage, NV + v);
+        fetched(x + v * VEC, stage, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) x[v * VEC + j] = 0.f;
+      }
     }
     float sum[1] = {row_part(x)};
     add(sum);
@@ -264,11 +275,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1) norm_bwd_kernel(const NormArgs
     float2 sq = both(0.f), sg = both(0.f), sgx = both(0.f);      // (x - mean)^2, g, g * (x - mean)
 #pragma unroll
     for (int i = 0; i < E / 2; ++i) {
-      pair(x, i) = __fadd2_rn(pair(x, i), r.where(i, -mean));
-      const float2 g = __fmul2_rn(gammas(i), pair(dy, i));       // where the row has ended dy is zero
-      sq = __ffma2_rn(pair(x, i), pair(x, i), sq);
-      sg = __fadd2_rn(sg, g);
-      sgx = __ffma2_rn(g, pair(x, i), sgx);
+      if (r.begins(2 * i / VEC)) {
+        pair(x, i) = __fadd2_rn(pair(x, i), r.where(i, -mean));
+        const float2 g = __fmul2_rn(gammas(i), pair(dy, i));       // in a pair that the row ends in dy is zero
+        sq = __ffma2_rn(pair(x, i), pair(x, i), sq);
+        sg = __fadd2_rn(sg, g);
+        sgx = __ffma2_rn(g, pair(x, i), sgx);
+      }
     }
     float three[3] = {sq.x + sq.y, sg.x + sg.y, sgx.x + sgx.y};
     add(three);
@@ -282,11 +295,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1) norm_bwd_kernel(const NormArgs
     const unsigned long long z = RES ? mix_start(seed, base) : 0;
 #pragma unroll
     for (int i = 0; i < E / 2; ++i) {
-      const float2 g = __fmul2_rn(gammas(i), pair(dy, i));
-      pair(dgamma, i) = __ffma2_rn(__fmul2_rn(pair(dy, i), inv2), pair(x, i), pair(dgamma, i));
-      pair(dbeta, i) = __fadd2_rn(pair(dbeta, i), pair(dy, i));
-      pair(x, i) = __ffma2_rn(g, inv2, __ffma2_rn(pair(x, i), slope, shift));
-      if (with_sum) pair(x, i) = __fadd2_rn(pair(x, i), pair(ds, i));
+      if (r.begins(2 * i / VEC)) {
+        const float2 g = __fmul2_rn(gammas(i), pair(dy, i));
+        pair(dgamma, i) = __ffma2_rn(__fmul2_rn(pair(dy, i), inv2), pair(x, i), pair(dgamma, i));
+        pair(dbeta, i) = __fadd2_rn(pair(dbeta, i), pair(dy, i));
+        pair(x, i) = __ffma2_rn(g, inv2, __ffma2_rn(pair(x, i), slope, shift));
+        if (with_sum) pair(x, i) = __fadd2_rn(pair(x, i), pair(ds, i));
+      }
     }
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
