@@ -53,6 +53,10 @@ template <int G> struct RowSum {
   static constexpr int kWarps = G / 32;
   float (*held)[2][3][kWarps];
   int group, turn = 0;
+  __device__ __forceinline__ void barrier() const {
+    if (G == 32) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(G) : "memory");
+  }
   template <int N> __device__ __forceinline__ void operator()(float (&v)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -64,7 +68,7 @@ template <int G> struct RowSum {
 #pragma unroll
       for (int i = 0; i < N; ++i) held[group][turn][i][w] = v[i];
     }
-    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(G) : "memory");
+    barrier();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       v[i] = held[group][turn][i][0];
@@ -190,51 +194,62 @@ __global__ void __launch_bounds__(G * R) norm_fwd_kernel(const NormArgs a) {
   amax_commit(a.am, __float_as_uint(m));
 }
 
-// A copy of this thread's own, or zeros
-template <int BYTES> __device__ __forceinline__ void copy_ahead(uint32_t to, const float* from, bool there) {
-  const int bytes = there ? BYTES : 0;
-  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES), "r"(bytes) : "memory");
+template <int BYTES> __device__ __forceinline__ void copy_ahead(uint32_t to, const float* from) {
+  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
 }
 
 // Persistent: blockDim / G groups, each taking every (grid * groups)-th row, so a thread always has the same columns and keeps their
 // parts of dgamma and dbeta in registers; the groups' parts are added in group order and left as one row of `part` per block.
-// A thread copies its elements of the rows ahead of the present one to shared memory itself (`depth` of them in flight), and nobody
-// else reads them: the copies need no barrier.
+// The rows ahead of the present one are copied to shared memory, `depth` of them in flight.  A thread copies what it will read itself, and
+// the copies need no barrier; but rows that only 4-byte accesses fit are copied in the 16-byte pieces that they lie in, which their
+// readers share (2000 x 4099: 41.0 us with copies of 4 bytes, 37.5 so; even widths are faster with copies of 8: 1000 x 2050 12.1 against 12.7).
 constexpr int kBwdThreads = 512;            // most threads of a block
-constexpr int kBwdSmem = 224 * 1024;
+constexpr int kBwdSmem = 225 * 1024;
+// bytes of a row in the ring: one that begins between boundaries takes a piece more
+template <int VEC, int G, int NV> constexpr uint32_t norm_pitch() { return G * NV * VEC * 4 + (VEC == 1 ? 32 : 0); }
 template <int VEC, int G, int NV, bool RES>
 __global__ void __launch_bounds__(kBwdThreads, 1) norm_bwd_kernel(const NormArgs a, int depth) {
   constexpr int kArrays = RES ? 3 : 2;
-  constexpr uint32_t kPiece = kBwdThreads * VEC * 4, kStage = kArrays * NV * kPiece;
+  constexpr uint32_t kPitch = norm_pitch<VEC, G, NV>(), kArray = kBwdThreads / G * kPitch, kStage = kArrays * kArray;      // bytes
   __shared__ float held[kBwdThreads / G][2][3][G / 32];
-  extern __shared__ __align__(16) float ring[];            // [depth][array][NV][kBwdThreads][VEC], then gamma; at the end the groups' sums [group][2 * D]
+  extern __shared__ __align__(16) float ring[];            // [depth][array][group][kPitch], then gamma; at the end the groups' sums [group][2 * D]
   float* const gamma = ring + depth * (kStage / 4);
   const int group = threadIdx.x / G, groups = blockDim.x / G, D = a.D;
   const Row<VEC, G, NV> r{D, (int)(threadIdx.x % G)};
   const float over_d = 1.f / (float)D;
   const bool with_sum = RES && a.dsum;
   const int64_t first = (int64_t)blockIdx.x * groups + group, stride = (int64_t)gridDim.x * groups;
-  const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * VEC * 4u;
+  const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring) + group * kPitch;
+  // elements from the 16-byte boundary in front of a row to it
+  auto shift_of = [&](const float* base, int64_t row) { return VEC > 1 ? 0 : (int)((reinterpret_cast<uintptr_t>(base) >> 2) + (uintptr_t)(row * D)) & 3; };
+  auto fetch_row = [&](const float* base, int64_t row, uint32_t to) {
+    const float* const from = base + row * D;
+    if (VEC > 1) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) if (r.has(v)) copy_ahead<VEC * 4>(to + r.at(v) * 4, from + r.at(v));
+    } else {
+      const int shift = shift_of(base, row), pieces = (shift + D + 3) / 4;
+      for (int i = r.t; i < pieces; i += G) {
+        const float* const piece = from - shift + 4 * i;
+        // a piece may hold the end of the row before and the start of the next, but nothing outside the array
+        if (piece >= base && piece + 4 <= base + a.rows * D) copy_ahead<16>(to + 16 * i, piece);
+        else
+          for (int j = 0; j < 4; ++j) if (piece + j >= from && piece + j < from + D) copy_ahead<4>(to + 16 * i + 4 * j, piece + j);
+      }
+    }
+  };
   auto fetch = [&](int64_t row, uint32_t stage) {          // `stage` in bytes
     if (row < a.rows) {
-      const int64_t from = row * D + r.t * VEC;
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        if (r.begins(v)) {
-          const bool there = r.has(v);
-          const int64_t e = there ? from + v * G * VEC : 0;
-          copy_ahead<VEC * 4>(mine + stage + v * kPiece, a.x + e, there);
-          copy_ahead<VEC * 4>(mine + stage + (NV + v) * kPiece, a.dy + e, there);
-          if (with_sum) copy_ahead<VEC * 4>(mine + stage + (2 * NV + v) * kPiece, a.dsum + e, there);
-        }
-      }
+      fetch_row(a.x, row, mine + stage);
+      fetch_row(a.dy, row, mine + stage + kArray);
+      if (with_sum) fetch_row(a.dsum, row, mine + stage + 2 * kArray);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  const char* const own = reinterpret_cast<const char*>(ring) + threadIdx.x * VEC * 4;
-  auto fetched = [&](float* to, uint32_t stage, int piece) {
-    *reinterpret_cast<typename Pieces<VEC>::T*>(to) = *reinterpret_cast<const typename Pieces<VEC>::T*>(own + stage + piece * kPiece);
+  const char* const own = reinterpret_cast<const char*>(ring) + group * kPitch;
+  auto fetched = [&](float* to, uint32_t stage, int array, int shift, int v) {
+    *reinterpret_cast<typename Pieces<VEC>::T*>(to) = *reinterpret_cast<const typename Pieces<VEC>::T*>(own + stage + array * kArray + (r.at(v) + shift) * 4);
   };
   // gamma of pair i of the thread's elements (what lies behind the last one meets zeros)
   auto gammas = [&](int i) -> float2 {
@@ -257,16 +272,19 @@ __global__ void __launch_bounds__(kBwdThreads, 1) norm_bwd_kernel(const NormArgs
     if (depth == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
     else if (depth == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
     else asm volatile("cp.async.wait_group 3;" ::: "memory");
+    if (VEC == 1) add.barrier();               // what the others of the group copied
     float x[E], dy[E], ds[RES ? E : 1];
+    const int shift_x = shift_of(a.x, row), shift_dy = shift_of(a.dy, row), shift_ds = RES ? shift_of(a.dsum, row) : 0;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      if (r.begins(v)) {
-        if (with_sum) fetched(ds + v * VEC, stage, 2 * NV + v);
-        fetched(dy + v * VEC, stage, NV + v);
-        fetched(x + v * VEC, stage, v);
+      if (r.has(v)) {
+        if (with_sum) fetched(ds + v * VEC, stage, 2, shift_ds, v);
+        fetched(dy + v * VEC, stage, 1, shift_dy, v);
+        fetched(x + v * VEC, stage, 0, shift_x, v);
       } else {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) x[v * VEC + j] = 0.f;
+        for (int j = 0; j < VEC; ++j) x[v * VEC + j] = dy[v * VEC + j] = 0.f;
+        if (RES) ds[v * VEC] = 0.f;
       }
     }
     float sum[1] = {row_part(x)};
@@ -285,7 +303,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) norm_bwd_kernel(const NormArgs
     }
     float three[3] = {sq.x + sq.y, sg.x + sg.y, sgx.x + sgx.y};
     add(three);
-    fetch(row + depth * stride, stage);        // what was there has been read: three depends on the last of it
+    fetch(row + depth * stride, stage);        // what was there has been read, by all: the sums had barriers, and depend on the last of it
     stage += kStage;
     if (stage == depth * kStage) stage = 0;
     const float inv = rsqrtf(fmaf(three[0], over_d, a.eps));
@@ -515,8 +533,8 @@ template <bool RES> static int run_norm_bwd(NormArgs a, float* dgamma, float* db
       blocks = (int)std::min<int64_t>((a.rows + groups - 1) / groups, sms);
       const size_t bytes = sizeof(float) * 2 * (size_t)a.D * blocks;
       if (sums && blocks && !(a.part = (float*)lease.scratch(kScratchNorm, bytes))) { out_of_memory = 1; shortage(bytes); return; }
-      const int stage = kBwdThreads * NV * VEC * (int)sizeof(float) * (RES ? 3 : 2), depth = std::min(4, (kBwdSmem - G * NV * VEC * (int)sizeof(float)) / stage);
-      static_assert(kBwdThreads * NV * VEC * 4 * 3 * 2 + G * NV * VEC * 4 <= kBwdSmem, "two rows ahead and gamma always fit");
+      const int stage = kBwdThreads / G * (int)norm_pitch<VEC, G, NV>() * (RES ? 3 : 2), depth = std::min(4, (kBwdSmem - G * NV * VEC * (int)sizeof(float)) / stage);
+      static_assert(kBwdThreads / G * norm_pitch<VEC, G, NV>() * 3 * 2 + G * NV * VEC * 4 <= kBwdSmem, "two rows ahead and gamma always fit");
       static const cudaError_t attr = cudaFuncSetAttribute(norm_bwd_kernel<VEC, G, NV, RES>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBwdSmem);
       e = attr;
       if (blocks && e == cudaSuccess)
