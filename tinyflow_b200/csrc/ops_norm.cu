@@ -12,8 +12,11 @@
 #include <math.h>
 #include <algorithm>
 #include <initializer_list>
+#include <cooperative_groups.h>
 #include <type_traits>
 #include "operands.h"
+
+namespace cg = cooperative_groups;
 
 namespace tf {
 
@@ -29,6 +32,7 @@ struct NormArgs {
   float* dx;                 // may be null
   float* dbranch;            // may be null
   float* part;               // [block][2 * D] sums of dy * xh and of dy, or null
+  float *dgamma, *dbeta;     // where a grid of one cluster leaves them itself (either may be null)
   float2* stats;             // per row: mean and inv (rows that do not fit the registers)
   int64_t rows;
   int D;
@@ -205,6 +209,7 @@ template <int BYTES> __device__ __forceinline__ void copy_ahead(uint32_t to, con
 // the copies need no barrier; but rows that only 4-byte accesses fit are copied in the 16-byte pieces that they lie in, which their
 // readers share (2000 x 4099: 41.0 us with copies of 4 bytes, 37.5 so; even widths are faster with copies of 8: 1000 x 2050 12.1 against 12.7).
 constexpr int kBwdThreads = 512;            // most threads of a block
+constexpr int kFewBlocks = 8;
 constexpr int kBwdSmem = 225 * 1024;
 // bytes of a row in the ring: one that begins between boundaries takes a piece more
 template <int VEC, int G, int NV> constexpr uint32_t norm_pitch() { return G * NV * VEC * 4 + (VEC == 1 ? 32 : 0); }
@@ -341,7 +346,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) norm_bwd_kernel(const NormArgs
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   amax_commit(a.am, __float_as_uint(m));
-  if (!a.part) return;
+  const bool direct = a.dgamma || a.dbeta;
+  if (!a.part && !direct) return;
   __syncthreads();
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
@@ -351,12 +357,28 @@ __global__ void __launch_bounds__(kBwdThreads, 1) norm_bwd_kernel(const NormArgs
     }
   }
   __syncthreads();
-  float* const out = a.part + (int64_t)blockIdx.x * 2 * D;
+  float* const out = direct ? ring : a.part + (int64_t)blockIdx.x * 2 * D;
   for (int c = threadIdx.x; c < 2 * D; c += blockDim.x) {
     float total = ring[c];
     for (int g = 1; g < groups; ++g) total += ring[(size_t)g * 2 * D + c];
     out[c] = total;
   }
+  if (!direct) return;
+  // few rows: the grid is one cluster, and its blocks add a share of the columns each
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = (int)cluster.num_blocks();
+  cluster.sync();
+  for (int c = (int)cluster.block_rank() * blockDim.x + threadIdx.x; c < 2 * D; c += ranks * blockDim.x) {
+    float v[kFewBlocks];
+#pragma unroll
+    for (int k = 0; k < kFewBlocks; ++k) v[k] = cluster.map_shared_rank(ring, min(k, ranks - 1))[c];
+    float total = v[0];
+#pragma unroll
+    for (int k = 1; k < kFewBlocks; ++k) if (k < ranks) total += v[k];
+    if (c < D) { if (a.dgamma) a.dgamma[c] = total; }
+    else if (a.dbeta) a.dbeta[c - D] = total;
+  }
+  cluster.sync();              // nobody leaves while its shared memory is still read
 }
 
 // Rows of any length, a block each: three passes over the row, which L1 and L2 hold from the second on.
@@ -523,22 +545,28 @@ template <bool RES> static int run_norm_bwd(NormArgs a, float* dgamma, float* db
   StreamLease lease(s);
   auto shortage = [&](size_t bytes) { if (memorytoSaving) *memorytoSaving = bytes > 0x7fffffffu ? 0x7fffffff : (int)bytes; return 0; };
   int blocks = 0, out_of_memory = 0;
+  bool few = false;
   cudaError_t e = cudaSuccess;
   auto run = [&](auto vec) {
     constexpr int VEC = decltype(vec)::value;
     return with_shape<VEC, kBwdThreads>(a.D, [&](auto g, auto, auto nv) {
       constexpr int G = decltype(g)::value, NV = decltype(nv)::value;
-      // one block per SM, with as many groups as there are rows for
-      const int sms = device_sm_count(), groups = (int)std::max<int64_t>(1, std::min<int64_t>(kBwdThreads / G, (a.rows + sms - 1) / sms)), threads = groups * G;
-      blocks = (int)std::min<int64_t>((a.rows + groups - 1) / groups, sms);
-      const size_t bytes = sizeof(float) * 2 * (size_t)a.D * blocks;
-      if (sums && blocks && !(a.part = (float*)lease.scratch(kScratchNorm, bytes))) { out_of_memory = 1; shortage(bytes); return; }
-      const int stage = kBwdThreads / G * (int)norm_pitch<VEC, G, NV>() * (RES ? 3 : 2), depth = std::min(4, (kBwdSmem - G * NV * VEC * (int)sizeof(float)) / stage);
-      static_assert(kBwdThreads / G * norm_pitch<VEC, G, NV>() * 3 * 2 + G * NV * VEC * 4 <= kBwdSmem, "two rows ahead and gamma always fit");
+      constexpr int kMost = kBwdThreads / G;           // groups of a block
+      const int sms = device_sm_count(), stage = kMost * (int)norm_pitch<VEC, G, NV>() * (RES ? 3 : 2), depth = std::min(4, (kBwdSmem - G * NV * VEC * (int)sizeof(float)) / stage);
+      static_assert(kMost * norm_pitch<VEC, G, NV>() * 3 * 2 + G * NV * VEC * 4 <= kBwdSmem, "two rows ahead and gamma always fit");
+      // Up to two rows a group in one cluster: the sums of its blocks go through shared memory, and there is no second launch (64 x 256: 7.1 us, TIMES).
+      // Else one block per SM, with as many groups as there are rows for.
+      few = sums && a.rows > 0 && a.rows <= 2 * kFewBlocks * kMost;
+      const int groups = few ? (int)std::min<int64_t>(kMost, (a.rows + kFewBlocks - 1) / kFewBlocks) : (int)std::max<int64_t>(1, std::min<int64_t>(kMost, (a.rows + sms - 1) / sms));
+      blocks = (int)std::min<int64_t>((a.rows + groups - 1) / groups, few ? kFewBlocks : sms);
+      const size_t bytes = sizeof(float) * 2 * (size_t)a.D * blocks, smem = (size_t)stage * depth + sizeof(float) * G * NV * VEC;
+      if (few) { a.dgamma = dgamma; a.dbeta = dbeta; }
+      else if (sums && blocks && !(a.part = (float*)lease.scratch(kScratchNorm, bytes))) { out_of_memory = 1; shortage(bytes); return; }
       static const cudaError_t attr = cudaFuncSetAttribute(norm_bwd_kernel<VEC, G, NV, RES>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBwdSmem);
       e = attr;
-      if (blocks && e == cudaSuccess)
-        e = launch_dep(norm_bwd_kernel<VEC, G, NV, RES>, dim3(blocks), dim3(threads), (size_t)stage * depth + sizeof(float) * G * NV * VEC, s, a, depth);
+      if (!blocks || e != cudaSuccess) return;
+      if (few) e = launch_cluster(norm_bwd_kernel<VEC, G, NV, RES>, blocks, dim3(blocks), dim3(groups * G), smem, s, a, depth);
+      else e = launch_dep(norm_bwd_kernel<VEC, G, NV, RES>, dim3(blocks), dim3(groups * G), smem, s, a, depth);
     });
   };
   if (!with_width(a.D, {a.x, a.gamma, a.dy, a.dsum, a.dx, a.dbranch}, run)) {
@@ -561,7 +589,7 @@ template <bool RES> static int run_norm_bwd(NormArgs a, float* dgamma, float* db
   if (out_of_memory) return 0;
   TF_CUDA(e);
   TF_AFTER(s, what);
-  if (sums) {
+  if (sums && !few) {
     TF_CUDA(launch_dep(norm_params_kernel, dim3((unsigned)((2ll * a.D + 31) / 32)), dim3(1024), 0, s, (const float*)a.part, dgamma, dbeta, blocks, a.D));
     TF_AFTER(s, what);
   }

@@ -222,9 +222,9 @@ def convolution_2d_forward_get_out_shape(input_shapes, filter_shapes, dataformat
 
 
 def _with_short(fn, *args):
-    short = _short_cell()
-    check_call(fn(*args[:-1], short, args[-1]))
-    return _LIB.getInt(short)
+    short = ctypes.c_int(0)
+    check_call(fn(*args[:-1], ctypes.byref(short), args[-1]))
+    return short.value
 
 
 def convolution_2d_forward(in_arr, in_filter, out_arr, cudnnlist, cudnnHandle, cudaStream):
