@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kRowThreads) rows_gated_kernel(const RowsGated
     float4 now[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) now[j] = w[j];
-    if (k + 8 < k1) fetch(k + 8);
+    if (MR < 16 && k + 8 < k1) fetch(k + 8);
 #pragma unroll
     for (int m = 0; m < MR; ++m) {
       const float4 x0 = *reinterpret_cast<const float4*>(rows_smem + m * seg + k), x1 = *reinterpret_cast<const float4*>(rows_smem + m * seg + k + 4);
@@ -263,6 +263,7 @@ __global__ void __launch_bounds__(kRowThreads) rows_gated_kernel(const RowsGated
         acc[m][1] = __ffma2_rn(xx, make_float2(now[j].z, now[j].w), acc[m][1]);
       }
     }
+    if (MR >= 16 && k + 8 < k1) fetch(k + 8);              // (two sets of weights beside 16 rows of sums take the registers of a second block)
   }
   __syncthreads();                       // the rows are done with
   float4* const part = reinterpret_cast<float4*>(rows_smem);               // [warp][MR][32 lanes]
@@ -304,12 +305,11 @@ __global__ void __launch_bounds__(kRowThreads) rows_gated_kernel(const RowsGated
 // (Four rows a warp halve those reads and take registers: the same time.)
 constexpr int kRowSet = 2;
 template <int MR>
-__global__ void __launch_bounds__(kRowThreads) rows_nt_kernel(const SimtGemm p) {
+__device__ __forceinline__ void rows_nt(const SimtGemm& p, int block) {
   constexpr int kSums = MR * kRowSet;
   __shared__ float part[kRowWarps][kSums];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, runs = (p.K + p.k_per_cta - 1) / p.k_per_cta;       // of K, neighbouring warps
-  grid_dep_sync();
-  const int set = ((int)blockIdx.x * kRowWarps + warp) / runs, run = warp % runs, n0 = set * kRowSet;
+  const int set = (block * kRowWarps + warp) / runs, run = warp % runs, n0 = set * kRowSet;
   const int kend = min(p.K, (run + 1) * p.k_per_cta);
   float2 acc[kSums];
 #pragma unroll
@@ -333,10 +333,10 @@ __global__ void __launch_bounds__(kRowThreads) rows_nt_kernel(const SimtGemm p) 
 #pragma unroll
   for (int i = 0; i < kSums; ++i) sum[i] = acc[i].x + acc[i].y;
   // kSums sums over 32 lanes: a step adds pairs of lanes and halves what each keeps, lane i ends up with sum i
-  if (kSums == 16) {
 #pragma unroll
-    for (int i = 0; i < kSums; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 16);
-  }
+  for (int o = 16; o >= kSums; o /= 2)
+#pragma unroll
+    for (int i = 0; i < kSums; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
 #pragma unroll
   for (int step = kSums / 2; step > 0; step /= 2)
 #pragma unroll
@@ -357,9 +357,8 @@ __global__ void __launch_bounds__(kRowThreads) rows_nt_kernel(const SimtGemm p) 
 // C = A[K x M]^T B[K x N] of at most KR rows: a thread keeps its 4 columns of B and writes them times one row of A^T after the other.
 constexpr int kOuterRows = 32;
 template <int KR>
-__global__ void __launch_bounds__(kRowThreads) rows_tn_kernel(const SimtGemm p) {
-  grid_dep_sync();
-  const int n = ((int)blockIdx.x * kRowThreads + threadIdx.x) * 4, m0 = blockIdx.y * kOuterRows;
+__device__ __forceinline__ void rows_tn(const SimtGemm& p, int block_x, int block_y) {
+  const int n = (block_x * kRowThreads + (int)threadIdx.x) * 4, m0 = block_y * kOuterRows;
   if (n >= p.N) return;
   float4 b[KR];
 #pragma unroll
@@ -385,6 +384,24 @@ __global__ void __launch_bounds__(kRowThreads) rows_tn_kernel(const SimtGemm p) 
   }
 }
 
+template <int MR> __global__ void __launch_bounds__(kRowThreads) rows_nt_kernel(const SimtGemm p) {
+  grid_dep_sync();
+  rows_nt<MR>(p, blockIdx.x);
+}
+template <int KR> __global__ void __launch_bounds__(kRowThreads) rows_tn_kernel(const SimtGemm p) {
+  grid_dep_sync();
+  rows_tn<KR>(p, blockIdx.x, blockIdx.y);
+}
+// Both gradients of a gated layer on up to 8 rows, from dz: one reads the weights, one writes theirs, side by side (1 x 1024 x 4096 with dz: 22.1
+// us in two launches, TIMES; with 16 rows the registers of the one cost the other its blocks, 51 us apart and 58 together)
+struct RowsBoth { SimtGemm dx, dw; int dx_blocks, dw_across; };
+template <int MR> __global__ void __launch_bounds__(kRowThreads) rows_both_kernel(const RowsBoth q) {
+  grid_dep_sync();
+  const int b = (int)blockIdx.x - q.dx_blocks;
+  if (b < 0) rows_nt<MR>(q.dx, blockIdx.x);
+  else rows_tn<MR>(q.dw, b % q.dw_across, b / q.dw_across);
+}
+
 // Takes the product if it is one of those: 1, 0 if not, -1 on error.  Below a million weights, or where these leave SMs without a block
 // (2048 x 1000: 13.4 us against 9.3), the tiles are faster; rows that cannot be read 16 bytes at a time stay with them, too.
 constexpr int kFewRows = 16;
@@ -403,20 +420,27 @@ template <int MR> static int launch_rows_nn(SimtGemm p, cudaStream_t s) {
   TF_CUDA(launch_cluster(rows_nn_kernel<MR>, cluster, dim3(groups * cluster), dim3(kRowThreads), smem(), s, p));
   return 1;
 }
+// Cuts the rows of B into runs of K for the warps: blocks, 0: too few for every SM
+static long long rows_nt_blocks(SimtGemm& q) {
+  const int sms = device_sm_count();
+  const long long sets = (q.N + kRowSet - 1) / kRowSet;
+  int runs = 1;
+  while (runs < kRowWarps && sets * runs < 24ll * sms && q.K >= 256 * runs) runs *= 2;
+  if (sets * runs < 8ll * sms) return 0;
+  q.k_per_cta = (int)(((q.K + runs - 1) / runs + 127) / 128 * 128);
+  runs = (q.K + q.k_per_cta - 1) / q.k_per_cta;
+  while (kRowWarps % runs) { q.k_per_cta += 128; runs = (q.K + q.k_per_cta - 1) / q.k_per_cta; }       // whole sets in a block
+  return (sets * runs + kRowWarps - 1) / kRowWarps;
+}
 static int rows_matmul(const SimtGemm& p, bool tA, bool tB, cudaStream_t s) {
   const int sms = device_sm_count();
   if (!tA && p.M <= kFewRows && (double)p.K * p.N >= 1e6) {
     if (!tB && p.b_vec && p.N % 4 == 0) return p.M <= 8 ? launch_rows_nn<8>(p, s) : launch_rows_nn<16>(p, s);
     if (tB && p.a_vec && p.b_vec && p.K % 4 == 0) {
-      const long long sets = (p.N + kRowSet - 1) / kRowSet;
-      int runs = 1;
-      while (runs < kRowWarps && sets * runs < 24ll * sms && p.K >= 256 * runs) runs *= 2;
-      if (sets * runs < 8ll * sms) return 0;
       SimtGemm q = p;
-      q.k_per_cta = (int)(((p.K + runs - 1) / runs + 127) / 128 * 128);
-      runs = (p.K + q.k_per_cta - 1) / q.k_per_cta;
-      while (kRowWarps % runs) { q.k_per_cta += 128; runs = (p.K + q.k_per_cta - 1) / q.k_per_cta; }       // whole sets in a block
-      const dim3 grid((unsigned)((sets * runs + kRowWarps - 1) / kRowWarps));
+      const long long blocks = rows_nt_blocks(q);
+      if (!blocks) return 0;
+      const dim3 grid((unsigned)blocks);
       KernelTimer kt("rows_gemm", s, 2.0 * (double)p.M * p.N * p.K, 0, 1);
       TF_CUDA(p.M <= 8 ? launch_dep(rows_nt_kernel<8>, grid, dim3(kRowThreads), 0, s, q) : launch_dep(rows_nt_kernel<16>, grid, dim3(kRowThreads), 0, s, q));
       return 1;
@@ -459,6 +483,21 @@ int rows_gated(const float* x, const float* w, float* gates, float* out, int64_t
   RowsGated q{SimtGemm{x, w, nullptr, (int)M, (int)(2 * F), (int)K, K, 2 * F, 0, 0, 0, 1, 0}, gates, out, (int)F, AmaxOut{}};
   note_compute_stream(s);
   return M == 1 ? launch_rows_gated<1>(q, activation, s) : M <= 8 ? launch_rows_gated<8>(q, activation, s) : launch_rows_gated<16>(q, activation, s);
+}
+
+// dx = dz W^T and dW = x^T dz in one launch: 1 done, 0 not for these kernels, -1 error
+int rows_gated_bwd(const float* x, const float* w, const float* dz, float* dx, float* dw, int64_t M, int64_t F, int64_t K, cudaStream_t s) {
+  if (M < 1 || M > 8 || (double)K * 2 * F < 1e6 || F % 2 || K % 4 || !aligned16(x) || !aligned16(w) || !aligned16(dz) || !aligned16(dw) || (K + kOuterRows - 1) / kOuterRows > 65535) return 0;
+  RowsBoth q{SimtGemm{dz, w, dx, (int)M, (int)K, (int)(2 * F), 2 * F, 2 * F, K, 0, 1, 1, 0}, SimtGemm{x, dz, dw, (int)K, (int)(2 * F), (int)M, K, 2 * F, 2 * F, 0, 1, 1, 1}, 0, 0};
+  q.dx_blocks = (int)rows_nt_blocks(q.dx);
+  if (!q.dx_blocks) return 0;
+  q.dw_across = (q.dw.N + 4 * kRowThreads - 1) / (4 * kRowThreads);
+  const dim3 grid((unsigned)(q.dx_blocks + q.dw_across * ((q.dw.M + kOuterRows - 1) / kOuterRows)));
+  note_compute_stream(s);
+  KernelTimer kt("rows_gated_bwd", s, 8.0 * (double)M * F * K, 0, 1);
+  TF_CUDA(M == 1 ? launch_dep(rows_both_kernel<1>, grid, dim3(kRowThreads), 0, s, q) : launch_dep(rows_both_kernel<8>, grid, dim3(kRowThreads), 0, s, q));
+  TF_AFTER(s, "rows_gated_bwd");
+  return 1;
 }
 
 static thread_local std::vector<SimtJob> t_held_simt;

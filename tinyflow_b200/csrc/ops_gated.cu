@@ -16,6 +16,7 @@ int matmul_any(const float* A, bool tA, const float* B, bool tB, float* C, int64
 int tc_gated_fwd(const float* x, const float* w, float* gates, float* out, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s, const char* what);
 int tc_gated_bwd(const float* x, const float* w, const float* z, const float* dout, float* dx, float* dw, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s, const char* what);
 int rows_gated(const float* x, const float* w, float* gates, float* out, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s);
+int rows_gated_bwd(const float* x, const float* w, const float* dz, float* dx, float* dw, int64_t M, int64_t F, int64_t K, cudaStream_t s);
 int gated_small_fwd(const float* x, const float* w, float* gates, float* out, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s, const char* what);
 int gated_small_bwd(const float* x, const float* w, const float* z, const float* dout, float* dx, float* dw, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s, const char* what);
 void note_contraction_path(int path);
@@ -202,6 +203,9 @@ int TfGatedLinearBackward(const DLArrayHandle input, const DLArrayHandle weight,
     KernelTimer kt(what, s, 0, 20.0 * M * F);
     TF_CUDA(launch_gate_gradient(activation, (const float*)gates->data, (const float*)doutput->data, dz, M, (int)F, amax_track_begin_on(dz, s), s));
     TF_AFTER(s, what);
+  }
+  if (dx && dw && contraction_path() != 2) {
+    if (const int r = rows_gated_bwd((const float*)input->data, (const float*)weight->data, dz, dx, dw, M, F, K, s)) { note_contraction_path(1); note_write(dz); return r < 0 ? -1 : 0; }
   }
   if (dx && matmul_any(dz, false, (const float*)weight->data, true, dx, M, K, 2 * F, s, what)) return -1;
   if (dw && matmul_any((const float*)input->data, true, dz, false, dw, K, 2 * F, M, s, what)) return -1;
