@@ -4,7 +4,7 @@
 // kernel computes the gate columns and the value columns that they meet in the same block and finishes them; the backward kernel holds the
 // tiles of dx and of dW, and forms dz from the projections while it loads, once per tile that reads it.  Long reductions are cut over the
 // CTAs of a cluster and added in rank order through distributed shared memory, as in the plain products.
-// 64 x 784 x 256, forward and backward: products and elementwise kernels one by one 30 us, so TIMES.
+// 64 x 784 x 256, forward and backward: products and elementwise kernels one by one 30 us, so 19.6.
 #include "common.h"
 #include <algorithm>
 #include <type_traits>
@@ -24,6 +24,9 @@ struct Small {
   float *gates, *out, *dx, *dw;
   int M, K, F;
   int per_cta;              // of the reduction that is cut (forward: K, a multiple of 32; dx: F, a multiple of 16)
+  int rows_per_cta;         // dW: of the batch, a multiple of 32
+  int dx_ranks, dw_ranks;   // CTAs of a cluster that share a tile: 1 up to its size
+  int dx_clusters;          // the first so many, the others are dW's
   int x_vec, w_vec, z_vec;  // 16-byte accesses allowed
   int dx_tiles, dw_tiles, dx_across, dw_across;
   AmaxOut am;
@@ -41,6 +44,34 @@ __device__ __forceinline__ void multiply(const Block& a, const Block& b, int ty,
     acc[2][0] = fmaf(r.z, c.x, acc[2][0]); acc[2][1] = fmaf(r.z, c.y, acc[2][1]);
     acc[3][0] = fmaf(r.w, c.x, acc[3][0]); acc[3][1] = fmaf(r.w, c.y, acc[3][1]);
   }
+}
+// Stores a tile: straight from the registers, or the sum over `ranks` CTAs of the cluster from `first` on, in order, each a slice of it
+template <class Store> __device__ __forceinline__ void finish_tile(int ranks, int first, float* part, const float (&acc)[4][2], int ty, int tx, Store&& store) {
+  if (ranks == 1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) store(ty * 4 + i, tx * 2 + j, acc[i][j]);
+    return;
+  }
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank() - first;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) part[(ty * 4 + i) * kTile + tx * 2 + j] = acc[i][j];
+  cluster.sync();
+  const int slice = (kTile * kTile + ranks - 1) / ranks, end = min(kTile * kTile, (rank + 1) * slice);
+  for (int e = rank * slice + threadIdx.x; e < end; e += kThreads) {
+    float a[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) a[r] = cluster.map_shared_rank(part, first + min(r, ranks - 1))[e];
+    float total = a[0];
+#pragma unroll
+    for (int r = 1; r < 8; ++r) if (r < ranks) total += a[r];
+    store(e / kTile, e % kTile, total);
+  }
+  cluster.sync();           // nobody leaves while its shared memory is still read
 }
 // four elements of a row from column c on, zeros from `cols` on
 __device__ __forceinline__ float4 four(const float* __restrict__ row, int c, int cols, bool vec) {
@@ -181,19 +212,26 @@ template <int ACT> __global__ void __launch_bounds__(kThreads) gated_small_fwd_k
   amax_commit(p.am, top);
 }
 
-// Clusters of `ranks`: the first dx_tiles of them a tile of dx each, cut over the cluster, the others `ranks` tiles of dW, one a CTA.
+// dx: cut over the columns; dW: cut over the rows of the batch where they are long and the weights few.
 // A step of 32 of the reduction is 16 columns of each half for dx, 32 rows for dW; a tile of dW is 32 rows x 16 columns of each half.
 constexpr int kLoads = 4;           // steps of dx whose loads are in flight at once
 template <int ACT> __global__ void __launch_bounds__(kThreads) gated_small_bwd_kernel(const Small p) {
   __shared__ __align__(16) Block as[2], bs[2];
   cg::cluster_group cluster = cg::this_cluster();
-  const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks(), id = (int)blockIdx.x / ranks;
+  const int size = (int)cluster.num_blocks(), at_rank = (int)cluster.block_rank(), id = (int)blockIdx.x / size;
   grid_dep_sync();
+  const bool for_dx = id < p.dx_clusters;
+  const int ranks = for_dx ? p.dx_ranks : p.dw_ranks, rank = at_rank % ranks, first = at_rank - rank;
+  const int tile = (for_dx ? id : id - p.dx_clusters) * (size / ranks) + at_rank / ranks;
+  if (tile >= (for_dx ? p.dx_tiles : p.dw_tiles)) {
+    if (ranks > 1) { cluster.sync(); cluster.sync(); }             // those of the tiles that are cut
+    return;
+  }
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16, line = threadIdx.x / 4, quad = threadIdx.x % 4 * 4;
   float acc[4][2] = {};
   GateGradient<ACT> dz[kLoads];
-  if (id < p.dx_tiles) {
-    const int m0 = id / p.dx_across * kTile, n0 = id % p.dx_across * kTile, fbeg = rank * p.per_cta, fend = min(p.F, fbeg + p.per_cta);
+  if (for_dx) {
+    const int m0 = tile / p.dx_across * kTile, n0 = tile % p.dx_across * kTile, fbeg = rank * p.per_cta, fend = min(p.F, fbeg + p.per_cta);
     float4 wg[kLoads], wv[kLoads];
     auto fetch = [&](int f, int at) {
       dz[at].fetch(p, f < fend ? m0 + line : p.M, f + quad);
@@ -227,43 +265,17 @@ template <int ACT> __global__ void __launch_bounds__(kThreads) gated_small_bwd_k
       }
       __syncthreads();
     }
-    if (ranks == 1) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int m = m0 + ty * 4 + i, n = n0 + tx * 2 + j;
-          if (m < p.M && n < p.K) p.dx[(long long)m * p.K + n] = acc[i][j];
-        }
-      return;
-    }
-    float* const part = &as[0][0][0];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) part[(ty * 4 + i) * kTile + tx * 2 + j] = acc[i][j];
-    cluster.sync();
-    const int slice = (kTile * kTile + ranks - 1) / ranks, end = min(kTile * kTile, (rank + 1) * slice);
-    for (int e = rank * slice + threadIdx.x; e < end; e += kThreads) {
-      float a[8];
-#pragma unroll
-      for (int r = 0; r < 8; ++r) a[r] = cluster.map_shared_rank(part, min(r, ranks - 1))[e];
-      float total = a[0];
-#pragma unroll
-      for (int r = 1; r < 8; ++r) if (r < ranks) total += a[r];
-      const int m = m0 + e / kTile, n = n0 + e % kTile;
-      if (m < p.M && n < p.K) p.dx[(long long)m * p.K + n] = total;
-    }
-    cluster.sync();
+    finish_tile(ranks, first, &as[0][0][0], acc, ty, tx, [&](int row, int col, float v) {
+      if (m0 + row < p.M && n0 + col < p.K) p.dx[(long long)(m0 + row) * p.K + n0 + col] = v;
+    });
     return;
   }
-  const int tile = (id - p.dx_tiles) * ranks + rank;
-  if (tile >= p.dw_tiles) return;
   const int k0 = tile / p.dw_across * kTile, f0 = tile % p.dw_across * 16;
+  const int mbeg = rank * p.rows_per_cta, mend = min(p.M, mbeg + p.rows_per_cta);
   BlockLoader<kTile, kDepth, kThreads, false> lx[2];
   auto fetch = [&](int m, int at) {
-    lx[at].fetch(p.x, p.K, k0, p.K, m, p.M, p.x_vec);
-    dz[at].fetch(p, m + line, f0 + quad);
+    lx[at].fetch(p.x, p.K, k0, p.K, m, mend, p.x_vec);
+    dz[at].fetch(p, m + line < mend ? m + line : p.M, f0 + quad);
   };
   auto put = [&](int at) {
     float dg[4], dv[4];
@@ -272,11 +284,11 @@ template <int ACT> __global__ void __launch_bounds__(kThreads) gated_small_bwd_k
     *reinterpret_cast<float4*>(&bs[at][line][quad]) = make_float4(dg[0], dg[1], dg[2], dg[3]);
     *reinterpret_cast<float4*>(&bs[at][line][16 + quad]) = make_float4(dv[0], dv[1], dv[2], dv[3]);
   };
-  if (p.M > 0) { fetch(0, 0); fetch(kDepth, 1); }
-  for (int m = 0; m < p.M; m += 2 * kDepth) {
+  if (mbeg < mend) { fetch(mbeg, 0); fetch(mbeg + kDepth, 1); }
+  for (int m = mbeg; m < mend; m += 2 * kDepth) {
 #pragma unroll
     for (int at = 0; at < 2; ++at) {
-      if (m + at * kDepth < p.M) {               // the same for the whole block
+      if (m + at * kDepth < mend) {              // the same for the whole block
         put(at);
         __syncthreads();
         fetch(m + (at + 2) * kDepth, at);
@@ -284,16 +296,15 @@ template <int ACT> __global__ void __launch_bounds__(kThreads) gated_small_bwd_k
       }
     }
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int k = k0 + ty * 4 + i, c = tx * 2 + j, f = f0 + (c & 15);
-      if (k < p.K && f < p.F) p.dw[(long long)k * 2 * p.F + (c < 16 ? 0 : p.F) + f] = acc[i][j];
-    }
+  __syncthreads();
+  finish_tile(ranks, first, &as[0][0][0], acc, ty, tx, [&](int row, int col, float v) {
+    const int k = k0 + row, f = f0 + (col & 15);
+    if (k < p.K && f < p.F) p.dw[(long long)k * 2 * p.F + (col < 16 ? 0 : p.F) + f] = v;
+  });
 }
 
-// Blocks of 64 x 64 would leave SMs idle: above that the plain products with their larger tiles are faster
+// Blocks of 64 x 64 would leave SMs idle: above that the plain products with their larger tiles are faster (backward, where dz is formed again for
+// every tile: 100 x 2000 x 500 73 us against 52)
 bool small_product(int64_t M, int64_t N) { return ((M + 63) / 64) * ((N + 63) / 64) < device_sm_count(); }
 int cluster_for(long long tiles, long long steps, int want) {
   int c = 1;
@@ -305,7 +316,8 @@ int cluster_for(long long tiles, long long steps, int want) {
 
 // 1: done, 0: too large, -1: error
 int gated_small_fwd(const float* x, const float* w, float* gates, float* out, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s, const char* what) {
-  if (!small_product(M, 2 * F)) return 0;
+  if (2.0 * M * F * K > 5e8) return 0;               // 64 x 64 tiles of the plain products (8000 x 64 x 64: 8.3 us against 18.1; 512 x 512 x 512: 24.6 for both)
+  if (M > 65535ll * kTile) return 0;                 // the grid's rows
   Small p;
   memset(&p, 0, sizeof(p));
   p.x = x; p.w = w; p.gates = gates; p.out = out; p.M = (int)M; p.K = (int)K; p.F = (int)F;
@@ -319,9 +331,13 @@ int gated_small_fwd(const float* x, const float* w, float* gates, float* out, in
   cudaError_t e = cudaSuccess;
   with_gate(activation, [&](auto act) {
     constexpr int ACT = decltype(act)::value;
-    static const cudaError_t attr = cudaFuncSetAttribute(gated_small_fwd_kernel<ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(FwdStep) * kAhead);
+    static const cudaError_t attr = [] {
+      const cudaError_t set = cudaFuncSetAttribute(gated_small_fwd_kernel<ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(FwdStep) * kAhead);
+      return set != cudaSuccess ? set : cudaFuncSetAttribute(gated_small_fwd_kernel<ACT>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    }();
     e = attr;
-    if (e == cudaSuccess) e = launch_cluster(gated_small_fwd_kernel<ACT>, cluster, dim3(across * cluster, down), dim3(kThreads), sizeof(FwdStep) * kAhead, s, p);
+    if (e == cudaSuccess) e = cluster > 1 ? launch_cluster(gated_small_fwd_kernel<ACT>, cluster, dim3(across * cluster, down), dim3(kThreads), sizeof(FwdStep) * kAhead, s, p)
+                                          : launch_dep(gated_small_fwd_kernel<ACT>, dim3(across, down), dim3(kThreads), sizeof(FwdStep) * kAhead, s, p);
   });
   TF_CUDA(e);
   TF_AFTER(s, what);
@@ -329,7 +345,7 @@ int gated_small_fwd(const float* x, const float* w, float* gates, float* out, in
 }
 int gated_small_bwd(const float* x, const float* w, const float* z, const float* dout, float* dx, float* dw, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s,
                     const char* what) {
-  if ((dx && !small_product(M, K)) || (dw && !small_product(K, 2 * F))) return 0;
+  if (!small_product(M, K) || !small_product(K, 2 * F)) return 0;              // of both, so that one gradient alone has the bits that it has beside the other
   Small p;
   memset(&p, 0, sizeof(p));
   p.x = x; p.w = w; p.z = z; p.dout = dout; p.dx = dx; p.dw = dw; p.M = (int)M; p.K = (int)K; p.F = (int)F;
@@ -338,9 +354,14 @@ int gated_small_bwd(const float* x, const float* w, const float* z, const float*
   p.dw_across = (int)((F + 15) / 16);
   p.dx_tiles = dx ? p.dx_across * (int)((M + kTile - 1) / kTile) : 0;
   p.dw_tiles = dw ? p.dw_across * (int)((K + kTile - 1) / kTile) : 0;
-  const int cluster = dx ? cluster_for(p.dx_tiles, (F + 15) / 16, device_sm_count()) : 1;
-  p.per_cta = (int)(((F + cluster - 1) / cluster + 15) / 16 * 16);
-  const int clusters = p.dx_tiles + (p.dw_tiles + cluster - 1) / cluster;
+  const int sms = device_sm_count();
+  p.dx_ranks = dx ? cluster_for(p.dx_tiles, (F + 15) / 16, sms) : 1;
+  p.dw_ranks = dw ? cluster_for(p.dw_tiles, (M + kDepth - 1) / kDepth, sms) : 1;
+  p.per_cta = (int)(((F + p.dx_ranks - 1) / p.dx_ranks + 15) / 16 * 16);
+  p.rows_per_cta = (int)(((M + p.dw_ranks - 1) / p.dw_ranks + kDepth - 1) / kDepth * kDepth);
+  const int cluster = std::max(p.dx_ranks, p.dw_ranks), dx_each = cluster / p.dx_ranks, dw_each = cluster / p.dw_ranks;
+  p.dx_clusters = (p.dx_tiles + dx_each - 1) / dx_each;
+  const int clusters = p.dx_clusters + (p.dw_tiles + dw_each - 1) / dw_each;
   if (clusters == 0) return 1;
   note_compute_stream(s);
   KernelTimer kt("gated_small_bwd", s, 4.0 * M * F * K * ((dx != nullptr) + (dw != nullptr)), 0, 1);

@@ -586,7 +586,7 @@ template <int NC, int BLOCKS> __device__ __forceinline__ void load_sum(uint32_t 
 //
 // A thread holds a row, so stores straight from the registers go to 32 rows at once, 16 bytes each: 10 us for the 96 KB of a tile, and
 // the products wait from the third accumulator group of the next tile on (4736 x 512 x 16384: 318 us).  Through 4 KB of shared memory per
-// warp every store instruction writes four runs of 128 bytes instead (TIMES).
+// warp every store instruction writes four runs of 128 bytes instead (269 us).
 constexpr int kGatedStage = 8 * 32 * 32 * 4;
 // a warp's 32 rows x 32 columns, row `lane` in v -> rows of pitch `pitch` at `to`, of which `rows` x `cols` are there
 __device__ __forceinline__ void store_block(float* stage, const float* v, float* to, long long pitch, int rows, int cols, int lane) {
@@ -1952,7 +1952,7 @@ __global__ void __launch_bounds__(256) pack_matrix_kernel(const float* __restric
 }
 
 // ---- operands of gated layers: all of a call in one launch for their maxima and one for their packs ------------------------------
-// (a launch each and the clearing of their words made eleven of the gradients' call; 777 x 500 x 1003 forward 35.2 us, so TIMES)
+// (a launch each and the clearing of their words made eleven of the gradients' call; 777 x 500 x 1003 forward 35.4 us, so 25.1; gradients 76, so 60)
 // kRows: a matrix as it lies.  kWeight: [K][gate columns | value columns] of F each -> 32 gate columns, the 32 value columns that they meet,
 // and so on, zeros past F, so that one epilogue thread of the product has both.  kGradient: dz = [dout * value * act'(gate) | dout * act(gate)],
 // formed from the projections wherever it is wanted and never written as numbers of its own.
@@ -2987,12 +2987,13 @@ int tc_matmul(const float* A, bool tA, const float* B, bool tB, float* C, int64_
 }
 
 // ---- gated dense layers (ops_gated.cu) ----------------------------------------------------------------
-// Row tiles of a band: a wave then covers about as many row tiles as column tiles.  8192 x 2048 x 16384: TIMES
+// Row tiles of a band: a wave then covers about as many row tiles as column tiles.  8192 x 2048 x 16384: 1776 us without, 1491
+// with; 4096 x 4096 x 4096 429 and 411, 4096 x 1024 x 8192 206 and 210
 static int band_of(const GemmParams& p) {
   const int want = 12, bands = std::max(1, (p.m_tiles + want / 2) / want);
   return p.n_tiles > 4 && p.m_tiles * p.n_tiles > device_sm_count() ? (p.m_tiles + bands - 1) / bands : 0;       // (up to 4 column tiles B may stay in shared memory)
 }
-static bool tc_takes(double M, double N, double K) { return M >= 16 && N >= 16 && K >= 64 && M * N * K >= (contraction_path() == 2 ? 4e6 : 1.5e8); }
+static bool tc_takes(double M, double N, double K) { return M >= 16 && N >= 16 && K >= 16 && M * N * K >= 4e6; }          // whether it pays is the caller's to know
 static int gemm_maps(GemmParams& p, int ar, const Pack& pa, const Pack& pb, int bn) {
   int rc = p.a_mn ? make_map_mn(&p.a_hi, ar, pa.hi, pa.rows, pa.pitch, BM) : make_map(&p.a_hi, ar, pa.hi, pa.rows, pa.cols, pa.pitch, BM);
   if (!rc) rc = p.a_mn ? make_map_mn(&p.a_lo, ar, pa.lo, pa.rows, pa.pitch, BM) : make_map(&p.a_lo, ar, pa.lo, pa.rows, pa.cols, pa.pitch, BM);

@@ -5,7 +5,9 @@
 //
 // Both projections are one product of 2F columns, 4 MKF operations; the gradients are two products of dz, 8 MKF.
 #include "common.h"
+#include <math.h>
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 #include "gated.h"
 #include "operands.h"
@@ -101,6 +103,19 @@ cudaError_t launch_gate_gradient(int activation, const float* z, const float* do
   return e;
 }
 
+// Whether the tensor path is the shorter road, in us.  It costs a chain of launches and 12 bytes of traffic per operand element (gradients: 32 for
+// dz) before the first product; the CUDA-core kernels cost per multiply-add of one product, and for long reductions over few tiles a chain of steps.
+// Fitted to 40 shapes of 8 to 8000 rows and 8 to 4096 columns, tensor path against CUDA cores: 512 x 512 x 512 forward 19.9 against 24.7, backward
+// 33.9 against 68.7; 64 x 512 x 1024 19.1 against 9.2 and 26.5 against 24.6; 64 x 2048 x 1024 32.1 against 23.0 and 41.0 against 56.5; 32 x 2048 x 2048
+// 41.2 against 23.0 and 63.4 against 55.9; 4000 x 128 x 128 16.1 against 13.2 and 29.9 against 43.6.
+bool tensor_path_pays(double M, double F, double K, bool backward) {
+  const double work = 2.0 * M * F * K, elements = 1e-6 * (M * K + 2.0 * K * F);
+  if (!backward) return 15.0 + 0.004 * K + 2.4 * elements + 7e-9 * work < 3.5 + 7.7e-8 * work;
+  const double tiles_dx = std::ceil(M / 32) * std::ceil(K / 32), tiles_dw = std::ceil(K / 32) * std::ceil(F / 16), sms = device_sm_count();
+  const double chain = std::max(0.03 * M / std::min(8.0, std::max(1.0, sms / tiles_dw)), 0.05 * F / std::min(8.0, std::max(1.0, sms / tiles_dx)));
+  return 25.0 + 3.4 * elements + 6.4e-6 * M * F + 1.4e-8 * work < 5.0 + std::max((M <= 32 && work < 1.5e8 ? 1.85e-7 : 2.4e-7) * work, chain);
+}
+
 // Products of scratch are launched at once, whatever the caller holds back.
 struct NoHolding {
   const bool held;
@@ -145,14 +160,17 @@ int TfGatedLinearForward(const DLArrayHandle input, const DLArrayHandle weight, 
   float* z = gates ? out_f32(gates) : nullptr;
   if (M == 0 || F == 0) return 0;
   const NoHolding launched;
-  if (!contraction_path_is_cuda_cores()) {
+  if (contraction_path() == 0) {           // (up to 16 rows against large weights)
+    if (const int r = rows_gated((const float*)input->data, (const float*)weight->data, z, out, M, F, K, activation, s)) { note_contraction_path(1); return r < 0 ? -1 : 0; }
+  }
+  if (contraction_path() == 2 || (contraction_path() == 0 && tensor_path_pays((double)M, (double)F, (double)K, false))) {
     if (const int r = tc_gated_fwd((const float*)input->data, (const float*)weight->data, z, out, M, F, K, activation, s, what)) {
       note_contraction_path(2);
       return r < 0 ? -1 : 0;
     }
   }
   if (contraction_path() != 2) {
-    int r = rows_gated((const float*)input->data, (const float*)weight->data, z, out, M, F, K, activation, s);
+    int r = contraction_path() == 1 ? rows_gated((const float*)input->data, (const float*)weight->data, z, out, M, F, K, activation, s) : 0;
     if (!r) r = gated_small_fwd((const float*)input->data, (const float*)weight->data, z, out, M, F, K, activation, s, what);
     if (r) { note_contraction_path(1); return r < 0 ? -1 : 0; }
   }
@@ -181,13 +199,14 @@ int TfGatedLinearBackward(const DLArrayHandle input, const DLArrayHandle weight,
   float *dx = dinput ? out_f32(dinput) : nullptr, *dw = dweight ? out_f32(dweight) : nullptr;
   if (!dx && !dw) return 0;
   const NoHolding launched;
-  if (!contraction_path_is_cuda_cores()) {
+  const bool few_rows = M <= 8 && (double)K * 2 * F >= 1e6;           // (against large weights: the products have kernels for them)
+  if (contraction_path() == 2 || (contraction_path() == 0 && !few_rows && tensor_path_pays((double)M, (double)F, (double)K, true))) {
     if (const int r = tc_gated_bwd((const float*)input->data, (const float*)weight->data, (const float*)gates->data, (const float*)doutput->data, dx, dw, M, F, K, activation, s, what)) {
       note_contraction_path(2);
       return r < 0 ? -1 : 0;
     }
   }
-  if (contraction_path() != 2 && !(M <= 16 && (double)K * 2 * F >= 1e6)) {          // (few rows against large weights: the products have kernels for them)
+  if (contraction_path() != 2 && !few_rows) {
     if (const int r = gated_small_bwd((const float*)input->data, (const float*)weight->data, (const float*)gates->data, (const float*)doutput->data, dx, dw, M, F, K, activation, s, what)) {
       note_contraction_path(1);
       return r < 0 ? -1 : 0;
