@@ -6,7 +6,7 @@ function, the division: 2 to 4 u; erfc far below zero has its argument's roundin
 import numpy as np
 import pytest
 
-from tests.test_gpu_norm import place, read, within
+from tests.test_gpu_norm import place, read, view, within
 from tests.test_gpu_ops import close_dot, env  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -91,6 +91,93 @@ def test_alignment_engines_and_arithmetics(env, M, K, F, misaligned, path, arith
 @pytest.mark.parametrize("M,K,F", [(64, 300, 150), (130, 129, 125), (128, 128, 130), (200, 70, 2000), (3000, 64, 33)])      # 4e6 multiply-adds are the least it takes
 def test_forced_onto_the_tensor_cores(env, M, K, F):
     check(env, M, K, F, "gelu", path=2)
+
+
+@pytest.mark.parametrize("M,K,F", [(4000, 16, 70), (16, 512, 600), (17, 40, 4000), (1000, 20, 130), (129, 17, 999)])
+def test_short_reductions_on_the_tensor_cores(env, M, K, F):
+    """Less than one step of the reduction in one product or another."""
+    check(env, M, K, F, "silu", path=2)
+
+
+@pytest.mark.parametrize("M,K,F", [(8000, 16, 16), (2500, 96, 80), (1501, 77, 53), (3001, 33, 9), (30, 500, 40), (32, 512, 2048), (40, 2100, 1024), (100, 1999, 500), (256, 256, 1000), (500, 512, 512),
+                                   (8, 100, 8000), (600, 8, 1000)])
+def test_between_the_paths(env, M, K, F):
+    """Long batches whose weight gradient is cut, and sizes on both sides of where the tensor path begins to pay."""
+    check(env, M, K, F, "tanh")
+
+
+def test_rows_beyond_the_small_grid(env):
+    check(env, 65535 * 32 + 70, 2, 3, "relu")
+
+
+def test_projections_beyond_32_bits(env):
+    """2^31 + projections.  The inputs are zero but for the last three rows, so those alone make the gradient of the weights."""
+    K, F = 64, 8192
+    M = (1 << 31) // (2 * F) + 130
+    op, nd = env.gpu_op, env.nd
+    shapes = [(M, K), (M, 2 * F), (M, F), (M, F), (M, K)]
+    arrays = []
+    for s in shapes:
+        arrays.append(nd.empty(s, env.ctx))
+        if isinstance(arrays[-1], int):
+            pytest.skip("not enough device memory")
+    X, Z, H, D, DX = arrays
+    x, w, dout = inputs(3, K, F)
+    W, DW = nd.array(w, env.ctx), nd.empty((K, 2 * F), env.ctx)
+    op.array_set(X, 0.0, env.stream)
+    op.array_set(D, 0.5, env.stream)
+    op.device_synchronize()
+    view(env, X, (M - 3) * K, (3, K))[:] = x
+    view(env, D, (M - 3) * F, (3, F))[:] = dout
+    assert op.gated_linear_forward(X, W, Z, H, "sigmoid", env.stream) == 0
+    z = view(env, Z, (M - 3) * 2 * F, (3, 2 * F)).asnumpy()
+    x64, w64 = x.astype(np.float64), w.astype(np.float64)
+    close_dot(z, x64 @ w64, np.abs(x64) @ np.abs(w64), what="gates")
+    z = z.astype(np.float64)
+    value, slope, bv, bs = value_bound("sigmoid", z[:, :F])
+    within(view(env, H, (M - 3) * F, (3, F)).asnumpy(), value * z[:, F:], bv * np.abs(z[:, F:]) + 2 * U * np.abs(value * z[:, F:]) + 1e-37, "out")
+    assert not view(env, H, (M - 8) * F, (5, F)).asnumpy().any()
+    assert op.gated_linear_backward(X, W, Z, D, DX, DW, "sigmoid", env.stream) == 0
+    d64 = dout.astype(np.float64)
+    dz = np.concatenate([d64 * z[:, F:] * slope, d64 * value], axis=1)
+    bound = np.concatenate([np.abs(d64 * z[:, F:]) * bs, np.abs(d64) * bv], axis=1) + 4 * U * np.abs(dz)
+    for name, got, want, size, slack in (("dx", view(env, DX, (M - 3) * K, (3, K)), dz @ w64.T, np.abs(dz) @ np.abs(w64).T, bound @ np.abs(w64).T),
+                                         ("dw", DW, x64.T @ dz, np.abs(x64).T @ np.abs(dz), np.abs(x64).T @ bound)):
+        close_dot(got.asnumpy(), want, size + slack / (8 * U), what=name)
+    del X, Z, H, D, DX, arrays
+    op.release_cached_memory()
+
+
+def test_no_rows_against_large_weights(env):
+    op, nd = env.gpu_op, env.nd
+    W, DW = nd.array(np.ones((1024, 2048), np.float32), env.ctx), nd.array(np.ones((1024, 2048), np.float32), env.ctx)
+    X, Z, H, DX = (nd.empty(s, env.ctx) for s in ((0, 1024), (0, 2048), (0, 1024), (0, 1024)))
+    assert op.gated_linear_forward(X, W, Z, H, "silu", env.stream) == 0
+    assert op.gated_linear_backward(X, W, Z, H, DX, DW, "silu", env.stream) == 0
+    assert not DW.asnumpy().any()
+
+
+def test_a_capture_without_a_call_before_it(env):
+    """The first use of a stream is a capture: its scratch is made in it."""
+    import ctypes
+    import torch
+    for M, K, F in ((40, 96, 64), (4, 1024, 2048), (600, 512, 520)):
+        x, w, dout = inputs(M, K, F)
+        X, W, D = (env.nd.array(v, env.ctx) for v in (x, w, dout))
+        Z, H, DX, DW = (env.nd.empty(s, env.ctx) for s in ((M, 2 * F), (M, F), (M, K), (K, 2 * F)))
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        cell = ctypes.pointer(ctypes.c_void_p(side.cuda_stream))
+        env.gpu_op.device_synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            assert env.gpu_op.gated_linear_forward(X, W, Z, H, "silu", cell) == 0
+            assert env.gpu_op.gated_linear_backward(X, W, Z, D, DX, DW, "silu", cell) == 0
+        for _ in range(2):
+            graph.replay()
+        torch.cuda.synchronize()
+        got = [v.asnumpy() for v in (Z, H, DX, DW)]
+        env.gpu_op.gated_linear_forward(X, W, Z, H, "silu", env.stream)
+        env.gpu_op.gated_linear_backward(X, W, Z, D, DX, DW, "silu", env.stream)
+        assert all(np.array_equal(g, v.asnumpy()) for g, v in zip(got, (Z, H, DX, DW)))
 
 
 def test_no_rows_no_inputs_no_outputs(env):
