@@ -302,6 +302,17 @@ inline cudaError_t launch_cluster(void (*kernel)(Params...), int cluster, dim3 g
   return launch_shaped(kernel, LaunchShape{grid, block, smem, true, cluster}, s, args...);
 }
 #endif
+// What a kernel is allowed belongs to the device: set() runs on every one that it is asked for on, once.
+template <class F> inline cudaError_t once_per_device(std::atomic<uint64_t>& done, F&& set) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); dev = 0; }
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  const cudaError_t e = set();
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  else cudaGetLastError();
+  return e;
+}
 cudaError_t clear_on_stream(void* p, size_t bytes, cudaStream_t s);                       // cudaMemsetAsync(p, 0, bytes, s), and its node
 cudaError_t clear_now(void* p, size_t bytes);                                             // of new memory, complete on return
 cudaError_t copy_on_stream(void* to, const void* from, size_t bytes, cudaStream_t s);     // device to device

@@ -331,11 +331,11 @@ int gated_small_fwd(const float* x, const float* w, float* gates, float* out, in
   cudaError_t e = cudaSuccess;
   with_gate(activation, [&](auto act) {
     constexpr int ACT = decltype(act)::value;
-    static const cudaError_t attr = [] {
+    static std::atomic<uint64_t> ready{0};
+    e = once_per_device(ready, [] {
       const cudaError_t set = cudaFuncSetAttribute(gated_small_fwd_kernel<ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(FwdStep) * kAhead);
       return set != cudaSuccess ? set : cudaFuncSetAttribute(gated_small_fwd_kernel<ACT>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-    }();
-    e = attr;
+    });
     if (e == cudaSuccess) e = cluster > 1 ? launch_cluster(gated_small_fwd_kernel<ACT>, cluster, dim3(across * cluster, down), dim3(kThreads), sizeof(FwdStep) * kAhead, s, p)
                                           : launch_dep(gated_small_fwd_kernel<ACT>, dim3(across, down), dim3(kThreads), sizeof(FwdStep) * kAhead, s, p);
   });
@@ -369,8 +369,8 @@ int gated_small_bwd(const float* x, const float* w, const float* z, const float*
   with_gate(activation, [&](auto act) {
     constexpr int ACT = decltype(act)::value;
     // as the forward kernel's: with another split of the SM's memory a step of 64 x 784 x 256 takes 22.8 us instead of 19.8 (128 x 784 x 256: 30.9 and 31.7)
-    static const cudaError_t attr = cudaFuncSetAttribute(gated_small_bwd_kernel<ACT>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-    e = attr;
+    static std::atomic<uint64_t> ready{0};
+    e = once_per_device(ready, [] { return cudaFuncSetAttribute(gated_small_bwd_kernel<ACT>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared); });
     if (e == cudaSuccess) e = launch_cluster(gated_small_bwd_kernel<ACT>, cluster, dim3((unsigned)(clusters * cluster)), dim3(kThreads), 0, s, p);
   });
   TF_CUDA(e);

@@ -131,7 +131,8 @@ __global__ void __launch_bounds__(128) simt_group_kernel(const __grid_constant__
 template <int BM, int BN, int TM, int TN, int BK, bool AK, bool BKF>
 static cudaError_t launch_simt(const SimtGemm& p, int cluster, cudaStream_t s) {
   if (cluster > 8) {
-    static const cudaError_t allowed = cudaFuncSetAttribute(simt_gemm_kernel<BM, BN, TM, TN, BK, AK, BKF>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    static std::atomic<uint64_t> ready{0};
+    const cudaError_t allowed = once_per_device(ready, [] { return cudaFuncSetAttribute(simt_gemm_kernel<BM, BN, TM, TN, BK, AK, BKF>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1); });
     if (allowed != cudaSuccess) return allowed;
   }
   return launch_cluster(simt_gemm_kernel<BM, BN, TM, TN, BK, AK, BKF>, cluster, dim3((unsigned)cluster * ((p.N + BN - 1) / BN), (p.M + BM - 1) / BM), dim3((BM / TM) * (BN / TN)), 0, s, p);
@@ -415,7 +416,8 @@ template <int MR> static int launch_rows_nn(SimtGemm p, cudaStream_t s) {
   cut();
   while (cluster < 8 && (groups * cluster < 2 * sms || smem() > kRowSmem / 2) && p.K >= 64 * kRowWarps * cluster) { cluster *= 2; cut(); }
   if (smem() > kRowSmem || groups * cluster < sms) return 0;
-  static const cudaError_t attr = cudaFuncSetAttribute(rows_nn_kernel<MR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRowSmem);
+  static std::atomic<uint64_t> ready{0};
+  const cudaError_t attr = once_per_device(ready, [] { return cudaFuncSetAttribute(rows_nn_kernel<MR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRowSmem); });
   TF_CUDA(attr);
   KernelTimer kt("rows_gemm", s, 2.0 * (double)p.M * p.N * p.K, 0, 1);
   TF_CUDA(launch_cluster(rows_nn_kernel<MR>, cluster, dim3(groups * cluster), dim3(kRowThreads), smem(), s, p));
@@ -471,8 +473,8 @@ template <int MR> static int launch_rows_gated(RowsGated q, int activation, cuda
   cudaError_t e = cudaSuccess;
   with_gate(activation, [&](auto act) {
     constexpr int ACT = decltype(act)::value;
-    static const cudaError_t attr = cudaFuncSetAttribute(rows_gated_kernel<MR, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRowSmem);
-    e = attr;
+    static std::atomic<uint64_t> ready{0};
+    e = once_per_device(ready, [] { return cudaFuncSetAttribute(rows_gated_kernel<MR, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRowSmem); });
     if (e == cudaSuccess) e = launch_cluster(rows_gated_kernel<MR, ACT>, cluster, dim3(groups * cluster), dim3(kRowThreads), smem(), s, q);
   });
   TF_CUDA(e);

@@ -84,20 +84,23 @@ struct AmaxSlot {
 static std::unordered_map<const void*, AmaxSlot> g_amax;
 // A key is an array's address, or an odd address in its first word (bound_key): such a word is as old as the array, whoever writes that.
 static uint64_t array_version_locked(const void* key) { return version_locked(reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(key) & ~uintptr_t(3))); }
-static uint32_t* g_amax_chunk = nullptr;
-static int g_amax_left = 0;
+struct AmaxChunk { uint32_t* next = nullptr; int left = 0; };
+static AmaxChunk g_amax_chunk[64];            // of every device: its kernels write there
 static uint32_t* amax_chunk_words(int n) {
-  if (g_amax_left < n) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return nullptr; }
+  AmaxChunk& words = g_amax_chunk[dev];
+  if (words.left < n) {
     const int kWords = 16384;
     uint32_t* chunk = nullptr;
     if (cudaMalloc((void**)&chunk, kWords * sizeof(uint32_t)) != cudaSuccess || clear_now(chunk, kWords * sizeof(uint32_t)) != cudaSuccess) {
       cudaGetLastError();
       return nullptr;
     }
-    g_amax_chunk = chunk; g_amax_left = kWords;
+    words.next = chunk; words.left = kWords;
   }
-  uint32_t* w = g_amax_chunk;
-  g_amax_chunk += n; g_amax_left -= n;
+  uint32_t* w = words.next;
+  words.next += n; words.left -= n;
   return w;
 }
 static void amax_enter_recording(AmaxSlot& sl) {
@@ -2477,8 +2480,8 @@ static int plan_smem(GemmParams& g, int bn, int grid, int reserved = 0) {
 
 // The kernel may use all shared memory: asked for ahead of its first launch and of the first question how many clusters of it fit
 template <int BN, int AR, int FORM = kPlain> static cudaError_t gemm_kernel_ready() {
-  static const cudaError_t attr = cudaFuncSetAttribute(gemm3x_kernel<BN, AR, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit + 1024);
-  return attr;
+  static std::atomic<uint64_t> ready{0};
+  return once_per_device(ready, [] { return cudaFuncSetAttribute(gemm3x_kernel<BN, AR, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit + 1024); });
 }
 template <int BN, int AR> static int max_clusters_of(int c) {
   static std::atomic<int> known[9];
@@ -3013,6 +3016,8 @@ template <int AR> static int launch_gated(GemmParams& p, cudaStream_t s, double 
     if (oom) *oom = bytes > 0x7fffffffu ? 0x7fffffff : (int)bytes;
     return 1;
   }
+  const AmaxOut am = amax_track_begin_on(p.out, s);           // nothing is short from here on
+  p.amax = am.word; p.amax_clear = am.clear;
   const int grid = plan_smem(p, BN, plan_grid(p), kGatedStage);
   note_compute_stream(s);
   KernelTimer kt(AR == kArithTF32 ? "gemm3xtf32_gated" : "gemm3xf16_gated", s, flops, 0, 1);
@@ -3100,8 +3105,6 @@ int tc_gated_fwd(const float* x, const float* w, float* gates, float* out, int64
   p.M = (int)M; p.N = (int)cols; p.m_tiles = (int)((M + BM - 1) / BM); p.n_tiles = (int)((cols + 127) / 128); p.tap_tiles = 1;
   p.k_total = (int)((K + bk - 1) / bk);
   p.out = out; p.gates = gates; p.gated_f = (int)F; p.activation = activation; p.err = error_word(); p.band = band_of(p);
-  const AmaxOut am = amax_track_begin_on(out, s);
-  p.amax = am.word; p.amax_clear = am.clear;
   rc = ar == kArithTF32 ? launch_gated<kArithTF32>(p, s, 4.0 * M * F * K, what, nullptr) : launch_gated<kArithF16>(p, s, 4.0 * M * F * K, what, nullptr);
   return rc < 0 ? -1 : (rc > 0 ? 0 : 1);
 }

@@ -308,6 +308,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) norm_bwd_kernel(const NormArgs
     }
     float three[3] = {sq.x + sq.y, sg.x + sg.y, sgx.x + sgx.y};
     add(three);
+    if (VEC == 1 && G == 32) __syncwarp();     // the copies of a lane may replace what another one has read (longer rows have had a barrier)
     fetch(row + depth * stride, stage);        // what was there has been read, by all: the sums had barriers, and depend on the last of it
     stage += kStage;
     if (stage == depth * kStage) stage = 0;
@@ -563,8 +564,9 @@ template <bool RES> static int run_norm_bwd(NormArgs a, float* dgamma, float* db
       const size_t bytes = sizeof(float) * 2 * (size_t)a.D * blocks, smem = (size_t)stage * depth + sizeof(float) * G * NV * VEC;
       if (few) { a.dgamma = dgamma; a.dbeta = dbeta; }
       else if (sums && blocks && !(a.part = (float*)lease.scratch(kScratchNorm, bytes))) { out_of_memory = 1; shortage(bytes); return; }
-      static const cudaError_t attr = cudaFuncSetAttribute(norm_bwd_kernel<VEC, G, NV, RES>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBwdSmem);
-      e = attr;
+      static std::atomic<uint64_t> ready{0};
+      const auto kernel = norm_bwd_kernel<VEC, G, NV, RES>;
+      e = once_per_device(ready, [kernel] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBwdSmem); });
       if (!blocks || e != cudaSuccess) return;
       if (few) e = launch_cluster(norm_bwd_kernel<VEC, G, NV, RES>, blocks, dim3(blocks), dim3(groups * G), smem, s, a, depth);
       else e = launch_dep(norm_bwd_kernel<VEC, G, NV, RES>, dim3(blocks), dim3(groups * G), smem, s, a, depth);
