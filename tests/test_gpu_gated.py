@@ -80,6 +80,7 @@ def test_large_layers(env, k):
 @pytest.mark.parametrize("activation", ACTIVATIONS)
 def test_every_activation_on_the_tensor_cores(env, activation):
     check(env, 1200, 300, 1100, activation)
+    check(env, 300, 520, 499, activation)                    # few tiles, cut over clusters
 
 
 @pytest.mark.parametrize("M,K,F", [(64, 784, 256), (777, 500, 1003), (1200, 300, 1100), (3, 900, 700)])

@@ -33,6 +33,15 @@ template <int ACT> __device__ __forceinline__ float gate_value(float g) {
   sigmoids(g, s, rest);
   return ACT == kGateSigmoid ? s : g * s;
 }
+__device__ __forceinline__ float gate_value_of(int activation, float g) {
+  switch (activation) {
+    case kGateSigmoid: return gate_value<kGateSigmoid>(g);
+    case kGateRelu: return gate_value<kGateRelu>(g);
+    case kGateTanh: return gate_value<kGateTanh>(g);
+    case kGateSilu: return gate_value<kGateSilu>(g);
+    default: return gate_value<kGateGelu>(g);
+  }
+}
 // The activation's value and its derivative
 template <int ACT> __device__ __forceinline__ void gate_slope(float g, float& value, float& slope) {
   if (ACT == kGateRelu) { value = gate_value<ACT>(g); slope = g > 0.f ? 1.f : g != g ? g : 0.f; return; }
