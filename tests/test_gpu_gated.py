@@ -101,7 +101,7 @@ def test_short_reductions_on_the_tensor_cores(env, M, K, F):
 
 
 @pytest.mark.parametrize("M,K,F", [(8000, 16, 16), (2500, 96, 80), (1501, 77, 53), (3001, 33, 9), (30, 500, 40), (32, 512, 2048), (40, 2100, 1024), (100, 1999, 500), (256, 256, 1000), (500, 512, 512),
-                                   (8, 100, 8000), (600, 8, 1000)])
+                                   (8, 100, 8000), (600, 8, 1000), (16, 100, 2000), (65, 30, 1600)])
 def test_between_the_paths(env, M, K, F):
     """Long batches whose weight gradient is cut, and sizes on both sides of where the tensor path begins to pay."""
     check(env, M, K, F, "tanh")
