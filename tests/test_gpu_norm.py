@@ -112,7 +112,7 @@ def read(arr):
 
 SHAPES = [(1, 1), (5, 1), (3, 2), (64, 3), (1, 4), (9, 5), (2, 31), (33, 32), (7, 33), (70, 127), (1, 128), (300, 129), (17, 130), (64, 256), (3, 257), (1003, 500), (40, 512),
           (5, 516), (4, 3, 5, 1000), (129, 1023), (6, 1024), (2, 1, 1028), (1, 2047), (300, 2048), (3, 2050), (2, 4096), (700, 4096), (5, 4097), (150, 8190), (2, 8191), (3, 8192), (1, 8196),
-          (2, 16383), (170, 16384), (3, 16385), (1, 16388), (2, 40001), (2500, 64), (1,), (7,), (2048,)]
+          (2, 16383), (170, 16384), (3, 16385), (1, 16388), (2, 40001), (2500, 64), (1,), (7,), (2048,), (310, 9001), (400, 12290), (160, 8194), (149, 12288), (1, 12292)]
 
 
 @pytest.mark.parametrize("shape", SHAPES)
@@ -130,7 +130,7 @@ def test_layer_norm(env, shape, misaligned):
 
 
 @pytest.mark.parametrize("shape", [(1, 1), (64, 3), (1, 4), (7, 33), (300, 129), (64, 256), (17, 516), (4, 3, 5, 1000), (6, 1024), (300, 2048), (3, 2050), (700, 4096), (5, 8191), (3, 8192),
-                                   (2, 16384), (3, 16385), (2500, 64)])
+                                   (2, 16384), (3, 16385), (2500, 64), (310, 9001), (300, 12290), (160, 8196)])
 @pytest.mark.parametrize("rate,seed,misaligned", [(0.0, 0, 0), (0.1, 7, 0), (0.5, 100, 1), (0.9, 2 ** 31 - 1, 0)])
 def test_residual_norm(env, shape, rate, seed, misaligned):
     x, gamma, beta, dy, rng = inputs(shape)
