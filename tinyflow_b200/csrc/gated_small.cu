@@ -45,6 +45,8 @@ __device__ __forceinline__ void multiply(const Block& a, const Block& b, int ty,
     acc[3][0] = fmaf(r.w, c.x, acc[3][0]); acc[3][1] = fmaf(r.w, c.y, acc[3][1]);
   }
 }
+// (16 CTAs are more than every GPU's clusters may have; this one's may)
+constexpr int kMostRanks = 16;
 // Stores a tile: straight from the registers, or the sum over `ranks` CTAs of the cluster from `first` on, in order, each a slice of it
 template <class Store> __device__ __forceinline__ void finish_tile(int ranks, int first, float* part, const float (&acc)[4][2], int ty, int tx, Store&& store) {
   if (ranks == 1) {
@@ -69,6 +71,7 @@ template <class Store> __device__ __forceinline__ void finish_tile(int ranks, in
     float total = a[0];
 #pragma unroll
     for (int r = 1; r < 8; ++r) if (r < ranks) total += a[r];
+    for (int r = 8; r < ranks; ++r) total += cluster.map_shared_rank(part, first + r)[e];
     store(e / kTile, e % kTile, total);
   }
   cluster.sync();           // nobody leaves while its shared memory is still read
@@ -306,9 +309,9 @@ template <int ACT> __global__ void __launch_bounds__(kThreads) gated_small_bwd_k
 // Blocks of 64 x 64 would leave SMs idle: above that the plain products with their larger tiles are faster (backward, where dz is formed again for
 // every tile: 100 x 2000 x 500 73 us against 52)
 bool small_product(int64_t M, int64_t N) { return ((M + 63) / 64) * ((N + 63) / 64) < device_sm_count(); }
-int cluster_for(long long tiles, long long steps, int want) {
+int cluster_for(long long tiles, long long steps, int want, int most) {
   int c = 1;
-  while (c < 8 && tiles * c < want && steps >= 4 * c) c *= 2;
+  while (c < most && tiles * c < want && steps >= 4 * c) c *= 2;
   return c;
 }
 
@@ -323,7 +326,7 @@ int gated_small_fwd(const float* x, const float* w, float* gates, float* out, in
   p.x = x; p.w = w; p.gates = gates; p.out = out; p.M = (int)M; p.K = (int)K; p.F = (int)F;
   p.x_vec = K % 4 == 0 && aligned16(x); p.w_vec = F % 4 == 0 && aligned16(w);
   const unsigned across = (unsigned)((F + kTile - 1) / kTile), down = (unsigned)((M + kTile - 1) / kTile);
-  const int cluster = cluster_for((long long)across * down, (K + kDepth - 1) / kDepth, 3 * device_sm_count());
+  const int cluster = cluster_for((long long)across * down, (K + kDepth - 1) / kDepth, 3 * device_sm_count(), 8);
   p.per_cta = (int)(((K + cluster - 1) / cluster + kDepth - 1) / kDepth * kDepth);
   p.am = amax_track_begin_on(out, s);
   note_compute_stream(s);
@@ -343,10 +346,12 @@ int gated_small_fwd(const float* x, const float* w, float* gates, float* out, in
   TF_AFTER(s, what);
   return 1;
 }
+// Of both products, so that one gradient alone has the bits that it has beside the other.  Wide layers of few rows would make dx a chain of 12
+// steps and more in every CTA (16 x 100 x 2000 26.2 us against 18.2, 64 x 100 x 1000 15.3 and 14.6).
+bool gated_small_bwd_takes(int64_t M, int64_t F, int64_t K) { return small_product(M, K) && small_product(K, 2 * F) && !(M <= 64 && F > 96 * 16); }
 int gated_small_bwd(const float* x, const float* w, const float* z, const float* dout, float* dx, float* dw, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s,
                     const char* what) {
-  if (!small_product(M, K) || !small_product(K, 2 * F)) return 0;              // of both, so that one gradient alone has the bits that it has beside the other
-  if (M <= 64 && F > 96 * 16) return 0;              // dx would be a chain of 12 steps and more in every CTA (16 x 100 x 2000 26.2 us against 18.2, 64 x 100 x 1000 15.3 and 14.6)
+  if (!gated_small_bwd_takes(M, F, K)) return 0;
   Small p;
   memset(&p, 0, sizeof(p));
   p.x = x; p.w = w; p.z = z; p.dout = dout; p.dx = dx; p.dw = dw; p.M = (int)M; p.K = (int)K; p.F = (int)F;
@@ -356,8 +361,8 @@ int gated_small_bwd(const float* x, const float* w, const float* z, const float*
   p.dx_tiles = dx ? p.dx_across * (int)((M + kTile - 1) / kTile) : 0;
   p.dw_tiles = dw ? p.dw_across * (int)((K + kTile - 1) / kTile) : 0;
   const int sms = device_sm_count();
-  p.dx_ranks = dx ? cluster_for(p.dx_tiles, (F + 15) / 16, sms) : 1;
-  p.dw_ranks = dw ? cluster_for(p.dw_tiles, (M + kDepth - 1) / kDepth, sms) : 1;
+  p.dx_ranks = dx ? cluster_for(p.dx_tiles, (F + 15) / 16, sms, kMostRanks) : 1;
+  p.dw_ranks = dw ? cluster_for(p.dw_tiles, (M + kDepth - 1) / kDepth, sms, kMostRanks) : 1;
   p.per_cta = (int)(((F + p.dx_ranks - 1) / p.dx_ranks + 15) / 16 * 16);
   p.rows_per_cta = (int)(((M + p.dw_ranks - 1) / p.dw_ranks + kDepth - 1) / kDepth * kDepth);
   const int cluster = std::max(p.dx_ranks, p.dw_ranks), dx_each = cluster / p.dx_ranks, dw_each = cluster / p.dw_ranks;
@@ -371,7 +376,10 @@ int gated_small_bwd(const float* x, const float* w, const float* z, const float*
     constexpr int ACT = decltype(act)::value;
     // as the forward kernel's: with another split of the SM's memory a step of 64 x 784 x 256 takes 22.8 us instead of 19.8 (128 x 784 x 256: 30.9 and 31.7)
     static std::atomic<uint64_t> ready{0};
-    e = once_per_device(ready, [] { return cudaFuncSetAttribute(gated_small_bwd_kernel<ACT>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared); });
+    e = once_per_device(ready, [] {
+      const cudaError_t set = cudaFuncSetAttribute(gated_small_bwd_kernel<ACT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      return set != cudaSuccess ? set : cudaFuncSetAttribute(gated_small_bwd_kernel<ACT>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    });
     if (e == cudaSuccess) e = launch_cluster(gated_small_bwd_kernel<ACT>, cluster, dim3((unsigned)(clusters * cluster)), dim3(kThreads), 0, s, p);
   });
   TF_CUDA(e);

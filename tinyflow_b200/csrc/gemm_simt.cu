@@ -226,21 +226,34 @@ __global__ void __launch_bounds__(kRowThreads) rows_nn_kernel(const SimtGemm p) 
 // meet in the upper one.  Bound by the weights' bytes: 1 x 1024 x 4096 reads 33.6 MB in 6.5 us where they lie in L2, 8.4 from memory (the product,
 // then the gate: 12.2).
 struct RowsGated { SimtGemm g; float* gates; float* out; int F; AmaxOut am; };
-template <int MR, int ACT>
+template <int MR, int ACT, bool VEC>
 __global__ void __launch_bounds__(kRowThreads) rows_gated_kernel(const RowsGated q) {
   extern __shared__ __align__(16) float rows_smem[];
   const SimtGemm& p = q.g;
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kw = p.k_per_cta / kRowWarps, seg = p.k_per_cta;
-  const int f = (int)(blockIdx.x / ranks) * 64 + (lane & 15) * 4;
+  // a lane's columns: f to f + 3, or (rows that cannot be read 16 bytes at a time) every 16th from f on
+  const int f = (int)(blockIdx.x / ranks) * 64 + (lane & 15) * (VEC ? 4 : 1);
   grid_dep_sync();
   const int kbeg = rank * seg, count = max(0, min(seg, p.K - kbeg)), k1 = min((warp + 1) * kw, count);
   float4 w[8];
   const float* const b0 = p.B + (long long)kbeg * p.ldb + (lane < 16 ? 0 : q.F) + f;
   auto fetch = [&](int k) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = f < q.F && k + j < k1 ? __ldg(reinterpret_cast<const float4*>(b0 + (long long)(k + j) * p.ldb)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j = 0; j < 8; ++j) {
+      const float* const from = b0 + (long long)(k + j) * p.ldb;
+      w[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k + j >= k1) continue;
+      if (VEC) {
+        if (f < q.F) w[j] = __ldg(reinterpret_cast<const float4*>(from));
+      } else {
+        if (f < q.F) w[j].x = __ldg(from);
+        if (f + 16 < q.F) w[j].y = __ldg(from + 16);
+        if (f + 32 < q.F) w[j].z = __ldg(from + 32);
+        if (f + 48 < q.F) w[j].w = __ldg(from + 48);
+      }
+    }
   };
   fetch(warp * kw);                      // the first rows of the weight come with those of x
   for (int m = warp; m < MR; m += kRowWarps)
@@ -282,8 +295,8 @@ __global__ void __launch_bounds__(kRowThreads) rows_gated_kernel(const RowsGated
   if (ranks > 1) cluster.sync(); else __syncthreads();
   uint32_t top = 0;
   for (int i = rank * kRowThreads + threadIdx.x; i < MR * 16; i += ranks * kRowThreads) {
-    const int m = i >> 4, l = i & 15, c = (int)(blockIdx.x / ranks) * 64 + l * 4;
-    if (m >= p.M || c >= q.F) continue;
+    const int m = i >> 4, l = i & 15, c0 = (int)(blockIdx.x / ranks) * 64 + l * (VEC ? 4 : 1);
+    if (m >= p.M || c0 >= q.F) continue;
     float4 g = make_float4(0.f, 0.f, 0.f, 0.f), v = g;
     for (int r = 0; r < ranks; ++r) {
       const float4* const from = ranks > 1 ? cluster.map_shared_rank(part, r) : part;
@@ -293,9 +306,11 @@ __global__ void __launch_bounds__(kRowThreads) rows_gated_kernel(const RowsGated
     const float gate[4] = {g.x, g.y, g.z, g.w}, value[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (q.gates) { q.gates[(long long)m * 2 * q.F + c + j] = gate[j]; q.gates[(long long)m * 2 * q.F + q.F + c + j] = value[j]; }
+      const int c = c0 + j * (VEC ? 1 : 16);
+      if (!VEC && c >= q.F) break;
+      if (q.gates) { q.gates[(long long)m * 2 * q.F + c] = gate[j]; q.gates[(long long)m * 2 * q.F + q.F + c] = value[j]; }
       const float o = gate_value<ACT>(gate[j]) * value[j];
-      q.out[(long long)m * q.F + c + j] = o;
+      q.out[(long long)m * q.F + c] = o;
       top = max(top, finite_bits(o));
     }
   }
@@ -306,7 +321,7 @@ __global__ void __launch_bounds__(kRowThreads) rows_gated_kernel(const RowsGated
 // C = A[M x K] B[N x K]^T: a warp owns two rows of B along a run of K, a lane 4 columns at a time; the rows of A come through L1.
 // (Four rows a warp halve those reads and take registers: the same time.)
 constexpr int kRowSet = 2;
-template <int MR>
+template <int MR, bool VEC = true>
 __device__ __forceinline__ void rows_nt(const SimtGemm& p, int block) {
   constexpr int kSums = MR * kRowSet;
   __shared__ float part[kRowWarps][kSums];
@@ -318,12 +333,17 @@ __device__ __forceinline__ void rows_nt(const SimtGemm& p, int block) {
   for (int i = 0; i < kSums; ++i) acc[i] = make_float2(0.f, 0.f);
   const float* const b0 = p.B + (long long)min(n0, p.N - 1) * p.ldb;
   const float* const b1 = p.B + (long long)min(n0 + 1, p.N - 1) * p.ldb;
+  // four elements of a row, for the lane: the next ones, or (rows that cannot be read 16 bytes at a time) every 32nd
+  auto four = [&](const float* row, int k) {
+    if (VEC) return __ldg(reinterpret_cast<const float4*>(row + k));
+    return make_float4(__ldg(row + k), k + 32 < kend ? __ldg(row + k + 32) : 0.f, k + 64 < kend ? __ldg(row + k + 64) : 0.f, k + 96 < kend ? __ldg(row + k + 96) : 0.f);
+  };
 #pragma unroll 4
-  for (int k = run * p.k_per_cta + lane * 4; k < kend; k += 128) {
-    const float4 w[kRowSet] = {__ldg(reinterpret_cast<const float4*>(b0 + k)), __ldg(reinterpret_cast<const float4*>(b1 + k))};
+  for (int k = run * p.k_per_cta + lane * (VEC ? 4 : 1); k < kend; k += 128) {
+    const float4 w[kRowSet] = {four(b0, k), four(b1, k)};
 #pragma unroll
     for (int m = 0; m < MR; ++m) {
-      const float4 x = __ldg(reinterpret_cast<const float4*>(p.A + (long long)min(m, p.M - 1) * p.lda + k));
+      const float4 x = four(p.A + (long long)min(m, p.M - 1) * p.lda, k);
 #pragma unroll
       for (int r = 0; r < kRowSet; ++r) {
         float2& a = acc[m * kRowSet + r];
@@ -358,13 +378,19 @@ __device__ __forceinline__ void rows_nt(const SimtGemm& p, int block) {
 
 // C = A[K x M]^T B[K x N] of at most KR rows: a thread keeps its 4 columns of B and writes them times one row of A^T after the other.
 constexpr int kOuterRows = 32;
-template <int KR>
+template <int KR, bool VEC = true>
 __device__ __forceinline__ void rows_tn(const SimtGemm& p, int block_x, int block_y) {
-  const int n = (block_x * kRowThreads + (int)threadIdx.x) * 4, m0 = block_y * kOuterRows;
+  constexpr int kApart = VEC ? 1 : kRowThreads;            // between the columns of a thread
+  const int n = block_x * kRowThreads * 4 + (int)threadIdx.x * (VEC ? 4 : 1), m0 = block_y * kOuterRows;
   if (n >= p.N) return;
   float4 b[KR];
 #pragma unroll
-  for (int k = 0; k < KR; ++k) b[k] = k < p.K ? __ldg(reinterpret_cast<const float4*>(p.B + (long long)k * p.ldb + n)) : make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < KR; ++k) {
+    const float* const row = p.B + (long long)k * p.ldb + n;
+    if (k >= p.K) b[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    else if (VEC) b[k] = __ldg(reinterpret_cast<const float4*>(row));
+    else b[k] = make_float4(__ldg(row), n + kApart < p.N ? __ldg(row + kApart) : 0.f, n + 2 * kApart < p.N ? __ldg(row + 2 * kApart) : 0.f, n + 3 * kApart < p.N ? __ldg(row + 3 * kApart) : 0.f);
+  }
   const int m1 = min(p.M, m0 + kOuterRows);
   for (int m = m0; m < m1; m += 4) {
     float4 out[4];
@@ -373,8 +399,14 @@ __device__ __forceinline__ void rows_tn(const SimtGemm& p, int block_x, int bloc
 #pragma unroll
     for (int k = 0; k < KR; ++k) {
       if (k >= p.K) break;
-      const float4 a4 = __ldg(reinterpret_cast<const float4*>(p.A + (long long)k * p.lda + m));
-      const float a[4] = {a4.x, a4.y, a4.z, a4.w};
+      float a[4];
+      const float* const from = p.A + (long long)k * p.lda + m;
+      if (VEC) {
+        *reinterpret_cast<float4*>(a) = __ldg(reinterpret_cast<const float4*>(from));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) a[j] = m + j < m1 ? __ldg(from + j) : 0.f;
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         out[j].x = fmaf(a[j], b[k].x, out[j].x); out[j].y = fmaf(a[j], b[k].y, out[j].y);
@@ -382,7 +414,17 @@ __device__ __forceinline__ void rows_tn(const SimtGemm& p, int block_x, int bloc
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(p.C + (long long)(m + j) * p.ldc + n) = out[j];
+    for (int j = 0; j < 4; ++j) {
+      float* const to = p.C + (long long)(m + j) * p.ldc + n;
+      if (VEC) {
+        *reinterpret_cast<float4*>(to) = out[j];
+      } else if (m + j < m1) {
+        to[0] = out[j].x;
+        if (n + kApart < p.N) to[kApart] = out[j].y;
+        if (n + 2 * kApart < p.N) to[2 * kApart] = out[j].z;
+        if (n + 3 * kApart < p.N) to[3 * kApart] = out[j].w;
+      }
+    }
   }
 }
 
@@ -394,14 +436,15 @@ template <int KR> __global__ void __launch_bounds__(kRowThreads) rows_tn_kernel(
   grid_dep_sync();
   rows_tn<KR>(p, blockIdx.x, blockIdx.y);
 }
-// Both gradients of a gated layer on up to 8 rows, from dz: one reads the weights, one writes theirs, side by side (1 x 1024 x 4096 with dz: 22.1
-// us in two launches, 16.8 in one; with 16 rows the registers of the one cost the other its blocks, 51 us apart and 58 together)
+// Both gradients of a gated layer on up to 8 rows, from dz: one reads the weights, one writes theirs, side by side, so the weights' bytes bound it
+// (1 x 1024 x 4096 with dz: 22.1 us in two launches, 16.8 in one; 16 rows would cost each other registers and blocks, 51 us apart and 58 together).
+// Widths that 16-byte accesses do not fit: 1 x 622 x 4027 38.6 us with tiles, 10.0 so; a long sum for few inputs: 1 x 64 x 8192 40.5 and 6.8.
 struct RowsBoth { SimtGemm dx, dw; int dx_blocks, dw_across; };
-template <int MR> __global__ void __launch_bounds__(kRowThreads) rows_both_kernel(const RowsBoth q) {
+template <int MR, bool NT_VEC, bool TN_VEC> __global__ void __launch_bounds__(kRowThreads) rows_both_kernel(const RowsBoth q) {
   grid_dep_sync();
   const int b = (int)blockIdx.x - q.dx_blocks;
-  if (b < 0) rows_nt<MR>(q.dx, blockIdx.x);
-  else rows_tn<MR>(q.dw, b % q.dw_across, b / q.dw_across);
+  if (b < 0) rows_nt<MR, NT_VEC>(q.dx, blockIdx.x);
+  else rows_tn<MR, TN_VEC>(q.dw, b % q.dw_across, b / q.dw_across);
 }
 
 // Takes the product if it is one of those: 1, 0 if not, -1 on error.  Below a million weights, or where these leave SMs without a block
@@ -424,12 +467,12 @@ template <int MR> static int launch_rows_nn(SimtGemm p, cudaStream_t s) {
   return 1;
 }
 // Cuts the rows of B into runs of K for the warps: blocks, 0: too few for every SM
-static long long rows_nt_blocks(SimtGemm& q) {
+static long long rows_nt_blocks(SimtGemm& q, long long least) {
   const int sms = device_sm_count();
   const long long sets = (q.N + kRowSet - 1) / kRowSet;
   int runs = 1;
   while (runs < kRowWarps && sets * runs < 24ll * sms && q.K >= 256 * runs) runs *= 2;
-  if (sets * runs < 8ll * sms) return 0;
+  if (sets * runs < least) return 0;
   q.k_per_cta = (int)(((q.K + runs - 1) / runs + 127) / 128 * 128);
   runs = (q.K + q.k_per_cta - 1) / q.k_per_cta;
   while (kRowWarps % runs) { q.k_per_cta += 128; runs = (q.K + q.k_per_cta - 1) / q.k_per_cta; }       // whole sets in a block
@@ -441,7 +484,7 @@ static int rows_matmul(const SimtGemm& p, bool tA, bool tB, cudaStream_t s) {
     if (!tB && p.b_vec && p.N % 4 == 0) return p.M <= 8 ? launch_rows_nn<8>(p, s) : launch_rows_nn<16>(p, s);
     if (tB && p.a_vec && p.b_vec && p.K % 4 == 0) {
       SimtGemm q = p;
-      const long long blocks = rows_nt_blocks(q);
+      const long long blocks = rows_nt_blocks(q, 8ll * sms);
       if (!blocks) return 0;
       const dim3 grid((unsigned)blocks);
       KernelTimer kt("rows_gemm", s, 2.0 * (double)p.M * p.N * p.K, 0, 1);
@@ -459,7 +502,7 @@ static int rows_matmul(const SimtGemm& p, bool tA, bool tB, cudaStream_t s) {
 }
 
 // A gated layer on up to 16 rows with a million weights and more: 1 done, 0 not one of those, -1 error
-template <int MR> static int launch_rows_gated(RowsGated q, int activation, cudaStream_t s) {
+template <int MR, bool VEC> static int launch_rows_gated(RowsGated q, int activation, cudaStream_t s) {
   SimtGemm& p = q.g;
   const int sms = device_sm_count(), groups = (q.F + 63) / 64;
   int cluster = 1;
@@ -467,6 +510,8 @@ template <int MR> static int launch_rows_gated(RowsGated q, int activation, cuda
   auto cut = [&] { p.k_per_cta = (int)(((long long)p.K + cluster * kRowWarps * 8 - 1) / (cluster * kRowWarps * 8)) * kRowWarps * 8; };        // a warp's run is a multiple of 8
   cut();
   while (cluster < 8 && (groups * cluster < 2 * sms || smem() > kRowSmem / 2) && p.K >= 64 * kRowWarps * cluster) { cluster *= 2; cut(); }
+  // shorter runs where that gives every SM a block (1 x 512 x 4096 12.9 us with tiles, 5.0 so; 1 x 1024 x 4096, whose blocks are enough, 6.6 and 10.1)
+  while (cluster < 8 && groups * cluster < sms && p.K >= 32 * kRowWarps * cluster) { cluster *= 2; cut(); }
   if (smem() > kRowSmem || groups * cluster < sms) return 0;
   KernelTimer kt("rows_gated", s, 4.0 * (double)p.M * q.F * p.K, 0, 1);
   q.am = amax_track_begin_on(q.out, s);
@@ -474,31 +519,35 @@ template <int MR> static int launch_rows_gated(RowsGated q, int activation, cuda
   with_gate(activation, [&](auto act) {
     constexpr int ACT = decltype(act)::value;
     static std::atomic<uint64_t> ready{0};
-    e = once_per_device(ready, [] { return cudaFuncSetAttribute(rows_gated_kernel<MR, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRowSmem); });
-    if (e == cudaSuccess) e = launch_cluster(rows_gated_kernel<MR, ACT>, cluster, dim3(groups * cluster), dim3(kRowThreads), smem(), s, q);
+    e = once_per_device(ready, [] { return cudaFuncSetAttribute(rows_gated_kernel<MR, ACT, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRowSmem); });
+    if (e == cudaSuccess) e = launch_cluster(rows_gated_kernel<MR, ACT, VEC>, cluster, dim3(groups * cluster), dim3(kRowThreads), smem(), s, q);
   });
   TF_CUDA(e);
   TF_AFTER(s, "rows_gated");
   return 1;
 }
 int rows_gated(const float* x, const float* w, float* gates, float* out, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s) {
-  if (M > kFewRows || (double)K * 2 * F < 1e6 || F % 4 || !aligned16(w)) return 0;
+  if (M > kFewRows || (double)K * 2 * F < 1e6) return 0;
   RowsGated q{SimtGemm{x, w, nullptr, (int)M, (int)(2 * F), (int)K, K, 2 * F, 0, 0, 0, 1, 0}, gates, out, (int)F, AmaxOut{}};
   note_compute_stream(s);
-  return M == 1 ? launch_rows_gated<1>(q, activation, s) : M <= 8 ? launch_rows_gated<8>(q, activation, s) : launch_rows_gated<16>(q, activation, s);
+  if (F % 4 || !aligned16(w)) return M == 1 ? launch_rows_gated<1, false>(q, activation, s) : M <= 8 ? launch_rows_gated<8, false>(q, activation, s) : launch_rows_gated<16, false>(q, activation, s);
+  return M == 1 ? launch_rows_gated<1, true>(q, activation, s) : M <= 8 ? launch_rows_gated<8, true>(q, activation, s) : launch_rows_gated<16, true>(q, activation, s);
 }
 
 // dx = dz W^T and dW = x^T dz in one launch: 1 done, 0 not for these kernels, -1 error
 int rows_gated_bwd(const float* x, const float* w, const float* dz, float* dx, float* dw, int64_t M, int64_t F, int64_t K, cudaStream_t s) {
-  if (M < 1 || M > 8 || (double)K * 2 * F < 1e6 || F % 2 || K % 4 || !aligned16(x) || !aligned16(w) || !aligned16(dz) || !aligned16(dw) || (K + kOuterRows - 1) / kOuterRows > 65535) return 0;
+  if (M < 1 || M > 8 || (double)K * 2 * F < 1e6) return 0;
+  const bool nt_vec = F % 2 == 0 && aligned16(w) && aligned16(dz), tn_vec = nt_vec && K % 4 == 0 && aligned16(x) && aligned16(dw);
   RowsBoth q{SimtGemm{dz, w, dx, (int)M, (int)K, (int)(2 * F), 2 * F, 2 * F, K, 0, 1, 1, 0}, SimtGemm{x, dz, dw, (int)K, (int)(2 * F), (int)M, K, 2 * F, 2 * F, 0, 1, 1, 1}, 0, 0};
-  q.dx_blocks = (int)rows_nt_blocks(q.dx);
+  q.dx_blocks = (int)rows_nt_blocks(q.dx, 1);
   if (!q.dx_blocks) return 0;
   q.dw_across = (q.dw.N + 4 * kRowThreads - 1) / (4 * kRowThreads);
   const dim3 grid((unsigned)(q.dx_blocks + q.dw_across * ((q.dw.M + kOuterRows - 1) / kOuterRows)));
   note_compute_stream(s);
   KernelTimer kt("rows_gated_bwd", s, 8.0 * (double)M * F * K, 0, 1);
-  TF_CUDA(M == 1 ? launch_dep(rows_both_kernel<1>, grid, dim3(kRowThreads), 0, s, q) : launch_dep(rows_both_kernel<8>, grid, dim3(kRowThreads), 0, s, q));
+  const auto kernel = M == 1 ? (tn_vec ? rows_both_kernel<1, true, true> : nt_vec ? rows_both_kernel<1, true, false> : rows_both_kernel<1, false, false>)
+                             : tn_vec ? rows_both_kernel<8, true, true> : nt_vec ? rows_both_kernel<8, true, false> : rows_both_kernel<8, false, false>;
+  TF_CUDA(launch_dep(kernel, grid, dim3(kRowThreads), 0, s, q));
   TF_AFTER(s, "rows_gated_bwd");
   return 1;
 }

@@ -20,6 +20,7 @@ int tc_gated_bwd(const float* x, const float* w, const float* z, const float* do
 int rows_gated(const float* x, const float* w, float* gates, float* out, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s);
 int rows_gated_bwd(const float* x, const float* w, const float* dz, float* dx, float* dw, int64_t M, int64_t F, int64_t K, cudaStream_t s);
 int gated_small_fwd(const float* x, const float* w, float* gates, float* out, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s, const char* what);
+bool gated_small_bwd_takes(int64_t M, int64_t F, int64_t K);
 int gated_small_bwd(const float* x, const float* w, const float* z, const float* dout, float* dx, float* dw, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s, const char* what);
 void note_contraction_path(int path);
 bool pause_holding();                    // what follows is not to wait; returns whether it could have
@@ -103,17 +104,25 @@ cudaError_t launch_gate_gradient(int activation, const float* z, const float* do
   return e;
 }
 
-// Whether the tensor path is the shorter road, in us.  It costs a chain of launches and 12 bytes of traffic per operand element (gradients: 32 for
-// dz) before the first product; the CUDA-core kernels cost per multiply-add of one product, and for long reductions over few tiles a chain of steps.
-// Fitted to 40 shapes of 8 to 8000 rows and 8 to 4096 columns, tensor path against CUDA cores: 512 x 512 x 512 forward 19.9 against 24.7, backward
-// 33.9 against 68.7; 64 x 512 x 1024 19.1 against 9.2 and 26.5 against 24.6; 64 x 2048 x 1024 32.1 against 23.0 and 41.0 against 56.5; 32 x 2048 x 2048
-// 41.2 against 23.0 and 63.4 against 55.9; 4000 x 128 x 128 16.1 against 13.2 and 29.9 against 43.6.
-bool tensor_path_pays(double M, double F, double K, bool backward) {
-  const double work = 2.0 * M * F * K, elements = 1e-6 * (M * K + 2.0 * K * F);
-  if (!backward) return 15.0 + 0.004 * K + 2.4 * elements + 7e-9 * work < 3.5 + 7.7e-8 * work;
-  const double tiles_dx = std::ceil(M / 32) * std::ceil(K / 32), tiles_dw = std::ceil(K / 32) * std::ceil(F / 16), sms = device_sm_count();
-  const double chain = std::max(0.03 * M / std::min(8.0, std::max(1.0, sms / tiles_dw)), 0.05 * F / std::min(8.0, std::max(1.0, sms / tiles_dx)));
-  return 25.0 + 3.4 * elements + 6.4e-6 * M * F + 1.4e-8 * work < 5.0 + std::max((M <= 32 && work < 1.5e8 ? 1.85e-7 : 2.4e-7) * work, chain);
+// Whether the tensor path is the shorter road, in us.  It costs a chain of launches and the traffic of the packs before the first product; the
+// CUDA-core kernels cost per multiply-add, more of it where rows cannot be read 16 bytes at a time, and for long reductions over few tiles a
+// chain of steps.  Fitted to 300 shapes of 16 to 8192 rows and 16 to 8192 columns with up to 3e9 multiply-adds, where the road it takes is on
+// average 1 % slower than the better one (backward 1.2 %, at most 1.5 times).  Tensor path against CUDA cores: 512 x 512 x 512 forward 19.9 against
+// 24.7, backward 33.9 against 68.7; 64 x 512 x 1024 19.1 against 9.2 and 26.5 against 24.6; 4000 x 128 x 128 16.1 against 13.2 and 29.9 against 43.6;
+// 748 x 16 x 5784 backward 55 against 232.
+bool tensor_path_pays(int64_t rows, int64_t outputs, int64_t inputs, bool backward) {
+  const double M = (double)rows, F = (double)outputs, K = (double)inputs, work = 2.0 * M * F * K, sms = device_sm_count();
+  const bool odd = outputs % 4 || inputs % 4;
+  const auto tiles = [](double a, double b, double of) { return std::ceil(a / 32) * std::ceil(b / of); };
+  if (!backward) {
+    const double whole = 2048.0 * tiles(M, F, 32) * K;                       // multiply-adds of whole tiles
+    return work > 3e8 || 15.2 + 0.0026 * K + 1e-6 * (2.3 * M * K + 3.85 * K * F + 5.1 * M * F) < 5.5 + (odd ? 9.6e-8 : 8e-8) * whole;
+  }
+  const double tensor = 23.2 + 1.4e-8 * work + 1e-6 * (3.9 * M * K + 8.6 * K * F + 11.5 * M * F) + (odd ? 4.6 : 0.0);
+  if (rows <= 16 && !odd && 2.0 * F * K >= 1e6) return tensor < 5.0 + 3.5e-7 * work;                // the products have kernels for those
+  if (!gated_small_bwd_takes(rows, outputs, inputs)) return tensor < 6.0 + 0.006 * F + (odd ? 8e-7 : 4e-7) * work;
+  const double cut_dw = std::min(8.0, std::max(1.0, sms / tiles(K, F, 16))), cut_dx = std::min(8.0, std::max(1.0, sms / tiles(M, K, 32)));
+  return tensor < 5.0 + (odd ? 1.8 : 1.0) * std::max(2.8e-7 * work, std::max(0.03 * M / cut_dw, 0.05 * F / cut_dx));
 }
 
 // Products of scratch are launched at once, whatever the caller holds back.
@@ -163,7 +172,7 @@ int TfGatedLinearForward(const DLArrayHandle input, const DLArrayHandle weight, 
   if (contraction_path() == 0) {           // (up to 16 rows against large weights)
     if (const int r = rows_gated((const float*)input->data, (const float*)weight->data, z, out, M, F, K, activation, s)) { note_contraction_path(1); return r < 0 ? -1 : 0; }
   }
-  if (contraction_path() == 2 || (contraction_path() == 0 && tensor_path_pays((double)M, (double)F, (double)K, false))) {
+  if (contraction_path() == 2 || (contraction_path() == 0 && tensor_path_pays(M, F, K, false))) {
     if (const int r = tc_gated_fwd((const float*)input->data, (const float*)weight->data, z, out, M, F, K, activation, s, what)) {
       note_contraction_path(2);
       return r < 0 ? -1 : 0;
@@ -200,7 +209,7 @@ int TfGatedLinearBackward(const DLArrayHandle input, const DLArrayHandle weight,
   if (!dx && !dw) return 0;
   const NoHolding launched;
   const bool few_rows = M <= 8 && (double)K * 2 * F >= 1e6;           // (against large weights: the products have kernels for them)
-  if (contraction_path() == 2 || (contraction_path() == 0 && !few_rows && tensor_path_pays((double)M, (double)F, (double)K, true))) {
+  if (contraction_path() == 2 || (contraction_path() == 0 && !few_rows && tensor_path_pays(M, F, K, true))) {
     if (const int r = tc_gated_bwd((const float*)input->data, (const float*)weight->data, (const float*)gates->data, (const float*)doutput->data, dx, dw, M, F, K, activation, s, what)) {
       note_contraction_path(2);
       return r < 0 ? -1 : 0;
