@@ -108,7 +108,7 @@ def test_between_the_paths(env, M, K, F):
 
 
 @pytest.mark.parametrize("misaligned", [0, 1])
-@pytest.mark.parametrize("M,K,F", [(1, 622, 4027), (1, 624, 4028), (3, 1001, 777), (8, 515, 1025), (13, 1023, 701), (1, 66, 8191), (5, 130, 5003), (1, 64, 8192), (6, 120, 7698), (16, 900, 1002)])
+@pytest.mark.parametrize("M,K,F", [(1, 622, 4027), (1, 624, 4028), (3, 1001, 777), (8, 515, 1025), (13, 1023, 701), (1, 66, 8191), (5, 130, 5003), (1, 64, 8192), (6, 120, 7698), (16, 900, 1002), (1, 25, 6935), (8, 13, 3001), (12, 8, 2999), (40, 27, 1801)])
 def test_few_rows_against_weights_of_every_width(env, M, K, F, misaligned):
     check(env, M, K, F, "gelu", misaligned)
 

@@ -346,9 +346,8 @@ int gated_small_fwd(const float* x, const float* w, float* gates, float* out, in
   TF_AFTER(s, what);
   return 1;
 }
-// Of both products, so that one gradient alone has the bits that it has beside the other.  Wide layers of few rows would make dx a chain of 12
-// steps and more in every CTA (16 x 100 x 2000 26.2 us against 18.2, 64 x 100 x 1000 15.3 and 14.6).
-bool gated_small_bwd_takes(int64_t M, int64_t F, int64_t K) { return small_product(M, K) && small_product(K, 2 * F) && !(M <= 64 && F > 96 * 16); }
+// Of both products, so that one gradient alone has the bits that it has beside the other.
+bool gated_small_bwd_takes(int64_t M, int64_t F, int64_t K) { return small_product(M, K) && small_product(K, 2 * F); }
 int gated_small_bwd(const float* x, const float* w, const float* z, const float* dout, float* dx, float* dw, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s,
                     const char* what) {
   if (!gated_small_bwd_takes(M, F, K)) return 0;

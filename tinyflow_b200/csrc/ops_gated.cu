@@ -18,6 +18,7 @@ int matmul_any(const float* A, bool tA, const float* B, bool tB, float* C, int64
 int tc_gated_fwd(const float* x, const float* w, float* gates, float* out, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s, const char* what);
 int tc_gated_bwd(const float* x, const float* w, const float* z, const float* dout, float* dx, float* dw, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s, const char* what);
 int rows_gated(const float* x, const float* w, float* gates, float* out, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s);
+bool rows_gated_bwd_takes(int64_t M, int64_t F, int64_t K);
 int rows_gated_bwd(const float* x, const float* w, const float* dz, float* dx, float* dw, int64_t M, int64_t F, int64_t K, cudaStream_t s);
 int gated_small_fwd(const float* x, const float* w, float* gates, float* out, int64_t M, int64_t F, int64_t K, int activation, cudaStream_t s, const char* what);
 bool gated_small_bwd_takes(int64_t M, int64_t F, int64_t K);
@@ -106,10 +107,10 @@ cudaError_t launch_gate_gradient(int activation, const float* z, const float* do
 
 // Whether the tensor path is the shorter road, in us.  It costs a chain of launches and the traffic of the packs before the first product; the
 // CUDA-core kernels cost per multiply-add, more of it where rows cannot be read 16 bytes at a time, and for long reductions over few tiles a
-// chain of steps.  Fitted to 300 shapes of 16 to 8192 rows and 16 to 8192 columns with up to 3e9 multiply-adds, where the road it takes is on
-// average 1 % slower than the better one (backward 1.2 %, at most 1.5 times).  Tensor path against CUDA cores: 512 x 512 x 512 forward 19.9 against
-// 24.7, backward 33.9 against 68.7; 64 x 512 x 1024 19.1 against 9.2 and 26.5 against 24.6; 4000 x 128 x 128 16.1 against 13.2 and 29.9 against 43.6;
-// 748 x 16 x 5784 backward 55 against 232.
+// chain of steps.  Fitted to 600 shapes of 16 to 8192 rows and 16 to 8192 columns with up to 3e9 multiply-adds, on which the road it takes is
+// on average 0.6 % slower than the better one, backward 1.2 % (at most 1.4 and 1.6 times).  Tensor path against CUDA cores: 512 x 512 x 512 forward
+// 19.9 us against 24.7, backward 33.9 against 68.7; 64 x 512 x 1024 19.1 against 9.2 and 26.5 against 24.6; 4000 x 128 x 128 16.1 against 13.2 and
+// 29.9 against 43.6; 437 x 28 x 5560 backward 40 against 183.
 bool tensor_path_pays(int64_t rows, int64_t outputs, int64_t inputs, bool backward) {
   const double M = (double)rows, F = (double)outputs, K = (double)inputs, work = 2.0 * M * F * K, sms = device_sm_count();
   const bool odd = outputs % 4 || inputs % 4;
@@ -120,9 +121,9 @@ bool tensor_path_pays(int64_t rows, int64_t outputs, int64_t inputs, bool backwa
   }
   const double tensor = 23.2 + 1.4e-8 * work + 1e-6 * (3.9 * M * K + 8.6 * K * F + 11.5 * M * F) + (odd ? 4.6 : 0.0);
   if (rows <= 16 && !odd && 2.0 * F * K >= 1e6) return tensor < 5.0 + 3.5e-7 * work;                // the products have kernels for those
-  if (!gated_small_bwd_takes(rows, outputs, inputs)) return tensor < 6.0 + 0.006 * F + (odd ? 8e-7 : 4e-7) * work;
-  const double cut_dw = std::min(8.0, std::max(1.0, sms / tiles(K, F, 16))), cut_dx = std::min(8.0, std::max(1.0, sms / tiles(M, K, 32)));
-  return tensor < 5.0 + (odd ? 1.8 : 1.0) * std::max(2.8e-7 * work, std::max(0.03 * M / cut_dw, 0.05 * F / cut_dx));
+  if (!gated_small_bwd_takes(rows, outputs, inputs)) return tensor < 10.0 + 0.006 * F + (odd ? 6e-7 : 4e-7) * work;
+  const double cut_dw = std::min(16.0, std::max(1.0, sms / tiles(K, F, 16))), cut_dx = std::min(16.0, std::max(1.0, sms / tiles(M, K, 32)));
+  return tensor < 5.0 + (odd ? 1.6 : 1.0) * std::max(3.2e-7 * work, std::max(0.02 * M / cut_dw, 0.08 * F / cut_dx));
 }
 
 // Products of scratch are launched at once, whatever the caller holds back.
@@ -208,7 +209,7 @@ int TfGatedLinearBackward(const DLArrayHandle input, const DLArrayHandle weight,
   float *dx = dinput ? out_f32(dinput) : nullptr, *dw = dweight ? out_f32(dweight) : nullptr;
   if (!dx && !dw) return 0;
   const NoHolding launched;
-  const bool few_rows = M <= 8 && (double)K * 2 * F >= 1e6;           // (against large weights: the products have kernels for them)
+  const bool few_rows = rows_gated_bwd_takes(M, F, K);
   if (contraction_path() == 2 || (contraction_path() == 0 && !few_rows && tensor_path_pays(M, F, K, true))) {
     if (const int r = tc_gated_bwd((const float*)input->data, (const float*)weight->data, (const float*)gates->data, (const float*)doutput->data, dx, dw, M, F, K, activation, s, what)) {
       note_contraction_path(2);
