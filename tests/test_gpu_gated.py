@@ -189,7 +189,7 @@ def test_a_capture_without_a_call_before_it(env):
 
 def test_no_rows_no_inputs_no_outputs(env):
     op, nd = env.gpu_op, env.nd
-    for M, K, F in ((0, 5, 4), (3, 5, 0)):
+    for M, K, F in ((0, 5, 4), (3, 5, 0), (3, 0, 2000), (0, 7, 2001)):
         arrays = [nd.empty(s, env.ctx) for s in ((M, K), (K, 2 * F), (M, 2 * F), (M, F), (M, K), (K, 2 * F), (M, F))]
         X, W, Z, H, DX, DW, D = arrays
         for a in (X, W, DX, DW):
@@ -205,7 +205,7 @@ def test_no_rows_no_inputs_no_outputs(env):
     assert not Z.asnumpy().any() and not H.asnumpy().any()
 
 
-@pytest.mark.parametrize("M,K,F", [(5, 40, 24), (9, 1024, 2048), (777, 500, 1003), (1300, 768, 1536)])
+@pytest.mark.parametrize("M,K,F", [(5, 40, 24), (9, 1024, 2048), (777, 500, 1003), (1300, 768, 1536), (1, 622, 4027), (7, 130, 2999), (8, 1024, 1024), (16, 645, 831), (4000, 20, 30), (300, 520, 500), (40, 27, 1801)])
 def test_one_gradient_alone_and_the_same_bits_every_time(env, M, K, F):
     x, w, dout = inputs(M, K, F)
     op = env.gpu_op

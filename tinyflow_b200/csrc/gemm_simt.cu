@@ -536,17 +536,16 @@ int rows_gated(const float* x, const float* w, float* gates, float* out, int64_t
 
 // Up to 8 rows against large weights, or wide ones, which would make dx a long chain in a few tiles (1 x 25 x 6935 37.6 us with tiles, 10.5 so)
 bool rows_gated_bwd_takes(int64_t M, int64_t F, int64_t K) { return M <= 8 && ((double)K * 2 * F >= 1e6 || F > 1536); }
-// dx = dz W^T and dW = x^T dz in one launch: 1 done, 0 not for these kernels, -1 error
+// dx = dz W^T and dW = x^T dz in one launch (either may be null: the other has the same bits): 1 done, 0 not for these kernels, -1 error
 int rows_gated_bwd(const float* x, const float* w, const float* dz, float* dx, float* dw, int64_t M, int64_t F, int64_t K, cudaStream_t s) {
-  if (M < 1 || !rows_gated_bwd_takes(M, F, K)) return 0;
+  if (M < 1 || K < 1 || !rows_gated_bwd_takes(M, F, K)) return 0;
   const bool nt_vec = F % 2 == 0 && aligned16(w) && aligned16(dz), tn_vec = nt_vec && K % 4 == 0 && aligned16(x) && aligned16(dw);
   RowsBoth q{SimtGemm{dz, w, dx, (int)M, (int)K, (int)(2 * F), 2 * F, 2 * F, K, 0, 1, 1, 0}, SimtGemm{x, dz, dw, (int)K, (int)(2 * F), (int)M, K, 2 * F, 2 * F, 0, 1, 1, 1}, 0, 0};
-  q.dx_blocks = (int)rows_nt_blocks(q.dx, 1);
-  if (!q.dx_blocks) return 0;
+  q.dx_blocks = dx ? (int)rows_nt_blocks(q.dx, 1) : 0;
   q.dw_across = (q.dw.N + 4 * kRowThreads - 1) / (4 * kRowThreads);
-  const dim3 grid((unsigned)(q.dx_blocks + q.dw_across * ((q.dw.M + kOuterRows - 1) / kOuterRows)));
+  const dim3 grid((unsigned)(q.dx_blocks + (dw ? q.dw_across * ((q.dw.M + kOuterRows - 1) / kOuterRows) : 0)));
   note_compute_stream(s);
-  KernelTimer kt("rows_gated_bwd", s, 8.0 * (double)M * F * K, 0, 1);
+  KernelTimer kt("rows_gated_bwd", s, 4.0 * (double)M * F * K * ((dx != nullptr) + (dw != nullptr)), 0, 1);
   const auto kernel = M == 1 ? (tn_vec ? rows_both_kernel<1, true, true> : nt_vec ? rows_both_kernel<1, true, false> : rows_both_kernel<1, false, false>)
                              : tn_vec ? rows_both_kernel<8, true, true> : nt_vec ? rows_both_kernel<8, true, false> : rows_both_kernel<8, false, false>;
   TF_CUDA(launch_dep(kernel, grid, dim3(kRowThreads), 0, s, q));

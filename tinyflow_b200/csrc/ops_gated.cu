@@ -233,7 +233,7 @@ int TfGatedLinearBackward(const DLArrayHandle input, const DLArrayHandle weight,
     TF_CUDA(launch_gate_gradient(activation, (const float*)gates->data, (const float*)doutput->data, dz, M, (int)F, amax_track_begin_on(dz, s), s));
     TF_AFTER(s, what);
   }
-  if (dx && dw && contraction_path() != 2) {
+  if (few_rows && contraction_path() != 2) {
     if (const int r = rows_gated_bwd((const float*)input->data, (const float*)weight->data, dz, dx, dw, M, F, K, s)) { note_contraction_path(1); note_write(dz); return r < 0 ? -1 : 0; }
   }
   if (dx && matmul_any(dz, false, (const float*)weight->data, true, dx, M, K, 2 * F, s, what)) return -1;
