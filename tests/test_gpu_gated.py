@@ -83,7 +83,7 @@ def test_every_activation_on_the_tensor_cores(env, activation):
     check(env, 300, 520, 499, activation)                    # few tiles, cut over clusters
 
 
-@pytest.mark.parametrize("M,K,F", [(64, 784, 256), (777, 500, 1003), (1200, 300, 1100), (3, 900, 700)])
+@pytest.mark.parametrize("M,K,F", [(64, 784, 256), (777, 500, 1003), (1200, 300, 1100), (3, 900, 700), (400, 300, 602)])
 @pytest.mark.parametrize("misaligned,path,arithmetic", [(1, 0, "3xfp16"), (0, 1, "3xfp16"), (0, 0, "3xtf32"), (1, 0, "3xtf32")])
 def test_alignment_engines_and_arithmetics(env, M, K, F, misaligned, path, arithmetic):
     check(env, M, K, F, "silu", misaligned, path, arithmetic)

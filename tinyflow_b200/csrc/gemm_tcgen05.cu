@@ -1995,7 +1995,7 @@ __global__ void __launch_bounds__(256) pack_matrix_kernel(const float* __restric
 // formed from the projections wherever it is wanted and never written as numbers of its own.
 enum { kRows = 0, kWeight = 1, kGradient = 2 };
 struct Operand {
-  int kind, F, vec;                // vec: kRows, kWeight: rows can be read 16 bytes at a time; kGradient: eight columns at a time
+  int kind, F, vec;                // vec: kRows, kWeight: rows can be read 16 bytes at a time; kGradient: columns at a time
   int first, blocks;               // of the launch
   const float *src, *dout;         // kGradient: the projections, and the gradient of the output
   void *hi, *lo;
@@ -2009,48 +2009,85 @@ __device__ __forceinline__ const Operand& operand_of(const Operands3& all) {
   while (k + 1 < all.n && (int)blockIdx.x >= all.op[k + 1].first) ++k;
   return all.op[k];
 }
-// dz of N columns from f on: 12 bytes read per column
-template <int ACT, int N> __device__ __forceinline__ void gate_gradient(const Operand& o, long long r, int f, float* dg, float* dv) {
-  const float *const z = o.src + r * 2 * o.F + f, *const d = o.dout + r * o.F + f;
-  float g[N], v[N], t[N];
-  if (N == 8) {
-#pragma unroll
-    for (int q = 0; q < N; q += 4) {
-      *reinterpret_cast<float4*>(g + q) = __ldg(reinterpret_cast<const float4*>(z + q));
-      *reinterpret_cast<float4*>(v + q) = __ldg(reinterpret_cast<const float4*>(z + o.F + q));
-      *reinterpret_cast<float4*>(t + q) = __ldg(reinterpret_cast<const float4*>(d + q));
-    }
+// N values -> N hi and N lo elements at hi + at, lo + at, a store each
+template <int N, class E> __device__ __forceinline__ void store_run(E* hi, E* lo, long long at, const float* v) {
+  if constexpr (N == 8) {
+    store8(hi, lo, at, v);
   } else {
-    g[0] = __ldg(z); v[0] = __ldg(z + o.F); t[0] = __ldg(d);
-  }
+    struct alignas(N * sizeof(E)) Run { E e[N]; } h, l;
 #pragma unroll
-  for (int q = 0; q < N; ++q) {
-    float value, slope;
-    gate_slope<ACT>(g[q], value, slope);
-    dg[q] = t[q] * v[q] * slope;
-    dv[q] = t[q] * value;
+    for (int q = 0; q < N; ++q) split_pair(v[q], h.e[q], l.e[q]);
+    *reinterpret_cast<Run*>(hi + at) = h;
+    *reinterpret_cast<Run*>(lo + at) = l;
   }
 }
-template <int ACT, int N> __device__ __forceinline__ uint32_t gradient_max(const Operand& o, long long first, long long stride) {
+// dz, N columns of both halves at a time (what F and the addresses allow), eight columns under way in a thread: f(row, column, dz of the gates, dz
+// of the values).  12 bytes read per column.  6728 x 220 x 2724, gradients: 367 us with single columns wherever eight do not fit, 258 so; 1863 x 79 x 8037, odd, 250 and 224.
+template <int ACT, int N, class F> __device__ __forceinline__ void each_gradient(const Operand& o, long long first, long long stride, F&& f) {
+  constexpr int U = N == 8 ? 1 : 2;
+  struct alignas(4 * N > 16 ? 16 : 4 * N) Run { float e[N]; };
   const int groups = o.F / N;
-  uint32_t top = 0;
-  for (long long i = first; i < o.rows * groups; i += stride) {
-    const long long r = i / groups;
-    float dg[N], dv[N];
-    gate_gradient<ACT, N>(o, r, (int)(i - r * groups) * N, dg, dv);
+  const long long total = o.rows * groups;
+  for (long long i = first; i < total; i += U * stride) {
+    Run g[U], v[U], d[U];
+    long long row[U];
+    int col[U];
 #pragma unroll
-    for (int q = 0; q < N; ++q) top = max(top, max(finite_bits(dg[q]), finite_bits(dv[q])));
+    for (int u = 0; u < U; ++u) {
+      const long long at = i + u * stride;
+      if (at >= total) continue;
+      row[u] = total <= 0xffffffffll ? (uint32_t)at / (uint32_t)groups : at / groups;
+      col[u] = (int)(at - row[u] * groups) * N;
+      const float *const z = o.src + row[u] * 2 * o.F + col[u], *const dout = o.dout + row[u] * o.F + col[u];
+      if constexpr (N == 8) {
+#pragma unroll
+        for (int q = 0; q < N; q += 4) {
+          *reinterpret_cast<float4*>(g[u].e + q) = __ldg(reinterpret_cast<const float4*>(z + q));
+          *reinterpret_cast<float4*>(v[u].e + q) = __ldg(reinterpret_cast<const float4*>(z + o.F + q));
+          *reinterpret_cast<float4*>(d[u].e + q) = __ldg(reinterpret_cast<const float4*>(dout + q));
+        }
+      } else {
+        g[u] = *reinterpret_cast<const Run*>(z); v[u] = *reinterpret_cast<const Run*>(z + o.F); d[u] = *reinterpret_cast<const Run*>(dout);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i + u * stride >= total) continue;
+#pragma unroll
+      for (int q = 0; q < N; ++q) {
+        float value, slope;
+        gate_slope<ACT>(g[u].e[q], value, slope);
+        g[u].e[q] = d[u].e[q] * v[u].e[q] * slope;
+        v[u].e[q] = d[u].e[q] * value;
+      }
+      f(row[u], col[u], g[u].e, v[u].e);
+    }
   }
-  return top;
 }
-template <int ACT> __global__ void __launch_bounds__(256) operand_max_kernel(const __grid_constant__ Operands3 all) {
+template <int ACT, class F> __device__ __forceinline__ void with_gradient(const Operand& o, F&& f) {
+  switch (o.vec) {
+    case 8: f(std::integral_constant<int, 8>()); break;
+    case 4: f(std::integral_constant<int, 4>()); break;
+    case 2: f(std::integral_constant<int, 2>()); break;
+    default: f(std::integral_constant<int, 1>()); break;
+  }
+}
+template <int ACT> __global__ void __launch_bounds__(256, 5) operand_max_kernel(const __grid_constant__ Operands3 all) {
   grid_dep_sync();
   const Operand& o = operand_of(all);
   if (!o.max) return;
   const long long first = (long long)((int)blockIdx.x - o.first) * blockDim.x + threadIdx.x, stride = (long long)o.blocks * blockDim.x;
   uint32_t top = 0;
   if (o.kind == kGradient) {
-    if (ACT >= 0) top = o.vec ? gradient_max<ACT < 0 ? 0 : ACT, 8>(o, first, stride) : gradient_max<ACT < 0 ? 0 : ACT, 1>(o, first, stride);
+    if constexpr (ACT >= 0) {
+      with_gradient<ACT>(o, [&](auto n) {
+        constexpr int N = decltype(n)::value;
+        each_gradient<ACT, N>(o, first, stride, [&](long long, int, const float* dg, const float* dv) {
+#pragma unroll
+          for (int q = 0; q < N; ++q) top = max(top, max(finite_bits(dg[q]), finite_bits(dv[q])));
+        });
+      });
+    }
   } else {
     const long long n = o.rows * o.cols;
     long long done = 0;
@@ -2070,8 +2107,8 @@ template <int ACT> __global__ void __launch_bounds__(256) operand_max_kernel(con
   top = __reduce_max_sync(0xffffffffu, top);
   if ((threadIdx.x & 31) == 0 && top) atomicMax(o.max, top);
 }
-// Eight packed columns a thread (kGradient: eight of each half, or one).  The block that arrives last clears the maxima for the next call.
-template <int ACT, class E> __global__ void __launch_bounds__(256) pack_operands_kernel(const __grid_constant__ Operands3 all) {
+// Eight packed columns a thread (kGradient: of each half, see each_gradient).  The block that arrives last clears the maxima for the next call.
+template <int ACT, class E> __global__ void __launch_bounds__(256, 5) pack_operands_kernel(const __grid_constant__ Operands3 all) {
   grid_dep_sync();
   const Operand& o = operand_of(all);
   const long long first = (long long)((int)blockIdx.x - o.first) * blockDim.x + threadIdx.x, stride = (long long)o.blocks * blockDim.x;
@@ -2079,27 +2116,15 @@ template <int ACT, class E> __global__ void __launch_bounds__(256) pack_operands
   E *const hi = (E*)o.hi, *const lo = (E*)o.lo;
   if (o.kind == kGradient) {
     if constexpr (ACT >= 0) {
-      if (o.vec) {
-        const int groups = o.F / 8;
-        for (long long i = first; i < o.rows * groups; i += stride) {
-          const long long r = i / groups;
-          const int f = (int)(i - r * groups) * 8;
-          float dg[8], dv[8];
-          gate_gradient<ACT, 8>(o, r, f, dg, dv);
+      with_gradient<ACT>(o, [&](auto n) {
+        constexpr int N = decltype(n)::value;
+        each_gradient<ACT, N>(o, first, stride, [&](long long r, int f, float* dg, float* dv) {
 #pragma unroll
-          for (int q = 0; q < 8; ++q) { dg[q] *= sc; dv[q] *= sc; }
-          store8(hi, lo, r * o.pitch + f, dg);
-          store8(hi, lo, r * o.pitch + o.F + f, dv);
-        }
-      } else {
-        for (long long i = first; i < o.rows * o.F; i += stride) {
-          const long long r = i / o.F, at = r * o.pitch + (i - r * o.F);
-          float dg, dv;
-          gate_gradient<ACT, 1>(o, r, (int)(i - r * o.F), &dg, &dv);
-          split_pair(dg * sc, hi[at], lo[at]);
-          split_pair(dv * sc, hi[at + o.F], lo[at + o.F]);
-        }
-      }
+          for (int q = 0; q < N; ++q) { dg[q] *= sc; dv[q] *= sc; }
+          store_run<N>(hi, lo, r * o.pitch + f, dg);
+          store_run<N>(hi, lo, r * o.pitch + o.F + f, dv);
+        });
+      });
     }
   } else {
     const int groups = (int)(o.pitch >> 3);
@@ -3082,7 +3107,8 @@ struct OperandPacks {
     if (!base) return 1;
     pk.hi = base; pk.lo = base + pk.bytes(); pk.words = (uint32_t*)(base + 2 * pk.bytes());
     o.kind = kind; o.F = F; o.src = src; o.dout = dout; o.hi = pk.hi; o.lo = pk.lo; o.rows = rows; o.cols = cols; o.pitch = pk.pitch;
-    o.vec = kind == kGradient ? F % 8 == 0 && aligned16(src) && aligned16(dout) : cols % 4 == 0 && (kind != kWeight || F % 4 == 0) && aligned16(src);
+    const uintptr_t bits = (uintptr_t)F * 4 | (uintptr_t)src | (uintptr_t)dout;
+    o.vec = kind == kGradient ? (bits % 16 == 0 ? (F % 8 == 0 ? 8 : 4) : bits % 8 == 0 ? 2 : 1) : cols % 4 == 0 && (kind != kWeight || F % 4 == 0) && aligned16(src);
     o.scale.scale = reinterpret_cast<float*>(pk.words + 2);
     return 0;
   }
@@ -3104,7 +3130,7 @@ struct OperandPacks {
       int at = 0;
       for (int i = 0; i < all.n; ++i) {
         Operand& o = all.op[i];
-        const long long items = o.kind == kGradient ? (o.vec ? o.rows * (o.F / 8) : o.rows * o.F / 4) : maxima ? o.rows * o.cols / 16 : o.rows * o.pitch / 8;
+        const long long items = o.kind == kGradient ? o.rows * o.F / (o.vec == 8 ? 8 : 4) : maxima ? o.rows * o.cols / 16 : o.rows * o.pitch / 8;
         o.first = at;
         o.blocks = maxima && !o.max ? 0 : grid_for(items, 256, 2);
         at += o.blocks;
