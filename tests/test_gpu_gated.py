@@ -241,6 +241,21 @@ def test_extreme_projections(env):
         assert np.all((np.abs(got[n:] - value) <= bv + 4 * U * np.abs(value)) | tiny), activation
 
 
+@pytest.mark.parametrize("activation", ["sigmoid", "silu", "tanh"])
+def test_slopes_of_many_projections(env, activation):
+    """2^17 gates: the reciprocal of every size of 1 + exp(-|g|) against 64 bits."""
+    n = 1 << 17
+    g = np.linspace(-30, 30, n).astype(np.float32)
+    Z = env.nd.array(np.concatenate([g, np.full(n, 1.0, np.float32)])[None, :], env.ctx)
+    D, X, W = (env.nd.array(np.ones(s, np.float32), env.ctx) for s in ((1, n), (1, 1), (1, 2 * n)))
+    DW = env.nd.empty((1, 2 * n), env.ctx)
+    env.gpu_op.gated_linear_backward(X, W, Z, D, None, DW, activation, env.stream)
+    got = DW.asnumpy()[0].astype(np.float64)                 # x is one: dW = dz
+    value, slope, bv, bs = value_bound(activation, g.astype(np.float64))
+    within(got[:n], slope, bs + 4 * U * np.abs(slope), "slope")
+    within(got[n:], value, bv + 4 * U * np.abs(value), "value")
+
+
 def test_the_call_does_not_wait_where_products_are_held(env):
     M, K, F = 40, 96, 64
     x, w, dout = inputs(M, K, F)

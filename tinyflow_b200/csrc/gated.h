@@ -19,18 +19,25 @@ template <class F> inline void with_gate(int a, F&& f) {
 }
 
 #ifdef __CUDACC__
+// 1 / d of a d from 1 to 2: the fast quotient, within 2 units of the last place, and a step of Newton's method, which squares that error and leaves
+// about one rounding.  (The general division takes a branch and 50 instructions more: 6728 x 64 x 2720 forward with silu 112 us, 92 so.)
+__device__ __forceinline__ float inverse(float d) {
+  const float r = __fdividef(1.f, d);
+  return fmaf(r, fmaf(-d, r, 1.f), r);
+}
 // 1 / (1 + exp(-g)) and one minus that, both without cancellation: exp of a number that is never positive
-__device__ __forceinline__ void sigmoids(float g, float& s, float& rest) {
-  const float e = expf(-fabsf(g)), r = 1.f / (1.f + e);
+// FAST: the short road to the reciprocal.  Where a thread has one or two outputs the general one is as fast (64 x 784 x 256 forward 8.9 us, 8.4 so).
+template <bool FAST = true> __device__ __forceinline__ void sigmoids(float g, float& s, float& rest) {
+  const float e = expf(-fabsf(g)), r = FAST ? inverse(1.f + e) : 1.f / (1.f + e);
   s = g >= 0.f ? r : e * r;
   rest = g >= 0.f ? e * r : r;
 }
-template <int ACT> __device__ __forceinline__ float gate_value(float g) {
+template <int ACT, bool FAST = true> __device__ __forceinline__ float gate_value(float g) {
   if (ACT == kGateRelu) return g > 0.f || g != g ? g : 0.f;
   if (ACT == kGateTanh) return tanhf(g);
   if (ACT == kGateGelu) return g * (0.5f * erfcf(-0.70710678118654752f * g));
   float s, rest;
-  sigmoids(g, s, rest);
+  sigmoids<FAST>(g, s, rest);
   return ACT == kGateSigmoid ? s : g * s;
 }
 __device__ __forceinline__ float gate_value_of(int activation, float g) {
@@ -46,7 +53,7 @@ __device__ __forceinline__ float gate_value_of(int activation, float g) {
 template <int ACT> __device__ __forceinline__ void gate_slope(float g, float& value, float& slope) {
   if (ACT == kGateRelu) { value = gate_value<ACT>(g); slope = g > 0.f ? 1.f : g != g ? g : 0.f; return; }
   if (ACT == kGateTanh) {
-    const float e = expf(-2.f * fabsf(g)), r = 1.f / (1.f + e);
+    const float e = expf(-2.f * fabsf(g)), r = inverse(1.f + e);
     value = tanhf(g);
     slope = 4.f * e * r * r;                   // 1 - tanh^2 without the subtraction
     return;
