@@ -274,7 +274,7 @@ def test_the_call_does_not_wait_where_products_are_held(env):
     assert all(np.array_equal(a, b) for a, b in zip(*got))
 
 
-@pytest.mark.parametrize("M,K,F", [(40, 96, 64), (9, 1024, 2048), (700, 512, 520), (20, 1024, 4100)])
+@pytest.mark.parametrize("M,K,F", [(40, 96, 64), (9, 1024, 2048), (700, 512, 520), (20, 1024, 4100), (3000, 32, 48), (3, 700, 1001), (200, 9001, 16)])
 def test_a_captured_block_replayed_on_other_data(env, M, K, F):
     """Norm, gated layer and both backward calls in a graph that the caller captures: its replays have the bits of ordinary calls whatever the
     sizes of the numbers were at the capture, before it and in the replays in between."""
@@ -435,6 +435,16 @@ def test_a_replayed_step_has_the_bits_of_the_ordinary_one(env, monkeypatch, opti
     assert runs[1][4] and not runs[0][4]
     assert all(np.array_equal(a, b) for a, b in zip(runs[0][2], runs[1][2]))
     assert all(np.array_equal(v, runs[1][3][n]) for n, v in runs[0][3].items())
+
+
+def test_a_replayed_step_of_a_long_batch(env, monkeypatch):
+    """Clusters of 16 in a recorded step.  The summed loss of so many rows makes the last steps overshoot to NaN, which both runs have to do alike."""
+    kind = dict(batch=2500, width=32, hidden=40, dropout=0.3)
+    runs = [block_step(monkeypatch, recorded, 9, **kind) for recorded in (False, True)]
+    assert runs[1][4] and not runs[0][4]
+    assert all(np.isfinite(v).all() for v in runs[0][2][:6])
+    assert all(np.array_equal(a, b, equal_nan=True) for a, b in zip(runs[0][2], runs[1][2]))
+    assert all(np.array_equal(v, runs[1][3][n], equal_nan=True) for n, v in runs[0][3].items())
 
 
 def _plan_swap(ex):
