@@ -100,3 +100,62 @@ def test_there_is_no_cpu_path(op, inputs):
     node = node[0] if isinstance(node, tuple) else node
     with pytest.raises(NotImplementedError):
         node.op.compute(node, [None] * inputs, [None, None], None, None, None, use_numpy=True)
+
+
+def residual_sum(readers):
+    """(sum, its normalisation, inputs, loss): the loss reads the normalisation and, `readers` times, the sum."""
+    from tinyflow_b200 import autodiff as ad
+    h, r, g, b = (ad.Variable(n) for n in "hrgb")
+    total, y = ad.dropout_add_layer_norm_op(h, r, g, b, 0.0)
+    whole = y * y * y
+    for _ in range(readers):
+        whole = whole + total * total
+    rng = np.random.RandomState(3)
+    return total, y, {n: rng.randn(*s) for n, s in ((h, (3, 5)), (r, (3, 5)), (g, (5,)), (b, (5,)))}, ad.reduce_sum_op(whole)
+
+
+@pytest.mark.parametrize("readers", [0, 1, 2])
+def test_the_gradient_of_a_residual_sum_itself(readers):
+    """Asked for by name it is what reaches the residual input (the sum is that plus the branch), once, however many read the sum."""
+    from oracle.graph_eval import OracleExecutor
+    from tinyflow_b200 import autodiff as ad
+    total, y, values, loss = residual_sum(readers)
+    h, r, g, b = values
+    grads = ad.gradients(loss, [total, r, h, y, g, b])
+    got = OracleExecutor(ad.find_topo_sort(grads + [loss])).run(values)
+    dtotal, dr, dh, dy = (got[n] for n in grads[:4])
+    np.testing.assert_allclose(dy, 3 * got[y] ** 2, rtol=1e-12)
+    np.testing.assert_array_equal(dtotal, dr)
+    np.testing.assert_array_equal(dtotal, dh)
+    order = ad.find_topo_sort([loss])
+
+    def at(**moved):
+        return float(OracleExecutor(order).run({n: moved.get(n.name, v) for n, v in values.items()})[loss].sum())
+
+    # central differences, step 1e-5: truncation of 1e-10 times a third derivative, cancellation of 1e-11 times the loss
+    for node, grad in zip((r, g, b), (dtotal, got[grads[4]], got[grads[5]])):
+        for i in np.ndindex(values[node].shape):
+            sides = []
+            for step in (1e-5, -1e-5):
+                v = values[node].copy()
+                v[i] += step
+                sides.append(at(**{node.name: v}))
+            want = (sides[0] - sides[1]) / 2e-5
+            assert abs(grad[i] - want) <= 1e-7 * (1 + abs(want)), (node.name, i)
+
+
+def test_two_normalisations_of_one_sum_and_gradients_taken_twice():
+    from oracle import ops
+    from oracle.graph_eval import OracleExecutor
+    from tinyflow_b200 import autodiff as ad
+    total, y, values, _ = residual_sum(0)
+    h, r, g, b = values
+    loss = ad.reduce_sum_op(y * y * y + ad.normalised_sum_op(total, g, b) * total)
+    first, second = ad.gradients(loss, [total, g]), ad.gradients(loss, [total, g])
+    got = OracleExecutor(ad.find_topo_sort(first + second)).run(values)
+    s = values[h] + values[r]
+    n = ops.layer_norm(s, values[g], values[b], 1e-5)[0]
+    dx, dg, _ = ops.layer_norm_backward(s, values[g], 3 * n * n + s, 1e-5)
+    for total_grad, gamma_grad in (first, second):
+        np.testing.assert_allclose(got[total_grad], dx + n, rtol=1e-9, atol=1e-12)
+        np.testing.assert_allclose(got[gamma_grad], dg, rtol=1e-9, atol=1e-12)

@@ -109,6 +109,10 @@ class Op(object):
     def gradient(self, node, output_grad):
         raise NotImplementedError
 
+    def adjoint(self, node, contributions):
+        """The gradient of ``node`` from what its readers contribute to it: their sum."""
+        return sum_node_list(contributions)
+
     def infer_shape(self, node, input_shapes, cudnnHandle):
         raise NotImplementedError
 
@@ -963,23 +967,26 @@ class DropoutAddLayerNormForwardOp(ManyOp):
         gpu_op.dropout_add_layer_norm_forward(*input_vals, *output_val, node.state[0], node.eps, cudaStream)
         return 0
 
-    def gradient(self, node, output_grad):
-        # The gradient through the normalisation is one of the summands; the kernel that computes it adds the others.
-        summands, through = [output_grad], None
-        while type(summands[0].op) is AddOp:
-            summands[:1] = summands[0].inputs
-        for g in summands:
-            if type(g.op) is PartOp and type(g.inputs[0].op) is DropoutAddLayerNormBackwardOp and g.part == 2 and g.inputs[0].inputs[0] is node and len(g.inputs[0].inputs) == 3:
-                through = g
-        if through is None:                       # the normalisation has no reader
-            whole = dropout_add_layer_norm_backward_op(node, node.inputs[2], zeroslike_op(node), node)
-            whole.inputs.append(output_grad)
-            return [part_op(whole, 3), part_op(whole, 2), whole, part_op(whole, 1)]
-        whole = through.inputs[0]
-        rest = [g for g in summands if g is not through]
+    def adjoint(self, node, contributions):
+        # The kernel that computes the gradient through the normalisation adds what else reaches the sum: its result is the whole of it.
+        through = next((g for g in contributions if self._through(g, node)), None)
+        if through is None:
+            return super().adjoint(node, contributions)
+        rest = [g for g in contributions if g is not through]
         if rest:
-            whole.inputs.append(sum_node_list(rest))
-        return [part_op(whole, 3), through]           # gamma and beta have theirs from the normalisation
+            through.inputs[0].inputs.append(sum_node_list(rest))
+        return through
+
+    @staticmethod
+    def _through(g, node):
+        return type(g.op) is PartOp and type(g.inputs[0].op) is DropoutAddLayerNormBackwardOp and g.part == 2 and g.inputs[0].inputs[0] is node
+
+    def gradient(self, node, output_grad):
+        if self._through(output_grad, node):
+            return [part_op(output_grad.inputs[0], 3), output_grad]           # gamma and beta have theirs from the normalisation
+        whole = dropout_add_layer_norm_backward_op(node, node.inputs[2], zeroslike_op(node), node)           # the normalisation has no reader
+        whole.inputs.append(output_grad)
+        return [part_op(whole, 3), part_op(whole, 2), whole, part_op(whole, 1)]
 
     def result_shapes(self, input_shapes):
         return input_shapes[0], input_shapes[0]
@@ -1283,7 +1290,7 @@ def gradients(output_node, node_list):
     pending = {output_node: [oneslike_op(output_node)]}
     grad_of = {}
     for node in reversed(find_topo_sort([output_node])):
-        grad = sum_node_list(pending[node])
+        grad = node.op.adjoint(node, pending[node])
         grad_of[node] = grad
         contributions = node.op.gradient(node, grad)
         for inp, g in zip(node.inputs, contributions or []):
