@@ -92,7 +92,7 @@ uint64_t version_of(const void* p);
 inline float* out_f32(DLArray* a) { note_write(a->data); return (float*)a->data; }
 void invalidate_all_versions();             // every tensor counts as rewritten (a recording was abandoned)
 
-// ---- largest magnitude of a tensor, tracked by its producer ---------------------------
+// ---- largest finite magnitude of a tensor, tracked by its producer ---------------------------
 // The tensor path scales each operand by a power of two chosen from max|x|.  Kernels that write a whole tensor
 // can fold that maximum into their pass: the launcher asks for a pair of device words after bumping the write
 // version (amax_track_begin), the kernel ends with amax_commit(), and the consumer gets the word back through
@@ -113,11 +113,13 @@ bool amax_carry_valid(const void* data);
 void amax_set_carry_valid(const void* data);
 void bump_versions(const void* const* ptrs, size_t n);
 #ifdef __CUDACC__
-__device__ __forceinline__ uint32_t amax_bits(float v) { return __float_as_uint(fabsf(v)); }
-// Of finite values only: an infinity or a NaN makes what reads it NaN whatever the scale, and the rows beside it keep their precision.
-__device__ __forceinline__ uint32_t finite_bits(float v) { const uint32_t b = amax_bits(v); return b < 0x7f800000u ? b : 0u; }
+// The words hold keys of magnitudes: of finite values only, since an infinity or a NaN makes what reads it NaN whatever the scale, and the rows
+// beside it keep their precision.  Twice the bits without the sign, and one of exponent more: finite values from kAmaxZero on in their order; infinities
+// and NaN wrap around to below it.  (A comparison per element in place of the wrap: 15.11 ms a ResNet-50 step, 14.81 so.)
+constexpr uint32_t kAmaxZero = 0x01000000u;
+__device__ __forceinline__ uint32_t amax_key(float v) { return __float_as_uint(v) * 2u + kAmaxZero; }
 __device__ __forceinline__ float finite_max(float m, float v) { v = fabsf(v); return v < __int_as_float(0x7f800000) ? fmaxf(m, v) : m; }
-// Every thread of the block calls this once, after its last store, with the largest bit pattern it produced.
+// Every thread of the block calls this once, after its last store, with the largest key it produced.
 __device__ __forceinline__ void amax_commit(const AmaxOut& am, uint32_t m) {
   if (!am.word) return;                                  // uniform over the grid
   __shared__ uint32_t amax_red[32];

@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kDirectThreads) direct_conv_kernel(const Direc
       if (o >= p.Co) continue;
       float* dst = p.out + (((long long)n * p.Co + o) * p.Ho + row) * p.Wo + 4 * g;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) if (4 * g + q < p.Wo) { dst[q] = acc[a][q]; big = max(big, amax_bits(acc[a][q])); }
+      for (int q = 0; q < 4; ++q) if (4 * g + q < p.Wo) { dst[q] = acc[a][q]; big = max(big, amax_key(acc[a][q])); }
     }
   }
   amax_commit(am, big);

@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(256) dp_apply_kernel(const __grid_constant__ A
     for (long long i = (long long)local * blockDim.x + threadIdx.x; i < e.count; i += stride) {
       float v = e.w[i] - scale * e.sum[i];
       e.w[i] = v;
-      mx = max(mx, amax_bits(v));
+      mx = max(mx, amax_key(v));
     }
   } else {
     for (long long i = (long long)local * blockDim.x + threadIdx.x; i < e.count; i += stride) {
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(256) dp_apply_kernel(const __grid_constant__ A
       if (e.w) {
         float w = e.w[i] - e.lr * mi / e.c1 / (sqrtf(vi / e.c2) + e.eps);
         e.w[i] = w;
-        mx = max(mx, amax_bits(w));
+        mx = max(mx, amax_key(w));
       }
     }
   }

@@ -182,7 +182,7 @@ template <int ACT> __global__ void __launch_bounds__(kThreads) gated_small_fwd_k
     if (p.gates) { p.gates[(long long)m * 2 * p.F + f] = gate; p.gates[(long long)m * 2 * p.F + p.F + f] = value; }
     value *= gate_value<ACT, false>(gate);
     p.out[(long long)m * p.F + f] = value;
-    top = max(top, finite_bits(value));
+    top = max(top, amax_key(value));
   };
   if (ranks == 1) {
 #pragma unroll

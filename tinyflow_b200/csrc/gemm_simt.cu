@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(kRowThreads) rows_gated_kernel(const RowsGated
       if (q.gates) { q.gates[(long long)m * 2 * q.F + c] = gate[j]; q.gates[(long long)m * 2 * q.F + q.F + c] = value[j]; }
       const float o = gate_value<ACT>(gate[j]) * value[j];
       q.out[(long long)m * q.F + c] = o;
-      top = max(top, finite_bits(o));
+      top = max(top, amax_key(o));
     }
   }
   if (ranks > 1) cluster.sync();           // nobody leaves while its shared memory is still read

@@ -619,7 +619,7 @@ template <int ACT> __device__ __forceinline__ uint32_t gate_run(const float* g, 
 #pragma unroll
   for (int q = 0; q < 32; ++q) {
     v[q] *= gate_value<ACT>(g[q]);
-    top = max(top, finite_bits(v[q]));
+    top = max(top, amax_key(v[q]));
   }
   return top;
 }
@@ -678,7 +678,7 @@ __device__ __forceinline__ uint32_t sum_gated(const GemmParams& p, const uint8_t
       if (f + q >= F) continue;
       sum[4 + q] *= gate_value_of(p.activation, sum[q]);
       p.out[(long long)m * F + f + q] = sum[4 + q];
-      top = max(top, finite_bits(sum[4 + q]));
+      top = max(top, amax_key(sum[4 + q]));
     }
   }
   return top;
@@ -1016,7 +1016,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm3x_kernel(const __grid_co
         if (!row_ok || c0 >= ncols) return;
         if (p.amax) {
 #pragma unroll
-          for (int q = 0; q < NC; ++q) top = max(top, amax_bits(v[q]));
+          for (int q = 0; q < NC; ++q) top = max(top, amax_key(v[q]));
         }
         char* dst = row_out + (uint64_t)col_bytes * (uint32_t)c0;
         if (vec_ok && c0 + NC <= ncols) {
@@ -1173,7 +1173,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm3x_kernel(const __grid_co
           const int c = c0 + j * kLanes;
           if (ra.ok && c < c1) {
             p.out[ra.base + (long long)(nt * BN + c) * ra.col_stride] = sum[j] * inv_scale;
-            top = max(top, amax_bits(sum[j] * inv_scale));
+            top = max(top, amax_key(sum[j] * inv_scale));
           }
         }
       }
@@ -1767,7 +1767,7 @@ __device__ __forceinline__ void reduce_tile(const GemmParams& p, int tile, int p
     const int n = nt * BN + c0 + q;
     if (ra.ok && n < p.N) {
       p.out[ra.base + (long long)n * ra.col_stride] = sum[q] * inv_scale;
-      top = max(top, amax_bits(sum[q] * inv_scale));
+      top = max(top, amax_key(sum[q] * inv_scale));
     }
   }
   if (!p.amax) return;
@@ -1843,7 +1843,7 @@ __global__ void __launch_bounds__(256) reduce_gated_kernel(const __grid_constant
     if (p.gates) { p.gates[(long long)m * 2 * F + f + q] = g; p.gates[(long long)m * 2 * F + F + f + q] = v; }
     v *= gate_value_of(p.activation, g);
     p.out[(long long)m * F + f + q] = v;
-    top = max(top, finite_bits(v));
+    top = max(top, amax_key(v));
   }
   if (!p.amax) return;
   top = __reduce_max_sync(0xffffffffu, top);
@@ -1877,13 +1877,13 @@ __global__ void barrier_timeout_probe_kernel(long long limit_cycles, int* err) {
 // ------------------------------------------------------------------------------------------------
 // packing kernels (fp32 -> power-of-two scale + hi / lo fp16 pair)
 // ------------------------------------------------------------------------------------------------
-// Largest magnitude of a tensor, as the bit pattern of a non-negative float (unsigned order = float order).
+// Largest finite magnitude of a tensor, as amax_key() writes it.
 __global__ void __launch_bounds__(256) amax_kernel(const float* __restrict__ src, long long n, uint32_t* __restrict__ amax) {
   grid_dep_sync();
   uint32_t m = 0;
   const long long stride = (long long)gridDim.x * blockDim.x, tid = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   auto fold = [&](float4 v) {
-    m = max(max(m, __float_as_uint(fabsf(v.x))), max(__float_as_uint(fabsf(v.y)), max(__float_as_uint(fabsf(v.z)), __float_as_uint(fabsf(v.w)))));
+    m = max(max(m, amax_key(v.x)), max(amax_key(v.y), max(amax_key(v.z), amax_key(v.w))));
   };
   if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
     const float4* s4 = reinterpret_cast<const float4*>(src);
@@ -1894,9 +1894,9 @@ __global__ void __launch_bounds__(256) amax_kernel(const float* __restrict__ src
       fold(a); fold(b); fold(c); fold(d);
     }
     for (; i < n4; i += stride) fold(__ldg(s4 + i));
-    for (long long k = n4 * 4 + tid; k < n; k += stride) m = max(m, __float_as_uint(fabsf(__ldg(src + k))));
+    for (long long k = n4 * 4 + tid; k < n; k += stride) m = max(m, amax_key(__ldg(src + k)));
   } else {
-    for (long long i = tid; i < n; i += stride) m = max(m, __float_as_uint(fabsf(__ldg(src + i))));
+    for (long long i = tid; i < n; i += stride) m = max(m, amax_key(__ldg(src + i)));
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -1907,9 +1907,9 @@ __global__ void __launch_bounds__(256) amax_kernel(const float* __restrict__ src
 // keep: where the maximum in force is left for other packs of the same tensor.
 struct ScaleRef { const uint32_t* amax_cur; uint32_t* amax_next; float* scale; uint32_t* keep; };
 // s = 2^(14 - floor(log2 amax)): amax * s lies in [2^14, 2^15), below the fp16 maximum 65504 after rounding
-__device__ __forceinline__ float scale_from_amax(uint32_t bits) {
-  int e = (int)((bits >> 23) & 0xff);
-  if (bits == 0 || e == 0xff) return 1.f;             // all zero, or Inf/NaN inside (the results are meaningless then)
+__device__ __forceinline__ float scale_from_amax(uint32_t key) {
+  if (key <= kAmaxZero) return 1.f;                   // nothing but zeros, infinities and NaN
+  int e = (int)((key - kAmaxZero) >> 24);
   if (e == 0) e = 1;
   int se = 14 - (e - 127);
   se = se > 120 ? 120 : (se < -120 ? -120 : se);
@@ -2084,7 +2084,7 @@ template <int ACT> __global__ void __launch_bounds__(256, 5) operand_max_kernel(
         constexpr int N = decltype(n)::value;
         each_gradient<ACT, N>(o, first, stride, [&](long long, int, const float* dg, const float* dv) {
 #pragma unroll
-          for (int q = 0; q < N; ++q) top = max(top, max(finite_bits(dg[q]), finite_bits(dv[q])));
+          for (int q = 0; q < N; ++q) top = max(top, max(amax_key(dg[q]), amax_key(dv[q])));
         });
       });
     }
@@ -2093,7 +2093,7 @@ template <int ACT> __global__ void __launch_bounds__(256, 5) operand_max_kernel(
     long long done = 0;
     if ((reinterpret_cast<uintptr_t>(o.src) & 15) == 0) {
       const float4* const s4 = reinterpret_cast<const float4*>(o.src);
-      auto fold = [&](float4 v) { top = max(max(top, finite_bits(v.x)), max(finite_bits(v.y), max(finite_bits(v.z), finite_bits(v.w)))); };
+      auto fold = [&](float4 v) { top = max(max(top, amax_key(v.x)), max(amax_key(v.y), max(amax_key(v.z), amax_key(v.w)))); };
       long long i = first;
       for (; i + 3 * stride < n / 4; i += 4 * stride) {       // four independent 16-byte loads in flight per thread
         const float4 a = __ldg(s4 + i), b = __ldg(s4 + i + stride), c = __ldg(s4 + i + 2 * stride), d = __ldg(s4 + i + 3 * stride);
@@ -2102,7 +2102,7 @@ template <int ACT> __global__ void __launch_bounds__(256, 5) operand_max_kernel(
       for (; i < n / 4; i += stride) fold(__ldg(s4 + i));
       done = n / 4 * 4;
     }
-    for (long long k = done + first; k < n; k += stride) top = max(top, finite_bits(__ldg(o.src + k)));
+    for (long long k = done + first; k < n; k += stride) top = max(top, amax_key(__ldg(o.src + k)));
   }
   top = __reduce_max_sync(0xffffffffu, top);
   if ((threadIdx.x & 31) == 0 && top) atomicMax(o.max, top);
@@ -2211,7 +2211,7 @@ __global__ void __launch_bounds__(256) pack_nchw_kernel(const float* __restrict_
         for (int k = 0; k < TC / 8; ++k) {
           const float x = v[k];
           if (MODE == kPackRelu) v[k] = x > 0.f ? x : (x != x ? x : 0.f);    // NaN propagates
-          if (8 * k < avail) { *yp = v[k]; m = max(m, amax_bits(v[k])); }
+          if (8 * k < avail) { *yp = v[k]; m = max(m, amax_key(v[k])); }
           yp += step;
         }
       }

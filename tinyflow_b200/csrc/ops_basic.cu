@@ -57,7 +57,7 @@ __device__ __forceinline__ bool arrives_last(uint32_t* counter, uint32_t blocks)
 template <class F, class = void> struct TracksAmax { static constexpr bool value = false; };
 template <class F> struct TracksAmax<F, decltype((void)F::kTrackAmax)> { static constexpr bool value = F::kTrackAmax; };
 __device__ __forceinline__ uint32_t amax4(uint32_t m, const float4& r) {
-  return max(max(m, amax_bits(r.x)), max(amax_bits(r.y), max(amax_bits(r.z), amax_bits(r.w))));
+  return max(max(m, amax_key(r.x)), max(amax_key(r.y), max(amax_key(r.z), amax_key(r.w))));
 }
 // Functors with begin() and end(): one thread of the launch calls them around its elements, end() with what begin() read, so that the read
 // is in flight meanwhile (a kernel of one wave would otherwise end with it).
@@ -77,7 +77,7 @@ template <class F> __global__ void __launch_bounds__(kBlock) map1_kernel(const f
     o4[i] = x;
     if (TracksAmax<F>::value) m = amax4(m, x);
   }
-  for (int64_t i = (nv << 2) + (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += stride) { float r = f(a[i]); o[i] = r; if (TracksAmax<F>::value) m = max(m, amax_bits(r)); }
+  for (int64_t i = (nv << 2) + (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += stride) { float r = f(a[i]); o[i] = r; if (TracksAmax<F>::value) m = max(m, amax_key(r)); }
   if constexpr (HasBegin<F>::value) if (blockIdx.x == 0 && threadIdx.x == 0) f.end(word);
   if (TracksAmax<F>::value) amax_commit(am, m);
 }
@@ -98,7 +98,7 @@ template <class F> __global__ void __launch_bounds__(kBlock) map2_kernel(const f
     o4[i] = r;
     if (TracksAmax<F>::value) m = amax4(m, r);
   }
-  for (int64_t i = (nv << 2) + (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += stride) { float r = f(a[i], b[i]); o[i] = r; if (TracksAmax<F>::value) m = max(m, amax_bits(r)); }
+  for (int64_t i = (nv << 2) + (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += stride) { float r = f(a[i], b[i]); o[i] = r; if (TracksAmax<F>::value) m = max(m, amax_key(r)); }
   if (TracksAmax<F>::value) amax_commit(am, m);
 }
 template <class F> __global__ void __launch_bounds__(kBlock) map2_scalar_kernel(const float* a, const float* b, float* o, int64_t n, F f) {
@@ -119,7 +119,7 @@ template <class F> __global__ void __launch_bounds__(kBlock) map3_kernel(const f
     o4[i] = r;
     if (TracksAmax<F>::value) m = amax4(m, r);
   }
-  for (int64_t i = (nv << 2) + (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += stride) { float r = f(a[i], b[i], c[i]); o[i] = r; if (TracksAmax<F>::value) m = max(m, amax_bits(r)); }
+  for (int64_t i = (nv << 2) + (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += stride) { float r = f(a[i], b[i], c[i]); o[i] = r; if (TracksAmax<F>::value) m = max(m, amax_key(r)); }
   if (TracksAmax<F>::value) amax_commit(am, m);
 }
 template <class F> __global__ void __launch_bounds__(kBlock) map3_scalar_kernel(const float* a, const float* b, const float* c, float* o, int64_t n, F f) {
@@ -500,7 +500,7 @@ template <int MODE> __global__ void __launch_bounds__(kBlock) loss_grad_kernel(c
 // V = float4 when all sizes and offsets are multiples of 4 floats, else float.  HBM-bound; kCopyUnroll independent loads a
 // thread, because one at a time left the small tensors of a late module waiting for memory.
 __device__ __forceinline__ uint32_t amax_of(const float4& v) { return amax4(0u, v); }
-__device__ __forceinline__ uint32_t amax_of(float v) { return amax_bits(v); }
+__device__ __forceinline__ uint32_t amax_of(float v) { return amax_key(v); }
 constexpr int kCopyUnroll = 4;
 template <typename V> __global__ void __launch_bounds__(kBlock) concat_kernel(const V* __restrict__ a, const V* __restrict__ b, V* __restrict__ whole, int64_t nrows, int64_t ia, int64_t ib, AmaxOut am) {
   grid_dep_sync();
@@ -588,7 +588,7 @@ __global__ void __launch_bounds__(kBlock) dropout_kernel(const float* __restrict
   for (int64_t i = (nv << 2) + tid; i < n; i += stride) {
     const float r = uniform01(seed, (unsigned long long)i) >= p ? in[i] * scale : 0.f;
     out[i] = r;
-    m = max(m, amax_bits(r));
+    m = max(m, amax_key(r));
   }
   amax_commit(am, m);
 }
@@ -633,7 +633,7 @@ template <bool ADAM> __global__ void __launch_bounds__(kBlock) multi_update_kern
     } else {
       w = sgd(w, g);
     }
-    big = max(big, amax_bits(w));
+    big = max(big, amax_key(w));
   };
   const long long v1 = e.vec ? i0 + ((i1 - i0) & ~3ll) : i0;
   for (long long i = i0 + 4 * threadIdx.x; i < v1; i += 4 * kBlock) {
@@ -768,7 +768,7 @@ __global__ void __launch_bounds__(kBlock) bias_kernel(const float* __restrict__ 
       if (!sum) continue;
       const float t = x[i] + b;
       sum[i] = t;
-      if (relu_out) { const float u = relu(t); relu_out[i] = u; m = max(m, amax_bits(u)); }
+      if (relu_out) { const float u = relu(t); relu_out[i] = u; m = max(m, amax_key(u)); }
     }
   }
   amax_commit(am, m);
@@ -824,7 +824,7 @@ __global__ void __launch_bounds__(kBlock) add_relu_kernel(const float* __restric
   for (int64_t i = (nv << 2) + (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += stride) {
     const float t = a[i] + b[i], u = relu(t);
     sum[i] = t; r[i] = u;
-    m = max(m, amax_bits(u));
+    m = max(m, amax_key(u));
   }
   amax_commit(am, m);
 }

@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(kThreads) gate_kernel(const float* __restrict_
       get<VEC>(g, zr + c);
       get<VEC>(v, zr + F + c);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) { v[j] *= gate_value<ACT>(g[j]); m = max(m, finite_bits(v[j])); }
+      for (int j = 0; j < VEC; ++j) { v[j] *= gate_value<ACT>(g[j]); m = max(m, amax_key(v[j])); }
       put<VEC>(out + row * F + c, v);
     }
   }
@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(kThreads) gate_gradient_kernel(const float* __
         gate_slope<ACT>(g[j], value, slope);
         g[j] = d[j] * v[j] * slope;
         v[j] = d[j] * value;
-        m = max(m, max(finite_bits(g[j]), finite_bits(v[j])));
+        m = max(m, max(amax_key(g[j]), amax_key(v[j])));
       }
       put<VEC>(dz + at + c, g);
       put<VEC>(dz + at + F + c, v);

@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(256) maxpool_fwd_kernel(const float* __restric
     v = a < 0 ? 0.f : v;
     if (y) y[i] = v;
     if (idx) idx[i] = a;
-    amax = max(amax, amax_bits(v));
+    amax = max(amax, amax_key(v));
   }
   amax_commit(am, amax);
 }
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(256) pool_bwd_gather_kernel(const int32_t* __r
         }
     }
     dx[i] = acc * scale;
-    top = max(top, amax_bits(acc * scale));
+    top = max(top, amax_key(acc * scale));
   }
   amax_commit(am, top);
 }
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(256) maxpool_bwd_3x3s2_kernel(const int32_t* _
 #pragma unroll
         for (int k = 0; k < 4; ++k) acc += id[k] == hw ? v[k] : 0.f;
         o[c] = acc;
-        top = max(top, amax_bits(acc));           // (0 past the last column: no index names it)
+        top = max(top, amax_key(acc));           // (0 past the last column: no index names it)
       }
       if (w0 + 1 < W) {
         if ((W & 1) == 0) *reinterpret_cast<float2*>(xp + h * W + w0) = make_float2(o[0], o[1]);
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(256) maxpool_bwd_2x2s2_kernel(const int32_t* _
     split_index(i, dPQ, dQ, plane, p, q);
     const int id = __ldg(idx + plane * PQ + p * Q + q);
     const float v = __ldg(dy + plane * PQ + p * Q + q);
-    top = max(top, amax_bits(v));
+    top = max(top, amax_key(v));
     float* xp = dx + plane * HW;
     const int h0 = 2 * p, w0 = 2 * q;
     const int h_end = p == P - 1 ? H : h0 + 2, w_end = q == Q - 1 ? W : w0 + 2;     // the last windows also clear the leftover edge
@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(256) avgpool_fwd_kernel(const float* __restric
       }
     }
     y[i] = acc * inv;
-    amax = max(amax, amax_bits(acc * inv));
+    amax = max(amax, amax_key(acc * inv));
   }
   amax_commit(am, amax);
 }
@@ -338,8 +338,8 @@ __global__ void __launch_bounds__(256) mean3_kernel(const float* __restrict__ x,
       if (h0 + k >= H) break;
       const float2 below = row(h0 + k + 1), v = make_float2((above.x + here.x + below.x) * scale, (above.y + here.y + below.y) * scale);
       out[k * W] = v.x;
-      top = max(top, amax_bits(v.x));
-      if (right) { out[k * W + 1] = v.y; top = max(top, amax_bits(v.y)); }
+      top = max(top, amax_key(v.x));
+      if (right) { out[k * W + 1] = v.y; top = max(top, amax_key(v.y)); }
       above = here; here = below;
     }
   }
@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(32 * G) bn_pa_fwd_regs_kernel(const float* __r
       V t;
       float* tp = reinterpret_cast<float*>(&t);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) { tp[k] = (v[i][k] - mean[k]) * inv[k]; amax = max(amax, amax_bits(tp[k])); }
+      for (int k = 0; k < VEC; ++k) { tp[k] = (v[i][k] - mean[k]) * inv[k]; amax = max(amax, amax_key(tp[k])); }
       yv[(int64_t)n * FV + fv] = t;
     }
   }
@@ -557,7 +557,7 @@ __global__ void __launch_bounds__(32 * G) bn_pa_bwd_regs_kernel(const float* __r
       V t;
       float* tp = reinterpret_cast<float*>(&t);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) { tp[k] = inv[k] * (g[i][k] - s1[k] * rn - xh[i][k] * s2[k] * rn); amax = max(amax, amax_bits(tp[k])); }
+      for (int k = 0; k < VEC; ++k) { tp[k] = inv[k] * (g[i][k] - s1[k] * rn - xh[i][k] * s2[k] * rn); amax = max(amax, amax_key(tp[k])); }
       ov[(int64_t)n * FV + fv] = t;
     }
   }
@@ -628,7 +628,7 @@ __global__ void __launch_bounds__(32 * G) bn_pa_bwd_relu_regs_kernel(const float
       V t;
       float* tp = reinterpret_cast<float*>(&t);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) { tp[k] = inv[k] * (g[i][k] - s1[k] * rn - xh[i][k] * s2[k] * rn); amax = max(amax, amax_bits(tp[k])); }
+      for (int k = 0; k < VEC; ++k) { tp[k] = inv[k] * (g[i][k] - s1[k] * rn - xh[i][k] * s2[k] * rn); amax = max(amax, amax_key(tp[k])); }
       ov[(int64_t)n * FV + fv] = t;
     }
   }

@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(G * R) norm_fwd_kernel(const NormArgs a) {
       }
     }
   }
-  amax_commit(a.am, __float_as_uint(m));
+  amax_commit(a.am, amax_key(m));
 }
 
 template <int BYTES> __device__ __forceinline__ void copy_ahead(uint32_t to, const float* from) {
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) norm_bwd_kernel(const NormArgs
     }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
-  amax_commit(a.am, __float_as_uint(m));
+  amax_commit(a.am, amax_key(m));
   const bool direct = a.dgamma || a.dbeta;
   if (!a.part && !direct) return;
   __syncthreads();
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) norm_wide_bwd_kernel(const No
     }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
-  amax_commit(a.am, __float_as_uint(m));
+  amax_commit(a.am, amax_key(m));
   if (!a.part) return;
   float* const out = a.part + (int64_t)blockIdx.x * 2 * D;
 #pragma unroll
@@ -521,7 +521,7 @@ template <bool RES> __global__ void __launch_bounds__(kLongThreads) norm_long_fw
     for (int c = threadIdx.x; c < D; c += kLongThreads) {
       const float y = fmaf((x[c] - mean) * inv, a.gamma[c], a.beta[c]);
       a.y[base + c] = y;
-      m = max(m, finite_bits(y));
+      m = max(m, amax_key(y));
     }
   }
   amax_commit(a.am, m);
@@ -556,9 +556,9 @@ template <bool RES> __global__ void __launch_bounds__(kLongThreads) norm_long_bw
       if (RES && a.dsum) d += a.dsum[row * D + c];
       if (a.dx) {
         a.dx[row * D + c] = d;
-        if (!RES || !a.dbranch) m = max(m, finite_bits(d));
+        if (!RES || !a.dbranch) m = max(m, amax_key(d));
       }
-      if (RES && a.dbranch) { d = dropped(a, mix_start(seed, row * D + c), d); a.dbranch[row * D + c] = d; m = max(m, finite_bits(d)); }
+      if (RES && a.dbranch) { d = dropped(a, mix_start(seed, row * D + c), d); a.dbranch[row * D + c] = d; m = max(m, amax_key(d)); }
     }
   }
   amax_commit(a.am, m);
