@@ -150,3 +150,147 @@ def test_a_weight_that_is_not_finite_leaves_the_other_columns_their_bits(env, ru
         rest = np.arange(clean.shape[1]) != column
         assert np.isfinite(clean).all() and not np.isfinite(got[:, column]).all()
         np.testing.assert_array_equal(got[:, rest], clean[:, rest])
+
+
+# ---- arrays that a graph of the caller's own writes -------------------------------------------------------------------
+def into(env, kind, x, y, stream):
+    """The call that writes y (M x K) from x of that size."""
+    op, ones = env.gpu_op, env.ones
+    as4 = lambda a, *s: view(env, a, 0, s)                 # noqa: E731
+    if kind == "relu":
+        cell = op.activation_get_cudnnlist((M, K), "NCHW", "relu")
+        return lambda: op.activation_forward(x, y, "relu", cell, env.cudnn, stream)
+    if kind == "dropout":
+        inputd = op.get_input_descriptor((M, K), "NCHW")
+        return lambda: op.dropout_forward(x, y, "NCHW", 0.3, 5, inputd, env.cudnn, stream)
+    if kind == "concat":
+        a, b, whole = as4(x, M, K // 2, 1, 1), as4(x, M, K // 2, 1, 1), as4(y, M, K, 1, 1)
+        return lambda: op.concat_forward(a, b, whole, stream)
+    if kind == "mean":
+        _, cell = op.pooling_2d_forward_get_out_shape((M, 8, 8, 8), "NCHW", "mean", 1, 1, 1, 1, 3, 3)
+        return lambda: op.pooling_2d_forward(as4(x, M, 8, 8, 8), as4(y, M, 8, 8, 8), cell, env.cudnn, stream)
+    if kind == "norm":                                     # gamma is what sizes its result
+        gamma = view(env, x, 0, (K,))
+        return lambda: op.layer_norm_forward(env.noise, gamma, gamma, y, 1e-5, stream)
+    if kind == "residual norm":
+        gamma, total, state = view(env, x, 0, (K,)), env.empty((M, K)), op.dropout_state(0.2, 3)
+        return lambda: op.dropout_add_layer_norm_forward(env.noise, env.noise, gamma, gamma, total, y, state, 1e-5, stream)
+    if kind == "norm gradient":
+        return lambda: op.layer_norm_backward(env.noise, ones, x, y, None, None, 1e-5, stream)
+    if kind == "gated small":                              # one launch of the CUDA-core kernel
+        a, w = view(env, x, 0, (M, 8)), env.weight8
+        return lambda: op.gated_linear_forward(a, w, None, y, "relu", stream)
+    if kind == "gated":
+        return lambda: op.gated_linear_forward(x, env.weight, None, y, "relu", stream)
+    if kind == "copy":
+        return lambda: op.copy_on_stream(x, y, stream)
+    assert kind == "sum of squares"
+    return lambda: op.matrix_elementwise_multiply(x, ones2(env, x), y, stream)
+
+
+def ones2(env, like):
+    if not hasattr(env, "ones_"):
+        env.ones_ = env.dev(np.ones((M, K)))
+    return env.ones_
+
+
+@pytest.fixture(scope="module")
+def stage(env):
+    rng = np.random.RandomState(2)
+    env.ones = env.dev(np.ones(K))
+    env.noise = env.dev(rng.randn(M, K))
+    env.weight8, env.weight = env.dev(rng.randn(8, 2 * K)), env.dev(rng.randn(K, 2 * K) * K ** -0.5)
+    ones2(env, None)
+    return env
+
+
+KINDS = ["relu", "dropout", "concat", "mean", "norm", "residual norm", "norm gradient", "gated small", "gated", "copy", "sum of squares"]
+
+
+def capture(call_on):
+    """A graph of call_on(stream cell)() on a stream of its own."""
+    import torch
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    cell = ctypes.pointer(ctypes.c_void_p(side.cuda_stream))
+    call = call_on(cell)
+    with torch.cuda.graph(graph, stream=side):
+        call()
+    graph.side = side
+    return graph
+
+
+def replay(graph):
+    import torch
+    graph.replay()
+    torch.cuda.synchronize()
+
+
+def same_as_a_copy(env, y, what):
+    """What reads y has the bits that it has on an uploaded copy of y."""
+    results = []
+    rng = np.random.RandomState(8)
+    w, dout = (rng.randn(K, 2 * F) * K ** -0.5).astype(np.float32), (0.1 * rng.randn(M, F)).astype(np.float32)
+    for X in (y, env.dev(y.asnumpy())):
+        got, dw = layer(env, X, w, dout)
+        results.append(dict(got, dweight=dw))
+    for name, v in results[0].items():
+        assert np.isfinite(v).all(), (what, name)
+        np.testing.assert_array_equal(v, results[1][name], err_msg="%s, %s" % (what, name))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("sizes", [(1.0, 1e4), (1e4, 1.0), (1e-3, 1e3)])
+def test_a_replay_that_rewrites_an_array(stage, kind, sizes):
+    """Ordinary call, then a replay of the same call on numbers of another size, and the same the other way round: what reads the array
+    afterwards scales by what is there."""
+    env = stage
+    rng = np.random.RandomState(4)
+    x, y = env.empty((M, K)), env.empty((M, K))
+    numbers = rng.randn(M, K).astype(np.float32)
+
+    def fill(size):
+        x[:] = numbers * np.float32(size)
+
+    fill(sizes[0])
+    ordinary = into(env, kind, x, y, env.stream)
+    for _ in range(2):
+        ordinary()
+    env.gpu_op.device_synchronize()
+    graph = capture(lambda cell: into(env, kind, x, y, cell))
+    for turn in range(3):
+        fill(sizes[0])
+        ordinary()                                         # leaves what it knows of y
+        if turn:
+            same_as_a_copy(env, y, "ordinary, turn %d" % turn)
+        fill(sizes[1])
+        replay(graph)
+        same_as_a_copy(env, y, "replayed, turn %d" % turn)
+        fill(sizes[0])
+        replay(graph)
+        same_as_a_copy(env, y, "replayed again, turn %d" % turn)
+
+
+def test_an_array_in_the_place_of_one_that_a_replay_wrote(stage):
+    """Freed memory has nothing of its past: what is written there by ordinary calls hands its maximum on again (a launch less)."""
+    env = stage
+    w, h = by_relu(env, np.ones((K, 2 * F), np.float32)), env.empty((M, F))
+    x = env.dev(np.random.RandomState(5).randn(M, K))
+
+    def launches(y):
+        into(env, "relu", x, y, env.stream)()
+        before = env.gpu_op.launch_count()
+        env.gpu_op.gated_linear_forward(y, w, None, h, "relu", env.stream)
+        return env.gpu_op.launch_count() - before
+
+    y = env.empty((M, K))
+    clean = launches(y)
+    graph = capture(lambda cell: into(env, "relu", x, y, cell))
+    assert launches(y) == clean + 1
+    at = y.data_ptr
+    del graph
+    y.free_gpu()
+    taken = []
+    while not taken or taken[-1].data_ptr != at:
+        taken.append(env.empty((M, K)))
+        assert len(taken) < 100
+    assert launches(taken[-1]) == clean

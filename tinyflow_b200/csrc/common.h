@@ -78,16 +78,30 @@ int launch_deferred_now(const DeferredOp& op);                  // the plain ele
 long long fused_relu_bn_bwd_count();
 long long fused_add_relu_count();
 
-inline cudaStream_t stream_of(void** cell) { flush_deferred(); return cell ? (cudaStream_t)(*cell) : (cudaStream_t)0; }
+// Whether the caller is capturing the present call's stream.  What the call launches then runs at the caller's replays, unseen by the host: nothing
+// is tracked, taken over from earlier calls or left to later ones, and the arrays that it writes count as rewritten at any time from then on.
+extern thread_local bool t_captured;
+inline cudaStream_t enter_call(cudaStream_t s);
+
+inline cudaStream_t stream_of(void** cell) { flush_deferred(); return enter_call(cell ? (cudaStream_t)(*cell) : (cudaStream_t)0); }
 cudaStream_t legacy_stream();               // of the operators that the reference runs without a stream: the legacy default stream, in a recording the recording's
-inline cudaStream_t stream_of_keep_deferred(void** cell) { return cell ? (cudaStream_t)(*cell) : (cudaStream_t)0; }
+inline cudaStream_t stream_of_keep_deferred(void** cell) { return enter_call(cell ? (cudaStream_t)(*cell) : (cudaStream_t)0); }
+inline bool capturing(cudaStream_t s) {
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(s, &capture) == cudaSuccess) return capture != cudaStreamCaptureStatusNone;
+  cudaGetLastError();
+  return true;
+}
+inline cudaStream_t enter_call(cudaStream_t s) { t_captured = !t_recording && capturing(s); return s; }
 void note_compute_stream(cudaStream_t s);   // remembered so side-stream copies can order after compute
 cudaStream_t last_compute_stream();         // launches a held-back kernel first
 
 // ---- write versions -------------------------------------------------------------
 // Every entry point that writes a device array bumps the version of its data pointer; cached
-// derived data (packed tensor-core operands) is valid only while the version is unchanged.
+// derived data (packed tensor-core operands) is valid only while the version is unchanged.  Inside a caller's capture, and for an array that a
+// captured call has written, version_of() is another number at every call, until the array is freed.  (A call knows its stream before it writes.)
 void note_write(const void* p);
+void note_free(const void* p);
 uint64_t version_of(const void* p);
 inline float* out_f32(DLArray* a) { note_write(a->data); return (float*)a->data; }
 void invalidate_all_versions();             // every tensor counts as rewritten (a recording was abandoned)
@@ -100,10 +114,8 @@ void invalidate_all_versions();             // every tensor counts as rewritten 
 // writes (the kernel of write k clears the word write k+1 will use), so no clearing launch is needed.
 struct AmaxOut { uint32_t* word = nullptr; uint32_t* clear = nullptr; };
 AmaxOut amax_track_begin(const void* data);
-// A graph that the caller captures replays the kernels and not what is kept on the host: a word that an earlier call left may be cleared or
-// belong to other data by then, and one that the graph fills is not cleared between replays.  Inside one, nothing is tracked or taken.
-bool stream_captured(cudaStream_t s);
-inline AmaxOut amax_track_begin_on(const void* data, cudaStream_t s) { return stream_captured(s) ? AmaxOut{} : amax_track_begin(data); }
+// (Inside a caller's capture there are no words: one that an earlier call left may be cleared or belong to other data at a replay, and one that
+// the graph fills would not be cleared between replays.)
 const uint32_t* amax_tracked(const void* data);
 // The maximum of a tensor that a recorded step reads before it writes it (see step_graph.cu): `carry` keeps the value
 // between replays, valid while the tensor's version is `*version`.

@@ -330,7 +330,7 @@ int gated_small_fwd(const float* x, const float* w, float* gates, float* out, in
   const unsigned across = (unsigned)((F + kTile - 1) / kTile), down = (unsigned)((M + kTile - 1) / kTile);
   const int cluster = cluster_for((long long)across * down, (K + kDepth - 1) / kDepth, 3 * device_sm_count(), 8);
   p.per_cta = (int)(((K + cluster - 1) / cluster + kDepth - 1) / kDepth * kDepth);
-  p.am = amax_track_begin_on(out, s);
+  p.am = amax_track_begin(out);
   note_compute_stream(s);
   KernelTimer kt("gated_small_fwd", s, 4.0 * M * F * K, 0, 1);
   cudaError_t e = cudaSuccess;

@@ -514,7 +514,7 @@ template <int MR, bool VEC> static int launch_rows_gated(RowsGated q, int activa
   while (cluster < 8 && groups * cluster < sms && p.K >= 32 * kRowWarps * cluster) { cluster *= 2; cut(); }
   if (smem() > kRowSmem || groups * cluster < sms) return 0;
   KernelTimer kt("rows_gated", s, 4.0 * (double)p.M * q.F * p.K, 0, 1);
-  q.am = amax_track_begin_on(q.out, s);
+  q.am = amax_track_begin(q.out);
   cudaError_t e = cudaSuccess;
   with_gate(activation, [&](auto act) {
     constexpr int ACT = decltype(act)::value;

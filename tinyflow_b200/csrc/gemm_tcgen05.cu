@@ -50,12 +50,28 @@ namespace tf {
 static std::mutex g_ver_mu;
 static std::unordered_map<const void*, uint64_t> g_versions;
 static uint64_t g_ver_counter = 1;
+constexpr uint64_t kRewrittenAnyTime = 0;              // by the replays of a graph that the caller captured
+static bool captured_locked(const void* p) {
+  if (t_captured) return true;
+  auto it = g_versions.find(p);
+  return it != g_versions.end() && it->second == kRewrittenAnyTime;
+}
 static uint64_t version_locked(const void* p) {
+  if (captured_locked(p)) return ++g_ver_counter;
   auto it = g_versions.find(p);
   if (it == g_versions.end()) { g_versions[p] = ++g_ver_counter; return g_ver_counter; }
   return it->second;
 }
+static void bump_locked(const void* p) {
+  if (t_captured) g_versions[p] = kRewrittenAnyTime;
+  else if (!captured_locked(p)) g_versions[p] = ++g_ver_counter;
+}
 void note_write(const void* p) {
+  if (t_recording) recording_note_write(p);
+  std::lock_guard<std::mutex> lk(g_ver_mu);
+  bump_locked(p);
+}
+void note_free(const void* p) {
   if (t_recording) recording_note_write(p);
   std::lock_guard<std::mutex> lk(g_ver_mu);
   g_versions[p] = ++g_ver_counter;
@@ -66,11 +82,11 @@ uint64_t version_of(const void* p) {
 }
 void bump_versions(const void* const* ptrs, size_t n) {
   std::lock_guard<std::mutex> lk(g_ver_mu);
-  for (size_t i = 0; i < n; ++i) g_versions[ptrs[i]] = ++g_ver_counter;
+  for (size_t i = 0; i < n; ++i) bump_locked(ptrs[i]);
 }
 void invalidate_all_versions() {
   std::lock_guard<std::mutex> lk(g_ver_mu);
-  for (auto& kv : g_versions) kv.second = ++g_ver_counter;
+  for (auto& kv : g_versions) if (kv.second != kRewrittenAnyTime) kv.second = ++g_ver_counter;
 }
 
 // producer-tracked maxima: two device words per tensor, handed out from zero-filled chunks.  A third word per tensor
@@ -83,7 +99,8 @@ struct AmaxSlot {
 };
 static std::unordered_map<const void*, AmaxSlot> g_amax;
 // A key is an array's address, or an odd address in its first word (bound_key): such a word is as old as the array, whoever writes that.
-static uint64_t array_version_locked(const void* key) { return version_locked(reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(key) & ~uintptr_t(3))); }
+static const void* array_of(const void* key) { return reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(key) & ~uintptr_t(3)); }
+static uint64_t array_version_locked(const void* key) { return version_locked(array_of(key)); }
 struct AmaxChunk { uint32_t* next = nullptr; int left = 0; };
 static AmaxChunk g_amax_chunk[64];            // of every device: its kernels write there
 static uint32_t* amax_chunk_words(int n) {
@@ -108,6 +125,7 @@ static void amax_enter_recording(AmaxSlot& sl) {
 }
 AmaxOut amax_track_begin(const void* data) {
   std::lock_guard<std::mutex> lk(g_ver_mu);
+  if (captured_locked(array_of(data))) return AmaxOut{};
   AmaxSlot& sl = g_amax[data];
   if (t_recording) {
     amax_enter_recording(sl);
@@ -2663,13 +2681,6 @@ void hold_products(bool on) { t_hold = on; }
 bool pause_holding() { const bool was = t_hold; t_hold = false; return was; }
 static void forget_held() { t_held.clear(); t_held_work = 0; t_waiting = false; drop_held_simt(); drop_held_sums(); drop_held_direct(); }
 void drop_held() { forget_held(); t_hold = false; }
-static bool capturing(cudaStream_t s) {
-  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(s, &capture) == cudaSuccess) return capture != cudaStreamCaptureStatusNone;
-  cudaGetLastError();
-  return true;
-}
-bool stream_captured(cudaStream_t s) { return !t_recording && capturing(s); }
 // The call may wait: its caller says so, nothing that waits was called on another stream, and no graph of the caller's own is being
 // captured (it would copy from a table that is gone).  True: the caller holds it now.
 bool may_hold(cudaStream_t s) {
@@ -2980,7 +2991,7 @@ static ScaleRef begin_pack(Pack& pk, const float* src, long long n, cudaStream_t
   r.amax_cur = bound ? bound : fresh;
   if (bound) return r;
   static const bool no_track = getenv("TINYFLOW_NO_AMAX_TRACKING") != nullptr;
-  if (const uint32_t* tracked = no_track || stream_captured(s) ? nullptr : amax_tracked(src)) {
+  if (const uint32_t* tracked = no_track ? nullptr : amax_tracked(src)) {
     r.amax_cur = tracked;               // the producer of src already reduced max|src| in its own pass
     return r;
   }
@@ -3076,7 +3087,7 @@ template <int AR> static int launch_gated(GemmParams& p, cudaStream_t s, double 
     if (oom) *oom = bytes > 0x7fffffffu ? 0x7fffffff : (int)bytes;
     return 1;
   }
-  const AmaxOut am = amax_track_begin_on(p.out, s);           // nothing is short from here on
+  const AmaxOut am = amax_track_begin(p.out);           // nothing is short from here on
   p.amax = am.word; p.amax_clear = am.clear;
   const int grid = plan_smem(p, BN, plan_grid(p), kGatedStage);
   TF_REQUIRE(p.cluster == 1 || BM * BN * 4 <= p.a_slots * p.a_rows * 256 + p.b_slots * BN * 256, "%s: a piece of a tile does not fit where its operands were", what);
@@ -3114,13 +3125,12 @@ struct OperandPacks {
   }
   template <int ACT> int run(StreamLease& lease, cudaStream_t s, const char* what) {
     static const bool no_track = getenv("TINYFLOW_NO_AMAX_TRACKING") != nullptr;
-    const bool captured = stream_captured(s);
     bool reduce = false;
     double bytes = 0;
     if (ar == kArithF16) {
       for (int i = 0; i < all.n; ++i) {
         Operand& o = all.op[i];
-        if (o.kind != kGradient && !no_track && !captured && (o.scale.amax_cur = amax_tracked(o.src))) continue;         // its producer reduced it
+        if (o.kind != kGradient && !no_track && (o.scale.amax_cur = amax_tracked(o.src))) continue;         // its producer reduced it
         if (!all.words && !(all.words = lease.counters(4))) return 1;
         o.scale.amax_cur = o.max = all.words + i;
         reduce = true;

@@ -157,6 +157,11 @@ template <class F> static int run_map3(const float* a, const float* b, const flo
   return 0;
 }
 
+// The output as an array: its write is noted here, where the call's stream is known (arguments are evaluated in any order)
+template <class F> static int run_map1(const float* a, DLArrayHandle o, int64_t n, cudaStream_t s, const char* what, F f) { return run_map1(a, out_f32(o), n, s, what, f); }
+template <class F> static int run_map2(const float* a, const float* b, DLArrayHandle o, int64_t n, cudaStream_t s, const char* what, F f) { return run_map2(a, b, out_f32(o), n, s, what, f); }
+template <class F> static int run_map3(const float* a, const float* b, const float* c, DLArrayHandle o, int64_t n, cudaStream_t s, const char* what, F f) { return run_map3(a, b, c, out_f32(o), n, s, what, f); }
+
 struct FSet { float v; __device__ float operator()(float) const { return v; } };
 struct FAddC { float c; __device__ float operator()(float x) const { return x + c; } };
 struct FMulC { float c; __device__ float operator()(float x) const { return x * c; } };
@@ -845,7 +850,7 @@ extern "C" {
 
 int DLGpuArraySet(DLArrayHandle arr, float value, void** cudaStream) {
   TF_REQUIRE(arr, "null array");
-  return run_map1(F(arr), FM(arr), numel(arr), stream_of(cudaStream), "DLGpuArraySet", FSet{value});
+  return run_map1(F(arr), arr, numel(arr), stream_of(cudaStream), "DLGpuArraySet", FSet{value});
 }
 
 int DLGpuBroadcastTo0(const DLArrayHandle input, DLArrayHandle output, void** cudaStream) {
@@ -1127,56 +1132,56 @@ int DLGpuMatrixElementwiseAdd(const DLArrayHandle matA, const DLArrayHandle matB
     defer_op(DeferredOp{kDeferAdd, F(matA), F(matB), FM(output), numel(output), s, BiasBcast{}});
     return 0;
   }
-  return run_map2(F(matA), F(matB), FM(output), numel(output), s, "DLGpuMatrixElementwiseAdd", FAdd{});
+  return run_map2(F(matA), F(matB), output, numel(output), s, "DLGpuMatrixElementwiseAdd", FAdd{});
 }
 int DLGpuMatrixElementwiseAddByConst(const DLArrayHandle input, float val, DLArrayHandle output, void** cudaStream) {
   TF_SAME(input, output, "DLGpuMatrixElementwiseAddByConst");
-  return run_map1(F(input), FM(output), numel(output), stream_of(cudaStream), "DLGpuMatrixElementwiseAddByConst", FAddC{val});
+  return run_map1(F(input), output, numel(output), stream_of(cudaStream), "DLGpuMatrixElementwiseAddByConst", FAddC{val});
 }
 int DLGpuMatrixElementwiseMultiply(const DLArrayHandle matA, const DLArrayHandle matB, DLArrayHandle output, void** cudaStream) {
   TF_SAME(matA, matB, "DLGpuMatrixElementwiseMultiply"); TF_SAME(matA, output, "DLGpuMatrixElementwiseMultiply");
-  return run_map2(F(matA), F(matB), FM(output), numel(output), stream_of(cudaStream), "DLGpuMatrixElementwiseMultiply", FMul{});
+  return run_map2(F(matA), F(matB), output, numel(output), stream_of(cudaStream), "DLGpuMatrixElementwiseMultiply", FMul{});
 }
 int DLGpuMatrixMultiplyByConst(const DLArrayHandle input, float val, DLArrayHandle output, void** cudaStream) {
   TF_SAME(input, output, "DLGpuMatrixMultiplyByConst");
-  return run_map1(F(input), FM(output), numel(output), stream_of(cudaStream), "DLGpuMatrixMultiplyByConst", FMulC{val});
+  return run_map1(F(input), output, numel(output), stream_of(cudaStream), "DLGpuMatrixMultiplyByConst", FMulC{val});
 }
 // The constant is the one element of a device array: no host read-back in the middle of a step.
 int TfMatrixElementwiseAddByArray(const DLArrayHandle input, const DLArrayHandle scalar, DLArrayHandle output, void** cudaStream) {
   TF_SAME(input, output, "TfMatrixElementwiseAddByArray");
   TF_REQUIRE(scalar && numel(scalar) == 1 && scalar->data != output->data, "TfMatrixElementwiseAddByArray: needs a one-element array that is not the output");
-  return run_map1(F(input), FM(output), numel(output), stream_of(cudaStream), "DLGpuMatrixElementwiseAddByConst", FAddArr{F(scalar)});
+  return run_map1(F(input), output, numel(output), stream_of(cudaStream), "DLGpuMatrixElementwiseAddByConst", FAddArr{F(scalar)});
 }
 int TfMatrixMultiplyByArray(const DLArrayHandle input, const DLArrayHandle scalar, DLArrayHandle output, void** cudaStream) {
   TF_SAME(input, output, "TfMatrixMultiplyByArray");
   TF_REQUIRE(scalar && numel(scalar) == 1 && scalar->data != output->data, "TfMatrixMultiplyByArray: needs a one-element array that is not the output");
-  return run_map1(F(input), FM(output), numel(output), stream_of(cudaStream), "DLGpuMatrixMultiplyByConst", FMulArr{F(scalar)});
+  return run_map1(F(input), output, numel(output), stream_of(cudaStream), "DLGpuMatrixMultiplyByConst", FMulArr{F(scalar)});
 }
 int DLGpuRelu(const DLArrayHandle input, DLArrayHandle output) {
   TF_SAME(input, output, "DLGpuRelu");
   int rc = 0;
   if (t_recording && relu_of_bias_sum(input, output, recording_stream(), &rc)) return rc;
-  return run_map1(F(input), FM(output), numel(output), last_compute_stream(), "DLGpuRelu", FRelu{});
+  return run_map1(F(input), output, numel(output), last_compute_stream(), "DLGpuRelu", FRelu{});
 }
 int DLGpuReluGradient(const DLArrayHandle input, const DLArrayHandle in_grad, DLArrayHandle output) {
   TF_SAME(input, in_grad, "DLGpuReluGradient"); TF_SAME(input, output, "DLGpuReluGradient");
-  return run_map2(F(input), F(in_grad), FM(output), numel(output), last_compute_stream(), "DLGpuReluGradient", FReluGrad{});
+  return run_map2(F(input), F(in_grad), output, numel(output), last_compute_stream(), "DLGpuReluGradient", FReluGrad{});
 }
 int DLGpuMatrixExp(const DLArrayHandle input, DLArrayHandle output) {
   TF_SAME(input, output, "DLGpuMatrixExp");
-  return run_map1(F(input), FM(output), numel(output), last_compute_stream(), "DLGpuMatrixExp", FExp{});
+  return run_map1(F(input), output, numel(output), last_compute_stream(), "DLGpuMatrixExp", FExp{});
 }
 int DLGpuMatrixLog(const DLArrayHandle input, DLArrayHandle output, void** cudaStream) {
   TF_SAME(input, output, "DLGpuMatrixLog");
-  return run_map1(F(input), FM(output), numel(output), stream_of(cudaStream), "DLGpuMatrixLog", FLog{});
+  return run_map1(F(input), output, numel(output), stream_of(cudaStream), "DLGpuMatrixLog", FLog{});
 }
 int DLGpuMatrixReverse(const DLArrayHandle input, DLArrayHandle output) {
   TF_SAME(input, output, "DLGpuMatrixReverse");
-  return run_map1(F(input), FM(output), numel(output), last_compute_stream(), "DLGpuMatrixReverse", FRecip{});
+  return run_map1(F(input), output, numel(output), last_compute_stream(), "DLGpuMatrixReverse", FRecip{});
 }
 int DLGpuMatrixPow(const DLArrayHandle input, const float val, DLArrayHandle output) {
   TF_SAME(input, output, "DLGpuMatrixPow");
-  return run_map1(F(input), FM(output), numel(output), last_compute_stream(), "DLGpuMatrixPow", FPow{val});
+  return run_map1(F(input), output, numel(output), last_compute_stream(), "DLGpuMatrixPow", FPow{val});
 }
 
 int DLGpuSoftmax(const DLArrayHandle input, DLArrayHandle output, void** cudaStream) {
@@ -1204,7 +1209,7 @@ int DLGpuSoftmaxCrossEntropy(const DLArrayHandle input_a, const DLArrayHandle in
 }
 int DLGpuCrossEntropy(const DLArrayHandle input_a, const DLArrayHandle input_b, DLArrayHandle output) {
   TF_SAME(input_a, input_b, "DLGpuCrossEntropy"); TF_SAME(input_a, output, "DLGpuCrossEntropy");
-  return run_map2(F(input_a), F(input_b), FM(output), numel(output), last_compute_stream(), "DLGpuCrossEntropy", FBce{});
+  return run_map2(F(input_a), F(input_b), output, numel(output), last_compute_stream(), "DLGpuCrossEntropy", FBce{});
 }
 static int row_loss(int mode, const DLArrayHandle a, const DLArrayHandle b, DLArrayHandle out, float scale, const char* what) {
   TF_REQUIRE(a && out && a->ndim >= 1 && numel(out) == 1, "%s: bad arguments", what);
@@ -1237,11 +1242,11 @@ int DLGpuL2regularGradient(const DLArrayHandle a, const DLArrayHandle g, DLArray
 
 int DLGpuCross(const DLArrayHandle x, const DLArrayHandle y, DLArrayHandle output, float b, void** cudaStream) {
   TF_SAME(x, y, "DLGpuCross"); TF_SAME(x, output, "DLGpuCross");
-  return run_map2(F(x), F(y), FM(output), numel(output), stream_of(cudaStream), "DLGpuCross", FCross{b});
+  return run_map2(F(x), F(y), output, numel(output), stream_of(cudaStream), "DLGpuCross", FCross{b});
 }
 int DLGpuCrossBackward(const DLArrayHandle x, const DLArrayHandle y, const DLArrayHandle doutput, DLArrayHandle output, float b, void** cudaStream) {
   TF_SAME(x, y, "DLGpuCrossBackward"); TF_SAME(x, output, "DLGpuCrossBackward"); TF_SAME(x, doutput, "DLGpuCrossBackward");
-  return run_map3(F(x), F(y), F(doutput), FM(output), numel(output), stream_of(cudaStream), "DLGpuCrossBackward", FCrossBwd{b});
+  return run_map3(F(x), F(y), F(doutput), output, numel(output), stream_of(cudaStream), "DLGpuCrossBackward", FCrossBwd{b});
 }
 
 static int concat_geom(const DLArrayHandle a, const DLArrayHandle b, int64_t* rows, int64_t* ia, int64_t* ib) {
@@ -1330,7 +1335,7 @@ int DLGpuActivationForward(const DLArrayHandle input, DLArrayHandle output, int 
   }
   cudaStream_t s = stream_of(cudaStream);
   switch (activationMode) {
-    case 0: return run_map1(F(input), FM(output), n, s, "DLGpuActivationForward(sigmoid)", FSigmoid{});
+    case 0: return run_map1(F(input), output, n, s, "DLGpuActivationForward(sigmoid)", FSigmoid{});
     case 1: {
       // when the tensor path is known to pack this output for a convolution next, one kernel writes y and the pack
       const void* node = plan_of<TensorPlan>(cudnnlist, kPlanTensor);
@@ -1344,7 +1349,7 @@ int DLGpuActivationForward(const DLArrayHandle input, DLArrayHandle output, int 
       tc_note_relu_output(node, output->data, input->data, relu.bound.to != nullptr);
       return rc;
     }
-    case 2: return run_map1(F(input), FM(output), n, s, "DLGpuActivationForward(tanh)", FTanh{});
+    case 2: return run_map1(F(input), output, n, s, "DLGpuActivationForward(tanh)", FTanh{});
     case 3: {
       // softmax over all non-batch elements of each sample (src/gpu_op.cu:3238-3248)
       TensorPlan* p = plan_of<TensorPlan>(cudnnlist, kPlanTensor);
@@ -1365,15 +1370,15 @@ int DLGpuActivationBackward(const DLArrayHandle input, DLArrayHandle dinput, con
   cudaStream_t s = stream_of(cudaStream);
   int64_t n = numel(input);
   switch (activationMode) {
-    case 0: return run_map2(F(output), F(doutput), FM(dinput), n, s, "DLGpuActivationBackward(sigmoid)", FSigmoidBwd{});
+    case 0: return run_map2(F(output), F(doutput), dinput, n, s, "DLGpuActivationBackward(sigmoid)", FSigmoidBwd{});
     case 1:
       // Held back for one call: if the batch-norm backward that consumes this gradient comes next, one kernel does both.
       if (deferral_enabled() && n >= (1 << 16)) {
         defer_op(DeferredOp{kDeferReluBwd, F(input), F(doutput), FM(dinput), n, s, BiasBcast{}});
         return 0;
       }
-      return run_map2(F(input), F(doutput), FM(dinput), n, s, "DLGpuActivationBackward(relu)", FReluGrad{});
-    case 2: return run_map2(F(output), F(doutput), FM(dinput), n, s, "DLGpuActivationBackward(tanh)", FTanhBwd{});
+      return run_map2(F(input), F(doutput), dinput, n, s, "DLGpuActivationBackward(relu)", FReluGrad{});
+    case 2: return run_map2(F(output), F(doutput), dinput, n, s, "DLGpuActivationBackward(tanh)", FTanhBwd{});
     case 3: {
       TensorPlan* p = plan_of<TensorPlan>(cudnnlist, kPlanTensor);
       int64_t rows = p ? p->batch : input->shape[0];
@@ -1435,7 +1440,7 @@ int DLGpuSgdUpdate(DLArrayHandle output, const DLArrayHandle m, float b, void** 
   int took = dp_sgd_update(FM(output), F(m), numel(output), b, s);
   if (took < 0) return -1;
   if (took) return 0;
-  return run_map2(F(output), F(m), FM(output), numel(output), s, "DLGpuSgdUpdate", FSgd{b});
+  return run_map2(F(output), F(m), output, numel(output), s, "DLGpuSgdUpdate", FSgd{b});
 }
 int DLGpuAdam_mv(DLArrayHandle m, DLArrayHandle v, const DLArrayHandle g, float b1, float b2, void** cudaStream) {
   TF_SAME(m, g, "DLGpuAdam_mv"); TF_SAME(v, g, "DLGpuAdam_mv");
@@ -1454,10 +1459,11 @@ int DLGpuAdam(DLArrayHandle output, const DLArrayHandle m, const DLArrayHandle v
   TF_SAME(output, m, "DLGpuAdam"); TF_SAME(output, v, "DLGpuAdam");
   TF_REQUIRE(!t_recording, "DLGpuAdam: the bias corrections of a recorded step change from replay to replay (TfAdamUpdateMany)");
   // data-parallel mode: the step joins the pending record of (m, v) and runs behind the all-reduce
-  int took = dp_adam_step(FM(output), F(m), F(v), 1.f - b1t, 1.f - b2t, e, learning_rate, stream_of(cudaStream));
+  const cudaStream_t s = stream_of(cudaStream);
+  int took = dp_adam_step(FM(output), F(m), F(v), 1.f - b1t, 1.f - b2t, e, learning_rate, s);
   if (took < 0) return -1;
   if (took) return 0;
-  return run_map3(F(output), F(m), F(v), FM(output), numel(output), stream_of(cudaStream), "DLGpuAdam", FAdamStep{1.f - b1t, 1.f - b2t, e, learning_rate});
+  return run_map3(F(output), F(m), F(v), output, numel(output), s, "DLGpuAdam", FAdamStep{1.f - b1t, 1.f - b2t, e, learning_rate});
 }
 
 // The update of many tensors: what DLGpuSgdUpdate / DLGpuAdam_mv + DLGpuAdam do for each, in one launch.  Not for

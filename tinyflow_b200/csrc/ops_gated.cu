@@ -190,7 +190,7 @@ int TfGatedLinearForward(const DLArrayHandle input, const DLArrayHandle weight, 
   if (matmul_any((const float*)input->data, false, (const float*)weight->data, false, z, M, 2 * F, K, s, what)) return -1;
   note_compute_stream(s);
   KernelTimer kt(what, s, 0, 12.0 * M * F);
-  TF_CUDA(launch_gate(activation, z, out, M, (int)F, amax_track_begin_on(out, s), s));
+  TF_CUDA(launch_gate(activation, z, out, M, (int)F, amax_track_begin(out), s));
   TF_AFTER(s, what);
   return 0;
 }
@@ -230,7 +230,7 @@ int TfGatedLinearBackward(const DLArrayHandle input, const DLArrayHandle weight,
   note_write(dz);                        // scratch: whatever was known of an array at this address does not hold
   if (M && F) {
     KernelTimer kt(what, s, 0, 20.0 * M * F);
-    TF_CUDA(launch_gate_gradient(activation, (const float*)gates->data, (const float*)doutput->data, dz, M, (int)F, amax_track_begin_on(dz, s), s));
+    TF_CUDA(launch_gate_gradient(activation, (const float*)gates->data, (const float*)doutput->data, dz, M, (int)F, amax_track_begin(dz), s));
     TF_AFTER(s, what);
   }
   if (few_rows && contraction_path() != 2) {

@@ -199,7 +199,8 @@ int DLGpuConvolution3DForward(const DLArrayHandle input, const DLArrayHandle fil
   TF_REQUIRE(input && numel(input) == (int64_t)p->N * p->C * p->D * p->H * p->W, "DLGpuConvolution3DForward: input does not match the descriptor");
   TF_REQUIRE(filter && numel(filter) == (int64_t)p->K * p->C * p->T * p->R * p->S, "DLGpuConvolution3DForward: filter does not match the descriptor");
   TF_REQUIRE(output && numel(output) == (int64_t)p->N * p->K * p->Od * p->P * p->Q, "DLGpuConvolution3DForward: output does not match the descriptor");
-  return cudacore_conv3d_fwd(&p->N, (const float*)input->data, (const float*)filter->data, out_f32(output), last_compute_stream());
+  const cudaStream_t s = last_compute_stream();
+  return cudacore_conv3d_fwd(&p->N, (const float*)input->data, (const float*)filter->data, out_f32(output), s);
 }
 
 int DLGpuPooling3DForwardGetOutShape(const int* input_shapes, int* output_shapes, int dataformat, int poolingMode, const int padding1, const int padding2,

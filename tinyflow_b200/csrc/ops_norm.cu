@@ -765,7 +765,7 @@ int TfLayerNormForward(const DLArrayHandle input, const DLArrayHandle gamma, con
   cudaStream_t s = stream_of(cudaStream);
   a.x = (const float*)input->data; a.gamma = (const float*)gamma->data; a.beta = (const float*)beta->data; a.y = out_f32(output); a.eps = eps;
   if (numel(input) == 0) return 0;
-  a.am = amax_track_begin_on(a.y, s);
+  a.am = amax_track_begin(a.y);
   note_compute_stream(s);
   KernelTimer kt(what, s, 0, 8.0 * numel(input));
   TF_CUDA(launch_norm_fwd<false>(a, s));
@@ -788,7 +788,7 @@ int TfLayerNormBackward(const DLArrayHandle input, const DLArrayHandle gamma, co
   a.dx = opt_out(dinput);
   float *dg = opt_out(dgamma), *db = opt_out(dbeta);
   if (a.D == 0 || !(a.dx || dg || db)) return 0;
-  if (a.dx && a.rows) a.am = amax_track_begin_on(a.dx, s);
+  if (a.dx && a.rows) a.am = amax_track_begin(a.dx);
   note_compute_stream(s);
   KernelTimer kt(what, s, 0, 12.0 * numel(input));
   return run_norm_bwd<false>(a, dg, db, memorytoSaving, s, what);
@@ -823,7 +823,7 @@ int TfDropoutAddLayerNormForward(const DLArrayHandle input, const DLArrayHandle 
   st->recording = recording_id();
   set_dropout(a, st); a.seed_word = st->seed_word;
   if (n == 0) return 0;
-  if (a.y) a.am = amax_track_begin_on(a.y, s);
+  if (a.y) a.am = amax_track_begin(a.y);
   note_compute_stream(s);
   KernelTimer kt(what, s, 0, 16.0 * n);
   TF_CUDA(launch_norm_fwd<true>(a, s));
@@ -851,7 +851,7 @@ int TfDropoutAddLayerNormBackward(const DLArrayHandle sum, const DLArrayHandle g
   set_dropout(a, st);
   a.seed_word = st->recording && st->recording == recording_id() ? st->seed_word : nullptr;
   if (a.D == 0 || !(a.dx || a.dbranch || dg || db)) return 0;
-  if (a.rows && (a.dx || a.dbranch)) a.am = amax_track_begin_on(a.dbranch ? a.dbranch : a.dx, s);
+  if (a.rows && (a.dx || a.dbranch)) a.am = amax_track_begin(a.dbranch ? a.dbranch : a.dx);
   note_compute_stream(s);
   KernelTimer kt(what, s, 0, 20.0 * n);
   return run_norm_bwd<true>(a, dg, db, memorytoSaving, s, what);

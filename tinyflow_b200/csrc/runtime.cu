@@ -118,8 +118,9 @@ cudaError_t clear_now(void* p, size_t bytes) {
 
 static std::atomic<cudaStream_t> g_compute_stream{(cudaStream_t)0};
 void note_compute_stream(cudaStream_t s) { if (!t_recording) g_compute_stream.store(s, std::memory_order_relaxed); }     // a recording's stream concerns nobody else
-cudaStream_t legacy_stream() { flush_deferred(); return t_recording ? recording_stream() : (cudaStream_t)0; }
-cudaStream_t last_compute_stream() { flush_deferred(); return t_recording ? recording_stream() : g_compute_stream.load(std::memory_order_relaxed); }
+thread_local bool t_captured = false;
+cudaStream_t legacy_stream() { flush_deferred(); return enter_call(t_recording ? recording_stream() : (cudaStream_t)0); }
+cudaStream_t last_compute_stream() { flush_deferred(); return enter_call(t_recording ? recording_stream() : g_compute_stream.load(std::memory_order_relaxed)); }
 
 // ---- the held-back elementwise call (see common.h) ----------------------------------------------
 std::atomic<int> g_deferred_pending{0};
@@ -492,7 +493,7 @@ int DLArrayFree(DLArrayHandle handle) {
   if (!handle) return 0;
   flush_deferred_if_uses(handle->data);      // a held-back kernel may read or write this array
   if (handle->data) {
-    if (handle->ctx.device_type == kGPU) note_write(handle->data);   // a recycled block is new data
+    if (handle->ctx.device_type == kGPU) note_free(handle->data);    // a recycled block is new data
     bool ok = (handle->ctx.device_type == kGPU) ? device_pool(handle->ctx.device_id).free(handle->data)
                                                 : host_pool().free(handle->data);
     if (!ok) TF_FAIL("DLArrayFree: array was not allocated by DLArrayAlloc");
@@ -518,6 +519,7 @@ int DLArrayCopyFromTo(DLArrayHandle from, DLArrayHandle to, DLStreamHandle strea
   TF_CUDA(cudaSetDevice(fg ? from->ctx.device_id : to->ctx.device_id));
   cudaMemcpyKind kind = fg && tg ? cudaMemcpyDeviceToDevice : (fg ? cudaMemcpyDeviceToHost : cudaMemcpyHostToDevice);
   if (bytes == 0) return 0;
+  enter_call(stream ? *(cudaStream_t*)stream : (cudaStream_t)0);
   if (tg) note_write(to->data);
   if (stream == nullptr) {
     // A blocking copy between host and device is how a training loop uploads its next batch and reads its loss: in
