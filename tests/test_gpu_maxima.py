@@ -294,3 +294,26 @@ def test_an_array_in_the_place_of_one_that_a_replay_wrote(stage):
         taken.append(env.empty((M, K)))
         assert len(taken) < 100
     assert launches(taken[-1]) == clean
+
+
+@pytest.mark.parametrize("last", ["sum", "relu gradient"])
+def test_a_capture_that_ends_with_a_call_that_would_wait(stage, last):
+    """Large sums and gradients of a ReLU wait for one call outside a capture; inside, their kernel is part of the graph."""
+    env = stage
+    rng = np.random.RandomState(6)
+    a, b, out = env.dev(rng.randn(M, K)), env.dev(rng.randn(M, K)), env.dev(np.zeros((M, K)))
+    cell_of = env.gpu_op.activation_get_cudnnlist((M, K), "NCHW", "relu")
+
+    def call_on(stream):
+        if last == "sum":
+            return lambda: env.gpu_op.matrix_elementwise_add(a, b, out, stream)
+        return lambda: env.gpu_op.activation_backward(a, out, a, b, "relu", cell_of, env.cudnn, stream)
+
+    env.gpu_op.device_synchronize()
+    graph = capture(call_on)
+    for size in (1.0, 3.0):
+        a[:] = (size * rng.randn(M, K)).astype(np.float32)
+        out[:] = np.full((M, K), np.nan, np.float32)
+        replay(graph)
+        x, y = a.asnumpy(), b.asnumpy()
+        np.testing.assert_array_equal(out.asnumpy(), x + y if last == "sum" else np.where(x > 0, y, 0))

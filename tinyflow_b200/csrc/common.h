@@ -56,6 +56,7 @@ struct KernelTimer {
 //    if it is the backward call of the convolution in front of the ReLU, the kernel that packs that convolution's dy computes it;
 //  * DLGpuMatrixElementwiseAdd: if the very next call is the ReLU forward of the sum (the end of a residual block), ONE
 //    kernel writes the sum and its ReLU.
+// Inside a caller's capture nothing waits: the capture may end first.
 // Every other way into the library - stream_of(), which every operator with a stream argument calls first,
 // last_compute_stream() and legacy_stream(), which the stream-less operators and the copies call, the array free, the synchronising calls -
 // launches the held-back kernel first (flush_deferred), so no caller can observe the difference.  One slot, guarded by

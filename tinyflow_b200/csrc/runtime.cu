@@ -116,9 +116,9 @@ cudaError_t clear_now(void* p, size_t bytes) {
   return e;
 }
 
+thread_local bool t_captured = false;
 static std::atomic<cudaStream_t> g_compute_stream{(cudaStream_t)0};
 void note_compute_stream(cudaStream_t s) { if (!t_recording) g_compute_stream.store(s, std::memory_order_relaxed); }     // a recording's stream concerns nobody else
-thread_local bool t_captured = false;
 cudaStream_t legacy_stream() { flush_deferred(); return enter_call(t_recording ? recording_stream() : (cudaStream_t)0); }
 cudaStream_t last_compute_stream() { flush_deferred(); return enter_call(t_recording ? recording_stream() : g_compute_stream.load(std::memory_order_relaxed)); }
 
@@ -127,6 +127,7 @@ std::atomic<int> g_deferred_pending{0};
 static std::mutex g_deferred_mu;
 static DeferredOp g_deferred;
 bool deferral_enabled() {
+  if (t_captured) return false;                 // the capture may end before another call comes
   static const bool on = [] {
     const char* e = getenv("TINYFLOW_DEFER");
     return (e ? atoi(e) != 0 : true) && getenv("TINYFLOW_SYNC") == nullptr;      // per-operator timing wants every operator launched in its own call
