@@ -317,3 +317,91 @@ def test_a_capture_that_ends_with_a_call_that_would_wait(stage, last):
         replay(graph)
         x, y = a.asnumpy(), b.asnumpy()
         np.testing.assert_array_equal(out.asnumpy(), x + y if last == "sum" else np.where(x > 0, y, 0))
+
+
+# N, C, H, W, filters, window, stride: 1x1 and windows, strided phases, patches of few channels, the CUDA cores' own kernels
+CONVOLUTIONS = [(8, 64, 14, 14, 96, 1, 1), (4, 32, 20, 20, 64, 3, 1), (4, 32, 21, 21, 64, 3, 2), (4, 3, 32, 32, 64, 7, 2), (4, 3, 30, 30, 16, 3, 1)]
+
+
+@pytest.mark.parametrize("geometry", CONVOLUTIONS)
+@pytest.mark.parametrize("before", [False, True])
+def test_captured_convolutions(stage, geometry, before):
+    """All three calls of a layer in a graph: replays on numbers of any size have the bits of ordinary calls on a descriptor of their own,
+    and so have ordinary calls on the graph's descriptor in between.  before: those come ahead of the capture, too."""
+    env = stage
+    op = env.gpu_op
+    N, C, H, W, filters, window, stride = geometry
+    rng = np.random.RandomState(C + window)
+    shapes = (N, C, H, W), (filters, C, window, window)
+    padding = "SAME" if stride == 1 else "VALID"
+    out, cell = op.convolution_2d_forward_get_out_shape(*shapes, "NCHW", padding, stride, stride)
+    other = op.convolution_2d_forward_get_out_shape(*shapes, "NCHW", padding, stride, stride)[1]
+    x, w, dy = (env.empty(s) for s in shapes + (tuple(out),))
+    numbers = [rng.randn(*v.shape).astype(np.float32) for v in (x, w, dy)]
+    results = {k: [env.empty(s) for s in (tuple(out),) + shapes] for k in ("graph", "same", "other")}
+
+    def fill(size):
+        for v, n in zip((x, w, dy), numbers):
+            v[:] = n * np.float32(size)
+
+    def calls(descriptor, into, stream):
+        def run():
+            assert op.convolution_2d_forward(x, w, into[0], descriptor, env.cudnn, stream) == 0
+            assert op.convolution_backward_data(x, dy, w, into[1], descriptor, env.cudnn, stream) == 0
+            assert op.convolution_backward_filter(x, dy, w, into[2], descriptor, env.cudnn, stream) == 0
+        return run
+
+    fill(30.0)
+    if before:
+        calls(cell, results["same"], env.stream)()
+    op.device_synchronize()
+    graph = capture(lambda stream: calls(cell, results["graph"], stream))
+    for size in (1.0, 1e4, 1e-3, 0.5):
+        fill(size)
+        calls(other, results["other"], env.stream)()
+        replay(graph)
+        calls(cell, results["same"], env.stream)()
+        replay(graph)
+        op.device_synchronize()
+        for k in ("graph", "same"):
+            for name, got, want in zip(("y", "dx", "dw"), results[k], results["other"]):
+                np.testing.assert_array_equal(got.asnumpy(), want.asnumpy(), err_msg="%s of %s at %g" % (name, k, size))
+
+
+def test_a_replay_between_a_convolutions_calls(stage):
+    """The descriptor's packs are what the replay left: the gradient behind it takes them anew from its own arrays."""
+    env = stage
+    op, rng = env.gpu_op, np.random.RandomState(9)
+    shapes = (4, 32, 20, 20), (64, 32, 3, 3)
+    out, cell = op.convolution_2d_forward_get_out_shape(*shapes, "NCHW", "SAME", 1, 1)
+    other = op.convolution_2d_forward_get_out_shape(*shapes, "NCHW", "SAME", 1, 1)[1]
+    x, x2, w, w2, dy = (env.dev(rng.randn(*s)) for s in (shapes[0], shapes[0], shapes[1], shapes[1], out))
+    y, y2, got, want = env.empty(out), env.empty(out), [env.empty(s) for s in shapes], [env.empty(s) for s in shapes]
+    op.device_synchronize()
+    graph = capture(lambda stream: lambda: op.convolution_2d_forward(x2, w2, y2, cell, env.cudnn, stream))
+    for descriptor, into in ((cell, got), (other, want)):
+        op.convolution_2d_forward(x, w, y, descriptor, env.cudnn, env.stream)
+        op.device_synchronize()
+        replay(graph)
+        op.convolution_backward_data(x, dy, w, into[0], descriptor, env.cudnn, env.stream)
+        op.convolution_backward_filter(x, dy, w, into[1], descriptor, env.cudnn, env.stream)
+    for a, b in zip(got, want):
+        np.testing.assert_array_equal(a.asnumpy(), b.asnumpy())
+
+
+def test_a_replay_between_the_calls_of_a_pooling(stage):
+    env = stage
+    op, rng = env.gpu_op, np.random.RandomState(10)
+    shape = (5, 7, 18, 18)
+    out, cell = op.pooling_2d_forward_get_out_shape(shape, "NCHW", "max", 0, 0, 2, 2, 2, 2)
+    other = op.pooling_2d_forward_get_out_shape(shape, "NCHW", "max", 0, 0, 2, 2, 2, 2)[1]
+    x, x2, dy = (env.dev(rng.randn(*s)) for s in (shape, shape, out))
+    y, y2, got, want = env.empty(out), env.empty(out), env.empty(shape), env.empty(shape)
+    op.device_synchronize()
+    graph = capture(lambda stream: lambda: op.pooling_2d_forward(x2, y2, cell, env.cudnn, stream))
+    for descriptor, into in ((cell, got), (other, want)):
+        op.pooling_2d_forward(x, y, descriptor, env.cudnn, env.stream)
+        op.device_synchronize()
+        replay(graph)
+        op.pooling_2d_backward(x, y, dy, into, descriptor, env.cudnn, env.stream)
+    np.testing.assert_array_equal(got.asnumpy(), want.asnumpy())

@@ -356,6 +356,7 @@ struct PoolPlan {
   const void* argmax_src;
   uint64_t argmax_version;
   uint64_t argmax_recording;   // the recording whose graph writes the indices, 0: an ordinary call did
+  bool argmax_captured;        // a graph that the caller captured writes them, too, unseen
 };
 struct TensorPlan {      // activation / dropout input descriptor
   int kind;

@@ -2924,13 +2924,14 @@ static inline long long round_up(long long a, long long b) { return (a + b - 1) 
 
 struct Pack {           // a packed operand living in pooled device memory
   void* hi = nullptr; void* lo = nullptr;
-  uint32_t* words = nullptr;       // device: amax[0], amax[1] (alternating between uses), scale (float), spare
+  uint32_t* words = nullptr;       // device: amax[0], amax[1] (alternating between uses), scale (float), amax of captured graphs
   unsigned uses = 0;
   int arith = kArithF16;           // element type of hi / lo
   long long rows = 0, cols = 0, pitch = 0;
   const void* src = nullptr; uint64_t version = 0; int tag = 0;   // cache key
   uint64_t recording = 0;          // the recording whose graph fills the pack, 0: an ordinary call did
-  void made_from(const void* s, uint64_t ver, int t) { src = s; version = ver; tag = t; recording = recording_id(); if (t_recording) recording_note_made(&src); }
+  bool captured = false;           // a graph that the caller captured fills it, too, unseen: no call finds it made
+  void made_from(const void* s, uint64_t ver, int t) { src = s; version = ver; tag = t; recording = recording_id(); captured |= t_captured; if (t_recording) recording_note_made(&src); }
   size_t bytes() const { return (size_t)rows * pitch * elem_of(arith); }
   const float* scale() const { return reinterpret_cast<const float*>(words + 2); }
 };
@@ -2953,11 +2954,16 @@ static int pack_alloc(Pack& pk, int ar, long long rows, long long cols, cudaStre
   if (!pk.words) {
     if (t_recording) TF_FAIL("a packed operand of a recorded step has never been packed before");    // its words could not be cleared now
     pk.words = (uint32_t*)pool_alloc(16);
-    if (!pk.words || cudaMemsetAsync(pk.words, 0, 16, s) != cudaSuccess) { if (oom) *oom = 16; return 1; }
+    if (!pk.words || (t_captured ? clear_now(pk.words, 16) : cudaMemsetAsync(pk.words, 0, 16, s)) != cudaSuccess) { if (oom) *oom = 16; return 1; }
     pk.uses = 0;
   }
+  if (t_captured) TF_CUDA(clear_on_stream(pk.words + 3, 4, s));        // the captured graph's own maximum, see begin_pack
   if (pk.hi && pk.rows == rows && pk.pitch == pitch && pk.arith == ar) { pk.cols = cols; return 0; }
-  if (pk.hi) { pool_free(pk.hi); pool_free(pk.lo); pk.hi = pk.lo = nullptr; bump_layout_epoch(); }
+  if (pk.hi) {
+    if (!pk.captured) { pool_free(pk.hi); pool_free(pk.lo); }          // what a captured graph names is left to it
+    pk.hi = pk.lo = nullptr;
+    bump_layout_epoch();
+  }
   pk.rows = rows; pk.cols = cols; pk.pitch = pitch; pk.src = nullptr; pk.arith = ar;
   pk.hi = pool_alloc(pk.bytes());
   pk.lo = pk.hi ? pool_alloc(pk.bytes()) : nullptr;
@@ -2973,6 +2979,7 @@ static void pack_release(Pack& pk) {
   if (pk.hi) { pool_free(pk.hi); pool_free(pk.lo); pk.hi = pk.lo = nullptr; }
   if (pk.words) pool_free(pk.words);
   pk.words = nullptr;
+  pk.captured = false;
 }
 // Starts one use of the pack: reduces max|src| over n contiguous floats into this use's amax word and returns the
 // references the pack kernel needs.  Several pack launches of the same use (stride phases) share one ScaleRef.
@@ -2983,6 +2990,8 @@ static ScaleRef begin_pack(Pack& pk, const float* src, long long n, cudaStream_t
   uint32_t* fresh;                      // zero when the amax kernel below adds to it
   if (t_recording) {
     fresh = recording_word();
+  } else if (t_captured) {              // the pair alternates between calls, and replays are calls that nobody counts
+    fresh = pk.words + 3;
   } else {
     const unsigned k = pk.uses++ & 1;
     fresh = pk.words + k;
@@ -3329,7 +3338,7 @@ static int launch_pack_nchw(Pack& pk, const ScaleRef& sr, const float* src, int 
 // between replays, and nothing of the step would pack it again), an ordinary call none that a recording has only announced.
 static bool pack_valid(const Pack& pk, int ar, const void* src, uint64_t ver, int tag, long long rows, long long cols) {
   return pk.hi && pk.arith == ar && pk.src == src && pk.version == ver && pk.tag == tag && pk.rows == rows && pk.cols == cols &&
-         pk.recording == recording_id();
+         pk.recording == recording_id() && !pk.captured;
 }
 // ---- producers that write a consumer's pack ---------------------------------------------------------------------------
 // The graph calls BN -> ReLU -> convolution as separate entry points, and the convolution then re-reads the ReLU's output

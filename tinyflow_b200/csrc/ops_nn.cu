@@ -791,6 +791,7 @@ int DLGpuPooling2DForward(const DLArrayHandle input, DLArrayHandle output, void*
     p->argmax_src = input->data;
     p->argmax_version = version_of(input->data);
     p->argmax_recording = recording_id();
+    p->argmax_captured |= t_captured;
     if (t_recording) recording_note_made(&p->argmax_src);
   }
   else {
@@ -815,7 +816,7 @@ int DLGpuPooling2DBackward(const DLArrayHandle input, const DLArrayHandle output
   note_compute_stream(s);
   KernelTimer kt("DLGpuPooling2DBackward", s, 0, 4.0 * ((p->mode == 0 ? 2 : 1) * numel(input) + numel(output)));
   if (p->mode == 0) {
-    if (p->argmax && p->argmax_src == input->data && p->argmax_version == version_of(input->data) && p->argmax_recording == recording_id())
+    if (p->argmax && p->argmax_src == input->data && p->argmax_version == version_of(input->data) && p->argmax_recording == recording_id() && !p->argmax_captured)
       launch_pool_gather<true>(p, p->argmax, (const float*)doutput->data, out_f32(dinput), total, 1.f, s);
     else
       launch_plain(maxpool_bwd_kernel, dim3(grid_for(total, 256)), dim3(256), 0, s, (const float*)input->data, (const float*)doutput->data, out_f32(dinput), total, geom_of(p));
