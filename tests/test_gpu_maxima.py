@@ -405,3 +405,72 @@ def test_a_replay_between_the_calls_of_a_pooling(stage):
         replay(graph)
         op.pooling_2d_backward(x, y, dy, into, descriptor, env.cudnn, env.stream)
     np.testing.assert_array_equal(got.asnumpy(), want.asnumpy())
+
+
+# ---- calls that are short of memory -------------------------------------------------------------------------------------
+class FullDevice:
+    """No scratch on any stream and no byte left in the pool."""
+    def __init__(self, env):
+        self.env = env
+
+    def __enter__(self):
+        op = self.env.gpu_op
+        op.device_synchronize()
+        op.set_memory_limit(1)
+        assert isinstance(self.env.empty((1 << 30,)), int)                 # the scratch of every stream goes back
+        op.release_cached_memory()
+        op.set_memory_limit(sum(op.allocator_stats()))
+
+    def __exit__(self, *error):
+        self.env.gpu_op.set_memory_limit(0)
+
+
+def product_bits(env, y, w):
+    out = env.empty((y.shape[0], w.shape[1]))
+    env.gpu_op.matrix_multiply(y, False, w, False, out, env.cublas, env.stream)
+    return out.asnumpy()
+
+
+@pytest.mark.parametrize("D", [512, 9000, 16400])
+@pytest.mark.parametrize("form", ["norm", "residual norm"])
+def test_norm_gradients_short_of_memory(stage, D, form):
+    """They leave no maximum behind: the next write of the array begins with a clear word."""
+    env = stage
+    op, rows = env.gpu_op, 300
+    rng = np.random.RandomState(D)
+    x, y, big, small = (env.dev(size * rng.randn(rows, D)) for size in (1.0, 1.0, 1e4, 1e-4))
+    gamma, dg, db, w = env.dev(np.ones(D)), env.empty((D,)), env.empty((D,)), env.dev(rng.randn(D, 1024))
+    other, state = op.create_cudaStream(), op.dropout_state(0.5, 1)
+    with FullDevice(env):
+        op.relu(big, y)
+        if form == "norm":
+            assert op.layer_norm_backward(x, gamma, big, y, dg, db, 1e-5, other) > 0
+        else:
+            assert op.dropout_add_layer_norm_backward(x, gamma, big, None, y, None, dg, db, state, 1e-5, other) > 0
+    op.relu(small, y)
+    np.testing.assert_array_equal(product_bits(env, y, w), product_bits(env, env.dev(y.asnumpy()), w))
+    op.destroy_cudaStream(other)
+
+
+def test_a_convolution_short_of_memory(stage):
+    env = stage
+    op, rng = env.gpu_op, np.random.RandomState(3)
+    shapes = (16, 256, 28, 28), (256, 256, 3, 3)
+    out, cell = op.convolution_2d_forward_get_out_shape(*shapes, "NCHW", "SAME", 1, 1)
+    next_cell = op.convolution_2d_forward_get_out_shape(out, (64, 256, 1, 1), "NCHW", "VALID", 1, 1)[1]
+    act = op.activation_get_cudnnlist(out, "NCHW", "relu")
+    x, w, w2, big, small = (env.dev(size * rng.randn(*s)) for size, s in ((1, shapes[0]), (1, shapes[1]), (1, (64, 256, 1, 1)), (1e6, out), (1e-6, out)))
+    y, r, z = env.empty(out), env.empty(out), env.empty((16, 64, 28, 28))
+    other = op.create_cudaStream()
+    for _ in range(2):                                     # the ReLU in front of the second layer asks for the maximum of the first one's output
+        assert op.convolution_2d_forward(x, w, y, cell, env.cudnn, env.stream) == 0
+        op.activation_forward(y, r, "relu", act, env.cudnn, env.stream)
+        assert op.convolution_2d_forward(r, w2, z, next_cell, env.cudnn, env.stream) == 0
+    with FullDevice(env):
+        op.relu(big, y)
+        assert op.convolution_2d_forward(x, w, y, cell, env.cudnn, other) > 0
+    op.relu(small, y)
+    rows = view(env, y, 0, (256 * 16, 28 * 28))
+    w3 = env.dev(rng.randn(28 * 28, 64))
+    np.testing.assert_array_equal(product_bits(env, rows, w3), product_bits(env, env.dev(rows.asnumpy()), w3))
+    op.destroy_cudaStream(other)

@@ -115,6 +115,7 @@ void invalidate_all_versions();             // every tensor counts as rewritten 
 // writes (the kernel of write k clears the word write k+1 will use), so no clearing launch is needed.
 struct AmaxOut { uint32_t* word = nullptr; uint32_t* clear = nullptr; };
 AmaxOut amax_track_begin(const void* data);
+void amax_track_abandon(const void* data);  // the launch did not come: the words are not as the next write expects them
 // (Inside a caller's capture there are no words: one that an earlier call left may be cleared or belong to other data at a replay, and one that
 // the graph fills would not be cleared between replays.)
 const uint32_t* amax_tracked(const void* data);

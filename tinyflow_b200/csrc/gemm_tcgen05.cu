@@ -139,6 +139,11 @@ AmaxOut amax_track_begin(const void* data) {
   sl.version = array_version_locked(data);
   return AmaxOut{sl.words + k, sl.words + (k ^ 1)};
 }
+void amax_track_abandon(const void* data) {
+  std::lock_guard<std::mutex> lk(g_ver_mu);
+  auto it = g_amax.find(data);
+  if (it != g_amax.end()) { it->second.words = nullptr; it->second.version = 0; }
+}
 const uint32_t* amax_tracked(const void* data) {
   std::lock_guard<std::mutex> lk(g_ver_mu);
   auto it = g_amax.find(data);
@@ -3668,7 +3673,9 @@ static int conv_like(const Pack& act, const Pack& filt, int ch_in, int ch_out, i
     g.amax = track->word; g.amax_clear = track->clear;
   }
   if (pairs) return ar == kArithTF32 ? launch_gemm_pair<kArithTF32>(g, s, flops, what) : launch_gemm_pair<kArithF16>(g, s, flops, what);
-  return launch_gemm_bn(bn, ar, g, s, flops, what, oom);
+  rc = launch_gemm_bn(bn, ar, g, s, flops, what, oom);
+  if (rc && g.amax && !t_recording) amax_track_abandon(out);
+  return rc;
 }
 static double conv_flops(const ConvPlan* p) { return 2.0 * p->N * p->K * p->P * p->Q * p->C * p->R * p->S; }
 // result of a tensor-path entry point from the launcher's code

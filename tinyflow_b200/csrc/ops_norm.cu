@@ -654,6 +654,8 @@ template <bool RES> static cudaError_t launch_norm_fwd(const NormArgs& a, cudaSt
 }
 template <bool RES> static int run_norm_bwd(NormArgs a, float* dgamma, float* dbeta, int* memorytoSaving, cudaStream_t s, const char* what) {
   const bool sums = dgamma || dbeta;
+  const float* const tracked = a.dbranch ? a.dbranch : a.dx;
+  auto track = [&] { if (tracked && a.rows) a.am = amax_track_begin(tracked); };              // once nothing is short: a launch writes the word
   StreamLease lease(s);
   auto shortage = [&](size_t bytes) { if (memorytoSaving) *memorytoSaving = bytes > 0x7fffffffu ? 0x7fffffff : (int)bytes; return 0; };
   int blocks = 0, out_of_memory = 0;
@@ -679,6 +681,7 @@ template <bool RES> static int run_norm_bwd(NormArgs a, float* dgamma, float* db
       const auto kernel = norm_bwd_kernel<VEC, G, NV, RES>;
       e = once_per_device(ready, [kernel] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBwdSmem); });
       if (!blocks || e != cudaSuccess) return;
+      track();
       if (few) e = launch_cluster(norm_bwd_kernel<VEC, G, NV, RES>, blocks, dim3(blocks), dim3(groups * G), smem, s, a, depth);
       else e = launch_dep(norm_bwd_kernel<VEC, G, NV, RES>, dim3(blocks), dim3(groups * G), smem, s, a, depth);
     });
@@ -693,7 +696,9 @@ template <bool RES> static int run_norm_bwd(NormArgs a, float* dgamma, float* db
       static std::atomic<uint64_t> ready{0};
       const auto kernel = norm_wide_bwd_kernel<VEC, E / VEC, RES>;
       e = once_per_device(ready, [kernel] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBwdSmem); });
-      if (blocks && e == cudaSuccess) e = launch_dep(kernel, dim3(blocks), dim3(kWideThreads), smem, s, a);
+      if (!blocks || e != cudaSuccess) return;
+      track();
+      e = launch_dep(kernel, dim3(blocks), dim3(kWideThreads), smem, s, a);
     };
     if (a.D <= 12 * kWideThreads) launch(std::integral_constant<int, 12>());
     else if (a.D <= 16 * kWideThreads) launch(std::integral_constant<int, 16>());
@@ -712,6 +717,7 @@ template <bool RES> static int run_norm_bwd(NormArgs a, float* dgamma, float* db
       if (!scratch) return shortage(part + stats);
       a.part = (float*)scratch; a.stats = (float2*)(scratch + part);
     }
+    track();
     if (a.rows) e = launch_dep(norm_long_bwd_kernel<RES>, dim3((unsigned)std::min<int64_t>(a.rows, 4 * device_sm_count())), dim3(kLongThreads), 0, s, a);
     if (e == cudaSuccess && sums && blocks) {
       e = launch_dep(norm_columns_kernel, dim3(across, (unsigned)blocks), dim3(256), 0, s, a, per_block);
@@ -788,7 +794,6 @@ int TfLayerNormBackward(const DLArrayHandle input, const DLArrayHandle gamma, co
   a.dx = opt_out(dinput);
   float *dg = opt_out(dgamma), *db = opt_out(dbeta);
   if (a.D == 0 || !(a.dx || dg || db)) return 0;
-  if (a.dx && a.rows) a.am = amax_track_begin(a.dx);
   note_compute_stream(s);
   KernelTimer kt(what, s, 0, 12.0 * numel(input));
   return run_norm_bwd<false>(a, dg, db, memorytoSaving, s, what);
@@ -851,7 +856,6 @@ int TfDropoutAddLayerNormBackward(const DLArrayHandle sum, const DLArrayHandle g
   set_dropout(a, st);
   a.seed_word = st->recording && st->recording == recording_id() ? st->seed_word : nullptr;
   if (a.D == 0 || !(a.dx || a.dbranch || dg || db)) return 0;
-  if (a.rows && (a.dx || a.dbranch)) a.am = amax_track_begin(a.dbranch ? a.dbranch : a.dx);
   note_compute_stream(s);
   KernelTimer kt(what, s, 0, 20.0 * n);
   return run_norm_bwd<true>(a, dg, db, memorytoSaving, s, what);
