@@ -2701,8 +2701,8 @@ constexpr size_t kGroupBytes = size_t(512) << 20;
 // 0: launched, -1: error, 1: too many at once, no memory for the table or the partial sums, or a graph of the caller's own is being captured
 // (its copy of the table would read host memory that is gone at a replay); nothing was launched
 template <int BN, int AR> static int launch_group(HeldProduct* const* products, int n, cudaStream_t s) {
-  static const cudaError_t attr = cudaFuncSetAttribute(gemm3x_group_kernel<BN, AR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGroupSmem<BN>);
-  TF_CUDA(attr);
+  static std::atomic<uint64_t> ready{0};
+  TF_CUDA(once_per_device(ready, [] { return cudaFuncSetAttribute(gemm3x_group_kernel<BN, AR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGroupSmem<BN>); }));
   if (!t_recording && capturing(s)) return 1;
   const int sms = device_sm_count();
   // Whole tiles, or chunks of their pieces, up to half of a CTA's share (a fifth: 0.3 % slower); longer reductions as their pieces.  Longest first, to the CTA that is free first.
@@ -2874,16 +2874,10 @@ template <int BN, int AR> static bool held_back(const GemmParams& p, size_t work
   return true;
 }
 // CTA-pair launch: 74 clusters of two CTAs, programmatic dependent launch as everywhere else.
-static bool g_pair_attr_done[2] = {false, false};
 template <int AR> static int launch_gemm_pair(const GemmParams& p, cudaStream_t s, double flops, const char* what) {
   using L = PairLayout;
-  {
-    std::lock_guard<std::mutex> lk(g_tc_mu);
-    if (!g_pair_attr_done[AR]) {
-      TF_CUDA(cudaFuncSetAttribute(gemm3x_pair_kernel<AR>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal));
-      g_pair_attr_done[AR] = true;
-    }
-  }
+  static std::atomic<uint64_t> ready{0};
+  TF_CUDA(once_per_device(ready, [] { return cudaFuncSetAttribute(gemm3x_pair_kernel<AR>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal); }));
   TF_REQUIRE(tensor_path_error() == 0, "%s: an earlier tensor-core kernel timed out on a barrier; refusing to launch", what);
   static const int group_iters = getenv("TINYFLOW_GROUP_ITERS") ? atoi(getenv("TINYFLOW_GROUP_ITERS")) : 0;
   const_cast<GemmParams&>(p).out_shift = (int)(reinterpret_cast<uintptr_t>(p.out) >> 2 & 3);
