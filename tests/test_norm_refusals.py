@@ -92,3 +92,15 @@ def test_states(op):
         refused(list(calls(op, arrays(), state=new_cell(3)))[k], "state")
     state = op.dropout_state(0.1, 1)
     assert op.dropout_state(0.2, 3, state) is state
+
+
+def test_a_cell_that_holds_another_descriptor(op):
+    """It keeps it: the state of a residual norm takes an empty cell, or one that holds such a state."""
+    cell = op.activation_get_cudnnlist((2, 3), "NCHW", "relu")
+    held = cell[0]
+    refused(lambda: op.dropout_state(0.5, 1, cell), "another descriptor")
+    import ctypes
+    address = lambda c: ctypes.cast(c, ctypes.c_void_p).value        # noqa: E731
+    assert address(cell[0]) == address(held)
+    state = op.dropout_state(0.5, 1)
+    assert op.dropout_state(0.25, 2, state) is state
