@@ -404,6 +404,11 @@ template <class T> T* plan_of(void*** cell, int kind) {
   if (!p || p->kind != kind) return nullptr;
   return p;
 }
+// Whether the cell holds a plan of any kind (an empty cell may hold pointers, down to a null one)
+inline bool holds_plan(void*** cell) {
+  const int* const kind = cell && *cell ? reinterpret_cast<const int*>((*cell)[0]) : nullptr;
+  return kind && (*kind & ~0xff) == 0x7f00;
+}
 // Allocates the slot array the reference allocates (so a caller that frees it stays valid).
 template <class T> T* new_plan(void*** cell, int kind, int slots) {
   void** arr = (void**)calloc(slots < 1 ? 1 : slots, sizeof(void*));

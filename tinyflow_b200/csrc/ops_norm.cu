@@ -805,7 +805,7 @@ int TfDropoutState(float dropout, int seed, void*** state) {
   TF_REQUIRE(state, "TfDropoutState: null cell");
   TF_REQUIRE(dropout >= 0.f && dropout < 1.f, "TfDropoutState: rate must be in [0,1)");
   ResidualDropoutState* st = plan_of<ResidualDropoutState>(state, kPlanResidualDropout);
-  TF_REQUIRE(st || !*state || !(*state)[0], "TfDropoutState: the cell holds another descriptor");
+  TF_REQUIRE(st || !holds_plan(state), "TfDropoutState: the cell holds another descriptor");
   if (!st) st = new_plan<ResidualDropoutState>(state, kPlanResidualDropout, 1);
   st->p = dropout; st->seed = (unsigned long long)(unsigned)seed;
   return 0;
