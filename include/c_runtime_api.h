@@ -312,6 +312,11 @@ int TfAdamUpdateMany(const DLArrayHandle *w, const DLArrayHandle *m, const DLArr
 /* Device-to-device copy enqueued on the stream; no host wait. */
 int TfArrayCopyOnStream(DLArrayHandle from, DLArrayHandle to, void **cudaStream);
 
+/* The array was written by something that the library does not see: a kernel or another library of the caller's, or a call on an array that
+ * begins elsewhere in the same memory.  What earlier calls know of its contents (its largest magnitude, packed operands) is forgotten.
+ * Host side only; the write itself is the caller's to order. */
+int TfArrayWritten(const DLArrayHandle array);
+
 /* Recording a step and replaying it with one call.  Between Begin and End the calling thread issues the step's calls on
  * the stream Begin returns; they are recorded, not executed.  Replays go to *replay_stream, whose scratch they share.
  * The arrays the calls name have to outlive the recording.

@@ -474,3 +474,28 @@ def test_a_convolution_short_of_memory(stage):
     w3 = env.dev(rng.randn(28 * 28, 64))
     np.testing.assert_array_equal(product_bits(env, rows, w3), product_bits(env, env.dev(rows.asnumpy()), w3))
     op.destroy_cudaStream(other)
+
+
+def test_a_write_that_the_library_does_not_see(stage):
+    """By another library over the same memory, and through an array that begins elsewhere in it: announced, it is taken as it is."""
+    import torch
+    env = stage
+    rng = np.random.RandomState(12)
+    numbers = rng.randn(M, K).astype(np.float32)
+
+    class Memory:
+        def __init__(self, array):
+            self.__cuda_array_interface__ = {"data": (array.data_ptr, False), "shape": array.shape, "typestr": "<f4", "version": 2}
+
+    y = by_relu(env, numbers)
+    env.gpu_op.device_synchronize()
+    torch.as_tensor(Memory(y), device="cuda").copy_(torch.from_numpy(numbers * np.float32(1e5)).cuda())
+    torch.cuda.synchronize()
+    env.gpu_op.array_written(y)
+    same_as_a_copy(env, y, "another library")
+    whole = env.empty((M + 4, K))
+    part = view(env, whole, 4 * K, (M, K))
+    env.gpu_op.relu(env.dev(numbers), part)
+    env.gpu_op.relu(env.dev(np.concatenate([numbers[:4], numbers * np.float32(1e5)])), whole)
+    env.gpu_op.array_written(part)
+    same_as_a_copy(env, part, "elsewhere in the same memory")

@@ -104,3 +104,10 @@ def test_a_cell_that_holds_another_descriptor(op):
     assert address(cell[0]) == address(held)
     state = op.dropout_state(0.5, 1)
     assert op.dropout_state(0.25, 2, state) is state
+
+
+def test_a_write_of_an_array_that_is_not_on_a_gpu(op):
+    refused(lambda: op.array_written(described((2, 3), MB, kind=1)), "device array")
+    refused(lambda: op.array_written(described((2, 3), 0)), "device array")
+    op.array_written(described((2, 3), MB))
+    op.array_written(described((0, 3), 0))

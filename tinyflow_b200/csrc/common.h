@@ -103,6 +103,7 @@ cudaStream_t last_compute_stream();         // launches a held-back kernel first
 // captured call has written, version_of() is another number at every call, until the array is freed.  (A call knows its stream before it writes.)
 void note_write(const void* p);
 void note_free(const void* p);
+void note_write_elsewhere(const void* p);   // by something that is no call of the library
 uint64_t version_of(const void* p);
 inline float* out_f32(DLArray* a) { note_write(a->data); return (float*)a->data; }
 void invalidate_all_versions();             // every tensor counts as rewritten (a recording was abandoned)

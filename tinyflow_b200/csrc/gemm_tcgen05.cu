@@ -71,6 +71,11 @@ void note_write(const void* p) {
   std::lock_guard<std::mutex> lk(g_ver_mu);
   bump_locked(p);
 }
+void note_write_elsewhere(const void* p) {
+  std::lock_guard<std::mutex> lk(g_ver_mu);
+  auto it = g_versions.find(p);
+  if (it == g_versions.end() || it->second != kRewrittenAnyTime) g_versions[p] = ++g_ver_counter;
+}
 void note_free(const void* p) {
   if (t_recording) recording_note_write(p);
   std::lock_guard<std::mutex> lk(g_ver_mu);

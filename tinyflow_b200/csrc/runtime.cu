@@ -567,6 +567,14 @@ int TfArrayCopyOnStream(DLArrayHandle from, DLArrayHandle to, void** cudaStream)
   return 0;
 }
 
+int TfArrayWritten(const DLArrayHandle array) {
+  flush_deferred();
+  TF_REQUIRE(array && (array->data || numel(array) == 0) && array->ctx.device_type == kGPU, "TfArrayWritten: needs a device array");
+  TF_REQUIRE(!t_recording, "TfArrayWritten: a recorded step is written by the library alone");
+  if (array->data) note_write_elsewhere(array->data);
+  return 0;
+}
+
 int DLGpuCreatecudaStream(void** cudaStream) {
   TF_REQUIRE(cudaStream, "null cell");
   cudaStream_t s;

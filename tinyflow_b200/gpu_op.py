@@ -414,6 +414,12 @@ def copy_on_stream(source, target, cudaStream):
     check_call(_LIB.TfArrayCopyOnStream(_h(source), _h(target), cudaStream))
 
 
+def array_written(arr):
+    """``arr`` was written by something other than a call of this module (another library over the same memory, say): what is known of its contents
+    is forgotten."""
+    check_call(_LIB.TfArrayWritten(_h(arr)))
+
+
 def data_parallel_active() -> bool:
     return _LIB.TfDpActive() != 0
 
