@@ -24,7 +24,7 @@ __device__ __forceinline__ void copy_async16(float* dst, const float* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copies_arrived() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-// Division of indices below 2^16 by a divisor below 2^16: a runtime division takes 20 instructions, and filling shared memory has two an element
+// Division of indices below 2^16 by a divisor below 2^16: filling shared memory has two of them an element
 struct FastDiv {
   uint32_t m;
   FastDiv(int d = 1) : m(d > 1 ? (uint32_t)((0x100000000ull + d - 1) / d) : 0u) {}
