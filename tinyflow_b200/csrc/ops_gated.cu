@@ -11,6 +11,7 @@
 #include <type_traits>
 #include "gated.h"
 #include "operands.h"
+#include "pieces.h"
 
 namespace tf {
 
@@ -30,12 +31,6 @@ void hold_products(bool on);
 namespace {
 
 constexpr int kThreads = 256;
-template <int VEC> struct Pieces;
-template <> struct Pieces<4> { typedef float4 T; };
-template <> struct Pieces<1> { typedef float T; };
-template <int VEC> __device__ __forceinline__ void get(float* v, const float* __restrict__ p) { *reinterpret_cast<typename Pieces<VEC>::T*>(v) = __ldg(reinterpret_cast<const typename Pieces<VEC>::T*>(p)); }
-template <int VEC> __device__ __forceinline__ void put(float* p, const float* v) { *reinterpret_cast<typename Pieces<VEC>::T*>(p) = *reinterpret_cast<const typename Pieces<VEC>::T*>(v); }
-
 // HBM-bound: 12 bytes per output.
 template <int ACT, int VEC>
 __global__ void __launch_bounds__(kThreads) gate_kernel(const float* __restrict__ z, float* __restrict__ out, int64_t rows, int F, AmaxOut am) {

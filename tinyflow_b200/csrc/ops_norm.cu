@@ -17,6 +17,7 @@
 #include <cooperative_groups.h>
 #include <type_traits>
 #include "operands.h"
+#include "pieces.h"
 
 namespace cg = cooperative_groups;
 
@@ -44,14 +45,6 @@ struct NormArgs {
   const uint32_t* seed_word;
   AmaxOut am;
 };
-
-template <int VEC> struct Pieces;
-template <> struct Pieces<4> { typedef float4 T; };
-template <> struct Pieces<2> { typedef float2 T; };
-template <> struct Pieces<1> { typedef float T; };
-template <int VEC> __device__ __forceinline__ void get(float* v, const float* __restrict__ p) { *reinterpret_cast<typename Pieces<VEC>::T*>(v) = __ldg(reinterpret_cast<const typename Pieces<VEC>::T*>(p)); }
-template <int VEC> __device__ __forceinline__ void held_at(float* v, const float* p) { *reinterpret_cast<typename Pieces<VEC>::T*>(v) = *reinterpret_cast<const typename Pieces<VEC>::T*>(p); }
-template <int VEC> __device__ __forceinline__ void put(float* p, const float* v) { *reinterpret_cast<typename Pieces<VEC>::T*>(p) = *reinterpret_cast<const typename Pieces<VEC>::T*>(v); }
 
 // Sums over the G threads that share a row, the same in all of them.  Two buffers in turn: a thread that writes one for the next sum
 // has passed the barrier behind which every thread had read the one before.
