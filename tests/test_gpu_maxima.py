@@ -499,3 +499,37 @@ def test_a_write_that_the_library_does_not_see(stage):
     env.gpu_op.relu(env.dev(np.concatenate([numbers[:4], numbers * np.float32(1e5)])), whole)
     env.gpu_op.array_written(part)
     same_as_a_copy(env, part, "elsewhere in the same memory")
+
+
+def test_a_captured_first_call_teaches_the_next_nothing(stage):
+    """The first ordinary step behind it has the bits of the second: both know the first layer's maximum, from which the ReLU's pack takes its scale."""
+    env = stage
+    op, rng = env.gpu_op, np.random.RandomState(13)
+    shapes = (13, 64, 40, 40), (64, 64, 1, 1)
+    out, first = op.convolution_2d_forward_get_out_shape(*shapes, "NCHW", "VALID", 1, 1)
+    second = op.convolution_2d_forward_get_out_shape(out, (64, 64, 1, 1), "NCHW", "VALID", 1, 1)[1]
+    act = op.activation_get_cudnnlist(out, "NCHW", "relu")
+    x = np.abs(rng.randn(*shapes[0])) * np.where(rng.rand(*shapes[0]) < 0.5, 1, 0)
+    w = np.zeros(shapes[1])
+    w[np.arange(64), np.arange(64), 0, 0] = np.where(np.arange(64) < 2, -1e8, 1)       # two channels far below zero, which the ReLU takes away
+    X, W, W2 = env.dev(x), env.dev(w), env.dev(rng.randn(64, 64, 1, 1))
+    y, r, z, kept = env.empty(out), env.empty(out), env.empty(out), env.empty(out)
+    op.device_synchronize()
+    op.set_contraction_path(2)
+    graph = capture(lambda stream: lambda: op.convolution_2d_forward(X, W, kept, first, env.cudnn, stream))
+    steps = []
+    op.set_contraction_path(2)
+    try:
+        for _ in range(4):
+            before = op.fused_relu_pack_count()
+            assert op.convolution_2d_forward(X, W, y, first, env.cudnn, env.stream) == 0
+            op.activation_forward(y, r, "relu", act, env.cudnn, env.stream)
+            assert op.convolution_2d_forward(r, W2, z, second, env.cudnn, env.stream) == 0
+            steps.append(z.asnumpy())
+        assert op.fused_relu_pack_count() == before + 1
+    finally:
+        op.set_contraction_path(0)
+    replay(graph)
+    np.testing.assert_array_equal(kept.asnumpy(), y.asnumpy())
+    for again in steps[1:]:
+        np.testing.assert_array_equal(steps[0], again)

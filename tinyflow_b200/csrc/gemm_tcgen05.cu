@@ -3244,8 +3244,8 @@ struct ConvTc {
   int cp = 0;                                            // class D: columns per stride phase (C rounded up to 64)
   bool dgrad_seen = false;                               // backward-data has run on this plan: forward also packs its filter layout
   bool track_y = false, track_dx = false;                // a ReLU asked for max|y| / max|dx|: the epilogue leaves it
-  bool y_made = false, dx_made = false;                  // ... and so does the first call, before anybody can have asked
-  static bool tracks(bool asked, bool* made, int ar) { const bool t = asked || !*made; if (ar == kArithF16) *made = true; return t; }
+  bool y_made = false, dx_made = false;                  // ... and so does the first call (that nobody captures), before anybody can have asked
+  static bool tracks(bool asked, bool* made, int ar) { const bool t = asked || !*made; if (ar == kArithF16 && !t_captured) *made = true; return t; }
   Pack x, dy, wf, wd;
   ConvTc* x_owner = this;                                // whose x pack the plan reads: another plan's of the same recorded step, or its own
   std::mutex mu;
