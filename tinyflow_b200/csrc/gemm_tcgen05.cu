@@ -57,24 +57,24 @@ static bool captured_locked(const void* p) {
   return it != g_versions.end() && it->second == kRewrittenAnyTime;
 }
 static uint64_t version_locked(const void* p) {
-  if (captured_locked(p)) return ++g_ver_counter;
-  auto it = g_versions.find(p);
-  if (it == g_versions.end()) { g_versions[p] = ++g_ver_counter; return g_ver_counter; }
-  return it->second;
+  if (t_captured) return ++g_ver_counter;
+  const auto at = g_versions.try_emplace(p, 0);
+  if (at.second) at.first->second = ++g_ver_counter;
+  return at.first->second == kRewrittenAnyTime ? ++g_ver_counter : at.first->second;
 }
-static void bump_locked(const void* p) {
-  if (t_captured) g_versions[p] = kRewrittenAnyTime;
-  else if (!captured_locked(p)) g_versions[p] = ++g_ver_counter;
+static void bump_locked(const void* p, bool captured) {
+  const auto at = g_versions.try_emplace(p, 0);
+  if (captured) at.first->second = kRewrittenAnyTime;
+  else if (at.second || at.first->second != kRewrittenAnyTime) at.first->second = ++g_ver_counter;
 }
 void note_write(const void* p) {
   if (t_recording) recording_note_write(p);
   std::lock_guard<std::mutex> lk(g_ver_mu);
-  bump_locked(p);
+  bump_locked(p, t_captured);
 }
 void note_write_elsewhere(const void* p) {
   std::lock_guard<std::mutex> lk(g_ver_mu);
-  auto it = g_versions.find(p);
-  if (it == g_versions.end() || it->second != kRewrittenAnyTime) g_versions[p] = ++g_ver_counter;
+  bump_locked(p, false);
 }
 void note_free(const void* p) {
   if (t_recording) recording_note_write(p);
@@ -87,7 +87,7 @@ uint64_t version_of(const void* p) {
 }
 void bump_versions(const void* const* ptrs, size_t n) {
   std::lock_guard<std::mutex> lk(g_ver_mu);
-  for (size_t i = 0; i < n; ++i) bump_locked(ptrs[i]);
+  for (size_t i = 0; i < n; ++i) bump_locked(ptrs[i], t_captured);
 }
 void invalidate_all_versions() {
   std::lock_guard<std::mutex> lk(g_ver_mu);
