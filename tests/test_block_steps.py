@@ -106,3 +106,42 @@ def test_a_replayed_step_of_a_long_batch_that_stays_finite(lib_path, monkeypatch
     assert all(np.isfinite(v).all() for v in runs[0][2]) and all(np.isfinite(v).all() for v in runs[0][3].values())
     assert all(np.array_equal(a, b) for a, b in zip(runs[0][2], runs[1][2]))
     assert all(np.array_equal(v, runs[1][3][n]) for n, v in runs[0][3].items())
+
+
+def _plan_every_forward_result(ex, kind):
+    """What a forward operator of several results has, released behind its last reader of the forward pass and computed again in front of the first one of
+    the backward pass: its own array ("whole"), its further results ("parts"), or all of them."""
+    users = {n: [] for n in ex.topo_order}
+    for n in ex.topo_order:
+        for i in n.inputs:
+            users[i].append(n)
+    release, again, loss = [], {}, ex.targetloss.index
+    for n in reversed(ex.topo_order):                      # what is computed again from another result needs that one back first
+        part = type(n.op).__name__ in ("PartOp", "NormalisedSumOp")
+        whole = n.inputs[0] if part else n
+        if type(whole.op).__name__ not in ("GatedLinearForwardOp", "DropoutAddLayerNormForwardOp") or n.index >= loss or kind not in ("all", "parts" if part else "whole"):
+            continue
+        if type(n.op).__name__ == "DropoutAddLayerNormForwardOp":
+            continue                                       # the next sums read it, and it takes its own inputs
+        readers = [u for u in users[n] if not (type(u.op).__name__ in ("PartOp", "NormalisedSumOp") and u.inputs[0] is n)]
+        forward, backward = [u.index for u in readers if u.index <= loss], [u.index for u in readers if u.index > loss]
+        if not backward:
+            continue
+        release.append((max(forward + [n.index]), n.index))
+        again[n] = min(backward + [at for m, at in again.items() if n in (m.inputs[0].inputs if type(m.op).__name__ == "PartOp" else m.inputs)])
+    assert again
+    return [], release, [(at, n.index) for n, at in reversed(list(again.items()))]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["whole", "parts", "all"])
+@pytest.mark.parametrize("optimizer", ["sgd", "adam"])
+def test_results_computed_again(lib_path, monkeypatch, kind, optimizer):
+    """A plan that lets go of every result it can: the bits of the step without one."""
+    from tests import test_gpu_gated
+    want = test_gpu_gated.block_step(monkeypatch, steps=3, dropout=0.4, optimizer=optimizer)
+    got = test_gpu_gated.block_step(monkeypatch, steps=3, dropout=0.4, optimizer=optimizer, plan=lambda ex: _plan_every_forward_result(ex, kind))
+    for a, b in zip(want[2], got[2]):
+        np.testing.assert_array_equal(a, b)
+    for name, v in want[3].items():
+        np.testing.assert_array_equal(v, got[3][name], err_msg=name)
