@@ -377,6 +377,46 @@ int TfGatedLinearForward(const DLArrayHandle input, const DLArrayHandle weight, 
 int TfGatedLinearBackward(const DLArrayHandle input, const DLArrayHandle weight, const DLArrayHandle gates, const DLArrayHandle doutput,
                           DLArrayHandle dinput, DLArrayHandle dweight, int activation, int *memorytoSaving, void **cudaStream);
 
+/* Rotary positions.  Arrays are matrices of tokens (sequences one after another) by heads x head_dim columns, as a matrix product makes them.
+ * A pair (a, b) of a head's elements at position t turns by the angle t * frequency of the pair: amplitude * (a cos - b sin, a sin + b cos); elements
+ * behind the 2 * pairs rotated ones stay as they are.  Pairs are (i, i + pairs), or (2 i, 2 i + 1) if interleaved; frequencies[i] in radians a position,
+ * angles are formed in 64 bits.  TfRotaryState makes the state that the calls take (in an empty cell), or gives an existing one other values; heads have up
+ * to 256 elements.  positions: one per token, any numbers; null: token r of an array stands at start + r % length.
+ * Backward: the rotation by the opposite angles. */
+int TfRotaryState(int head_dim, int pairs, int interleaved, const double *frequencies, float amplitude, void ***state);
+int TfRotaryForward(const DLArrayHandle input, const DLArrayHandle positions, DLArrayHandle output, int64_t length, int64_t start, void ***state,
+                    void **cudaStream);
+int TfRotaryBackward(const DLArrayHandle doutput, const DLArrayHandle positions, DLArrayHandle dinput, int64_t length, int64_t start, void ***state,
+                     void **cudaStream);
+/* Norms of query and key heads and the rotation behind them, in one pass over both: every head x becomes gamma * x / sqrt(mean(x^2) + eps), rotated.
+ * gamma_query and gamma_key have head_dim elements.  key, gamma_key and key_out (backward: dkey_out) may be null together.
+ * Backward: dquery, dkey, dgamma_query and dgamma_key may each be null; the sums of dgamma are in a fixed order. */
+int TfHeadNormRotaryForward(const DLArrayHandle query, const DLArrayHandle key, const DLArrayHandle gamma_query, const DLArrayHandle gamma_key,
+                            const DLArrayHandle positions, DLArrayHandle query_out, DLArrayHandle key_out, int64_t length, int64_t start, float eps,
+                            void ***state, void **cudaStream);
+int TfHeadNormRotaryBackward(const DLArrayHandle query, const DLArrayHandle key, const DLArrayHandle gamma_query, const DLArrayHandle gamma_key,
+                             const DLArrayHandle positions, const DLArrayHandle dquery_out, const DLArrayHandle dkey_out, DLArrayHandle dquery,
+                             DLArrayHandle dkey, DLArrayHandle dgamma_query, DLArrayHandle dgamma_key, int64_t length, int64_t start, float eps,
+                             void ***state, int *memorytoSaving, void **cudaStream);
+
+/* Attention of query heads over key-value heads that they share (heads / kv_heads neighbours each): query (sequences * length) x (heads * head_dim),
+ * key and value (sequences * keys) x (kv_heads * head_dim), heads of up to 256 elements.  length is the state's, the others follow from the arrays.
+ * Query i of a sequence stands at position i + keys - length, so that a single query is the sequence's last token.
+ *   score = scale * query . key, then cap * tanh(score / cap) if the cap is not 0, then - slopes[head] * |distance| if slopes is given
+ *   output = sum of value over the keys that the query sees, weighted by the softmax of their scores
+ * A query sees the keys up to its own position (causal) that are less than `window` away (window not 0), and whatever these say the first prefix[sequence] keys;
+ * with documents (one number a key; keys >= length) only keys of its own document, and a negative number is padding that sees nothing and is not seen.
+ * A query that sees nothing gives zeros and has no gradient.  A key, value, query or output gradient that is not finite makes what depends on it NaN, and
+ * nothing else.  documents, prefix and slopes may be null; they are constants.
+ * stats (2 for every sequence, head and query: the largest score in units of log 2 and the reciprocal of the sum of 2^(score - largest)) is for the backward call; null: not kept.
+ * Backward: output and stats of the forward call; dquery, dkey and dvalue may each be null.  Sums are in a fixed order. */
+int TfAttentionState(int64_t length, int heads, int kv_heads, int causal, int window, float scale, float cap, void ***state);
+int TfAttentionForward(const DLArrayHandle query, const DLArrayHandle key, const DLArrayHandle value, const DLArrayHandle documents, const DLArrayHandle prefix,
+                       const DLArrayHandle slopes, DLArrayHandle output, DLArrayHandle stats, void ***state, int *memorytoSaving, void **cudaStream);
+int TfAttentionBackward(const DLArrayHandle query, const DLArrayHandle key, const DLArrayHandle value, const DLArrayHandle documents, const DLArrayHandle prefix,
+                        const DLArrayHandle slopes, const DLArrayHandle output, const DLArrayHandle stats, const DLArrayHandle doutput, DLArrayHandle dquery,
+                        DLArrayHandle dkey, DLArrayHandle dvalue, void ***state, int *memorytoSaving, void **cudaStream);
+
 /* Test / profiling hooks. */
 int TfPoolingArgmax(const DLArrayHandle input, int32_t *indices_dev, void ***cudnnlist,
                     void **cudaStream);   /* first-maximum index (h*W+w in the input plane) per output */

@@ -29,6 +29,19 @@ class OracleExecutor:
     def _residual_dropout(self, forward, x):
         return x.copy() if forward.dropout == 0 else ops.dropout(x, forward.dropout, self.dropout_seeds.get(forward, forward.seed[0]))
 
+    def _turns(self, node, x, positions):
+        from tinyflow_b200.gpu_op import rotary_frequencies
+        of = dict(node.rotation)
+        layout, rotated = of.pop("layout", "half"), of.pop("rotated", None)
+        f, amplitude = rotary_frequencies(node.head_dim // 2 * 2 if rotated is None else rotated, **of)
+        return node.head_dim, ops.rotary_angles(x.shape[0], node.length, node.start, positions[0] if positions else None, f), amplitude, layout
+
+    def _attended(self, node, ins):
+        rest = iter(ins[3:6])
+        given = {name: next(rest) for name, there in zip(("documents", "prefix", "slopes"), node.given) if there}
+        scale = (ins[0].shape[1] // node.heads) ** -0.5 if node.scale is None else node.scale
+        return dict(length=node.length, heads=node.heads, kv_heads=node.kv_heads, causal=node.causal, window=node.window, scale=scale, cap=node.cap, **given)
+
     def run(self, feed):
         v = self.values = {n: np.asarray(a, dtype=self.dtype) for n, a in feed.items()}
         for node in self.topo:
@@ -156,7 +169,7 @@ class OracleExecutor:
             w, m, vv = ops.adam(ins[0], ins[1], ins[2], ins[3], dt(node.b1), dt(node.b2), dt(b1t), dt(b2t), dt(node.e), dt(node.learning_rate))
             self.values[node.inputs[0]], self.values[node.inputs[1]], self.values[node.inputs[2]] = w, m, vv
             return None
-        if kind in ("PartOp", "NormalisedSumOp"):
+        if kind in ("PartOp", "NormalisedSumOp", "NormedKeysOp"):
             return self.parts[node.inputs[0]][node.part - 1]
         if kind == "LayerNormForwardOp":
             return ops.layer_norm(ins[0], ins[1], ins[2], node.eps)[0]
@@ -182,6 +195,25 @@ class OracleExecutor:
             dx, dweight = ops.gated_linear_backward(ins[0], ins[1], ins[2], ins[3], node.activation)
             self.parts[node] = (dx,)
             return dweight
+        if kind in ("RotaryForwardOp", "RotaryBackwardOp"):
+            return ops.rotary(ins[0], *self._turns(node, ins[0], ins[1:]), back=kind == "RotaryBackwardOp")
+        if kind == "HeadNormRotaryForwardOp":
+            turns = self._turns(node, ins[0], ins[4:])
+            self.parts[node] = (ops.head_norm_rotary(ins[1], ins[3], *turns, node.eps),)
+            return ops.head_norm_rotary(ins[0], ins[2], *turns, node.eps)
+        if kind == "HeadNormRotaryBackwardOp":
+            turns = self._turns(node, ins[0], ins[6 if node.keys else 3:])
+            dquery, dgamma = ops.head_norm_rotary_backward(*ins[:3], *turns, node.eps)
+            self.parts[node] = (dgamma,) + (ops.head_norm_rotary_backward(*ins[3:6], *turns, node.eps) if node.keys else ())
+            return dquery
+        if kind == "AttentionForwardOp":
+            out, stats = ops.attention(*ins[:3], **self._attended(node, ins))
+            self.parts[node] = (stats.reshape(-1, 2),)
+            return out
+        if kind == "AttentionBackwardOp":
+            dquery, dkey, dvalue = ops.attention_backward(*ins[:3], ins[-1], **self._attended(node, ins))
+            self.parts[node] = (dkey, dvalue)
+            return dquery
         if kind == "ExpOp":
             return np.exp(ins[0])
         if kind == "LogOp":

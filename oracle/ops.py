@@ -456,3 +456,100 @@ def gated_linear_backward(x, weight, z, dout, activation):
     value, slope = gate(activation, z[:, :half])
     dz = np.concatenate([dout * z[:, half:] * slope, dout * value], axis=1)
     return dz @ weight.T, x.T @ dz
+
+
+def rotary_angles(tokens, length, start, positions, frequencies):
+    """Angle of every token's pairs."""
+    at = np.arange(tokens) % length + start if positions is None else positions
+    return np.asarray(at, np.float64).reshape(-1, 1, 1) * np.asarray(frequencies, np.float64)
+
+
+def rotary(x, head_dim, angles, amplitude, layout, back=False):
+    """Heads of x (tokens x heads * head_dim) rotated by their tokens' angles."""
+    y = x.reshape(x.shape[0], -1, head_dim).copy()
+    pairs = angles.shape[-1]
+    a, b = (slice(0, pairs), slice(pairs, 2 * pairs)) if layout == "half" else (slice(0, 2 * pairs, 2), slice(1, 2 * pairs, 2))
+    cos, sin = amplitude * np.cos(angles), amplitude * np.sin(angles) * (-1 if back else 1)
+    u, v = y[..., a].copy(), y[..., b].copy()
+    y[..., a], y[..., b] = u * cos - v * sin, u * sin + v * cos
+    return y.reshape(x.shape)
+
+
+def head_norm_rotary(x, gamma, head_dim, angles, amplitude, layout, eps):
+    h = x.reshape(x.shape[0], -1, head_dim)
+    n = h / np.sqrt((h * h).mean(axis=-1, keepdims=True) + eps)
+    return rotary((n * gamma).reshape(x.shape), head_dim, angles, amplitude, layout)
+
+
+def head_norm_rotary_backward(x, gamma, dy, head_dim, angles, amplitude, layout, eps):
+    """(dx, dgamma)"""
+    h = x.reshape(x.shape[0], -1, head_dim)
+    inv = 1 / np.sqrt((h * h).mean(axis=-1, keepdims=True) + eps)
+    n = h * inv
+    u = rotary(dy, head_dim, angles, amplitude, layout, back=True).reshape(h.shape)
+    g = u * gamma
+    return (inv * (g - n * (g * n).mean(axis=-1, keepdims=True))).reshape(x.shape), (u * n).sum(axis=(0, 1))
+
+
+def attention_seen(queries, keys, causal, window, prefix=0, documents=None):
+    """Which keys the queries of one sequence see."""
+    i, j = np.arange(keys - queries, keys)[:, None], np.arange(keys)[None, :]
+    seen = np.ones((queries, keys), bool)
+    if causal:
+        seen &= j <= i
+    if window:
+        seen &= np.abs(i - j) < window
+    seen |= j < prefix
+    if documents is not None:
+        seen &= (documents[keys - queries:, None] == documents[None, :]) & (documents >= 0)
+    return seen
+
+
+def attention_parts(q, k, length, heads, kv_heads, causal, window, scale, cap, documents, prefix, slopes):
+    """For every sequence and head: (sequence, head, its queries' rows, its keys' rows, probabilities, derivative of the cap, scores in units of log 2, maxima, 1 / sums)."""
+    batch, D = q.shape[0] // length, q.shape[1] // heads
+    keys = k.shape[0] // batch
+    away = np.abs(np.arange(keys - length, keys)[:, None] - np.arange(keys)[None, :])
+    for b in range(batch):
+        rows, cols = slice(b * length, (b + 1) * length), slice(b * keys, (b + 1) * keys)
+        seen = attention_seen(length, keys, causal, window, 0 if prefix is None else prefix[b], None if documents is None else documents[cols])
+        for h in range(heads):
+            kv = h // (heads // kv_heads)
+            s = scale * q[rows, h * D:(h + 1) * D] @ k[cols, kv * D:(kv + 1) * D].T
+            inner = np.ones_like(s)
+            if cap:
+                t = np.tanh(s / cap)
+                s, inner = cap * t, 1 - t * t
+            if slopes is not None:
+                s = s - slopes[h] * away
+            z = np.where(seen, s * np.log2(np.e), -np.inf)
+            most = z.max(axis=1, keepdims=True) if keys else np.full((length, 1), -np.inf)
+            most = np.where(np.isneginf(most), 0, most)
+            p = np.exp2(z - most)
+            total = p.sum(axis=1, keepdims=True)
+            inv = np.where(total > 0, 1 / np.where(total > 0, total, 1), 0)
+            yield b, h, kv, rows, cols, p * inv, inner, z, most[:, 0], inv[:, 0]
+
+
+def attention(q, k, v, length, heads, kv_heads, causal, window, scale, cap, documents=None, prefix=None, slopes=None):
+    """(output, maxima and reciprocal sums of sequences x heads x queries)"""
+    D = q.shape[1] // heads
+    out, stats = np.zeros_like(q), np.zeros((q.shape[0] // length, heads, length, 2), q.dtype)
+    for b, h, kv, rows, cols, p, _, _, most, inv in attention_parts(q, k, length, heads, kv_heads, causal, window, scale, cap, documents, prefix, slopes):
+        out[rows, h * D:(h + 1) * D] = p @ v[cols, kv * D:(kv + 1) * D]
+        stats[b, h, :, 0], stats[b, h, :, 1] = most, inv
+    return out, stats
+
+
+def attention_backward(q, k, v, dout, length, heads, kv_heads, causal, window, scale, cap, documents=None, prefix=None, slopes=None):
+    """(dq, dk, dv)"""
+    D = q.shape[1] // heads
+    dq, dk, dv = np.zeros_like(q), np.zeros_like(k), np.zeros_like(v)
+    for _, h, kv, rows, cols, p, inner, _, _, _ in attention_parts(q, k, length, heads, kv_heads, causal, window, scale, cap, documents, prefix, slopes):
+        mine, theirs = slice(h * D, (h + 1) * D), slice(kv * D, (kv + 1) * D)
+        dp = dout[rows, mine] @ v[cols, theirs].T
+        ds = scale * inner * p * (dp - (p * dp).sum(axis=1, keepdims=True))
+        dq[rows, mine] = ds @ k[cols, theirs]
+        dk[cols, theirs] += ds.T @ q[rows, mine]
+        dv[cols, theirs] += p.T @ dout[rows, mine]
+    return dq, dk, dv

@@ -335,7 +335,7 @@ cudaError_t clear_now(void* p, size_t bytes);                                   
 cudaError_t copy_on_stream(void* to, const void* from, size_t bytes, cudaStream_t s);     // device to device
 
 // ---- plan structs stored in slot 0 of a descriptor list ----------------------
-enum PlanKind : int { kPlanConv = 0x7f01, kPlanPool, kPlanAct, kPlanReduce, kPlanBN, kPlanTensor, kPlanDropout, kPlanResidualDropout };
+enum PlanKind : int { kPlanConv = 0x7f01, kPlanPool, kPlanAct, kPlanReduce, kPlanBN, kPlanTensor, kPlanDropout, kPlanResidualDropout, kPlanRotary, kPlanAttention };
 
 struct ConvPlan {
   int kind;

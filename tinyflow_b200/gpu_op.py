@@ -8,6 +8,7 @@ bytes the library failed to allocate (0 on success), as the reference does.
 from __future__ import annotations
 
 import ctypes
+import math
 
 from . import ndarray as _nd
 from ._base import _LIB, c_array, check_call, new_cell
@@ -512,6 +513,83 @@ def gated_linear_forward(in_arr, weight, gates, out_arr, activation, cudaStream)
 def gated_linear_backward(in_arr, weight, gates, dout_arr, din_arr, dweight, activation, cudaStream):
     """Gradients of :func:`gated_linear_forward`; either of ``din_arr`` and ``dweight`` may be None."""
     return _with_short(_LIB.TfGatedLinearBackward, _h(in_arr), _h(weight), _h(gates), _h(dout_arr), _o(din_arr), _o(dweight), _code(_GATE, activation), cudaStream)
+
+
+# ---- rotary positions, norms of heads, attention (no counterpart in the reference) -----------------------------------------
+_LAYOUT = {"half": 0, "interleaved": 1}
+_I64 = ctypes.c_int64
+
+
+def rotary_frequencies(rotated, base=10000.0, scaling="none", factor=1.0, trained=0, low=1.0, high=32.0):
+    """([radians a position of each of ``rotated / 2`` pairs], amplitude).  ``scaling`` stretches positions by ``factor``: "linear" all pairs alike;
+    "stretched" by a larger base, the last pair by the factor and the first not at all; "parts" pairs that turn less than ``low`` times within the ``trained``
+    length by the factor, those that turn more than ``high`` times not at all, those between in proportion, with an amplitude of 1 + log(factor) / 10."""
+    pairs = rotated // 2
+    assert rotated >= 0 and rotated % 2 == 0 and base > 0 and factor > 0
+    if scaling not in ("none", "linear", "stretched", "parts"):
+        raise AssertionError("unknown option %r (expected one of %s)" % (scaling, ["linear", "none", "parts", "stretched"]))
+    if scaling == "stretched" and pairs > 1:
+        base = base * factor ** (rotated / (rotated - 2.0))
+    f = [base ** (-2.0 * i / rotated) for i in range(pairs)]
+    if scaling == "linear":
+        f = [v / factor for v in f]
+    if scaling != "parts":
+        return f, 1.0
+    assert trained > 0 and high > low
+    kept = [min(1.0, max(0.0, (trained * v / (2 * math.pi) - low) / (high - low))) for v in f]
+    return [v * (r + (1.0 - r) / factor) for v, r in zip(f, kept)], 1.0 + 0.1 * math.log(factor)
+
+
+def rotary_state(head_dim, rotated=None, layout="half", base=10000.0, scaling="none", factor=1.0, trained=0, low=1.0, high=32.0, state=None):
+    """What the calls of this section take: heads of ``head_dim`` elements, the first ``rotated`` of them (None: as many as make pairs) turned, ``layout`` "half"
+    (pairs i and i + rotated / 2) or "interleaved" (2 i and 2 i + 1), frequencies as :func:`rotary_frequencies` makes them.  With ``state`` that one gets them."""
+    rotated = head_dim // 2 * 2 if rotated is None else rotated
+    f, amplitude = rotary_frequencies(rotated, base, scaling, factor, trained, low, high)
+    state = new_cell(3) if state is None else state
+    check_call(_LIB.TfRotaryState(int(head_dim), len(f), _code(_LAYOUT, layout), (ctypes.c_double * max(1, len(f)))(*f), _F(amplitude), state))
+    return state
+
+
+def rotary_forward(in_arr, positions, out_arr, length, start, state, cudaStream):
+    """Heads of every token rotated by its position: that of ``positions``, or if it is None ``start`` + its place in its sequence of ``length`` tokens."""
+    check_call(_LIB.TfRotaryForward(_h(in_arr), _o(positions), _h(out_arr), _I64(length), _I64(start), state, cudaStream))
+
+
+def rotary_backward(dout_arr, positions, din_arr, length, start, state, cudaStream):
+    """Gradient of :func:`rotary_forward`."""
+    check_call(_LIB.TfRotaryBackward(_h(dout_arr), _o(positions), _h(din_arr), _I64(length), _I64(start), state, cudaStream))
+
+
+def head_norm_rotary_forward(query, key, gamma_query, gamma_key, positions, query_out, key_out, length, start, eps, state, cudaStream):
+    """Every head of ``query`` and ``key`` divided by its root mean square, times gamma, rotated.  ``key``, ``gamma_key`` and ``key_out`` may be None."""
+    check_call(_LIB.TfHeadNormRotaryForward(_h(query), _o(key), _h(gamma_query), _o(gamma_key), _o(positions), _h(query_out), _o(key_out), _I64(length), _I64(start),
+                                            _F(eps), state, cudaStream))
+
+
+def head_norm_rotary_backward(query, key, gamma_query, gamma_key, positions, dquery_out, dkey_out, dquery, dkey, dgamma_query, dgamma_key, length, start, eps, state,
+                              cudaStream):
+    """Gradients of :func:`head_norm_rotary_forward`; each of ``dquery``, ``dkey``, ``dgamma_query``, ``dgamma_key`` may be None."""
+    return _with_short(_LIB.TfHeadNormRotaryBackward, _h(query), _o(key), _h(gamma_query), _o(gamma_key), _o(positions), _h(dquery_out), _o(dkey_out), _o(dquery),
+                       _o(dkey), _o(dgamma_query), _o(dgamma_key), _I64(length), _I64(start), _F(eps), state, cudaStream)
+
+
+def attention_state(length, heads, kv_heads, causal=True, window=0, scale=1.0, cap=0.0, state=None):
+    """What both attention calls take: sequences of ``length`` queries, heads, what a query sees, scale and cap of the scores.  With ``state`` that one gets them."""
+    state = new_cell(3) if state is None else state
+    check_call(_LIB.TfAttentionState(_I64(length), int(heads), int(kv_heads), int(bool(causal)), int(window), _F(scale), _F(cap), state))
+    return state
+
+
+def attention_forward(query, key, value, documents, prefix, slopes, out_arr, stats, state, cudaStream):
+    """Attention of ``query`` over ``key`` and ``value``; ``documents`` (a number per key), ``prefix`` (keys that all of a sequence see) and ``slopes`` (of the bias by
+    distance, per head) may be None.  ``stats`` gets what the gradient needs, 2 numbers per sequence, head and query; None: it is not kept."""
+    return _with_short(_LIB.TfAttentionForward, _h(query), _h(key), _h(value), _o(documents), _o(prefix), _o(slopes), _h(out_arr), _o(stats), state, cudaStream)
+
+
+def attention_backward(query, key, value, documents, prefix, slopes, out_arr, stats, dout_arr, dquery, dkey, dvalue, state, cudaStream):
+    """Gradients of :func:`attention_forward`; each of ``dquery``, ``dkey``, ``dvalue`` may be None."""
+    return _with_short(_LIB.TfAttentionBackward, _h(query), _h(key), _h(value), _o(documents), _o(prefix), _o(slopes), _h(out_arr), _h(stats), _h(dout_arr), _o(dquery),
+                       _o(dkey), _o(dvalue), state, cudaStream)
 
 
 def getInt(intp):

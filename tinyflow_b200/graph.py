@@ -1065,6 +1065,190 @@ class GatedLinearBackwardOp(ManyOp):
         return input_shapes[1], input_shapes[0]
 
 
+# ---- rotary positions, alone and behind the norms of query and key heads (no counterpart in the reference) ----
+class _Rotated(object):
+    """Operators over tokens x (heads * head_dim) whose heads are rotated by their tokens' positions: ``start`` + the place in a sequence of ``length`` tokens, or
+    what ``positions`` (a node, one number per token) says."""
+
+    def _state(self, node):
+        if node.state[0] is None:
+            node.state[0] = gpu_op.rotary_state(node.head_dim, **node.rotation)
+        return node.state[0]
+
+
+class RotaryForwardOp(_Rotated, Op):
+    """``rotation``: the further arguments of :func:`gpu_op.rotary_state`."""
+    name = "RotaryForward"
+
+    def __call__(self, node_A, head_dim, length, positions=None, start=0, **rotation):
+        return self._node([node_A] + [positions] * (positions is not None), head_dim=head_dim, length=length, start=start, rotation=rotation, state=[None])
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        gpu_op.rotary_forward(input_vals[0], input_vals[1] if len(input_vals) > 1 else None, output_val, node.length, node.start, self._state(node), cudaStream)
+        return 0
+
+    def gradient(self, node, output_grad):
+        return [rotary_backward_op(output_grad, node)] + [zeroslike_op(n) for n in node.inputs[1:]]
+
+    def infer_shape(self, node, input_shapes, cudnnHandle):
+        return input_shapes[0]
+
+
+class RotaryBackwardOp(_Rotated, Op):
+    name = "RotaryBackward"
+
+    def __call__(self, node_A, forward):
+        return self._node([node_A] + forward.inputs[1:], head_dim=forward.head_dim, length=forward.length, start=forward.start, rotation=forward.rotation, state=forward.state)
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        gpu_op.rotary_backward(input_vals[0], input_vals[1] if len(input_vals) > 1 else None, output_val, node.length, node.start, self._state(node), cudaStream)
+        return 0
+
+    def infer_shape(self, node, input_shapes, cudnnHandle):
+        return input_shapes[0]
+
+
+class HeadNormRotaryForwardOp(_Rotated, ManyOp):
+    """Norms of the heads of two tensors of the same tokens and their rotation: the operator gives both nodes.  Results: the queries; the keys."""
+    name = "HeadNormRotaryForward"
+    parts = 1
+
+    def __call__(self, query, key, gamma_query, gamma_key, head_dim, length, positions=None, start=0, eps=1e-6, **rotation):
+        whole = self._node([query, key, gamma_query, gamma_key] + [positions] * (positions is not None), head_dim=head_dim, length=length, start=start, eps=eps,
+                           rotation=rotation, state=[None], of_keys=[])
+        return whole, normed_keys_op(whole)
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        query, key, gamma_query, gamma_key = input_vals[:4]
+        if output_val[1] is None:                         # nobody reads the keys
+            key = gamma_key = None
+        gpu_op.head_norm_rotary_forward(query, key, gamma_query, gamma_key, input_vals[4] if len(input_vals) > 4 else None, output_val[0], output_val[1], node.length,
+                                        node.start, node.eps, self._state(node), cudaStream)
+        return 0
+
+    def adjoint(self, node, contributions):
+        # what reaches the keys comes by way of their node; one kernel takes both
+        keys = [g.inputs[0] for g in contributions if type(g.op) is KeysGradientOp]
+        rest = [g for g in contributions if type(g.op) is not KeysGradientOp]
+        node.of_keys[:] = [sum_node_list(keys)] if keys else []
+        return sum_node_list(rest) if rest else zeroslike_op(node)
+
+    def gradient(self, node, output_grad):
+        others = [zeroslike_op(n) for n in node.inputs[4:]]
+        if not node.of_keys:
+            dquery = head_norm_rotary_backward_op(node, output_grad, None)
+            return [dquery, zeroslike_op(node.inputs[1]), part_op(dquery, 1), zeroslike_op(node.inputs[3])] + others
+        dquery = head_norm_rotary_backward_op(node, output_grad, node.of_keys[0])
+        return [dquery, part_op(dquery, 2), part_op(dquery, 1), part_op(dquery, 3)] + others
+
+    def result_shapes(self, input_shapes):
+        return input_shapes[0], input_shapes[1]
+
+
+class NormedKeysOp(PartOp):
+    name = "NormedKeys"
+
+    def __call__(self, whole):
+        return self._node([whole], part=1)
+
+    def gradient(self, node, output_grad):
+        return [keys_gradient_op(output_grad)]
+
+
+class KeysGradientOp(Op):
+    """Carries the gradient of the keys to the operator that made them; no part of a graph."""
+    name = "KeysGradient"
+
+    def __call__(self, node_A):
+        return self._node([node_A])
+
+
+class HeadNormRotaryBackwardOp(_Rotated, ManyOp):
+    """Results: dquery; dgamma_query, dkey, dgamma_key.  Without a gradient of the keys: the first two."""
+    name = "HeadNormRotaryBackward"
+    parts = 3
+
+    def __call__(self, forward, dquery_out, dkey_out):
+        query, key, gamma_query, gamma_key = forward.inputs[:4]
+        inputs = [query, gamma_query, dquery_out] + ([] if dkey_out is None else [key, gamma_key, dkey_out])
+        return self._node(inputs + forward.inputs[4:], head_dim=forward.head_dim, length=forward.length, start=forward.start, eps=forward.eps, rotation=forward.rotation,
+                          state=forward.state, keys=dkey_out is not None)
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        query, gamma_query, dquery_out = input_vals[:3]
+        key, gamma_key, dkey_out = input_vals[3:6] if node.keys else (None, None, None)
+        positions = input_vals[6 if node.keys else 3:]
+        dquery, dgamma_query, dkey, dgamma_key = output_val
+        return gpu_op.head_norm_rotary_backward(query, key, gamma_query, gamma_key, positions[0] if positions else None, dquery_out, dkey_out, dquery, dkey, dgamma_query,
+                                                dgamma_key, node.length, node.start, node.eps, self._state(node), cudaStream)
+
+    def result_shapes(self, input_shapes):
+        return (input_shapes[0], input_shapes[1]) + (tuple(input_shapes[3:5]) if len(input_shapes) > 4 else ())
+
+
+# ---- attention (no counterpart in the reference) ---------------------------------------------------
+class AttentionForwardOp(ManyOp):
+    """Attention of query heads over the key-value heads that they share; sequences of ``length`` queries.  ``scale`` None: head_dim ** -0.5.  ``documents``, ``prefix``
+    and ``slopes`` are nodes without a gradient, or None.  Results: the output; the rows' maxima and sums, where a gradient needs them."""
+    name = "AttentionForward"
+    parts = 1
+
+    def __call__(self, query, key, value, heads, length, kv_heads=None, causal=True, window=0, scale=None, cap=0.0, documents=None, prefix=None, slopes=None):
+        given = [documents, prefix, slopes]
+        return self._node([query, key, value] + [n for n in given if n is not None], given=[n is not None for n in given], heads=heads, length=length,
+                          kv_heads=heads if kv_heads is None else kv_heads, causal=causal, window=window, scale=scale, cap=cap, state=[None], kept=[None])
+
+    @staticmethod
+    def arguments(node, input_vals):
+        """(query, key, value, documents, prefix, slopes) and the state of both directions' calls."""
+        rest = iter(input_vals[3:6])
+        masks = [next(rest) if there else None for there in node.given]
+        query = input_vals[0]
+        scale = (query.shape[1] // node.heads) ** -0.5 if node.scale is None else node.scale
+        node.state[0] = gpu_op.attention_state(node.length, node.heads, node.kv_heads, node.causal, node.window, scale, node.cap, node.state[0])
+        return list(input_vals[:3]) + masks
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        arrays = self.arguments(node, input_vals)
+        return gpu_op.attention_forward(*arrays, output_val[0], output_val[1], node.state[0], cudaStream)
+
+    def gradient(self, node, output_grad):
+        if node.kept[0] is None:
+            node.kept[0] = part_op(node, 1)
+        dquery = attention_backward_op(node, node.kept[0], output_grad)
+        return [dquery, part_op(dquery, 1), part_op(dquery, 2)] + [zeroslike_op(n) for n in node.inputs[3:]]
+
+    def infer_shape(self, node, input_shapes, cudnnHandle):
+        node.shapes[:] = [input_shapes[0], (input_shapes[0][0] * node.heads, 2)]
+        return input_shapes[0]
+
+    def result_shapes(self, shapes):
+        return tuple(shapes)
+
+
+class AttentionBackwardOp(ManyOp):
+    """Results: dquery; dkey, dvalue."""
+    name = "AttentionBackward"
+    parts = 2
+
+    def __call__(self, forward, stats, node_B):
+        return self._node(forward.inputs + [forward, stats, node_B], given=forward.given, heads=forward.heads, length=forward.length, kv_heads=forward.kv_heads,
+                          causal=forward.causal, window=forward.window, scale=forward.scale, cap=forward.cap, state=[None])
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        arrays = AttentionForwardOp.arguments(node, input_vals[:-3])
+        return gpu_op.attention_backward(*arrays, *input_vals[-3:], *output_val, node.state[0], cudaStream)
+
+    def result_shapes(self, input_shapes):
+        return tuple(input_shapes[:3])
+
+
 # ---- concat (ConcatForwardOp / ConcatBackwardOp: autodiff.py:1935-1984) ---------------------------
 class ConcatForwardOp(Op):
     name = "ConcatForward"
@@ -1255,6 +1439,14 @@ dropout_add_layer_norm_backward_op = DropoutAddLayerNormBackwardOp()
 normalised_sum_op = NormalisedSumOp()
 gated_linear_op = GatedLinearForwardOp()
 gated_linear_backward_op = GatedLinearBackwardOp()
+rotary_op = RotaryForwardOp()
+rotary_backward_op = RotaryBackwardOp()
+head_norm_rotary_op = HeadNormRotaryForwardOp()
+head_norm_rotary_backward_op = HeadNormRotaryBackwardOp()
+normed_keys_op = NormedKeysOp()
+keys_gradient_op = KeysGradientOp()
+attention_op = AttentionForwardOp()
+attention_backward_op = AttentionBackwardOp()
 
 
 # ---- autodiff and graph utilities (autodiff.py:2894-3027) ------------------------------------------------
