@@ -125,6 +125,32 @@ SMALL = [
 ]
 
 
-@pytest.mark.parametrize("kind", SMALL, ids=lambda k: "-".join("%s%s" % (n[0], v) for n, v in k.items()))
-def test_small(env, kind):
+LARGE = [
+    dict(batch=1, queries=128, keys=128, heads=1, kv_heads=1, dim=64, causal=False),
+    dict(batch=1, queries=128, keys=384, heads=1, kv_heads=1, dim=128),
+    dict(batch=2, queries=256, keys=256, heads=4, kv_heads=2, dim=64),
+    dict(batch=1, queries=300, keys=300, heads=6, kv_heads=2, dim=72, prefix=[100], bias=True),
+    dict(batch=2, queries=333, keys=500, heads=2, kv_heads=1, dim=80, window=150, cap=4.0),
+    dict(batch=2, queries=401, keys=401, heads=3, kv_heads=3, dim=33, causal=False, window=65, cap=20.0, bias=True),
+    dict(batch=2, queries=517, keys=517, heads=2, kv_heads=2, dim=128, documents="packed"),
+    dict(batch=2, queries=260, keys=517, heads=4, kv_heads=1, dim=16, documents="mixed", prefix=[30, 600], cap=2.0),
+    dict(batch=1, queries=700, keys=130, heads=2, kv_heads=1, dim=96),
+    dict(batch=1, queries=1025, keys=1025, heads=1, kv_heads=1, dim=128, bias=True, cap=30.0),
+]
+IDS = lambda k: "-".join("%s%s" % (n[0], v) for n, v in k.items())      # noqa: E731
+
+
+@pytest.fixture(params=["exact", "tensor"])
+def path(request, env):
+    env.gpu_op.set_contraction_path({"exact": 1, "tensor": 2}[request.param])
+    yield request.param
+    env.gpu_op.set_contraction_path(0)
+
+
+@pytest.mark.parametrize("kind", SMALL + LARGE, ids=IDS)
+def test_formula(env, path, kind):
+    if path == "tensor" and kind["dim"] > 128:
+        pytest.skip("heads of up to 128 elements")
     check(env, Case(**kind))
+    assert env.gpu_op.tensor_path_error() == 0
+    assert env.gpu_op.last_contraction_path() == {"exact": 1, "tensor": 2}[path]

@@ -1,0 +1,846 @@
+// Tensor-core path of attention: scores and outputs as 3xFP16 products on tcgen05, the probabilities between them in registers and TMEM.
+//
+// One kernel, four kinds.  A CTA holds 128 rows and streams tiles of 128 columns of the other side past them:
+//
+//   kind  rows     scores                      weights                          product           results
+//   fwd   queries  S = Q K^T                   P = 2^(z - running max)          P V               o, row maxima and sums
+//   dq    queries  S = Q K^T, Y = dO' V^T      E (Y - D') (cap's derivative)    dS K              dq
+//   dk    keys     S = K Q^T, Y = V dO'^T      the same, transposed             dS^T Q            dk
+//   dv    keys     S = K Q^T                   E = 2^(z - max of the column)    E^T dO'           dv
+//
+// with dO' and D' the output gradient and its product with the output, divided by the row's sum: P is E over that sum.  Gradients form the scores
+// again, twice as often as one kernel of all three would (8 products of the tile's size instead of 5), but nothing is added across CTAs: no
+// atomics, the same bits every run.
+//
+// Operands.  A packing kernel writes every tile of 128 tokens x one head as fp16 halves hi and lo of x times a power of two that the tile's largest finite
+// element chooses, in the 128-byte swizzle of the shared-memory descriptors, so a tile part is one bulk copy and no tensor map is needed.  The same image is read
+// with the head along K (scores) and with the tokens along K (products), by descriptors of the other major.  Products are hi*lo + lo*hi + hi*hi, the small ones first.
+// Weights are split in registers and go back to TMEM as the A operand, over the scores they came from; each is scaled by a power of two so that their largest
+// (bounded for gradients by the norms of dO' rows and V) is just below 2^15.  Scales of a tile are undone where its product is added up: the tensor core
+// truncates as it accumulates, so every tile's product is added to fp32 registers (round to nearest) by the warps that make the weights.
+//
+// Bound by the tensor rate: 3 products of 16-bit halves for each product.  The tile of the next scores is issued ahead of the product of the present weights,
+// so the tensor cores work while 8 warps (two a TMEM lane quarter, half the columns each) make weights.
+//
+// A token that holds a value which is not finite is packed as if that value were zero and marked; weights that see it become NaN.  So it reaches what depends on it and nothing
+// else, while a zero weight times it would reach every row of the tile.
+#include "attention.h"
+#include <cuda_fp16.h>
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+#include "tcgen05.h"
+
+namespace tf {
+namespace {
+
+enum { kFwd, kDq, kDk, kDv };
+constexpr int kTile = 128;
+constexpr int kThreads = 320;                    // warps: 0 copies, 1 issues MMAs and owns TMEM, 2-9 weights
+constexpr int kWeightExp = 14;                   // weights are scaled to below 2^15
+constexpr int kFar = 1 << 26;                    // beyond every position
+
+// Of one tile of one head
+struct __align__(16) TileInfo {
+  float inv, top;                                // 1 / scale; largest finite magnitude
+  float norm, delta;                             // dO': largest row norm and |D'|
+  uint32_t bad[4];                               // tokens with values that are not finite
+};
+struct Packed { const char* image; const TileInfo* info; };
+struct TcArgs {
+  AttentionArgs a;
+  Packed q, k, v, d;
+  const float *row_max, *row_delta, *row_norm;   // of every sequence, head and query, tiles padded with zeros
+  const float4* documents;                       // of every sequence and key tile: smallest, largest, whether there is padding
+  int q_tiles, k_tiles, D16;
+  int* err;
+};
+
+// ---- packing ----------------------------------------------------------------------------------------------------------------
+struct PackJob {
+  const float* x;
+  char* image;
+  TileInfo* info;
+  int heads, length, tiles;
+  int gradient;                                  // dout: times 1 / sum, with its row's D' and norm
+};
+struct PackArgs {
+  AttentionArgs a;
+  PackJob job[4];
+  int first[5];                                  // blocks of the jobs
+  int jobs;
+  float *row_max, *row_delta, *row_norm;
+  float4* documents;
+  int document_job;
+};
+
+__device__ __forceinline__ uint32_t halves(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// 2^e as a float
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
+__device__ __forceinline__ int exponent_of(float positive) { return (int)((__float_as_uint(positive) >> 23) & 255u) - 127; }
+
+// A block of 256 threads packs one tile of one head.  16 G threads a row, 4 columns each.
+template <int G, bool WIDE>
+__global__ void __launch_bounds__(256) attention_pack_kernel(const __grid_constant__ PackArgs p) {
+  constexpr int kAcross = 16 * G, kRowsAtOnce = 32 / kAcross, kSteps = 16 / kRowsAtOnce;      // a warp packs 16 rows
+  __shared__ float red[8];
+  __shared__ float red_norm[8], red_delta[8];
+  __shared__ uint32_t bad_words[4];
+  grid_dep_sync();
+  int j = 0;
+  while (j + 1 < p.jobs && (int)blockIdx.x >= p.first[j + 1]) ++j;
+  const PackJob& job = p.job[j];
+  const int index = (int)blockIdx.x - p.first[j], tile = index % job.tiles, bh = index / job.tiles, h = bh % job.heads, b = bh / job.heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = (lane % kAcross) * 4, sub = lane / kAcross;
+  const int D = p.a.D;
+  if (threadIdx.x < 4) bad_words[threadIdx.x] = 0u;
+  float v[kSteps][4];
+  float most = 0.f, most_norm = 0.f, most_delta = 0.f;
+  __syncthreads();
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    const int r = warp * 16 + s * kRowsAtOnce + sub, t = tile * kTile + r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[s][i] = 0.f;
+    if (t < job.length && col < D) {
+      const float* const from = job.x + (((int64_t)b * job.length + t) * job.heads + h) * D + col;
+      if (WIDE) { const float4 w = __ldg(reinterpret_cast<const float4*>(from)); v[s][0] = w.x; v[s][1] = w.y; v[s][2] = w.z; v[s][3] = w.w; }
+      else
+#pragma unroll
+        for (int i = 0; i < 4; ++i) if (col + i < D) v[s][i] = __ldg(from + i);
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    const int r = warp * 16 + s * kRowsAtOnce + sub, t = tile * kTile + r;
+    bool fine = true;
+    float stat_max = 0.f, stat_inv = 1.f, delta = 0.f, norm = 0.f;
+    if (job.gradient) {
+      stat_inv = 0.f;
+      float o[4] = {0.f, 0.f, 0.f, 0.f};
+      if (t < job.length) {
+        const int64_t stat = ((int64_t)b * job.heads + h) * job.length + t;
+        stat_max = __ldg(p.a.stats + 2 * stat); stat_inv = __ldg(p.a.stats + 2 * stat + 1);
+        if (col < D) {
+          const float* const from = p.a.out + (((int64_t)b * job.length + t) * job.heads + h) * D + col;
+          if (WIDE) { const float4 w = __ldg(reinterpret_cast<const float4*>(from)); o[0] = w.x; o[1] = w.y; o[2] = w.z; o[3] = w.w; }
+          else
+#pragma unroll
+            for (int i = 0; i < 4; ++i) if (col + i < D) o[i] = __ldg(from + i);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[s][i] *= stat_inv;
+        delta = fmaf(v[s][i], o[i], delta);
+        norm = fmaf(v[s][i], v[s][i], norm);
+      }
+#pragma unroll
+      for (int o2 = kAcross / 2; o2 > 0; o2 >>= 1) { delta += __shfl_xor_sync(0xffffffffu, delta, o2); norm += __shfl_xor_sync(0xffffffffu, norm, o2); }
+      norm = sqrtf(norm);
+      fine = fabsf(delta) < INFINITY && norm < INFINITY && fabsf(stat_max) < INFINITY && fabsf(stat_inv) < INFINITY;
+      if (!fine) { stat_max = 0.f; delta = 0.f; norm = 0.f; }
+      if (col == 0) {
+        const int64_t at = ((int64_t)bh * job.tiles + tile) * kTile + r;
+        p.row_max[at] = stat_max; p.row_delta[at] = delta; p.row_norm[at] = norm;
+      }
+      most_norm = fmaxf(most_norm, norm); most_delta = fmaxf(most_delta, fabsf(delta));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (!(fabsf(v[s][i]) < INFINITY)) { v[s][i] = 0.f; fine = false; }
+      most = fmaxf(most, fabsf(v[s][i]));
+    }
+    if (!fine) atomicOr(&bad_words[r >> 5], 1u << (r & 31));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    most_norm = fmaxf(most_norm, __shfl_xor_sync(0xffffffffu, most_norm, o));
+    most_delta = fmaxf(most_delta, __shfl_xor_sync(0xffffffffu, most_delta, o));
+  }
+  if (lane == 0) { red[warp] = most; red_norm[warp] = most_norm; red_delta[warp] = most_delta; }
+  __syncthreads();
+  most = red[lane & 7]; most_norm = red_norm[lane & 7]; most_delta = red_delta[lane & 7];
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) {
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    most_norm = fmaxf(most_norm, __shfl_xor_sync(0xffffffffu, most_norm, o));
+    most_delta = fmaxf(most_delta, __shfl_xor_sync(0xffffffffu, most_delta, o));
+  }
+  // max * scale in [2^14, 2^15); subnormal maxima, and those from 2^126, as far as the scale and its reciprocal are normal numbers
+  const int e = most > 0.f ? min(126, max(-126, 14 - exponent_of(most))) : 0;
+  const float scale = power_of_two(e);
+  if (threadIdx.x == 0) {
+    TileInfo& info = job.info[(int64_t)bh * job.tiles + tile];
+    info.inv = power_of_two(-e); info.top = most; info.norm = most_norm; info.delta = most_delta;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) info.bad[i] = bad_words[i];
+  }
+  char* const image = job.image + ((int64_t)bh * job.tiles + tile) * (2 * G * 16384);
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    const int r = warp * 16 + s * kRowsAtOnce + sub;
+    float hi[4], x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[i] = v[s][i] * scale; hi[i] = __half2float(__float2half_rn(x[i])); }
+    const int at = (col >> 6) * 16384 + r * 128 + ((((col & 63) >> 3) ^ (r & 7)) << 4) + (col & 4) * 2;
+    *reinterpret_cast<uint2*>(image + at) = make_uint2(halves(hi[0], hi[1]), halves(hi[2], hi[3]));
+    *reinterpret_cast<uint2*>(image + G * 16384 + at) = make_uint2(halves(x[0] - hi[0], x[1] - hi[1]), halves(x[2] - hi[2], x[3] - hi[3]));
+  }
+  if (p.documents && j == p.document_job && h == 0 && warp == 0) {       // what the tile's documents are
+    float low = INFINITY, high = -INFINITY;
+    int padding = 0;
+    for (int r = lane; r < kTile; r += 32) {
+      const float d = document_of(p.a, b, tile * kTile + r);
+      if (d >= 0.f) { low = fminf(low, d); high = fmaxf(high, d); } else padding = 1;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) { low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o)); high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o)); }
+    padding = __any_sync(0xffffffffu, padding);
+    if (lane == 0) p.documents[(int64_t)b * job.tiles + tile] = make_float4(low, high, padding ? 1.f : 0.f, 0.f);
+  }
+}
+
+// ---- which tiles of the other side a CTA's rows see ------------------------------------------------------------------------------
+// A warp looks at 32 tiles at a time.  Every role walks the same list.
+template <int KIND> struct Walk {
+  static constexpr bool kRowsAreKeys = KIND == kDk || KIND == kDv;
+  const TcArgs& p;
+  int b, head, heads_end, tiles, base, prefix;
+  int from, to;                                  // rows: positions of queries, or keys
+  float low, high;                               // their documents
+  bool padding;
+  uint32_t any, whole;
+  __device__ __forceinline__ Walk(const TcArgs& args, int b_, int row_head, int tile) : p(args), b(b_) {
+    const AttentionArgs& a = p.a;
+    const int off = a.Tk - a.Tq;
+    prefix = prefix_of(a, b);
+    tiles = kRowsAreKeys ? p.q_tiles : p.k_tiles;
+    if (kRowsAreKeys) { head = row_head * a.group; heads_end = head + a.group; from = tile * kTile; to = min(from + kTile, a.Tk) - 1; }
+    else { head = row_head; heads_end = head + 1; from = tile * kTile + off; to = min(from + kTile - 1, a.Tk - 1); }
+    low = high = 0.f; padding = false;
+    if (p.documents) documents(from, to, low, high, padding);
+    base = -32; any = whole = 0u;
+  }
+  __device__ __forceinline__ void documents(int first, int last, float& lo, float& hi, bool& pad) const {
+    const float4 u = p.documents[(int64_t)b * p.k_tiles + first / kTile], w = p.documents[(int64_t)b * p.k_tiles + last / kTile];
+    lo = fminf(u.x, w.x); hi = fmaxf(u.y, w.y); pad = u.z + w.z > 0.f;
+  }
+  __device__ __forceinline__ void look(int lane) {
+    const AttentionArgs& a = p.a;
+    const int t = base + lane;
+    bool sees_any = false, sees_whole = false;
+    if (t < tiles) {
+      const int off = a.Tk - a.Tq;
+      // first and last query position, first and last key
+      const int p0 = kRowsAreKeys ? t * kTile + off : from, p1 = kRowsAreKeys ? min(p0 + kTile - 1, a.Tk - 1) : to;
+      const int j0 = kRowsAreKeys ? from : t * kTile, j1 = kRowsAreKeys ? to : j0 + kTile - 1;
+      const Sight first = sight_of(a, p0), last = sight_of(a, p1);
+      sees_any = j0 < prefix || (j0 <= last.hi && j1 >= first.lo);
+      const bool full_tile = (kRowsAreKeys ? t * kTile + kTile <= a.Tq : j1 < a.Tk);            // columns behind the end are hidden one by one
+      sees_whole = full_tile && (j1 < prefix || (j1 <= first.hi && j0 >= last.lo));
+      if (sees_any && p.documents) {
+        float lo, hi;
+        bool pad;
+        if (kRowsAreKeys) documents(p0, p1, lo, hi, pad); else documents(j0, min(j1, a.Tk - 1), lo, hi, pad);
+        sees_any = lo <= high && low <= hi;
+        sees_whole = sees_whole && !pad && !padding && lo == hi && low == high && lo == low;
+      }
+      if (sees_whole) {
+        const int64_t at = kRowsAreKeys ? ((int64_t)b * a.H + head) * tiles + t : ((int64_t)b * a.G + head / a.group) * tiles + t;
+        const uint4 u = *reinterpret_cast<const uint4*>((kRowsAreKeys ? p.q : p.k).info[at].bad), w = *reinterpret_cast<const uint4*>((kRowsAreKeys ? p.d : p.v).info[at].bad);
+        sees_whole = (u.x | u.y | u.z | u.w | w.x | w.y | w.z | w.w) == 0u;
+      }
+    }
+    any = __ballot_sync(0xffffffffu, sees_any);
+    whole = __ballot_sync(0xffffffffu, sees_whole);
+  }
+  // The next tile: its head and number, and whether every row sees all of it
+  __device__ __forceinline__ bool next(int lane, int& at_head, int& t, bool& all) {
+    while (!any) {
+      base += 32;
+      if (base >= tiles) {
+        if (++head >= heads_end) return false;
+        base = 0;
+      }
+      look(lane);
+    }
+    const int bit = __ffs(any) - 1;
+    any &= any - 1;
+    at_head = head; t = base + bit; all = (whole >> bit) & 1u;
+    return true;
+  }
+};
+
+// ---- the kernel ----------------------------------------------------------------------------------------------------------------
+template <int KIND, int G> struct Shape {
+  static constexpr bool kTwo = KIND == kDq || KIND == kDk;           // two score products
+  static constexpr bool kRowsAreKeys = KIND == kDk || KIND == kDv;
+  static constexpr int kPart = G * 16384;                            // one half (hi or lo) of a tile
+  static constexpr int kResident = (kTwo ? 4 : 2) * kPart;
+  static constexpr int kControl = 3072;
+  static constexpr int kStages = (232448 - kControl - kResident) / kPart < 8 ? (232448 - kControl - kResident) / kPart : 8;
+  static constexpr int kSmem = kResident + kStages * kPart + kControl;
+  static constexpr int kOuts = kTwo && G == 2 ? 1 : 2;               // TMEM: scores 0 and 128, second scores 256, products behind
+  static constexpr int kOutAt = kTwo ? 384 : 256;
+  static_assert(kStages >= 3 && kOutAt + kOuts * 64 * G <= 512, "fits");
+};
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t keep) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(keep) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t keep) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(keep) : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ float reciprocal(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+
+// cap * tanh(x / cap) of 32 numbers, t = the tanh.  Up to 0.35 by the series of odd powers (x^13 behind it is 4e-9 of x there), whose error is relative; above by
+// 1 - 2 / (e^2x + 1), whose error is a rounding of 1.  Scores far below the cap, most of all, take the series alone.
+__device__ __forceinline__ void tanh32(float* t) {
+  float most = 0.f;
+#pragma unroll
+  for (int k = 0; k < 32; ++k) most = fmaxf(most, fabsf(t[k]));
+  const bool large = __any_sync(0xffffffffu, !(most < 0.35f));
+#pragma unroll
+  for (int k = 0; k < 32; ++k) {
+    const float x = t[k], s = x * x;
+    float y = -1382.f / 155925.f;
+    y = fmaf(y, s, 62.f / 2835.f); y = fmaf(y, s, -17.f / 315.f); y = fmaf(y, s, 2.f / 15.f); y = fmaf(y, s, -1.f / 3.f);
+    y = fmaf(y * s, x, x);
+    if (large) {
+      const float far = 1.f - 2.f * reciprocal(exp2_fast(2.f * kLog2e * fabsf(x)) + 1.f);
+      y = fabsf(x) < 0.35f ? y : copysignf(far, x);
+    }
+    t[k] = y;
+  }
+}
+// hi and lo halves of 32 weights, as the A operand has them: 16 words each
+__device__ __forceinline__ void split32(const float* w, uint32_t* words) {
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    // the upper 11 bits, which fp16 holds exactly down to 2^-14; below, the rounding is 2^-25 of weights that reach 2^14
+    const float a = __uint_as_float(__float_as_uint(w[2 * k]) & 0xffffe000u), b = __uint_as_float(__float_as_uint(w[2 * k + 1]) & 0xffffe000u);
+    words[k] = halves(a, b);
+    words[16 + k] = halves(w[2 * k] - a, w[2 * k + 1] - b);
+  }
+}
+__device__ __forceinline__ uint32_t bits_between(int lo, int hi) {               // bits lo .. hi of a word, as far as it has them
+  const uint32_t below = hi >= 31 ? 0xffffffffu : hi < 0 ? 0u : (2u << hi) - 1u;
+  return lo <= 0 ? below : lo > 31 ? 0u : below & (0xffffffffu << lo);
+}
+
+template <int KIND, int G, bool CAP>
+__global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_constant__ TcArgs p) {
+  using S = Shape<KIND, G>;
+  constexpr bool kTwo = S::kTwo, kRowsAreKeys = S::kRowsAreKeys;
+  constexpr int kPart = S::kPart, kStages = S::kStages, kOuts = S::kOuts;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* const resident = smem;
+  uint8_t* const ring = smem + S::kResident;
+  uint64_t* const full = reinterpret_cast<uint64_t*>(ring + kStages * kPart);
+  uint64_t* const empty = full + 8;
+  uint64_t* const resident_full = empty + 8;
+  uint64_t* const s_full = resident_full + 1;    // [2] scores are in TMEM
+  uint64_t* const w_full = s_full + 2;           // [2] weights are
+  uint64_t* const y_full = w_full + 2;           // second scores are in TMEM
+  uint64_t* const y_empty = y_full + 1;          // and have been read
+  uint64_t* const o_full = y_empty + 1;          // [2] the product is
+  uint64_t* const o_empty = o_full + 2;          // [2] and has been added up
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 2);
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* const exchange = reinterpret_cast<float*>(full + 32);       // [2][2][128]
+  const AttentionArgs& a = p.a;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int i = 0; i < kStages; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
+      mbar_init(resident_full, 1);
+      for (int i = 0; i < 2; ++i) { mbar_init(s_full + i, 1); mbar_init(w_full + i, 8); mbar_init(o_full + i, 1); mbar_init(o_empty + i, 8); }
+      mbar_init(y_full, 1); mbar_init(y_empty, 8);
+      *abort_flag = (smem_u32(smem) & 1023u) ? 1 : 0;                // nothing is issued then
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncwarp();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  grid_dep_sync();
+
+  // rows that see most go first
+  const int row_heads = kRowsAreKeys ? a.G : a.H, b = blockIdx.x / row_heads, row_head = blockIdx.x - b * row_heads;
+  const int tile = kRowsAreKeys ? (int)blockIdx.y : (int)(gridDim.y - 1 - blockIdx.y);
+  const int col_tiles = kRowsAreKeys ? p.q_tiles : p.k_tiles, row_tiles = kRowsAreKeys ? p.k_tiles : p.q_tiles;
+  const int64_t row_at = ((int64_t)b * row_heads + row_head) * row_tiles + tile;
+  const Packed &r1 = kRowsAreKeys ? p.k : p.q, &r2 = kRowsAreKeys ? p.v : p.d;                 // rows
+  const Packed &c1 = kRowsAreKeys ? p.q : p.k, &c2 = kRowsAreKeys ? p.d : p.v;                 // columns
+  const auto col_at = [&](int head, int t) { return kRowsAreKeys ? ((int64_t)b * a.H + head) * col_tiles + t : ((int64_t)b * a.G + head / a.group) * col_tiles + t; };
+  Walk<KIND> walk(p, b, row_head, tile);
+  int head, t, bad = *abort_flag;
+  bool all;
+
+  if (warp == 0) {
+    // ---- copies: the rows once, then tiles in the order in which the MMAs take them, the lo half first
+    int stage = 0;
+    uint32_t phase = 0, armed = 0, phases = 0;
+    bool rows_armed = false;
+    if (!bad) {
+      if (elect_one()) {
+        mbar_expect_tx(resident_full, S::kResident);
+        bulk_load(resident, r1.image + row_at * 2 * kPart, 2 * kPart, resident_full);
+        if (kTwo) bulk_load(resident + 2 * kPart, r2.image + row_at * 2 * kPart, 2 * kPart, resident_full);
+      }
+      rows_armed = true;
+    }
+    const auto load = [&](const Packed& from, int64_t at) {
+#pragma unroll
+      for (int lo = 1; lo >= 0; --lo) {
+        mbar_wait_mark(&empty[stage], phase ^ 1, abort_flag, bad);
+        bad = __any_sync(0xffffffffu, bad);
+        if (!bad) {
+          if (elect_one()) {
+            mbar_expect_tx(&full[stage], kPart);
+            bulk_load(ring + stage * kPart, from.image + (at * 2 + lo) * kPart, kPart, &full[stage]);
+          }
+          armed |= 1u << stage;
+          phases = (phases & ~(1u << stage)) | phase << stage;
+        }
+        if (++stage == kStages) { stage = 0; phase ^= 1; }
+      }
+    };
+    int64_t before = -1;
+    while (walk.next(lane, head, t, all)) {
+      const int64_t at = col_at(head, t);
+      load(c1, at);
+      if (kTwo) load(c2, at);
+      if (before >= 0) load(kTwo ? c1 : c2, before);
+      before = at;
+    }
+    if (before >= 0) load(kTwo ? c1 : c2, before);
+    __syncwarp();
+    if (*abort_flag) {                           // copies in flight land before the CTA gives its shared memory back
+      for (int i = -1; i < kStages; ++i) {
+        if (i < 0 ? !rows_armed : !((armed >> i) & 1u)) continue;
+        const long long t0 = clock64();
+        while (!mbar_try_wait(i < 0 ? resident_full : &full[i], i < 0 ? 0 : (phases >> i) & 1u) && clock64() - t0 < 100000000ll) {}
+      }
+    } else if (rows_armed) {
+      mbar_wait_mark(resident_full, 0, abort_flag, bad);             // rows that see nothing: nobody else waits for them
+    }
+  } else if (warp == 1) {
+    // ---- MMAs
+    constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(kTile >> 4) << 24), kScores = kIdesc | ((uint32_t)(kTile >> 3) << 17);
+    const uint32_t products = kIdesc | (1u << 16) | ((uint32_t)(p.D16 >> 3) << 17);            // the B operand has its columns (the head) along the rows of memory
+    const int steps = p.D16 / 16;
+    int stage = 0;
+    uint32_t phase = 0;
+    const auto k_major = [](uint32_t at, int ks) { return umma_desc(at + (ks >> 2) * 16384 + (ks & 3) * 32, 16, 1024, 2); };
+    const auto wait_stage = [&] { mbar_wait_mark(&full[stage], phase, abort_flag, bad); bad = __any_sync(0xffffffffu, bad); tcgen05_fence_after(); };
+    const auto next_stage = [&] { if (++stage == kStages) { stage = 0; phase ^= 1; } };
+    const auto scores = [&](uint32_t d, uint32_t rows, uint64_t* done) {
+      wait_stage();
+      uint32_t at = smem_u32(ring + stage * kPart);
+      if (!bad && elect_one()) {
+        for (int ks = 0; ks < steps; ++ks) mma_ss(d, k_major(rows, ks), k_major(at, ks), kScores, ks > 0);
+        tcgen05_commit(&empty[stage]);
+      }
+      __syncwarp();
+      next_stage();
+      wait_stage();
+      at = smem_u32(ring + stage * kPart);
+      if (!bad && elect_one()) {
+        for (int ks = 0; ks < steps; ++ks) mma_ss(d, k_major(rows + kPart, ks), k_major(at, ks), kScores, 1u);
+        for (int ks = 0; ks < steps; ++ks) mma_ss(d, k_major(rows, ks), k_major(at, ks), kScores, 1u);
+        tcgen05_commit(&empty[stage]);
+        tcgen05_commit(done);
+      }
+      __syncwarp();
+      next_stage();
+    };
+    const auto product = [&](int n) {
+      const uint32_t w = tmem + (n & 1) * 128, d = tmem + S::kOutAt + (kOuts == 2 ? (n & 1) * 64 * G : 0);
+      const int out = kOuts == 2 ? n & 1 : 0;
+      mbar_wait_mark(&w_full[n & 1], (n >> 1) & 1, abort_flag, bad);
+      mbar_wait_mark(&o_empty[out], ((n / kOuts) & 1) ^ 1, abort_flag, bad);
+      const auto a_at = [&](int ks, int lo) { return w + 32 * (ks >> 1) + 8 * (ks & 1) + 16 * lo; };
+      const auto b_at = [](uint32_t at, int ks) { return umma_desc(at + ks * 2048, 16384, 1024, 2); };
+      wait_stage();
+      uint32_t at = smem_u32(ring + stage * kPart);
+      if (!bad && elect_one()) {
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) mma_ts(d, a_at(ks, 0), b_at(at, ks), products, ks > 0);
+        tcgen05_commit(&empty[stage]);
+      }
+      __syncwarp();
+      next_stage();
+      wait_stage();
+      at = smem_u32(ring + stage * kPart);
+      if (!bad && elect_one()) {
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) mma_ts(d, a_at(ks, 1), b_at(at, ks), products, 1u);
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) mma_ts(d, a_at(ks, 0), b_at(at, ks), products, 1u);
+        tcgen05_commit(&empty[stage]);
+        tcgen05_commit(&o_full[out]);
+      }
+      __syncwarp();
+      next_stage();
+    };
+    mbar_wait_mark(resident_full, 0, abort_flag, bad);
+    const uint32_t rows = smem_u32(resident);
+    int n = 0;
+    while (walk.next(lane, head, t, all)) {
+      scores(tmem + (n & 1) * 128, rows, &s_full[n & 1]);
+      if (kTwo) {
+        mbar_wait_mark(y_empty, (n & 1) ^ 1, abort_flag, bad);
+        scores(tmem + 256, rows + 2 * kPart, y_full);
+      }
+      if (n > 0) product(n - 1);
+      ++n;
+    }
+    if (n > 0) product(n - 1);
+  } else {
+    // ---- weights
+    const int quarter = warp & 3, half = (warp - 2) >> 2, row = quarter * 32 + lane;
+    const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
+    const int off = a.Tk - a.Tq, self = tile * kTile + row;            // query or key
+    const bool there = self < (kRowsAreKeys ? a.Tk : a.Tq);
+    // columns that the row sees: positions [lo, hi] and those before `extra`
+    int lo, hi, extra;
+    if (kRowsAreKeys) {
+      lo = a.causal ? self : a.window ? self - a.window + 1 : -kFar;
+      hi = min(a.window ? self + a.window - 1 : kFar, a.Tk - 1);       // no query is behind the last key
+      extra = self < prefix_of(a, b) ? a.Tk : -kFar;
+    } else {
+      const Sight s = sight_of(a, self + off);
+      lo = s.lo; hi = min(s.hi, a.Tk - 1); extra = prefix_of(a, b);
+    }
+    const float document = p.documents ? document_of(a, b, kRowsAreKeys ? self : self + off) : 0.f;
+    const TileInfo& info1 = r1.info[row_at];
+    bool spoiled = (info1.bad[quarter] >> lane) & 1u;
+    if (kTwo) spoiled = spoiled || ((r2.info[row_at].bad[quarter] >> lane) & 1u);
+    const bool careful = __any_sync(0xffffffffu, spoiled);
+    const float inv1 = info1.inv, inv2 = kTwo ? r2.info[row_at].inv : 0.f;
+    const float unit = CAP ? a.scale / a.cap : a.scale * kLog2e, wide = CAP ? a.cap * kLog2e : 1.f;
+    float row_max = 0.f, row_delta = 0.f, row_norm = 0.f;
+    if (KIND == kDq) { row_max = p.row_max[row_at * kTile + row]; row_delta = p.row_delta[row_at * kTile + row]; row_norm = p.row_norm[row_at * kTile + row] * sqrtf((float)a.D); }
+    const float norm_top = KIND == kDk ? r2.info[row_at].top * sqrtf((float)a.D) : 0.f;
+    float acc[32 * G];
+#pragma unroll
+    for (int i = 0; i < 32 * G; ++i) acc[i] = 0.f;
+    float most = -INFINITY, sum = 0.f;                                 // fwd
+    float alpha = 1.f, out_factor = 0.f;                               // of the product in flight
+    float slope = 0.f;
+    int slope_head = -1;
+
+    const auto arrive = [&](uint64_t* bar) { tcgen05_fence_before(); __syncwarp(); if (lane == 0) mbar_arrive(bar); };
+    const auto wait_for = [&](uint64_t* bar, uint32_t parity) { mbar_wait_mark(bar, parity, abort_flag, bad); __syncwarp(); tcgen05_fence_after(); };
+    const auto add_up = [&](int n) {
+      const int out = kOuts == 2 ? n & 1 : 0;
+      wait_for(&o_full[out], (n / kOuts) & 1);
+      const bool scaled = KIND == kFwd && __any_sync(0xffffffffu, alpha != 1.f);
+#pragma unroll
+      for (int c = 0; c < G; ++c) {
+        float o[32];
+        tmem_ld32(mine + S::kOutAt + out * 64 * G + half * 32 * G + 32 * c, o);
+        tmem_ld_wait();
+        if (scaled) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) acc[32 * c + k] = fmaf(o[k], out_factor, acc[32 * c + k] * alpha);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) acc[32 * c + k] = fmaf(o[k], out_factor, acc[32 * c + k]);
+        }
+      }
+      arrive(&o_empty[out]);
+    };
+
+    int n = 0;
+    while (walk.next(lane, head, t, all)) {
+      const int64_t at = col_at(head, t);
+      const TileInfo &i1 = c1.info[at], &i2 = c2.info[at];
+      const float f = inv1 * i1.inv * unit;
+      if (a.slopes && slope_head != (kRowsAreKeys ? head : row_head)) { slope_head = kRowsAreKeys ? head : row_head; slope = __ldg(a.slopes + slope_head) * kLog2e; }
+      const int col0 = t * kTile + (kRowsAreKeys ? off : 0) + half * 64;                        // position of the first column
+      const int at_row = kRowsAreKeys ? self : self + off;
+      const bool masked = !all || careful;
+      // scores of a chunk of 32 columns, capped and biased, in units of log 2; inner: the cap's tanh
+      const auto score32 = [&](float* z, float* inner, int c) {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) z[k] *= f;
+        if (CAP) {
+          tanh32(z);
+#pragma unroll
+          for (int k = 0; k < 32; ++k) { if (inner) inner[k] = z[k]; z[k] *= wide; }
+        }
+        if (a.slopes) {
+          const float away = (float)(at_row - (col0 + 32 * c));
+#pragma unroll
+          for (int k = 0; k < 32; ++k) z[k] = fmaf(-slope, fabsf(away - (float)k), z[k]);
+        }
+      };
+      // which of a chunk's columns the row sees, and which of those make it NaN
+      const auto seen32 = [&](int c, uint32_t& spoils) {
+        const int first = col0 + 32 * c;
+        uint32_t seen = bits_between(lo - first, hi - first) | bits_between(-1, extra - 1 - first);
+        if (p.documents) {
+          uint32_t same = 0u;
+          const float* const from = a.documents + (int64_t)b * a.Tk;
+#pragma unroll 8
+          for (int k = 0; k < 32; ++k) if (first + k < a.Tk && __ldg(from + first + k) == document) same |= 1u << k;
+          seen &= document >= 0.f ? same : 0u;
+        }
+        spoils = seen & (spoiled ? 0xffffffffu : i1.bad[half * 2 + c] | i2.bad[half * 2 + c]);
+        return seen;
+      };
+
+      if (KIND == kFwd) {
+        float z[64];
+        wait_for(&s_full[n & 1], (n >> 1) & 1);
+        tmem_ld32(mine + (n & 1) * 128 + half * 64, z);
+        tmem_ld32(mine + (n & 1) * 128 + half * 64 + 32, z + 32);
+        tmem_ld_wait();
+        float m = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          score32(z + 32 * c, nullptr, c);
+          if (masked) {
+            uint32_t spoils;
+            const uint32_t seen = seen32(c, spoils);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) z[32 * c + k] = (seen >> k) & 1u ? z[32 * c + k] : -INFINITY;
+            if (spoils) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) if ((spoils >> k) & 1u) z[32 * c + k] = NAN;
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 32; ++k) m = fmaxf(m, z[32 * c + k]);
+        }
+        float* const others = exchange + (n & 1) * 256;
+        others[half * 128 + row] = m;
+        asm volatile("barrier.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+        m = fmaxf(most, fmaxf(m, others[(half ^ 1) * 128 + row]));
+        const float base = max_of_finite_or(m), shifted = base - (float)kWeightExp, faded = exp2_fast(most - base);
+        most = m;
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < 64; ++k) { z[k] = exp2_fast(z[k] - shifted); s += z[k]; }
+        sum = sum * faded + s;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t words[32];
+          split32(z + 32 * c, words);
+          tmem_st32(mine + (n & 1) * 128 + half * 64 + 32 * c, words);
+        }
+        tmem_st_wait();
+        arrive(&w_full[n & 1]);
+        if (n > 0) add_up(n - 1);
+        alpha = faded;
+        out_factor = i2.inv;
+      } else {
+        float factor, kk = 0.f, fy = 0.f;
+        int shift = kWeightExp;
+        if (KIND == kDv) {
+          factor = i2.inv * power_of_two(-kWeightExp);
+        } else {
+          const float bound = KIND == kDq ? fmaf(row_norm, i2.top, fabsf(row_delta)) : fmaf(i2.norm, norm_top, i2.delta);
+          shift = min(100, max(-100, kWeightExp - exponent_of(bound)));
+          factor = i1.inv * power_of_two(-shift);
+          fy = inv2 * i2.inv;
+        }
+        kk = (float)shift;
+        const float* const col_max = kRowsAreKeys ? p.row_max + at * kTile + half * 64 : nullptr;
+        const float* const col_delta = kRowsAreKeys ? p.row_delta + at * kTile + half * 64 : nullptr;
+        wait_for(&s_full[n & 1], (n >> 1) & 1);
+        if (kTwo) wait_for(y_full, n & 1);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float z[32], y[32], inner[CAP ? 32 : 1];
+          tmem_ld32(mine + (n & 1) * 128 + half * 64 + 32 * c, z);
+          if (kTwo) tmem_ld32(mine + 256 + half * 64 + 32 * c, y);
+          tmem_ld_wait();
+          if (kTwo && c == 1) arrive(y_empty);
+          score32(z, CAP ? inner : nullptr, c);
+          if (kRowsAreKeys) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 4) {
+              const float4 m4 = __ldg(reinterpret_cast<const float4*>(col_max + 32 * c + k));
+              z[k] += kk - m4.x; z[k + 1] += kk - m4.y; z[k + 2] += kk - m4.z; z[k + 3] += kk - m4.w;
+              if (KIND == kDk) {
+                const float4 d4 = __ldg(reinterpret_cast<const float4*>(col_delta + 32 * c + k));
+                y[k] = fmaf(y[k], fy, -d4.x); y[k + 1] = fmaf(y[k + 1], fy, -d4.y); y[k + 2] = fmaf(y[k + 2], fy, -d4.z); y[k + 3] = fmaf(y[k + 3], fy, -d4.w);
+              }
+            }
+          } else {
+            const float less = kk - row_max;
+#pragma unroll
+            for (int k = 0; k < 32; ++k) { z[k] += less; y[k] = fmaf(y[k], fy, -row_delta); }
+          }
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            z[k] = exp2_fast(z[k]);
+            if (kTwo) z[k] *= y[k];
+            if (kTwo && CAP) z[k] *= fmaf(-inner[k], inner[k], 1.f);
+          }
+          if (masked) {
+            uint32_t spoils;
+            const uint32_t seen = seen32(c, spoils);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) z[k] = (seen >> k) & 1u ? z[k] : 0.f;
+            if (spoils) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) if ((spoils >> k) & 1u) z[k] = NAN;
+            }
+          }
+          uint32_t words[32];
+          split32(z, words);
+          tmem_st32(mine + (n & 1) * 128 + half * 64 + 32 * c, words);
+        }
+        tmem_st_wait();
+        arrive(&w_full[n & 1]);
+        if (n > 0) add_up(n - 1);
+        out_factor = factor;
+      }
+      ++n;
+    }
+    if (n > 0) add_up(n - 1);
+
+    float last = KIND == kDv ? 1.f : a.scale;
+    if (KIND == kFwd) {
+      exchange[half * 128 + row] = sum;                                // the barrier of the last tile but one has passed for both
+      asm volatile("barrier.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+      sum = exchange[row] + exchange[128 + row];                       // in the same order in both
+      last = sum == 0.f ? 0.f : 1.f / sum;
+      if (a.stats && half == 0 && there) {
+        float* const to = a.stats + 2 * (((int64_t)b * a.H + row_head) * a.Tq + self);
+        to[0] = max_of_finite_or(most); to[1] = last * (float)(1 << kWeightExp);
+      }
+    }
+    if (there && !*abort_flag) {
+      float* const result = KIND == kFwd ? a.o : KIND == kDq ? a.dq : KIND == kDk ? a.dk : a.dv;
+      float* const to = result + (((int64_t)b * (kRowsAreKeys ? a.Tk : a.Tq) + self) * row_heads + row_head) * a.D + half * 32 * G;
+      const int cols = a.D - half * 32 * G;
+      if (a.D % 4 == 0 && (reinterpret_cast<uintptr_t>(result) & 15) == 0) {
+#pragma unroll
+        for (int k = 0; k < 32 * G; k += 4) if (k < cols) *reinterpret_cast<float4*>(to + k) = make_float4(acc[k] * last, acc[k + 1] * last, acc[k + 2] * last, acc[k + 3] * last);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 32 * G; ++k) if (k < cols) to[k] = acc[k] * last;
+      }
+    }
+  }
+
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+  if (threadIdx.x == 0 && *abort_flag && p.err) atomicExch(p.err, 1);
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------------
+template <int KIND, int G, bool CAP> cudaError_t launch_kind(const TcArgs& p, cudaStream_t s) {
+  static std::atomic<uint64_t> ready{0};
+  const auto kernel = attention_tc_kernel<KIND, G, CAP>;
+  const int bytes = Shape<KIND, G>::kSmem;
+  const cudaError_t e = once_per_device(ready, [kernel, bytes] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
+  if (e != cudaSuccess) return e;
+  constexpr bool kRowsAreKeys = Shape<KIND, G>::kRowsAreKeys;
+  return launch_dep(kernel, dim3((unsigned)(p.a.B * (kRowsAreKeys ? p.a.G : p.a.H)), (unsigned)(kRowsAreKeys ? p.k_tiles : p.q_tiles)), dim3(kThreads), (size_t)bytes, s, p);
+}
+template <int KIND> cudaError_t launch_any(const TcArgs& p, cudaStream_t s) {
+  const bool cap = p.a.cap > 0.f;
+  if (p.a.D <= 64) return cap ? launch_kind<KIND, 1, true>(p, s) : launch_kind<KIND, 1, false>(p, s);
+  return cap ? launch_kind<KIND, 2, true>(p, s) : launch_kind<KIND, 2, false>(p, s);
+}
+
+}  // namespace
+
+// Whether the path takes the call: heads of up to 128 elements, grids that the launch can have
+bool attention_tc_takes(const AttentionArgs& a) {
+  const int64_t q_tiles = (a.Tq + kTile - 1) / kTile, k_tiles = (a.Tk + kTile - 1) / kTile;
+  return a.D <= 128 && a.Tk > 0 && std::max(q_tiles, k_tiles) <= 65535 && (int64_t)a.B * (2 * a.H * q_tiles + 2 * a.G * k_tiles) < (1ll << 31);
+}
+// Scratch, in bytes, of a forward or a backward call; with `base`, where its parts lie
+static size_t lay_out(const AttentionArgs& a, bool backward, char* base, PackArgs* pack, TcArgs* tc) {
+  const int q_tiles = (a.Tq + kTile - 1) / kTile, k_tiles = (a.Tk + kTile - 1) / kTile, g = a.D <= 64 ? 1 : 2;
+  const size_t nq = (size_t)a.B * a.H * q_tiles, nk = (size_t)a.B * a.G * k_tiles, image = (size_t)2 * g * 16384;
+  size_t at = 0;
+  const auto take = [&](size_t bytes) { const size_t from = at; at += (bytes + 255) / 256 * 256; return base ? base + from : nullptr; };
+  const int jobs = backward ? 4 : 3;
+  const float* const from[4] = {a.q, a.k, a.v, a.dout};
+  Packed* const to[4] = {tc ? &tc->q : nullptr, tc ? &tc->k : nullptr, tc ? &tc->v : nullptr, tc ? &tc->d : nullptr};
+  int blocks = 0;
+  for (int j = 0; j < jobs; ++j) {
+    const bool queries = j == 0 || j == 3;
+    const size_t n = queries ? nq : nk;
+    char* const img = take(n * image);
+    char* const info = take(n * sizeof(TileInfo));
+    if (base) {
+      pack->job[j] = PackJob{from[j], img, (TileInfo*)info, queries ? a.H : a.G, queries ? a.Tq : a.Tk, queries ? q_tiles : k_tiles, j == 3};
+      pack->first[j] = blocks;
+      *to[j] = Packed{img, (const TileInfo*)info};
+    }
+    blocks += (int)n;
+  }
+  char* rows[3] = {nullptr, nullptr, nullptr};
+  if (backward) for (char*& r : rows) r = take(nq * kTile * sizeof(float));
+  char* const docs = a.documents ? take((size_t)a.B * k_tiles * sizeof(float4)) : nullptr;
+  if (base) {
+    pack->a = a; pack->jobs = jobs; pack->first[jobs] = blocks; pack->document_job = 1;
+    pack->row_max = (float*)rows[0]; pack->row_delta = (float*)rows[1]; pack->row_norm = (float*)rows[2]; pack->documents = (float4*)docs;
+    tc->a = a; tc->row_max = pack->row_max; tc->row_delta = pack->row_delta; tc->row_norm = pack->row_norm; tc->documents = pack->documents;
+    tc->q_tiles = q_tiles; tc->k_tiles = k_tiles; tc->D16 = (a.D + 15) / 16 * 16; tc->err = tensor_error_word();
+  }
+  return at;
+}
+// 0: launched; -1: error; 1: short of *bytes
+int attention_tc(const AttentionArgs& a, bool backward, size_t* bytes, cudaStream_t s, const char* what) {
+  TF_REQUIRE(tensor_path_error() == 0, "%s: an earlier tensor-core kernel timed out on a barrier; refusing to launch", what);
+  StreamLease lease(s);
+  *bytes = lay_out(a, backward, nullptr, nullptr, nullptr);
+  char* const base = (char*)lease.scratch(kScratchAttention, *bytes);
+  if (!base) return 1;
+  PackArgs pack;
+  TcArgs tc;
+  memset(&pack, 0, sizeof(pack));
+  memset(&tc, 0, sizeof(tc));
+  lay_out(a, backward, base, &pack, &tc);
+  uintptr_t bits = (uintptr_t)a.D * sizeof(float);
+  for (const void* x : {(const void*)a.q, (const void*)a.k, (const void*)a.v, (const void*)a.dout, (const void*)a.out}) bits |= reinterpret_cast<uintptr_t>(x);
+  const bool wide = bits % 16 == 0;
+  const dim3 blocks((unsigned)pack.first[pack.jobs]);
+  if (a.D <= 64) TF_CUDA(wide ? launch_dep(attention_pack_kernel<1, true>, blocks, dim3(256), 0, s, pack) : launch_dep(attention_pack_kernel<1, false>, blocks, dim3(256), 0, s, pack));
+  else TF_CUDA(wide ? launch_dep(attention_pack_kernel<2, true>, blocks, dim3(256), 0, s, pack) : launch_dep(attention_pack_kernel<2, false>, blocks, dim3(256), 0, s, pack));
+  TF_AFTER(s, what);
+  if (!backward) {
+    TF_CUDA(launch_any<kFwd>(tc, s));
+    TF_AFTER(s, what);
+    return 0;
+  }
+  if (a.dv) { TF_CUDA(launch_any<kDv>(tc, s)); TF_AFTER(s, what); }
+  if (a.dk) { TF_CUDA(launch_any<kDk>(tc, s)); TF_AFTER(s, what); }
+  if (a.dq) { TF_CUDA(launch_any<kDq>(tc, s)); TF_AFTER(s, what); }
+  return 0;
+}
+
+}  // namespace tf

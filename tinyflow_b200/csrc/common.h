@@ -237,7 +237,7 @@ void pool_free(void* p);
 // block to the last launch that uses it.  A block is the same at every call until a larger one is asked for; slot ids are per
 // purpose, so that what one operator uses together does not collide.
 struct StreamScratch;
-enum { kScratchSums = 0, kScratchTiles = 1, kScratchSplit = 2, kScratchContract = 3, kScratchPackA = 4, kScratchPackB = 5, kScratchGroup = 6, kScratchNorm = 7, kScratchGates = 8, kScratchSlots = 9 };
+enum { kScratchSums = 0, kScratchTiles = 1, kScratchSplit = 2, kScratchContract = 3, kScratchPackA = 4, kScratchPackB = 5, kScratchGroup = 6, kScratchNorm = 7, kScratchGates = 8, kScratchAttention = 9, kScratchSlots = 10 };
 class StreamLease {
  public:
   explicit StreamLease(cudaStream_t s);

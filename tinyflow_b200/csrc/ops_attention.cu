@@ -10,6 +10,11 @@
 #include "operands.h"
 
 namespace tf {
+
+bool attention_tc_takes(const AttentionArgs& a);
+int attention_tc(const AttentionArgs& a, bool backward, size_t* bytes, cudaStream_t s, const char* what);
+void note_contraction_path(int path);
+
 namespace {
 
 constexpr int kThreads = 128;
@@ -435,6 +440,19 @@ int check_attention(const char* what, const AttentionState* st, const DLArray* q
   a->causal = st->causal; a->window = std::min(st->window, 1 << 25); a->scale = st->scale; a->cap = st->cap;
   return 0;
 }
+bool tensor_path_pays(const AttentionArgs& a, bool backward) { return (int64_t)a.Tq >= 64 && a.Tk >= 64; }
+// 0: the exact kernels are to run, 1: launched, or short of memory; -1: error
+int run_tensor_path(const AttentionArgs& a, bool backward, int* memorytoSaving, cudaStream_t s, const char* what) {
+  if (contraction_path() == 1) return 0;
+  const bool takes = attention_tc_takes(a);
+  TF_REQUIRE(contraction_path() != 2 || takes, "%s: the tensor path takes heads of up to 128 elements and at least one key", what);
+  if (!takes || (contraction_path() == 0 && !tensor_path_pays(a, backward))) return 0;
+  size_t bytes = 0;
+  const int r = attention_tc(a, backward, &bytes, s, what);
+  if (r > 0 && memorytoSaving) *memorytoSaving = bytes > 0x7fffffffu ? 0x7fffffff : (int)bytes;
+  if (r >= 0) note_contraction_path(2);
+  return r < 0 ? -1 : 1;
+}
 const float* opt_in(const DLArray* a) { return a ? (const float*)a->data : nullptr; }
 
 }  // namespace
@@ -478,6 +496,8 @@ int TfAttentionForward(const DLArrayHandle query, const DLArrayHandle key, const
   if (a.B == 0) return 0;
   note_compute_stream(s);
   KernelTimer kt(what, s, 4.0 * a.B * a.H * (double)a.Tq * a.Tk * a.D, 4.0 * (2.0 * numel(query) + 2.0 * numel(key)));
+  if (const int r = run_tensor_path(a, false, memorytoSaving, s, what)) return r < 0 ? -1 : 0;
+  note_contraction_path(1);
   TF_CUDA(tile_fwd(a, s));
   TF_AFTER(s, what);
   return 0;
@@ -504,6 +524,8 @@ int TfAttentionBackward(const DLArrayHandle query, const DLArrayHandle key, cons
   if (a.B == 0 || !(a.dq || a.dk || a.dv)) return 0;
   note_compute_stream(s);
   KernelTimer kt(what, s, 10.0 * a.B * a.H * (double)a.Tq * a.Tk * a.D, 4.0 * (4.0 * nq + 4.0 * nk));
+  if (const int r = run_tensor_path(a, true, memorytoSaving, s, what)) return r < 0 ? -1 : 0;
+  note_contraction_path(1);
   TF_CUDA(tile_bwd(a, s));
   TF_AFTER(s, what);
   return 0;
