@@ -36,7 +36,9 @@ namespace {
 
 enum { kFwd, kDq, kDk, kDv };
 constexpr int kTile = 128;
-constexpr int kThreads = 320;                    // warps: 0 copies, 1 issues MMAs and owns TMEM, 2-9 weights
+constexpr int kThreads = 384;                    // warps: 0 copies, 1 issues MMAs and owns TMEM, 2 and 3 idle, 4-11 weights
+// Registers a thread: 168 at the launch (64,512 of the block); the first four warps give 112 of theirs, the others take 56 each, the same sum.
+constexpr int kFewRegisters = 56, kManyRegisters = 224;
 constexpr int kWeightExp = 14;                   // weights are scaled to below 2^15
 constexpr int kFar = 1 << 26;                    // beyond every position
 
@@ -82,12 +84,12 @@ __device__ __forceinline__ uint32_t halves(float a, float b) {
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
 __device__ __forceinline__ int exponent_of(float positive) { return (int)((__float_as_uint(positive) >> 23) & 255u) - 127; }
 
-// A block of 256 threads packs one tile of one head.  16 G threads a row, 4 columns each.
+// A block of 512 threads packs one tile of one head, two blocks an SM.  16 G threads a row, 4 columns each.  HBM-bound: 4 bytes an element read and written, for dout 8 read.
+constexpr int kPackThreads = 512, kPackWarps = kPackThreads / 32;
 template <int G, bool WIDE>
-__global__ void __launch_bounds__(256) attention_pack_kernel(const __grid_constant__ PackArgs p) {
-  constexpr int kAcross = 16 * G, kRowsAtOnce = 32 / kAcross, kSteps = 16 / kRowsAtOnce;      // a warp packs 16 rows
-  __shared__ float red[8];
-  __shared__ float red_norm[8], red_delta[8];
+__global__ void __launch_bounds__(kPackThreads, 2) attention_pack_kernel(const __grid_constant__ PackArgs p) {
+  constexpr int kAcross = 16 * G, kRowsAtOnce = 32 / kAcross, kRowsOfWarp = kTile / kPackWarps, kSteps = kRowsOfWarp / kRowsAtOnce;
+  __shared__ float red[kPackWarps], red_norm[kPackWarps], red_delta[kPackWarps];
   __shared__ uint32_t bad_words[4];
   grid_dep_sync();
   int j = 0;
@@ -99,56 +101,63 @@ __global__ void __launch_bounds__(256) attention_pack_kernel(const __grid_consta
   if (threadIdx.x < 4) bad_words[threadIdx.x] = 0u;
   float v[kSteps][4];
   float most = 0.f, most_norm = 0.f, most_delta = 0.f;
-  __syncthreads();
+  const auto load4 = [&](const float* from, int t, float* w) {
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    const int r = warp * 16 + s * kRowsAtOnce + sub, t = tile * kTile + r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[s][i] = 0.f;
+    for (int i = 0; i < 4; ++i) w[i] = 0.f;
     if (t < job.length && col < D) {
-      const float* const from = job.x + (((int64_t)b * job.length + t) * job.heads + h) * D + col;
-      if (WIDE) { const float4 w = __ldg(reinterpret_cast<const float4*>(from)); v[s][0] = w.x; v[s][1] = w.y; v[s][2] = w.z; v[s][3] = w.w; }
+      from += (((int64_t)b * job.length + t) * job.heads + h) * D + col;
+      if (WIDE) { const float4 x = __ldg(reinterpret_cast<const float4*>(from)); w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w; }
       else
 #pragma unroll
-        for (int i = 0; i < 4; ++i) if (col + i < D) v[s][i] = __ldg(from + i);
+        for (int i = 0; i < 4; ++i) if (col + i < D) w[i] = __ldg(from + i);
+    }
+  };
+  const auto row_of = [&](int s) { return warp * kRowsOfWarp + s * kRowsAtOnce + sub; };
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) load4(job.x, tile * kTile + row_of(s), v[s]);
+  __syncthreads();
+  uint32_t unfit = 0u;                           // steps whose row's statistics are not finite
+  if (job.gradient) {
+#pragma unroll
+    for (int s0 = 0; s0 < kSteps; s0 += 4) {
+      float o[4][4], stat_max[4], stat_inv[4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int t = tile * kTile + row_of(s0 + s);
+        load4(p.a.out, t, o[s]);
+        const int64_t stat = 2 * (((int64_t)b * job.heads + h) * job.length + t);
+        stat_max[s] = t < job.length ? __ldg(p.a.stats + stat) : 0.f;
+        stat_inv[s] = t < job.length ? __ldg(p.a.stats + stat + 1) : 0.f;
+      }
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        float delta = 0.f, norm = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float& w = v[s0 + s][i];
+          w *= stat_inv[s];
+          delta = fmaf(w, o[s][i], delta);
+          norm = fmaf(w, w, norm);
+        }
+#pragma unroll
+        for (int k = kAcross / 2; k > 0; k >>= 1) { delta += __shfl_xor_sync(0xffffffffu, delta, k); norm += __shfl_xor_sync(0xffffffffu, norm, k); }
+        norm = sqrtf(norm);
+        if (!(fabsf(delta) < INFINITY && norm < INFINITY && fabsf(stat_max[s]) < INFINITY && fabsf(stat_inv[s]) < INFINITY)) {
+          unfit |= 1u << (s0 + s);
+          stat_max[s] = delta = norm = 0.f;
+        }
+        if (col == 0) {
+          const int64_t at = ((int64_t)bh * job.tiles + tile) * kTile + row_of(s0 + s);
+          p.row_max[at] = stat_max[s]; p.row_delta[at] = delta; p.row_norm[at] = norm;
+        }
+        most_norm = fmaxf(most_norm, norm); most_delta = fmaxf(most_delta, fabsf(delta));
+      }
     }
   }
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
-    const int r = warp * 16 + s * kRowsAtOnce + sub, t = tile * kTile + r;
-    bool fine = true;
-    float stat_max = 0.f, stat_inv = 1.f, delta = 0.f, norm = 0.f;
-    if (job.gradient) {
-      stat_inv = 0.f;
-      float o[4] = {0.f, 0.f, 0.f, 0.f};
-      if (t < job.length) {
-        const int64_t stat = ((int64_t)b * job.heads + h) * job.length + t;
-        stat_max = __ldg(p.a.stats + 2 * stat); stat_inv = __ldg(p.a.stats + 2 * stat + 1);
-        if (col < D) {
-          const float* const from = p.a.out + (((int64_t)b * job.length + t) * job.heads + h) * D + col;
-          if (WIDE) { const float4 w = __ldg(reinterpret_cast<const float4*>(from)); o[0] = w.x; o[1] = w.y; o[2] = w.z; o[3] = w.w; }
-          else
-#pragma unroll
-            for (int i = 0; i < 4; ++i) if (col + i < D) o[i] = __ldg(from + i);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[s][i] *= stat_inv;
-        delta = fmaf(v[s][i], o[i], delta);
-        norm = fmaf(v[s][i], v[s][i], norm);
-      }
-#pragma unroll
-      for (int o2 = kAcross / 2; o2 > 0; o2 >>= 1) { delta += __shfl_xor_sync(0xffffffffu, delta, o2); norm += __shfl_xor_sync(0xffffffffu, norm, o2); }
-      norm = sqrtf(norm);
-      fine = fabsf(delta) < INFINITY && norm < INFINITY && fabsf(stat_max) < INFINITY && fabsf(stat_inv) < INFINITY;
-      if (!fine) { stat_max = 0.f; delta = 0.f; norm = 0.f; }
-      if (col == 0) {
-        const int64_t at = ((int64_t)bh * job.tiles + tile) * kTile + r;
-        p.row_max[at] = stat_max; p.row_delta[at] = delta; p.row_norm[at] = norm;
-      }
-      most_norm = fmaxf(most_norm, norm); most_delta = fmaxf(most_delta, fabsf(delta));
-    }
+    const int r = row_of(s);
+    bool fine = !((unfit >> s) & 1u);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (!(fabsf(v[s][i]) < INFINITY)) { v[s][i] = 0.f; fine = false; }
@@ -164,9 +173,9 @@ __global__ void __launch_bounds__(256) attention_pack_kernel(const __grid_consta
   }
   if (lane == 0) { red[warp] = most; red_norm[warp] = most_norm; red_delta[warp] = most_delta; }
   __syncthreads();
-  most = red[lane & 7]; most_norm = red_norm[lane & 7]; most_delta = red_delta[lane & 7];
+  most = red[lane & (kPackWarps - 1)]; most_norm = red_norm[lane & (kPackWarps - 1)]; most_delta = red_delta[lane & (kPackWarps - 1)];
 #pragma unroll
-  for (int o = 4; o > 0; o >>= 1) {
+  for (int o = kPackWarps / 2; o > 0; o >>= 1) {
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
     most_norm = fmaxf(most_norm, __shfl_xor_sync(0xffffffffu, most_norm, o));
     most_delta = fmaxf(most_delta, __shfl_xor_sync(0xffffffffu, most_delta, o));
@@ -183,7 +192,7 @@ __global__ void __launch_bounds__(256) attention_pack_kernel(const __grid_consta
   char* const image = job.image + ((int64_t)bh * job.tiles + tile) * (2 * G * 16384);
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
-    const int r = warp * 16 + s * kRowsAtOnce + sub;
+    const int r = row_of(s);
     float hi[4], x[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) { x[i] = v[s][i] * scale; hi[i] = __half2float(__float2half_rn(x[i])); }
@@ -341,7 +350,7 @@ __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {              
 }
 
 template <int KIND, int G, bool CAP>
-__global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_constant__ TcArgs p) {
+__device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
   using S = Shape<KIND, G>;
   constexpr bool kTwo = S::kTwo, kRowsAreKeys = S::kRowsAreKeys;
   constexpr int kPart = S::kPart, kStages = S::kStages, kOuts = S::kOuts;
@@ -385,9 +394,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   grid_dep_sync();
 
   // rows that see most go first
-  const int row_heads = kRowsAreKeys ? a.G : a.H, b = blockIdx.x / row_heads, row_head = blockIdx.x - b * row_heads;
-  const int tile = kRowsAreKeys ? (int)blockIdx.y : (int)(gridDim.y - 1 - blockIdx.y);
-  const int col_tiles = kRowsAreKeys ? p.q_tiles : p.k_tiles, row_tiles = kRowsAreKeys ? p.k_tiles : p.q_tiles;
+  const int row_heads = kRowsAreKeys ? a.G : a.H, col_tiles = kRowsAreKeys ? p.q_tiles : p.k_tiles, row_tiles = kRowsAreKeys ? p.k_tiles : p.q_tiles;
+  const int order = block / (a.B * row_heads), lane_of = block - order * (a.B * row_heads), b = lane_of / row_heads, row_head = lane_of - b * row_heads;
+  const int tile = kRowsAreKeys ? order : row_tiles - 1 - order;
   const int64_t row_at = ((int64_t)b * row_heads + row_head) * row_tiles + tile;
   const Packed &r1 = kRowsAreKeys ? p.k : p.q, &r2 = kRowsAreKeys ? p.v : p.d;                 // rows
   const Packed &c1 = kRowsAreKeys ? p.q : p.k, &c2 = kRowsAreKeys ? p.d : p.v;                 // columns
@@ -396,6 +405,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   int head, t, bad = *abort_flag;
   bool all;
 
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
   if (warp == 0) {
     // ---- copies: the rows once, then tiles in the order in which the MMAs take them, the lo half first
     int stage = 0;
@@ -516,9 +527,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
       ++n;
     }
     if (n > 0) product(n - 1);
+  }
   } else {
     // ---- weights
-    const int quarter = warp & 3, half = (warp - 2) >> 2, row = quarter * 32 + lane;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
+    const int quarter = warp & 3, half = (warp - 4) >> 2, row = quarter * 32 + lane;
     const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
     const int off = a.Tk - a.Tq, self = tile * kTile + row;            // query or key
     const bool there = self < (kRowsAreKeys ? a.Tk : a.Tq);
@@ -602,9 +615,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
         uint32_t seen = bits_between(lo - first, hi - first) | bits_between(-1, extra - 1 - first);
         if (p.documents) {
           uint32_t same = 0u;
-          const float* const from = a.documents + (int64_t)b * a.Tk;
-#pragma unroll 8
-          for (int k = 0; k < 32; ++k) if (first + k < a.Tk && __ldg(from + first + k) == document) same |= 1u << k;
+          const float theirs = document_of(a, b, first + lane);
+#pragma unroll
+          for (int k = 0; k < 32; ++k) same |= __shfl_sync(0xffffffffu, theirs, k) == document ? 1u << k : 0u;
           seen &= document >= 0.f ? same : 0u;
         }
         spoils = seen & (spoiled ? 0xffffffffu : i1.bad[half * 2 + c] | i2.bad[half * 2 + c]);
@@ -757,20 +770,35 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tc_kernel(const __grid_
   if (threadIdx.x == 0 && *abort_flag && p.err) atomicExch(p.err, 1);
 }
 
-// ---- host side ------------------------------------------------------------------------------------------------------------
-template <int KIND, int G, bool CAP> cudaError_t launch_kind(const TcArgs& p, cudaStream_t s) {
-  static std::atomic<uint64_t> ready{0};
-  const auto kernel = attention_tc_kernel<KIND, G, CAP>;
-  const int bytes = Shape<KIND, G>::kSmem;
-  const cudaError_t e = once_per_device(ready, [kernel, bytes] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
-  if (e != cudaSuccess) return e;
-  constexpr bool kRowsAreKeys = Shape<KIND, G>::kRowsAreKeys;
-  return launch_dep(kernel, dim3((unsigned)(p.a.B * (kRowsAreKeys ? p.a.G : p.a.H)), (unsigned)(kRowsAreKeys ? p.k_tiles : p.q_tiles)), dim3(kThreads), (size_t)bytes, s, p);
+template <int G, bool CAP> __global__ void __launch_bounds__(kThreads, 1) attention_tc_fwd_kernel(const __grid_constant__ TcArgs p) { attention_rows<kFwd, G, CAP>(p, blockIdx.x); }
+// All gradients in one launch, the longest first: dk and dv of the first keys see all queries of all heads that share them.
+template <int G, bool CAP> __global__ void __launch_bounds__(kThreads, 1) attention_tc_bwd_kernel(const __grid_constant__ TcArgs p, int dk_blocks, int dv_blocks) {
+  const int block = blockIdx.x;
+  if (block < dk_blocks) attention_rows<kDk, G, CAP>(p, block);
+  else if (block < dk_blocks + dv_blocks) attention_rows<kDv, G, CAP>(p, block - dk_blocks);
+  else attention_rows<kDq, G, CAP>(p, block - dk_blocks - dv_blocks);
 }
-template <int KIND> cudaError_t launch_any(const TcArgs& p, cudaStream_t s) {
-  const bool cap = p.a.cap > 0.f;
-  if (p.a.D <= 64) return cap ? launch_kind<KIND, 1, true>(p, s) : launch_kind<KIND, 1, false>(p, s);
-  return cap ? launch_kind<KIND, 2, true>(p, s) : launch_kind<KIND, 2, false>(p, s);
+
+// ---- host side ------------------------------------------------------------------------------------------------------------
+template <int G, bool CAP> cudaError_t launch_fwd(const TcArgs& p, cudaStream_t s) {
+  static std::atomic<uint64_t> ready{0};
+  const auto kernel = attention_tc_fwd_kernel<G, CAP>;
+  const int bytes = Shape<kFwd, G>::kSmem;
+  const cudaError_t e = once_per_device(ready, [kernel, bytes] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
+  return e != cudaSuccess ? e : launch_dep(kernel, dim3((unsigned)(p.a.B * p.a.H * p.q_tiles)), dim3(kThreads), (size_t)bytes, s, p);
+}
+template <int G, bool CAP> cudaError_t launch_bwd(const TcArgs& p, cudaStream_t s) {
+  static std::atomic<uint64_t> ready{0};
+  const auto kernel = attention_tc_bwd_kernel<G, CAP>;
+  const int bytes = std::max(std::max(Shape<kDq, G>::kSmem, Shape<kDk, G>::kSmem), Shape<kDv, G>::kSmem);
+  const cudaError_t e = once_per_device(ready, [kernel, bytes] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
+  const int keys = p.a.B * p.a.G * p.k_tiles, dk = p.a.dk ? keys : 0, dv = p.a.dv ? keys : 0, dq = p.a.dq ? p.a.B * p.a.H * p.q_tiles : 0;
+  return e != cudaSuccess ? e : launch_dep(kernel, dim3((unsigned)(dk + dv + dq)), dim3(kThreads), (size_t)bytes, s, p, dk, dv);
+}
+template <class F> cudaError_t with_form(const AttentionArgs& a, F&& f) {
+  const bool cap = a.cap > 0.f;
+  if (a.D <= 64) return cap ? f(std::integral_constant<int, 1>(), std::true_type()) : f(std::integral_constant<int, 1>(), std::false_type());
+  return cap ? f(std::integral_constant<int, 2>(), std::true_type()) : f(std::integral_constant<int, 2>(), std::false_type());
 }
 
 }  // namespace
@@ -778,7 +806,7 @@ template <int KIND> cudaError_t launch_any(const TcArgs& p, cudaStream_t s) {
 // Whether the path takes the call: heads of up to 128 elements, grids that the launch can have
 bool attention_tc_takes(const AttentionArgs& a) {
   const int64_t q_tiles = (a.Tq + kTile - 1) / kTile, k_tiles = (a.Tk + kTile - 1) / kTile;
-  return a.D <= 128 && a.Tk > 0 && std::max(q_tiles, k_tiles) <= 65535 && (int64_t)a.B * (2 * a.H * q_tiles + 2 * a.G * k_tiles) < (1ll << 31);
+  return a.D <= 128 && a.Tk > 0 && (int64_t)a.B * (2 * a.H * q_tiles + 2 * a.G * k_tiles) < (1ll << 31);
 }
 // Scratch, in bytes, of a forward or a backward call; with `base`, where its parts lie
 static size_t lay_out(const AttentionArgs& a, bool backward, char* base, PackArgs* pack, TcArgs* tc) {
@@ -829,17 +857,11 @@ int attention_tc(const AttentionArgs& a, bool backward, size_t* bytes, cudaStrea
   for (const void* x : {(const void*)a.q, (const void*)a.k, (const void*)a.v, (const void*)a.dout, (const void*)a.out}) bits |= reinterpret_cast<uintptr_t>(x);
   const bool wide = bits % 16 == 0;
   const dim3 blocks((unsigned)pack.first[pack.jobs]);
-  if (a.D <= 64) TF_CUDA(wide ? launch_dep(attention_pack_kernel<1, true>, blocks, dim3(256), 0, s, pack) : launch_dep(attention_pack_kernel<1, false>, blocks, dim3(256), 0, s, pack));
-  else TF_CUDA(wide ? launch_dep(attention_pack_kernel<2, true>, blocks, dim3(256), 0, s, pack) : launch_dep(attention_pack_kernel<2, false>, blocks, dim3(256), 0, s, pack));
+  if (a.D <= 64) TF_CUDA(wide ? launch_dep(attention_pack_kernel<1, true>, blocks, dim3(kPackThreads), 0, s, pack) : launch_dep(attention_pack_kernel<1, false>, blocks, dim3(kPackThreads), 0, s, pack));
+  else TF_CUDA(wide ? launch_dep(attention_pack_kernel<2, true>, blocks, dim3(kPackThreads), 0, s, pack) : launch_dep(attention_pack_kernel<2, false>, blocks, dim3(kPackThreads), 0, s, pack));
   TF_AFTER(s, what);
-  if (!backward) {
-    TF_CUDA(launch_any<kFwd>(tc, s));
-    TF_AFTER(s, what);
-    return 0;
-  }
-  if (a.dv) { TF_CUDA(launch_any<kDv>(tc, s)); TF_AFTER(s, what); }
-  if (a.dk) { TF_CUDA(launch_any<kDk>(tc, s)); TF_AFTER(s, what); }
-  if (a.dq) { TF_CUDA(launch_any<kDq>(tc, s)); TF_AFTER(s, what); }
+  TF_CUDA(with_form(a, [&](auto g, auto cap) { return backward ? launch_bwd<decltype(g)::value, decltype(cap)::value>(tc, s) : launch_fwd<decltype(g)::value, decltype(cap)::value>(tc, s); }));
+  TF_AFTER(s, what);
   return 0;
 }
 
