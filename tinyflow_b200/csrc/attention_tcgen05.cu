@@ -36,9 +36,11 @@ namespace {
 
 enum { kFwd, kDq, kDk, kDv };
 constexpr int kTile = 128;
-constexpr int kThreads = 384;                    // warps: 0 copies, 1 issues MMAs and owns TMEM, 2 and 3 idle, 4-11 weights
-// Registers a thread: 168 at the launch (64,512 of the block); the first four warps give 112 of theirs, the others take 56 each, the same sum.
-constexpr int kFewRegisters = 56, kManyRegisters = 224;
+constexpr int kParts = 2;                        // warps that share the columns of a TMEM lane quarter
+constexpr int kWeightWarps = 4 * kParts, kThreads = 128 + 32 * kWeightWarps;       // warps: 0 copies, 1 issues MMAs and owns TMEM, 2 and 3 idle, the others make weights
+constexpr int kChunks = 4 / kParts;                  // of 32 columns, a thread
+// Registers a thread: what the launch has (168 x 384 = 64,512 or 96 x 640 = 61,440), dealt anew: the sums are the same.
+constexpr int kFewRegisters = kParts == 2 ? 56 : 64, kManyRegisters = kParts == 2 ? 224 : 104;
 constexpr int kWeightExp = 14;                   // weights are scaled to below 2^15
 constexpr int kFar = 1 << 26;                    // beyond every position
 
@@ -291,7 +293,7 @@ template <int KIND, int G> struct Shape {
   static constexpr bool kRowsAreKeys = KIND == kDk || KIND == kDv;
   static constexpr int kPart = G * 16384;                            // one half (hi or lo) of a tile
   static constexpr int kResident = (kTwo ? 4 : 2) * kPart;
-  static constexpr int kControl = 3072;
+  static constexpr int kControl = 256 + (KIND == kFwd ? 2 * kParts * 128 * 4 : 0);
   static constexpr int kStages = (232448 - kControl - kResident) / kPart < 8 ? (232448 - kControl - kResident) / kPart : 8;
   static constexpr int kSmem = kResident + kStages * kPart + kControl;
   static constexpr int kOuts = kTwo && G == 2 ? 1 : 2;               // TMEM: scores 0 and 128, second scores 256, products behind
@@ -303,13 +305,14 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t keep) {
+// Descriptors in two words each
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_low, uint32_t a_high, uint32_t b_low, uint32_t b_high, uint32_t idesc, uint32_t keep) {
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(keep) : "memory");
+               ::"r"(d), "l"((uint64_t)a_low | (uint64_t)a_high << 32), "l"((uint64_t)b_low | (uint64_t)b_high << 32), "r"(idesc), "r"(keep) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t keep) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_low, uint32_t b_high, uint32_t idesc, uint32_t keep) {
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(keep) : "memory");
+               ::"r"(d), "r"(a), "l"((uint64_t)b_low | (uint64_t)b_high << 32), "r"(idesc), "r"(keep) : "memory");
 }
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float reciprocal(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
@@ -349,7 +352,7 @@ __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {              
   return lo <= 0 ? below : lo > 31 ? 0u : below & (0xffffffffu << lo);
 }
 
-template <int KIND, int G, bool CAP>
+template <int KIND, int G, bool SHAPED>
 __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
   using S = Shape<KIND, G>;
   constexpr bool kTwo = S::kTwo, kRowsAreKeys = S::kRowsAreKeys;
@@ -368,7 +371,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
   uint64_t* const o_empty = o_full + 2;          // [2] and has been added up
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 2);
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* const exchange = reinterpret_cast<float*>(full + 32);       // [2][2][128]
+  float* const exchange = reinterpret_cast<float*>(full + 32);       // [2][kParts][128]
   const AttentionArgs& a = p.a;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
@@ -376,8 +379,8 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     if (lane == 0) {
       for (int i = 0; i < kStages; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
       mbar_init(resident_full, 1);
-      for (int i = 0; i < 2; ++i) { mbar_init(s_full + i, 1); mbar_init(w_full + i, 8); mbar_init(o_full + i, 1); mbar_init(o_empty + i, 8); }
-      mbar_init(y_full, 1); mbar_init(y_empty, 8);
+      for (int i = 0; i < 2; ++i) { mbar_init(s_full + i, 1); mbar_init(w_full + i, kWeightWarps); mbar_init(o_full + i, 1); mbar_init(o_empty + i, kWeightWarps); }
+      mbar_init(y_full, 1); mbar_init(y_empty, kWeightWarps);
       *abort_flag = (smem_u32(smem) & 1023u) ? 1 : 0;                // nothing is issued then
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -462,23 +465,34 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     const int steps = p.D16 / 16;
     int stage = 0;
     uint32_t phase = 0;
-    const auto k_major = [](uint32_t at, int ks) { return umma_desc(at + (ks >> 2) * 16384 + (ks & 3) * 32, 16, 1024, 2); };
-    const auto wait_stage = [&] { mbar_wait_mark(&full[stage], phase, abort_flag, bad); bad = __any_sync(0xffffffffu, bad); tcgen05_fence_after(); };
+    // Descriptors differ in their low word alone, by constants from one MMA to the next
+    constexpr uint32_t kHigh = (1024u >> 4) | 1u << 14 | 2u << 29;
+    const auto k_major = [](uint32_t at) { return (at & 0x3FFFFu) >> 4 | 1u << 16; };
+    const auto mn_major = [](uint32_t at) { return (at & 0x3FFFFu) >> 4 | (16384u >> 4) << 16; };
+    const auto wait_stage = [&] { mbar_wait_mark(&full[stage], phase, abort_flag, bad); __syncwarp(); tcgen05_fence_after(); };
     const auto next_stage = [&] { if (++stage == kStages) { stage = 0; phase ^= 1; } };
-    const auto scores = [&](uint32_t d, uint32_t rows, uint64_t* done) {
+    const auto score_steps = [&](uint32_t d, uint32_t rows_low, uint32_t cols_low, uint32_t keep) {
+#pragma unroll
+      for (int ks = 0; ks < 4 * G; ++ks)
+        if (ks < steps) mma_ss(d, rows_low + (ks >> 2) * 1024 + (ks & 3) * 2, kHigh, cols_low + (ks >> 2) * 1024 + (ks & 3) * 2, kHigh, kScores, ks ? 1u : keep);
+    };
+    const auto product_steps = [&](uint32_t d, uint32_t w, uint32_t cols_low, uint32_t keep) {
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) mma_ts(d, w + 32 * (ks >> 1) + 8 * (ks & 1), cols_low + ks * 128, kHigh, products, ks ? 1u : keep);
+    };
+    const auto scores = [&](uint32_t d, uint32_t rows_hi, uint64_t* done) {
       wait_stage();
-      uint32_t at = smem_u32(ring + stage * kPart);
       if (!bad && elect_one()) {
-        for (int ks = 0; ks < steps; ++ks) mma_ss(d, k_major(rows, ks), k_major(at, ks), kScores, ks > 0);
+        score_steps(d, rows_hi, k_major(smem_u32(ring + stage * kPart)), 0u);
         tcgen05_commit(&empty[stage]);
       }
       __syncwarp();
       next_stage();
       wait_stage();
-      at = smem_u32(ring + stage * kPart);
       if (!bad && elect_one()) {
-        for (int ks = 0; ks < steps; ++ks) mma_ss(d, k_major(rows + kPart, ks), k_major(at, ks), kScores, 1u);
-        for (int ks = 0; ks < steps; ++ks) mma_ss(d, k_major(rows, ks), k_major(at, ks), kScores, 1u);
+        const uint32_t at = k_major(smem_u32(ring + stage * kPart));
+        score_steps(d, rows_hi + (kPart >> 4), at, 1u);
+        score_steps(d, rows_hi, at, 1u);
         tcgen05_commit(&empty[stage]);
         tcgen05_commit(done);
       }
@@ -490,24 +504,18 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
       const int out = kOuts == 2 ? n & 1 : 0;
       mbar_wait_mark(&w_full[n & 1], (n >> 1) & 1, abort_flag, bad);
       mbar_wait_mark(&o_empty[out], ((n / kOuts) & 1) ^ 1, abort_flag, bad);
-      const auto a_at = [&](int ks, int lo) { return w + 32 * (ks >> 1) + 8 * (ks & 1) + 16 * lo; };
-      const auto b_at = [](uint32_t at, int ks) { return umma_desc(at + ks * 2048, 16384, 1024, 2); };
       wait_stage();
-      uint32_t at = smem_u32(ring + stage * kPart);
       if (!bad && elect_one()) {
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks) mma_ts(d, a_at(ks, 0), b_at(at, ks), products, ks > 0);
+        product_steps(d, w, mn_major(smem_u32(ring + stage * kPart)), 0u);
         tcgen05_commit(&empty[stage]);
       }
       __syncwarp();
       next_stage();
       wait_stage();
-      at = smem_u32(ring + stage * kPart);
       if (!bad && elect_one()) {
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks) mma_ts(d, a_at(ks, 1), b_at(at, ks), products, 1u);
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks) mma_ts(d, a_at(ks, 0), b_at(at, ks), products, 1u);
+        const uint32_t at = mn_major(smem_u32(ring + stage * kPart));
+        product_steps(d, w + 16, at, 1u);
+        product_steps(d, w, at, 1u);
         tcgen05_commit(&empty[stage]);
         tcgen05_commit(&o_full[out]);
       }
@@ -515,13 +523,13 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
       next_stage();
     };
     mbar_wait_mark(resident_full, 0, abort_flag, bad);
-    const uint32_t rows = smem_u32(resident);
+    const uint32_t rows = k_major(smem_u32(resident));
     int n = 0;
     while (walk.next(lane, head, t, all)) {
       scores(tmem + (n & 1) * 128, rows, &s_full[n & 1]);
       if (kTwo) {
         mbar_wait_mark(y_empty, (n & 1) ^ 1, abort_flag, bad);
-        scores(tmem + 256, rows + 2 * kPart, y_full);
+        scores(tmem + 256, rows + (2 * kPart >> 4), y_full);
       }
       if (n > 0) product(n - 1);
       ++n;
@@ -531,7 +539,8 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
   } else {
     // ---- weights
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
-    const int quarter = warp & 3, half = (warp - 4) >> 2, row = quarter * 32 + lane;
+    constexpr int kCols = 128 / kParts, kOuts16 = 4 * G / kParts;      // columns of a thread; of products, in sixteens
+    const int quarter = warp & 3, part = (warp - 4) >> 2, row = quarter * 32 + lane;
     const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
     const int off = a.Tk - a.Tq, self = tile * kTile + row;            // query or key
     const bool there = self < (kRowsAreKeys ? a.Tk : a.Tq);
@@ -550,14 +559,15 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     bool spoiled = (info1.bad[quarter] >> lane) & 1u;
     if (kTwo) spoiled = spoiled || ((r2.info[row_at].bad[quarter] >> lane) & 1u);
     const bool careful = __any_sync(0xffffffffu, spoiled);
-    const float inv1 = info1.inv, inv2 = kTwo ? r2.info[row_at].inv : 0.f;
-    const float unit = CAP ? a.scale / a.cap : a.scale * kLog2e, wide = CAP ? a.cap * kLog2e : 1.f;
+    const bool cap = SHAPED && a.cap > 0.f;
+    const float inv2 = kTwo ? r2.info[row_at].inv : 0.f;
+    const float unit = info1.inv * (cap ? a.scale / a.cap : a.scale * kLog2e), wide = cap ? a.cap * kLog2e : 1.f;
     float row_max = 0.f, row_delta = 0.f, row_norm = 0.f;
     if (KIND == kDq) { row_max = p.row_max[row_at * kTile + row]; row_delta = p.row_delta[row_at * kTile + row]; row_norm = p.row_norm[row_at * kTile + row] * sqrtf((float)a.D); }
     const float norm_top = KIND == kDk ? r2.info[row_at].top * sqrtf((float)a.D) : 0.f;
-    float acc[32 * G];
+    float acc[16 * kOuts16];
 #pragma unroll
-    for (int i = 0; i < 32 * G; ++i) acc[i] = 0.f;
+    for (int i = 0; i < 16 * kOuts16; ++i) acc[i] = 0.f;
     float most = -INFINITY, sum = 0.f;                                 // fwd
     float alpha = 1.f, out_factor = 0.f;                               // of the product in flight
     float slope = 0.f;
@@ -568,40 +578,57 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     const auto add_up = [&](int n) {
       const int out = kOuts == 2 ? n & 1 : 0;
       wait_for(&o_full[out], (n / kOuts) & 1);
-      const bool scaled = KIND == kFwd && __any_sync(0xffffffffu, alpha != 1.f);
+      const uint32_t from = mine + S::kOutAt + out * 64 * G + part * 16 * kOuts16;
+      float o[16 * kOuts16];
 #pragma unroll
-      for (int c = 0; c < G; ++c) {
-        float o[32];
-        tmem_ld32(mine + S::kOutAt + out * 64 * G + half * 32 * G + 32 * c, o);
-        tmem_ld_wait();
-        if (scaled) {
-#pragma unroll
-          for (int k = 0; k < 32; ++k) acc[32 * c + k] = fmaf(o[k], out_factor, acc[32 * c + k] * alpha);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 32; ++k) acc[32 * c + k] = fmaf(o[k], out_factor, acc[32 * c + k]);
-        }
+      for (int c = 0; c < kOuts16; c += 2) {
+        if (kOuts16 > 1) tmem_ld32(from + 16 * c, o + 16 * c); else tmem_ld16(from, o);
       }
+      tmem_ld_wait();
       arrive(&o_empty[out]);
+      if (KIND == kFwd) {
+#pragma unroll
+        for (int k = 0; k < 16 * kOuts16; ++k) acc[k] *= alpha;
+      }
+#pragma unroll
+      for (int k = 0; k < 16 * kOuts16; ++k) acc[k] = fmaf(o[k], out_factor, acc[k]);
+    };
+    // What the next tile needs from memory is asked for a tile ahead
+    struct Next { int head, t; bool there, all; float inv1, inv2, top, norm, delta; int64_t at; };
+    const auto look_ahead = [&] {
+      Next x;
+      x.there = walk.next(lane, x.head, x.t, x.all);
+      x.at = x.there ? col_at(x.head, x.t) : 0;
+      const TileInfo &i1 = c1.info[x.at], &i2 = c2.info[x.at];
+      x.inv1 = i1.inv; x.inv2 = i2.inv; x.top = KIND == kDq ? i2.top : 0.f; x.norm = KIND == kDk ? i2.norm : 0.f; x.delta = KIND == kDk ? i2.delta : 0.f;
+      return x;
     };
 
     int n = 0;
-    while (walk.next(lane, head, t, all)) {
-      const int64_t at = col_at(head, t);
-      const TileInfo &i1 = c1.info[at], &i2 = c2.info[at];
-      const float f = inv1 * i1.inv * unit;
-      if (a.slopes && slope_head != (kRowsAreKeys ? head : row_head)) { slope_head = kRowsAreKeys ? head : row_head; slope = __ldg(a.slopes + slope_head) * kLog2e; }
-      const int col0 = t * kTile + (kRowsAreKeys ? off : 0) + half * 64;                        // position of the first column
+    Next next = look_ahead();
+    while (next.there) {
+      const Next now = next;
+      next = look_ahead();
+      const float f = now.inv1 * unit;
+      if (SHAPED && a.slopes && slope_head != (kRowsAreKeys ? now.head : row_head)) {
+        slope_head = kRowsAreKeys ? now.head : row_head;
+        slope = __ldg(a.slopes + slope_head) * kLog2e;
+      }
+      const int col0 = now.t * kTile + (kRowsAreKeys ? off : 0) + part * kCols;                 // position of the first column
       const int at_row = kRowsAreKeys ? self : self + off;
-      const bool masked = !all || careful;
-      // scores of a chunk of 32 columns, capped and biased, in units of log 2; inner: the cap's tanh
-      const auto score32 = [&](float* z, float* inner, int c) {
+      const bool masked = !now.all || careful;
+      const uint32_t from = mine + (n & 1) * 128 + part * kCols;
+      // scores of a chunk of 32 columns, capped and biased, in units of log 2; turned: 1 - the cap's tanh squared
+      const auto shape32 = [&](float* z, float* turned, int c) {
 #pragma unroll
         for (int k = 0; k < 32; ++k) z[k] *= f;
-        if (CAP) {
+        if (cap) {
           tanh32(z);
 #pragma unroll
-          for (int k = 0; k < 32; ++k) { if (inner) inner[k] = z[k]; z[k] *= wide; }
+          for (int k = 0; k < 32; ++k) { if (turned) turned[k] = fmaf(-z[k], z[k], 1.f); z[k] *= wide; }
+        } else if (turned) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) turned[k] = 1.f;
         }
         if (a.slopes) {
           const float away = (float)(at_row - (col0 + 32 * c));
@@ -609,8 +636,8 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
           for (int k = 0; k < 32; ++k) z[k] = fmaf(-slope, fabsf(away - (float)k), z[k]);
         }
       };
-      // which of a chunk's columns the row sees, and which of those make it NaN
-      const auto seen32 = [&](int c, uint32_t& spoils) {
+      // hides the columns of a chunk that the row does not see, and makes NaN of those that are not finite
+      const auto mask32 = [&](float* z, int c, float hidden) {
         const int first = col0 + 32 * c;
         uint32_t seen = bits_between(lo - first, hi - first) | bits_between(-1, extra - 1 - first);
         if (p.documents) {
@@ -620,83 +647,93 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
           for (int k = 0; k < 32; ++k) same |= __shfl_sync(0xffffffffu, theirs, k) == document ? 1u << k : 0u;
           seen &= document >= 0.f ? same : 0u;
         }
-        spoils = seen & (spoiled ? 0xffffffffu : i1.bad[half * 2 + c] | i2.bad[half * 2 + c]);
-        return seen;
+        const uint32_t spoils = seen & (spoiled ? 0xffffffffu : c1.info[now.at].bad[part * kChunks + c] | c2.info[now.at].bad[part * kChunks + c]);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) z[k] = (seen >> k) & 1u ? z[k] : hidden;
+        if (__builtin_expect(spoils != 0u, 0)) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) if ((spoils >> k) & 1u) z[k] = NAN;
+        }
       };
 
+      wait_for(&s_full[n & 1], (n >> 1) & 1);
       if (KIND == kFwd) {
-        float z[64];
-        wait_for(&s_full[n & 1], (n >> 1) & 1);
-        tmem_ld32(mine + (n & 1) * 128 + half * 64, z);
-        tmem_ld32(mine + (n & 1) * 128 + half * 64 + 32, z + 32);
-        tmem_ld_wait();
-        float m = -INFINITY;
+        // Scores that are not plain products are written back, so that both passes read them
+        const bool rewritten = SHAPED || masked || f < 0.f;
+        float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+        for (int c = 0; c < kChunks; ++c) {
+          float z[32];
+          tmem_ld32(from + 32 * c, z);
+          tmem_ld_wait();
+          if (__builtin_expect(rewritten, SHAPED)) {
+            if (SHAPED) shape32(z, nullptr, c);
+            else
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          score32(z + 32 * c, nullptr, c);
-          if (masked) {
-            uint32_t spoils;
-            const uint32_t seen = seen32(c, spoils);
-#pragma unroll
-            for (int k = 0; k < 32; ++k) z[32 * c + k] = (seen >> k) & 1u ? z[32 * c + k] : -INFINITY;
-            if (spoils) {
-#pragma unroll
-              for (int k = 0; k < 32; ++k) if ((spoils >> k) & 1u) z[32 * c + k] = NAN;
-            }
+              for (int k = 0; k < 32; ++k) z[k] *= f;
+            if (masked) mask32(z, c, -INFINITY);
+            tmem_st32(from + 32 * c, reinterpret_cast<const uint32_t*>(z));
           }
 #pragma unroll
-          for (int k = 0; k < 32; ++k) m = fmaxf(m, z[32 * c + k]);
+          for (int k = 0; k < 32; ++k) m[k & 3] = fmaxf(m[k & 3], z[k]);
         }
-        float* const others = exchange + (n & 1) * 256;
-        others[half * 128 + row] = m;
-        asm volatile("barrier.sync %0, 64;" ::"r"(1 + quarter) : "memory");
-        m = fmaxf(most, fmaxf(m, others[(half ^ 1) * 128 + row]));
-        const float base = max_of_finite_or(m), shifted = base - (float)kWeightExp, faded = exp2_fast(most - base);
-        most = m;
-        float s = 0.f;
+        if (rewritten) tmem_st_wait();
+        const float g = rewritten ? 1.f : f;
+        float* const others = exchange + (n & 1) * (kParts * 128) + row;
+        m[0] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * g;        // of -infinity: NaN if g is 0, which the maximum leaves out
+        others[part * 128] = m[0];
+        asm volatile("barrier.sync %0, %1;" ::"r"(1 + quarter), "n"(32 * kParts) : "memory");
 #pragma unroll
-        for (int k = 0; k < 64; ++k) { z[k] = exp2_fast(z[k] - shifted); s += z[k]; }
-        sum = sum * faded + s;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int i = 0; i < kParts; ++i) m[i] = others[i * 128];
+        const float over = kParts == 2 ? fmaxf(m[0], m[1]) : fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+        const float at_most = fmaxf(most, over), base = max_of_finite_or(at_most), shifted = base - (float)kWeightExp, faded = exp2_fast(most - base);
+        most = at_most;
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int c = 0; c < kChunks; ++c) {
+          float z[32];
           uint32_t words[32];
-          split32(z + 32 * c, words);
-          tmem_st32(mine + (n & 1) * 128 + half * 64 + 32 * c, words);
+          tmem_ld32(from + 32 * c, z);
+          tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < 32; ++k) { z[k] = exp2_fast(fmaf(z[k], g, -shifted)); s[k & 3] += z[k]; }
+          split32(z, words);
+          tmem_st32(from + 32 * c, words);
         }
         tmem_st_wait();
         arrive(&w_full[n & 1]);
+        sum = fmaf(sum, faded, (s[0] + s[1]) + (s[2] + s[3]));
         if (n > 0) add_up(n - 1);
         alpha = faded;
-        out_factor = i2.inv;
+        out_factor = now.inv2;
       } else {
-        float factor, kk = 0.f, fy = 0.f;
+        float factor;
         int shift = kWeightExp;
         if (KIND == kDv) {
-          factor = i2.inv * power_of_two(-kWeightExp);
+          factor = now.inv2 * power_of_two(-kWeightExp);
         } else {
-          const float bound = KIND == kDq ? fmaf(row_norm, i2.top, fabsf(row_delta)) : fmaf(i2.norm, norm_top, i2.delta);
+          const float bound = KIND == kDq ? fmaf(row_norm, now.top, fabsf(row_delta)) : fmaf(now.norm, norm_top, now.delta);
           shift = min(100, max(-100, kWeightExp - exponent_of(bound)));
-          factor = i1.inv * power_of_two(-shift);
-          fy = inv2 * i2.inv;
+          factor = now.inv1 * power_of_two(-shift);
         }
-        kk = (float)shift;
-        const float* const col_max = kRowsAreKeys ? p.row_max + at * kTile + half * 64 : nullptr;
-        const float* const col_delta = kRowsAreKeys ? p.row_delta + at * kTile + half * 64 : nullptr;
-        wait_for(&s_full[n & 1], (n >> 1) & 1);
+        const float kk = (float)shift, fy = inv2 * now.inv2;
+        const float* const col_max = kRowsAreKeys ? p.row_max + now.at * kTile + part * kCols : nullptr;
+        const float* const col_delta = kRowsAreKeys ? p.row_delta + now.at * kTile + part * kCols : nullptr;
         if (kTwo) wait_for(y_full, n & 1);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float z[32], y[32], inner[CAP ? 32 : 1];
-          tmem_ld32(mine + (n & 1) * 128 + half * 64 + 32 * c, z);
-          if (kTwo) tmem_ld32(mine + 256 + half * 64 + 32 * c, y);
+#pragma unroll 1
+        for (int c = 0; c < kChunks; ++c) {
+          float z[32], y[32], turned[SHAPED && kTwo ? 32 : 1];
+          tmem_ld32(from + 32 * c, z);
+          if (kTwo) tmem_ld32(mine + 256 + part * kCols + 32 * c, y);
           tmem_ld_wait();
-          if (kTwo && c == 1) arrive(y_empty);
-          score32(z, CAP ? inner : nullptr, c);
+          if (kTwo && c == kChunks - 1) arrive(y_empty);
+          if (SHAPED) shape32(z, kTwo ? turned : nullptr, c);
+          const float g = SHAPED ? 1.f : f;
           if (kRowsAreKeys) {
 #pragma unroll
             for (int k = 0; k < 32; k += 4) {
               const float4 m4 = __ldg(reinterpret_cast<const float4*>(col_max + 32 * c + k));
-              z[k] += kk - m4.x; z[k + 1] += kk - m4.y; z[k + 2] += kk - m4.z; z[k + 3] += kk - m4.w;
+              z[k] = fmaf(z[k], g, kk - m4.x); z[k + 1] = fmaf(z[k + 1], g, kk - m4.y); z[k + 2] = fmaf(z[k + 2], g, kk - m4.z); z[k + 3] = fmaf(z[k + 3], g, kk - m4.w);
               if (KIND == kDk) {
                 const float4 d4 = __ldg(reinterpret_cast<const float4*>(col_delta + 32 * c + k));
                 y[k] = fmaf(y[k], fy, -d4.x); y[k + 1] = fmaf(y[k + 1], fy, -d4.y); y[k + 2] = fmaf(y[k + 2], fy, -d4.z); y[k + 3] = fmaf(y[k + 3], fy, -d4.w);
@@ -705,27 +742,17 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
           } else {
             const float less = kk - row_max;
 #pragma unroll
-            for (int k = 0; k < 32; ++k) { z[k] += less; y[k] = fmaf(y[k], fy, -row_delta); }
+            for (int k = 0; k < 32; ++k) { z[k] = fmaf(z[k], g, less); y[k] = fmaf(y[k], fy, -row_delta); }
           }
 #pragma unroll
           for (int k = 0; k < 32; ++k) {
             z[k] = exp2_fast(z[k]);
-            if (kTwo) z[k] *= y[k];
-            if (kTwo && CAP) z[k] *= fmaf(-inner[k], inner[k], 1.f);
+            if (kTwo) z[k] *= SHAPED ? y[k] * turned[k] : y[k];
           }
-          if (masked) {
-            uint32_t spoils;
-            const uint32_t seen = seen32(c, spoils);
-#pragma unroll
-            for (int k = 0; k < 32; ++k) z[k] = (seen >> k) & 1u ? z[k] : 0.f;
-            if (spoils) {
-#pragma unroll
-              for (int k = 0; k < 32; ++k) if ((spoils >> k) & 1u) z[k] = NAN;
-            }
-          }
+          if (__builtin_expect(masked, 0)) mask32(z, c, 0.f);
           uint32_t words[32];
           split32(z, words);
-          tmem_st32(mine + (n & 1) * 128 + half * 64 + 32 * c, words);
+          tmem_st32(from + 32 * c, words);
         }
         tmem_st_wait();
         arrive(&w_full[n & 1]);
@@ -738,25 +765,27 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
 
     float last = KIND == kDv ? 1.f : a.scale;
     if (KIND == kFwd) {
-      exchange[half * 128 + row] = sum;                                // the barrier of the last tile but one has passed for both
-      asm volatile("barrier.sync %0, 64;" ::"r"(1 + quarter) : "memory");
-      sum = exchange[row] + exchange[128 + row];                       // in the same order in both
+      exchange[part * 128 + row] = sum;                                // nobody reads the last tile's maxima any more: its product has been added up
+      asm volatile("barrier.sync %0, %1;" ::"r"(1 + quarter), "n"(32 * kParts) : "memory");
+      sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) sum += exchange[i * 128 + row]; // in the same order everywhere
       last = sum == 0.f ? 0.f : 1.f / sum;
-      if (a.stats && half == 0 && there) {
+      if (a.stats && part == 0 && there) {
         float* const to = a.stats + 2 * (((int64_t)b * a.H + row_head) * a.Tq + self);
         to[0] = max_of_finite_or(most); to[1] = last * (float)(1 << kWeightExp);
       }
     }
     if (there && !*abort_flag) {
       float* const result = KIND == kFwd ? a.o : KIND == kDq ? a.dq : KIND == kDk ? a.dk : a.dv;
-      float* const to = result + (((int64_t)b * (kRowsAreKeys ? a.Tk : a.Tq) + self) * row_heads + row_head) * a.D + half * 32 * G;
-      const int cols = a.D - half * 32 * G;
+      float* const to = result + (((int64_t)b * (kRowsAreKeys ? a.Tk : a.Tq) + self) * row_heads + row_head) * a.D + part * 16 * kOuts16;
+      const int cols = a.D - part * 16 * kOuts16;
       if (a.D % 4 == 0 && (reinterpret_cast<uintptr_t>(result) & 15) == 0) {
 #pragma unroll
-        for (int k = 0; k < 32 * G; k += 4) if (k < cols) *reinterpret_cast<float4*>(to + k) = make_float4(acc[k] * last, acc[k + 1] * last, acc[k + 2] * last, acc[k + 3] * last);
+        for (int k = 0; k < 16 * kOuts16; k += 4) if (k < cols) *reinterpret_cast<float4*>(to + k) = make_float4(acc[k] * last, acc[k + 1] * last, acc[k + 2] * last, acc[k + 3] * last);
       } else {
 #pragma unroll
-        for (int k = 0; k < 32 * G; ++k) if (k < cols) to[k] = acc[k] * last;
+        for (int k = 0; k < 16 * kOuts16; ++k) if (k < cols) to[k] = acc[k] * last;
       }
     }
   }
@@ -770,35 +799,35 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
   if (threadIdx.x == 0 && *abort_flag && p.err) atomicExch(p.err, 1);
 }
 
-template <int G, bool CAP> __global__ void __launch_bounds__(kThreads, 1) attention_tc_fwd_kernel(const __grid_constant__ TcArgs p) { attention_rows<kFwd, G, CAP>(p, blockIdx.x); }
+template <int G, bool SHAPED> __global__ void __launch_bounds__(kThreads, 1) attention_tc_fwd_kernel(const __grid_constant__ TcArgs p) { attention_rows<kFwd, G, SHAPED>(p, blockIdx.x); }
 // All gradients in one launch, the longest first: dk and dv of the first keys see all queries of all heads that share them.
-template <int G, bool CAP> __global__ void __launch_bounds__(kThreads, 1) attention_tc_bwd_kernel(const __grid_constant__ TcArgs p, int dk_blocks, int dv_blocks) {
+template <int G, bool SHAPED> __global__ void __launch_bounds__(kThreads, 1) attention_tc_bwd_kernel(const __grid_constant__ TcArgs p, int dk_blocks, int dv_blocks) {
   const int block = blockIdx.x;
-  if (block < dk_blocks) attention_rows<kDk, G, CAP>(p, block);
-  else if (block < dk_blocks + dv_blocks) attention_rows<kDv, G, CAP>(p, block - dk_blocks);
-  else attention_rows<kDq, G, CAP>(p, block - dk_blocks - dv_blocks);
+  if (block < dk_blocks) attention_rows<kDk, G, SHAPED>(p, block);
+  else if (block < dk_blocks + dv_blocks) attention_rows<kDv, G, SHAPED>(p, block - dk_blocks);
+  else attention_rows<kDq, G, SHAPED>(p, block - dk_blocks - dv_blocks);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------
-template <int G, bool CAP> cudaError_t launch_fwd(const TcArgs& p, cudaStream_t s) {
+template <int G, bool SHAPED> cudaError_t launch_fwd(const TcArgs& p, cudaStream_t s) {
   static std::atomic<uint64_t> ready{0};
-  const auto kernel = attention_tc_fwd_kernel<G, CAP>;
+  const auto kernel = attention_tc_fwd_kernel<G, SHAPED>;
   const int bytes = Shape<kFwd, G>::kSmem;
   const cudaError_t e = once_per_device(ready, [kernel, bytes] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
   return e != cudaSuccess ? e : launch_dep(kernel, dim3((unsigned)(p.a.B * p.a.H * p.q_tiles)), dim3(kThreads), (size_t)bytes, s, p);
 }
-template <int G, bool CAP> cudaError_t launch_bwd(const TcArgs& p, cudaStream_t s) {
+template <int G, bool SHAPED> cudaError_t launch_bwd(const TcArgs& p, cudaStream_t s) {
   static std::atomic<uint64_t> ready{0};
-  const auto kernel = attention_tc_bwd_kernel<G, CAP>;
+  const auto kernel = attention_tc_bwd_kernel<G, SHAPED>;
   const int bytes = std::max(std::max(Shape<kDq, G>::kSmem, Shape<kDk, G>::kSmem), Shape<kDv, G>::kSmem);
   const cudaError_t e = once_per_device(ready, [kernel, bytes] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
   const int keys = p.a.B * p.a.G * p.k_tiles, dk = p.a.dk ? keys : 0, dv = p.a.dv ? keys : 0, dq = p.a.dq ? p.a.B * p.a.H * p.q_tiles : 0;
   return e != cudaSuccess ? e : launch_dep(kernel, dim3((unsigned)(dk + dv + dq)), dim3(kThreads), (size_t)bytes, s, p, dk, dv);
 }
 template <class F> cudaError_t with_form(const AttentionArgs& a, F&& f) {
-  const bool cap = a.cap > 0.f;
-  if (a.D <= 64) return cap ? f(std::integral_constant<int, 1>(), std::true_type()) : f(std::integral_constant<int, 1>(), std::false_type());
-  return cap ? f(std::integral_constant<int, 2>(), std::true_type()) : f(std::integral_constant<int, 2>(), std::false_type());
+  const bool shaped = a.cap > 0.f || a.slopes;
+  if (a.D <= 64) return shaped ? f(std::integral_constant<int, 1>(), std::true_type()) : f(std::integral_constant<int, 1>(), std::false_type());
+  return shaped ? f(std::integral_constant<int, 2>(), std::true_type()) : f(std::integral_constant<int, 2>(), std::false_type());
 }
 
 }  // namespace
@@ -860,7 +889,7 @@ int attention_tc(const AttentionArgs& a, bool backward, size_t* bytes, cudaStrea
   if (a.D <= 64) TF_CUDA(wide ? launch_dep(attention_pack_kernel<1, true>, blocks, dim3(kPackThreads), 0, s, pack) : launch_dep(attention_pack_kernel<1, false>, blocks, dim3(kPackThreads), 0, s, pack));
   else TF_CUDA(wide ? launch_dep(attention_pack_kernel<2, true>, blocks, dim3(kPackThreads), 0, s, pack) : launch_dep(attention_pack_kernel<2, false>, blocks, dim3(kPackThreads), 0, s, pack));
   TF_AFTER(s, what);
-  TF_CUDA(with_form(a, [&](auto g, auto cap) { return backward ? launch_bwd<decltype(g)::value, decltype(cap)::value>(tc, s) : launch_fwd<decltype(g)::value, decltype(cap)::value>(tc, s); }));
+  TF_CUDA(with_form(a, [&](auto g, auto shaped) { return backward ? launch_bwd<decltype(g)::value, decltype(shaped)::value>(tc, s) : launch_fwd<decltype(g)::value, decltype(shaped)::value>(tc, s); }));
   TF_AFTER(s, what);
   return 0;
 }
