@@ -36,11 +36,11 @@ namespace {
 
 enum { kFwd, kDq, kDk, kDv };
 constexpr int kTile = 128;
-constexpr int kParts = 2;                        // warps that share the columns of a TMEM lane quarter
-constexpr int kWeightWarps = 4 * kParts, kThreads = 128 + 32 * kWeightWarps;       // warps: 0 copies, 1 issues MMAs and owns TMEM, 2 and 3 idle, the others make weights
-constexpr int kChunks = 4 / kParts;                  // of 32 columns, a thread
-// Registers a thread: what the launch has (168 x 384 = 64,512 or 96 x 640 = 61,440), dealt anew: the sums are the same.
-constexpr int kFewRegisters = kParts == 2 ? 56 : 64, kManyRegisters = kParts == 2 ? 224 : 104;
+// Warps: 0 copies, 1 issues MMAs and owns TMEM, 2 and 3 idle, 4-7 and 8-11 make weights.  With one score product the two groups take every other tile, each thread a whole
+// row, so that one computes while the other waits; with two, whose second scores have one buffer, both take half the columns of every tile.
+constexpr int kThreads = 384;
+// Registers a thread: 168 at the launch (64,512 of the block); the first four warps give 96 of theirs, the others take 48 each, the same sum.
+constexpr int kFewRegisters = 72, kManyRegisters = 216;
 constexpr int kWeightExp = 14;                   // weights are scaled to below 2^15
 constexpr int kFar = 1 << 26;                    // beyond every position
 
@@ -291,14 +291,27 @@ template <int KIND> struct Walk {
 template <int KIND, int G> struct Shape {
   static constexpr bool kTwo = KIND == kDq || KIND == kDk;           // two score products
   static constexpr bool kRowsAreKeys = KIND == kDk || KIND == kDv;
+  static constexpr bool kTurns = !kTwo;                              // groups of warps take turns
+  static constexpr int kWeightWarps = kTurns ? 4 : 8;                // of a tile
+  static constexpr int kChunks = kTurns ? 4 : 2;                     // of 32 columns, a thread
+  static constexpr int kSums = kTurns ? 64 * G : 32 * G;             // columns of the product that a thread adds up
+  // Heads of up to 64: the hi halves of the weights multiply both halves of the other operand at once, side by side in N.  An MMA of N = 64 takes as long as one of 128.
+  static constexpr bool kBeside = G == 1;
   static constexpr int kPart = G * 16384;                            // one half (hi or lo) of a tile
   static constexpr int kResident = (kTwo ? 4 : 2) * kPart;
-  static constexpr int kControl = 256 + (KIND == kFwd ? 2 * kParts * 128 * 4 : 0);
-  static constexpr int kStages = (232448 - kControl - kResident) / kPart < 8 ? (232448 - kControl - kResident) / kPart : 8;
+  static constexpr int kControl = 768 + (KIND == kFwd ? 1024 : 0) + (kRowsAreKeys ? 2048 : 0);
+  static constexpr int kFits = (232448 - kControl - kResident) / kPart, kStages = kFits < 8 ? kFits : 8;
   static constexpr int kSmem = kResident + kStages * kPart + kControl;
-  static constexpr int kOuts = kTwo && G == 2 ? 1 : 2;               // TMEM: scores 0 and 128, second scores 256, products behind
+  static constexpr int kOutCols = kBeside ? 128 : 64 * G;            // TMEM: scores 0 and 128, second scores 256, products behind
+  static constexpr int kOuts = kTwo ? 1 : 2;
   static constexpr int kOutAt = kTwo ? 384 : 256;
-  static_assert(kStages >= 3 && kOutAt + kOuts * 64 * G <= 512, "fits");
+  static_assert(kStages >= 3 && (!kBeside || kStages % 2 == 0) && kOutAt + kOuts * kOutCols <= 512, "fits");
+};
+// Of one tile of columns, for the warps: written by the copying warp, which walks the list.  Eight of them in turn: by the time a copy for tile n + 8 can be issued,
+// the weights of tile n + 4 have been made.
+struct __align__(16) Entry {
+  int flags, head, col, at;                      // 1: there is a tile, 2: every row sees all of it; position of its first column; its number
+  float inv1, inv2, x, y;                        // 1 / scale of both operands; dq: largest magnitude of V, dk: largest norm and |D'| of dO'
 };
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -337,19 +350,30 @@ __device__ __forceinline__ void tanh32(float* t) {
     t[k] = y;
   }
 }
-// hi and lo halves of 32 weights, as the A operand has them: 16 words each
+// hi and lo halves of 32 weights, as the A operand has them: 16 weights are 8 words of hi and 8 of lo
 __device__ __forceinline__ void split32(const float* w, uint32_t* words) {
 #pragma unroll
   for (int k = 0; k < 16; ++k) {
     // the upper 11 bits, which fp16 holds exactly down to 2^-14; below, the rounding is 2^-25 of weights that reach 2^14
     const float a = __uint_as_float(__float_as_uint(w[2 * k]) & 0xffffe000u), b = __uint_as_float(__float_as_uint(w[2 * k + 1]) & 0xffffe000u);
-    words[k] = halves(a, b);
-    words[16 + k] = halves(w[2 * k] - a, w[2 * k + 1] - b);
+    words[(k >> 3) * 16 + (k & 7)] = halves(a, b);
+    words[(k >> 3) * 16 + 8 + (k & 7)] = halves(w[2 * k] - a, w[2 * k + 1] - b);
   }
 }
 __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {               // bits lo .. hi of a word, as far as it has them
   const uint32_t below = hi >= 31 ? 0xffffffffu : hi < 0 ? 0u : (2u << hi) - 1u;
   return lo <= 0 ? below : lo > 31 ? 0u : below & (0xffffffffu << lo);
+}
+
+// mbar_wait_mark in few instructions: eight warps and the issuer share the instruction cache
+__device__ __forceinline__ void await(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int& bad) {
+  if (bad || mbar_try_wait(bar, parity)) return;
+  const long long t0 = clock64();
+#pragma unroll 1
+  while (!mbar_try_wait(bar, parity)) {
+    if (*abort_flag) { bad = 1; break; }
+    if (clock64() - t0 > kWaitCycles) { *abort_flag = 1; bad = 1; break; }
+  }
 }
 
 template <int KIND, int G, bool SHAPED>
@@ -362,25 +386,37 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
   uint8_t* const ring = smem + S::kResident;
   uint64_t* const full = reinterpret_cast<uint64_t*>(ring + kStages * kPart);
   uint64_t* const empty = full + 8;
-  uint64_t* const resident_full = empty + 8;
+  uint64_t* const entry_full = empty + 8;        // [8] an entry is written
+  uint64_t* const resident_full = entry_full + 8;
   uint64_t* const s_full = resident_full + 1;    // [2] scores are in TMEM
   uint64_t* const w_full = s_full + 2;           // [2] weights are
-  uint64_t* const y_full = w_full + 2;           // second scores are in TMEM
-  uint64_t* const y_empty = y_full + 1;          // and have been read
-  uint64_t* const o_full = y_empty + 1;          // [2] the product is
+  uint64_t* const y_full = w_full + 2;           // [2] second scores are in TMEM
+  uint64_t* const y_empty = y_full + 2;          // [2] and have been read
+  uint64_t* const o_full = y_empty + 2;          // [2] the product is
   uint64_t* const o_empty = o_full + 2;          // [2] and has been added up
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 2);
+  uint64_t* const columns_full = o_empty + 2;    // [2] maxima and D' of a tile of queries
+  uint64_t* const merge = columns_full + 2;      // the second group's sums are in shared memory
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(merge + 1);
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* const exchange = reinterpret_cast<float*>(full + 32);       // [2][kParts][128]
+  Entry* const entries = reinterpret_cast<Entry*>(full + 64);        // [8]
+  float* const statistics = reinterpret_cast<float*>(entries + 8);   // fwd: [2][128] of the second group
+  float* const columns = statistics;                                 // dk, dv: [2][2][128]
+  static_assert(8 + 8 + 8 + 1 + 7 * 2 + 1 + 1 <= 64, "barriers fit");
   const AttentionArgs& a = p.a;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (warp == 0) {
     if (lane == 0) {
       for (int i = 0; i < kStages; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
+      for (int i = 0; i < 8; ++i) mbar_init(entry_full + i, 1);
       mbar_init(resident_full, 1);
-      for (int i = 0; i < 2; ++i) { mbar_init(s_full + i, 1); mbar_init(w_full + i, kWeightWarps); mbar_init(o_full + i, 1); mbar_init(o_empty + i, kWeightWarps); }
-      mbar_init(y_full, 1); mbar_init(y_empty, kWeightWarps);
+      for (int i = 0; i < 2; ++i) {              // tiles take turns, also where one buffer serves both
+        mbar_init(s_full + i, 1); mbar_init(w_full + i, S::kWeightWarps);
+        mbar_init(y_full + i, 1); mbar_init(y_empty + i, S::kWeightWarps);
+        mbar_init(o_full + i, 1); mbar_init(o_empty + i, S::kWeightWarps);
+        mbar_init(columns_full + i, 1);
+      }
+      mbar_init(merge, 4);
       *abort_flag = (smem_u32(smem) & 1023u) ? 1 : 0;                // nothing is issued then
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -404,16 +440,14 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
   const Packed &r1 = kRowsAreKeys ? p.k : p.q, &r2 = kRowsAreKeys ? p.v : p.d;                 // rows
   const Packed &c1 = kRowsAreKeys ? p.q : p.k, &c2 = kRowsAreKeys ? p.d : p.v;                 // columns
   const auto col_at = [&](int head, int t) { return kRowsAreKeys ? ((int64_t)b * a.H + head) * col_tiles + t : ((int64_t)b * a.G + head / a.group) * col_tiles + t; };
-  Walk<KIND> walk(p, b, row_head, tile);
-  int head, t, bad = *abort_flag;
-  bool all;
+  int bad = *abort_flag;
 
   if (warp < 4) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
   if (warp == 0) {
     // ---- copies: the rows once, then tiles in the order in which the MMAs take them, the lo half first
     int stage = 0;
-    uint32_t phase = 0, armed = 0, phases = 0;
+    uint32_t phase = 0, armed = 0, phases = 0, columns_armed = 0;
     bool rows_armed = false;
     if (!bad) {
       if (elect_one()) {
@@ -423,10 +457,21 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
       }
       rows_armed = true;
     }
+    Walk<KIND> walk(p, b, row_head, tile);
+    // What an entry says is asked for a tile ahead
+    struct Next { bool there, all; int head, t; int64_t at; float inv1, inv2, x, y; };
+    const auto look_ahead = [&] {
+      Next x;
+      x.there = walk.next(lane, x.head, x.t, x.all);
+      x.at = x.there ? col_at(x.head, x.t) : 0;
+      const TileInfo &i1 = c1.info[x.at], &i2 = c2.info[x.at];
+      x.inv1 = i1.inv; x.inv2 = i2.inv; x.x = KIND == kDq ? i2.top : i2.norm; x.y = i2.delta;
+      return x;
+    };
     const auto load = [&](const Packed& from, int64_t at) {
 #pragma unroll
       for (int lo = 1; lo >= 0; --lo) {
-        mbar_wait_mark(&empty[stage], phase ^ 1, abort_flag, bad);
+        await(&empty[stage], phase ^ 1, abort_flag, bad);
         bad = __any_sync(0xffffffffu, bad);
         if (!bad) {
           if (elect_one()) {
@@ -440,12 +485,35 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
       }
     };
     int64_t before = -1;
-    while (walk.next(lane, head, t, all)) {
-      const int64_t at = col_at(head, t);
-      load(c1, at);
-      if (kTwo) load(c2, at);
+    Next next = look_ahead();
+    for (int n = 0;; ++n) {
+      const Next now = next;
+      if (lane == 0) {
+        entries[n & 7] = Entry{now.there ? 1 | (int)now.all << 1 : 0, now.head, now.t * kTile + (kRowsAreKeys ? a.Tk - a.Tq : 0), (int)now.at, now.inv1, now.inv2, now.x, now.y};
+        mbar_arrive(entry_full + (n & 7));
+      }
+      __syncwarp();
+      if (!now.there) {                          // and for the other group, whose tile would be the next
+        if (lane == 0) { entries[(n + 1) & 7].flags = 0; mbar_arrive(entry_full + ((n + 1) & 7)); }
+        break;
+      }
+      next = look_ahead();
+      load(c1, now.at);
+      if (kTwo) load(c2, now.at);
+      if (kRowsAreKeys) {                        // maxima and D' of the tile's queries, when the weights of the tile before the last are made
+        if (n >= 2) await(&w_full[n & 1], ((n - 2) >> 1) & 1, abort_flag, bad);
+        bad = __any_sync(0xffffffffu, bad);
+        if (!bad) {
+          if (elect_one()) {
+            mbar_expect_tx(columns_full + (n & 1), kTwo ? 1024 : 512);
+            bulk_load(columns + (n & 1) * 256, p.row_max + now.at * kTile, 512, columns_full + (n & 1));
+            if (kTwo) bulk_load(columns + (n & 1) * 256 + 128, p.row_delta + now.at * kTile, 512, columns_full + (n & 1));
+          }
+          columns_armed = n + 1;
+        }
+      }
       if (before >= 0) load(kTwo ? c1 : c2, before);
-      before = at;
+      before = now.at;
     }
     if (before >= 0) load(kTwo ? c1 : c2, before);
     __syncwarp();
@@ -455,13 +523,18 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
         const long long t0 = clock64();
         while (!mbar_try_wait(i < 0 ? resident_full : &full[i], i < 0 ? 0 : (phases >> i) & 1u) && clock64() - t0 < 100000000ll) {}
       }
+      for (uint32_t n = columns_armed > 2 ? columns_armed - 2 : 0; n < columns_armed; ++n) {
+        const long long t0 = clock64();
+        while (!mbar_try_wait(columns_full + (n & 1), (n >> 1) & 1) && clock64() - t0 < 100000000ll) {}
+      }
     } else if (rows_armed) {
-      mbar_wait_mark(resident_full, 0, abort_flag, bad);             // rows that see nothing: nobody else waits for them
+      await(resident_full, 0, abort_flag, bad);             // rows that see nothing: nobody else waits for them
     }
   } else if (warp == 1) {
     // ---- MMAs
     constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(kTile >> 4) << 24), kScores = kIdesc | ((uint32_t)(kTile >> 3) << 17);
     const uint32_t products = kIdesc | (1u << 16) | ((uint32_t)(p.D16 >> 3) << 17);            // the B operand has its columns (the head) along the rows of memory
+    const uint32_t beside = products + (64u >> 3 << 17);
     const int steps = p.D16 / 16;
     int stage = 0;
     uint32_t phase = 0;
@@ -469,30 +542,35 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     constexpr uint32_t kHigh = (1024u >> 4) | 1u << 14 | 2u << 29;
     const auto k_major = [](uint32_t at) { return (at & 0x3FFFFu) >> 4 | 1u << 16; };
     const auto mn_major = [](uint32_t at) { return (at & 0x3FFFFu) >> 4 | (16384u >> 4) << 16; };
-    const auto wait_stage = [&] { mbar_wait_mark(&full[stage], phase, abort_flag, bad); __syncwarp(); tcgen05_fence_after(); };
+    // both halves of a tile are there; the lo half is in the present stage
+    const auto wait_tile = [&] {
+      const bool wraps = stage + 1 == kStages;
+      await(&full[stage], phase, abort_flag, bad);
+      await(&full[wraps ? 0 : stage + 1], wraps ? phase ^ 1 : phase, abort_flag, bad);
+      __syncwarp();
+      tcgen05_fence_after();
+    };
     const auto next_stage = [&] { if (++stage == kStages) { stage = 0; phase ^= 1; } };
     const auto score_steps = [&](uint32_t d, uint32_t rows_low, uint32_t cols_low, uint32_t keep) {
 #pragma unroll
       for (int ks = 0; ks < 4 * G; ++ks)
         if (ks < steps) mma_ss(d, rows_low + (ks >> 2) * 1024 + (ks & 3) * 2, kHigh, cols_low + (ks >> 2) * 1024 + (ks & 3) * 2, kHigh, kScores, ks ? 1u : keep);
     };
-    const auto product_steps = [&](uint32_t d, uint32_t w, uint32_t cols_low, uint32_t keep) {
+    const auto product_steps = [&](uint32_t d, uint32_t w, uint32_t cols_low, uint32_t idesc, uint32_t keep) {
 #pragma unroll
-      for (int ks = 0; ks < 8; ++ks) mma_ts(d, w + 32 * (ks >> 1) + 8 * (ks & 1), cols_low + ks * 128, kHigh, products, ks ? 1u : keep);
+      for (int ks = 0; ks < 8; ++ks) mma_ts(d, w + 16 * ks, cols_low + ks * 128, kHigh, idesc, ks ? 1u : keep);
     };
     const auto scores = [&](uint32_t d, uint32_t rows_hi, uint64_t* done) {
-      wait_stage();
-      if (!bad && elect_one()) {
-        score_steps(d, rows_hi, k_major(smem_u32(ring + stage * kPart)), 0u);
-        tcgen05_commit(&empty[stage]);
-      }
-      __syncwarp();
+      wait_tile();
+      const int lo = stage;
       next_stage();
-      wait_stage();
       if (!bad && elect_one()) {
-        const uint32_t at = k_major(smem_u32(ring + stage * kPart));
-        score_steps(d, rows_hi + (kPart >> 4), at, 1u);
-        score_steps(d, rows_hi, at, 1u);
+        const uint32_t at_lo = k_major(smem_u32(ring + lo * kPart)), at_hi = k_major(smem_u32(ring + stage * kPart));
+#pragma unroll 1
+        for (int pass = 0; pass < 3; ++pass) {   // hi * lo, lo * hi, hi * hi
+          score_steps(d, rows_hi + (pass == 1 ? kPart >> 4 : 0), pass ? at_hi : at_lo, pass);
+          if (pass == 0) tcgen05_commit(&empty[lo]);
+        }
         tcgen05_commit(&empty[stage]);
         tcgen05_commit(done);
       }
@@ -500,47 +578,52 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
       next_stage();
     };
     const auto product = [&](int n) {
-      const uint32_t w = tmem + (n & 1) * 128, d = tmem + S::kOutAt + (kOuts == 2 ? (n & 1) * 64 * G : 0);
       const int out = kOuts == 2 ? n & 1 : 0;
-      mbar_wait_mark(&w_full[n & 1], (n >> 1) & 1, abort_flag, bad);
-      mbar_wait_mark(&o_empty[out], ((n / kOuts) & 1) ^ 1, abort_flag, bad);
-      wait_stage();
-      if (!bad && elect_one()) {
-        product_steps(d, w, mn_major(smem_u32(ring + stage * kPart)), 0u);
-        tcgen05_commit(&empty[stage]);
-      }
-      __syncwarp();
+      const uint32_t w = tmem + (n & 1) * 128, d = tmem + S::kOutAt + out * S::kOutCols;
+      await(&w_full[n & 1], (n >> 1) & 1, abort_flag, bad);
+      if (n >= kOuts) await(&o_empty[(n - kOuts) & 1], ((n - kOuts) >> 1) & 1, abort_flag, bad);
+      wait_tile();
+      const int lo = stage;
       next_stage();
-      wait_stage();
       if (!bad && elect_one()) {
-        const uint32_t at = mn_major(smem_u32(ring + stage * kPart));
-        product_steps(d, w + 16, at, 1u);
-        product_steps(d, w, at, 1u);
+        const uint32_t at_lo = mn_major(smem_u32(ring + lo * kPart)), at_hi = mn_major(smem_u32(ring + stage * kPart));
+        if (S::kBeside) {                        // hi * [lo | hi], then lo * hi on top of the first
+          product_steps(d, w, at_lo, beside, 0u);
+          tcgen05_commit(&empty[lo]);
+          product_steps(d, w + 8, at_hi, products, 1u);
+        } else {
+#pragma unroll 1
+          for (int pass = 0; pass < 3; ++pass) {
+            product_steps(d, w + (pass == 1 ? 8 : 0), pass ? at_hi : at_lo, products, pass);
+            if (pass == 0) tcgen05_commit(&empty[lo]);
+          }
+        }
         tcgen05_commit(&empty[stage]);
-        tcgen05_commit(&o_full[out]);
+        tcgen05_commit(&o_full[n & 1]);
       }
       __syncwarp();
       next_stage();
     };
-    mbar_wait_mark(resident_full, 0, abort_flag, bad);
+    await(resident_full, 0, abort_flag, bad);
     const uint32_t rows = k_major(smem_u32(resident));
     int n = 0;
-    while (walk.next(lane, head, t, all)) {
+    for (;; ++n) {
+      await(entry_full + (n & 7), (n >> 3) & 1, abort_flag, bad);
+      bad = __any_sync(0xffffffffu, bad);
+      if (bad || !(entries[n & 7].flags & 1)) break;
       scores(tmem + (n & 1) * 128, rows, &s_full[n & 1]);
       if (kTwo) {
-        mbar_wait_mark(y_empty, (n & 1) ^ 1, abort_flag, bad);
-        scores(tmem + 256, rows + (2 * kPart >> 4), y_full);
+        if (n >= 1) await(&y_empty[(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag, bad);
+        scores(tmem + 256, rows + (2 * kPart >> 4), &y_full[n & 1]);
       }
       if (n > 0) product(n - 1);
-      ++n;
     }
     if (n > 0) product(n - 1);
   }
   } else {
     // ---- weights
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
-    constexpr int kCols = 128 / kParts, kOuts16 = 4 * G / kParts;      // columns of a thread; of products, in sixteens
-    const int quarter = warp & 3, part = (warp - 4) >> 2, row = quarter * 32 + lane;
+    const int quarter = warp & 3, group = (warp - 4) >> 2, row = quarter * 32 + lane;
     const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
     const int off = a.Tk - a.Tq, self = tile * kTile + row;            // query or key
     const bool there = self < (kRowsAreKeys ? a.Tk : a.Tq);
@@ -565,59 +648,54 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     float row_max = 0.f, row_delta = 0.f, row_norm = 0.f;
     if (KIND == kDq) { row_max = p.row_max[row_at * kTile + row]; row_delta = p.row_delta[row_at * kTile + row]; row_norm = p.row_norm[row_at * kTile + row] * sqrtf((float)a.D); }
     const float norm_top = KIND == kDk ? r2.info[row_at].top * sqrtf((float)a.D) : 0.f;
-    float acc[16 * kOuts16];
+    constexpr bool kTurns = S::kTurns;
+    constexpr int kSums = S::kSums;
+    const int col_part = kTurns ? 0 : group * 64, sum_part = kTurns ? 0 : group * kSums;       // of the tile and of the product
+    float acc[kSums];
 #pragma unroll
-    for (int i = 0; i < 16 * kOuts16; ++i) acc[i] = 0.f;
+    for (int i = 0; i < kSums; ++i) acc[i] = 0.f;
     float most = -INFINITY, sum = 0.f;                                 // fwd
     float alpha = 1.f, out_factor = 0.f;                               // of the product in flight
     float slope = 0.f;
     int slope_head = -1;
 
     const auto arrive = [&](uint64_t* bar) { tcgen05_fence_before(); __syncwarp(); if (lane == 0) mbar_arrive(bar); };
-    const auto wait_for = [&](uint64_t* bar, uint32_t parity) { mbar_wait_mark(bar, parity, abort_flag, bad); __syncwarp(); tcgen05_fence_after(); };
+    const auto wait_for = [&](uint64_t* bar, uint32_t parity) { await(bar, parity, abort_flag, bad); __syncwarp(); tcgen05_fence_after(); };
     const auto add_up = [&](int n) {
-      const int out = kOuts == 2 ? n & 1 : 0;
-      wait_for(&o_full[out], (n / kOuts) & 1);
-      const uint32_t from = mine + S::kOutAt + out * 64 * G + part * 16 * kOuts16;
-      float o[16 * kOuts16];
+      wait_for(&o_full[n & 1], (n >> 1) & 1);
+      const uint32_t from = mine + S::kOutAt + (kOuts == 2 ? (n & 1) * S::kOutCols : 0) + sum_part;
 #pragma unroll
-      for (int c = 0; c < kOuts16; c += 2) {
-        if (kOuts16 > 1) tmem_ld32(from + 16 * c, o + 16 * c); else tmem_ld16(from, o);
+      for (int c = 0; c < kSums / 32; ++c) {
+        float o[32], cross[S::kBeside ? 32 : 1];
+        tmem_ld32(from + 32 * c, o);
+        if (S::kBeside) tmem_ld32(from + 64 + 32 * c, cross);
+        tmem_ld_wait();
+        if (c == kSums / 32 - 1) arrive(&o_empty[n & 1]);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          if (S::kBeside) o[k] += cross[k];
+          if (KIND == kFwd) acc[32 * c + k] *= alpha;
+          acc[32 * c + k] = fmaf(o[k], out_factor, acc[32 * c + k]);
+        }
       }
-      tmem_ld_wait();
-      arrive(&o_empty[out]);
-      if (KIND == kFwd) {
-#pragma unroll
-        for (int k = 0; k < 16 * kOuts16; ++k) acc[k] *= alpha;
-      }
-#pragma unroll
-      for (int k = 0; k < 16 * kOuts16; ++k) acc[k] = fmaf(o[k], out_factor, acc[k]);
-    };
-    // What the next tile needs from memory is asked for a tile ahead
-    struct Next { int head, t; bool there, all; float inv1, inv2, top, norm, delta; int64_t at; };
-    const auto look_ahead = [&] {
-      Next x;
-      x.there = walk.next(lane, x.head, x.t, x.all);
-      x.at = x.there ? col_at(x.head, x.t) : 0;
-      const TileInfo &i1 = c1.info[x.at], &i2 = c2.info[x.at];
-      x.inv1 = i1.inv; x.inv2 = i2.inv; x.top = KIND == kDq ? i2.top : 0.f; x.norm = KIND == kDk ? i2.norm : 0.f; x.delta = KIND == kDk ? i2.delta : 0.f;
-      return x;
     };
 
-    int n = 0;
-    Next next = look_ahead();
-    while (next.there) {
-      const Next now = next;
-      next = look_ahead();
+    int n = kTurns ? group : 0;
+    for (;; n += kTurns ? 2 : 1) {
+      await(entry_full + (n & 7), (n >> 3) & 1, abort_flag, bad);
+      bad = __any_sync(0xffffffffu, bad);
+      const Entry now = entries[n & 7];
+      if (bad || !(now.flags & 1)) break;
+      if (kTurns && n >= 2) add_up(n - 2);       // while the scores are being made
       const float f = now.inv1 * unit;
       if (SHAPED && a.slopes && slope_head != (kRowsAreKeys ? now.head : row_head)) {
         slope_head = kRowsAreKeys ? now.head : row_head;
         slope = __ldg(a.slopes + slope_head) * kLog2e;
       }
-      const int col0 = now.t * kTile + (kRowsAreKeys ? off : 0) + part * kCols;                 // position of the first column
+      const int col0 = now.col + col_part;       // position of the first column
       const int at_row = kRowsAreKeys ? self : self + off;
-      const bool masked = !now.all || careful;
-      const uint32_t from = mine + (n & 1) * 128 + part * kCols;
+      const bool masked = !(now.flags & 2) || careful;
+      const uint32_t from = mine + (n & 1) * 128 + col_part;
       // scores of a chunk of 32 columns, capped and biased, in units of log 2; turned: 1 - the cap's tanh squared
       const auto shape32 = [&](float* z, float* turned, int c) {
 #pragma unroll
@@ -647,7 +725,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
           for (int k = 0; k < 32; ++k) same |= __shfl_sync(0xffffffffu, theirs, k) == document ? 1u << k : 0u;
           seen &= document >= 0.f ? same : 0u;
         }
-        const uint32_t spoils = seen & (spoiled ? 0xffffffffu : c1.info[now.at].bad[part * kChunks + c] | c2.info[now.at].bad[part * kChunks + c]);
+        const uint32_t spoils = seen & (spoiled ? 0xffffffffu : c1.info[now.at].bad[col_part / 32 + c] | c2.info[now.at].bad[col_part / 32 + c]);
 #pragma unroll
         for (int k = 0; k < 32; ++k) z[k] = (seen >> k) & 1u ? z[k] : hidden;
         if (__builtin_expect(spoils != 0u, 0)) {
@@ -662,7 +740,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
         const bool rewritten = SHAPED || masked || f < 0.f;
         float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
-        for (int c = 0; c < kChunks; ++c) {
+        for (int c = 0; c < S::kChunks; ++c) {
           float z[32];
           tmem_ld32(from + 32 * c, z);
           tmem_ld_wait();
@@ -679,18 +757,13 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
         }
         if (rewritten) tmem_st_wait();
         const float g = rewritten ? 1.f : f;
-        float* const others = exchange + (n & 1) * (kParts * 128) + row;
-        m[0] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * g;        // of -infinity: NaN if g is 0, which the maximum leaves out
-        others[part * 128] = m[0];
-        asm volatile("barrier.sync %0, %1;" ::"r"(1 + quarter), "n"(32 * kParts) : "memory");
-#pragma unroll
-        for (int i = 0; i < kParts; ++i) m[i] = others[i * 128];
-        const float over = kParts == 2 ? fmaxf(m[0], m[1]) : fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-        const float at_most = fmaxf(most, over), base = max_of_finite_or(at_most), shifted = base - (float)kWeightExp, faded = exp2_fast(most - base);
+        // of -infinity: NaN if g is 0, which the maximum leaves out
+        const float at_most = fmaxf(most, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * g), base = max_of_finite_or(at_most);
+        const float shifted = base - (float)kWeightExp, faded = exp2_fast(most - base);
         most = at_most;
         float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-        for (int c = 0; c < kChunks; ++c) {
+        for (int c = 0; c < S::kChunks; ++c) {
           float z[32];
           uint32_t words[32];
           tmem_ld32(from + 32 * c, z);
@@ -703,7 +776,6 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
         tmem_st_wait();
         arrive(&w_full[n & 1]);
         sum = fmaf(sum, faded, (s[0] + s[1]) + (s[2] + s[3]));
-        if (n > 0) add_up(n - 1);
         alpha = faded;
         out_factor = now.inv2;
       } else {
@@ -712,30 +784,30 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
         if (KIND == kDv) {
           factor = now.inv2 * power_of_two(-kWeightExp);
         } else {
-          const float bound = KIND == kDq ? fmaf(row_norm, now.top, fabsf(row_delta)) : fmaf(now.norm, norm_top, now.delta);
+          const float bound = KIND == kDq ? fmaf(row_norm, now.x, fabsf(row_delta)) : fmaf(now.x, norm_top, now.y);
           shift = min(100, max(-100, kWeightExp - exponent_of(bound)));
           factor = now.inv1 * power_of_two(-shift);
         }
         const float kk = (float)shift, fy = inv2 * now.inv2;
-        const float* const col_max = kRowsAreKeys ? p.row_max + now.at * kTile + part * kCols : nullptr;
-        const float* const col_delta = kRowsAreKeys ? p.row_delta + now.at * kTile + part * kCols : nullptr;
-        if (kTwo) wait_for(y_full, n & 1);
+        const float *const col_max = columns + (n & 1) * 256 + col_part, *const col_delta = col_max + 128;
+        if (kRowsAreKeys) await(&columns_full[n & 1], (n >> 1) & 1, abort_flag, bad);
+        if (kTwo) wait_for(&y_full[n & 1], (n >> 1) & 1);
 #pragma unroll 1
-        for (int c = 0; c < kChunks; ++c) {
+        for (int c = 0; c < S::kChunks; ++c) {
           float z[32], y[32], turned[SHAPED && kTwo ? 32 : 1];
           tmem_ld32(from + 32 * c, z);
-          if (kTwo) tmem_ld32(mine + 256 + part * kCols + 32 * c, y);
+          if (kTwo) tmem_ld32(mine + 256 + col_part + 32 * c, y);
           tmem_ld_wait();
-          if (kTwo && c == kChunks - 1) arrive(y_empty);
+          if (kTwo && c == S::kChunks - 1) arrive(&y_empty[n & 1]);
           if (SHAPED) shape32(z, kTwo ? turned : nullptr, c);
           const float g = SHAPED ? 1.f : f;
           if (kRowsAreKeys) {
 #pragma unroll
             for (int k = 0; k < 32; k += 4) {
-              const float4 m4 = __ldg(reinterpret_cast<const float4*>(col_max + 32 * c + k));
+              const float4 m4 = *reinterpret_cast<const float4*>(col_max + 32 * c + k);
               z[k] = fmaf(z[k], g, kk - m4.x); z[k + 1] = fmaf(z[k + 1], g, kk - m4.y); z[k + 2] = fmaf(z[k + 2], g, kk - m4.z); z[k + 3] = fmaf(z[k + 3], g, kk - m4.w);
               if (KIND == kDk) {
-                const float4 d4 = __ldg(reinterpret_cast<const float4*>(col_delta + 32 * c + k));
+                const float4 d4 = *reinterpret_cast<const float4*>(col_delta + 32 * c + k);
                 y[k] = fmaf(y[k], fy, -d4.x); y[k + 1] = fmaf(y[k + 1], fy, -d4.y); y[k + 2] = fmaf(y[k + 2], fy, -d4.z); y[k + 3] = fmaf(y[k + 3], fy, -d4.w);
               }
             }
@@ -756,36 +828,62 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
         }
         tmem_st_wait();
         arrive(&w_full[n & 1]);
-        if (n > 0) add_up(n - 1);
+        if (!kTurns && n >= 1) add_up(n - 1);
         out_factor = factor;
       }
-      ++n;
     }
-    if (n > 0) add_up(n - 1);
+    if (n >= (kTurns ? 2 : 1)) add_up(n - (kTurns ? 2 : 1));           // n: where the list ends for this warp
 
     float last = KIND == kDv ? 1.f : a.scale;
-    if (KIND == kFwd) {
-      exchange[part * 128 + row] = sum;                                // nobody reads the last tile's maxima any more: its product has been added up
-      asm volatile("barrier.sync %0, %1;" ::"r"(1 + quarter), "n"(32 * kParts) : "memory");
-      sum = 0.f;
+    if (kTurns) {
+      // The second group's sums go through the memory of the rows, which no MMA reads any more: those of the last tile were issued before the product
+      // of the tile before it.  Columns by rows, so that a warp's words lie side by side.
+      float* const handed = reinterpret_cast<float*>(resident);
+      volatile int* const any_handed = abort_flag + 1;
+      if (group == 1) {
+        if (n >= 3) {
 #pragma unroll
-      for (int i = 0; i < kParts; ++i) sum += exchange[i * 128 + row]; // in the same order everywhere
-      last = sum == 0.f ? 0.f : 1.f / sum;
-      if (a.stats && part == 0 && there) {
-        float* const to = a.stats + 2 * (((int64_t)b * a.H + row_head) * a.Tq + self);
-        to[0] = max_of_finite_or(most); to[1] = last * (float)(1 << kWeightExp);
+          for (int k = 0; k < kSums; ++k) handed[k * kTile + row] = acc[k];
+        }
+        if (KIND == kFwd) { statistics[row] = most; statistics[kTile + row] = sum; }
+        if (lane == 0) *any_handed = n >= 3;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(merge);
+      } else {
+        await(merge, 0, abort_flag, bad);
+        float other = last;
+        if (KIND == kFwd) {
+          const float base = max_of_finite_or(fmaxf(most, statistics[row])), here = exp2_fast(most - base), over_there = exp2_fast(statistics[row] - base);
+          sum = sum * here + statistics[kTile + row] * over_there;
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          last = inv * here; other = inv * over_there;
+          if (a.stats && there) {
+            float* const to = a.stats + 2 * (((int64_t)b * a.H + row_head) * a.Tq + self);
+            to[0] = base; to[1] = inv * (float)(1 << kWeightExp);
+          }
+        }
+        if (*any_handed) {
+#pragma unroll
+          for (int k = 0; k < kSums; ++k) acc[k] = fmaf(handed[k * kTile + row], other, acc[k] * last);
+        } else {
+#pragma unroll
+          for (int k = 0; k < kSums; ++k) acc[k] *= last;
+        }
       }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kSums; ++k) acc[k] *= last;
     }
-    if (there && !*abort_flag) {
+    if (there && !*abort_flag && !(kTurns && group == 1)) {
       float* const result = KIND == kFwd ? a.o : KIND == kDq ? a.dq : KIND == kDk ? a.dk : a.dv;
-      float* const to = result + (((int64_t)b * (kRowsAreKeys ? a.Tk : a.Tq) + self) * row_heads + row_head) * a.D + part * 16 * kOuts16;
-      const int cols = a.D - part * 16 * kOuts16;
+      float* const to = result + (((int64_t)b * (kRowsAreKeys ? a.Tk : a.Tq) + self) * row_heads + row_head) * a.D + sum_part;
+      const int cols = a.D - sum_part;
       if (a.D % 4 == 0 && (reinterpret_cast<uintptr_t>(result) & 15) == 0) {
 #pragma unroll
-        for (int k = 0; k < 16 * kOuts16; k += 4) if (k < cols) *reinterpret_cast<float4*>(to + k) = make_float4(acc[k] * last, acc[k + 1] * last, acc[k + 2] * last, acc[k + 3] * last);
+        for (int k = 0; k < kSums; k += 4) if (k < cols) *reinterpret_cast<float4*>(to + k) = make_float4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]);
       } else {
 #pragma unroll
-        for (int k = 0; k < 16 * kOuts16; ++k) if (k < cols) to[k] = acc[k] * last;
+        for (int k = 0; k < kSums; ++k) if (k < cols) to[k] = acc[k];
       }
     }
   }
