@@ -137,7 +137,26 @@ LARGE = [
     dict(batch=1, queries=700, keys=130, heads=2, kv_heads=1, dim=96),
     dict(batch=1, queries=1025, keys=1025, heads=1, kv_heads=1, dim=128, bias=True, cap=30.0),
 ]
+FEW = [
+    dict(batch=3, queries=1, keys=1, heads=4, kv_heads=2, dim=64),
+    dict(batch=2, queries=1, keys=1000, heads=8, kv_heads=2, dim=128),
+    dict(batch=1, queries=1, keys=4097, heads=8, kv_heads=1, dim=64, bias=True, cap=30.0),
+    dict(batch=9, queries=1, keys=130, heads=24, kv_heads=12, dim=72, window=50),
+    dict(batch=2, queries=3, keys=700, heads=4, kv_heads=2, dim=33, causal=False, window=100, prefix=[0, 20]),
+    dict(batch=2, queries=5, keys=611, heads=3, kv_heads=1, dim=80, documents="mixed"),
+    dict(batch=2, queries=2, keys=900, heads=2, kv_heads=2, dim=256, prefix=[40, 1000], cap=5.0),
+    dict(batch=1, queries=4, keys=3, heads=2, kv_heads=1, dim=16),
+    dict(batch=40, queries=1, keys=65, heads=16, kv_heads=16, dim=128),
+]
 IDS = lambda k: "-".join("%s%s" % (n[0], v) for n, v in k.items())      # noqa: E731
+
+
+@pytest.mark.parametrize("kind", FEW, ids=IDS)
+@pytest.mark.parametrize("misaligned", [0, 1])
+def test_few_queries(env, kind, misaligned):
+    """The forward call of few queries; the backward call takes its statistics."""
+    c = Case(**kind)
+    check(env, c, misaligned=misaligned)
 
 
 @pytest.fixture(params=["exact", "tensor"])

@@ -24,6 +24,10 @@ struct AttentionArgs {
 #ifdef __CUDACC__
 constexpr float kLog2e = 1.4426950408889634f;
 
+// Both of 2 ulp; below 2^-126 zero
+__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ float reciprocal(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+
 // The keys of a query at position `at`: those of [lo, hi] and those before `prefix`, if of its document.
 struct Sight { int lo, hi; };
 __device__ __forceinline__ Sight sight_of(const AttentionArgs& a, int at) {

@@ -327,8 +327,6 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_low, u
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
                ::"r"(d), "r"(a), "l"((uint64_t)b_low | (uint64_t)b_high << 32), "r"(idesc), "r"(keep) : "memory");
 }
-__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ float reciprocal(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
 // cap * tanh(x / cap) of 32 numbers, t = the tanh.  Up to 0.35 by the series of odd powers (x^13 behind it is 4e-9 of x there), whose error is relative; above by
 // 1 - 2 / (e^2x + 1), whose error is a rounding of 1.  Scores far below the cap, most of all, take the series alone.

@@ -12,6 +12,7 @@
 namespace tf {
 
 bool attention_tc_takes(const AttentionArgs& a);
+int attention_few(const AttentionArgs& a, size_t* bytes, cudaStream_t s, const char* what);
 int attention_tc(const AttentionArgs& a, bool backward, size_t* bytes, cudaStream_t s, const char* what);
 void note_contraction_path(int path);
 
@@ -440,6 +441,8 @@ int check_attention(const char* what, const AttentionState* st, const DLArray* q
   a->causal = st->causal; a->window = std::min(st->window, 1 << 25); a->scale = st->scale; a->cap = st->cap;
   return 0;
 }
+// Up to 16 rows a key-value head, whose keys the kernel of few queries reads once for every four
+bool few_queries(const AttentionArgs& a) { return (int64_t)a.group * a.Tq <= 16 && a.Tk > 0; }
 bool tensor_path_pays(const AttentionArgs& a, bool backward) { return (int64_t)a.Tq >= 64 && a.Tk >= 64; }
 // 0: the exact kernels are to run, 1: launched, or short of memory; -1: error
 int run_tensor_path(const AttentionArgs& a, bool backward, int* memorytoSaving, cudaStream_t s, const char* what) {
@@ -496,8 +499,17 @@ int TfAttentionForward(const DLArrayHandle query, const DLArrayHandle key, const
   if (a.B == 0) return 0;
   note_compute_stream(s);
   KernelTimer kt(what, s, 4.0 * a.B * a.H * (double)a.Tq * a.Tk * a.D, 4.0 * (2.0 * numel(query) + 2.0 * numel(key)));
-  if (const int r = run_tensor_path(a, false, memorytoSaving, s, what)) return r < 0 ? -1 : 0;
+  const bool few = few_queries(a) && contraction_path() != 2;
+  if (!few) {
+    if (const int r = run_tensor_path(a, false, memorytoSaving, s, what)) return r < 0 ? -1 : 0;
+  }
   note_contraction_path(1);
+  if (few) {
+    size_t bytes = 0;
+    const int r = attention_few(a, &bytes, s, what);
+    if (r > 0 && memorytoSaving) *memorytoSaving = bytes > 0x7fffffffu ? 0x7fffffff : (int)bytes;
+    return r < 0 ? -1 : 0;
+  }
   TF_CUDA(tile_fwd(a, s));
   TF_AFTER(s, what);
   return 0;
