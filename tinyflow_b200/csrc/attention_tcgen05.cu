@@ -295,22 +295,25 @@ template <int KIND, int G> struct Shape {
   static constexpr int kWeightWarps = kTurns ? 4 : 8;                // of a tile
   static constexpr int kChunks = kTurns ? 4 : 2;                     // of 32 columns, a thread
   static constexpr int kSums = kTurns ? 64 * G : 32 * G;             // columns of the product that a thread adds up
-  // Heads of up to 64: the hi halves of the weights multiply both halves of the other operand at once, side by side in N.  An MMA of N = 64 takes as long as one of 128.
-  static constexpr bool kBeside = G == 1;
+  // The rows' first operand lies in TMEM where there is room beside scores and products: an MMA of 128 columns takes 73 cycles then, 102 with both operands in shared memory.
+  static constexpr bool kRowsInTmem = !kTwo || G == 1;
   static constexpr int kPart = G * 16384;                            // one half (hi or lo) of a tile
-  static constexpr int kResident = (kTwo ? 4 : 2) * kPart;
+  static constexpr int kResident = (kTwo ? 2 : 0) * kPart + (kRowsInTmem ? 0 : 2) * kPart;
   static constexpr int kControl = 768 + (KIND == kFwd ? 1024 : 0) + (kRowsAreKeys ? 2048 : 0);
   static constexpr int kFits = (232448 - kControl - kResident) / kPart, kStages = kFits < 8 ? kFits : 8;
   static constexpr int kSmem = kResident + kStages * kPart + kControl;
-  static constexpr int kOutCols = kBeside ? 128 : 64 * G;            // TMEM: scores 0 and 128, second scores 256, products behind
-  static constexpr int kOuts = kTwo ? 1 : 2;
-  static constexpr int kOutAt = kTwo ? 384 : 256;
-  static_assert(kStages >= 3 && (!kBeside || kStages % 2 == 0) && kOutAt + kOuts * kOutCols <= 512, "fits");
+  // TMEM columns: scores 0 and 128, then
+  static constexpr int kYAt = 256;                                   // second scores
+  static constexpr int kOuts = !kTwo && G == 1 ? 2 : 1;
+  static constexpr int kRowsAt = kTwo ? 448 : 256;                   // hi, then lo
+  static constexpr int kOutAt = kTwo ? 384 : 256 + 64 * G;
+  static_assert(kStages >= 3 && kOutAt + kOuts * 64 * G <= (kTwo && G == 1 ? 448 : 512), "fits");
+  static_assert(!kTurns || kStages * kPart >= kSums * kTile * 4, "the sums of a group fit the ring");
 };
 // Of one tile of columns, for the warps: written by the copying warp, which walks the list.  Eight of them in turn: by the time a copy for tile n + 8 can be issued,
 // the weights of tile n + 4 have been made.
 struct __align__(16) Entry {
-  int flags, head, col, at;                      // 1: there is a tile, 2: every row sees all of it; position of its first column; its number
+  int flags, head, col, at;                      // 1: there is a tile, 2: every row sees all of it; position of its first column; its number, or behind the last how many there were
   float inv1, inv2, x, y;                        // 1 / scale of both operands; dq: largest magnitude of V, dk: largest norm and |D'| of dO'
 };
 
@@ -394,12 +397,13 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
   uint64_t* const o_empty = o_full + 2;          // [2] and has been added up
   uint64_t* const columns_full = o_empty + 2;    // [2] maxima and D' of a tile of queries
   uint64_t* const merge = columns_full + 2;      // the second group's sums are in shared memory
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(merge + 1);
+  uint64_t* const rows_full = merge + 1;         // the rows are in TMEM
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(rows_full + 1);
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   Entry* const entries = reinterpret_cast<Entry*>(full + 64);        // [8]
   float* const statistics = reinterpret_cast<float*>(entries + 8);   // fwd: [2][128] of the second group
   float* const columns = statistics;                                 // dk, dv: [2][2][128]
-  static_assert(8 + 8 + 8 + 1 + 7 * 2 + 1 + 1 <= 64, "barriers fit");
+  static_assert(8 + 8 + 8 + 1 + 7 * 2 + 2 + 2 <= 64, "barriers fit");
   const AttentionArgs& a = p.a;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
@@ -414,7 +418,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
         mbar_init(o_full + i, 1); mbar_init(o_empty + i, S::kWeightWarps);
         mbar_init(columns_full + i, 1);
       }
-      mbar_init(merge, 4);
+      mbar_init(merge, 4); mbar_init(rows_full, 8);
       *abort_flag = (smem_u32(smem) & 1023u) ? 1 : 0;                // nothing is issued then
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -447,11 +451,11 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     int stage = 0;
     uint32_t phase = 0, armed = 0, phases = 0, columns_armed = 0;
     bool rows_armed = false;
-    if (!bad) {
+    if (S::kResident && !bad) {
       if (elect_one()) {
         mbar_expect_tx(resident_full, S::kResident);
-        bulk_load(resident, r1.image + row_at * 2 * kPart, 2 * kPart, resident_full);
-        if (kTwo) bulk_load(resident + 2 * kPart, r2.image + row_at * 2 * kPart, 2 * kPart, resident_full);
+        bulk_load(resident, r2.image + row_at * 2 * kPart, 2 * kPart, resident_full);
+        if (!S::kRowsInTmem) bulk_load(resident + 2 * kPart, r1.image + row_at * 2 * kPart, 2 * kPart, resident_full);
       }
       rows_armed = true;
     }
@@ -487,12 +491,12 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     for (int n = 0;; ++n) {
       const Next now = next;
       if (lane == 0) {
-        entries[n & 7] = Entry{now.there ? 1 | (int)now.all << 1 : 0, now.head, now.t * kTile + (kRowsAreKeys ? a.Tk - a.Tq : 0), (int)now.at, now.inv1, now.inv2, now.x, now.y};
+        entries[n & 7] = Entry{now.there ? 1 | (int)now.all << 1 : 0, now.head, now.t * kTile + (kRowsAreKeys ? a.Tk - a.Tq : 0), now.there ? (int)now.at : n, now.inv1, now.inv2, now.x, now.y};
         mbar_arrive(entry_full + (n & 7));
       }
       __syncwarp();
       if (!now.there) {                          // and for the other group, whose tile would be the next
-        if (lane == 0) { entries[(n + 1) & 7].flags = 0; mbar_arrive(entry_full + ((n + 1) & 7)); }
+        if (lane == 0) { entries[(n + 1) & 7].flags = 0; entries[(n + 1) & 7].at = n; mbar_arrive(entry_full + ((n + 1) & 7)); }
         break;
       }
       next = look_ahead();
@@ -532,7 +536,6 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     // ---- MMAs
     constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(kTile >> 4) << 24), kScores = kIdesc | ((uint32_t)(kTile >> 3) << 17);
     const uint32_t products = kIdesc | (1u << 16) | ((uint32_t)(p.D16 >> 3) << 17);            // the B operand has its columns (the head) along the rows of memory
-    const uint32_t beside = products + (64u >> 3 << 17);
     const int steps = p.D16 / 16;
     int stage = 0;
     uint32_t phase = 0;
@@ -549,16 +552,21 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
       tcgen05_fence_after();
     };
     const auto next_stage = [&] { if (++stage == kStages) { stage = 0; phase ^= 1; } };
-    const auto score_steps = [&](uint32_t d, uint32_t rows_low, uint32_t cols_low, uint32_t keep) {
+    // rows: the low word of their descriptor, or where they lie in TMEM
+    const auto score_steps = [&](uint32_t d, uint32_t rows, bool in_tmem, uint32_t cols_low, uint32_t keep) {
 #pragma unroll
-      for (int ks = 0; ks < 4 * G; ++ks)
-        if (ks < steps) mma_ss(d, rows_low + (ks >> 2) * 1024 + (ks & 3) * 2, kHigh, cols_low + (ks >> 2) * 1024 + (ks & 3) * 2, kHigh, kScores, ks ? 1u : keep);
+      for (int ks = 0; ks < 4 * G; ++ks) {
+        const uint32_t step = (ks >> 2) * 1024 + (ks & 3) * 2;
+        if (ks >= steps) continue;
+        if (in_tmem) mma_ts(d, rows + 8 * ks, cols_low + step, kHigh, kScores, ks ? 1u : keep);
+        else mma_ss(d, rows + step, kHigh, cols_low + step, kHigh, kScores, ks ? 1u : keep);
+      }
     };
     const auto product_steps = [&](uint32_t d, uint32_t w, uint32_t cols_low, uint32_t idesc, uint32_t keep) {
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) mma_ts(d, w + 16 * ks, cols_low + ks * 128, kHigh, idesc, ks ? 1u : keep);
     };
-    const auto scores = [&](uint32_t d, uint32_t rows_hi, uint64_t* done) {
+    const auto scores = [&](uint32_t d, uint32_t rows_hi, auto in_tmem, uint64_t* done) {
       wait_tile();
       const int lo = stage;
       next_stage();
@@ -566,7 +574,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
         const uint32_t at_lo = k_major(smem_u32(ring + lo * kPart)), at_hi = k_major(smem_u32(ring + stage * kPart));
 #pragma unroll 1
         for (int pass = 0; pass < 3; ++pass) {   // hi * lo, lo * hi, hi * hi
-          score_steps(d, rows_hi + (pass == 1 ? kPart >> 4 : 0), pass ? at_hi : at_lo, pass);
+          score_steps(d, rows_hi + (pass != 1 ? 0 : decltype(in_tmem)::value ? 32 * G : kPart >> 4), decltype(in_tmem)::value, pass ? at_hi : at_lo, pass);
           if (pass == 0) tcgen05_commit(&empty[lo]);
         }
         tcgen05_commit(&empty[stage]);
@@ -577,7 +585,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     };
     const auto product = [&](int n) {
       const int out = kOuts == 2 ? n & 1 : 0;
-      const uint32_t w = tmem + (n & 1) * 128, d = tmem + S::kOutAt + out * S::kOutCols;
+      const uint32_t w = tmem + (n & 1) * 128, d = tmem + S::kOutAt + out * 64 * G;
       await(&w_full[n & 1], (n >> 1) & 1, abort_flag, bad);
       if (n >= kOuts) await(&o_empty[(n - kOuts) & 1], ((n - kOuts) >> 1) & 1, abort_flag, bad);
       wait_tile();
@@ -585,16 +593,10 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
       next_stage();
       if (!bad && elect_one()) {
         const uint32_t at_lo = mn_major(smem_u32(ring + lo * kPart)), at_hi = mn_major(smem_u32(ring + stage * kPart));
-        if (S::kBeside) {                        // hi * [lo | hi], then lo * hi on top of the first
-          product_steps(d, w, at_lo, beside, 0u);
-          tcgen05_commit(&empty[lo]);
-          product_steps(d, w + 8, at_hi, products, 1u);
-        } else {
 #pragma unroll 1
-          for (int pass = 0; pass < 3; ++pass) {
-            product_steps(d, w + (pass == 1 ? 8 : 0), pass ? at_hi : at_lo, products, pass);
-            if (pass == 0) tcgen05_commit(&empty[lo]);
-          }
+        for (int pass = 0; pass < 3; ++pass) {
+          product_steps(d, w + (pass == 1 ? 8 : 0), pass ? at_hi : at_lo, products, pass);
+          if (pass == 0) tcgen05_commit(&empty[lo]);
         }
         tcgen05_commit(&empty[stage]);
         tcgen05_commit(&o_full[n & 1]);
@@ -602,17 +604,18 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
       __syncwarp();
       next_stage();
     };
-    await(resident_full, 0, abort_flag, bad);
-    const uint32_t rows = k_major(smem_u32(resident));
+    if (S::kResident) await(resident_full, 0, abort_flag, bad);
+    if (S::kRowsInTmem) { await(rows_full, 0, abort_flag, bad); __syncwarp(); tcgen05_fence_after(); }
+    const uint32_t rows2 = k_major(smem_u32(resident)), rows1 = S::kRowsInTmem ? tmem + S::kRowsAt : rows2 + (2 * kPart >> 4);
     int n = 0;
     for (;; ++n) {
       await(entry_full + (n & 7), (n >> 3) & 1, abort_flag, bad);
       bad = __any_sync(0xffffffffu, bad);
       if (bad || !(entries[n & 7].flags & 1)) break;
-      scores(tmem + (n & 1) * 128, rows, &s_full[n & 1]);
+      scores(tmem + (n & 1) * 128, rows1, std::integral_constant<bool, S::kRowsInTmem>(), &s_full[n & 1]);
       if (kTwo) {
         if (n >= 1) await(&y_empty[(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag, bad);
-        scores(tmem + 256, rows + (2 * kPart >> 4), &y_full[n & 1]);
+        scores(tmem + S::kYAt, rows2, std::false_type(), &y_full[n & 1]);
       }
       if (n > 0) product(n - 1);
     }
@@ -623,6 +626,20 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
     const int quarter = warp & 3, group = (warp - 4) >> 2, row = quarter * 32 + lane;
     const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
+    if (S::kRowsInTmem) {                        // one group moves the hi halves of the rows, the other the lo halves
+      const char* const image = r1.image + (row_at * 2 + group) * kPart + row * 128;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        uint4 words[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) words[c] = *reinterpret_cast<const uint4*>(image + g * 16384 + ((c ^ (row & 7)) << 4));
+        tmem_st32(mine + S::kRowsAt + group * 32 * G + g * 32, reinterpret_cast<const uint32_t*>(words));
+      }
+      tmem_st_wait();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(rows_full);
+    }
     const int off = a.Tk - a.Tq, self = tile * kTile + row;            // query or key
     const bool there = self < (kRowsAreKeys ? a.Tk : a.Tq);
     // columns that the row sees: positions [lo, hi] and those before `extra`
@@ -661,17 +678,15 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     const auto wait_for = [&](uint64_t* bar, uint32_t parity) { await(bar, parity, abort_flag, bad); __syncwarp(); tcgen05_fence_after(); };
     const auto add_up = [&](int n) {
       wait_for(&o_full[n & 1], (n >> 1) & 1);
-      const uint32_t from = mine + S::kOutAt + (kOuts == 2 ? (n & 1) * S::kOutCols : 0) + sum_part;
+      const uint32_t from = mine + S::kOutAt + (kOuts == 2 ? (n & 1) * 64 * G : 0) + sum_part;
 #pragma unroll
       for (int c = 0; c < kSums / 32; ++c) {
-        float o[32], cross[S::kBeside ? 32 : 1];
+        float o[32];
         tmem_ld32(from + 32 * c, o);
-        if (S::kBeside) tmem_ld32(from + 64 + 32 * c, cross);
         tmem_ld_wait();
         if (c == kSums / 32 - 1) arrive(&o_empty[n & 1]);
 #pragma unroll
         for (int k = 0; k < 32; ++k) {
-          if (S::kBeside) o[k] += cross[k];
           if (KIND == kFwd) acc[32 * c + k] *= alpha;
           acc[32 * c + k] = fmaf(o[k], out_factor, acc[32 * c + k]);
         }
@@ -794,7 +809,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
         for (int c = 0; c < S::kChunks; ++c) {
           float z[32], y[32], turned[SHAPED && kTwo ? 32 : 1];
           tmem_ld32(from + 32 * c, z);
-          if (kTwo) tmem_ld32(mine + 256 + col_part + 32 * c, y);
+          if (kTwo) tmem_ld32(mine + S::kYAt + col_part + 32 * c, y);
           tmem_ld_wait();
           if (kTwo && c == S::kChunks - 1) arrive(&y_empty[n & 1]);
           if (SHAPED) shape32(z, kTwo ? turned : nullptr, c);
@@ -834,17 +849,18 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
 
     float last = KIND == kDv ? 1.f : a.scale;
     if (kTurns) {
-      // The second group's sums go through the memory of the rows, which no MMA reads any more: those of the last tile were issued before the product
-      // of the tile before it.  Columns by rows, so that a warp's words lie side by side.
-      float* const handed = reinterpret_cast<float*>(resident);
+      // The second group's sums go through the ring, once the last product has read it.  Columns by rows, so that a warp's words lie side by side.
+      float* const handed = reinterpret_cast<float*>(ring);
       volatile int* const any_handed = abort_flag + 1;
       if (group == 1) {
-        if (n >= 3) {
+        const int tiles = entries[n & 7].at;
+        if (n >= 3 && !bad) await(&o_full[(tiles - 1) & 1], ((tiles - 1) >> 1) & 1, abort_flag, bad);
+        if (n >= 3 && !bad) {
 #pragma unroll
           for (int k = 0; k < kSums; ++k) handed[k * kTile + row] = acc[k];
         }
         if (KIND == kFwd) { statistics[row] = most; statistics[kTile + row] = sum; }
-        if (lane == 0) *any_handed = n >= 3;
+        if (lane == 0) *any_handed = n >= 3 && !bad;
         __syncwarp();
         if (lane == 0) mbar_arrive(merge);
       } else {
