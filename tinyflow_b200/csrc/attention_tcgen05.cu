@@ -56,7 +56,8 @@ struct TcArgs {
   Packed q, k, v, d;
   const float *row_max, *row_delta, *row_norm;   // of every sequence, head and query, tiles padded with zeros
   const float4* documents;                       // of every sequence and key tile: smallest, largest, whether there is padding
-  int q_tiles, k_tiles, D16;
+  float *dk_part, *dv_part;                      // where the query heads of a key-value head are dealt to several CTAs: their sums, one after another
+  int q_tiles, k_tiles, D16, shares;
   int* err;
 };
 
@@ -226,12 +227,12 @@ template <int KIND> struct Walk {
   float low, high;                               // their documents
   bool padding;
   uint32_t any, whole;
-  __device__ __forceinline__ Walk(const TcArgs& args, int b_, int row_head, int tile) : p(args), b(b_) {
+  __device__ __forceinline__ Walk(const TcArgs& args, int b_, int row_head, int share, int tile) : p(args), b(b_) {
     const AttentionArgs& a = p.a;
     const int off = a.Tk - a.Tq;
     prefix = prefix_of(a, b);
     tiles = kRowsAreKeys ? p.q_tiles : p.k_tiles;
-    if (kRowsAreKeys) { head = row_head * a.group; heads_end = head + a.group; from = tile * kTile; to = min(from + kTile, a.Tk) - 1; }
+    if (kRowsAreKeys) { heads_end = a.group / p.shares; head = row_head * a.group + share * heads_end; heads_end += head; from = tile * kTile; to = min(from + kTile, a.Tk) - 1; }
     else { head = row_head; heads_end = head + 1; from = tile * kTile + off; to = min(from + kTile - 1, a.Tk - 1); }
     low = high = 0.f; padding = false;
     if (p.documents) documents(from, to, low, high, padding);
@@ -436,7 +437,8 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
 
   // rows that see most go first
   const int row_heads = kRowsAreKeys ? a.G : a.H, col_tiles = kRowsAreKeys ? p.q_tiles : p.k_tiles, row_tiles = kRowsAreKeys ? p.k_tiles : p.q_tiles;
-  const int order = block / (a.B * row_heads), lane_of = block - order * (a.B * row_heads), b = lane_of / row_heads, row_head = lane_of - b * row_heads;
+  const int shares = kRowsAreKeys ? p.shares : 1, across = a.B * row_heads * shares, order = block / across, place = block - order * across;
+  const int b = place / (row_heads * shares), row_head = place / shares - b * row_heads, share = place % shares;
   const int tile = kRowsAreKeys ? order : row_tiles - 1 - order;
   const int64_t row_at = ((int64_t)b * row_heads + row_head) * row_tiles + tile;
   const Packed &r1 = kRowsAreKeys ? p.k : p.q, &r2 = kRowsAreKeys ? p.v : p.d;                 // rows
@@ -459,7 +461,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
       }
       rows_armed = true;
     }
-    Walk<KIND> walk(p, b, row_head, tile);
+    Walk<KIND> walk(p, b, row_head, share, tile);
     // What an entry says is asked for a tile ahead
     struct Next { bool there, all; int head, t; int64_t at; float inv1, inv2, x, y; };
     const auto look_ahead = [&] {
@@ -889,7 +891,8 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
       for (int k = 0; k < kSums; ++k) acc[k] *= last;
     }
     if (there && !*abort_flag && !(kTurns && group == 1)) {
-      float* const result = KIND == kFwd ? a.o : KIND == kDq ? a.dq : KIND == kDk ? a.dk : a.dv;
+      float* result = KIND == kFwd ? a.o : KIND == kDq ? a.dq : KIND == kDk ? a.dk : a.dv;
+      if (shares > 1) result = (KIND == kDk ? p.dk_part : p.dv_part) + share * ((int64_t)a.B * a.Tk * a.G * a.D);
       float* const to = result + (((int64_t)b * (kRowsAreKeys ? a.Tk : a.Tq) + self) * row_heads + row_head) * a.D + sum_part;
       const int cols = a.D - sum_part;
       if (a.D % 4 == 0 && (reinterpret_cast<uintptr_t>(result) & 15) == 0) {
@@ -920,6 +923,20 @@ template <int G, bool SHAPED> __global__ void __launch_bounds__(kThreads, 1) att
   else attention_rows<kDq, G, SHAPED>(p, block - dk_blocks - dv_blocks);
 }
 
+// The sums of the shares, in their order; dk (y 0) and dv (y 1).
+__global__ void __launch_bounds__(256) attention_add_kernel(const float* __restrict__ dk_part, const float* __restrict__ dv_part, float* dk, float* dv, int64_t n, int shares) {
+  grid_dep_sync();
+  const float* const part = blockIdx.y ? dv_part : dk_part;
+  float* const to = blockIdx.y ? dv : dk;
+  if (!to) return;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    float s = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < shares; ++k) s += __ldg(part + k * n + i);
+    to[i] = s;
+  }
+}
+
 // ---- host side ------------------------------------------------------------------------------------------------------------
 template <int G, bool SHAPED> cudaError_t launch_fwd(const TcArgs& p, cudaStream_t s) {
   static std::atomic<uint64_t> ready{0};
@@ -933,7 +950,7 @@ template <int G, bool SHAPED> cudaError_t launch_bwd(const TcArgs& p, cudaStream
   const auto kernel = attention_tc_bwd_kernel<G, SHAPED>;
   const int bytes = std::max(std::max(Shape<kDq, G>::kSmem, Shape<kDk, G>::kSmem), Shape<kDv, G>::kSmem);
   const cudaError_t e = once_per_device(ready, [kernel, bytes] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
-  const int keys = p.a.B * p.a.G * p.k_tiles, dk = p.a.dk ? keys : 0, dv = p.a.dv ? keys : 0, dq = p.a.dq ? p.a.B * p.a.H * p.q_tiles : 0;
+  const int keys = p.a.B * p.a.G * p.shares * p.k_tiles, dk = p.a.dk ? keys : 0, dv = p.a.dv ? keys : 0, dq = p.a.dq ? p.a.B * p.a.H * p.q_tiles : 0;
   return e != cudaSuccess ? e : launch_dep(kernel, dim3((unsigned)(dk + dv + dq)), dim3(kThreads), (size_t)bytes, s, p, dk, dv);
 }
 template <class F> cudaError_t with_form(const AttentionArgs& a, F&& f) {
@@ -947,7 +964,20 @@ template <class F> cudaError_t with_form(const AttentionArgs& a, F&& f) {
 // Whether the path takes the call: heads of up to 128 elements, grids that the launch can have
 bool attention_tc_takes(const AttentionArgs& a) {
   const int64_t q_tiles = (a.Tq + kTile - 1) / kTile, k_tiles = (a.Tk + kTile - 1) / kTile;
-  return a.D <= 128 && a.Tk > 0 && (int64_t)a.B * (2 * a.H * q_tiles + 2 * a.G * k_tiles) < (1ll << 31);
+  return a.D <= 128 && a.Tk > 0 && (int64_t)a.B * (2 * a.H * q_tiles + 2 * a.H * k_tiles) < (1ll << 31);
+}
+// CTAs that the query heads of a key-value head are dealt to in dk and dv.  One, unless the longest CTA would outlast the others: then as few as end that, if what they save (2.5 us a
+// tile) is more than adding up their sums takes.  2 x 6 heads over 2, 777 queries: 105 us with one, 49 with three.
+static int shares_of(const AttentionArgs& a) {
+  const double qt = (a.Tq + kTile - 1) / kTile, kt = (a.Tk + kTile - 1) / kTile, sms = device_sm_count();
+  const double total = (double)a.B * a.H * qt * kt * 8 * (a.causal && !a.prefix ? 0.5 : 1.0), nk = (double)a.B * a.Tk * a.G * a.D;
+  for (int s = 1; s <= a.group; ++s) {
+    if (a.group % s) continue;
+    const double longest = 3.0 * (a.group / s) * qt;
+    if (longest <= 0.6 * total / sms || s == a.group)
+      return (a.group - a.group / s) * qt * 2.5 > 3.0 + nk * 16 * s / 5e6 ? s : 1;
+  }
+  return 1;
 }
 // Scratch, in bytes, of a forward or a backward call; with `base`, where its parts lie
 static size_t lay_out(const AttentionArgs& a, bool backward, char* base, PackArgs* pack, TcArgs* tc) {
@@ -973,12 +1003,16 @@ static size_t lay_out(const AttentionArgs& a, bool backward, char* base, PackArg
   }
   char* rows[3] = {nullptr, nullptr, nullptr};
   if (backward) for (char*& r : rows) r = take(nq * kTile * sizeof(float));
+  const int shares = backward ? shares_of(a) : 1;
+  const size_t part = shares > 1 ? (size_t)shares * a.B * a.Tk * a.G * a.D * sizeof(float) : 0;
+  char *const dk_part = a.dk && part ? take(part) : nullptr, *const dv_part = a.dv && part ? take(part) : nullptr;
   char* const docs = a.documents ? take((size_t)a.B * k_tiles * sizeof(float4)) : nullptr;
   if (base) {
     pack->a = a; pack->jobs = jobs; pack->first[jobs] = blocks; pack->document_job = 1;
     pack->row_max = (float*)rows[0]; pack->row_delta = (float*)rows[1]; pack->row_norm = (float*)rows[2]; pack->documents = (float4*)docs;
     tc->a = a; tc->row_max = pack->row_max; tc->row_delta = pack->row_delta; tc->row_norm = pack->row_norm; tc->documents = pack->documents;
     tc->q_tiles = q_tiles; tc->k_tiles = k_tiles; tc->D16 = (a.D + 15) / 16 * 16; tc->err = tensor_error_word();
+    tc->shares = shares; tc->dk_part = (float*)dk_part; tc->dv_part = (float*)dv_part;
   }
   return at;
 }
@@ -1003,6 +1037,11 @@ int attention_tc(const AttentionArgs& a, bool backward, size_t* bytes, cudaStrea
   TF_AFTER(s, what);
   TF_CUDA(with_form(a, [&](auto g, auto shaped) { return backward ? launch_bwd<decltype(g)::value, decltype(shaped)::value>(tc, s) : launch_fwd<decltype(g)::value, decltype(shaped)::value>(tc, s); }));
   TF_AFTER(s, what);
+  if (tc.shares > 1) {
+    const int64_t n = (int64_t)a.B * a.Tk * a.G * a.D;
+    TF_CUDA(launch_dep(attention_add_kernel, dim3((unsigned)grid_for(n, 256, 4), 2), dim3(256), 0, s, (const float*)tc.dk_part, (const float*)tc.dv_part, a.dk, a.dv, n, tc.shares));
+    TF_AFTER(s, what);
+  }
   return 0;
 }
 
