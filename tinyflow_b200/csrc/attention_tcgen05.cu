@@ -262,11 +262,6 @@ template <int KIND> struct Walk {
         sees_any = lo <= high && low <= hi;
         sees_whole = sees_whole && !pad && !padding && lo == hi && low == high && lo == low;
       }
-      if (sees_whole) {
-        const int64_t at = kRowsAreKeys ? ((int64_t)b * a.H + head) * tiles + t : ((int64_t)b * a.G + head / a.group) * tiles + t;
-        const uint4 u = *reinterpret_cast<const uint4*>((kRowsAreKeys ? p.q : p.k).info[at].bad), w = *reinterpret_cast<const uint4*>((kRowsAreKeys ? p.d : p.v).info[at].bad);
-        sees_whole = (u.x | u.y | u.z | u.w | w.x | w.y | w.z | w.w) == 0u;
-      }
     }
     any = __ballot_sync(0xffffffffu, sees_any);
     whole = __ballot_sync(0xffffffffu, sees_whole);
@@ -314,7 +309,7 @@ template <int KIND, int G> struct Shape {
 // Of one tile of columns, for the warps: written by the copying warp, which walks the list.  Eight of them in turn: by the time a copy for tile n + 8 can be issued,
 // the weights of tile n + 4 have been made.
 struct __align__(16) Entry {
-  int flags, head, col, at;                      // 1: there is a tile, 2: every row sees all of it; position of its first column; its number, or behind the last how many there were
+  int flags, head, col, at;                      // 1: there is a tile, 2: every row sees all of it, and all of it is finite; position of its first column; its number, or behind the last how many there were
   float inv1, inv2, x, y;                        // 1 / scale of both operands; dq: largest magnitude of V, dk: largest norm and |D'| of dO'
 };
 
@@ -463,13 +458,15 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     }
     Walk<KIND> walk(p, b, row_head, share, tile);
     // What an entry says is asked for a tile ahead
-    struct Next { bool there, all; int head, t; int64_t at; float inv1, inv2, x, y; };
+    struct Next { bool there, all; int head, t; int64_t at; float inv1, inv2, x, y; uint32_t spoils; };
     const auto look_ahead = [&] {
       Next x;
       x.there = walk.next(lane, x.head, x.t, x.all);
       x.at = x.there ? col_at(x.head, x.t) : 0;
       const TileInfo &i1 = c1.info[x.at], &i2 = c2.info[x.at];
       x.inv1 = i1.inv; x.inv2 = i2.inv; x.x = KIND == kDq ? i2.top : i2.norm; x.y = i2.delta;
+      const uint4 u = *reinterpret_cast<const uint4*>(i1.bad), w = *reinterpret_cast<const uint4*>(i2.bad);
+      x.spoils = u.x | u.y | u.z | u.w | w.x | w.y | w.z | w.w;
       return x;
     };
     const auto load = [&](const Packed& from, int64_t at) {
@@ -493,7 +490,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     for (int n = 0;; ++n) {
       const Next now = next;
       if (lane == 0) {
-        entries[n & 7] = Entry{now.there ? 1 | (int)now.all << 1 : 0, now.head, now.t * kTile + (kRowsAreKeys ? a.Tk - a.Tq : 0), now.there ? (int)now.at : n, now.inv1, now.inv2, now.x, now.y};
+        entries[n & 7] = Entry{now.there ? 1 | (int)(now.all && now.spoils == 0u) << 1 : 0, now.head, now.t * kTile + (kRowsAreKeys ? a.Tk - a.Tq : 0), now.there ? (int)now.at : n, now.inv1, now.inv2, now.x, now.y};
         mbar_arrive(entry_full + (n & 7));
       }
       __syncwarp();
@@ -730,14 +727,21 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
         }
       };
       // hides the columns of a chunk that the row does not see, and makes NaN of those that are not finite
+      float theirs[S::kChunks];                  // a column's document in every lane, asked for while the scores are being made
+      if (p.documents && masked) {
+#pragma unroll
+        for (int c = 0; c < S::kChunks; ++c) theirs[c] = document_of(a, b, col0 + 32 * c + lane);
+      }
       const auto mask32 = [&](float* z, int c, float hidden) {
         const int first = col0 + 32 * c;
         uint32_t seen = bits_between(lo - first, hi - first) | bits_between(-1, extra - 1 - first);
         if (p.documents) {
           uint32_t same = 0u;
-          const float theirs = document_of(a, b, first + lane);
+          float of = theirs[0];
 #pragma unroll
-          for (int k = 0; k < 32; ++k) same |= __shfl_sync(0xffffffffu, theirs, k) == document ? 1u << k : 0u;
+          for (int i = 1; i < S::kChunks; ++i) of = c == i ? theirs[i] : of;
+#pragma unroll
+          for (int k = 0; k < 32; ++k) same |= __shfl_sync(0xffffffffu, of, k) == document ? 1u << k : 0u;
           seen &= document >= 0.f ? same : 0u;
         }
         const uint32_t spoils = seen & (spoiled ? 0xffffffffu : c1.info[now.at].bad[col_part / 32 + c] | c2.info[now.at].bad[col_part / 32 + c]);
@@ -890,17 +894,34 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
 #pragma unroll
       for (int k = 0; k < kSums; ++k) acc[k] *= last;
     }
-    if (there && !*abort_flag && !(kTurns && group == 1)) {
+    if (!(kTurns && group == 1) && !*abort_flag) {
+      // A warp turns its rows around in the ring, which nothing else uses any more, so that it stores whole lines: rows are 4 floats apart from each other's banks.
+      constexpr int kPitch = 64 * G + 4;
+      static_assert((kTurns ? kSums * kTile * 4 : 0) + kTile * kPitch * 4 <= kStages * kPart, "rows fit the ring");
+      float* const turned = reinterpret_cast<float*>(ring) + (kTurns ? kSums * kTile : 0) + quarter * 32 * kPitch + sum_part;
+#pragma unroll
+      for (int k = 0; k < kSums; k += 4) *reinterpret_cast<float4*>(turned + lane * kPitch + k) = make_float4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]);
+      __syncwarp();
       float* result = KIND == kFwd ? a.o : KIND == kDq ? a.dq : KIND == kDk ? a.dk : a.dv;
       if (shares > 1) result = (KIND == kDk ? p.dk_part : p.dv_part) + share * ((int64_t)a.B * a.Tk * a.G * a.D);
-      float* const to = result + (((int64_t)b * (kRowsAreKeys ? a.Tk : a.Tq) + self) * row_heads + row_head) * a.D + sum_part;
-      const int cols = a.D - sum_part;
-      if (a.D % 4 == 0 && (reinterpret_cast<uintptr_t>(result) & 15) == 0) {
-#pragma unroll
-        for (int k = 0; k < kSums; k += 4) if (k < cols) *reinterpret_cast<float4*>(to + k) = make_float4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < kSums; ++k) if (k < cols) to[k] = acc[k];
+      const int length = kRowsAreKeys ? a.Tk : a.Tq, first = tile * kTile + quarter * 32, cols = a.D - sum_part;
+      const int64_t stride = (int64_t)row_heads * a.D;
+      result += ((int64_t)b * length + first) * stride + row_head * a.D + sum_part;
+      const bool wide_rows = a.D % 4 == 0 && (reinterpret_cast<uintptr_t>(result) & 15) == 0;
+      constexpr int kAcross = kSums / 4;         // lanes of a row
+#pragma unroll 4
+      for (int i = lane; i < 32 * kAcross; i += 32) {
+        const int r = i / kAcross, k = (i - r * kAcross) * 4;
+        if (first + r >= length || k >= cols) continue;
+        const float4 v = *reinterpret_cast<const float4*>(turned + r * kPitch + k);
+        float* const to = result + r * stride + k;
+        if (wide_rows) *reinterpret_cast<float4*>(to) = v;
+        else {
+          to[0] = v.x;
+          if (k + 1 < cols) to[1] = v.y;
+          if (k + 2 < cols) to[2] = v.z;
+          if (k + 3 < cols) to[3] = v.w;
+        }
       }
     }
   }
