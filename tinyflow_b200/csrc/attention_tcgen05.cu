@@ -909,19 +909,16 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
       result += ((int64_t)b * length + first) * stride + row_head * a.D + sum_part;
       const bool wide_rows = a.D % 4 == 0 && (reinterpret_cast<uintptr_t>(result) & 15) == 0;
       constexpr int kAcross = kSums / 4;         // lanes of a row
-#pragma unroll 4
-      for (int i = lane; i < 32 * kAcross; i += 32) {
-        const int r = i / kAcross, k = (i - r * kAcross) * 4;
-        if (first + r >= length || k >= cols) continue;
-        const float4 v = *reinterpret_cast<const float4*>(turned + r * kPitch + k);
-        float* const to = result + r * stride + k;
-        if (wide_rows) *reinterpret_cast<float4*>(to) = v;
-        else {
-          to[0] = v.x;
-          if (k + 1 < cols) to[1] = v.y;
-          if (k + 2 < cols) to[2] = v.z;
-          if (k + 3 < cols) to[3] = v.w;
-        }
+      constexpr int kRowsAtOnce = 32 / kAcross > 0 ? 32 / kAcross : 1;         // rows of a store
+      const int k = lane % kAcross * 4, r0 = lane / kAcross;
+      if (wide_rows && k < cols) {
+#pragma unroll 8
+        for (int r = r0; r < 32; r += kRowsAtOnce)
+          if (first + r < length) *reinterpret_cast<float4*>(result + r * stride + k) = *reinterpret_cast<const float4*>(turned + r * kPitch + k);
+      } else if (k < cols) {
+        for (int r = r0; r < 32 && first + r < length; r += kRowsAtOnce)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) if (k + i < cols) result[r * stride + k + i] = turned[r * kPitch + k + i];
       }
     }
   }
