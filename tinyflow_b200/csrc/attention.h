@@ -28,6 +28,28 @@ constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float reciprocal(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
+// Two numbers an instruction, rounded as each alone would be
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ unsigned long long pair_of(float2 v) { unsigned long long p; asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(v.x), "f"(v.y)); return p; }
+__device__ __forceinline__ float2 of_pair(unsigned long long p) { float2 v; asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(p)); return v; }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(pair_of(a)), "l"(pair_of(b)), "l"(pair_of(c)));
+  return of_pair(d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_of(a)), "l"(pair_of(b)));
+  return of_pair(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_of(a)), "l"(pair_of(b)));
+  return of_pair(d);
+}
+__device__ __forceinline__ float2 at2(const float* v, int k) { return make_float2(v[k], v[k + 1]); }
+__device__ __forceinline__ void put2(float* v, int k, float2 x) { v[k] = x.x; v[k + 1] = x.y; }
+
 // The keys of a query at position `at`: those of [lo, hi] and those before `prefix`, if of its document.
 struct Sight { int lo, hi; };
 __device__ __forceinline__ Sight sight_of(const AttentionArgs& a, int at) {

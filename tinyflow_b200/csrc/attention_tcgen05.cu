@@ -327,24 +327,28 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_low, u
                ::"r"(d), "r"(a), "l"((uint64_t)b_low | (uint64_t)b_high << 32), "r"(idesc), "r"(keep) : "memory");
 }
 
-// cap * tanh(x / cap) of 32 numbers, t = the tanh.  Up to 0.35 by the series of odd powers (x^13 behind it is 4e-9 of x there), whose error is relative; above by
-// 1 - 2 / (e^2x + 1), whose error is a rounding of 1.  Scores far below the cap, most of all, take the series alone.
+// tanh of 32 numbers.  Up to 0.35 by the series of odd powers (x^13 behind it is 1.2e-8 of x there), whose error is relative; above by 1 - 2 / (e^2x + 1), whose error
+// is a rounding of 1.  Scores far below the cap, most of all, take the series alone, and below 0.15 only its first terms (x^9 behind them is 6e-9 of x).
 __device__ __forceinline__ void tanh32(float* t) {
   float most = 0.f;
 #pragma unroll
   for (int k = 0; k < 32; ++k) most = fmaxf(most, fabsf(t[k]));
-  const bool large = __any_sync(0xffffffffu, !(most < 0.35f));
+  const bool small = __all_sync(0xffffffffu, most < 0.15f), large = __any_sync(0xffffffffu, !(most < 0.35f));
 #pragma unroll
-  for (int k = 0; k < 32; ++k) {
-    const float x = t[k], s = x * x;
-    float y = -1382.f / 155925.f;
-    y = fmaf(y, s, 62.f / 2835.f); y = fmaf(y, s, -17.f / 315.f); y = fmaf(y, s, 2.f / 15.f); y = fmaf(y, s, -1.f / 3.f);
-    y = fmaf(y * s, x, x);
-    if (large) {
-      const float far = 1.f - 2.f * reciprocal(exp2_fast(2.f * kLog2e * fabsf(x)) + 1.f);
-      y = fabsf(x) < 0.35f ? y : copysignf(far, x);
+  for (int k = 0; k < 32; k += 2) {
+    const float2 x = at2(t, k), s = mul2(x, x);
+    float2 y = both(-17.f / 315.f);
+    if (!small) y = fma2(fma2(both(-1382.f / 155925.f), s, both(62.f / 2835.f)), s, y);
+    y = fma2(fma2(y, s, both(2.f / 15.f)), s, both(-1.f / 3.f));
+    y = fma2(mul2(y, s), x, x);
+    if (__builtin_expect(large, 0)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float v = i ? x.y : x.x, far = 1.f - 2.f * reciprocal(exp2_fast(2.f * kLog2e * fabsf(v)) + 1.f);
+        if (!(fabsf(v) < 0.35f)) (i ? y.y : y.x) = copysignf(far, v);
+      }
     }
-    t[k] = y;
+    put2(t, k, y);
   }
 }
 // hi and lo halves of 32 weights, as the A operand has them: 16 weights are 8 words of hi and 8 of lo
@@ -353,8 +357,9 @@ __device__ __forceinline__ void split32(const float* w, uint32_t* words) {
   for (int k = 0; k < 16; ++k) {
     // the upper 11 bits, which fp16 holds exactly down to 2^-14; below, the rounding is 2^-25 of weights that reach 2^14
     const float a = __uint_as_float(__float_as_uint(w[2 * k]) & 0xffffe000u), b = __uint_as_float(__float_as_uint(w[2 * k + 1]) & 0xffffe000u);
+    const float2 rest = add2(at2(w, 2 * k), make_float2(-a, -b));
     words[(k >> 3) * 16 + (k & 7)] = halves(a, b);
-    words[(k >> 3) * 16 + 8 + (k & 7)] = halves(w[2 * k] - a, w[2 * k + 1] - b);
+    words[(k >> 3) * 16 + 8 + (k & 7)] = halves(rest.x, rest.y);
   }
 }
 __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {               // bits lo .. hi of a word, as far as it has them
@@ -685,9 +690,10 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
         tmem_ld_wait();
         if (c == kSums / 32 - 1) arrive(&o_empty[n & 1]);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) {
-          if (KIND == kFwd) acc[32 * c + k] *= alpha;
-          acc[32 * c + k] = fmaf(o[k], out_factor, acc[32 * c + k]);
+        for (int k = 0; k < 32; k += 2) {
+          float2 x = at2(acc, 32 * c + k);
+          if (KIND == kFwd) x = mul2(x, both(alpha));
+          put2(acc, 32 * c + k, fma2(at2(o, k), both(out_factor), x));
         }
       }
     };
@@ -711,11 +717,15 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
       // scores of a chunk of 32 columns, capped and biased, in units of log 2; turned: 1 - the cap's tanh squared
       const auto shape32 = [&](float* z, float* turned, int c) {
 #pragma unroll
-        for (int k = 0; k < 32; ++k) z[k] *= f;
+        for (int k = 0; k < 32; k += 2) put2(z, k, mul2(at2(z, k), both(f)));
         if (cap) {
           tanh32(z);
 #pragma unroll
-          for (int k = 0; k < 32; ++k) { if (turned) turned[k] = fmaf(-z[k], z[k], 1.f); z[k] *= wide; }
+          for (int k = 0; k < 32; k += 2) {
+            const float2 t = at2(z, k);
+            if (turned) put2(turned, k, fma2(mul2(t, both(-1.f)), t, both(1.f)));
+            put2(z, k, mul2(t, both(wide)));
+          }
         } else if (turned) {
 #pragma unroll
           for (int k = 0; k < 32; ++k) turned[k] = 1.f;
@@ -780,7 +790,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
         const float at_most = fmaxf(most, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * g), base = max_of_finite_or(at_most);
         const float shifted = base - (float)kWeightExp, faded = exp2_fast(most - base);
         most = at_most;
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        float2 s[2] = {both(0.f), both(0.f)};
 #pragma unroll 1
         for (int c = 0; c < S::kChunks; ++c) {
           float z[32];
@@ -788,13 +798,17 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
           tmem_ld32(from + 32 * c, z);
           tmem_ld_wait();
 #pragma unroll
-          for (int k = 0; k < 32; ++k) { z[k] = exp2_fast(fmaf(z[k], g, -shifted)); s[k & 3] += z[k]; }
+          for (int k = 0; k < 32; k += 2) {
+            const float2 e = fma2(at2(z, k), both(g), both(-shifted)), w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+            s[(k >> 1) & 1] = add2(s[(k >> 1) & 1], w);
+            put2(z, k, w);
+          }
           split32(z, words);
           tmem_st32(from + 32 * c, words);
         }
         tmem_st_wait();
         arrive(&w_full[n & 1]);
-        sum = fmaf(sum, faded, (s[0] + s[1]) + (s[2] + s[3]));
+        sum = fmaf(sum, faded, (s[0].x + s[0].y) + (s[1].x + s[1].y));
         alpha = faded;
         out_factor = now.inv2;
       } else {
@@ -824,21 +838,24 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
 #pragma unroll
             for (int k = 0; k < 32; k += 4) {
               const float4 m4 = *reinterpret_cast<const float4*>(col_max + 32 * c + k);
-              z[k] = fmaf(z[k], g, kk - m4.x); z[k + 1] = fmaf(z[k + 1], g, kk - m4.y); z[k + 2] = fmaf(z[k + 2], g, kk - m4.z); z[k + 3] = fmaf(z[k + 3], g, kk - m4.w);
+              put2(z, k, fma2(at2(z, k), both(g), make_float2(kk - m4.x, kk - m4.y)));
+              put2(z, k + 2, fma2(at2(z, k + 2), both(g), make_float2(kk - m4.z, kk - m4.w)));
               if (KIND == kDk) {
                 const float4 d4 = *reinterpret_cast<const float4*>(col_delta + 32 * c + k);
-                y[k] = fmaf(y[k], fy, -d4.x); y[k + 1] = fmaf(y[k + 1], fy, -d4.y); y[k + 2] = fmaf(y[k + 2], fy, -d4.z); y[k + 3] = fmaf(y[k + 3], fy, -d4.w);
+                put2(y, k, fma2(at2(y, k), both(fy), make_float2(-d4.x, -d4.y)));
+                put2(y, k + 2, fma2(at2(y, k + 2), both(fy), make_float2(-d4.z, -d4.w)));
               }
             }
           } else {
             const float less = kk - row_max;
 #pragma unroll
-            for (int k = 0; k < 32; ++k) { z[k] = fmaf(z[k], g, less); y[k] = fmaf(y[k], fy, -row_delta); }
+            for (int k = 0; k < 32; k += 2) { put2(z, k, fma2(at2(z, k), both(g), both(less))); put2(y, k, fma2(at2(y, k), both(fy), both(-row_delta))); }
           }
 #pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            z[k] = exp2_fast(z[k]);
-            if (kTwo) z[k] *= SHAPED ? y[k] * turned[k] : y[k];
+          for (int k = 0; k < 32; k += 2) {
+            float2 w = make_float2(exp2_fast(z[k]), exp2_fast(z[k + 1]));
+            if (kTwo) w = mul2(w, SHAPED ? mul2(at2(y, k), at2(turned, k)) : at2(y, k));
+            put2(z, k, w);
           }
           if (__builtin_expect(masked, 0)) mask32(z, c, 0.f);
           uint32_t words[32];
