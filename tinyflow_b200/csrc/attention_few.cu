@@ -46,7 +46,6 @@ template <int kLanes, int N> __device__ __forceinline__ float over_lanes(float* 
 
 // A part: sums [rows][D], then the rows' maxima and the sums of their weights
 __host__ __device__ constexpr int part_floats(int rows, int D) { return (rows * (D + 2) + 3) / 4 * 4; }
-template <int VEC> __device__ __forceinline__ void get_beyond_l1(float* v, const float* p) { *reinterpret_cast<typename Pieces<VEC>::T*>(v) = __ldcg(reinterpret_cast<const typename Pieces<VEC>::T*>(p)); }
 
 template <int kLanes, int DL, int ROWS, int VEC, bool SHAPED>
 __global__ void __launch_bounds__(kThreads, kBlocks) attention_few_kernel(const __grid_constant__ FewArgs p) {

@@ -76,15 +76,19 @@ template <int VEC> __device__ __forceinline__ void place(const RotaryArgs& p, in
   else if (p.interleaved) { a = 2 * VEC * c; b = a + VEC; }
   else { a = VEC * c; b = p.pairs + VEC * c; }
 }
+__device__ __forceinline__ void turn_pair(float2 t, float s, float& a, float& b) {
+  const float x = a * t.x - b * s;
+  b = a * s + b * t.x;
+  a = x;
+}
 // v: 2 VEC elements; cs: cosines and sines of the chunk's VEC pairs
 template <int VEC> __device__ __forceinline__ void rotate(const RotaryArgs& p, const float2* __restrict__ cs, float* v, bool back) {
+  if (p.interleaved) {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    const float2 t = cs[i];
-    const float s = back ? -t.y : t.y;
-    float a = p.interleaved ? v[2 * i] : v[i], b = p.interleaved ? v[2 * i + 1] : v[VEC + i];
-    const float x = a * t.x - b * s, y = a * s + b * t.x;
-    if (p.interleaved) { v[2 * i] = x; v[2 * i + 1] = y; } else { v[i] = x; v[VEC + i] = y; }
+    for (int i = 0; i < VEC; ++i) { const float2 t = cs[i]; turn_pair(t, back ? -t.y : t.y, v[2 * i], v[2 * i + 1]); }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) { const float2 t = cs[i]; turn_pair(t, back ? -t.y : t.y, v[i], v[VEC + i]); }
   }
 }
 template <int VEC> __device__ __forceinline__ void load_chunk(const RotaryArgs& p, const float* __restrict__ row, int c, float* v) {
@@ -185,7 +189,8 @@ template <int VEC, int L, int N, int U>
 __global__ void __launch_bounds__(kThreads) head_norm_bwd_kernel(const __grid_constant__ RotaryArgs p, const __grid_constant__ Quarters f) {
   extern __shared__ __align__(16) float2 cs[];
   __shared__ bool last;
-  constexpr int kGroups = kThreads / L;
+  __shared__ unsigned short token_of[U * kThreads / L];
+  constexpr int kGroups = kThreads / L, kPart = VEC == 4 ? 4 : 1;
   grid_dep_sync();
   const int which = (int)blockIdx.x >= p.blocks[0], block = (int)blockIdx.x - (which ? p.blocks[0] : 0), blocks = p.blocks[which];
   const HeadArgs& h = p.h[which];
@@ -212,14 +217,14 @@ __global__ void __launch_bounds__(kThreads) head_norm_bwd_kernel(const __grid_co
           for (int j = 0; j < 2 * VEC; ++j) x[u][n][j] = d[u][n][j] = 0.f;
     }
     __syncthreads();                             // the pass before is done with the angles
+    if (threadIdx.x < U * kGroups) token_of[threadIdx.x] = (unsigned short)(((unsigned)r0 % (unsigned)h.heads + threadIdx.x) / (unsigned)h.heads);
     make_turns(p, f, cs, r0, r1, h.heads);
     __syncthreads();
-    const unsigned in_token = (unsigned)r0 % (unsigned)h.heads;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t r = r0 + u * kGroups + group;
       const bool there = r < r1;
-      const unsigned token = there ? (in_token + (unsigned)(u * kGroups + group)) / (unsigned)h.heads : 0u;
+      const unsigned token = token_of[u * kGroups + group];
       float ss = 0.f;
 #pragma unroll
       for (int n = 0; n < N; ++n) {
@@ -281,17 +286,24 @@ __global__ void __launch_bounds__(kThreads) head_norm_bwd_kernel(const __grid_co
   __syncthreads();
   if (!last) return;
   __threadfence();
-  const int ways = kThreads / p.D > 0 ? kThreads / p.D : 1, way = threadIdx.x / p.D, e = threadIdx.x - way * p.D;      // D <= kThreads
+  const int wide = p.D / kPart, ways = kThreads / wide, way = threadIdx.x / wide, e = (threadIdx.x - way * wide) * kPart;      // D <= kThreads
   if (way < ways) {
-    float s = 0.f;
+    float sum[kPart] = {};
     for (int b = way; b < blocks; b += 8 * ways) {             // eight loads in flight
-      float w[8];
+      float w[8][kPart];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = b + i * ways < blocks ? __ldcg(h.part + (int64_t)(b + i * ways) * p.D + e) : 0.f;
+      for (int i = 0; i < 8; ++i)
+        if (b + i * ways < blocks) get_beyond_l1<kPart>(w[i], h.part + (int64_t)(b + i * ways) * p.D + e);
+        else
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s += w[i];
+          for (int j = 0; j < kPart; ++j) w[i][j] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < kPart; ++j) sum[j] += w[i][j];
     }
-    held[way * p.D + e] = s;
+#pragma unroll
+    for (int j = 0; j < kPart; ++j) held[way * p.D + e + j] = sum[j];
   }
   __syncthreads();
   for (int c = threadIdx.x; c < p.D; c += kThreads) {
