@@ -22,6 +22,7 @@ namespace tf {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kNormBlocks = 4;       // blocks of the norm's gradients that an SM holds
 constexpr int kMostPairs = 128, kMostDim = 2 * kMostPairs;
 
 struct RotaryState {
@@ -186,7 +187,7 @@ __global__ void __launch_bounds__(kThreads) heads_kernel(const __grid_constant__
 // Gradients of the norm and the rotation.  A block works through every gridDim-th pass of its array, adds up dgamma in registers, then over
 // its groups of threads and, in the block that comes last, over the blocks: always in the same order, in one launch.
 template <int VEC, int L, int N, int U>
-__global__ void __launch_bounds__(kThreads) head_norm_bwd_kernel(const __grid_constant__ RotaryArgs p, const __grid_constant__ Quarters f) {
+__global__ void __launch_bounds__(kThreads, kNormBlocks) head_norm_bwd_kernel(const __grid_constant__ RotaryArgs p, const __grid_constant__ Quarters f) {
   extern __shared__ __align__(16) float2 cs[];
   __shared__ bool last;
   __shared__ unsigned short token_of[U * kThreads / L];
@@ -493,8 +494,9 @@ int TfHeadNormRotaryBackward(const DLArrayHandle query, const DLArrayHandle key,
   const int64_t rows = a.h[0].rows + a.h[1].rows;
   if (rows == 0) return 0;
   StreamLease lease(s);
-  // Three blocks an SM, as many as its registers take: 114 us at 16384 tokens x (16 + 4) heads of 128, with two 160
-  const int64_t most = 3 * device_sm_count();
+  // Four blocks an SM with one head a thread group and pass: 94 us at 16384 tokens x (16 + 4) heads of 128, 5.3 TB/s.  More in flight is slower, reads and writes
+  // get in one another's way: three or four blocks of two heads 98 and 115, five of one 106, the next pass asked for in advance 115.
+  const int64_t most = kNormBlocks * device_sm_count();
   const size_t bytes = sizeof(float) * (size_t)(most + 1) * a.D;
   float* const part = (float*)lease.scratch(kScratchNorm, bytes);
   uint32_t* const count = part ? lease.counters(2) : nullptr;
@@ -504,7 +506,7 @@ int TfHeadNormRotaryBackward(const DLArrayHandle query, const DLArrayHandle key,
   KernelTimer kt(what, s, 0, 12.0 * rows * a.D);
   cudaError_t e = cudaSuccess;
   with_shape(a.D, a.pairs, bits, [&](auto vec, auto l, auto n) {
-    constexpr int VEC = decltype(vec)::value, L = decltype(l)::value, N = decltype(n)::value, U = 2;
+    constexpr int VEC = decltype(vec)::value, L = decltype(l)::value, N = decltype(n)::value, U = 1;
     a.chunks = (a.D + 2 * VEC - 1) / (2 * VEC);
     a.per_block = pass_of(kThreads / L, U, rows);
     int64_t passes[2], all = 0;
