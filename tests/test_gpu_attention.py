@@ -255,6 +255,40 @@ def test_what_is_not_finite_reaches_what_depends_on_it_and_nothing_else(env, pat
         assert np.array_equal(g, w), name
 
 
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+@pytest.mark.parametrize("where", ["q", "k", "v"])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_what_is_not_finite_reaches_the_answers_that_depend_on_it(env, where, bad, cap):
+    """A score of minus infinity has no weight, and a cap makes it finite: the answer is not finite all the same."""
+    c = Case(2, 2, 90, 4, 2, 24, window=60, cap=cap)
+    clean, = run(env, c, backward=False)
+    array = getattr(c, where)
+    token, head = (3, 1) if where == "q" else (90 + 29, 1)   # of the second sequence: its last query; a key that its first query sees and its last does not
+    array[token, head * c.dim + 3] = bad
+    got, = run(env, c, backward=False)
+    touched = [(3, 1)] if where == "q" else [(2, 2), (2, 3)]
+    got, clean = got.reshape(4, 4, c.dim), clean.reshape(4, 4, c.dim)
+    for at in touched:
+        assert not np.isfinite(got[at]).all(), at
+        got[at] = clean[at]
+    assert np.array_equal(got, clean)
+
+
+@pytest.mark.parametrize("queries, path", [(2, 1), (17, 1), (17, 2)])
+def test_more_sequences_than_a_grid_has_rows(env, queries, path):
+    c = Case(70001, queries, queries, 1, 1, 4)
+    env.gpu_op.set_contraction_path(path)
+    got = run(env, c)
+    env.gpu_op.set_contraction_path(0)
+    some = [0, 65534, 65535, 65536, 70000]
+    few = Case(len(some), queries, queries, 1, 1, 4)
+    take = lambda a: a.reshape(c.batch, queries, 4)[some].reshape(-1, 4)      # noqa: E731
+    few.q, few.k, few.v, few.dout = (take(a) for a in (c.q, c.k, c.v, c.dout))
+    want, bound = few.bounds()
+    for name, g, w, e in zip(("out", "dq", "dk", "dv"), got, want, bound):
+        within(take(g), w, e, name)
+
+
 def test_unseen_keys_may_hold_anything(env, path):
     """Keys behind the last query's sight, of other documents and padding: NaN there changes no bit of the exact kernels' results.  On the tensor path a finite value there has
     a part in its tile's scale, a power of two, and NaN has none: values that were representable in 22 bits below 2^14 are so below 2^15, and the roundings are others of the same

@@ -132,6 +132,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) attention_few_kernel(const 
         dots[r * kUnroll + u] = dot.x + dot.y;
       }
     float s = over_lanes<kLanes, kScores>(dots) * scale;
+    if (!(fabsf(s) < INFINITY)) s = NAN;         // a cap or a weight of zero would hide what is not finite
     const int j = j0 + my_u * kAtOnce + sub;
     if (SHAPED) {
       if (a.cap > 0.f) s = a.cap * tanhf(s / a.cap);

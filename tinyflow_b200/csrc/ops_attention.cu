@@ -177,14 +177,14 @@ template <int DP> struct TileSmem {
 
 // Latency-bound at the sizes that take it.
 template <int DP, bool WIDE>
-__global__ void __launch_bounds__(kThreads) attention_tile_fwd_kernel(const __grid_constant__ AttentionArgs a) {
+__global__ void __launch_bounds__(kThreads) attention_tile_fwd_kernel(const __grid_constant__ AttentionArgs a, int row_blocks) {
   extern __shared__ __align__(16) char raw[];
   TileSmem<DP>& sm = *reinterpret_cast<TileSmem<DP>*>(raw);
   grid_dep_sync();
-  const int b = blockIdx.y / a.G, kv = blockIdx.y - b * a.G;
+  const int bg = blockIdx.x / row_blocks, block = blockIdx.x - bg * row_blocks, b = bg / a.G, kv = bg - b * a.G;
   const Rows rows{a, b, kv};
   const Keys keys{a, b, kv};
-  const int count = a.group * a.Tq, first = (gridDim.x - 1 - blockIdx.x) * kRows;       // the rows that see most go first
+  const int count = a.group * a.Tq, first = (row_blocks - 1 - block) * kRows;       // the rows that see most go first
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int prefix = prefix_of(a, b);
   RowSight rs[2];
@@ -253,13 +253,13 @@ __global__ void __launch_bounds__(kThreads) attention_tile_fwd_kernel(const __gr
   store_rows<DP>(a.o, rows, first, count, a.D, ty, tx, acc);
 }
 
-// The first blocks of x make dq of their rows, the others dk and dv of their keys.
+// Of a key-value head's blocks the first make dq of their rows, the others dk and dv of their keys.
 template <int DP, bool WIDE>
-__global__ void __launch_bounds__(kThreads) attention_tile_bwd_kernel(const __grid_constant__ AttentionArgs a, int row_blocks) {
+__global__ void __launch_bounds__(kThreads) attention_tile_bwd_kernel(const __grid_constant__ AttentionArgs a, int row_blocks, int blocks) {
   extern __shared__ __align__(16) char raw[];
   TileSmem<DP>& sm = *reinterpret_cast<TileSmem<DP>*>(raw);
   grid_dep_sync();
-  const int b = blockIdx.y / a.G, kv = blockIdx.y - b * a.G;
+  const int bg = blockIdx.x / blocks, block = blockIdx.x - bg * blocks, b = bg / a.G, kv = bg - b * a.G;
   const Rows rows{a, b, kv};
   const Keys keys{a, b, kv};
   const int count = a.group * a.Tq;
@@ -278,8 +278,8 @@ __global__ void __launch_bounds__(kThreads) attention_tile_bwd_kernel(const __gr
     for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
     return d;
   };
-  if ((int)blockIdx.x < row_blocks) {
-    const int first = (row_blocks - 1 - (int)blockIdx.x) * kRows;
+  if (block < row_blocks) {
+    const int first = (row_blocks - 1 - block) * kRows;
     RowSight rs[2];
     float most[2], inv[2];
 #pragma unroll
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kThreads) attention_tile_bwd_kernel(const __gr
     if (a.dq) store_rows<DP>(a.dq, rows, first, count, a.D, ty, tx, one);
     return;
   }
-  const int first = ((int)blockIdx.x - row_blocks) * kRows;
+  const int first = (block - row_blocks) * kRows;
   load_rows<DP, kRows, WIDE>(sm.A[0], a.k, keys, first, a.Tk, a.D, nullptr);
   load_rows<DP, kRows, WIDE>(sm.A[1], a.v, keys, first, a.Tk, a.D, nullptr);
   float document[2];
@@ -398,8 +398,8 @@ cudaError_t tile_fwd(const AttentionArgs& a, cudaStream_t s) {
       const auto kernel = attention_tile_fwd_kernel<DP, decltype(w)::value>;
       const int bytes = (int)sizeof(TileSmem<DP>);
       e = once_per_device(ready, [kernel, bytes] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
-      const int64_t count = (int64_t)a.group * a.Tq;
-      if (e == cudaSuccess) e = launch_dep(kernel, dim3((unsigned)((count + kRows - 1) / kRows), (unsigned)(a.B * a.G)), dim3(kThreads), (size_t)bytes, s, a);
+      const int row_blocks = (int)(((int64_t)a.group * a.Tq + kRows - 1) / kRows);
+      if (e == cudaSuccess) e = launch_dep(kernel, dim3((unsigned)(row_blocks * a.B * a.G)), dim3(kThreads), (size_t)bytes, s, a, row_blocks);
     };
     if (wide(a)) run(std::true_type()); else run(std::false_type());
   });
@@ -415,7 +415,7 @@ cudaError_t tile_bwd(const AttentionArgs& a, cudaStream_t s) {
       const int bytes = (int)sizeof(TileSmem<DP>);
       e = once_per_device(ready, [kernel, bytes] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
       const int row_blocks = a.dq ? (int)(((int64_t)a.group * a.Tq + kRows - 1) / kRows) : 0, key_blocks = a.dk || a.dv ? (a.Tk + kRows - 1) / kRows : 0;
-      if (e == cudaSuccess && row_blocks + key_blocks) e = launch_dep(kernel, dim3((unsigned)(row_blocks + key_blocks), (unsigned)(a.B * a.G)), dim3(kThreads), (size_t)bytes, s, a, row_blocks);
+      if (e == cudaSuccess && row_blocks + key_blocks) e = launch_dep(kernel, dim3((unsigned)((row_blocks + key_blocks) * a.B * a.G)), dim3(kThreads), (size_t)bytes, s, a, row_blocks, row_blocks + key_blocks);
     };
     if (wide(a)) run(std::true_type()); else run(std::false_type());
   });
@@ -434,7 +434,7 @@ int check_attention(const char* what, const AttentionState* st, const DLArray* q
   TF_REQUIRE(B > 0 ? k->shape[0] >= 0 && k->shape[0] % B == 0 : k->shape[0] == 0, "%s: the keys are not those of %lld sequences", what, (long long)B);
   const int64_t Tk = B ? k->shape[0] / B : 0;
   TF_REQUIRE(st->length <= (1 << 24) && Tk <= (1 << 24) && st->length * (st->heads / st->kv_heads) <= (1ll << 28), "%s: sequences are too long", what);
-  TF_REQUIRE(B * st->heads <= 65535, "%s: more than 65535 sequences x heads", what);
+  TF_REQUIRE(B * (st->heads * (st->length / kRows + 1) + st->kv_heads * (Tk / kRows + 1)) < (1ll << 31), "%s: more blocks than a launch has", what);
   TF_REQUIRE(!documents || Tk >= st->length, "%s: documents need a key for every query", what);
   memset(a, 0, sizeof(*a));
   a->B = (int)B; a->H = st->heads; a->G = st->kv_heads; a->group = st->heads / st->kv_heads; a->Tq = (int)st->length; a->Tk = (int)Tk; a->D = (int)D;
