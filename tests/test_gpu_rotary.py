@@ -3,7 +3,7 @@
 Tolerances count roundings, u = 2^-24 each: an angle reduced to an eighth of a turn is rounded by u / 2 of less than 1, its sine and cosine by
 2 u, the amplitude's product by u, and a rotated value is two products and a sum of those: 8 u A (|a| + |b|).  A head's sum of squares has chains of 8
 elements in a thread and 5 of shuffles, its root and reciprocal 2 u: 20 u of the normed value.  dgamma is added up over at most tokens x heads / 100 +
-200 terms in a row (every third of an SM's share, 16 groups of a block, the blocks)."""
+200 terms in a row (every fourth of an SM's share, up to 64 groups of a block, eights of the blocks and up to 32 sums of those)."""
 import ctypes
 
 import numpy as np

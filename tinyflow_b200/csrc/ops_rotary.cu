@@ -287,10 +287,11 @@ __global__ void __launch_bounds__(kThreads, kNormBlocks) head_norm_bwd_kernel(co
   __syncthreads();
   if (!last) return;
   __threadfence();
-  const int wide = p.D / kPart, ways = kThreads / wide, way = threadIdx.x / wide, e = (threadIdx.x - way * wide) * kPart;      // D <= kThreads
+  // Eight loads in flight, added as a tree: chains of blocks / (8 ways) sums, then the ways'
+  const int wide = p.D / kPart, ways = min(kThreads / wide, 32), way = threadIdx.x / wide, e = (threadIdx.x - way * wide) * kPart;      // D <= kThreads
   if (way < ways) {
     float sum[kPart] = {};
-    for (int b = way; b < blocks; b += 8 * ways) {             // eight loads in flight
+    for (int b = way; b < blocks; b += 8 * ways) {
       float w[8][kPart];
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -299,9 +300,7 @@ __global__ void __launch_bounds__(kThreads, kNormBlocks) head_norm_bwd_kernel(co
 #pragma unroll
           for (int j = 0; j < kPart; ++j) w[i][j] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int j = 0; j < kPart; ++j) sum[j] += w[i][j];
+      for (int j = 0; j < kPart; ++j) sum[j] += ((w[0][j] + w[1][j]) + (w[2][j] + w[3][j])) + ((w[4][j] + w[5][j]) + (w[6][j] + w[7][j]));
     }
 #pragma unroll
     for (int j = 0; j < kPart; ++j) held[way * p.D + e + j] = sum[j];
