@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 
 from oracle import ops
-from tests.test_gpu_norm import place, read, within
+from tests.test_gpu_norm import place, read, view, within
 from tests.test_gpu_ops import env  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -200,3 +200,29 @@ def test_products_take_the_maxima_that_these_kernels_leave(env):
             assert np.array_equal(z.asnumpy(), noted[at])
     finally:
         op.set_contraction_path(0)
+
+
+@pytest.mark.parametrize("offset", [5, 64])
+def test_part_of_a_block_that_was_freed(env, offset):
+    """What is known of an array that was a part of another goes with that: the next array there has other magnitudes."""
+    M, K, N = 1300, 768, 256
+    rng = np.random.RandomState(0)
+
+    def part(value):
+        whole = np.zeros(M * K + 128, np.float32)
+        whole[offset:offset + M * K] = value.ravel()
+        return view(env, env.nd.array(whole, env.ctx), offset, (M, K))
+    env.gpu_op.set_contraction_path(2)
+    small = part((2.0 ** -90 * rng.randn(M, K)).astype(np.float32))
+    out = part(np.zeros((M, K), np.float32))
+    env.gpu_op.rotary_forward(small, None, out, M, 0, env.gpu_op.rotary_state(64), env.stream)
+    env.gpu_op.device_synchronize()
+    at = out.data_ptr
+    del out
+    a, b = rng.randn(M, K).astype(np.float32), rng.randn(K, N).astype(np.float32)
+    A, B, C = part(a), env.nd.array(b, env.ctx), env.nd.empty((M, N), env.ctx)
+    assert A.data_ptr == at                      # the block is used again
+    env.gpu_op.matrix_multiply(A, False, B, False, C, env.cublas, env.stream)
+    env.gpu_op.set_contraction_path(0)
+    want, magnitude = a.astype(np.float64) @ b.astype(np.float64), np.abs(a).astype(np.float64) @ np.abs(b).astype(np.float64)
+    within(C.asnumpy(), want, (4 + 3 * K / 8) * U * magnitude, "product")

@@ -102,7 +102,8 @@ cudaStream_t last_compute_stream();         // launches a held-back kernel first
 // derived data (packed tensor-core operands) is valid only while the version is unchanged.  Inside a caller's capture, and for an array that a
 // captured call has written, version_of() is another number at every call, until the array is freed.  (A call knows its stream before it writes.)
 void note_write(const void* p);
-void note_free(const void* p);
+void note_alloc(const void* p);              // an array of its own begins here
+void note_free(const void* p, size_t bytes);             // with what is known of arrays that were parts of it
 void note_write_elsewhere(const void* p);   // by something that is no call of the library
 uint64_t version_of(const void* p);
 inline float* out_f32(DLArray* a) { note_write(a->data); return (float*)a->data; }

@@ -37,6 +37,7 @@
 #include <cuda_fp16.h>
 #include <algorithm>
 #include <mutex>
+#include <set>
 #include <type_traits>
 #include <unordered_map>
 #include <vector>
@@ -49,24 +50,32 @@ namespace tf {
 // write versions: lets cached packs detect that their source tensor changed
 // ------------------------------------------------------------------------------------------------
 static std::mutex g_ver_mu;
-static std::unordered_map<const void*, uint64_t> g_versions;
+struct Version { uint64_t number = 0; bool block = false, inner = false; };      // block: an allocated array begins here; inner: in g_inner
+static std::unordered_map<const void*, Version> g_versions;
+static std::set<const void*> g_inner;                  // where arrays begin that were not allocated as such: parts of others, which go when those do
 static uint64_t g_ver_counter = 1;
 constexpr uint64_t kRewrittenAnyTime = 0;              // by the replays of a graph that the caller captured
 static bool captured_locked(const void* p) {
   if (t_captured) return true;
   auto it = g_versions.find(p);
-  return it != g_versions.end() && it->second == kRewrittenAnyTime;
+  return it != g_versions.end() && it->second.number == kRewrittenAnyTime;
+}
+static Version& entry_locked(const void* p) {
+  const auto at = g_versions.try_emplace(p);
+  Version& v = at.first->second;
+  if (at.second) v.number = ++g_ver_counter;
+  if (!v.block && !v.inner) { g_inner.insert(p); v.inner = true; }
+  return v;
 }
 static uint64_t version_locked(const void* p) {
   if (t_captured) return ++g_ver_counter;
-  const auto at = g_versions.try_emplace(p, 0);
-  if (at.second) at.first->second = ++g_ver_counter;
-  return at.first->second == kRewrittenAnyTime ? ++g_ver_counter : at.first->second;
+  const Version& v = entry_locked(p);
+  return v.number == kRewrittenAnyTime ? ++g_ver_counter : v.number;
 }
 static void bump_locked(const void* p, bool captured) {
-  const auto at = g_versions.try_emplace(p, 0);
-  if (captured) at.first->second = kRewrittenAnyTime;
-  else if (at.second || at.first->second != kRewrittenAnyTime) at.first->second = ++g_ver_counter;
+  Version& v = entry_locked(p);
+  if (captured) v.number = kRewrittenAnyTime;
+  else if (v.number != kRewrittenAnyTime) v.number = ++g_ver_counter;
 }
 void note_write(const void* p) {
   if (t_recording) recording_note_write(p);
@@ -77,10 +86,26 @@ void note_write_elsewhere(const void* p) {
   std::lock_guard<std::mutex> lk(g_ver_mu);
   bump_locked(p, false);
 }
-void note_free(const void* p) {
+void note_alloc(const void* p) {
+  std::lock_guard<std::mutex> lk(g_ver_mu);
+  const auto at = g_versions.try_emplace(p);
+  Version& v = at.first->second;
+  if (at.second) v.number = ++g_ver_counter;
+  if (v.inner) { g_inner.erase(p); v.inner = false; }
+  v.block = true;
+}
+void note_free(const void* p, size_t bytes) {
   if (t_recording) recording_note_write(p);
   std::lock_guard<std::mutex> lk(g_ver_mu);
-  g_versions[p] = ++g_ver_counter;
+  Version& v = g_versions[p];
+  v.number = ++g_ver_counter;
+  v.block = false;
+  for (auto it = g_inner.lower_bound(p); it != g_inner.end() && (const char*)*it < (const char*)p + bytes; it = g_inner.erase(it)) {
+    if (t_recording) recording_note_write(*it);
+    Version& part = g_versions[*it];
+    part.number = ++g_ver_counter;
+    part.inner = false;
+  }
 }
 uint64_t version_of(const void* p) {
   std::lock_guard<std::mutex> lk(g_ver_mu);
@@ -92,7 +117,7 @@ void bump_versions(const void* const* ptrs, size_t n) {
 }
 void invalidate_all_versions() {
   std::lock_guard<std::mutex> lk(g_ver_mu);
-  for (auto& kv : g_versions) if (kv.second != kRewrittenAnyTime) kv.second = ++g_ver_counter;
+  for (auto& kv : g_versions) if (kv.second.number != kRewrittenAnyTime) kv.second.number = ++g_ver_counter;
 }
 
 // producer-tracked maxima: two device words per tensor, handed out from zero-filled chunks.  A third word per tensor

@@ -479,6 +479,7 @@ int DLArrayAlloc(const index_t* shape, index_t ndim_in, DLContext ctx, DLArrayHa
     if (memorytoSaving) *memorytoSaving = bytes > 0x7fffffffu ? 0x7fffffff : (int)bytes;
     return 0;
   }
+  if (ctx.device_type == kGPU) note_alloc(data);
   DLArray* arr = new DLArray;
   arr->data = data;
   arr->ctx = ctx;
@@ -494,7 +495,11 @@ int DLArrayFree(DLArrayHandle handle) {
   if (!handle) return 0;
   flush_deferred_if_uses(handle->data);      // a held-back kernel may read or write this array
   if (handle->data) {
-    if (handle->ctx.device_type == kGPU) note_free(handle->data);    // a recycled block is new data
+    if (handle->ctx.device_type == kGPU) {                           // a recycled block is new data
+      size_t n = 1;
+      for (int i = 0; i < handle->ndim; ++i) n *= (size_t)handle->shape[i];
+      note_free(handle->data, n * 4);
+    }
     bool ok = (handle->ctx.device_type == kGPU) ? device_pool(handle->ctx.device_id).free(handle->data)
                                                 : host_pool().free(handle->data);
     if (!ok) TF_FAIL("DLArrayFree: array was not allocated by DLArrayAlloc");
