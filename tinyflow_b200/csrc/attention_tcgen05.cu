@@ -89,10 +89,13 @@ __device__ __forceinline__ uint32_t halves(float a, float b) {
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
 __device__ __forceinline__ int exponent_of(float positive) { return (int)((__float_as_uint(positive) >> 23) & 255u) - 127; }
 
-// A block of 512 threads packs one tile of one head, two blocks an SM.  16 G threads a row, 4 columns each.  HBM-bound: 4 bytes an element read and written, for dout 8 read.
-constexpr int kPackThreads = 512, kPackWarps = kPackThreads / 32;
-template <int G, bool WIDE>
-__global__ void __launch_bounds__(kPackThreads, 2) attention_pack_kernel(const __grid_constant__ PackArgs p) {
+// A block packs one tile of one head, 16 G threads a row, 4 columns each.  HBM-bound: 4 bytes an element read and written, for dout 8 read.  Half the rows' loads in flight a
+// thread where there are few tiles (2 x 777 tokens, 6 over 2 heads of 72, both directions: 91 us of the step's time with twice the threads, 95 without; 8 x 1024 tokens, 16
+// heads of 64: 512 and 497).
+constexpr int pack_threads(int G, bool few) { return (few ? 512 : 256) * G; }
+template <int G, bool WIDE, bool FEW>
+__global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, FEW)) attention_pack_kernel(const __grid_constant__ PackArgs p) {
+  constexpr int kPackWarps = pack_threads(G, FEW) / 32;
   constexpr int kAcross = 16 * G, kRowsAtOnce = 32 / kAcross, kRowsOfWarp = kTile / kPackWarps, kSteps = kRowsOfWarp / kRowsAtOnce;
   __shared__ float red[kPackWarps], red_norm[kPackWarps], red_delta[kPackWarps];
   __shared__ uint32_t bad_words[4];
@@ -1069,8 +1072,14 @@ int attention_tc(const AttentionArgs& a, bool backward, size_t* bytes, cudaStrea
   for (const void* x : {(const void*)a.q, (const void*)a.k, (const void*)a.v, (const void*)a.dout, (const void*)a.out}) bits |= reinterpret_cast<uintptr_t>(x);
   const bool wide = bits % 16 == 0;
   const dim3 blocks((unsigned)pack.first[pack.jobs]);
-  if (a.D <= 64) TF_CUDA(wide ? launch_dep(attention_pack_kernel<1, true>, blocks, dim3(kPackThreads), 0, s, pack) : launch_dep(attention_pack_kernel<1, false>, blocks, dim3(kPackThreads), 0, s, pack));
-  else TF_CUDA(wide ? launch_dep(attention_pack_kernel<2, true>, blocks, dim3(kPackThreads), 0, s, pack) : launch_dep(attention_pack_kernel<2, false>, blocks, dim3(kPackThreads), 0, s, pack));
+  const auto run_pack = [&](auto g, auto w, auto few) {
+    constexpr int G = decltype(g)::value;
+    constexpr bool kFew = decltype(few)::value;
+    return launch_dep(attention_pack_kernel<G, decltype(w)::value, kFew>, blocks, dim3(pack_threads(G, kFew)), 0, s, pack);
+  };
+  const auto with_width = [&](auto g, auto few) { return wide ? run_pack(g, std::true_type(), few) : run_pack(g, std::false_type(), few); };
+  const auto with_few = [&](auto g) { return (int)blocks.x <= 2 * device_sm_count() ? with_width(g, std::true_type()) : with_width(g, std::false_type()); };
+  TF_CUDA(a.D <= 64 ? with_few(std::integral_constant<int, 1>()) : with_few(std::integral_constant<int, 2>()));
   TF_AFTER(s, what);
   TF_CUDA(with_form(a, [&](auto g, auto shaped) { return backward ? launch_bwd<decltype(g)::value, decltype(shaped)::value>(tc, s) : launch_fwd<decltype(g)::value, decltype(shaped)::value>(tc, s); }));
   TF_AFTER(s, what);
