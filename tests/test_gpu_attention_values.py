@@ -1,0 +1,80 @@
+"""Attention of values that differ in size from token to token, or are not finite, against the formulas in 64 bits.
+
+Tolerances as in test_gpu_attention.py, but what is lost of small values is counted by token, not by the whole array: no value of one token may cost bits of another's that
+does not depend on it.  On the tensor path a tile of 128 tokens shares a scale only where their largest magnitudes are near each other:
+* queries, keys, values: the arrays here are within 16 of each other, or so far apart that every token has a scale of its own: an element is off by 2^-39 of 16 times
+  its token's largest, twice for both operands of a product: 2^-34;
+* output gradients over their row's sum: within 2^15: 2^-23;
+* weights are off by 2^-38 of what scales them: 1 for the probabilities, for the gradients the norm of the row's output gradient times sqrt(D) times the largest value near it
+  (dq), and up to 1024 times that of any query that the key sees (dk)."""
+import numpy as np
+import pytest
+
+from oracle import ops
+from tests.test_gpu_attention import U, Case, env, path, run  # noqa: F401
+from tests.test_gpu_norm import within
+
+pytestmark = pytest.mark.gpu
+
+
+class Fine(Case):
+    def bounds(self):
+        q, k, v, do = (np.asarray(a, np.float64) for a in (self.q, self.k, self.v, self.dout))
+        want = (ops.attention(q, k, v, **self.formula())[0],) + ops.attention_backward(q, k, v, do, **self.formula())
+        D, cap, chain_k, chain_q = self.dim, self.cap, (self.keys / 16 + 96) * U, (self.queries * self.heads / self.kv_heads / 16 + 96) * U
+        e_out, e_dq, e_dk, e_dv = (np.zeros_like(a) for a in want)
+        near, s = 2.0 ** -34, abs(float(self.scale))
+        for _, h, kv, rows, cols, p, inner, z, _, inv in ops.attention_parts(q, k, **self.formula()):
+            m, t = slice(h * D, (h + 1) * D), slice(kv * D, (kv + 1) * D)
+            Q, K, V, dO, inv = q[rows, m], k[cols, t], v[cols, t], do[rows, m], inv[:, None]
+            seen = np.isfinite(z)
+            qm, km, vm, dm = (np.abs(a).max(1) for a in (Q, K, V, dO))
+            mag = s * np.abs(Q) @ np.abs(K).T
+            ez = (D + 16) * U * mag + s * D * near * np.outer(qm, km) + (8 * U * cap if cap else 0) + 6 * U * (np.abs(np.where(seen, z, 0)) + mag)
+            ep = ez + 12 * U + chain_k
+            ep = ep + (p * ep).sum(1, keepdims=True)
+            e_out[rows, m] = (p * ep) @ np.abs(V) + chain_k * p @ np.abs(V) + 2.0 ** -32 * (p @ vm)[:, None] + 2.0 ** -38 * inv * (seen @ np.abs(V))
+            dp = dO @ V.T
+            edp = (D + 16) * U * np.abs(dO) @ np.abs(V).T + D * 2.0 ** -23 * np.outer(dm, vm)
+            delta = (dO * want[0][rows, m]).sum(1, keepdims=True)
+            edelta = (np.abs(dO) * e_out[rows, m]).sum(1, keepdims=True) + (D + 2) * U * (np.abs(dO) * np.abs(want[0][rows, m])).sum(1, keepdims=True)
+            ds = s * inner * p * (dp - delta)
+            einner = 2 * (ez / cap + 10 * U) if cap else 0.0
+            eds = s * p * (inner * (ep * np.abs(dp - delta) + edp + edelta + 4 * U * (np.abs(dp) + np.abs(delta))) + einner * np.abs(dp - delta))
+            weight = s * 2.0 ** -38 * inv * seen * (16 * D ** 0.5 * np.outer(np.linalg.norm(dO, axis=1), vm) + np.abs(delta))
+            e_dq[rows, m] = eds @ np.abs(K) + chain_k * np.abs(ds) @ np.abs(K) + weight @ np.abs(K) + 2.0 ** -32 * (np.abs(ds) @ km)[:, None]
+            e_dk[cols, t] += eds.T @ np.abs(Q) + chain_q * np.abs(ds).T @ np.abs(Q) + 1024 * weight.T @ np.abs(Q) + 2.0 ** -32 * (np.abs(ds).T @ qm)[:, None]
+            e_dv[cols, t] += (p * ep).T @ np.abs(dO) + chain_q * p.T @ np.abs(dO) + 2.0 ** -23 * (p.T @ dm)[:, None] + 2.0 ** -38 * (inv * seen).T @ np.abs(dO)
+        return want, tuple(e + 1e-35 for e in (e_out, e_dq, e_dk, e_dv))
+
+
+def check(got, want, bound, names=("out", "dq", "dk", "dv")):
+    for name, g, w, e in zip(names, got, want, bound):
+        assert np.isfinite(g).all(), name
+        within(g, w, e, name)
+
+
+# ---- what is not finite -----------------------------------------------------------------------------
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("kind", [dict(queries=40, dim=24), dict(queries=150, dim=64), dict(queries=24, dim=200)], ids=lambda k: "%(queries)d-%(dim)d" % k)
+@pytest.mark.parametrize("first", [True, False])
+def test_a_query_that_is_not_finite_has_no_answer(env, path, kind, bad, cap, first):
+    """The first of its sequence, which sees one key, and one that sees several: the answer and the query's gradient are not finite, nor are the gradients of the keys that it sees,
+    and everything else keeps its bits.  A score of minus infinity alone would have no weight, and a cap would make it finite."""
+    if path == "tensor" and kind["dim"] > 128:
+        pytest.skip("heads of up to 128 elements")
+    c = Case(2, kind["queries"], kind["queries"], 4, 2, kind["dim"], window=6, cap=cap)
+    clean = run(env, c)
+    start = kind["queries"]
+    token, head = start if first else start + 20, 1
+    c.q[token, head * c.dim + 3] = bad
+    got = run(env, c)
+    keys = range(max(start, token - 5), token + 1)
+    for name, g, w, n, touched in (("out", got[0], clean[0], 4, [(token, 1)]), ("dq", got[1], clean[1], 4, [(token, 1)]), ("dk", got[2], clean[2], 2, [(j, 0) for j in keys]),
+                                   ("dv", got[3], clean[3], 2, [(j, 0) for j in keys])):
+        g, w = g.reshape(len(g), n, c.dim).copy(), w.reshape(len(w), n, c.dim)
+        for at in touched:
+            assert not np.isfinite(g[at]).any() if name in ("out", "dq") else not np.isfinite(g[at]).all(), (name, at)
+            g[at] = w[at]
+        assert np.array_equal(g, w), name

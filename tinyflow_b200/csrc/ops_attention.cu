@@ -124,9 +124,10 @@ __device__ __forceinline__ void store_rows(float* to, const Where& where, int fi
     }
   }
 }
-// The score of a product that the query sees, in units of log 2, and the derivative of the cap.
+// The score of a product that the query sees, in units of log 2, and the derivative of the cap.  NaN where the product is not finite: a cap or a weight of zero would hide that.
 __device__ __forceinline__ float score(const AttentionArgs& a, float product, float slope, int away, float& inner) {
   float c = product * a.scale;
+  if (!(fabsf(c) < INFINITY)) c = NAN;
   inner = 1.f;
   if (a.cap > 0.f) {
     const float t = tanhf(c / a.cap);
