@@ -11,7 +11,7 @@ import numpy as np
 import pytest
 
 from oracle import ops
-from tests.test_gpu_attention import U, Case, env, path, run  # noqa: F401
+from tests.test_gpu_attention import IDS, U, Case, env, path, run  # noqa: F401
 from tests.test_gpu_norm import within
 
 pytestmark = pytest.mark.gpu
@@ -78,3 +78,29 @@ def test_a_query_that_is_not_finite_has_no_answer(env, path, kind, bad, cap, fir
             assert not np.isfinite(g[at]).any() if name in ("out", "dq") else not np.isfinite(g[at]).all(), (name, at)
             g[at] = w[at]
         assert np.array_equal(g, w), name
+
+
+@pytest.mark.parametrize("kind", [dict(queries=300, keys=300, heads=4, kv_heads=2, dim=64), dict(queries=260, keys=260, heads=2, kv_heads=2, dim=128, cap=5.0, bias=True),
+                                  dict(queries=140, keys=200, heads=2, kv_heads=1, dim=40, causal=False, documents="packed")], ids=IDS)
+def test_gradients_scale_with_the_output_gradient_bit_by_bit(env, path, kind):
+    """A power of two times the output gradient is that times every gradient."""
+    c = Case(2, **kind)
+    whole = run(env, c)
+    for size in (2.0 ** -3, 2.0 ** -20, 2.0 ** 10):
+        scaled = Case(2, **kind)
+        scaled.dout *= np.float32(size)
+        for name, g, w in zip(("out", "dq", "dk", "dv"), run(env, scaled), whole):
+            assert np.array_equal(g, w * np.float32(1 if name == "out" else size)), (name, size)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_tokens_that_see_themselves_alone(env, path, dim):
+    """Documents of one token: a probability of 1, so the value's gradient is the output gradient, but for the score's distance from itself.  That is z - max, where max is z rounded: half a step
+    of |z| + 1, log 2 of it a change of the weight; 2 u each for the exponential, the reciprocal and their product; 2^-22 for both operands' halves and what their product drops, and
+    2 u for each of three products' accumulations; 2^-32 of the largest value for those far below it."""
+    c = Case(1, 512, 512, 2, 2, dim, documents=np.arange(512).astype(np.float32), seed=9)
+    out, dq, dk, dv = run(env, c)
+    z = np.abs((np.asarray(c.q, np.float64) * c.k).reshape(512, 2, dim).sum(-1)) * float(c.scale) * np.log2(np.e)
+    allowed = np.repeat(U * (np.log(2) * (z + 1) + 6 + 4 + 6), dim, axis=1)
+    within(dv, np.asarray(c.dout, np.float64), allowed * np.abs(c.dout) + 2.0 ** -32 * np.abs(c.dout).max(), "dv")
+    within(out, np.asarray(c.v, np.float64), allowed * np.abs(c.v) + 2.0 ** -32 * np.abs(c.v).max(), "out")

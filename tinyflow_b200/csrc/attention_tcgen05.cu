@@ -44,6 +44,7 @@ constexpr int kThreads = 384;
 // Registers a thread: 168 at the launch (64,512 of the block); the first four warps give 96 of theirs, the others take 48 each, the same sum.
 constexpr int kFewRegisters = 72, kManyRegisters = 216;
 constexpr int kWeightExp = 14;                   // weights are scaled to below 2^15
+constexpr float kWeightScale = 1 << kWeightExp;
 constexpr int kFar = 1 << 26;                    // beyond every position
 
 // Of one tile of one head
@@ -793,7 +794,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
         const float g = rewritten ? 1.f : f;
         // of -infinity: NaN if g is 0, which the maximum leaves out
         const float at_most = fmaxf(most, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * g), base = max_of_finite_or(at_most);
-        const float shifted = base - (float)kWeightExp, faded = exp2_fast(most - base);
+        const float faded = exp2_fast(most - base);
         most = at_most;
         float2 s[2] = {both(0.f), both(0.f)};
 #pragma unroll 1
@@ -804,9 +805,9 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
           tmem_ld_wait();
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
-            const float2 e = fma2(at2(z, k), both(g), both(-shifted)), w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+            const float2 e = fma2(at2(z, k), both(g), both(-base)), w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
             s[(k >> 1) & 1] = add2(s[(k >> 1) & 1], w);
-            put2(z, k, w);
+            put2(z, k, mul2(w, both(kWeightScale)));
           }
           split32(z, words);
           tmem_st32(from + 32 * c, words);
@@ -815,18 +816,19 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
         arrive(&w_full[n & 1]);
         sum = fmaf(sum, faded, (s[0].x + s[0].y) + (s[1].x + s[1].y));
         alpha = faded;
-        out_factor = now.inv2;
+        out_factor = now.inv2 * (1.f / kWeightScale);
       } else {
-        float factor;
-        int shift = kWeightExp;
+        // The weights' power of two is a factor: added to the exponent's argument it would cost bits of that, the more the smaller the output gradient (dq 6e-7 off at 1e-7 of it instead of 1e-7)
+        float factor, lift = kWeightScale;
         if (KIND == kDv) {
-          factor = now.inv2 * power_of_two(-kWeightExp);
+          factor = now.inv2 * (1.f / kWeightScale);
         } else {
           const float bound = KIND == kDq ? fmaf(row_norm, now.x, fabsf(row_delta)) : fmaf(now.x, norm_top, now.y);
-          shift = min(100, max(-100, kWeightExp - exponent_of(bound)));
+          const int shift = min(100, max(-100, kWeightExp - exponent_of(bound)));
+          lift = power_of_two(shift);
           factor = now.inv1 * power_of_two(-shift);
         }
-        const float kk = (float)shift, fy = inv2 * now.inv2;
+        const float fy = KIND == kDq ? inv2 * lift * now.inv2 : inv2 * now.inv2;         // dq: the row's numbers have it, the others' weights
         const float *const col_max = columns + (n & 1) * 256 + col_part, *const col_delta = col_max + 128;
         if (kRowsAreKeys) await(&columns_full[n & 1], (n >> 1) & 1, abort_flag, bad);
         if (kTwo) wait_for(&y_full[n & 1], (n >> 1) & 1);
@@ -843,8 +845,8 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
 #pragma unroll
             for (int k = 0; k < 32; k += 4) {
               const float4 m4 = *reinterpret_cast<const float4*>(col_max + 32 * c + k);
-              put2(z, k, fma2(at2(z, k), both(g), make_float2(kk - m4.x, kk - m4.y)));
-              put2(z, k + 2, fma2(at2(z, k + 2), both(g), make_float2(kk - m4.z, kk - m4.w)));
+              put2(z, k, fma2(at2(z, k), both(g), make_float2(-m4.x, -m4.y)));
+              put2(z, k + 2, fma2(at2(z, k + 2), both(g), make_float2(-m4.z, -m4.w)));
               if (KIND == kDk) {
                 const float4 d4 = *reinterpret_cast<const float4*>(col_delta + 32 * c + k);
                 put2(y, k, fma2(at2(y, k), both(fy), make_float2(-d4.x, -d4.y)));
@@ -852,13 +854,14 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
               }
             }
           } else {
-            const float less = kk - row_max;
+            const float delta = row_delta * lift;
 #pragma unroll
-            for (int k = 0; k < 32; k += 2) { put2(z, k, fma2(at2(z, k), both(g), both(less))); put2(y, k, fma2(at2(y, k), both(fy), both(-row_delta))); }
+            for (int k = 0; k < 32; k += 2) { put2(z, k, fma2(at2(z, k), both(g), both(-row_max))); put2(y, k, fma2(at2(y, k), both(fy), both(-delta))); }
           }
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
             float2 w = make_float2(exp2_fast(z[k]), exp2_fast(z[k + 1]));
+            if (kRowsAreKeys) w = mul2(w, both(lift));
             if (kTwo) w = mul2(w, SHAPED ? mul2(at2(y, k), at2(turned, k)) : at2(y, k));
             put2(z, k, w);
           }
@@ -901,7 +904,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
           last = inv * here; other = inv * over_there;
           if (a.stats && there) {
             float* const to = a.stats + 2 * (((int64_t)b * a.H + row_head) * a.Tq + self);
-            to[0] = base; to[1] = inv * (float)(1 << kWeightExp);
+            to[0] = base; to[1] = inv;
           }
         }
         if (*any_handed) {
