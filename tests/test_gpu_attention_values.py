@@ -104,3 +104,40 @@ def test_tokens_that_see_themselves_alone(env, path, dim):
     allowed = np.repeat(U * (np.log(2) * (z + 1) + 6 + 4 + 6), dim, axis=1)
     within(dv, np.asarray(c.dout, np.float64), allowed * np.abs(c.dout) + 2.0 ** -32 * np.abs(c.dout).max(), "dv")
     within(out, np.asarray(c.v, np.float64), allowed * np.abs(c.v) + 2.0 ** -32 * np.abs(c.v).max(), "out")
+
+
+@pytest.mark.parametrize("size", [2.0 ** 12, 2.0 ** 24, 2.0 ** 34, 2.0 ** 60, 2.0 ** 110])
+@pytest.mark.parametrize("kind", [dict(queries=300, keys=300, heads=4, kv_heads=2, dim=64), dict(queries=150, keys=270, heads=2, kv_heads=1, dim=128, causal=False), dict(queries=2, keys=700, heads=4, kv_heads=2, dim=40),
+                                  dict(queries=200, keys=200, heads=2, kv_heads=2, dim=48, bias=True)], ids=IDS)
+def test_scores_of_any_size(env, path, kind, size):
+    """Where the largest score is 150 above the next, in units of log 2, it takes all: the answer is its value, and the value's gradient the sum of the output gradients of the queries that it
+    answers.  u: 2 each for exponential, sum, reciprocal and products, 4 for the halves, 6 for the accumulations, and the sum over queries (the calls of few queries form scores in an
+    order of their own: their answers alone)."""
+    c = Case(1, **kind)
+    c.q *= np.float32(size ** 0.5)
+    c.k *= np.float32(size ** 0.5)
+    got = run(env, c)
+    assert all(np.isfinite(g).all() for g in got)
+    D, want, dv, allowed = c.dim, np.zeros(c.q.shape), np.zeros(c.v.shape), np.zeros(c.v.shape)
+    clear = np.zeros((c.queries, c.heads), bool)
+    for _, h, kv, rows, cols, p, _, z, _, _ in ops.attention_parts(c.q.astype(np.float64), c.k.astype(np.float64), **c.formula()):
+        m, t = slice(h * D, (h + 1) * D), slice(kv * D, (kv + 1) * D)
+        best = z.argmax(1)
+        rest = z.copy()
+        rest[np.arange(c.queries), best] = -np.inf
+        noise = (D + 16) * U * float(c.scale) * np.log2(np.e) * (np.abs(c.q[:, m].astype(np.float64)) @ np.abs(c.k[:, t].astype(np.float64)).T).max(1)
+        clear[:, h] = z.max(1) - rest.max(1) > 150 + 2 * noise
+        want[:, m] = c.v[best, t]
+    assert clear.mean() > (0.2 if size < 2.0 ** 20 else 0.9)
+    of_out = np.repeat(clear, D, axis=1)
+    within(got[0][of_out], want[of_out], 16 * U * np.abs(want[of_out]) + 2.0 ** -32 * np.abs(c.v).max(), "out")
+    if c.queries * c.heads // c.kv_heads <= 16:
+        return
+    c.dout[~of_out] = 0
+    got = run(env, c)
+    for _, h, kv, rows, cols, p, _, z, _, _ in ops.attention_parts(c.q.astype(np.float64), c.k.astype(np.float64), **c.formula()):
+        m, t = slice(h * D, (h + 1) * D), slice(kv * D, (kv + 1) * D)
+        for i, j in enumerate(z.argmax(1)):
+            dv[j, t] += c.dout[i, m]
+            allowed[j, t] += np.abs(c.dout[i, m])
+    within(got[3], dv, (16 + c.queries / 16 + 96) * U * allowed + 2.0 ** -30 * np.abs(c.dout).max(), "dv")

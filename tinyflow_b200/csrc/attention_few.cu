@@ -131,12 +131,12 @@ __global__ void __launch_bounds__(kThreads, kBlocks) attention_few_kernel(const 
         for (int d = 2; d < DL; d += 2) dot = fma2(at2(q[r], d), at2(k[u], d), dot);
         dots[r * kUnroll + u] = dot.x + dot.y;
       }
-    float s = over_lanes<kLanes, kScores>(dots) * scale;
+    float s = __fmul_rn(over_lanes<kLanes, kScores>(dots), scale);   // rounded before the maximum is taken off, however large it is
     if (!(fabsf(s) < INFINITY)) s = NAN;         // a cap or a weight of zero would hide what is not finite
     const int j = j0 + my_u * kAtOnce + sub;
     if (SHAPED) {
       if (a.cap > 0.f) s = a.cap * tanhf(s / a.cap);
-      s = (s - my_slope * fabsf((float)(my_at - j))) * kLog2e;
+      s = __fmul_rn(fmaf(-my_slope, fabsf((float)(my_at - j)), s), kLog2e);
     }
     unsigned seen_by = 0xffffffffu;
     if (!whole) {

@@ -357,6 +357,11 @@ __device__ __forceinline__ void tanh32(float* t) {
     put2(t, k, y);
   }
 }
+// g z less m, g z rounded as the maximum m was: the largest score is 0 then, in both directions, however large it is.  In one rounding it would be what rounding m took off, 2^8 for
+// a score of 2^32 (and the compiler makes one rounding of a packed product and a sum behind it).  Shaped scores are whole, their g is 1.
+template <bool SHAPED> __device__ __forceinline__ float2 less(float2 z, float g, float2 m) {
+  return add2(SHAPED ? z : make_float2(__fmul_rn(z.x, g), __fmul_rn(z.y, g)), make_float2(-m.x, -m.y));
+}
 // hi and lo halves of 32 weights, as the A operand has them: 16 weights are 8 words of hi and 8 of lo
 __device__ __forceinline__ void split32(const float* w, uint32_t* words) {
 #pragma unroll
@@ -576,16 +581,18 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) mma_ts(d, w + 16 * ks, cols_low + ks * 128, kHigh, idesc, ks ? 1u : keep);
     };
-    const auto scores = [&](uint32_t d, uint32_t rows_hi, auto in_tmem, uint64_t* done) {
+    // Scores add up the queries' lo halves times the keys' hi halves, then the other way around, then both hi halves, whichever are the rows, so that both directions truncate alike
+    // and form the same scores.  `lo_pass` reads the columns' lo half, whose stage is given back behind it.
+    const auto scores = [&](uint32_t d, uint32_t rows_hi, auto in_tmem, int lo_pass, uint64_t* done) {
       wait_tile();
       const int lo = stage;
       next_stage();
       if (!bad && elect_one()) {
         const uint32_t at_lo = k_major(smem_u32(ring + lo * kPart)), at_hi = k_major(smem_u32(ring + stage * kPart));
 #pragma unroll 1
-        for (int pass = 0; pass < 3; ++pass) {   // hi * lo, lo * hi, hi * hi
-          score_steps(d, rows_hi + (pass != 1 ? 0 : decltype(in_tmem)::value ? 32 * G : kPart >> 4), decltype(in_tmem)::value, pass ? at_hi : at_lo, pass);
-          if (pass == 0) tcgen05_commit(&empty[lo]);
+        for (int pass = 0; pass < 3; ++pass) {
+          score_steps(d, rows_hi + (pass != 1 - lo_pass ? 0 : decltype(in_tmem)::value ? 32 * G : kPart >> 4), decltype(in_tmem)::value, pass == lo_pass ? at_lo : at_hi, pass);
+          if (pass == lo_pass) tcgen05_commit(&empty[lo]);
         }
         tcgen05_commit(&empty[stage]);
         tcgen05_commit(done);
@@ -622,10 +629,10 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
       await(entry_full + (n & 7), (n >> 3) & 1, abort_flag, bad);
       bad = __any_sync(0xffffffffu, bad);
       if (bad || !(entries[n & 7].flags & 1)) break;
-      scores(tmem + (n & 1) * 128, rows1, std::integral_constant<bool, S::kRowsInTmem>(), &s_full[n & 1]);
+      scores(tmem + (n & 1) * 128, rows1, std::integral_constant<bool, S::kRowsInTmem>(), kRowsAreKeys ? 0 : 1, &s_full[n & 1]);
       if (kTwo) {
         if (n >= 1) await(&y_empty[(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag, bad);
-        scores(tmem + S::kYAt, rows2, std::false_type(), &y_full[n & 1]);
+        scores(tmem + S::kYAt, rows2, std::false_type(), 0, &y_full[n & 1]);
       }
       if (n > 0) product(n - 1);
     }
@@ -805,7 +812,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
           tmem_ld_wait();
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
-            const float2 e = fma2(at2(z, k), both(g), both(-base)), w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+            const float2 e = less<SHAPED>(at2(z, k), g, both(base)), w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
             s[(k >> 1) & 1] = add2(s[(k >> 1) & 1], w);
             put2(z, k, mul2(w, both(kWeightScale)));
           }
@@ -845,8 +852,8 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
 #pragma unroll
             for (int k = 0; k < 32; k += 4) {
               const float4 m4 = *reinterpret_cast<const float4*>(col_max + 32 * c + k);
-              put2(z, k, fma2(at2(z, k), both(g), make_float2(-m4.x, -m4.y)));
-              put2(z, k + 2, fma2(at2(z, k + 2), both(g), make_float2(-m4.z, -m4.w)));
+              put2(z, k, less<SHAPED>(at2(z, k), g, make_float2(m4.x, m4.y)));
+              put2(z, k + 2, less<SHAPED>(at2(z, k + 2), g, make_float2(m4.z, m4.w)));
               if (KIND == kDk) {
                 const float4 d4 = *reinterpret_cast<const float4*>(col_delta + 32 * c + k);
                 put2(y, k, fma2(at2(y, k), both(fy), make_float2(-d4.x, -d4.y)));
@@ -856,7 +863,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
           } else {
             const float delta = row_delta * lift;
 #pragma unroll
-            for (int k = 0; k < 32; k += 2) { put2(z, k, fma2(at2(z, k), both(g), both(-row_max))); put2(y, k, fma2(at2(y, k), both(fy), both(-delta))); }
+            for (int k = 0; k < 32; k += 2) { put2(z, k, less<SHAPED>(at2(z, k), g, both(row_max))); put2(y, k, fma2(at2(y, k), both(fy), both(-delta))); }
           }
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {

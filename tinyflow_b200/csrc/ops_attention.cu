@@ -134,7 +134,12 @@ __device__ __forceinline__ float score(const AttentionArgs& a, float product, fl
     c = a.cap * t;
     inner = 1.f - t * t;
   }
-  return (c - slope * fabsf((float)away)) * kLog2e;
+  return __fmul_rn(fmaf(-slope, fabsf((float)away), c), kLog2e);     // rounded before a maximum is taken off, in both directions alike: the largest is 0 then, however large the scores are
+}
+// 2^(score - most) for the gradients: at most 1, also where another kernel's forward call rounded the score otherwise and it is above the largest
+__device__ __forceinline__ float weight(float score, float most) {
+  const float x = score - most;
+  return exp2f(x > 0.f ? 0.f : x);               // NaN stays
 }
 __device__ __forceinline__ float half_warp_max(float v) {
 #pragma unroll
@@ -318,7 +323,7 @@ __global__ void __launch_bounds__(kThreads) attention_tile_bwd_kernel(const __gr
           const int j = tx + 16 * c;
           float w = 0.f, inner;
           if (row_sees(a, rs[i], prefix, j0 + j, a.documents ? sm.document[j] : 0.f)) {
-            w = exp2f(score(a, x[i][c], rs[i].slope, rs[i].at - j0 - j, inner) - most[i]) * inv[i];
+            w = weight(score(a, x[i][c], rs[i].slope, rs[i].at - j0 - j, inner), most[i]) * inv[i];
             w = sm.bad[j] ? NAN : w * (y[i][c] - sm.delta[2 * ty + i]) * inner * a.scale;
           }
           sm.W[0][(2 * ty + i) * kPitchW + j] = w;
@@ -364,7 +369,7 @@ __global__ void __launch_bounds__(kThreads) attention_tile_bwd_kernel(const __gr
         const int j = first + 2 * ty + i;
         float p = 0.f, w = 0.f, inner;
         if (row_sees(a, rs, prefix, j, document[i])) {
-          p = sm.bad[r] ? NAN : exp2f(score(a, x[i][c], rs.slope, rs.at - j, inner) - sm.stat[r][0]) * sm.stat[r][1];
+          p = sm.bad[r] ? NAN : weight(score(a, x[i][c], rs.slope, rs.at - j, inner), sm.stat[r][0]) * sm.stat[r][1];
           w = sm.bad[r] ? NAN : p * (y[i][c] - sm.stat[r][2]) * inner * a.scale;
         }
         sm.W[0][(2 * ty + i) * kPitchW + r] = w;
