@@ -141,3 +141,13 @@ def test_scores_of_any_size(env, path, kind, size):
             dv[j, t] += c.dout[i, m]
             allowed[j, t] += np.abs(c.dout[i, m])
     within(got[3], dv, (16 + c.queries / 16 + 96) * U * allowed + 2.0 ** -30 * np.abs(c.dout).max(), "dv")
+
+
+@pytest.mark.parametrize("size", [2.0 ** -100, 2.0 ** -75, 2.0 ** -64, 2.0 ** 62, 2.0 ** 80])
+@pytest.mark.parametrize("dim", [40, 128])
+def test_output_gradients_whose_squares_leave_float32(env, path, dim, size):
+    c = Fine(1, 400, 400, 2, 1, dim, causal=False, seed=10)
+    want, bound = c.bounds()
+    c.dout *= np.float32(size)
+    got = run(env, c)
+    check([g.astype(np.float64) / (size if i else 1) for i, g in enumerate(got)], want, bound)

@@ -150,7 +150,16 @@ __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, F
         }
 #pragma unroll
         for (int k = kAcross / 2; k > 0; k >>= 1) { delta += __shfl_xor_sync(0xffffffffu, delta, k); norm += __shfl_xor_sync(0xffffffffu, norm, k); }
+        const bool leaves = !(norm > 1e-30f && norm < 1e37f);            // the squares leave the numbers' range, or are zero
         norm = sqrtf(norm);
+        if (__any_sync(0xffffffffu, leaves)) {   // a bound in its place
+          float top = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(v[s0 + s][i]));
+#pragma unroll
+          for (int k = kAcross / 2; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+          if (leaves) norm = fminf(top * sqrtf((float)D), 3e38f);
+        }
         if (!(fabsf(delta) < INFINITY && norm < INFINITY && fabsf(stat_max[s]) < INFINITY && fabsf(stat_inv[s]) < INFINITY)) {
           unfit |= 1u << (s0 + s);
           stat_max[s] = delta = norm = 0.f;
