@@ -151,3 +151,13 @@ def test_output_gradients_whose_squares_leave_float32(env, path, dim, size):
     c.dout *= np.float32(size)
     got = run(env, c)
     check([g.astype(np.float64) / (size if i else 1) for i, g in enumerate(got)], want, bound)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_tokens_that_see_themselves_alone_behind_a_cap(env, path, dim):
+    """The same, with scores of 20 to 30 behind a cap of 30.  The score is what the answer's was, bit by bit, so its weight is 1."""
+    c = Case(1, 512, 512, 2, 2, dim, documents=np.arange(512).astype(np.float32), cap=30.0, seed=9)
+    c.k = (c.q * np.random.RandomState(1).uniform(3, 9, (512, 1))).astype(np.float32)
+    out, dq, dk, dv = run(env, c)
+    within(dv, np.asarray(c.dout, np.float64), 16 * U * np.abs(c.dout) + 2.0 ** -32 * np.abs(c.dout).max(), "dv")
+    within(out, np.asarray(c.v, np.float64), 16 * U * np.abs(c.v) + 2.0 ** -32 * np.abs(c.v).max(), "out")
