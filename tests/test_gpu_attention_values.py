@@ -161,3 +161,106 @@ def test_tokens_that_see_themselves_alone_behind_a_cap(env, path, dim):
     out, dq, dk, dv = run(env, c)
     within(dv, np.asarray(c.dout, np.float64), 16 * U * np.abs(c.dout) + 2.0 ** -32 * np.abs(c.dout).max(), "dv")
     within(out, np.asarray(c.v, np.float64), 16 * U * np.abs(c.v) + 2.0 ** -32 * np.abs(c.v).max(), "out")
+
+
+# ---- tokens of different sizes ---------------------------------------------------------------------
+KINDS = [dict(heads=4, kv_heads=2, dim=64), dict(heads=2, kv_heads=2, dim=128, causal=False), dict(heads=3, kv_heads=1, dim=33, cap=4.0, bias=True), dict(heads=2, kv_heads=1, dim=96, causal=False, cap=20.0),
+         dict(heads=1, kv_heads=1, dim=16, bias=True)]
+
+
+def among_others(alone, lead, tail, seed=1):
+    """Documents of `lead` and `tail` tokens around the tokens of `alone`, all of one row."""
+    n, total = alone.queries, lead + alone.queries + tail
+    c = Case(1, total, total, alone.heads, alone.kv_heads, alone.dim, alone.causal, cap=alone.cap, bias=alone.slopes is not None, seed=seed)
+    c.documents = np.repeat([1.0, 2.0, 3.0], [lead, n, tail]).astype(np.float32)
+    mine = slice(lead, lead + n)
+    for name in ("q", "k", "v", "dout"):
+        getattr(c, name)[mine] = getattr(alone, name)
+    return c, mine, [t for t in range(total) if not lead <= t < lead + n]
+
+
+@pytest.mark.parametrize("size", [2.0 ** 13, 2.0 ** 20, 2.0 ** 40, 2.0 ** 100, 2.0 ** -20])
+@pytest.mark.parametrize("where", ["q", "k", "all"])
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+def test_other_documents_of_any_size_cost_nothing(env, path, kind, where, size):
+    alone = Fine(1, 140, 140, seed=3, **kind)
+    want, bound = alone.bounds()
+    c, mine, others = among_others(alone, 60, 75)
+    clean = run(env, c)
+    for name in ("q", "k", "v") if where == "all" else (where,):
+        getattr(c, name)[others] *= np.float32(size ** 0.5 if where == "all" else size)
+    got = run(env, c)
+    check([g[mine] for g in got], want, bound)
+    if path == "exact":
+        for g, w in zip(got, clean):
+            assert np.array_equal(g[mine], w[mine])
+
+
+@pytest.mark.parametrize("size", [2.0 ** 20, 2.0 ** 60, 2.0 ** 120])
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+def test_padding_of_any_size_costs_nothing(env, path, kind, size):
+    """Padding behind every sequence: no result depends on it."""
+    c = Fine(2, 150, 150, documents=np.where(np.arange(300) % 150 < 141, 1.0, -1.0).astype(np.float32), seed=2, **kind)
+    want, bound = c.bounds()
+    padding = np.flatnonzero(c.documents < 0)
+    for array in (c.q, c.k, c.v, c.dout):
+        array[padding] *= np.float32(size)
+    check(run(env, c), want, bound)
+
+
+@pytest.mark.parametrize("size", [2.0 ** 20, 2.0 ** 60])
+@pytest.mark.parametrize("kind", [k for k in KINDS if k.get("causal", True)], ids=IDS)
+def test_tokens_behind_a_query_cost_nothing(env, path, kind, size):
+    """Tokens 90 to 99 of 200 diverge: the answers and gradients of the queries in front of them."""
+    c = Fine(1, 200, 200, seed=4, **kind)
+    c.dout[90:] = 0                                        # the keys' gradients are those of the queries in front
+    want, bound = c.bounds()
+    for array in (c.q, c.k, c.v):
+        array[90:100] *= np.float32(size)
+    got = run(env, c)
+    check([g[:90] for g in got], [w[:90] for w in want], [e[:90] for e in bound])
+
+
+@pytest.mark.parametrize("where", ["v", "k", "q"])
+@pytest.mark.parametrize("size", [2.0 ** 13, 2.0 ** 20, 2.0 ** 40, 2.0 ** -13, 2.0 ** -40])
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+def test_one_token_of_another_size_among_those_that_are_seen(env, path, kind, where, size):
+    """What depends on the token is as near to the formula as its own magnitudes allow, what does not is not touched.  Larger queries and keys come with a smaller scale, so that scores stay
+    in an exponential's range, and smaller others: their scores are next to nothing, whichever of them."""
+    c = Fine(1, 200, 200, seed=5, scale=kind["dim"] ** -0.5 * (min(1.0, 1 / size) if where != "v" else 1.0), **kind)
+    getattr(c, where)[37] *= np.float32(size)
+    getattr(c, where)[161] *= np.float32(size)
+    check(run(env, c), *c.bounds())
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+def test_every_token_of_a_size_of_its_own(env, path, kind):
+    """Values from 2^-30 to 2^30, queries and output gradients too, keys the other way around."""
+    rng = np.random.RandomState(11)
+    c = Fine(2, 270, 270, seed=6, **kind)
+    sizes = lambda: (2.0 ** rng.randint(-30, 31, (540, 1))).astype(np.float32)      # noqa: E731
+    c.v *= sizes()
+    by_query = sizes()
+    c.q *= by_query
+    c.dout *= sizes()
+    c.scale = np.float32(c.scale * 2.0 ** -30)
+    check(run(env, c), *c.bounds())
+
+
+@pytest.mark.parametrize("shared", [True, False])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_sequences_and_heads_of_any_size_side_by_side(env, path, dim, shared):
+    """One sequence and head diverges token by token; the others do not notice."""
+    c = Fine(3, 260, 260, 4, 2 if shared else 4, dim, seed=7)
+    want, bound = c.bounds()
+    rows = slice(260, 520)
+    sizes = (2.0 ** np.random.RandomState(3).randint(-40, 41, (260, 1))).astype(np.float32)
+    for a in (c.q, c.k, c.v, c.dout):
+        a[rows, :dim] *= sizes
+    got = run(env, c)
+    for name, g, w, e, n in zip(("out", "dq", "dk", "dv"), got, want, bound, (4, 4, c.kv_heads, c.kv_heads)):
+        view = lambda a: np.delete(a.reshape(3, 260, n, dim), 0, axis=2)[1] if n > 1 else a[:0]      # noqa: E731
+        for b in (0, 2):
+            within(g[260 * b:260 * (b + 1)], w[260 * b:260 * (b + 1)], e[260 * b:260 * (b + 1)], name)
+        if not shared:
+            within(view(g), view(w), view(e), name)

@@ -19,6 +19,10 @@
 // (bounded for gradients by the norms of dO' rows and V) is just below 2^15.  Scales of a tile are undone where its product is added up: the tensor core
 // truncates as it accumulates, so every tile's product is added to fp32 registers (round to nearest) by the warps that make the weights.
 //
+// Tokens of different sizes.  What a row does not see (padding, other documents, tokens behind it) may be of any size, and must not cost it bits.  Where a tile's tokens are further
+// apart than a scale serves (kOrders), each is packed with a scale of its own.  The warps undo those in the scores, put those of the product's operand into the weights, and scale a row's
+// weights by the largest that it sees, found first: a second pass over such tiles, in code of its own beside the loop that all others take.
+//
 // Bound by the tensor rate: 3 products of 16-bit halves for each product.  The tile of the next scores is issued ahead of the product of the present weights,
 // so the tensor cores work while 8 warps (two a TMEM lane quarter) make weights.  4 x 4096 tokens, 8 heads of 128, every key seen: forward 755 us (364 TFLOP/s of the formula,
 // three times that in halves), gradients 2812; heads of 64: 422 and 1520.  There the power limit holds the clock at 1.45 to 1.6 GHz of 1.97.  A CTA's start and end take 8 us,
@@ -49,11 +53,11 @@ constexpr int kFar = 1 << 26;                    // beyond every position
 
 // Of one tile of one head
 struct __align__(16) TileInfo {
-  float inv, top;                                // 1 / scale; largest finite magnitude
+  float inv, top;                                // 1 / scale; negative where every token has one of its own; largest finite magnitude
   float norm, delta;                             // dO': largest row norm and |D'|
   uint32_t bad[4];                               // tokens with values that are not finite
 };
-struct Packed { const char* image; const TileInfo* info; };
+struct Packed { const char* image; const TileInfo* info; const float* scale; };           // 1 / scale of every token; 0 for tokens of zeros among others with scales of their own
 struct TcArgs {
   AttentionArgs a;
   Packed q, k, v, d;
@@ -61,6 +65,7 @@ struct TcArgs {
   const float4* documents;                       // of every sequence and key tile: smallest, largest, whether there is padding
   float *dk_part, *dv_part;                      // where the query heads of a key-value head are dealt to several CTAs: their sums, one after another
   int q_tiles, k_tiles, D16, shares;
+  float one;                                     // 1
   int* err;
 };
 
@@ -69,6 +74,7 @@ struct PackJob {
   const float* x;
   char* image;
   TileInfo* info;
+  float* scale;
   int heads, length, tiles;
   int gradient;                                  // dout: times 1 / sum, with its row's D' and norm
 };
@@ -90,6 +96,24 @@ __device__ __forceinline__ uint32_t halves(float a, float b) {
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
 __device__ __forceinline__ int exponent_of(float positive) { return (int)((__float_as_uint(positive) >> 23) & 255u) - 127; }
 
+// Joins four numbers over kAcross lanes; lane l is left with that of number l / (kAcross / 4)
+template <int kAcross, class F> __device__ __forceinline__ float joined(const float* v, F&& join) {
+  const bool upper = threadIdx.x & (kAcross / 2), odd = threadIdx.x & (kAcross / 4);
+  float w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) w[i] = join(upper ? v[i + 2] : v[i], __shfl_xor_sync(0xffffffffu, upper ? v[i] : v[i + 2], kAcross / 2));
+  float x = join(odd ? w[1] : w[0], __shfl_xor_sync(0xffffffffu, odd ? w[0] : w[1], kAcross / 4));
+#pragma unroll
+  for (int o = kAcross / 8; o > 0; o >>= 1) x = join(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
+}
+// Binary orders between the largest magnitudes of two tokens of a tile up to which they share a scale.  A value is held to 2^-39 of the tile's largest, so 8 orders leave 2^-31 of the
+// token's own, and the scale of the gradients' weights, which goes by the largest value, 8 bits of 25 to spare.  Output gradients over their row's sum, which differ by as much as the
+// sums do, up to the number of keys: 14 orders leave 2^-25.
+constexpr int kOrders = 8, kOrdersOfGradient = 14;
+// max * scale in [2^14, 2^15); subnormal maxima, and those from 2^126, as far as the scale and its reciprocal are normal numbers
+__device__ __forceinline__ int scale_exponent(float most) { return most > 0.f ? min(126, max(-126, 14 - exponent_of(most))) : 0; }
+
 // A block packs one tile of one head, 16 G threads a row, 4 columns each.  HBM-bound: 4 bytes an element read and written, for dout 8 read.  Half the rows' loads in flight a
 // thread where there are few tiles (2 x 777 tokens, 6 over 2 heads of 72, both directions: 91 us of the step's time with twice the threads, 95 without; 8 x 1024 tokens, 16
 // heads of 64: 512 and 497).
@@ -98,7 +122,8 @@ template <int G, bool WIDE, bool FEW>
 __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, FEW)) attention_pack_kernel(const __grid_constant__ PackArgs p) {
   constexpr int kPackWarps = pack_threads(G, FEW) / 32;
   constexpr int kAcross = 16 * G, kRowsAtOnce = 32 / kAcross, kRowsOfWarp = kTile / kPackWarps, kSteps = kRowsOfWarp / kRowsAtOnce;
-  __shared__ float red[kPackWarps], red_norm[kPackWarps], red_delta[kPackWarps];
+  constexpr int kShare = kAcross / 4, kGroups = kSteps / 4;            // of four steps' rows a lane looks after one, with kShare - 1 others
+  __shared__ float red[kPackWarps], red_least[kPackWarps], red_norm[kPackWarps], red_delta[kPackWarps], token_scale[kTile];
   __shared__ uint32_t bad_words[4];
   grid_dep_sync();
   int j = 0;
@@ -109,7 +134,7 @@ __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, F
   const int D = p.a.D;
   if (threadIdx.x < 4) bad_words[threadIdx.x] = 0u;
   float v[kSteps][4];
-  float most = 0.f, most_norm = 0.f, most_delta = 0.f;
+  float most_norm = 0.f, most_delta = 0.f;
   const auto load4 = [&](const float* from, int t, float* w) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = 0.f;
@@ -125,92 +150,116 @@ __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, F
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) load4(job.x, tile * kTile + row_of(s), v[s]);
   __syncthreads();
-  uint32_t unfit = 0u;                           // steps whose row's statistics are not finite
+  const auto own_row = [&](int g) { return row_of(4 * g + lane % kAcross / kShare); };
+  const auto add = [](float x, float y) { return x + y; };
+  const auto larger = [](float x, float y) { return fmaxf(x, y); };
+  float own_max[kGroups], own_delta[kGroups], own_norm[kGroups], own_top[kGroups];
   if (job.gradient) {
+    const float* const stats = p.a.stats + 2 * (((int64_t)b * job.heads + h) * job.length + tile * kTile);
+    const int rows = job.length - tile * kTile;
 #pragma unroll
-    for (int s0 = 0; s0 < kSteps; s0 += 4) {
-      float o[4][4], stat_max[4], stat_inv[4];
+    for (int g = 0; g < kGroups; ++g) {
+      float o[4][4], stat_inv[4], delta[4], norm[4];
+      own_max[g] = own_row(g) < rows ? __ldg(stats + 2 * own_row(g)) : 0.f;
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        const int t = tile * kTile + row_of(s0 + s);
-        load4(p.a.out, t, o[s]);
-        const int64_t stat = 2 * (((int64_t)b * job.heads + h) * job.length + t);
-        stat_max[s] = t < job.length ? __ldg(p.a.stats + stat) : 0.f;
-        stat_inv[s] = t < job.length ? __ldg(p.a.stats + stat + 1) : 0.f;
+        load4(p.a.out, tile * kTile + row_of(4 * g + s), o[s]);
+        stat_inv[s] = row_of(4 * g + s) < rows ? __ldg(stats + 2 * row_of(4 * g + s) + 1) : 0.f;
       }
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        float delta = 0.f, norm = 0.f;
+        delta[s] = norm[s] = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float& w = v[s0 + s][i];
+          float& w = v[4 * g + s][i];
           w *= stat_inv[s];
-          delta = fmaf(w, o[s][i], delta);
-          norm = fmaf(w, w, norm);
+          delta[s] = fmaf(w, o[s][i], delta[s]);
+          norm[s] = fmaf(w, w, norm[s]);
         }
-#pragma unroll
-        for (int k = kAcross / 2; k > 0; k >>= 1) { delta += __shfl_xor_sync(0xffffffffu, delta, k); norm += __shfl_xor_sync(0xffffffffu, norm, k); }
-        const bool leaves = !(norm > 1e-30f && norm < 1e37f);            // the squares leave the numbers' range, or are zero
-        norm = sqrtf(norm);
-        if (__any_sync(0xffffffffu, leaves)) {   // a bound in its place
-          float top = 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(v[s0 + s][i]));
-#pragma unroll
-          for (int k = kAcross / 2; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-          if (leaves) norm = fminf(top * sqrtf((float)D), 3e38f);
-        }
-        if (!(fabsf(delta) < INFINITY && norm < INFINITY && fabsf(stat_max[s]) < INFINITY && fabsf(stat_inv[s]) < INFINITY)) {
-          unfit |= 1u << (s0 + s);
-          stat_max[s] = delta = norm = 0.f;
-        }
-        if (col == 0) {
-          const int64_t at = ((int64_t)bh * job.tiles + tile) * kTile + row_of(s0 + s);
-          p.row_max[at] = stat_max[s]; p.row_delta[at] = delta; p.row_norm[at] = norm;
-        }
-        most_norm = fmaxf(most_norm, norm); most_delta = fmaxf(most_delta, fabsf(delta));
       }
+      own_delta[g] = joined<kAcross>(delta, add);
+      own_norm[g] = joined<kAcross>(norm, add);
+    }
+  }
+  float most = 0.f, least = INFINITY;
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    float top[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      bool fine = true;
+      top[s] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float& w = v[4 * g + s][i];
+        if (!(fabsf(w) < INFINITY)) { w = 0.f; fine = false; }
+        top[s] = fmaxf(top[s], fabsf(w));
+      }
+      if (!fine) atomicOr(&bad_words[row_of(4 * g + s) >> 5], 1u << (row_of(4 * g + s) & 31));
+    }
+    own_top[g] = joined<kAcross>(top, larger);
+    most = fmaxf(most, own_top[g]);
+    if (own_top[g] > 0.f) least = fminf(least, own_top[g]);
+    if (job.gradient) {
+      const int r = own_row(g);
+      // where squares leave the numbers' range, a bound
+      float norm = own_norm[g] > 1e-30f && own_norm[g] < 1e37f ? sqrtf(own_norm[g]) : fminf(own_top[g] * sqrtf((float)D), 3e38f);
+      if (!(fabsf(own_delta[g]) < INFINITY && fabsf(own_max[g]) < INFINITY)) {
+        atomicOr(&bad_words[r >> 5], 1u << (r & 31));
+        own_max[g] = own_delta[g] = norm = 0.f;
+      }
+      if (lane % kShare == 0) {
+        const int64_t at = ((int64_t)bh * job.tiles + tile) * kTile + r;
+        p.row_max[at] = own_max[g]; p.row_delta[at] = own_delta[g]; p.row_norm[at] = norm;
+      }
+      most_norm = fmaxf(most_norm, norm); most_delta = fmaxf(most_delta, fabsf(own_delta[g]));
     }
   }
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    const int r = row_of(s);
-    bool fine = !((unfit >> s) & 1u);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (!(fabsf(v[s][i]) < INFINITY)) { v[s][i] = 0.f; fine = false; }
-      most = fmaxf(most, fabsf(v[s][i]));
-    }
-    if (!fine) atomicOr(&bad_words[r >> 5], 1u << (r & 31));
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
+  for (int o = 16; o >= kShare; o >>= 1) {
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    most_norm = fmaxf(most_norm, __shfl_xor_sync(0xffffffffu, most_norm, o));
-    most_delta = fmaxf(most_delta, __shfl_xor_sync(0xffffffffu, most_delta, o));
+    least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
   }
-  if (lane == 0) { red[warp] = most; red_norm[warp] = most_norm; red_delta[warp] = most_delta; }
+  if (job.gradient) {
+#pragma unroll
+    for (int o = 16; o >= kShare; o >>= 1) {
+      most_norm = fmaxf(most_norm, __shfl_xor_sync(0xffffffffu, most_norm, o));
+      most_delta = fmaxf(most_delta, __shfl_xor_sync(0xffffffffu, most_delta, o));
+    }
+  }
+  if (lane == 0) { red[warp] = most; red_least[warp] = least; red_norm[warp] = most_norm; red_delta[warp] = most_delta; }
   __syncthreads();
-  most = red[lane & (kPackWarps - 1)]; most_norm = red_norm[lane & (kPackWarps - 1)]; most_delta = red_delta[lane & (kPackWarps - 1)];
+  most = red[lane & (kPackWarps - 1)]; least = red_least[lane & (kPackWarps - 1)]; most_norm = red_norm[lane & (kPackWarps - 1)]; most_delta = red_delta[lane & (kPackWarps - 1)];
 #pragma unroll
   for (int o = kPackWarps / 2; o > 0; o >>= 1) {
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
     most_norm = fmaxf(most_norm, __shfl_xor_sync(0xffffffffu, most_norm, o));
     most_delta = fmaxf(most_delta, __shfl_xor_sync(0xffffffffu, most_delta, o));
   }
-  // max * scale in [2^14, 2^15); subnormal maxima, and those from 2^126, as far as the scale and its reciprocal are normal numbers
-  const int e = most > 0.f ? min(126, max(-126, 14 - exponent_of(most))) : 0;
-  const float scale = power_of_two(e);
+  const bool apart = most > 0.f && exponent_of(most) - exponent_of(least) > (job.gradient ? kOrdersOfGradient : kOrders);
+  const int e = scale_exponent(most);
+  const int64_t at_tile = (int64_t)bh * job.tiles + tile;
+  if (lane % kShare == 0) {
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const int of_token = apart ? scale_exponent(own_top[g]) : e;
+      token_scale[own_row(g)] = power_of_two(of_token);                // its warp's rows
+      job.scale[at_tile * kTile + own_row(g)] = apart && own_top[g] == 0.f ? 0.f : power_of_two(-of_token);
+    }
+  }
   if (threadIdx.x == 0) {
-    TileInfo& info = job.info[(int64_t)bh * job.tiles + tile];
-    info.inv = power_of_two(-e); info.top = most; info.norm = most_norm; info.delta = most_delta;
+    TileInfo& info = job.info[at_tile];
+    info.inv = apart ? -1.f : power_of_two(-e); info.top = most; info.norm = most_norm; info.delta = most_delta;
 #pragma unroll
     for (int i = 0; i < 4; ++i) info.bad[i] = bad_words[i];
   }
-  char* const image = job.image + ((int64_t)bh * job.tiles + tile) * (2 * G * 16384);
+  __syncwarp();
+  char* const image = job.image + at_tile * (2 * G * 16384);
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
     const int r = row_of(s);
+    const float scale = apart ? token_scale[r] : power_of_two(e);
     float hi[4], x[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) { x[i] = v[s][i] * scale; hi[i] = __half2float(__float2half_rn(x[i])); }
@@ -310,7 +359,7 @@ template <int KIND, int G> struct Shape {
   static constexpr bool kRowsInTmem = !kTwo || G == 1;
   static constexpr int kPart = G * 16384;                            // one half (hi or lo) of a tile
   static constexpr int kResident = (kTwo ? 2 : 0) * kPart + (kRowsInTmem ? 0 : 2) * kPart;
-  static constexpr int kControl = 768 + (KIND == kFwd ? 1024 : 0) + (kRowsAreKeys ? 2048 : 0);
+  static constexpr int kControl = 768 + (KIND == kFwd ? 1024 : 0) + (kRowsAreKeys ? 2048 : 0) + (kTwo ? 256 : 0);
   static constexpr int kFits = (232448 - kControl - kResident) / kPart, kStages = kFits < 8 ? kFits : 8;
   static constexpr int kSmem = kResident + kStages * kPart + kControl;
   // TMEM columns: scores 0 and 128, then
@@ -324,7 +373,7 @@ template <int KIND, int G> struct Shape {
 // Of one tile of columns, for the warps: written by the copying warp, which walks the list.  Eight of them in turn: by the time a copy for tile n + 8 can be issued,
 // the weights of tile n + 4 have been made.
 struct __align__(16) Entry {
-  int flags, head, col, at;                      // 1: there is a tile, 2: every row sees all of it, and all of it is finite; position of its first column; its number, or behind the last how many there were
+  int flags, head, col, at;                      // 1: there is a tile, 2: every row sees all of it, and all of it is finite, 4: its tokens or the rows have scales of their own; position of its first column; its number, or behind the last how many there were
   float inv1, inv2, x, y;                        // 1 / scale of both operands; dq: largest magnitude of V, dk: largest norm and |D'| of dO'
 };
 
@@ -367,9 +416,18 @@ __device__ __forceinline__ void tanh32(float* t) {
   }
 }
 // g z less m, g z rounded as the maximum m was: the largest score is 0 then, in both directions, however large it is.  In one rounding it would be what rounding m took off, 2^8 for
-// a score of 2^32 (and the compiler makes one rounding of a packed product and a sum behind it).  Shaped scores are whole, their g is 1.
-template <bool SHAPED> __device__ __forceinline__ float2 less(float2 z, float g, float2 m) {
-  return add2(SHAPED ? z : make_float2(__fmul_rn(z.x, g), __fmul_rn(z.y, g)), make_float2(-m.x, -m.y));
+// a score of 2^32.  `one` is 1 where the compiler does not see it, which makes one rounding of a packed product and a sum behind it.  Shaped scores are whole, their g is 1.
+template <bool SHAPED> __device__ __forceinline__ float2 less(float2 z, float g, float2 m, float one) {
+  const float2 n = make_float2(-m.x, -m.y);
+  return SHAPED ? add2(z, n) : fma2(mul2(z, both(g)), both(one), n);
+}
+// 32 numbers times `by` and a scale each, a power of two or zero; no sum behind it takes in the rounding
+__device__ __forceinline__ void times32(float* z, const float* __restrict__ scale, float by) {
+#pragma unroll
+  for (int k = 0; k < 32; k += 4) {
+    const float4 f = __ldg(reinterpret_cast<const float4*>(scale + k));
+    z[k] = __fmul_rn(z[k], f.x * by); z[k + 1] = __fmul_rn(z[k + 1], f.y * by); z[k + 2] = __fmul_rn(z[k + 2], f.z * by); z[k + 3] = __fmul_rn(z[k + 3], f.w * by);
+  }
 }
 // hi and lo halves of 32 weights, as the A operand has them: 16 weights are 8 words of hi and 8 of lo
 __device__ __forceinline__ void split32(const float* w, uint32_t* words) {
@@ -419,12 +477,14 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
   uint64_t* const columns_full = o_empty + 2;    // [2] maxima and D' of a tile of queries
   uint64_t* const merge = columns_full + 2;      // the second group's sums are in shared memory
   uint64_t* const rows_full = merge + 1;         // the rows are in TMEM
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(rows_full + 1);
+  uint64_t* const swap_full = rows_full + 1;     // both groups' largest weights of every row are in shared memory
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(swap_full + 1);
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   Entry* const entries = reinterpret_cast<Entry*>(full + 64);        // [8]
   float* const statistics = reinterpret_cast<float*>(entries + 8);   // fwd: [2][128] of the second group
   float* const columns = statistics;                                 // dk, dv: [2][2][128]
-  static_assert(8 + 8 + 8 + 1 + 7 * 2 + 2 + 2 <= 64, "barriers fit");
+  uint8_t* const swapped = reinterpret_cast<uint8_t*>(columns + (S::kRowsAreKeys ? 512 : 0));            // dq, dk: [2][128] exponents of the groups' largest weights
+  static_assert(8 + 8 + 8 + 1 + 7 * 2 + 3 + 2 <= 64, "barriers fit");
   const AttentionArgs& a = p.a;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
@@ -439,7 +499,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
         mbar_init(o_full + i, 1); mbar_init(o_empty + i, S::kWeightWarps);
         mbar_init(columns_full + i, 1);
       }
-      mbar_init(merge, 4); mbar_init(rows_full, 8);
+      mbar_init(merge, 4); mbar_init(rows_full, 8); mbar_init(swap_full, 8);
       *abort_flag = (smem_u32(smem) & 1023u) ? 1 : 0;                // nothing is issued then
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -482,8 +542,9 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
       rows_armed = true;
     }
     Walk<KIND> walk(p, b, row_head, share, tile);
+    const bool rows_apart = r1.info[row_at].inv < 0.f || (kTwo && r2.info[row_at].inv < 0.f);
     // What an entry says is asked for a tile ahead
-    struct Next { bool there, all; int head, t; int64_t at; float inv1, inv2, x, y; uint32_t spoils; };
+    struct Next { bool there, all, apart; int head, t; int64_t at; float inv1, inv2, x, y; uint32_t spoils; };
     const auto look_ahead = [&] {
       Next x;
       x.there = walk.next(lane, x.head, x.t, x.all);
@@ -491,6 +552,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
       const TileInfo &i1 = c1.info[x.at], &i2 = c2.info[x.at];
       x.inv1 = i1.inv; x.inv2 = i2.inv; x.x = KIND == kDq ? i2.top : i2.norm; x.y = i2.delta;
       const uint4 u = *reinterpret_cast<const uint4*>(i1.bad), w = *reinterpret_cast<const uint4*>(i2.bad);
+      x.apart = rows_apart || fminf(x.inv1, x.inv2) < 0.f;
       x.spoils = u.x | u.y | u.z | u.w | w.x | w.y | w.z | w.w;
       return x;
     };
@@ -515,7 +577,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     for (int n = 0;; ++n) {
       const Next now = next;
       if (lane == 0) {
-        entries[n & 7] = Entry{now.there ? 1 | (int)(now.all && now.spoils == 0u) << 1 : 0, now.head, now.t * kTile + (kRowsAreKeys ? a.Tk - a.Tq : 0), now.there ? (int)now.at : n, now.inv1, now.inv2, now.x, now.y};
+        entries[n & 7] = Entry{now.there ? 1 | (int)(now.all && now.spoils == 0u) << 1 | (int)now.apart << 2 : 0, now.head, now.t * kTile + (kRowsAreKeys ? a.Tk - a.Tq : 0), now.there ? (int)now.at : n, now.inv1, now.inv2, now.x, now.y};
         mbar_arrive(entry_full + (n & 7));
       }
       __syncwarp();
@@ -685,7 +747,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     const bool careful = __any_sync(0xffffffffu, spoiled);
     const bool cap = SHAPED && a.cap > 0.f;
     const float inv2 = kTwo ? r2.info[row_at].inv : 0.f;
-    const float unit = info1.inv * (cap ? a.scale / a.cap : a.scale * kLog2e), wide = cap ? a.cap * kLog2e : 1.f;
+    const float by = cap ? a.scale / a.cap : a.scale * kLog2e, unit = info1.inv * by, wide = cap ? a.cap * kLog2e : 1.f;           // rows with scales of their own: see below
     float row_max = 0.f, row_delta = 0.f, row_norm = 0.f;
     if (KIND == kDq) { row_max = p.row_max[row_at * kTile + row]; row_delta = p.row_delta[row_at * kTile + row]; row_norm = p.row_norm[row_at * kTile + row] * sqrtf((float)a.D); }
     const float norm_top = KIND == kDk ? r2.info[row_at].top * sqrtf((float)a.D) : 0.f;
@@ -699,6 +761,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     float alpha = 1.f, out_factor = 0.f;                               // of the product in flight
     float slope = 0.f;
     int slope_head = -1;
+    uint32_t swaps = 0;                                                // dq, dk
 
     const auto arrive = [&](uint64_t* bar) { tcgen05_fence_before(); __syncwarp(); if (lane == 0) mbar_arrive(bar); };
     const auto wait_for = [&](uint64_t* bar, uint32_t parity) { await(bar, parity, abort_flag, bad); __syncwarp(); tcgen05_fence_after(); };
@@ -721,72 +784,82 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     };
 
     int n = kTurns ? group : 0;
-    for (;; n += kTurns ? 2 : 1) {
-      await(entry_full + (n & 7), (n >> 3) & 1, abort_flag, bad);
-      bad = __any_sync(0xffffffffu, bad);
-      const Entry now = entries[n & 7];
-      if (bad || !(now.flags & 1)) break;
-      if (kTurns && n >= 2) add_up(n - 2);       // while the scores are being made
-      const float f = now.inv1 * unit;
-      if (SHAPED && a.slopes && slope_head != (kRowsAreKeys ? now.head : row_head)) {
-        slope_head = kRowsAreKeys ? now.head : row_head;
-        slope = __ldg(a.slopes + slope_head) * kLog2e;
+    constexpr int kStep = kTurns ? 2 : 1;
+    const int at_row = kRowsAreKeys ? self : self + off;
+    // of the tile at hand
+    Entry now = {};
+    int col0 = 0;                                 // position of the first column
+    bool masked = false;
+    uint32_t from = 0;
+    float theirs[S::kChunks] = {};                  // a column's document in every lane
+    // scores of a chunk of 32 columns, capped and biased, in units of log 2; turned: 1 - the cap's tanh squared
+    const auto shape32 = [&](float* z, float* turned, int c, float by) {
+#pragma unroll
+      for (int k = 0; k < 32; k += 2) put2(z, k, mul2(at2(z, k), both(by)));
+      if (cap) {
+        tanh32(z);
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) {
+          const float2 t = at2(z, k);
+          if (turned) put2(turned, k, fma2(mul2(t, both(-1.f)), t, both(1.f)));
+          put2(z, k, mul2(t, both(wide)));
+        }
+      } else if (turned) {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) turned[k] = 1.f;
       }
-      const int col0 = now.col + col_part;       // position of the first column
-      const int at_row = kRowsAreKeys ? self : self + off;
-      const bool masked = !(now.flags & 2) || careful;
-      const uint32_t from = mine + (n & 1) * 128 + col_part;
-      // scores of a chunk of 32 columns, capped and biased, in units of log 2; turned: 1 - the cap's tanh squared
-      const auto shape32 = [&](float* z, float* turned, int c) {
+      if (a.slopes) {
+        const float away = (float)(at_row - (col0 + 32 * c));
 #pragma unroll
-        for (int k = 0; k < 32; k += 2) put2(z, k, mul2(at2(z, k), both(f)));
-        if (cap) {
-          tanh32(z);
-#pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            const float2 t = at2(z, k);
-            if (turned) put2(turned, k, fma2(mul2(t, both(-1.f)), t, both(1.f)));
-            put2(z, k, mul2(t, both(wide)));
-          }
-        } else if (turned) {
-#pragma unroll
-          for (int k = 0; k < 32; ++k) turned[k] = 1.f;
-        }
-        if (a.slopes) {
-          const float away = (float)(at_row - (col0 + 32 * c));
-#pragma unroll
-          for (int k = 0; k < 32; ++k) z[k] = fmaf(-slope, fabsf(away - (float)k), z[k]);
-        }
-      };
-      // hides the columns of a chunk that the row does not see, and makes NaN of those that are not finite
-      float theirs[S::kChunks];                  // a column's document in every lane, asked for while the scores are being made
-      if (p.documents && masked) {
-#pragma unroll
-        for (int c = 0; c < S::kChunks; ++c) theirs[c] = document_of(a, b, col0 + 32 * c + lane);
+        for (int k = 0; k < 32; ++k) z[k] = fmaf(-slope, fabsf(away - (float)k), z[k]);
       }
-      const auto mask32 = [&](float* z, int c, float hidden) {
-        const int first = col0 + 32 * c;
-        uint32_t seen = bits_between(lo - first, hi - first) | bits_between(-1, extra - 1 - first);
-        if (p.documents) {
-          uint32_t same = 0u;
-          float of = theirs[0];
+    };
+    // hides the columns of a chunk that the row does not see, and makes NaN of those that are not finite
+    const auto mask32 = [&](float* z, int c, float hidden) {
+      const int first = col0 + 32 * c;
+      uint32_t seen = bits_between(lo - first, hi - first) | bits_between(-1, extra - 1 - first);
+      if (p.documents) {
+        uint32_t same = 0u;
+        float of = theirs[0];
 #pragma unroll
-          for (int i = 1; i < S::kChunks; ++i) of = c == i ? theirs[i] : of;
+        for (int i = 1; i < S::kChunks; ++i) of = c == i ? theirs[i] : of;
 #pragma unroll
-          for (int k = 0; k < 32; ++k) same |= __shfl_sync(0xffffffffu, of, k) == document ? 1u << k : 0u;
-          seen &= document >= 0.f ? same : 0u;
-        }
-        const uint32_t spoils = seen & (spoiled ? 0xffffffffu : c1.info[now.at].bad[col_part / 32 + c] | c2.info[now.at].bad[col_part / 32 + c]);
+        for (int k = 0; k < 32; ++k) same |= __shfl_sync(0xffffffffu, of, k) == document ? 1u << k : 0u;
+        seen &= document >= 0.f ? same : 0u;
+      }
+      const uint32_t spoils = seen & (spoiled ? 0xffffffffu : c1.info[now.at].bad[col_part / 32 + c] | c2.info[now.at].bad[col_part / 32 + c]);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) z[k] = (seen >> k) & 1u ? z[k] : hidden;
-        if (__builtin_expect(spoils != 0u, 0)) {
+      for (int k = 0; k < 32; ++k) z[k] = (seen >> k) & 1u ? z[k] : hidden;
+      if (__builtin_expect(spoils != 0u, 0)) {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) if ((spoils >> k) & 1u) z[k] = NAN;
-        }
-      };
+        for (int k = 0; k < 32; ++k) if ((spoils >> k) & 1u) z[k] = NAN;
+      }
+    };
 
-      wait_for(&s_full[n & 1], (n >> 1) & 1);
-      if (KIND == kFwd) {
+    for (;;) {
+      bool apart = false;
+      // Tiles whose tokens share a scale: nothing else in this loop, which the instruction cache is small for
+      for (;; n += kStep) {
+        await(entry_full + (n & 7), (n >> 3) & 1, abort_flag, bad);
+        bad = __any_sync(0xffffffffu, bad);
+        now = entries[n & 7];
+        if (bad || !(now.flags & 1)) break;
+        if (kTurns && n >= 2) add_up(n - 2);     // while the scores are being made
+        if (SHAPED && a.slopes && slope_head != (kRowsAreKeys ? now.head : row_head)) {
+          slope_head = kRowsAreKeys ? now.head : row_head;
+          slope = __ldg(a.slopes + slope_head) * kLog2e;
+        }
+        col0 = now.col + col_part;
+        masked = !(now.flags & 2) || careful;
+        from = mine + (n & 1) * 128 + col_part;
+        if (p.documents && masked) {             // asked for while the scores are being made
+#pragma unroll
+          for (int c = 0; c < S::kChunks; ++c) theirs[c] = document_of(a, b, col0 + 32 * c + lane);
+        }
+        wait_for(&s_full[n & 1], (n >> 1) & 1);
+        if (now.flags & 4) { apart = true; break; }
+        const float f = now.inv1 * unit;
+        if (KIND == kFwd) {
         // Scores that are not plain products are written back, so that both passes read them
         const bool rewritten = SHAPED || masked || f < 0.f;
         float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -796,7 +869,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
           tmem_ld32(from + 32 * c, z);
           tmem_ld_wait();
           if (__builtin_expect(rewritten, SHAPED)) {
-            if (SHAPED) shape32(z, nullptr, c);
+            if (SHAPED) shape32(z, nullptr, c, f);
             else
 #pragma unroll
               for (int k = 0; k < 32; ++k) z[k] *= f;
@@ -821,7 +894,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
           tmem_ld_wait();
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
-            const float2 e = less<SHAPED>(at2(z, k), g, both(base)), w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+            const float2 e = less<SHAPED>(at2(z, k), g, both(base), p.one), w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
             s[(k >> 1) & 1] = add2(s[(k >> 1) & 1], w);
             put2(z, k, mul2(w, both(kWeightScale)));
           }
@@ -855,14 +928,14 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
           if (kTwo) tmem_ld32(mine + S::kYAt + col_part + 32 * c, y);
           tmem_ld_wait();
           if (kTwo && c == S::kChunks - 1) arrive(&y_empty[n & 1]);
-          if (SHAPED) shape32(z, kTwo ? turned : nullptr, c);
+          if (SHAPED) shape32(z, kTwo ? turned : nullptr, c, f);
           const float g = SHAPED ? 1.f : f;
           if (kRowsAreKeys) {
 #pragma unroll
             for (int k = 0; k < 32; k += 4) {
               const float4 m4 = *reinterpret_cast<const float4*>(col_max + 32 * c + k);
-              put2(z, k, less<SHAPED>(at2(z, k), g, make_float2(m4.x, m4.y)));
-              put2(z, k + 2, less<SHAPED>(at2(z, k + 2), g, make_float2(m4.z, m4.w)));
+              put2(z, k, less<SHAPED>(at2(z, k), g, make_float2(m4.x, m4.y), p.one));
+              put2(z, k + 2, less<SHAPED>(at2(z, k + 2), g, make_float2(m4.z, m4.w), p.one));
               if (KIND == kDk) {
                 const float4 d4 = *reinterpret_cast<const float4*>(col_delta + 32 * c + k);
                 put2(y, k, fma2(at2(y, k), both(fy), make_float2(-d4.x, -d4.y)));
@@ -872,7 +945,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
           } else {
             const float delta = row_delta * lift;
 #pragma unroll
-            for (int k = 0; k < 32; k += 2) { put2(z, k, less<SHAPED>(at2(z, k), g, both(row_max))); put2(y, k, fma2(at2(y, k), both(fy), both(-delta))); }
+            for (int k = 0; k < 32; k += 2) { put2(z, k, less<SHAPED>(at2(z, k), g, both(row_max), p.one)); put2(y, k, fma2(at2(y, k), both(fy), both(-delta))); }
           }
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
@@ -890,7 +963,95 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
         arrive(&w_full[n & 1]);
         if (!kTurns && n >= 1) add_up(n - 1);
         out_factor = factor;
+        }
       }
+      if (!apart) break;
+      // Tokens of different sizes, among the columns or the rows.  Their scales go into the scores and, those of the product's operand, into the weights, which are held in TMEM until the largest of their row is known
+      // and scales them: so no token costs a bit of what does not depend on it.
+      const float row_unit = r1.scale[row_at * kTile + row] * by, row_inv2 = kTwo ? r2.scale[row_at * kTile + row] : 0.f;
+      const float *const scale1 = c1.scale + (int64_t)now.at * kTile + col_part, *const scale2 = c2.scale + (int64_t)now.at * kTile + col_part;
+      const float *const col_max = columns + (n & 1) * 256 + col_part, *const col_delta = col_max + 128;
+      if (kRowsAreKeys) await(&columns_full[n & 1], (n >> 1) & 1, abort_flag, bad);
+      if (kTwo) wait_for(&y_full[n & 1], (n >> 1) & 1);
+      float at_most = most;
+#pragma unroll 1
+      for (int c = 0; c < (KIND == kFwd ? S::kChunks : 0); ++c) {      // the maximum first
+        float z[32];
+        tmem_ld32(from + 32 * c, z);
+        tmem_ld_wait();
+        times32(z, scale1 + 32 * c, row_unit);
+        if (SHAPED) shape32(z, nullptr, c, 1.f);
+        if (masked) mask32(z, c, -INFINITY);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) at_most = fmaxf(at_most, z[k]);
+        tmem_st32(from + 32 * c, reinterpret_cast<const uint32_t*>(z));
+      }
+      if (KIND == kFwd) tmem_st_wait();
+      const float base = max_of_finite_or(at_most);
+      float s = 0.f, heaviest = 0.f;
+#pragma unroll 1
+      for (int c = 0; c < S::kChunks; ++c) {
+        float z[32], other[kTwo ? 32 : 1];       // the cap's derivatives, then the second scores
+        tmem_ld32(from + 32 * c, z);
+        tmem_ld_wait();
+        if (KIND != kFwd) {
+          times32(z, scale1 + 32 * c, row_unit);
+          if (SHAPED) shape32(z, kTwo ? other : nullptr, c, 1.f);
+        }
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {           // scores above the row's statistics: another kernel's forward call rounded them otherwise
+          z[k] = exp2_fast(KIND == kFwd ? z[k] - base : fminf(z[k] - (kRowsAreKeys ? col_max[32 * c + k] : row_max), 0.f));
+          if (KIND == kFwd) s += z[k];
+        }
+        if (kTwo) {
+          if (SHAPED)
+#pragma unroll
+            for (int k = 0; k < 32; ++k) z[k] *= other[k];
+          tmem_ld32(mine + S::kYAt + col_part + 32 * c, other);
+          tmem_ld_wait();
+          times32(other, scale2 + 32 * c, row_inv2);
+#pragma unroll
+          for (int k = 0; k < 32; ++k) z[k] *= other[k] - (kRowsAreKeys ? col_delta[32 * c + k] : row_delta);
+        }
+        times32(z, (kTwo ? scale1 : scale2) + 32 * c, 1.f);
+        if (KIND != kFwd && masked) mask32(z, c, 0.f);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) heaviest = fmaxf(heaviest, fabsf(z[k]));
+        tmem_st32(from + 32 * c, reinterpret_cast<const uint32_t*>(z));
+      }
+      tmem_st_wait();
+      int e = (int)(__float_as_uint(heaviest) >> 23);
+      if (kTwo) {                                // the groups have half of the row's weights each
+        swapped[group * kTile + row] = (uint8_t)e;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(swap_full);
+        await(swap_full, swaps++ & 1, abort_flag, bad);
+        __syncwarp();
+        e = max(e, (int)swapped[(group ^ 1) * kTile + row]);
+        arrive(&y_empty[n & 1]);                 // behind it, so that nobody is at the next tile's exchange before
+      }
+      const int shift = min(126, max(-126, kWeightExp + 127 - e));
+#pragma unroll 1
+      for (int c = 0; c < S::kChunks; ++c) {
+        float z[32];
+        uint32_t words[32];
+        tmem_ld32(from + 32 * c, z);
+        tmem_ld_wait();
+#pragma unroll
+        for (int k = 0; k < 32; ++k) z[k] *= power_of_two(shift);
+        split32(z, words);
+        tmem_st32(from + 32 * c, words);
+      }
+      tmem_st_wait();
+      arrive(&w_full[n & 1]);
+      if (KIND == kFwd) {
+        alpha = exp2_fast(most - base);
+        most = at_most;
+        sum = fmaf(sum, alpha, s);
+      }
+      if (!kTurns && n >= 1) add_up(n - 1);
+      out_factor = power_of_two(-shift);
+      n += kStep;
     }
     if (n >= (kTurns ? 2 : 1)) add_up(n - (kTurns ? 2 : 1));           // n: where the list ends for this warp
 
@@ -1053,10 +1214,11 @@ static size_t lay_out(const AttentionArgs& a, bool backward, char* base, PackArg
     const size_t n = queries ? nq : nk;
     char* const img = take(n * image);
     char* const info = take(n * sizeof(TileInfo));
+    char* const scale = take(n * kTile * sizeof(float));
     if (base) {
-      pack->job[j] = PackJob{from[j], img, (TileInfo*)info, queries ? a.H : a.G, queries ? a.Tq : a.Tk, queries ? q_tiles : k_tiles, j == 3};
+      pack->job[j] = PackJob{from[j], img, (TileInfo*)info, (float*)scale, queries ? a.H : a.G, queries ? a.Tq : a.Tk, queries ? q_tiles : k_tiles, j == 3};
       pack->first[j] = blocks;
-      *to[j] = Packed{img, (const TileInfo*)info};
+      *to[j] = Packed{img, (const TileInfo*)info, (const float*)scale};
     }
     blocks += (int)n;
   }
@@ -1070,7 +1232,7 @@ static size_t lay_out(const AttentionArgs& a, bool backward, char* base, PackArg
     pack->a = a; pack->jobs = jobs; pack->first[jobs] = blocks; pack->document_job = 1;
     pack->row_max = (float*)rows[0]; pack->row_delta = (float*)rows[1]; pack->row_norm = (float*)rows[2]; pack->documents = (float4*)docs;
     tc->a = a; tc->row_max = pack->row_max; tc->row_delta = pack->row_delta; tc->row_norm = pack->row_norm; tc->documents = pack->documents;
-    tc->q_tiles = q_tiles; tc->k_tiles = k_tiles; tc->D16 = (a.D + 15) / 16 * 16; tc->err = tensor_error_word();
+    tc->q_tiles = q_tiles; tc->k_tiles = k_tiles; tc->D16 = (a.D + 15) / 16 * 16; tc->err = tensor_error_word(); tc->one = 1.f;
     tc->shares = shares; tc->dk_part = (float*)dk_part; tc->dv_part = (float*)dv_part;
   }
   return at;
