@@ -180,7 +180,7 @@ def among_others(alone, lead, tail, seed=1):
 
 
 @pytest.mark.parametrize("size", [2.0 ** 13, 2.0 ** 20, 2.0 ** 40, 2.0 ** 100, 2.0 ** -20])
-@pytest.mark.parametrize("where", ["q", "k", "all"])
+@pytest.mark.parametrize("where", ["q", "k", "v", "all"])
 @pytest.mark.parametrize("kind", KINDS, ids=IDS)
 def test_other_documents_of_any_size_cost_nothing(env, path, kind, where, size):
     alone = Fine(1, 140, 140, seed=3, **kind)
@@ -264,3 +264,23 @@ def test_sequences_and_heads_of_any_size_side_by_side(env, path, dim, shared):
             within(g[260 * b:260 * (b + 1)], w[260 * b:260 * (b + 1)], e[260 * b:260 * (b + 1)], name)
         if not shared:
             within(view(g), view(w), view(e), name)
+
+
+# ---- gradients of different sizes -------------------------------------------------------------------
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+def test_a_document_of_smaller_gradients_keeps_its_bits(env, path, kind):
+    """Output gradients of the others up to 2^50 larger."""
+    alone = Fine(1, 140, 140, seed=3, **kind)
+    want, bound = alone.bounds()
+    for size in (2.0 ** 5, 2.0 ** 10, 2.0 ** 13, 2.0 ** 17, 2.0 ** 20, 2.0 ** 50):
+        c, mine, others = among_others(alone, 60, 75)
+        c.dout[others] *= np.float32(size)
+        check([g[mine] for g in run(env, c)], want, bound)
+
+
+@pytest.mark.parametrize("kind", KINDS[:4], ids=IDS)
+def test_later_queries_of_smaller_gradients(env, path, kind):
+    """Each query's output gradient half of the one's before: the last keys are seen by the smallest alone."""
+    c = Fine(1, 100, 100, seed=8, **dict(kind, causal=True))
+    c.dout *= (2.0 ** -np.arange(100)).astype(np.float32)[:, None]
+    check(run(env, c), *c.bounds())

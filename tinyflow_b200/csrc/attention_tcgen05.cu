@@ -56,6 +56,7 @@ struct __align__(16) TileInfo {
   float inv, top;                                // 1 / scale; negative where every token has one of its own; largest finite magnitude
   float norm, delta;                             // dO': largest row norm and |D'|
   uint32_t bad[4];                               // tokens with values that are not finite
+  float low, unused[3];                          // dO': smallest row norm that is not zero
 };
 struct Packed { const char* image; const TileInfo* info; const float* scale; };           // 1 / scale of every token; 0 for tokens of zeros among others with scales of their own
 struct TcArgs {
@@ -111,6 +112,8 @@ template <int kAcross, class F> __device__ __forceinline__ float joined(const fl
 // token's own, and the scale of the gradients' weights, which goes by the largest value, 8 bits of 25 to spare.  Output gradients over their row's sum, which differ by as much as the
 // sums do, up to the number of keys: 14 orders leave 2^-25.
 constexpr int kOrders = 8, kOrdersOfGradient = 14;
+// Of the weights of dk below the bound that scales them: a weight is held to 2^-39 of that, and what scales it is about 2^4 above the largest of them.
+constexpr int kOrdersOfBound = 7, kOrdersOfSeen = 10;
 // max * scale in [2^14, 2^15); subnormal maxima, and those from 2^126, as far as the scale and its reciprocal are normal numbers
 __device__ __forceinline__ int scale_exponent(float most) { return most > 0.f ? min(126, max(-126, 14 - exponent_of(most))) : 0; }
 
@@ -123,7 +126,7 @@ __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, F
   constexpr int kPackWarps = pack_threads(G, FEW) / 32;
   constexpr int kAcross = 16 * G, kRowsAtOnce = 32 / kAcross, kRowsOfWarp = kTile / kPackWarps, kSteps = kRowsOfWarp / kRowsAtOnce;
   constexpr int kShare = kAcross / 4, kGroups = kSteps / 4;            // of four steps' rows a lane looks after one, with kShare - 1 others
-  __shared__ float red[kPackWarps], red_least[kPackWarps], red_norm[kPackWarps], red_delta[kPackWarps], token_scale[kTile];
+  __shared__ float red[kPackWarps], red_least[kPackWarps], red_norm[kPackWarps], red_delta[kPackWarps], red_low[kPackWarps], token_scale[kTile];
   __shared__ uint32_t bad_words[4];
   grid_dep_sync();
   int j = 0;
@@ -134,7 +137,7 @@ __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, F
   const int D = p.a.D;
   if (threadIdx.x < 4) bad_words[threadIdx.x] = 0u;
   float v[kSteps][4];
-  float most_norm = 0.f, most_delta = 0.f;
+  float most_norm = 0.f, most_delta = 0.f, low = INFINITY;
   const auto load4 = [&](const float* from, int t, float* w) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = 0.f;
@@ -213,6 +216,7 @@ __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, F
         p.row_max[at] = own_max[g]; p.row_delta[at] = own_delta[g]; p.row_norm[at] = norm;
       }
       most_norm = fmaxf(most_norm, norm); most_delta = fmaxf(most_delta, fabsf(own_delta[g]));
+      if (norm > 0.f) low = fminf(low, norm);
     }
   }
 #pragma unroll
@@ -225,17 +229,19 @@ __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, F
     for (int o = 16; o >= kShare; o >>= 1) {
       most_norm = fmaxf(most_norm, __shfl_xor_sync(0xffffffffu, most_norm, o));
       most_delta = fmaxf(most_delta, __shfl_xor_sync(0xffffffffu, most_delta, o));
+      low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
     }
   }
-  if (lane == 0) { red[warp] = most; red_least[warp] = least; red_norm[warp] = most_norm; red_delta[warp] = most_delta; }
+  if (lane == 0) { red[warp] = most; red_least[warp] = least; red_norm[warp] = most_norm; red_delta[warp] = most_delta; red_low[warp] = low; }
   __syncthreads();
-  most = red[lane & (kPackWarps - 1)]; least = red_least[lane & (kPackWarps - 1)]; most_norm = red_norm[lane & (kPackWarps - 1)]; most_delta = red_delta[lane & (kPackWarps - 1)];
+  most = red[lane & (kPackWarps - 1)]; least = red_least[lane & (kPackWarps - 1)]; most_norm = red_norm[lane & (kPackWarps - 1)]; most_delta = red_delta[lane & (kPackWarps - 1)]; low = red_low[lane & (kPackWarps - 1)];
 #pragma unroll
   for (int o = kPackWarps / 2; o > 0; o >>= 1) {
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
     least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
     most_norm = fmaxf(most_norm, __shfl_xor_sync(0xffffffffu, most_norm, o));
     most_delta = fmaxf(most_delta, __shfl_xor_sync(0xffffffffu, most_delta, o));
+    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
   }
   const bool apart = most > 0.f && exponent_of(most) - exponent_of(least) > (job.gradient ? kOrdersOfGradient : kOrders);
   const int e = scale_exponent(most);
@@ -250,7 +256,7 @@ __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, F
   }
   if (threadIdx.x == 0) {
     TileInfo& info = job.info[at_tile];
-    info.inv = apart ? -1.f : power_of_two(-e); info.top = most; info.norm = most_norm; info.delta = most_delta;
+    info.inv = apart ? -1.f : power_of_two(-e); info.top = most; info.norm = most_norm; info.delta = most_delta; info.low = low;
 #pragma unroll
     for (int i = 0; i < 4; ++i) info.bad[i] = bad_words[i];
   }
@@ -543,6 +549,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     }
     Walk<KIND> walk(p, b, row_head, share, tile);
     const bool rows_apart = r1.info[row_at].inv < 0.f || (kTwo && r2.info[row_at].inv < 0.f);
+    const float rows_top = KIND == kDk ? r2.info[row_at].top * sqrtf((float)a.D) : 0.f;
     // What an entry says is asked for a tile ahead
     struct Next { bool there, all, apart; int head, t; int64_t at; float inv1, inv2, x, y; uint32_t spoils; };
     const auto look_ahead = [&] {
@@ -554,6 +561,9 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
       const uint4 u = *reinterpret_cast<const uint4*>(i1.bad), w = *reinterpret_cast<const uint4*>(i2.bad);
       x.apart = rows_apart || fminf(x.inv1, x.inv2) < 0.f;
       x.spoils = u.x | u.y | u.z | u.w | w.x | w.y | w.z | w.w;
+      // dk: one bound of the tile's queries scales the weights of all keys.  Where a key may see the smallest of them alone, and that is kOrdersOfBound below it, or where all see all,
+      // kOrdersOfSeen, the tile goes the way of tokens that are apart.
+      if (KIND == kDk && fmaf(x.x, rows_top, x.y) > (float)(1 << (x.all && x.spoils == 0u ? kOrdersOfSeen : kOrdersOfBound)) * (i2.low * rows_top)) x.apart = true;
       return x;
     };
     const auto load = [&](const Packed& from, int64_t at) {
