@@ -32,8 +32,11 @@ class OracleExecutor:
     def _turns(self, node, x, positions):
         from tinyflow_b200.gpu_op import rotary_frequencies
         of = dict(node.rotation)
-        layout, rotated = of.pop("layout", "half"), of.pop("rotated", None)
-        f, amplitude = rotary_frequencies(node.head_dim // 2 * 2 if rotated is None else rotated, **of)
+        layout, rotated, f, amplitude = of.pop("layout", "half"), of.pop("rotated", None), of.pop("frequencies", None), of.pop("amplitude", None)
+        usual = 1.0
+        if f is None:
+            f, usual = rotary_frequencies(node.head_dim // 2 * 2 if rotated is None else rotated, **of)
+        amplitude = usual if amplitude is None else amplitude
         return node.head_dim, ops.rotary_angles(x.shape[0], node.length, node.start, positions[0] if positions else None, f), amplitude, layout
 
     def _attended(self, node, ins):

@@ -540,11 +540,22 @@ def rotary_frequencies(rotated, base=10000.0, scaling="none", factor=1.0, traine
     return [v * (r + (1.0 - r) / factor) for v, r in zip(f, kept)], 1.0 + 0.1 * math.log(factor)
 
 
-def rotary_state(head_dim, rotated=None, layout="half", base=10000.0, scaling="none", factor=1.0, trained=0, low=1.0, high=32.0, state=None):
+def _turns(head_dim, rotated=None, base=10000.0, scaling="none", factor=1.0, trained=0, low=1.0, high=32.0, frequencies=None, amplitude=None):
+    if rotated is None:
+        rotated = head_dim // 2 * 2 if frequencies is None else 2 * len(frequencies)
+    if frequencies is None:
+        frequencies, usual = rotary_frequencies(rotated, base, scaling, factor, trained, low, high)
+    else:
+        assert rotated == 2 * len(frequencies) and scaling == "none", "frequencies are given, one of each pair"
+        frequencies, usual = [float(f) for f in frequencies], 1.0
+    return frequencies, usual if amplitude is None else amplitude
+
+
+def rotary_state(head_dim, rotated=None, layout="half", base=10000.0, scaling="none", factor=1.0, trained=0, low=1.0, high=32.0, state=None, frequencies=None, amplitude=None):
     """What the calls of this section take: heads of ``head_dim`` elements, the first ``rotated`` of them (None: as many as make pairs) turned, ``layout`` "half"
-    (pairs i and i + rotated / 2) or "interleaved" (2 i and 2 i + 1), frequencies as :func:`rotary_frequencies` makes them.  With ``state`` that one gets them."""
-    rotated = head_dim // 2 * 2 if rotated is None else rotated
-    f, amplitude = rotary_frequencies(rotated, base, scaling, factor, trained, low, high)
+    (pairs i and i + rotated / 2) or "interleaved" (2 i and 2 i + 1), frequencies and amplitude as :func:`rotary_frequencies` makes them, or those given: radians a
+    position of each pair, and a factor of what is turned.  With ``state`` that one gets them."""
+    f, amplitude = _turns(head_dim, rotated, base, scaling, factor, trained, low, high, frequencies, amplitude)
     state = new_cell(3) if state is None else state
     check_call(_LIB.TfRotaryState(int(head_dim), len(f), _code(_LAYOUT, layout), (ctypes.c_double * max(1, len(f)))(*f), _F(amplitude), state))
     return state
