@@ -520,6 +520,13 @@ _LAYOUT = {"half": 0, "interleaved": 1}
 _I64 = ctypes.c_int64
 
 
+def _i32(value, name):
+    """An int as the library has them: one that does not fit would arrive as another."""
+    if not -2 ** 31 <= value < 2 ** 31:
+        raise AssertionError("%s: %r does not fit 32 bits" % (name, value))
+    return int(value)
+
+
 def rotary_frequencies(rotated, base=10000.0, scaling="none", factor=1.0, trained=0, low=1.0, high=32.0):
     """([radians a position of each of ``rotated / 2`` pairs], amplitude).  ``scaling`` stretches positions by ``factor``: "linear" all pairs alike;
     "stretched" by a larger base, the last pair by the factor and the first not at all; "parts" pairs that turn less than ``low`` times within the ``trained``
@@ -557,7 +564,7 @@ def rotary_state(head_dim, rotated=None, layout="half", base=10000.0, scaling="n
     position of each pair, and a factor of what is turned.  With ``state`` that one gets them."""
     f, amplitude = _turns(head_dim, rotated, base, scaling, factor, trained, low, high, frequencies, amplitude)
     state = new_cell(3) if state is None else state
-    check_call(_LIB.TfRotaryState(int(head_dim), len(f), _code(_LAYOUT, layout), (ctypes.c_double * max(1, len(f)))(*f), _F(amplitude), state))
+    check_call(_LIB.TfRotaryState(_i32(head_dim, "head_dim"), len(f), _code(_LAYOUT, layout), (ctypes.c_double * max(1, len(f)))(*f), _F(amplitude), state))
     return state
 
 
@@ -587,7 +594,7 @@ def head_norm_rotary_backward(query, key, gamma_query, gamma_key, positions, dqu
 def attention_state(length, heads, kv_heads, causal=True, window=0, scale=1.0, cap=0.0, state=None):
     """What both attention calls take: sequences of ``length`` queries, heads, what a query sees, scale and cap of the scores.  With ``state`` that one gets them."""
     state = new_cell(3) if state is None else state
-    check_call(_LIB.TfAttentionState(_I64(length), int(heads), int(kv_heads), int(bool(causal)), int(window), _F(scale), _F(cap), state))
+    check_call(_LIB.TfAttentionState(_I64(length), _i32(heads, "heads"), _i32(kv_heads, "kv_heads"), int(bool(causal)), _i32(window, "window"), _F(scale), _F(cap), state))
     return state
 
 
