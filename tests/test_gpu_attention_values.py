@@ -284,3 +284,34 @@ def test_later_queries_of_smaller_gradients(env, path, kind):
     c = Fine(1, 100, 100, seed=8, **dict(kind, causal=True))
     c.dout *= (2.0 ** -np.arange(100)).astype(np.float32)[:, None]
     check(run(env, c), *c.bounds())
+
+
+@pytest.mark.parametrize("size", [2.0 ** 12, 2.0 ** 22, 2.0 ** 40, 2.0 ** 100])
+@pytest.mark.parametrize("kind", [dict(queries=130, keys=130, heads=4, kv_heads=2, dim=64), dict(queries=4, keys=300, heads=2, kv_heads=1, dim=40), dict(queries=200, keys=200, heads=2, kv_heads=2, dim=128, bias=True)], ids=IDS)
+@pytest.mark.parametrize("first, second", [(1, 2), (2, 1), (0, 2), (0, 1)])
+def test_scores_of_any_size_where_the_directions_run_on_different_kernels(env, kind, size, first, second):
+    """Then their scores differ by roundings, which are more than an exponent of 1 from 2^20 on: probabilities are at most 1 all the same, so the values' gradients are at most the sum
+    of the output gradients, and all are finite."""
+    c = Case(1, **kind)
+    c.q *= np.float32(size ** 0.5)
+    c.k *= np.float32(size ** 0.5)
+    on = lambda v: None if v is None else env.nd.array(v, env.ctx)      # noqa: E731
+    q, k, v, dout, slopes = (on(a) for a in (c.q, c.k, c.v, c.dout, c.slopes))
+    out, stats = env.nd.empty(c.q.shape, env.ctx), env.nd.empty((1, c.heads, c.queries, 2), env.ctx)
+    grads = [env.nd.empty(a.shape, env.ctx) for a in (c.q, c.k, c.v)]
+    state = c.state(env)
+    try:
+        env.gpu_op.set_contraction_path(first)
+        assert not env.gpu_op.attention_forward(q, k, v, None, None, slopes, out, stats, state, env.stream)
+        env.gpu_op.set_contraction_path(second)
+        assert not env.gpu_op.attention_backward(q, k, v, None, None, slopes, out, stats, dout, *grads, state, env.stream)
+    finally:
+        env.gpu_op.set_contraction_path(0)
+    for a in (out, *grads):
+        assert np.isfinite(a.asnumpy()).all()
+    total = np.abs(c.dout).reshape(c.queries, c.kv_heads, -1, c.dim).sum((0, 2)).reshape(-1)
+    allowed = 2.0 ** -10                                     # the sums
+    if size < 2.0 ** 20:                                     # below 2^16 weights are taken as they come, and both kernels' scores are off by (D + 16) u of their terms
+        norms = [np.linalg.norm(a.reshape(len(a), -1, c.dim).astype(np.float64), axis=2).max() for a in (c.q, c.k)]
+        allowed += 2.0 ** (2 * (c.dim + 16) * U * float(c.scale) * np.log2(np.e) * norms[0] * norms[1]) - 1
+    assert (np.abs(grads[2].asnumpy()) <= total * (1 + allowed)).all()

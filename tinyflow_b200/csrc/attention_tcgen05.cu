@@ -56,7 +56,7 @@ struct __align__(16) TileInfo {
   float inv, top;                                // 1 / scale; negative where every token has one of its own; largest finite magnitude
   float norm, delta;                             // dO': largest row norm and |D'|
   uint32_t bad[4];                               // tokens with values that are not finite
-  float low, unused[3];                          // dO': smallest row norm that is not zero
+  float low, peak, unused[2];                    // dO': smallest row norm that is not zero; largest magnitude of the rows' maxima
 };
 struct Packed { const char* image; const TileInfo* info; const float* scale; };           // 1 / scale of every token; 0 for tokens of zeros among others with scales of their own
 struct TcArgs {
@@ -114,6 +114,9 @@ template <int kAcross, class F> __device__ __forceinline__ float joined(const fl
 constexpr int kOrders = 8, kOrdersOfGradient = 14;
 // Of the weights of dk below the bound that scales them: a weight is held to 2^-39 of that, and what scales it is about 2^4 above the largest of them.
 constexpr int kOrdersOfBound = 7, kOrdersOfSeen = 10;
+// Largest maximum, in units of log 2, of rows whose weights are taken as they come in the gradients.  Above it a forward call of other kernels may have rounded scores by so much that a
+// weight is 2 and more, not 1: the way of tokens that are apart takes at most 1.
+constexpr float kPeak = 65536.f;
 // max * scale in [2^14, 2^15); subnormal maxima, and those from 2^126, as far as the scale and its reciprocal are normal numbers
 __device__ __forceinline__ int scale_exponent(float most) { return most > 0.f ? min(126, max(-126, 14 - exponent_of(most))) : 0; }
 
@@ -126,7 +129,7 @@ __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, F
   constexpr int kPackWarps = pack_threads(G, FEW) / 32;
   constexpr int kAcross = 16 * G, kRowsAtOnce = 32 / kAcross, kRowsOfWarp = kTile / kPackWarps, kSteps = kRowsOfWarp / kRowsAtOnce;
   constexpr int kShare = kAcross / 4, kGroups = kSteps / 4;            // of four steps' rows a lane looks after one, with kShare - 1 others
-  __shared__ float red[kPackWarps], red_least[kPackWarps], red_norm[kPackWarps], red_delta[kPackWarps], red_low[kPackWarps], token_scale[kTile];
+  __shared__ float red[kPackWarps], red_least[kPackWarps], red_norm[kPackWarps], red_delta[kPackWarps], red_low[kPackWarps], red_peak[kPackWarps], token_scale[kTile];
   __shared__ uint32_t bad_words[4];
   grid_dep_sync();
   int j = 0;
@@ -137,7 +140,7 @@ __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, F
   const int D = p.a.D;
   if (threadIdx.x < 4) bad_words[threadIdx.x] = 0u;
   float v[kSteps][4];
-  float most_norm = 0.f, most_delta = 0.f, low = INFINITY;
+  float most_norm = 0.f, most_delta = 0.f, low = INFINITY, peak = 0.f;
   const auto load4 = [&](const float* from, int t, float* w) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = 0.f;
@@ -217,6 +220,7 @@ __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, F
       }
       most_norm = fmaxf(most_norm, norm); most_delta = fmaxf(most_delta, fabsf(own_delta[g]));
       if (norm > 0.f) low = fminf(low, norm);
+      peak = fmaxf(peak, fabsf(own_max[g]));
     }
   }
 #pragma unroll
@@ -230,11 +234,12 @@ __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, F
       most_norm = fmaxf(most_norm, __shfl_xor_sync(0xffffffffu, most_norm, o));
       most_delta = fmaxf(most_delta, __shfl_xor_sync(0xffffffffu, most_delta, o));
       low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+      peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, o));
     }
   }
-  if (lane == 0) { red[warp] = most; red_least[warp] = least; red_norm[warp] = most_norm; red_delta[warp] = most_delta; red_low[warp] = low; }
+  if (lane == 0) { red[warp] = most; red_least[warp] = least; red_norm[warp] = most_norm; red_delta[warp] = most_delta; red_low[warp] = low; red_peak[warp] = peak; }
   __syncthreads();
-  most = red[lane & (kPackWarps - 1)]; least = red_least[lane & (kPackWarps - 1)]; most_norm = red_norm[lane & (kPackWarps - 1)]; most_delta = red_delta[lane & (kPackWarps - 1)]; low = red_low[lane & (kPackWarps - 1)];
+  most = red[lane & (kPackWarps - 1)]; least = red_least[lane & (kPackWarps - 1)]; most_norm = red_norm[lane & (kPackWarps - 1)]; most_delta = red_delta[lane & (kPackWarps - 1)]; low = red_low[lane & (kPackWarps - 1)]; peak = red_peak[lane & (kPackWarps - 1)];
 #pragma unroll
   for (int o = kPackWarps / 2; o > 0; o >>= 1) {
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -242,6 +247,7 @@ __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, F
     most_norm = fmaxf(most_norm, __shfl_xor_sync(0xffffffffu, most_norm, o));
     most_delta = fmaxf(most_delta, __shfl_xor_sync(0xffffffffu, most_delta, o));
     low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+    peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, o));
   }
   const bool apart = most > 0.f && exponent_of(most) - exponent_of(least) > (job.gradient ? kOrdersOfGradient : kOrders);
   const int e = scale_exponent(most);
@@ -256,7 +262,7 @@ __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, F
   }
   if (threadIdx.x == 0) {
     TileInfo& info = job.info[at_tile];
-    info.inv = apart ? -1.f : power_of_two(-e); info.top = most; info.norm = most_norm; info.delta = most_delta; info.low = low;
+    info.inv = apart ? -1.f : power_of_two(-e); info.top = most; info.norm = most_norm; info.delta = most_delta; info.low = low; info.peak = peak;
 #pragma unroll
     for (int i = 0; i < 4; ++i) info.bad[i] = bad_words[i];
   }
@@ -548,7 +554,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
       rows_armed = true;
     }
     Walk<KIND> walk(p, b, row_head, share, tile);
-    const bool rows_apart = r1.info[row_at].inv < 0.f || (kTwo && r2.info[row_at].inv < 0.f);
+    const bool rows_apart = r1.info[row_at].inv < 0.f || (kTwo && r2.info[row_at].inv < 0.f) || (KIND == kDq && r2.info[row_at].peak > kPeak);
     const float rows_top = KIND == kDk ? r2.info[row_at].top * sqrtf((float)a.D) : 0.f;
     // What an entry says is asked for a tile ahead
     struct Next { bool there, all, apart; int head, t; int64_t at; float inv1, inv2, x, y; uint32_t spoils; };
@@ -559,7 +565,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
       const TileInfo &i1 = c1.info[x.at], &i2 = c2.info[x.at];
       x.inv1 = i1.inv; x.inv2 = i2.inv; x.x = KIND == kDq ? i2.top : i2.norm; x.y = i2.delta;
       const uint4 u = *reinterpret_cast<const uint4*>(i1.bad), w = *reinterpret_cast<const uint4*>(i2.bad);
-      x.apart = rows_apart || fminf(x.inv1, x.inv2) < 0.f;
+      x.apart = rows_apart || fminf(x.inv1, x.inv2) < 0.f || (kRowsAreKeys && i2.peak > kPeak);
       x.spoils = u.x | u.y | u.z | u.w | w.x | w.y | w.z | w.w;
       // dk: one bound of the tile's queries scales the weights of all keys.  Where a key may see the smallest of them alone, and that is kOrdersOfBound below it, or where all see all,
       // kOrdersOfSeen, the tile goes the way of tokens that are apart.
@@ -757,7 +763,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     const bool careful = __any_sync(0xffffffffu, spoiled);
     const bool cap = SHAPED && a.cap > 0.f;
     const float inv2 = kTwo ? r2.info[row_at].inv : 0.f;
-    const float by = cap ? a.scale / a.cap : a.scale * kLog2e, unit = info1.inv * by, wide = cap ? a.cap * kLog2e : 1.f;           // rows with scales of their own: see below
+    const float by = cap ? a.scale / a.cap : a.scale * kLog2e, unit = info1.inv * by, wide = cap ? a.cap * kLog2e : 1.f;           // of rows that share a scale
     float row_max = 0.f, row_delta = 0.f, row_norm = 0.f;
     if (KIND == kDq) { row_max = p.row_max[row_at * kTile + row]; row_delta = p.row_delta[row_at * kTile + row]; row_norm = p.row_norm[row_at * kTile + row] * sqrtf((float)a.D); }
     const float norm_top = KIND == kDk ? r2.info[row_at].top * sqrtf((float)a.D) : 0.f;
@@ -798,10 +804,10 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     const int at_row = kRowsAreKeys ? self : self + off;
     // of the tile at hand
     Entry now = {};
-    int col0 = 0;                                 // position of the first column
+    int col0 = 0;                                // position of the first column
     bool masked = false;
     uint32_t from = 0;
-    float theirs[S::kChunks] = {};                  // a column's document in every lane
+    float theirs[S::kChunks] = {};               // a column's document in every lane
     // scores of a chunk of 32 columns, capped and biased, in units of log 2; turned: 1 - the cap's tanh squared
     const auto shape32 = [&](float* z, float* turned, int c, float by) {
 #pragma unroll
@@ -870,109 +876,109 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
         if (now.flags & 4) { apart = true; break; }
         const float f = now.inv1 * unit;
         if (KIND == kFwd) {
-        // Scores that are not plain products are written back, so that both passes read them
-        const bool rewritten = SHAPED || masked || f < 0.f;
-        float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          // Scores that are not plain products are written back, so that both passes read them
+          const bool rewritten = SHAPED || masked || f < 0.f;
+          float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
-        for (int c = 0; c < S::kChunks; ++c) {
-          float z[32];
-          tmem_ld32(from + 32 * c, z);
-          tmem_ld_wait();
-          if (__builtin_expect(rewritten, SHAPED)) {
-            if (SHAPED) shape32(z, nullptr, c, f);
-            else
+          for (int c = 0; c < S::kChunks; ++c) {
+            float z[32];
+            tmem_ld32(from + 32 * c, z);
+            tmem_ld_wait();
+            if (__builtin_expect(rewritten, SHAPED)) {
+              if (SHAPED) shape32(z, nullptr, c, f);
+              else
 #pragma unroll
-              for (int k = 0; k < 32; ++k) z[k] *= f;
-            if (masked) mask32(z, c, -INFINITY);
-            tmem_st32(from + 32 * c, reinterpret_cast<const uint32_t*>(z));
-          }
-#pragma unroll
-          for (int k = 0; k < 32; ++k) m[k & 3] = fmaxf(m[k & 3], z[k]);
-        }
-        if (rewritten) tmem_st_wait();
-        const float g = rewritten ? 1.f : f;
-        // of -infinity: NaN if g is 0, which the maximum leaves out
-        const float at_most = fmaxf(most, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * g), base = max_of_finite_or(at_most);
-        const float faded = exp2_fast(most - base);
-        most = at_most;
-        float2 s[2] = {both(0.f), both(0.f)};
-#pragma unroll 1
-        for (int c = 0; c < S::kChunks; ++c) {
-          float z[32];
-          uint32_t words[32];
-          tmem_ld32(from + 32 * c, z);
-          tmem_ld_wait();
-#pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            const float2 e = less<SHAPED>(at2(z, k), g, both(base), p.one), w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
-            s[(k >> 1) & 1] = add2(s[(k >> 1) & 1], w);
-            put2(z, k, mul2(w, both(kWeightScale)));
-          }
-          split32(z, words);
-          tmem_st32(from + 32 * c, words);
-        }
-        tmem_st_wait();
-        arrive(&w_full[n & 1]);
-        sum = fmaf(sum, faded, (s[0].x + s[0].y) + (s[1].x + s[1].y));
-        alpha = faded;
-        out_factor = now.inv2 * (1.f / kWeightScale);
-      } else {
-        // The weights' power of two is a factor: added to the exponent's argument it would cost bits of that, the more the smaller the output gradient (dq 6e-7 off at 1e-7 of it instead of 1e-7)
-        float factor, lift = kWeightScale;
-        if (KIND == kDv) {
-          factor = now.inv2 * (1.f / kWeightScale);
-        } else {
-          const float bound = KIND == kDq ? fmaf(row_norm, now.x, fabsf(row_delta)) : fmaf(now.x, norm_top, now.y);
-          const int shift = min(100, max(-100, kWeightExp - exponent_of(bound)));
-          lift = power_of_two(shift);
-          factor = now.inv1 * power_of_two(-shift);
-        }
-        const float fy = KIND == kDq ? inv2 * lift * now.inv2 : inv2 * now.inv2;         // dq: the row's numbers have it, the others' weights
-        const float *const col_max = columns + (n & 1) * 256 + col_part, *const col_delta = col_max + 128;
-        if (kRowsAreKeys) await(&columns_full[n & 1], (n >> 1) & 1, abort_flag, bad);
-        if (kTwo) wait_for(&y_full[n & 1], (n >> 1) & 1);
-#pragma unroll 1
-        for (int c = 0; c < S::kChunks; ++c) {
-          float z[32], y[32], turned[SHAPED && kTwo ? 32 : 1];
-          tmem_ld32(from + 32 * c, z);
-          if (kTwo) tmem_ld32(mine + S::kYAt + col_part + 32 * c, y);
-          tmem_ld_wait();
-          if (kTwo && c == S::kChunks - 1) arrive(&y_empty[n & 1]);
-          if (SHAPED) shape32(z, kTwo ? turned : nullptr, c, f);
-          const float g = SHAPED ? 1.f : f;
-          if (kRowsAreKeys) {
-#pragma unroll
-            for (int k = 0; k < 32; k += 4) {
-              const float4 m4 = *reinterpret_cast<const float4*>(col_max + 32 * c + k);
-              put2(z, k, less<SHAPED>(at2(z, k), g, make_float2(m4.x, m4.y), p.one));
-              put2(z, k + 2, less<SHAPED>(at2(z, k + 2), g, make_float2(m4.z, m4.w), p.one));
-              if (KIND == kDk) {
-                const float4 d4 = *reinterpret_cast<const float4*>(col_delta + 32 * c + k);
-                put2(y, k, fma2(at2(y, k), both(fy), make_float2(-d4.x, -d4.y)));
-                put2(y, k + 2, fma2(at2(y, k + 2), both(fy), make_float2(-d4.z, -d4.w)));
-              }
+                for (int k = 0; k < 32; ++k) z[k] *= f;
+              if (masked) mask32(z, c, -INFINITY);
+              tmem_st32(from + 32 * c, reinterpret_cast<const uint32_t*>(z));
             }
+#pragma unroll
+            for (int k = 0; k < 32; ++k) m[k & 3] = fmaxf(m[k & 3], z[k]);
+          }
+          if (rewritten) tmem_st_wait();
+          const float g = rewritten ? 1.f : f;
+          // of -infinity: NaN if g is 0, which the maximum leaves out
+          const float at_most = fmaxf(most, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * g), base = max_of_finite_or(at_most);
+          const float faded = exp2_fast(most - base);
+          most = at_most;
+          float2 s[2] = {both(0.f), both(0.f)};
+#pragma unroll 1
+          for (int c = 0; c < S::kChunks; ++c) {
+            float z[32];
+            uint32_t words[32];
+            tmem_ld32(from + 32 * c, z);
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 32; k += 2) {
+              const float2 e = less<SHAPED>(at2(z, k), g, both(base), p.one), w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+              s[(k >> 1) & 1] = add2(s[(k >> 1) & 1], w);
+              put2(z, k, mul2(w, both(kWeightScale)));
+            }
+            split32(z, words);
+            tmem_st32(from + 32 * c, words);
+          }
+          tmem_st_wait();
+          arrive(&w_full[n & 1]);
+          sum = fmaf(sum, faded, (s[0].x + s[0].y) + (s[1].x + s[1].y));
+          alpha = faded;
+          out_factor = now.inv2 * (1.f / kWeightScale);
+        } else {
+          // The weights' power of two is a factor: added to the exponent's argument it would cost bits of that, the more the smaller the output gradient (dq 6e-7 off at 1e-7 of it instead of 1e-7)
+          float factor, lift = kWeightScale;
+          if (KIND == kDv) {
+            factor = now.inv2 * (1.f / kWeightScale);
           } else {
-            const float delta = row_delta * lift;
-#pragma unroll
-            for (int k = 0; k < 32; k += 2) { put2(z, k, less<SHAPED>(at2(z, k), g, both(row_max), p.one)); put2(y, k, fma2(at2(y, k), both(fy), both(-delta))); }
+            const float bound = KIND == kDq ? fmaf(row_norm, now.x, fabsf(row_delta)) : fmaf(now.x, norm_top, now.y);
+            const int shift = min(100, max(-100, kWeightExp - exponent_of(bound)));
+            lift = power_of_two(shift);
+            factor = now.inv1 * power_of_two(-shift);
           }
+          const float fy = KIND == kDq ? inv2 * lift * now.inv2 : inv2 * now.inv2;         // dq: the row's numbers have it, the others' weights
+          const float *const col_max = columns + (n & 1) * 256 + col_part, *const col_delta = col_max + 128;
+          if (kRowsAreKeys) await(&columns_full[n & 1], (n >> 1) & 1, abort_flag, bad);
+          if (kTwo) wait_for(&y_full[n & 1], (n >> 1) & 1);
+#pragma unroll 1
+          for (int c = 0; c < S::kChunks; ++c) {
+            float z[32], y[32], turned[SHAPED && kTwo ? 32 : 1];
+            tmem_ld32(from + 32 * c, z);
+            if (kTwo) tmem_ld32(mine + S::kYAt + col_part + 32 * c, y);
+            tmem_ld_wait();
+            if (kTwo && c == S::kChunks - 1) arrive(&y_empty[n & 1]);
+            if (SHAPED) shape32(z, kTwo ? turned : nullptr, c, f);
+            const float g = SHAPED ? 1.f : f;
+            if (kRowsAreKeys) {
 #pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            float2 w = make_float2(exp2_fast(z[k]), exp2_fast(z[k + 1]));
-            if (kRowsAreKeys) w = mul2(w, both(lift));
-            if (kTwo) w = mul2(w, SHAPED ? mul2(at2(y, k), at2(turned, k)) : at2(y, k));
-            put2(z, k, w);
+              for (int k = 0; k < 32; k += 4) {
+                const float4 m4 = *reinterpret_cast<const float4*>(col_max + 32 * c + k);
+                put2(z, k, less<SHAPED>(at2(z, k), g, make_float2(m4.x, m4.y), p.one));
+                put2(z, k + 2, less<SHAPED>(at2(z, k + 2), g, make_float2(m4.z, m4.w), p.one));
+                if (KIND == kDk) {
+                  const float4 d4 = *reinterpret_cast<const float4*>(col_delta + 32 * c + k);
+                  put2(y, k, fma2(at2(y, k), both(fy), make_float2(-d4.x, -d4.y)));
+                  put2(y, k + 2, fma2(at2(y, k + 2), both(fy), make_float2(-d4.z, -d4.w)));
+                }
+              }
+            } else {
+              const float delta = row_delta * lift;
+#pragma unroll
+              for (int k = 0; k < 32; k += 2) { put2(z, k, less<SHAPED>(at2(z, k), g, both(row_max), p.one)); put2(y, k, fma2(at2(y, k), both(fy), both(-delta))); }
+            }
+#pragma unroll
+            for (int k = 0; k < 32; k += 2) {
+              float2 w = make_float2(exp2_fast(z[k]), exp2_fast(z[k + 1]));
+              if (kRowsAreKeys) w = mul2(w, both(lift));
+              if (kTwo) w = mul2(w, SHAPED ? mul2(at2(y, k), at2(turned, k)) : at2(y, k));
+              put2(z, k, w);
+            }
+            if (__builtin_expect(masked, 0)) mask32(z, c, 0.f);
+            uint32_t words[32];
+            split32(z, words);
+            tmem_st32(from + 32 * c, words);
           }
-          if (__builtin_expect(masked, 0)) mask32(z, c, 0.f);
-          uint32_t words[32];
-          split32(z, words);
-          tmem_st32(from + 32 * c, words);
-        }
-        tmem_st_wait();
-        arrive(&w_full[n & 1]);
-        if (!kTurns && n >= 1) add_up(n - 1);
-        out_factor = factor;
+          tmem_st_wait();
+          arrive(&w_full[n & 1]);
+          if (!kTurns && n >= 1) add_up(n - 1);
+          out_factor = factor;
         }
       }
       if (!apart) break;
