@@ -554,23 +554,27 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
       rows_armed = true;
     }
     Walk<KIND> walk(p, b, row_head, share, tile);
-    const bool rows_apart = r1.info[row_at].inv < 0.f || (kTwo && r2.info[row_at].inv < 0.f) || (KIND == kDq && r2.info[row_at].peak > kPeak);
-    const float rows_top = KIND == kDk ? r2.info[row_at].top * sqrtf((float)a.D) : 0.f;
-    // What an entry says is asked for a tile ahead
-    struct Next { bool there, all, apart; int head, t; int64_t at; float inv1, inv2, x, y; uint32_t spoils; };
+    const TileInfo& rows2 = kTwo ? r2.info[row_at] : r1.info[row_at];
+    const float rows_inv1 = r1.info[row_at].inv, rows_inv2 = rows2.inv, rows_top = rows2.top, rows_peak = rows2.peak;
+    // What an entry says is asked for a tile ahead, and looked at behind the tile's first copies
+    struct Next { bool there, all; int head, t; int64_t at; float inv1, inv2, x, y, low, peak; uint4 bad1, bad2; };
     const auto look_ahead = [&] {
       Next x;
       x.there = walk.next(lane, x.head, x.t, x.all);
       x.at = x.there ? col_at(x.head, x.t) : 0;
       const TileInfo &i1 = c1.info[x.at], &i2 = c2.info[x.at];
-      x.inv1 = i1.inv; x.inv2 = i2.inv; x.x = KIND == kDq ? i2.top : i2.norm; x.y = i2.delta;
-      const uint4 u = *reinterpret_cast<const uint4*>(i1.bad), w = *reinterpret_cast<const uint4*>(i2.bad);
-      x.apart = rows_apart || fminf(x.inv1, x.inv2) < 0.f || (kRowsAreKeys && i2.peak > kPeak);
-      x.spoils = u.x | u.y | u.z | u.w | w.x | w.y | w.z | w.w;
+      x.inv1 = i1.inv; x.inv2 = i2.inv; x.x = KIND == kDq ? i2.top : i2.norm; x.y = i2.delta; x.low = i2.low; x.peak = i2.peak;
+      x.bad1 = *reinterpret_cast<const uint4*>(i1.bad); x.bad2 = *reinterpret_cast<const uint4*>(i2.bad);
+      return x;
+    };
+    const auto flags_of = [&](const Next& x) {
+      const bool spoils = (x.bad1.x | x.bad1.y | x.bad1.z | x.bad1.w | x.bad2.x | x.bad2.y | x.bad2.z | x.bad2.w) != 0u, whole = x.all && !spoils;
+      bool apart = fminf(fminf(rows_inv1, rows_inv2), fminf(x.inv1, x.inv2)) < 0.f || (KIND != kFwd && (kRowsAreKeys ? x.peak : rows_peak) > kPeak);
       // dk: one bound of the tile's queries scales the weights of all keys.  Where a key may see the smallest of them alone, and that is kOrdersOfBound below it, or where all see all,
       // kOrdersOfSeen, the tile goes the way of tokens that are apart.
-      if (KIND == kDk && fmaf(x.x, rows_top, x.y) > (float)(1 << (x.all && x.spoils == 0u ? kOrdersOfSeen : kOrdersOfBound)) * (i2.low * rows_top)) x.apart = true;
-      return x;
+      const float top = rows_top * sqrtf((float)a.D);
+      if (KIND == kDk && fmaf(x.x, top, x.y) > (float)(1 << (whole ? kOrdersOfSeen : kOrdersOfBound)) * (x.low * top)) apart = true;
+      return 1 | (int)whole << 1 | (int)apart << 2;
     };
     const auto load = [&](const Packed& from, int64_t at) {
 #pragma unroll
@@ -592,8 +596,9 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     Next next = look_ahead();
     for (int n = 0;; ++n) {
       const Next now = next;
+      if (now.there) load(c1, now.at);           // before the entry, which waits for what it says; it waits for no tile but those in front of it
       if (lane == 0) {
-        entries[n & 7] = Entry{now.there ? 1 | (int)(now.all && now.spoils == 0u) << 1 | (int)now.apart << 2 : 0, now.head, now.t * kTile + (kRowsAreKeys ? a.Tk - a.Tq : 0), now.there ? (int)now.at : n, now.inv1, now.inv2, now.x, now.y};
+        entries[n & 7] = Entry{now.there ? flags_of(now) : 0, now.head, now.t * kTile + (kRowsAreKeys ? a.Tk - a.Tq : 0), now.there ? (int)now.at : n, now.inv1, now.inv2, now.x, now.y};
         mbar_arrive(entry_full + (n & 7));
       }
       __syncwarp();
@@ -602,7 +607,6 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
         break;
       }
       next = look_ahead();
-      load(c1, now.at);
       if (kTwo) load(c2, now.at);
       if (kRowsAreKeys) {                        // maxima and D' of the tile's queries, when the weights of the tile before the last are made
         if (n >= 2) await(&w_full[n & 1], ((n - 2) >> 1) & 1, abort_flag, bad);

@@ -460,7 +460,7 @@ bool tensor_path_pays(const AttentionArgs& a, bool backward) {
   if (!backward) {
     const double exact = 4.0 + std::max(1.0, sequences * row_blocks / (per_sm * sms)) * (a.D <= 64 ? 0.1 : 0.2) * std::max(24.0, (double)a.Tk);
     const double waves = std::max(1.0, (double)a.B * a.H * q_tiles / sms);
-    return more * (6.2 + 4.6 + (waves - 1) * 11.0 + waves * (k_tiles - 1) * 2.0) < exact;
+    return more * (6.2 + 4.25 + (waves - 1) * 11.0 + waves * (k_tiles - 1) * 2.0) < exact;
   }
   const double exact = 8.0 + std::max(1.0, sequences * (row_blocks + key_blocks) / (per_sm * sms)) * (a.D <= 64 ? 0.25 : 0.4) * std::max((double)a.Tk, rows);
   const double waves = std::max(1.0, (2 * sequences * k_tiles + (double)a.B * a.H * q_tiles) / sms);
