@@ -13,7 +13,7 @@
 // atomics, the same bits every run.
 //
 // Operands.  A packing kernel writes every tile of 128 tokens x one head as fp16 halves hi and lo of x times a power of two that the tile's largest finite
-// element chooses, in the 128-byte swizzle of the shared-memory descriptors, so a tile part is one bulk copy and no tensor map is needed.  The same image is read
+// element chooses (queries also times the mantissa of what scores are scaled by, so that a score is a product times a power of two), in the 128-byte swizzle of the shared-memory descriptors, so a tile part is one bulk copy and no tensor map is needed.  The same image is read
 // with the head along K (scores) and with the tokens along K (products), by descriptors of the other major.  Products are hi*lo + lo*hi + hi*hi, the small ones first.
 // Weights are split in registers and go back to TMEM as the A operand, over the scores they came from; each is scaled by a power of two so that their largest
 // (bounded for gradients by the norms of dO' rows and V) is just below 2^15.  Scales of a tile are undone where its product is added up: the tensor core
@@ -21,12 +21,13 @@
 //
 // Tokens of different sizes.  What a row does not see (padding, other documents, tokens behind it) may be of any size, and must not cost it bits.  Where a tile's tokens are further
 // apart than a scale serves (kOrders), each is packed with a scale of its own.  The warps undo those in the scores, put those of the product's operand into the weights, and scale a row's
-// weights by the largest that it sees, found first: a second pass over such tiles, in code of its own beside the loop that all others take.
+// weights by the largest that it sees, found first: a second pass over such tiles, in code of its own beside the loop that all others take.  With every tile of the values like that
+// 2 x 4096 tokens, 16 over 4 heads of 128, causal, take 475 us forward instead of 393 and 1607 back instead of 1534; 8 heads of 64, every key seen, 710 instead of 426 and 2129 of 1720.
 //
 // Bound by the tensor rate: 3 products of 16-bit halves for each product.  The tile of the next scores is issued ahead of the product of the present weights,
-// so the tensor cores work while 8 warps (two a TMEM lane quarter) make weights.  4 x 4096 tokens, 8 heads of 128, every key seen: forward 755 us (364 TFLOP/s of the formula,
-// three times that in halves), gradients 2812; heads of 64: 422 and 1520.  There the power limit holds the clock at 1.45 to 1.6 GHz of 1.97.  A CTA's start and end take 8 us,
-// so rows that see few tiles are bound by those.
+// so the tensor cores work while 8 warps (two a TMEM lane quarter) make weights.  4 x 4096 tokens, 8 heads of 128, every key seen: forward 750 us (366 TFLOP/s of the formula,
+// three times that in halves), gradients 3096; heads of 64: 419 and 1690.  There the power limit holds the clock at 1.45 to 1.6 GHz of 1.97, which differs by a tenth from box to box.
+// A CTA's start and end take 8 us, so rows that see few tiles are bound by those.
 //
 // A token that holds a value which is not finite is packed as if that value were zero and marked; weights that see it become NaN.  So it reaches what depends on it and nothing
 // else, while a zero weight times it would reach every row of the tile.
@@ -34,6 +35,7 @@
 #include <cuda_fp16.h>
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 #include "tcgen05.h"
 
@@ -66,7 +68,7 @@ struct TcArgs {
   const float4* documents;                       // of every sequence and key tile: smallest, largest, whether there is padding
   float *dk_part, *dv_part;                      // where the query heads of a key-value head are dealt to several CTAs: their sums, one after another
   int q_tiles, k_tiles, D16, shares;
-  float one;                                     // 1
+  float by, dk_factor;                           // power of two of scores (0: all are 0); what dk's sums are multiplied by, their queries being so already
   int* err;
 };
 
@@ -78,6 +80,7 @@ struct PackJob {
   float* scale;
   int heads, length, tiles;
   int gradient;                                  // dout: times 1 / sum, with its row's D' and norm
+  float times;                                   // 1; queries: what scores are scaled by, but for its power of two, so that scores are products times a power of two and not rounded again
 };
 struct PackArgs {
   AttentionArgs a;
@@ -117,12 +120,12 @@ constexpr int kOrdersOfBound = 7, kOrdersOfSeen = 10;
 // Largest maximum, in units of log 2, of rows whose weights are taken as they come in the gradients.  Above it a forward call of other kernels may have rounded scores by so much that a
 // weight is 2 and more, not 1: the way of tokens that are apart takes at most 1.
 constexpr float kPeak = 65536.f;
-// max * scale in [2^14, 2^15); subnormal maxima, and those from 2^126, as far as the scale and its reciprocal are normal numbers
-__device__ __forceinline__ int scale_exponent(float most) { return most > 0.f ? min(126, max(-126, 14 - exponent_of(most))) : 0; }
+// max * scale in [2^13, 2^14), and then times a factor of less than 2; subnormal maxima, and those from 2^126, as far as the scale and its reciprocal are normal numbers
+__device__ __forceinline__ int scale_exponent(float most, int below) { return most > 0.f ? min(126, max(-126, below - exponent_of(most))) : 0; }
 
 // A block packs one tile of one head, 16 G threads a row, 4 columns each.  HBM-bound: 4 bytes an element read and written, for dout 8 read.  Half the rows' loads in flight a
-// thread where there are few tiles (2 x 777 tokens, 6 over 2 heads of 72, both directions: 91 us of the step's time with twice the threads, 95 without; 8 x 1024 tokens, 16
-// heads of 64: 512 and 497).
+// thread where there are few tiles (2 x 777 tokens, 6 over 2 heads of 72: 27.0 us forward and 54.5 back with twice the threads, 29.0 and 56.4 without; 8 x 1024 tokens, 16
+// heads of 64: 138.5 and 367, 125.7 and 359).
 constexpr int pack_threads(int G, bool few) { return (few ? 512 : 256) * G; }
 template <int G, bool WIDE, bool FEW>
 __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, FEW)) attention_pack_kernel(const __grid_constant__ PackArgs p) {
@@ -250,13 +253,13 @@ __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, F
     peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, o));
   }
   const bool apart = most > 0.f && exponent_of(most) - exponent_of(least) > (job.gradient ? kOrdersOfGradient : kOrders);
-  const int e = scale_exponent(most);
+  const int below = job.times == 1.f ? 14 : 13, e = scale_exponent(most, below);
   const int64_t at_tile = (int64_t)bh * job.tiles + tile;
   if (lane % kShare == 0) {
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-      const int of_token = apart ? scale_exponent(own_top[g]) : e;
-      token_scale[own_row(g)] = power_of_two(of_token);                // its warp's rows
+      const int of_token = apart ? scale_exponent(own_top[g], below) : e;
+      token_scale[own_row(g)] = power_of_two(of_token) * job.times;    // its warp's rows
       job.scale[at_tile * kTile + own_row(g)] = apart && own_top[g] == 0.f ? 0.f : power_of_two(-of_token);
     }
   }
@@ -271,7 +274,7 @@ __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, F
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
     const int r = row_of(s);
-    const float scale = apart ? token_scale[r] : power_of_two(e);
+    const float scale = apart ? token_scale[r] : power_of_two(e) * job.times;
     float hi[4], x[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) { x[i] = v[s][i] * scale; hi[i] = __half2float(__float2half_rn(x[i])); }
@@ -427,18 +430,12 @@ __device__ __forceinline__ void tanh32(float* t) {
     put2(t, k, y);
   }
 }
-// g z less m, g z rounded as the maximum m was: the largest score is 0 then, in both directions, however large it is.  In one rounding it would be what rounding m took off, 2^8 for
-// a score of 2^32.  `one` is 1 where the compiler does not see it, which makes one rounding of a packed product and a sum behind it.  Shaped scores are whole, their g is 1.
-template <bool SHAPED> __device__ __forceinline__ float2 less(float2 z, float g, float2 m, float one) {
-  const float2 n = make_float2(-m.x, -m.y);
-  return SHAPED ? add2(z, n) : fma2(mul2(z, both(g)), both(one), n);
-}
-// 32 numbers times `by` and a scale each, a power of two or zero; no sum behind it takes in the rounding
+// 32 numbers times `by` and a scale each, powers of two or zero
 __device__ __forceinline__ void times32(float* z, const float* __restrict__ scale, float by) {
 #pragma unroll
   for (int k = 0; k < 32; k += 4) {
     const float4 f = __ldg(reinterpret_cast<const float4*>(scale + k));
-    z[k] = __fmul_rn(z[k], f.x * by); z[k + 1] = __fmul_rn(z[k + 1], f.y * by); z[k + 2] = __fmul_rn(z[k + 2], f.z * by); z[k + 3] = __fmul_rn(z[k + 3], f.w * by);
+    z[k] *= f.x * by; z[k + 1] *= f.y * by; z[k + 2] *= f.z * by; z[k + 3] *= f.w * by;
   }
 }
 // hi and lo halves of 32 weights, as the A operand has them: 16 weights are 8 words of hi and 8 of lo
@@ -767,7 +764,8 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     const bool careful = __any_sync(0xffffffffu, spoiled);
     const bool cap = SHAPED && a.cap > 0.f;
     const float inv2 = kTwo ? r2.info[row_at].inv : 0.f;
-    const float by = cap ? a.scale / a.cap : a.scale * kLog2e, unit = info1.inv * by, wide = cap ? a.cap * kLog2e : 1.f;           // of rows that share a scale
+    // The unit of rows that share a scale.  Powers of two: a score less its maximum is rounded once, in both directions alike, and the largest is 0, however large it is.
+    const float unit = info1.inv * p.by, wide = cap ? a.cap * kLog2e : 1.f;
     float row_max = 0.f, row_delta = 0.f, row_norm = 0.f;
     if (KIND == kDq) { row_max = p.row_max[row_at * kTile + row]; row_delta = p.row_delta[row_at * kTile + row]; row_norm = p.row_norm[row_at * kTile + row] * sqrtf((float)a.D); }
     const float norm_top = KIND == kDk ? r2.info[row_at].top * sqrtf((float)a.D) : 0.f;
@@ -881,7 +879,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
         const float f = now.inv1 * unit;
         if (KIND == kFwd) {
           // Scores that are not plain products are written back, so that both passes read them
-          const bool rewritten = SHAPED || masked || f < 0.f;
+          const bool rewritten = SHAPED || masked;
           float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
           for (int c = 0; c < S::kChunks; ++c) {
@@ -914,7 +912,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
             tmem_ld_wait();
 #pragma unroll
             for (int k = 0; k < 32; k += 2) {
-              const float2 e = less<SHAPED>(at2(z, k), g, both(base), p.one), w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+              const float2 e = fma2(at2(z, k), both(g), both(-base)), w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
               s[(k >> 1) & 1] = add2(s[(k >> 1) & 1], w);
               put2(z, k, mul2(w, both(kWeightScale)));
             }
@@ -927,7 +925,8 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
           alpha = faded;
           out_factor = now.inv2 * (1.f / kWeightScale);
         } else {
-          // The weights' power of two is a factor: added to the exponent's argument it would cost bits of that, the more the smaller the output gradient (dq 6e-7 off at 1e-7 of it instead of 1e-7)
+          // The weights' power of two is a factor: added to the exponential's argument it would cost bits of that, the more the smaller the output gradient (dq 6e-7 off at 1e-7 of it
+          // instead of 1e-7)
           float factor, lift = kWeightScale;
           if (KIND == kDv) {
             factor = now.inv2 * (1.f / kWeightScale);
@@ -954,8 +953,8 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
 #pragma unroll
               for (int k = 0; k < 32; k += 4) {
                 const float4 m4 = *reinterpret_cast<const float4*>(col_max + 32 * c + k);
-                put2(z, k, less<SHAPED>(at2(z, k), g, make_float2(m4.x, m4.y), p.one));
-                put2(z, k + 2, less<SHAPED>(at2(z, k + 2), g, make_float2(m4.z, m4.w), p.one));
+                put2(z, k, fma2(at2(z, k), both(g), make_float2(-m4.x, -m4.y)));
+                put2(z, k + 2, fma2(at2(z, k + 2), both(g), make_float2(-m4.z, -m4.w)));
                 if (KIND == kDk) {
                   const float4 d4 = *reinterpret_cast<const float4*>(col_delta + 32 * c + k);
                   put2(y, k, fma2(at2(y, k), both(fy), make_float2(-d4.x, -d4.y)));
@@ -965,7 +964,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
             } else {
               const float delta = row_delta * lift;
 #pragma unroll
-              for (int k = 0; k < 32; k += 2) { put2(z, k, less<SHAPED>(at2(z, k), g, both(row_max), p.one)); put2(y, k, fma2(at2(y, k), both(fy), both(-delta))); }
+              for (int k = 0; k < 32; k += 2) { put2(z, k, fma2(at2(z, k), both(g), both(-row_max))); put2(y, k, fma2(at2(y, k), both(fy), both(-delta))); }
             }
 #pragma unroll
             for (int k = 0; k < 32; k += 2) {
@@ -986,9 +985,9 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
         }
       }
       if (!apart) break;
-      // Tokens of different sizes, among the columns or the rows.  Their scales go into the scores and, those of the product's operand, into the weights, which are held in TMEM until the largest of their row is known
-      // and scales them: so no token costs a bit of what does not depend on it.
-      const float row_unit = r1.scale[row_at * kTile + row] * by, row_inv2 = kTwo ? r2.scale[row_at * kTile + row] : 0.f;
+      // Tokens of different sizes, among the columns or the rows.  Their scales go into the scores and, those of the product's operand, into the weights, which are held in TMEM until
+      // the largest of their row is known and scales them: so no token costs a bit of what does not depend on it.
+      const float row_unit = r1.scale[row_at * kTile + row] * p.by, row_inv2 = kTwo ? r2.scale[row_at * kTile + row] : 0.f;
       const float *const scale1 = c1.scale + (int64_t)now.at * kTile + col_part, *const scale2 = c2.scale + (int64_t)now.at * kTile + col_part;
       const float *const col_max = columns + (n & 1) * 256 + col_part, *const col_delta = col_max + 128;
       if (kRowsAreKeys) await(&columns_full[n & 1], (n >> 1) & 1, abort_flag, bad);
@@ -1075,7 +1074,7 @@ __device__ __forceinline__ void attention_rows(const TcArgs& p, int block) {
     }
     if (n >= (kTurns ? 2 : 1)) add_up(n - (kTurns ? 2 : 1));           // n: where the list ends for this warp
 
-    float last = KIND == kDv ? 1.f : a.scale;
+    float last = KIND == kDv ? 1.f : KIND == kDk ? p.dk_factor : a.scale;
     if (kTurns) {
       // The second group's sums go through the ring, once the last product has read it.  Columns by rows, so that a warp's words lie side by side.
       float* const handed = reinterpret_cast<float*>(ring);
@@ -1226,6 +1225,10 @@ static size_t lay_out(const AttentionArgs& a, bool backward, char* base, PackArg
   size_t at = 0;
   const auto take = [&](size_t bytes) { const size_t from = at; at += (bytes + 255) / 256 * 256; return base ? base + from : nullptr; };
   const int jobs = backward ? 4 : 3;
+  // What products are multiplied by to make scores in units of log 2, or of the cap: mantissa (with its sign) and power of two
+  const double by = a.cap > 0.f ? (double)a.scale / a.cap : a.scale * 1.4426950408889634;
+  int exponent = 0;
+  const float mantissa = by == 0.0 ? 1.f : (float)(2.0 * std::frexp(by, &exponent));
   const float* const from[4] = {a.q, a.k, a.v, a.dout};
   Packed* const to[4] = {tc ? &tc->q : nullptr, tc ? &tc->k : nullptr, tc ? &tc->v : nullptr, tc ? &tc->d : nullptr};
   int blocks = 0;
@@ -1236,7 +1239,7 @@ static size_t lay_out(const AttentionArgs& a, bool backward, char* base, PackArg
     char* const info = take(n * sizeof(TileInfo));
     char* const scale = take(n * kTile * sizeof(float));
     if (base) {
-      pack->job[j] = PackJob{from[j], img, (TileInfo*)info, (float*)scale, queries ? a.H : a.G, queries ? a.Tq : a.Tk, queries ? q_tiles : k_tiles, j == 3};
+      pack->job[j] = PackJob{from[j], img, (TileInfo*)info, (float*)scale, queries ? a.H : a.G, queries ? a.Tq : a.Tk, queries ? q_tiles : k_tiles, j == 3, j == 0 ? mantissa : 1.f};
       pack->first[j] = blocks;
       *to[j] = Packed{img, (const TileInfo*)info, (const float*)scale};
     }
@@ -1252,7 +1255,7 @@ static size_t lay_out(const AttentionArgs& a, bool backward, char* base, PackArg
     pack->a = a; pack->jobs = jobs; pack->first[jobs] = blocks; pack->document_job = 1;
     pack->row_max = (float*)rows[0]; pack->row_delta = (float*)rows[1]; pack->row_norm = (float*)rows[2]; pack->documents = (float4*)docs;
     tc->a = a; tc->row_max = pack->row_max; tc->row_delta = pack->row_delta; tc->row_norm = pack->row_norm; tc->documents = pack->documents;
-    tc->q_tiles = q_tiles; tc->k_tiles = k_tiles; tc->D16 = (a.D + 15) / 16 * 16; tc->err = tensor_error_word(); tc->one = 1.f;
+    tc->q_tiles = q_tiles; tc->k_tiles = k_tiles; tc->D16 = (a.D + 15) / 16 * 16; tc->err = tensor_error_word(); tc->by = by == 0.0 ? 0.f : (float)std::ldexp(1.0, std::min(127, std::max(-126, exponent - 1))); tc->dk_factor = (float)(a.scale / (double)mantissa);
     tc->shares = shares; tc->dk_part = (float*)dk_part; tc->dv_part = (float*)dv_part;
   }
   return at;

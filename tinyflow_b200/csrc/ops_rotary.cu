@@ -493,7 +493,7 @@ int TfHeadNormRotaryBackward(const DLArrayHandle query, const DLArrayHandle key,
   const int64_t rows = a.h[0].rows + a.h[1].rows;
   if (rows == 0) return 0;
   StreamLease lease(s);
-  // Four blocks an SM with one head a thread group and pass: 94 us at 16384 tokens x (16 + 4) heads of 128, 5.3 TB/s.  More in flight is slower, reads and writes
+  // Four blocks an SM with one head a thread group and pass: 94 to 100 us by box at 16384 tokens x (16 + 4) heads of 128, 5.0 to 5.3 TB/s.  More in flight is slower, reads and writes
   // get in one another's way: three or four blocks of two heads 98 and 115, five of one 106, the next pass asked for in advance 115.
   const int64_t most = kNormBlocks * device_sm_count();
   const size_t bytes = sizeof(float) * (size_t)(most + 1) * a.D;
