@@ -111,6 +111,15 @@ template <int kAcross, class F> __device__ __forceinline__ float joined(const fl
   for (int o = kAcross / 8; o > 0; o >>= 1) x = join(x, __shfl_xor_sync(0xffffffffu, x, o));
   return x;
 }
+// The largest of each, of numbers that are not negative: where a row has all lanes, a reduction instruction each is less than the exchange
+template <int kAcross> __device__ __forceinline__ float largest(const float* v) {
+  if (kAcross < 32) return joined<kAcross>(v, [](float x, float y) { return fmaxf(x, y); });
+  uint32_t x[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = __reduce_max_sync(0xffffffffu, __float_as_uint(v[i]));
+  const int mine = threadIdx.x / (kAcross / 4) % 4;
+  return __uint_as_float(mine & 2 ? (mine & 1 ? x[3] : x[2]) : (mine & 1 ? x[1] : x[0]));
+}
 // Binary orders between the largest magnitudes of two tokens of a tile up to which they share a scale.  A value is held to 2^-39 of the tile's largest, so 8 orders leave 2^-31 of the
 // token's own, and the scale of the gradients' weights, which goes by the largest value, 8 bits of 25 to spare.  Output gradients over their row's sum, which differ by as much as the
 // sums do, up to the number of keys: 14 orders leave 2^-25.
@@ -161,7 +170,6 @@ __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, F
   __syncthreads();
   const auto own_row = [&](int g) { return row_of(4 * g + lane % kAcross / kShare); };
   const auto add = [](float x, float y) { return x + y; };
-  const auto larger = [](float x, float y) { return fmaxf(x, y); };
   float own_max[kGroups], own_delta[kGroups], own_norm[kGroups], own_top[kGroups];
   if (job.gradient) {
     const float* const stats = p.a.stats + 2 * (((int64_t)b * job.heads + h) * job.length + tile * kTile);
@@ -206,7 +214,7 @@ __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, F
       }
       if (!fine) atomicOr(&bad_words[row_of(4 * g + s) >> 5], 1u << (row_of(4 * g + s) & 31));
     }
-    own_top[g] = joined<kAcross>(top, larger);
+    own_top[g] = largest<kAcross>(top);
     most = fmaxf(most, own_top[g]);
     if (own_top[g] > 0.f) least = fminf(least, own_top[g]);
     if (job.gradient) {
@@ -242,15 +250,21 @@ __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, F
   }
   if (lane == 0) { red[warp] = most; red_least[warp] = least; red_norm[warp] = most_norm; red_delta[warp] = most_delta; red_low[warp] = low; red_peak[warp] = peak; }
   __syncthreads();
-  most = red[lane & (kPackWarps - 1)]; least = red_least[lane & (kPackWarps - 1)]; most_norm = red_norm[lane & (kPackWarps - 1)]; most_delta = red_delta[lane & (kPackWarps - 1)]; low = red_low[lane & (kPackWarps - 1)]; peak = red_peak[lane & (kPackWarps - 1)];
+  most = red[lane & (kPackWarps - 1)]; least = red_least[lane & (kPackWarps - 1)];
 #pragma unroll
   for (int o = kPackWarps / 2; o > 0; o >>= 1) {
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
     least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
-    most_norm = fmaxf(most_norm, __shfl_xor_sync(0xffffffffu, most_norm, o));
-    most_delta = fmaxf(most_delta, __shfl_xor_sync(0xffffffffu, most_delta, o));
-    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-    peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, o));
+  }
+  if (job.gradient && warp == 0) {
+    most_norm = red_norm[lane & (kPackWarps - 1)]; most_delta = red_delta[lane & (kPackWarps - 1)]; low = red_low[lane & (kPackWarps - 1)]; peak = red_peak[lane & (kPackWarps - 1)];
+#pragma unroll
+    for (int o = kPackWarps / 2; o > 0; o >>= 1) {
+      most_norm = fmaxf(most_norm, __shfl_xor_sync(0xffffffffu, most_norm, o));
+      most_delta = fmaxf(most_delta, __shfl_xor_sync(0xffffffffu, most_delta, o));
+      low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+      peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, o));
+    }
   }
   const bool apart = most > 0.f && exponent_of(most) - exponent_of(least) > (job.gradient ? kOrdersOfGradient : kOrders);
   const int below = job.times == 1.f ? 14 : 13, e = scale_exponent(most, below);
@@ -259,7 +273,7 @@ __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, F
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       const int of_token = apart ? scale_exponent(own_top[g], below) : e;
-      token_scale[own_row(g)] = power_of_two(of_token) * job.times;    // its warp's rows
+      if (apart) token_scale[own_row(g)] = power_of_two(of_token) * job.times;    // its warp's rows
       job.scale[at_tile * kTile + own_row(g)] = apart && own_top[g] == 0.f ? 0.f : power_of_two(-of_token);
     }
   }
@@ -269,7 +283,7 @@ __global__ void __launch_bounds__(pack_threads(G, FEW), 1024 / pack_threads(G, F
 #pragma unroll
     for (int i = 0; i < 4; ++i) info.bad[i] = bad_words[i];
   }
-  __syncwarp();
+  if (apart) __syncwarp();
   char* const image = job.image + at_tile * (2 * G * 16384);
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
