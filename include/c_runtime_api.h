@@ -407,7 +407,7 @@ int TfHeadNormRotaryBackward(const DLArrayHandle query, const DLArrayHandle key,
  * A query sees the keys up to its own position (causal) that are less than `window` away (window not 0), and whatever these say the first prefix[sequence] keys;
  * with documents (one number a key; keys >= length) only keys of its own document, and a negative number is padding that sees nothing and is not seen.
  * A query that sees nothing gives zeros and has no gradient.  A key, value, query or output gradient that is not finite makes what depends on it not finite, and
- * nothing else.  documents, prefix and slopes may be null; they are constants.
+ * nothing else; scores have to be numbers of float32, of any size.  documents, prefix and slopes may be null; they are constants.
  * stats (2 for every sequence, head and query: the largest score in units of log 2 and the reciprocal of the sum of 2^(score - largest)) is for the backward call; null: not kept.
  * Backward: output and stats of the forward call; dquery, dkey and dvalue may each be null.  Sums are in a fixed order. */
 int TfAttentionState(int64_t length, int heads, int kv_heads, int causal, int window, float scale, float cap, void ***state);

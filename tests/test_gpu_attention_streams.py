@@ -108,3 +108,33 @@ def test_norms_of_heads_on_several_streams_at_once(env):
             assert np.array_equal(a.asnumpy(), b)
     for s in streams:
         op.destroy_cudaStream(s)
+
+
+@pytest.mark.parametrize("kind", [SEVERAL[0], SEVERAL[1], SEVERAL[4]], ids=["shared", "documents", "cap"])
+def test_replays_of_a_captured_step_on_tokens_near_and_apart(env, kind):
+    """Which way a tile goes is found in the data, so a replay goes another way than the capture did."""
+    import ctypes
+
+    import torch
+    c = Case(**kind)
+    h, graph, side = Held(env, c), torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    cell = ctypes.pointer(ctypes.c_void_p(side.cuda_stream))
+    with torch.cuda.graph(graph, stream=side):
+        h.step(cell)
+    rng = np.random.RandomState(2)
+    for apart in (False, True, False, True):
+        for a in (*h.arrays, h.dout):
+            values = rng.randn(*a.shape).astype(np.float32)
+            if apart:
+                values *= (2.0 ** rng.randint(-12, 1, (len(values), 1))).astype(np.float32)
+                values[5] *= np.float32(2.0 ** 10)
+            a[:] = values
+        h.spoil()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = h.results()
+        h.spoil()
+        h.step(env.stream)
+        env.gpu_op.device_synchronize()
+        for g, w in zip(got, h.results()):
+            assert np.isfinite(g).all() and np.array_equal(g, w)
