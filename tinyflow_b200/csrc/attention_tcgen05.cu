@@ -129,7 +129,7 @@ constexpr int kOrdersOfBound = 7, kOrdersOfSeen = 10;
 // Largest maximum, in units of log 2, of rows whose weights are taken as they come in the gradients.  Above it a forward call of other kernels may have rounded scores by so much that a
 // weight is 2 and more, not 1: the way of tokens that are apart takes at most 1.
 constexpr float kPeak = 65536.f;
-// max * scale in [2^13, 2^14), and then times a factor of less than 2; subnormal maxima, and those from 2^126, as far as the scale and its reciprocal are normal numbers
+// max * scale in [2^below, 2^(below + 1)): 14, or 13 where a factor of less than 2 follows; subnormal maxima, and those from 2^126, as far as the scale and its reciprocal are normal numbers
 __device__ __forceinline__ int scale_exponent(float most, int below) { return most > 0.f ? min(126, max(-126, below - exponent_of(most))) : 0; }
 
 // A block packs one tile of one head, 16 G threads a row, 4 columns each.  HBM-bound: 4 bytes an element read and written, for dout 8 read.  Half the rows' loads in flight a
